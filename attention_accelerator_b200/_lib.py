@@ -31,6 +31,7 @@ GQA_ERR_ROPE_THETA = 16
 GQA_ERR_FLAGS = 17
 GQA_ERR_MEMORY = 18
 GQA_ERR_KV_HEADS = 19
+GQA_ERR_PAGES = 20
 
 #: codes that describe a bad call configuration (the reference's config_error)
 CONFIG_ERRORS = {GQA_ERR_GEOMETRY, GQA_ERR_SEQ_LEN, GQA_ERR_N_KV_TILES, GQA_ERR_SCALE,
@@ -41,6 +42,10 @@ GQA_FLAG_PARTIAL_OUT = 0x1
 GQA_FLAG_K_ROTATED = 0x2
 GQA_FLAG_Q_ROTATED = 0x4
 PARTIAL_FLOATS = 132
+
+GQA_CODE_INT8 = 0
+GQA_CODE_E4M3 = 1
+PAGED_MAX_BATCH = 8192
 
 
 class GqaParams(ctypes.Structure):
@@ -73,6 +78,26 @@ class GqaChunkParams(ctypes.Structure):
                 ("first_position", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
                 ("q_query_stride", ctypes.c_int64), ("out_query_stride", ctypes.c_int64),
                 ("k_batch_stride", ctypes.c_int64), ("v_batch_stride", ctypes.c_int64)]
+
+
+class GqaPagedCache(ctypes.Structure):
+    """Mirror of ``struct gqa_paged_cache``."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("code", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("page_len", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("scale_page_stride", ctypes.c_int64)]
+
+
+class GqaPagedParams(ctypes.Structure):
+    """Mirror of ``struct gqa_paged_params``."""
+    _fields_ = [("batch", ctypes.c_int32), ("rows", ctypes.c_int32), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32), ("flags", ctypes.c_uint32),
+                ("seq_lens", ctypes.c_void_p), ("query_positions", ctypes.c_void_p), ("first_query", ctypes.c_void_p),
+                ("doc_starts", ctypes.c_void_p), ("prefix_ends", ctypes.c_void_p), ("slopes", ctypes.c_void_p),
+                ("scale", ctypes.c_float), ("score_cap", ctypes.c_float), ("rope_theta", ctypes.c_float),
+                ("reserved", ctypes.c_uint32), ("q_row_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("out_row_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64)]
 
 
 CHUNKED_WORKSPACE_BYTES = 256
@@ -124,6 +149,16 @@ _SIGNATURES = {
     "gqa_mem_decode": (ctypes.c_int, [_P, ctypes.c_size_t, ctypes.c_int, _P, ctypes.c_uint64, _P, _P,
                                       ctypes.c_size_t, _P]),
     "gqa_mem_encode_bytes": (ctypes.c_size_t, [ctypes.c_uint64, ctypes.c_int]),
+    "gqa_plan_pages": (ctypes.c_int, [_P, _P, ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int, _P,
+                                      ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "gqa_append_paged": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                        ctypes.c_int64, _P, _P, ctypes.c_float, ctypes.POINTER(GqaPagedCache), _P]),
+    "gqa_read_paged": (ctypes.c_int, [ctypes.POINTER(GqaPagedCache), _P, ctypes.c_int, _P, _P, _P]),
+    "gqa_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(GqaPagedCache), ctypes.POINTER(GqaPagedParams)]),
+    "gqa_decode_paged": (ctypes.c_int, [_P, _P, ctypes.POINTER(GqaPagedCache), ctypes.POINTER(GqaPagedParams), _P,
+                                        ctypes.c_size_t, _P]),
+    "gqa_decode_paged_chunked": (ctypes.c_int, [_P, _P, ctypes.POINTER(GqaPagedCache),
+                                                ctypes.POINTER(GqaPagedParams), _P, ctypes.c_size_t, _P]),
     "gqa_mem_encode": (ctypes.c_int, [_P, ctypes.c_uint64, ctypes.c_int, _P, _P]),
 }
 

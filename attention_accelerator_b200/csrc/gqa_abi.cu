@@ -411,6 +411,8 @@ int fill_args(gqa::DecodeArgs& a, const void* q, const void* k, const void* v, v
 
 }  // namespace
 
+int gqa::device_sms(int* sms) { return current_device(sms); }
+
 extern "C" {
 
 const char* gqa_status_string(int status) {
@@ -435,6 +437,7 @@ const char* gqa_status_string(int status) {
         case GQA_ERR_FLAGS: return "gqa_params.flags holds a bit this entry point does not support";
         case GQA_ERR_MEMORY: return "a tensor, table or workspace pointer is not memory of the current GPU";
         case GQA_ERR_KV_HEADS: return "KV-head range is empty or outside [0, 8)";
+        case GQA_ERR_PAGES: return "page planning refused: too few free pages, a block-table row too short, more new tokens than max_tokens, or a length out of range";
         default: return "unknown status";
     }
 }

@@ -17,6 +17,10 @@ namespace gqa {
 // boundary becomes a status instead of a memory fault on the GPU.
 int check_device_memory(std::initializer_list<const void*> ptrs);
 
+// SM count of the current device; prepares the kernels on first use.  A status
+// (GQA_ERR_UNSUPPORTED_DEVICE where it is not an sm_100 GPU).
+int device_sms(int* sms);
+
 struct DecodeArgs;
 struct RopeTable;
 

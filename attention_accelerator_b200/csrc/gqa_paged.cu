@@ -1,0 +1,708 @@
+// gqa_paged.cu -- the paged 8-bit KV cache: argument checks of its C entry
+// points, page planning, append (RoPE, quantisation) and read-back kernels.
+#include "gqa_paged.cuh"
+#include "gqa_internal.h"
+
+#include <cmath>
+#include <cstring>
+
+namespace gqa {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Page planning.
+//
+// Three running sums over the requests (new tokens, pages needed, pages given
+// back) place everything: every CTA computes them all in shared memory -- a few
+// KB of reads from L2, cheaper than a second launch or a wait between CTAs --
+// and then fills its share of the slots, table entries and stack entries, each
+// found by a binary search in the sums.  A popped page comes from the pages
+// given back in this very call or from below them on the stack, so no CTA reads
+// what another writes.  lens_out and n_free_out may be the inputs: the last CTA
+// to have read those writes them.
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+
+struct PlanArgs {
+    const int32_t *lens, *new_lens;
+    int32_t* block_table;
+    int64_t table_stride;
+    int32_t* free_pages;
+    const int32_t* n_free;
+    int32_t *lens_out, *n_free_out, *first_token;
+    int64_t* slots;
+    int32_t *positions, *counts;
+    uint32_t* ticket;
+    int32_t requests, table_width, free_capacity, page_shift, max_tokens;
+};
+
+// Last index r in [0, n) with first[r] <= x (first is non-decreasing, first[0] = 0).
+__device__ __forceinline__ int last_at_most(const int32_t* first, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_constant__ PlanArgs a) {
+    extern __shared__ int32_t sums[];  // tokens, needs, gives: [requests + 1] each
+    __shared__ long long warp_sum[3][32];
+    __shared__ int s_bad;
+    __shared__ bool s_last;
+    const int n = a.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int32_t* tokens = sums;
+    int32_t* needs = sums + (n + 1);
+    int32_t* gives = sums + 2 * (n + 1);
+    const int page_mask = (1 << a.page_shift) - 1;
+    auto pages_of = [&](long long len) { return (int)((len + page_mask) >> a.page_shift); };
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+
+    // Each thread sums a stretch of consecutive requests, then the block scans the stretches.
+    const int per = (n + kPlanThreads - 1) / kPlanThreads;
+    const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
+    long long sum[3] = {0, 0, 0};
+    bool bad = false;
+    for (int r = r0; r < r1; ++r) {
+        const int len = a.lens[r], add = a.new_lens[r];
+        bad |= len < 0 || pages_of(len) > a.table_width;
+        if (add < 0) {
+            sum[2] += pages_of(len);
+        } else {
+            const long long after = (long long)len + add;
+            bad |= after > 0x7FFFFFFF || pages_of(after) > a.table_width;
+            sum[0] += add;
+            sum[1] += pages_of(after) - pages_of(len);
+        }
+    }
+    long long incl[3] = {sum[0], sum[1], sum[2]};
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const long long x = __shfl_up_sync(0xffffffffu, incl[i], d);
+            if (lane >= d) incl[i] += x;
+        }
+    }
+    if (lane == 31)
+        for (int i = 0; i < 3; ++i) warp_sum[i][warp] = incl[i];
+    if (bad) s_bad = 1;
+    __syncthreads();
+    long long total[3] = {0, 0, 0}, base[3] = {0, 0, 0};
+    for (int w = 0; w < 32; ++w) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            if (w < warp) base[i] += warp_sum[i][w];
+            total[i] += warp_sum[i][w];
+        }
+    }
+    const int n_free = *a.n_free;
+    // All or nothing.  (The sums in shared memory are 32-bit: with `ok` they fit.)
+    const bool ok = !s_bad && n_free >= 0 && total[0] <= a.max_tokens && n_free + total[2] <= a.free_capacity &&
+                    total[1] <= n_free + total[2];
+    {
+        long long at[3] = {base[0] + incl[0] - sum[0], base[1] + incl[1] - sum[1], base[2] + incl[2] - sum[2]};
+        for (int r = r0; r < r1; ++r) {
+            const int len = a.lens[r], add = a.new_lens[r];
+            tokens[r] = ok ? (int32_t)at[0] : 0;
+            needs[r] = (int32_t)at[1];
+            gives[r] = (int32_t)at[2];
+            if (add < 0) {
+                at[2] += pages_of(len);
+            } else {
+                at[0] += add;
+                at[1] += pages_of((long long)len + add) - pages_of(len);
+            }
+        }
+        if (tid == 0) {
+            tokens[n] = ok ? (int32_t)total[0] : 0;
+            needs[n] = (int32_t)total[1];
+            gives[n] = (int32_t)total[2];
+        }
+    }
+    __syncthreads();
+
+    const int stride = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
+    const int n_tokens = tokens[n], n_need = ok ? needs[n] : 0, n_give = ok ? gives[n] : 0;
+    for (int r = first; r <= n; r += stride) a.first_token[r] = tokens[r];
+    // Page given back number i: its request is the last whose sum is at most i
+    // and which gives any (requests that give none repeat the next one's sum).
+    auto given = [&](int i) {
+        const int r = last_at_most(gives, n, i);
+        return a.block_table[r * a.table_stride + (i - gives[r])];
+    };
+    // Page popped number j: the top of the stack with this call's pages pushed on it.
+    auto popped = [&](int j) { return j < n_give ? given(n_give - 1 - j) : a.free_pages[n_free - 1 - (j - n_give)]; };
+    for (int t = first; t < a.max_tokens; t += stride) {
+        int64_t slot = -1;
+        int pos = -1;
+        if (t < n_tokens) {
+            const int r = last_at_most(tokens, n, t);
+            const int len = a.lens[r], held = pages_of(len);
+            pos = len + (t - tokens[r]);
+            const int col = pos >> a.page_shift;
+            const int page = col < held ? a.block_table[r * a.table_stride + col] : popped(needs[r] + col - held);
+            slot = ((int64_t)page << a.page_shift) + (pos & page_mask);
+        }
+        a.slots[t] = slot;
+        a.positions[t] = pos;
+    }
+    for (int j = first; j < n_need; j += stride) {
+        const int r = last_at_most(needs, n, j);
+        a.block_table[r * a.table_stride + pages_of(a.lens[r]) + (j - needs[r])] = popped(j);
+    }
+    for (int i = first; i < n_give; i += stride) a.free_pages[n_free + i] = given(i);
+    if (blockIdx.x == 0 && tid == 0) {
+        a.counts[0] = n_tokens;
+        a.counts[1] = n_need;
+        a.counts[2] = n_give;
+        a.counts[3] = ok ? GQA_OK : GQA_ERR_PAGES;
+    }
+    // Every CTA has read lens and n_free once all have arrived here.
+    __syncthreads();
+    if (tid == 0) {
+        bool last = true;
+        if (gridDim.x > 1) {
+            __threadfence();
+            last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+            __threadfence();
+            if (last) *a.ticket = 0;
+        }
+        s_last = last;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    for (int r = tid; r < n; r += kPlanThreads) {
+        const int len = a.lens[r], add = a.new_lens[r];
+        a.lens_out[r] = !ok ? len : add < 0 ? 0 : len + add;
+    }
+    if (tid == 0) *a.n_free_out = ok ? n_free + n_give - n_need : n_free;
+}
+
+// ---------------------------------------------------------------------------
+// Append: RoPE of K, quantisation, and the rescale of a page's earlier codes.
+//
+// A CTA takes the runs that start in its window of tokens, for one head of K or
+// V (grid: windows x heads x {K, V}).  With 2 * page_len threads a run's rows fit
+// the registers (8 threads a row, each 8 rotate_half pairs; 4 rows a thread), so
+// that the rows are read once: amax over the block, then the codes.
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+    PagedCacheView c;
+    const __nv_bfloat16 *k, *v;
+    int64_t k_tstride, k_hstride, v_tstride, v_hstride;
+    const int64_t* slots;
+    const int32_t* positions;
+    int n_tokens, window;
+    RopeSteps rope;
+};
+
+constexpr float kMinBlockScale = 0x1p-100f;  // keeps 1 / scale finite for a block of zeros
+
+template <int kCode>
+__device__ __forceinline__ uint64_t encode8(const float* x, float inv) {
+    uint64_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= (uint64_t)value_code<kCode>(x[e] * inv) << (8 * e);
+    return w;
+}
+
+__device__ __forceinline__ void unpack8(uint4 w, float* x) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = bf16x2_to_float2(ws[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+
+template <int kCode>
+__global__ void __launch_bounds__(2 * kPagedMaxPage) append_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ float s_max[2 * kPagedMaxPage / 32];
+    __shared__ int s_len[2 * kPagedMaxPage / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
+    const int head = blockIdx.y;
+    const bool is_k = blockIdx.z == 0;
+    const int page_len = a.c.page_len, page_mask = page_len - 1;
+    const int64_t n_slots = (int64_t)a.c.pages << a.c.page_shift;
+    const __nv_bfloat16* src = (is_k ? a.k : a.v) + head * (is_k ? a.k_hstride : a.v_hstride);
+    const int64_t tstride = is_k ? a.k_tstride : a.v_tstride;
+    uint8_t* codes = (is_k ? a.c.k : a.c.v) + head * a.c.head_stride;
+    float* scales = (is_k ? a.c.k_scale : a.c.v_scale) + head;
+    const float qmax = kCode == GQA_CODE_INT8 ? 127.f : 448.f;
+    const int chunk = tid & 7, row0 = tid >> 3, rows_per_pass = blockDim.x >> 3;  // page_len / 4
+
+    const int w0 = blockIdx.x * a.window, w1 = min(a.n_tokens, w0 + a.window);
+    for (int t0 = w0; t0 < w1; ++t0) {
+        const int64_t slot = a.slots[t0];
+        if (slot < 0 || slot >= n_slots) continue;  // the whole CTA: slot is uniform
+        const int r0 = (int)(slot & page_mask);
+        if (t0 > 0 && r0 != 0 && a.slots[t0 - 1] == slot - 1) continue;  // inside another run
+        // Rows of the run: up to the page's end, the call's end or the first slot that does not follow.
+        const bool in = tid < page_len - r0 && t0 + tid < a.n_tokens && a.slots[t0 + tid] == slot + tid;
+        const unsigned miss = ~__ballot_sync(0xffffffffu, in);
+        if (lane == 0) s_len[warp] = miss ? __ffs(miss) - 1 : 32;
+        __syncthreads();
+        int len = 0;
+        for (int w = 0; w < n_warps; ++w) {
+            len += s_len[w];
+            if (s_len[w] < 32) break;
+        }
+        const int64_t page = slot >> a.c.page_shift;
+        uint8_t* base = codes + page * a.c.page_stride;
+        float* scale_at = scales + page * a.c.scale_page_stride;
+        const float old = r0 ? *scale_at : 0.f;
+
+        // Rows row0, row0 + rows_per_pass, ...: dims 8 chunk .. and 64 + 8 chunk ..
+        float x[4][16];
+        float most = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int r = row0 + p * rows_per_pass;
+            if (r >= len) continue;
+            const __nv_bfloat16* row = src + (int64_t)(t0 + r) * tstride;
+            unpack8(*reinterpret_cast<const uint4*>(row + 8 * chunk), x[p]);
+            unpack8(*reinterpret_cast<const uint4*>(row + 64 + 8 * chunk), x[p] + 8);
+            if (is_k && a.positions) {
+                const int pos = a.positions[t0 + r];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 f = rope_factor(a.rope.step[8 * chunk + e], pos);
+                    const float re = x[p][e], im = x[p][8 + e];
+                    x[p][e] = re * f.x - im * f.y;
+                    x[p][8 + e] = re * f.y + im * f.x;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                most = fmaxf(most, fabsf(x[p][e]));
+                finite &= fabsf(x[p][e]) <= 3.402823466e38f;
+            }
+        }
+        if (!finite) most = INFINITY;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        if (lane == 0) s_max[warp] = most;
+        __syncthreads();
+        most = s_max[0];
+        for (int w = 1; w < n_warps; ++w) most = fmaxf(most, s_max[w]);
+        const float mine = most == INFINITY ? __int_as_float(0x7fffffff) : fmaxf(__fdiv_rn(most, qmax), kMinBlockScale);
+        const float scale = mine > old || mine != mine ? mine : old;
+        const float inv = scale == scale ? __frcp_rn(scale) : 0.f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int r = row0 + p * rows_per_pass;
+            if (r >= len) continue;
+            if (!(scale == scale))
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[p][e] = 0.f;
+            uint8_t* row = base + (r0 + r) * a.c.row_stride;
+            *reinterpret_cast<uint64_t*>(row + 8 * chunk) = encode8<kCode>(x[p], inv);
+            *reinterpret_cast<uint64_t*>(row + 64 + 8 * chunk) = encode8<kCode>(x[p] + 8, inv);
+        }
+        if (mine > old) {
+            for (int r = row0; r < r0; r += rows_per_pass) {
+                uint8_t* row = base + r * a.c.row_stride;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint64_t* at = reinterpret_cast<uint64_t*>(row + 64 * half + 8 * chunk);
+                    const uint64_t w = *at;
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = code_value<kCode>((uint8_t)(w >> (8 * e))) * old;
+                    *at = encode8<kCode>(y, inv);
+                }
+            }
+        }
+        __syncthreads();  // everyone has read the old scale, s_len and s_max
+        if (tid == 0) *scale_at = scale;
+    }
+}
+
+// Rows back to BF16: one warp a (row, K or V), 4 dims a lane and head.
+struct ReadArgs {
+    PagedCacheView c;
+    const int64_t* slots;
+    __nv_bfloat16 *out_k, *out_v;
+    int n;
+};
+
+template <int kCode>
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadArgs a) {
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= a.n) return;
+    const int64_t slot = a.slots[row];
+    const bool real = slot >= 0 && slot < ((int64_t)a.c.pages << a.c.page_shift);
+    const int64_t page = real ? slot >> a.c.page_shift : 0;
+    const int64_t at = page * a.c.page_stride + (real ? slot & (a.c.page_len - 1) : 0) * a.c.row_stride;
+    const uint8_t* codes = (blockIdx.y ? a.c.v : a.c.k) + at + 4 * lane;
+    const float* scales = (blockIdx.y ? a.c.v_scale : a.c.k_scale) + page * a.c.scale_page_stride;
+    __nv_bfloat16* out = (blockIdx.y ? a.out_v : a.out_k) + (int64_t)row * a.c.kv_heads * kHeadDim + 4 * lane;
+    for (int h = 0; h < a.c.kv_heads; ++h) {
+        uint2 o = make_uint2(0u, 0u);
+        if (real) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + h * a.c.head_stride);
+            const float s = scales[h];
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = code_value<kCode>((uint8_t)(w >> (8 * e))) * s;
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
+            o = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+        *reinterpret_cast<uint2*>(out + h * kHeadDim) = o;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Attention, one warp a Q head, one CTA a (query row, KV head): 32 keys at a
+// time, a key a lane for the scores, 4 dims a lane for the values.
+// ---------------------------------------------------------------------------
+struct SimpleArgs {
+    PagedCall p;
+    RopeSteps rope;
+};
+
+template <int kCode>
+__global__ void __launch_bounds__(kGroup * 32) paged_attention_kernel(const __grid_constant__ SimpleArgs a) {
+    __shared__ float s_q[kGroup][kHeadDim];
+    const PagedCall& p = a.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.x, h = blockIdx.y, qh = h * kGroup + warp;
+    int b = row;
+    int64_t m;
+    if (p.first_query) {
+        if (row >= p.first_query[p.batch]) return;
+        b = 0;
+        while (p.first_query[b + 1] <= row) ++b;
+        m = (int64_t)p.seq_lens[b] - (p.first_query[b + 1] - p.first_query[b]) + (row - p.first_query[b]);
+    } else {
+        m = p.query_positions ? p.query_positions[b] : (int64_t)p.seq_lens[b] - 1;
+    }
+    const KeyRange range = paged_range(p, row, m, paged_length(p, b));
+    const __nv_bfloat16* q = p.q + row * p.q_row_stride + qh * p.q_head_stride;
+    for (int i = lane; i < kPairs; i += 32) {
+        float x = __bfloat162float(q[i]), y = __bfloat162float(q[i + kPairs]);
+        if (!p.q_rotated) {
+            const float2 f = rope_factor(a.rope.step[i], m);
+            const float re = x * f.x - y * f.y;
+            y = x * f.y + y * f.x;
+            x = re;
+        }
+        s_q[warp][i] = x * p.scale;
+        s_q[warp][i + kPairs] = y * p.scale;
+    }
+    __syncwarp();
+    float top = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = range.lo; k0 < range.hi; k0 += 32) {
+        const int key = k0 + lane;
+        const bool seen = key < range.hi;
+        int page = seen ? p.block_table[b * p.table_stride + (key >> p.c.page_shift)] : -1;
+        if (page >= p.c.pages) page = -1;
+        const int64_t at = page < 0 ? 0 : page * p.c.page_stride + (key & (p.c.page_len - 1)) * p.c.row_stride +
+                                              h * p.c.head_stride;
+        float z = 0.f;
+        if (page >= 0) {
+            for (int d = 0; d < kHeadDim; d += 16) {
+                const uint4 w = *reinterpret_cast<const uint4*>(p.c.k + at + d);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    z = fmaf(code_value<kCode>((uint8_t)(ws[e >> 2] >> (8 * (e & 3)))), s_q[warp][d + e], z);
+            }
+            z *= p.c.k_scale[page * p.c.scale_page_stride + h];
+        }
+        if (p.cap > 0.f) z = p.cap * tanhf(z / p.cap);
+        if (p.slopes) z -= p.slopes[qh] * (float)llabs(m - key);
+        if (!seen) z = -INFINITY;
+        float mx = z;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float now = fmaxf(top, mx);
+        const float use = now == -INFINITY ? 0.f : now;
+        const float alpha = expf(top - use);
+        const float w = seen ? expf(z - use) : 0.f;
+        total = total * alpha + w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= alpha;
+        top = now;
+        const float wv = page >= 0 ? w * p.c.v_scale[page * p.c.scale_page_stride + h] : 0.f;
+        const int n = min(32, range.hi - k0);
+        for (int i = 0; i < n; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, wv, i);
+            const int64_t ai = __shfl_sync(0xffffffffu, at, i);
+            if (__shfl_sync(0xffffffffu, page, i) < 0) continue;
+            const uint32_t c = *reinterpret_cast<const uint32_t*>(p.c.v + ai + 4 * lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(wi, code_value<kCode>((uint8_t)(c >> (8 * e))), acc[e]);
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    __nv_bfloat16* out = p.out + row * p.out_row_stride + qh * p.out_head_stride + 4 * lane;
+    const bool any = range.hi > range.lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = __float2bfloat16_rn(any ? acc[e] / total : 0.f);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// A pure function of theta, kept per thread for the value last asked.
+const RopeSteps& rope_steps_of(float theta) {
+    static thread_local float last = 0.f;
+    static thread_local RopeSteps steps;
+    if (last != theta) {
+        for (int i = 0; i < kPairs; ++i) {
+            const double inv = std::pow((double)theta, -2.0 * i / (double)kHeadDim);
+            steps.step[i] = (uint64_t)std::llround(inv / (2.0 * M_PI) * 18446744073709551616.0);
+        }
+        last = theta;
+    }
+    return steps;
+}
+
+int check_cache(const gqa_paged_cache* c, PagedCacheView* v) {
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return GQA_ERR_NULL_POINTER;
+    if (c->kv_heads < 1 || c->kv_heads > kNumKVHeads) return GQA_ERR_KV_HEADS;
+    if (c->code != GQA_CODE_INT8 && c->code != GQA_CODE_E4M3) return GQA_ERR_FLAGS;
+    int shift = 4;
+    while (shift < 7 && (1 << shift) != c->page_len) ++shift;
+    if ((1 << shift) != c->page_len || c->page_len < kPagedMinPage) return GQA_ERR_KV_BLOCK_LEN;
+    if (c->pages < 1) return GQA_ERR_KV_RANGE;
+    if (!aligned16(c->k) || !aligned16(c->v) || ((uintptr_t)c->k_scale & 3) || ((uintptr_t)c->v_scale & 3))
+        return GQA_ERR_ALIGNMENT;
+    // TMA strides: multiples of 16 bytes below 2^40.
+    for (const int64_t s : {c->page_stride, c->row_stride, c->head_stride})
+        if (s < kHeadDim || s % 16 || s >= (int64_t)1 << 40) return GQA_ERR_ALIGNMENT;
+    if (c->scale_page_stride < c->kv_heads) return GQA_ERR_ALIGNMENT;
+    v->k = static_cast<uint8_t*>(c->k);
+    v->v = static_cast<uint8_t*>(c->v);
+    v->k_scale = c->k_scale;
+    v->v_scale = c->v_scale;
+    v->kv_heads = c->kv_heads;
+    v->page_len = c->page_len;
+    v->page_shift = shift;
+    v->pages = c->pages;
+    v->page_stride = c->page_stride;
+    v->row_stride = c->row_stride;
+    v->head_stride = c->head_stride;
+    v->scale_page_stride = c->scale_page_stride;
+    return GQA_OK;
+}
+
+// Checks both attention calls share; fills `call`.
+int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_paged_params* p, bool chunked,
+               PagedCall* call) {
+    if (!q || !out || !c || !p || !p->block_table || !p->seq_lens || (chunked && !p->first_query))
+        return GQA_ERR_NULL_POINTER;
+    std::memset(call, 0, sizeof(*call));
+    const int st = check_cache(c, &call->c);
+    if (st != GQA_OK) return st;
+    if (p->batch < 1 || p->batch > GQA_PAGED_MAX_BATCH || p->rows < 0 || (!chunked && p->rows != p->batch) ||
+        p->table_width < 1 || p->reserved != 0)
+        return GQA_ERR_BATCH;
+    if (p->batch > 1 && p->table_stride < p->table_width) return GQA_ERR_BATCH;
+    if (p->flags & ~GQA_FLAG_Q_ROTATED) return GQA_ERR_FLAGS;
+    if (!(p->scale != 0.f) || !std::isfinite(p->scale)) return GQA_ERR_SCALE;
+    if (!(p->score_cap >= 0.f) || !std::isfinite(p->score_cap)) return GQA_ERR_SCALE;
+    if (!(p->rope_theta > 0.f) || !std::isfinite(p->rope_theta)) return GQA_ERR_ROPE_THETA;
+    if (!aligned16(q) || !aligned16(out)) return GQA_ERR_ALIGNMENT;
+    for (const int64_t s : {p->q_row_stride, p->q_head_stride, p->out_row_stride, p->out_head_stride})
+        if (s < 0 || s % 8) return GQA_ERR_ALIGNMENT;
+    call->q = static_cast<const __nv_bfloat16*>(q);
+    call->out = static_cast<__nv_bfloat16*>(out);
+    call->block_table = p->block_table;
+    call->seq_lens = p->seq_lens;
+    call->query_positions = chunked ? nullptr : p->query_positions;
+    call->first_query = chunked ? p->first_query : nullptr;
+    call->doc_starts = p->doc_starts;
+    call->prefix_ends = p->prefix_ends;
+    call->slopes = p->slopes;
+    call->table_stride = p->table_stride;
+    call->q_row_stride = p->q_row_stride;
+    call->q_head_stride = p->q_head_stride;
+    call->out_row_stride = p->out_row_stride;
+    call->out_head_stride = p->out_head_stride;
+    call->batch = p->batch;
+    call->rows = p->rows;
+    call->table_width = p->table_width;
+    call->scale = p->scale;
+    call->cap = p->score_cap;
+    call->q_rotated = (p->flags & GQA_FLAG_Q_ROTATED) != 0;
+    int sms = 0;
+    const int dev = device_sms(&sms);
+    if (dev != GQA_OK) return dev;
+    return check_device_memory({q, out, c->k, c->v, c->k_scale, c->v_scale, p->block_table, p->seq_lens,
+                                call->query_positions, call->first_query, p->doc_starts, p->prefix_ends, p->slopes});
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA; }
+
+int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p, void* workspace,
+           size_t workspace_bytes, void* stream, bool chunked) {
+    SimpleArgs a;
+    int st = check_call(q, out, cache, p, chunked, &a.p);
+    if (st != GQA_OK) return st;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < gqa_paged_workspace_bytes(cache, p))
+        return GQA_ERR_WORKSPACE;
+    st = check_device_memory({workspace});
+    if (st != GQA_OK) return st;
+    if (p->rows == 0) return GQA_OK;
+    a.rope = rope_steps_of(p->rope_theta);
+    const dim3 grid(p->rows, cache->kv_heads);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (cache->code == GQA_CODE_INT8)
+        paged_attention_kernel<GQA_CODE_INT8><<<grid, kGroup * 32, 0, s>>>(a);
+    else
+        paged_attention_kernel<GQA_CODE_E4M3><<<grid, kGroup * 32, 0, s>>>(a);
+    return launched();
+}
+
+}  // namespace
+
+}  // namespace gqa
+
+using namespace gqa;
+
+extern "C" {
+
+int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, int32_t* block_table,
+                   int64_t table_stride, int table_width, int32_t* free_pages, int free_capacity,
+                   const int32_t* n_free, int page_len, int max_tokens, int32_t* lens_out, int32_t* n_free_out,
+                   int32_t* first_token, int64_t* slots, int32_t* positions, int32_t* counts, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    if (!lens || !new_lens || !block_table || !free_pages || !n_free || !lens_out || !n_free_out || !first_token ||
+        !counts || (max_tokens > 0 && (!slots || !positions)))
+        return GQA_ERR_NULL_POINTER;
+    if (requests < 1 || requests > GQA_PAGED_MAX_BATCH || table_width < 1 || free_capacity < 0 || max_tokens < 0 ||
+        (requests > 1 && table_stride < table_width))
+        return GQA_ERR_BATCH;
+    int shift = 4;
+    while (shift < 7 && (1 << shift) != page_len) ++shift;
+    if ((1 << shift) != page_len) return GQA_ERR_KV_BLOCK_LEN;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < GQA_CHUNKED_WORKSPACE_BYTES) return GQA_ERR_WORKSPACE;
+    int sms = 0;
+    int st = device_sms(&sms);
+    if (st != GQA_OK) return st;
+    st = check_device_memory({lens, new_lens, block_table, free_pages, n_free, lens_out, n_free_out, first_token,
+                                  slots, positions, counts, workspace});
+    if (st != GQA_OK) return st;
+    PlanArgs a;
+    a.lens = lens;
+    a.new_lens = new_lens;
+    a.block_table = block_table;
+    a.table_stride = table_stride;
+    a.free_pages = free_pages;
+    a.n_free = n_free;
+    a.lens_out = lens_out;
+    a.n_free_out = n_free_out;
+    a.first_token = first_token;
+    a.slots = slots;
+    a.positions = positions;
+    a.counts = counts;
+    a.ticket = static_cast<uint32_t*>(workspace) + 1;
+    a.requests = requests;
+    a.table_width = table_width;
+    a.free_capacity = free_capacity;
+    a.page_shift = shift;
+    a.max_tokens = max_tokens;
+    const size_t smem = 3 * (size_t)(requests + 1) * sizeof(int32_t);
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)smem) != cudaSuccess)
+        return GQA_ERR_CUDA;
+    const int64_t items = max_tokens > requests ? max_tokens : requests;
+    int64_t grid = (items + kPlanThreads - 1) / kPlanThreads;
+    if (grid > 128) grid = 128;
+    plan_pages_kernel<<<(int)grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+    return launched();
+}
+
+int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, const int32_t* positions,
+                     float rope_theta, const gqa_paged_cache* cache, void* stream) {
+    if (!k || !v || !slots || !cache) return GQA_ERR_NULL_POINTER;
+    AppendArgs a;
+    int st = check_cache(cache, &a.c);
+    if (st != GQA_OK) return st;
+    if (n_tokens < 0) return GQA_ERR_BATCH;
+    if (!(rope_theta > 0.f) || !std::isfinite(rope_theta)) return GQA_ERR_ROPE_THETA;
+    if (!aligned16(k) || !aligned16(v)) return GQA_ERR_ALIGNMENT;
+    for (const int64_t s : {k_token_stride, k_head_stride, v_token_stride, v_head_stride})
+        if (s < 0 || s % 8) return GQA_ERR_ALIGNMENT;
+    int sms = 0;
+    st = device_sms(&sms);
+    if (st != GQA_OK) return st;
+    st = check_device_memory({k, v, slots, positions, cache->k, cache->v, cache->k_scale, cache->v_scale});
+    if (st != GQA_OK) return st;
+    if (n_tokens == 0) return GQA_OK;
+    a.k = static_cast<const __nv_bfloat16*>(k);
+    a.v = static_cast<const __nv_bfloat16*>(v);
+    a.k_tstride = k_token_stride;
+    a.k_hstride = k_head_stride;
+    a.v_tstride = v_token_stride;
+    a.v_hstride = v_head_stride;
+    a.slots = slots;
+    a.positions = positions;
+    a.n_tokens = n_tokens;
+    a.window = n_tokens <= 2048 ? 1 : 16;
+    a.rope = rope_steps_of(rope_theta);
+    const dim3 grid((n_tokens + a.window - 1) / a.window, cache->kv_heads, 2);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (cache->code == GQA_CODE_INT8)
+        append_kernel<GQA_CODE_INT8><<<grid, 2 * cache->page_len, 0, s>>>(a);
+    else
+        append_kernel<GQA_CODE_E4M3><<<grid, 2 * cache->page_len, 0, s>>>(a);
+    return launched();
+}
+
+int gqa_read_paged(const gqa_paged_cache* cache, const int64_t* slots, int n, void* out_k, void* out_v, void* stream) {
+    if (!cache || !slots || !out_k || !out_v) return GQA_ERR_NULL_POINTER;
+    ReadArgs a;
+    int st = check_cache(cache, &a.c);
+    if (st != GQA_OK) return st;
+    if (n < 0) return GQA_ERR_BATCH;
+    if (!aligned16(out_k) || !aligned16(out_v)) return GQA_ERR_ALIGNMENT;
+    int sms = 0;
+    st = device_sms(&sms);
+    if (st != GQA_OK) return st;
+    st = check_device_memory({cache->k, cache->v, cache->k_scale, cache->v_scale, slots, out_k, out_v});
+    if (st != GQA_OK) return st;
+    if (n == 0) return GQA_OK;
+    a.slots = slots;
+    a.out_k = static_cast<__nv_bfloat16*>(out_k);
+    a.out_v = static_cast<__nv_bfloat16*>(out_v);
+    a.n = n;
+    const dim3 grid((n + 7) / 8, 2);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (cache->code == GQA_CODE_INT8)
+        read_kernel<GQA_CODE_INT8><<<grid, 256, 0, s>>>(a);
+    else
+        read_kernel<GQA_CODE_E4M3><<<grid, 256, 0, s>>>(a);
+    return launched();
+}
+
+size_t gqa_paged_workspace_bytes(const gqa_paged_cache* cache, const gqa_paged_params* p) {
+    if (!cache || !p || p->batch < 1 || p->batch > GQA_PAGED_MAX_BATCH || p->rows < 0 || cache->kv_heads < 1 ||
+        cache->kv_heads > kNumKVHeads)
+        return 0;
+    return GQA_CHUNKED_WORKSPACE_BYTES;
+}
+
+int gqa_decode_paged(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(q, out, cache, p, workspace, workspace_bytes, stream, false);
+}
+
+int gqa_decode_paged_chunked(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(q, out, cache, p, workspace, workspace_bytes, stream, true);
+}
+
+}  // extern "C"

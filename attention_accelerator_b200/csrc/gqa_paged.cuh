@@ -1,0 +1,92 @@
+// gqa_paged.cuh -- what the paged 8-bit cache's kernels share: the cache and
+// call descriptions they take by value, the visible range of a query and the
+// conversions between codes and values.
+#pragma once
+
+#include "gqa_b200.h"
+#include "gqa_device.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace gqa {
+
+constexpr int kPagedMinPage = 16, kPagedMaxPage = 128;
+
+// Q0.64 turns per position of each rotate_half pair, passed by value.
+struct RopeSteps {
+    uint64_t step[kPairs];
+};
+
+struct PagedCacheView {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    int32_t kv_heads, page_len, page_shift, pages;
+    int64_t page_stride, row_stride, head_stride, scale_page_stride;
+};
+
+// One attention call over the cache (gqa_paged_params, checked).
+struct PagedCall {
+    PagedCacheView c;
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    const int32_t* block_table;
+    const int32_t *seq_lens, *query_positions, *first_query;
+    const int32_t *doc_starts, *prefix_ends;
+    const float* slopes;
+    int64_t table_stride;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    int32_t batch, rows, table_width;
+    float scale, cap;
+    int32_t q_rotated;
+};
+
+// Keys of sequence b that can be visible at all: its length, cut to what its
+// block-table row can name.
+__device__ __forceinline__ int paged_length(const PagedCall& a, int b) {
+    const int64_t room = (int64_t)a.table_width << a.c.page_shift;
+    const int n = a.seq_lens[b];
+    return n < 0 ? 0 : (int)(n < room ? n : room);
+}
+
+struct KeyRange {
+    int lo, hi;  // visible keys lo <= p < hi (none where hi <= lo)
+};
+
+// Visible keys of query row `row` at position m of a sequence with `len` keys.
+__device__ __forceinline__ KeyRange paged_range(const PagedCall& a, int row, int64_t m, int len) {
+    int64_t hi = m + 1;
+    if (a.prefix_ends) {
+        const int e = a.prefix_ends[row];
+        if (e > hi) hi = e;
+    }
+    if (hi > len) hi = len;
+    if (hi < 0) hi = 0;
+    int lo = a.doc_starts ? a.doc_starts[row] : 0;
+    if (lo < 0) lo = 0;
+    return KeyRange{lo, (int)hi};
+}
+
+// Value of one code.
+template <int kCode>
+__device__ __forceinline__ float code_value(uint8_t c) {
+    if constexpr (kCode == GQA_CODE_INT8) {
+        return (float)(int8_t)c;
+    } else {
+        const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+        return __half2float(__half(h));
+    }
+}
+
+// Code of a value already divided by its scale: round to nearest even, saturating.
+template <int kCode>
+__device__ __forceinline__ uint8_t value_code(float y) {
+    if constexpr (kCode == GQA_CODE_INT8) {
+        const int i = __float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
+        return (uint8_t)(int8_t)i;
+    } else {
+        return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    }
+}
+
+}  // namespace gqa

@@ -59,7 +59,10 @@ enum gqa_status {
     GQA_ERR_FLAGS = 17,            /* gqa_params.flags holds a bit this entry point does not know */
     GQA_ERR_MEMORY = 18,           /* a tensor, table or workspace pointer is not memory of the current
                                       GPU (host memory, pageable or pinned, or another GPU's memory) */
-    GQA_ERR_KV_HEADS = 19          /* KV-head range empty or outside [0, 8) (gqa_decode_heads) */
+    GQA_ERR_KV_HEADS = 19,         /* KV-head range empty or outside [0, 8) (gqa_decode_heads), or a paged
+                                      cache's head count outside [1, 8] */
+    GQA_ERR_PAGES = 20             /* page planning refused: too few free pages, a block-table row too
+                                      short, more new tokens than max_tokens, or a length out of range */
 };
 
 /* GQA_FLAG_* values for gqa_params.flags. */
@@ -463,6 +466,138 @@ size_t gqa_mem_encode_bytes(uint64_t n_rows, int elements);
  * gqa_mem_encode_bytes(n_rows, elements) bytes.  Asynchronous on `stream`.
  */
 int gqa_mem_encode(const void *rows, uint64_t n_rows, int elements, void *text, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged 8-bit KV cache.
+ *
+ * The cache is a pool of `pages` pages of `page_len` tokens.  Each (page, KV
+ * head) block of K, and of V, holds 8-bit codes and one FP32 scale: the value
+ * of a code c is c * scale.  A sequence's key p lives in page
+ * block_table[b][p / page_len], row p % page_len.  Page planning, the append
+ * and both attention calls take their lengths from device memory, so a step's
+ * lengths may change under a captured CUDA graph.  No reference counterpart:
+ * the reference streams one contiguous K/V transport per START
+ * (gen_gqa_wrapper_vectors.py:116-119).
+ * ------------------------------------------------------------------------- */
+#define GQA_CODE_INT8 0   /* round to nearest even of value / scale, in [-127, 127] */
+#define GQA_CODE_E4M3 1   /* FP8: 4 exponent bits, 3 mantissa bits, largest 448 */
+#define GQA_PAGED_MAX_BATCH 8192
+
+/*
+ * Strides are in bytes (= codes), multiples of 16, the same for K and V; the
+ * code of (page, row, head, dim) is at page*page_stride + row*row_stride +
+ * head*head_stride + dim.  The scale of (page, head) is at
+ * page*scale_page_stride + head (floats).  k and v are 16-byte aligned.
+ */
+typedef struct gqa_paged_cache {
+    void   *k, *v;
+    float  *k_scale, *v_scale;
+    int32_t code;       /* GQA_CODE_* */
+    int32_t kv_heads;   /* 1..8 (8, or a head shard's) */
+    int32_t page_len;   /* 16, 32, 64 or 128 */
+    int32_t pages;
+    int64_t page_stride, row_stride, head_stride;
+    int64_t scale_page_stride;
+} gqa_paged_cache;
+
+/*
+ * Page planning of one step, entirely on the GPU.  Request r holds lens[r]
+ * tokens and gets new_lens[r] more (0: none); new_lens[r] < 0 says that it has
+ * finished: its pages go back and its length becomes 0.
+ *  - free_pages is a stack of free page numbers, entries [0, *n_free) valid.
+ *    The pages of finished requests are pushed (in the order of requests, then
+ *    columns), then the new pages of growing requests are popped from the top in
+ *    the order of requests and stored in block_table[r][ceil(lens[r] / page_len)...].
+ *  - first_token[0..requests]: running sum of the new tokens.  For new token t
+ *    of request r, i = t - first_token[r]: positions[t] = lens[r] + i, slots[t] =
+ *    block_table[r][positions[t] / page_len] * page_len + positions[t] % page_len.
+ *    Entries past the total, up to max_tokens, are -1.
+ *  - lens_out / n_free_out: lengths and stack height after the step; they may be
+ *    lens / n_free themselves.
+ *  - counts[4]: new tokens, pages taken, pages given back, status.
+ * All or nothing: when the free pages do not suffice, a row of block_table is too
+ * short, the tokens exceed max_tokens, the stack would pass free_capacity, or a
+ * length is negative, counts[3] is GQA_ERR_PAGES, slots and positions are -1,
+ * first_token 0, and no page, length or stack entry changes.
+ * `workspace`: GQA_CHUNKED_WORKSPACE_BYTES bytes, zero at allocation, used by no
+ * other call at the same time.  requests <= GQA_PAGED_MAX_BATCH.  Asynchronous.
+ */
+int gqa_plan_pages(const int32_t *lens, const int32_t *new_lens, int requests, int32_t *block_table,
+                   int64_t table_stride, int table_width, int32_t *free_pages, int free_capacity,
+                   const int32_t *n_free, int page_len, int max_tokens, int32_t *lens_out, int32_t *n_free_out,
+                   int32_t *first_token, int64_t *slots, int32_t *positions, int32_t *counts, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/*
+ * Append n_tokens K and V rows (BF16, token t head h at k + t*k_token_stride +
+ * h*k_head_stride elements) to the cache at slots[t] (-1: skipped, as is a slot
+ * outside the cache).  With `positions`, K is rotated at positions[t] first, in
+ * FP32 (rope_half_split, gen_gqa_wrapper_vectors.py:25-35); NULL stores it as it is.
+ * The tokens of one page must be consecutive in the call with consecutive slots
+ * (a "run"), as gqa_plan_pages lays them out.  For each run and head:
+ *   scale = max(old scale (0 if the run starts the page), amax / Qmax, 2^-100), Qmax 127 or 448
+ *   code  = RNE(x * (1 / scale)); if the scale grew, the page's earlier codes c
+ *           become RNE((c * old scale) * (1 / scale)).
+ * A run with a NaN or infinity gives its block a NaN scale (and codes of 0).
+ */
+int gqa_append_paged(const void *k, const void *v, int n_tokens, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, const int64_t *slots, const int32_t *positions,
+                     float rope_theta, const gqa_paged_cache *cache, void *stream);
+
+/*
+ * Read rows back: out_k / out_v BF16 [n][kv_heads][128] contiguous, row i the
+ * values code * scale of slots[i] (zeros for a slot outside the cache).
+ */
+int gqa_read_paged(const gqa_paged_cache *cache, const int64_t *slots, int n, void *out_k, void *out_v, void *stream);
+
+/*
+ * Attention over the paged cache.  Query row i (of sequence b, at position m,
+ * rotated at m unless GQA_FLAG_Q_ROTATED) and Q head qh of KV head h = qh / 4:
+ *   z_p = scale * <q, K_p>;  with score_cap > 0: z_p = cap * tanh(z_p / cap);
+ *   with slopes: z_p -= slopes[qh] * |m - p|;
+ *   visible keys: max(0, doc_starts[i]) <= p < min(seq_lens[b], max(m + 1, prefix_ends[i]));
+ *   out = softmax(z) V over the visible keys, BF16; a row that sees no key is 0.
+ * doc_starts (document mask: the first key of the query's document; default 0)
+ * and prefix_ends (prefix mask: keys below it are visible whatever the query's
+ * position; default 0) are per query row, NULL for none.  Keys outside the
+ * visible range never influence a result, whatever their codes; a block's NaN
+ * scale reaches a row only through a visible key.  Page numbers outside
+ * [0, pages) read as zeros, and no key at or past table_width * page_len is visible.
+ */
+typedef struct gqa_paged_params {
+    int32_t batch;               /* 1..GQA_PAGED_MAX_BATCH */
+    int32_t rows;                /* query rows: batch for gqa_decode_paged */
+    const int32_t *block_table;  /* [batch][table_width], rows table_stride apart */
+    int64_t table_stride;
+    int32_t table_width;
+    uint32_t flags;              /* 0 or GQA_FLAG_Q_ROTATED */
+    const int32_t *seq_lens;     /* [batch] */
+    const int32_t *query_positions; /* gqa_decode_paged: [batch], or NULL: seq_len - 1 */
+    const int32_t *first_query;  /* gqa_decode_paged_chunked: [batch + 1] running sum of each sequence's
+                                    queries; query i of sequence b sits at seq_lens[b] - n_b + i */
+    const int32_t *doc_starts;   /* [rows] or NULL */
+    const int32_t *prefix_ends;  /* [rows] or NULL */
+    const float   *slopes;       /* [4 * kv_heads] or NULL */
+    float   scale;
+    float   score_cap;           /* 0: none */
+    float   rope_theta;
+    uint32_t reserved;           /* must be 0 */
+    int64_t q_row_stride, q_head_stride;      /* elements, multiples of 8 */
+    int64_t out_row_stride, out_head_stride;
+} gqa_paged_params;
+
+/* Device workspace of either call, on the current device (0 on invalid input):
+ * zero at allocation, kept between calls, used by the paged calls of one stream only. */
+size_t gqa_paged_workspace_bytes(const gqa_paged_cache *cache, const gqa_paged_params *p);
+
+/* One query a sequence: q, out [batch][4 * kv_heads][128]. */
+int gqa_decode_paged(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
+/* Any number of queries a sequence, packed: q, out [rows][4 * kv_heads][128].
+ * Rows at or past first_query[batch] are not written. */
+int gqa_decode_paged_chunked(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
+                             void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
