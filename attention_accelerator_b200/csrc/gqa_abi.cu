@@ -4,6 +4,7 @@
 #include "gqa_b200.h"
 #include "gqa_device.cuh"
 #include "gqa_internal.h"
+#include "gqa_paged_internal.h"
 
 #include <cudaTypedefs.h>
 
@@ -80,7 +81,8 @@ int current_device(int* sms) {
         }
         if (major != 10 || minor != 0) {
             di.status = GQA_ERR_UNSUPPORTED_DEVICE;
-        } else if (gqa::decode_prepare(dev) != cudaSuccess || gqa::chunked_prepare() != cudaSuccess) {
+        } else if (gqa::decode_prepare(dev) != cudaSuccess || gqa::chunked_prepare() != cudaSuccess ||
+                   gqa::paged_decode_prepare() != cudaSuccess) {
             di.status = GQA_ERR_CUDA;
         }
         di.sms = n;
@@ -412,6 +414,20 @@ int fill_args(gqa::DecodeArgs& a, const void* q, const void* k, const void* v, v
 }  // namespace
 
 int gqa::device_sms(int* sms) { return current_device(sms); }
+
+int gqa::paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+    if (!encode) return GQA_ERR_CUDA;
+    const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)c.page_len, (cuuint64_t)c.kv_heads,
+                                (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.row_stride, (cuuint64_t)c.head_stride, (cuuint64_t)c.page_stride};
+    const cuuint32_t box[4] = {(cuuint32_t)kHeadDim, (cuuint32_t)(c.page_len < 64 ? c.page_len : 64), 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box,
+                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? GQA_OK : GQA_ERR_ALIGNMENT;
+}
 
 extern "C" {
 

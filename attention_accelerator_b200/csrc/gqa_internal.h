@@ -21,6 +21,8 @@ int check_device_memory(std::initializer_list<const void*> ptrs);
 // (GQA_ERR_UNSUPPORTED_DEVICE where it is not an sm_100 GPU).
 int device_sms(int* sms);
 
+cudaError_t paged_decode_prepare();
+
 struct DecodeArgs;
 struct RopeTable;
 

@@ -2,6 +2,7 @@
 // points, page planning, append (RoPE, quantisation) and read-back kernels.
 #include "gqa_paged.cuh"
 #include "gqa_internal.h"
+#include "gqa_paged_internal.h"
 
 #include <cmath>
 #include <cstring>
@@ -536,9 +537,10 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
     call->scale = p->scale;
     call->cap = p->score_cap;
     call->q_rotated = (p->flags & GQA_FLAG_Q_ROTATED) != 0;
-    int sms = 0;
-    const int dev = device_sms(&sms);
-    if (dev != GQA_OK) return dev;
+    // Key positions and tile counts are 32-bit.
+    if ((int64_t)p->table_width * c->page_len > 0x7FFFFFFF ||
+        (int64_t)p->batch * p->table_width * (c->page_len / 64 + 1) > 0x7FFFFFFF)
+        return GQA_ERR_BATCH;
     return check_device_memory({q, out, c->k, c->v, c->k_scale, c->v_scale, p->block_table, p->seq_lens,
                                 call->query_positions, call->first_query, p->doc_starts, p->prefix_ends, p->slopes});
 }
@@ -550,14 +552,26 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     SimpleArgs a;
     int st = check_call(q, out, cache, p, chunked, &a.p);
     if (st != GQA_OK) return st;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < gqa_paged_workspace_bytes(cache, p))
-        return GQA_ERR_WORKSPACE;
+    if (!workspace || !aligned16(workspace)) return GQA_ERR_WORKSPACE;
+    int sms = 0;
+    st = device_sms(&sms);
+    if (st != GQA_OK) return st;
+    if (workspace_bytes < paged_decode_workspace(sms)) return GQA_ERR_WORKSPACE;
     st = check_device_memory({workspace});
     if (st != GQA_OK) return st;
     if (p->rows == 0) return GQA_OK;
     a.rope = rope_steps_of(p->rope_theta);
     const dim3 grid(p->rows, cache->kv_heads);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!chunked) {
+        CUtensorMap kmap, vmap;
+        if ((st = paged_map(&kmap, a.p.c.k, a.p.c)) != GQA_OK || (st = paged_map(&vmap, a.p.c.v, a.p.c)) != GQA_OK)
+            return st;
+        return launch_paged_decode(a.p, a.rope, cache->code, kmap, vmap, sms, static_cast<uint8_t*>(workspace), s) ==
+                       cudaSuccess
+                   ? GQA_OK
+                   : GQA_ERR_CUDA;
+    }
     if (cache->code == GQA_CODE_INT8)
         paged_attention_kernel<GQA_CODE_INT8><<<grid, kGroup * 32, 0, s>>>(a);
     else
@@ -692,7 +706,9 @@ size_t gqa_paged_workspace_bytes(const gqa_paged_cache* cache, const gqa_paged_p
     if (!cache || !p || p->batch < 1 || p->batch > GQA_PAGED_MAX_BATCH || p->rows < 0 || cache->kv_heads < 1 ||
         cache->kv_heads > kNumKVHeads)
         return 0;
-    return GQA_CHUNKED_WORKSPACE_BYTES;
+    int sms = 0;
+    if (device_sms(&sms) != GQA_OK) return 0;
+    return paged_decode_workspace(sms);
 }
 
 int gqa_decode_paged(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,

@@ -1,0 +1,703 @@
+// gqa_paged_decode.cu -- one token a sequence over the paged 8-bit cache.
+//
+// Work.  A unit is one (sequence, KV head); its visible keys are cut into tiles
+// of 64 on a grid of absolute positions.  All tiles of all units, in order, are
+// dealt out evenly: CTA i of G (one per SM) takes tiles [T i / G, T (i + 1) / G),
+// whatever the lengths -- which only the GPU knows, so every CTA first sums the
+// sequences' tiles itself.  A unit inside one CTA's share is written out by it; a
+// unit that crosses shares leaves FP32 partial rows (at most two per CTA), and
+// the last of its CTAs to finish merges them in CTA order, so that results do not
+// depend on which one that is.
+//
+// A CTA is 8 consumer warps, a loader warp and a query warp.
+//   loader   block-table entries and scales 32 pages at a time, one a lane; per
+//            tile one TMA box per page of K and of V (64 rows of 128 codes in
+//            all, 128-byte swizzle) into a ring of 16 KB stages, and the pages'
+//            scales beside them.  Pages with no visible key are not loaded.
+//   query    per unit, the 4 Q rows rotated in FP32, divided by a power of two
+//            that brings the row's largest below 1, and split into two FP16
+//            parts (22 bits): 8 columns, the N of an m16n8k16 product.
+//   consumer takes whole tiles, the ring's every 8th.  The M of its products is
+//            the keys: S^T = K Q^T, 16 keys x (4 heads x {high, low}), 8 products
+//            deep; codes become FP16 exactly, so a score carries FP32's error
+//            only.  Softmax runs in the result's layout (lane: 2 keys of one
+//            head) without a shuffle but for the maximum.  The weights, times
+//            their page's V scale over a running power of two, split into two
+//            FP16 parts again, and movmatrix turns them into the other product's
+//            operand: O^T = V^T P^T, M 16 dims, whose operand lanes build from
+//            the 16-byte pieces of 4 keys by byte permutes.
+// Why mma.sync and not tcgen05: with 4 queries a KV head there is nothing to
+// amortise a 16-bit copy of K and V in shared memory over; here a code goes from
+// its 8-bit stage through registers into the product once.
+#include "gqa_internal.h"
+#include "gqa_paged.cuh"
+#include "gqa_paged_internal.h"
+
+#include <cstring>
+
+namespace gqa {
+
+namespace {
+
+constexpr int kWarps = 8;                      // consumer warps
+constexpr int kConsumers = kWarps * 32;
+constexpr int kLoaderWarp = kWarps, kQueryWarp = kWarps + 1;
+constexpr int kThreads = (kWarps + 2) * 32;
+constexpr int kTile = 64;                      // keys
+constexpr int kHalfBytes = kTile * kHeadDim;   // K or V of a tile
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kMaxStages = 12;
+constexpr int kPagesPerTile = kTile / kPagedMinPage;
+constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
+
+// Shared memory behind the ring (bytes).
+constexpr int kRowF = kHeadDim + 4;  // padded partial row
+struct alignas(16) Slot {            // one unit's queries (two slots)
+    __half q[2 * kGroup][kHeadDim];  // row 2 head: high parts, 2 head + 1: low parts
+    float factor[kGroup];            // scale * log2(e) (or / cap) * the row's power of two
+    float slope[kGroup];             // times log2(e)
+    int lo, hi, m, pad;
+};
+struct alignas(16) Shared {
+    uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2];
+    float scales[kMaxStages][2][kPagesPerTile];  // K, V
+    Slot slot[2];
+    float acc[kWarps][kGroup][kRowF];
+    float m[kWarps][kGroup], l[kWarps][kGroup];
+    int last;
+    int sum[kThreads / 32];
+};
+
+struct alignas(64) DecodePagedArgs {
+    CUtensorMap kmap, vmap;  // (128, page_len, heads, pages) bytes, box (128, min(page_len, 64), 1, 1)
+    PagedCall p;
+    RopeSteps rope;
+    uint32_t* status;
+    uint32_t* arrivals;  // [batch * heads], zero between calls
+    float* partials;     // [grid][2][4][132]
+    int stages;
+};
+
+__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int row, int head, int page,
+                                              uint64_t* bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(head), "r"(page), "r"(smem_addr(bar)), "l"(policy)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// The sequences' tiles, in shared memory: first[b] the running sum (per head),
+// base[b] the first visible tile.
+struct TileIndex {
+    const int *first, *base;
+    int batch, heads;
+};
+
+// A CTA's walk through its share of the tiles, one unit's piece at a time.
+struct Walk {
+    int64_t x, end;      // next tile, end of the share
+    int b, h;            // unit
+    int tile, n;         // absolute first tile and tiles of the piece
+    int64_t unit_first;  // the unit's first tile in the whole order
+    int unit_tiles;
+    __device__ __forceinline__ void start(const TileIndex& t, int64_t x0, int64_t x1) {
+        x = x0;
+        end = x1;
+        n = 0;
+        if (x >= end) return;
+        int lo = 0, hi = t.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((int64_t)t.first[mid] * t.heads <= x) lo = mid; else hi = mid;
+        }
+        b = lo;
+        unit_tiles = t.first[b + 1] - t.first[b];
+        const int64_t rem = x - (int64_t)t.first[b] * t.heads;
+        h = (int)(rem / unit_tiles);
+        place(t);
+    }
+    __device__ __forceinline__ void place(const TileIndex& t) {
+        unit_first = (int64_t)t.first[b] * t.heads + (int64_t)h * unit_tiles;
+        const int j = (int)(x - unit_first);
+        tile = t.base[b] + j;
+        n = (int)min((int64_t)(unit_tiles - j), end - x);
+    }
+    // To the next piece; false at the share's end.
+    __device__ __forceinline__ bool next(const TileIndex& t) {
+        x += n;
+        if (x >= end) return false;
+        if (++h == t.heads) {
+            h = 0;
+            do ++b;
+            while (t.first[b + 1] == t.first[b]);
+            unit_tiles = t.first[b + 1] - t.first[b];
+        }
+        place(t);
+        return true;
+    }
+};
+
+// Four codes of a word to two FP16 pairs, exactly.
+template <int kCode>
+__device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (kCode == GQA_CODE_INT8) {
+        // 1024 + (c + 128) is the FP16 number 0x6400 | byte; minus 1152 it is c.
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
+        const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
+        lo = *reinterpret_cast<const uint32_t*>(&a);
+        hi = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+// tanh to about 2^-22: 1 - 2 / (e^2x + 1).
+__device__ __forceinline__ float tanh_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * 2.8853900817779268f) + 1.f));
+    return fmaf(-2.f, r, 1.f);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Running state of a consumer warp for the current unit.  Lane (g, t) = (lane / 4,
+// lane % 4): head t's maximum and sum (the sum over this lane's keys only), and
+// O for head t, dims 16 g + 2 i (o[i][0] high parts, [1] low) and + 1 ([2], [3]).
+struct State {
+    float o[8][4];
+    float m, l;
+    float vref, vinv;  // a power of two no page's V scale so far exceeds twice, and kWeightScale over it
+};
+
+template <int kCode, bool kCap, bool kBias>
+__device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float (*scales)[kPagesPerTile],
+                                             const uint32_t (&qf)[16], float factor, float slope, float cap2,
+                                             int key0, int lo, int hi, int m_pos, int page_shift, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    // Pages of the tile: step i (16 keys) lies in page i >> sh of it (page_len 64 and 128: page 0).
+    const int sh = page_shift >= 6 ? 2 : page_shift - 4;
+    float z[4][2];
+    {
+        const uint8_t* k = stage + g * kHeadDim;
+        const int c0 = ((2 * t) ^ g) << 4, c1 = ((2 * t + 1) ^ g) << 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint4 a = lds128(k + (16 * i) * kHeadDim + c0), b = lds128(k + (16 * i + 8) * kHeadDim + c0);
+            const uint4 c = lds128(k + (16 * i) * kHeadDim + c1), d = lds128(k + (16 * i + 8) * kHeadDim + c1);
+            const uint32_t up[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+            const uint32_t dn[8] = {b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint32_t a0, a1, a2, a3;
+                to_half4<kCode>(up[e], a0, a2);
+                to_half4<kCode>(dn[e], a1, a3);
+                mma_16x8x16(s, a0, a1, a2, a3, qf[2 * e], qf[2 * e + 1]);
+            }
+            const float f = factor * scales[0][i >> sh];
+            z[i][0] = (s[0] + s[1]) * f;
+            z[i][1] = (s[2] + s[3]) * f;
+        }
+    }
+    if constexpr (kCap) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) z[i][e] = cap2 * tanh_fast(z[i][e]);
+    }
+    if constexpr (kBias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                z[i][e] = fmaf(-slope, fabsf((float)(m_pos - (key0 + 16 * i + 8 * e + g))), z[i][e]);
+    }
+    const bool edge = key0 < lo || key0 + kTile > hi;  // of the whole warp
+    if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 16 * i + 8 * e + g;
+                if (key < lo || key >= hi) z[i][e] = -INFINITY;
+            }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1])),
+                     fmaxf(fmaxf(z[2][0], z[2][1]), fmaxf(z[3][0], z[3][1])));
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float m_new = fmaxf(st.m, mx);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    // V scales: where a page's passes the running power of two, that grows.
+    float vmax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPagesPerTile; ++i) {
+        const float a = fabsf(scales[1][i]);  // zero where the tile has fewer pages
+        if (a <= 3.402823466e38f) vmax = fmaxf(vmax, a);
+    }
+    float vscale = 1.f;
+    if (vmax > 2.f * st.vref) {
+        // The power of two below it, within the range where both vinv and its inverse are normal numbers.
+        const float ref = __int_as_float(min(253, max(13, __float_as_int(vmax) >> 23)) << 23);
+        vscale = st.vref / ref;
+        st.vref = ref;
+        st.vinv = kWeightScale / ref;
+    }
+    if (__any_sync(0xffffffffu, m_new != st.m) || vscale != 1.f) {
+        const float alpha = fast_exp2(st.m - m_use);
+        const float f = alpha * vscale;
+        st.l *= alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[i][e] *= f;
+        st.m = m_new;
+    }
+    const uint8_t* v = stage + kHalfBytes;
+    const int r0 = 2 * t * kHeadDim + ((g ^ (2 * t)) << 4), r1 = (2 * t + 1) * kHeadDim + ((g ^ (2 * t + 1)) << 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float r = scales[1][i >> sh] * st.vinv;
+        float w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float p = fast_exp2(z[i][e] - m_use);
+            st.l += p;
+            w[e] = p * r;
+            if (edge && z[i][e] == -INFINITY) w[e] = 0.f;  // not NaN, whatever the page's scale
+        }
+        const float h0 = __half2float(__float2half_rn(w[0])), h1 = __half2float(__float2half_rn(w[1]));
+        const uint32_t b0 = transpose_8x8(pack_half2(h0, w[0] - h0));
+        const uint32_t b1 = transpose_8x8(pack_half2(h1, w[1] - h1));
+        const uint8_t* vi = v + 16 * i * kHeadDim;
+        uint4 x0 = lds128(vi + r0), x1 = lds128(vi + r1);
+        uint4 x2 = lds128(vi + 8 * kHeadDim + r0), x3 = lds128(vi + 8 * kHeadDim + r1);
+        if (kCode == GQA_CODE_E4M3 && edge) {  // codes of keys out of sight may be NaN
+            const int key = key0 + 16 * i + 2 * t;
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            if (key < lo || key >= hi) x0 = zero;
+            if (key + 1 < lo || key + 1 >= hi) x1 = zero;
+            if (key + 8 < lo || key + 8 >= hi) x2 = zero;
+            if (key + 9 < lo || key + 9 >= hi) x3 = zero;
+        }
+        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+        const uint32_t w2[4] = {x2.x, x2.y, x2.z, x2.w}, w3[4] = {x3.x, x3.y, x3.z, x3.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, a2, a3;
+            to_half4<kCode>(__byte_perm(w0[j], w1[j], 0x5140), a0, a1);
+            to_half4<kCode>(__byte_perm(w2[j], w3[j], 0x5140), a2, a3);
+            mma_16x8x16(st.o[2 * j], a0, a1, a2, a3, b0, b1);
+            to_half4<kCode>(__byte_perm(w0[j], w1[j], 0x7362), a0, a1);
+            to_half4<kCode>(__byte_perm(w2[j], w3[j], 0x7362), a2, a3);
+            mma_16x8x16(st.o[2 * j + 1], a0, a1, a2, a3, b0, b1);
+        }
+    }
+}
+
+template <int kCode, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_constant__ DecodePagedArgs a) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* ring = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);  // 128-byte swizzle atoms
+    Shared& s = *reinterpret_cast<Shared*>(ring + a.stages * kStageBytes);
+    int* first = reinterpret_cast<int*>(&s + 1);
+    int* base = first + (a.p.batch + 1);
+    const PagedCall& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int batch = p.batch, heads = p.c.kv_heads, stages = a.stages;
+
+    if (tid == 0) {
+        for (int i = 0; i < stages; ++i) {
+            mbar_init(&s.full[i], 1);
+            mbar_init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.qfull[i], 1);
+            mbar_init(&s.qempty[i], kWarps);
+        }
+        fence_barrier_init();
+        prefetch_tensormap(&a.kmap);
+        prefetch_tensormap(&a.vmap);
+    }
+    // Tiles of every sequence and their running sum.
+    auto range_of = [&](int b) {
+        const int64_t m = p.query_positions ? p.query_positions[b] : (int64_t)p.seq_lens[b] - 1;
+        return paged_range(p, b, m, paged_length(p, b));
+    };
+    {
+        const int per = (batch + kThreads - 1) / kThreads;
+        const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
+        int sum = 0;
+        for (int b = b0; b < b1; ++b) {
+            const KeyRange r = range_of(b);
+            const int n = r.hi > r.lo ? (r.hi + kTile - 1) / kTile - r.lo / kTile : 0;
+            base[b] = r.lo / kTile;
+            first[b] = n;
+            sum += n;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += x;
+        }
+        if (lane == 31) s.sum[warp] = incl;
+        __syncthreads();
+        int at = incl - sum;
+        for (int w = 0; w < warp; ++w) at += s.sum[w];
+        for (int b = b0; b < b1; ++b) {
+            const int n = first[b];
+            first[b] = at;
+            at += n;
+        }
+        if (b0 < batch && b1 == batch) first[batch] = at;
+        __syncthreads();
+    }
+    const TileIndex index{first, base, batch, heads};
+    const int64_t total = (int64_t)first[batch] * heads;
+    const int64_t G = min((int64_t)gridDim.x, total), me = blockIdx.x;  // CTAs with a share: one tile at least
+    Walk walk;
+    walk.start(index, me < G ? total * me / G : 0, me < G ? total * (me + 1) / G : 0);
+
+    if (warp == kLoaderWarp) {
+        // ============================ loader ============================
+        const uint64_t policy = l2_evict_first_policy();
+        const int shift = p.c.page_shift;
+        const int box_rows = min(p.c.page_len, kTile), box_bytes = box_rows * kHeadDim;
+        const int per_tile = max(1, kTile >> shift);  // pages of a tile
+        int pos = 0;                                  // ring position
+        bool ok = true;
+        while (walk.n > 0 && ok) {
+            const KeyRange r = range_of(walk.b);
+            const int32_t* row = p.block_table + walk.b * p.table_stride;
+            int have = -1;  // first page column of the 32 the lanes hold
+            int page = -1;
+            float ks = 0.f, vs = 0.f;
+            for (int j = 0; j < walk.n && ok; ++j, ++pos) {
+                const int tile = walk.tile + j, col0 = (tile * kTile) >> shift;
+                if (have < 0 || col0 + per_tile > have + 32) {
+                    have = col0;
+                    const int col = col0 + lane;
+                    const int key = col << shift;
+                    page = -1;
+                    ks = vs = 0.f;
+                    if (key < r.hi && key + p.c.page_len > r.lo) {
+                        page = row[col];
+                        if (page >= 0 && page < p.c.pages) {
+                            ks = p.c.k_scale[page * p.c.scale_page_stride + walk.h];
+                            vs = p.c.v_scale[page * p.c.scale_page_stride + walk.h];
+                        } else {
+                            page = p.c.pages;  // out of the map: TMA fills zeros
+                        }
+                    }
+                }
+                const int st = pos % stages;
+                if (pos >= stages) ok = mbar_wait(&s.empty[st], ((pos / stages) - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int i = lane + have - col0;  // this lane's page in the tile
+                const bool mine = i >= 0 && i < per_tile;
+                const bool load = mine && page >= 0;
+                if (mine) {
+                    s.scales[st][0][i] = ks;
+                    s.scales[st][1][i] = vs;
+                }
+                if (lane >= per_tile && lane < kPagesPerTile) {
+                    s.scales[st][0][lane] = 0.f;
+                    s.scales[st][1][lane] = 0.f;
+                }
+                const int boxes = __popc(__ballot_sync(0xffffffffu, load));
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&s.full[st], 2 * boxes * box_bytes);
+                __syncwarp();
+                if (load) {
+                    uint8_t* dst = ring + st * kStageBytes + i * box_bytes;
+                    const int prow = (tile * kTile) & (p.c.page_len - 1);  // 64 for the second half of a 128-token page
+                    tma_load_page(dst, &a.kmap, per_tile > 1 ? 0 : prow, walk.h, page, &s.full[st], policy);
+                    tma_load_page(dst + kHalfBytes, &a.vmap, per_tile > 1 ? 0 : prow, walk.h, page, &s.full[st], policy);
+                }
+            }
+            if (!walk.next(index)) break;
+        }
+        if (!ok) {
+            if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
+            // Do not leave while copies into this CTA's shared memory are in flight.
+            for (int q = max(0, pos - stages); q < pos; ++q) mbar_wait(&s.full[q % stages], (q / stages) & 1);
+        }
+        return;
+    }
+    if (warp == kQueryWarp) {
+        // ============================ queries ============================
+        int n = 0;
+        while (walk.n > 0) {
+            const int sl = n & 1;
+            if (n >= 2 && !mbar_wait(&s.qempty[sl], ((n >> 1) - 1) & 1)) {
+                if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
+                break;
+            }
+            __syncwarp();
+            Slot& slot = s.slot[sl];
+            const int64_t m = p.query_positions ? p.query_positions[walk.b] : (int64_t)p.seq_lens[walk.b] - 1;
+            const KeyRange r = paged_range(p, walk.b, m, paged_length(p, walk.b));
+            float2 f0 = make_float2(1.f, 0.f), f1 = f0;
+            if (!p.q_rotated) {
+                f0 = rope_factor(a.rope.step[2 * lane], m);
+                f1 = rope_factor(a.rope.step[2 * lane + 1], m);
+            }
+#pragma unroll
+            for (int hq = 0; hq < kGroup; ++hq) {
+                const __nv_bfloat16* q = p.q + walk.b * p.q_row_stride + (walk.h * kGroup + hq) * p.q_head_stride;
+                const float2 x = bf16x2_to_float2(*reinterpret_cast<const uint32_t*>(q + 2 * lane));
+                const float2 y = bf16x2_to_float2(*reinterpret_cast<const uint32_t*>(q + kPairs + 2 * lane));
+                float v[4] = {x.x * f0.x - y.x * f0.y, x.y * f1.x - y.y * f1.y, x.x * f0.y + y.x * f0.x,
+                              x.y * f1.y + y.y * f1.x};
+                float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                bool fine = most <= 3.402823466e38f && v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3];
+#pragma unroll
+                for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                fine = __all_sync(0xffffffffu, fine);
+                // 2^e just above the largest (2^-126 at least), e <= 127 so that its inverse is a normal number.
+                const int e = min(253, max(1, (__float_as_int(most) >> 23) + 1));
+                const float up = __int_as_float(e << 23), down = __int_as_float((254 - e) << 23);
+                float hp[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] *= down;
+                    hp[i] = __half2float(__float2half_rn(v[i]));
+                }
+                *reinterpret_cast<uint32_t*>(&slot.q[2 * hq][2 * lane]) = pack_half2(hp[0], hp[1]);
+                *reinterpret_cast<uint32_t*>(&slot.q[2 * hq][kPairs + 2 * lane]) = pack_half2(hp[2], hp[3]);
+                *reinterpret_cast<uint32_t*>(&slot.q[2 * hq + 1][2 * lane]) = pack_half2(v[0] - hp[0], v[1] - hp[1]);
+                *reinterpret_cast<uint32_t*>(&slot.q[2 * hq + 1][kPairs + 2 * lane]) =
+                    pack_half2(v[2] - hp[2], v[3] - hp[3]);
+                if (lane == 0) {
+                    const float unit = kCap ? p.scale / p.cap : p.scale * 1.4426950408889634f;
+                    slot.factor[hq] = fine ? unit * up : __int_as_float(0x7fffffff);
+                    slot.slope[hq] = kBias ? p.slopes[walk.h * kGroup + hq] * 1.4426950408889634f : 0.f;
+                }
+            }
+            if (lane == 0) {
+                slot.lo = r.lo;
+                slot.hi = r.hi;
+                slot.m = (int)m;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.qfull[sl]);
+            ++n;
+            if (!walk.next(index)) break;
+        }
+        return;
+    }
+
+    // ============================ consumers ============================
+    // Sequences that see nothing.
+    for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+        if (first[b + 1] != first[b]) continue;
+        for (int i = tid; i < heads * kGroup * (kHeadDim / 2); i += kConsumers)
+            *reinterpret_cast<uint32_t*>(p.out + b * p.out_row_stride + (i / (kHeadDim / 2)) * p.out_head_stride +
+                                         2 * (i % (kHeadDim / 2))) = 0u;
+    }
+    const int g = lane >> 2, t = lane & 3;
+    int pos = 0;   // ring position of the piece's first tile
+    bool ok = true;  // after a wait that timed out: no more waits, but every barrier is kept
+    for (int n = 0; walk.n > 0; ++n) {
+        const int sl = n & 1;
+        if (ok) ok = mbar_wait(&s.qfull[sl], (n >> 1) & 1);
+        const Slot& slot = s.slot[sl];
+        uint32_t qf[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 w = lds128(&slot.q[g][32 * t + 8 * i]);
+            qf[4 * i] = w.x;
+            qf[4 * i + 1] = w.y;
+            qf[4 * i + 2] = w.z;
+            qf[4 * i + 3] = w.w;
+        }
+        const float factor = slot.factor[t], slope = slot.slope[t];
+        const int lo = slot.lo, hi = slot.hi, m_pos = slot.m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.qempty[sl]);
+
+        State st;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[i][e] = 0.f;
+        st.m = -INFINITY;
+        st.l = 0.f;
+        st.vref = 0.f;
+        st.vinv = 0.f;
+        // This warp's tiles: ring positions that are warp (mod kWarps).
+        for (int j = (warp - pos % kWarps + kWarps) % kWarps; j < walk.n; j += kWarps) {
+            const int q = pos + j, stg = q % stages;
+            if (ok) ok = mbar_wait(&s.full[stg], (q / stages) & 1);
+            consume_tile<kCode, kCap, kBias>(st, ring + stg * kStageBytes, s.scales[stg], qf, factor, slope,
+                                             p.cap * 1.4426950408889634f, (walk.tile + j) * kTile, lo, hi, m_pos,
+                                             p.c.page_shift, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.empty[stg]);
+        }
+        pos += walk.n;
+
+        // Merge the warps.
+        float l = st.l;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        const float back = st.vref * (1.f / kWeightScale);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(&s.acc[warp][t][16 * g + 4 * i]) =
+                make_float4((st.o[2 * i][0] + st.o[2 * i][1]) * back, (st.o[2 * i][2] + st.o[2 * i][3]) * back,
+                            (st.o[2 * i + 1][0] + st.o[2 * i + 1][1]) * back,
+                            (st.o[2 * i + 1][2] + st.o[2 * i + 1][3]) * back);
+        if (g == 0) {
+            s.m[warp][t] = st.m;
+            s.l[warp][t] = l;
+        }
+        named_barrier_sync(1, kConsumers);
+        const int hq = tid >> 6, d0 = 2 * (tid & 63);
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s.m[w][hq]);
+        const float Mu = M == -INFINITY ? 0.f : M;
+        float L = 0.f, A0 = 0.f, A1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = fast_exp2(s.m[w][hq] - Mu);
+            const float2 x = *reinterpret_cast<const float2*>(&s.acc[w][hq][d0]);
+            L = fmaf(f, s.l[w][hq], L);
+            A0 = fmaf(f, x.x, A0);
+            A1 = fmaf(f, x.y, A1);
+        }
+        uint32_t* out = reinterpret_cast<uint32_t*>(p.out + walk.b * p.out_row_stride +
+                                                    (walk.h * kGroup + hq) * p.out_head_stride + d0);
+        auto write = [&](float x, float y, float sum) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(x / sum, y / sum);
+            *out = *reinterpret_cast<const uint32_t*>(&v);
+        };
+        if (walk.n == walk.unit_tiles) {
+            write(A0, A1, L);
+            named_barrier_sync(1, kConsumers);  // s.acc is free again
+        } else {
+            // A piece of a unit: store it, and the unit's last CTA merges all.
+            // Tile x lies in the share of CTA ceil((x + 1) G / T) - 1; a share's
+            // first piece goes to its slot 0, its last to slot 1.
+            auto piece = [&](int64_t c) {
+                const int second = total * c / G < walk.unit_first ? 1 : 0;
+                return a.partials + ((c * 2 + second) * kGroup + hq) * kPartialFloats;
+            };
+            float* mine = piece(me);
+            *reinterpret_cast<float2*>(mine + d0) = make_float2(A0, A1);
+            if (d0 == 0) *reinterpret_cast<float2*>(mine + kHeadDim) = make_float2(M, L);
+            __threadfence();
+            named_barrier_sync(1, kConsumers);
+            const int64_t c0 = ((walk.unit_first + 1) * G + total - 1) / total - 1;
+            const int64_t c1 = ((walk.unit_first + walk.unit_tiles) * G + total - 1) / total - 1;
+            if (tid == 0) {
+                uint32_t* count = a.arrivals + walk.b * heads + walk.h;
+                const bool last = atomicAdd(count, 1u) == (uint32_t)(c1 - c0);
+                if (last) *count = 0;
+                __threadfence();
+                s.last = last;
+            }
+            named_barrier_sync(1, kConsumers);
+            const bool last = s.last != 0;
+            if (last) {
+                M = -INFINITY;
+                for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(piece(c) + kHeadDim));
+                const float use = M == -INFINITY ? 0.f : M;
+                L = A0 = A1 = 0.f;
+#pragma unroll 4
+                for (int64_t c = c0; c <= c1; ++c) {
+                    const float* x = piece(c);
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
+                    const float2 v = __ldcg(reinterpret_cast<const float2*>(x + d0));
+                    const float f = fast_exp2(ml.x - use);
+                    L = fmaf(f, ml.y, L);
+                    A0 = fmaf(f, v.x, A0);
+                    A1 = fmaf(f, v.y, A1);
+                }
+                write(A0, A1, L);
+            }
+            named_barrier_sync(1, kConsumers);
+        }
+        if (!walk.next(index)) break;
+    }
+    if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+}
+
+int decode_stages(int batch) {
+    const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (2 * (int64_t)batch + 1) * 4;
+    const int64_t n = room / kStageBytes;
+    return (int)(n < kMaxStages ? n : kMaxStages);
+}
+
+using Kernel = void (*)(DecodePagedArgs);
+
+Kernel kernel_for(int code, bool cap, bool bias) {
+    if (code == GQA_CODE_INT8) {
+        if (cap) return bias ? paged_decode_kernel<0, true, true> : paged_decode_kernel<0, true, false>;
+        return bias ? paged_decode_kernel<0, false, true> : paged_decode_kernel<0, false, false>;
+    }
+    if (cap) return bias ? paged_decode_kernel<1, true, true> : paged_decode_kernel<1, true, false>;
+    return bias ? paged_decode_kernel<1, false, true> : paged_decode_kernel<1, false, false>;
+}
+
+}  // namespace
+
+// The counters come first, as many as any call can have: a region that moved with
+// the batch would meet another call's partial rows.
+size_t paged_decode_workspace(int sms) {
+    return kPagedPartialsOffset + (size_t)sms * 2 * kGroup * kPartialFloats * sizeof(float);
+}
+
+cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
+                                const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
+    DecodePagedArgs a;
+    a.kmap = kmap;
+    a.vmap = vmap;
+    a.p = call;
+    a.rope = rope;
+    a.status = reinterpret_cast<uint32_t*>(ws);
+    a.arrivals = reinterpret_cast<uint32_t*>(ws + kPagedArrivalsOffset);
+    a.partials = reinterpret_cast<float*>(ws + kPagedPartialsOffset);
+    a.stages = decode_stages(call.batch);
+    const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (2 * (size_t)call.batch + 1) * 4;
+    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+cudaError_t paged_decode_prepare() {
+    for (int i = 0; i < 8; ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4),
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+}  // namespace gqa

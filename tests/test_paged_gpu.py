@@ -600,6 +600,23 @@ def test_side_streams_and_graphs():
         assert torch.equal(out.view(torch.int16), want.view(torch.int16))
 
 
+def test_calls_of_different_sizes_share_a_workspace():
+    """Calls in turn on one stream: what one leaves in the workspace does not reach the next."""
+    calls = []
+    for lens, page_len, heads in (([3000, 500] * 20, 64, 8), ([4000], 16, 1), ([900, 2000, 40] * 5, 32, 8),
+                                  ([20000], 64, 8), ([129] * 300, 16, 2)):
+        s = Setup(lens, seed=len(lens), page_len=page_len, heads=heads)
+        calls.append((s, s.queries(len(lens)), ints(s.table), ints(lens)))
+    first = [gqa.decode_paged(q, s.cache, t, n) for s, q, t, n in calls]
+    for _ in range(3):
+        again = [gqa.decode_paged(q, s.cache, t, n) for s, q, t, n in calls]
+        for a, b in zip(first, again):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    for (s, q, _, _), got in zip(calls, again):
+        pick = list(range(0, len(s.lens), max(1, len(s.lens) // 6)))
+        check(got[pick], q[pick], s, pick, [s.lens[i] - 1 for i in pick], unit=DECODE_UNIT)
+
+
 def test_many_sequences():
     lens = [(i * 37) % 150 for i in range(1500)]
     s = Setup(lens, seed=30, page_len=16, code="e4m3", heads=2)
