@@ -48,6 +48,7 @@ constexpr int kHalfBytes = kTile * kHeadDim;   // K or V of a tile
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kMaxStages = 12;
 constexpr int kPagesPerTile = kTile / kPagedMinPage;
+constexpr int kMaxCtas = kWarps * 66;          // pieces of a unit: their (m, l) fit where the warps' rows were
 constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
 
 // Shared memory behind the ring (bytes).
@@ -389,64 +390,97 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         const int shift = p.c.page_shift;
         const int box_rows = min(p.c.page_len, kTile), box_bytes = box_rows * kHeadDim;
         const int per_tile = max(1, kTile >> shift);  // pages of a tile
-        int pos = 0;                                  // ring position
+        int stg = 0, round = 0;                       // stage, times round the ring
         bool ok = true;
-        while (walk.n > 0 && ok) {
+        for (; walk.n > 0 && ok;) {
             const KeyRange r = range_of(walk.b);
             const int32_t* row = p.block_table + walk.b * p.table_stride;
-            int have = -1;  // first page column of the 32 the lanes hold
-            int page = -1;
-            float ks = 0.f, vs = 0.f;
-            for (int j = 0; j < walk.n && ok; ++j, ++pos) {
-                const int tile = walk.tile + j, col0 = (tile * kTile) >> shift;
-                if (have < 0 || col0 + per_tile > have + 32) {
-                    have = col0;
-                    const int col = col0 + lane;
-                    const int key = col << shift;
-                    page = -1;
-                    ks = vs = 0.f;
-                    if (key < r.hi && key + p.c.page_len > r.lo) {
-                        page = row[col];
-                        if (page >= 0 && page < p.c.pages) {
-                            ks = p.c.k_scale[page * p.c.scale_page_stride + walk.h];
-                            vs = p.c.v_scale[page * p.c.scale_page_stride + walk.h];
-                        } else {
-                            page = p.c.pages;  // out of the map: TMA fills zeros
-                        }
+            // Pages in batches of 32 columns, one a lane, each step a batch ahead of the next: table
+            // entries two batches ahead, scales one, so that no load is waited for but a piece's first.
+            int base_col = (walk.tile * kTile) >> shift;  // column of lane 0's page in the current batch
+            auto entry = [&](int col) {
+                const int64_t key = (int64_t)col << shift;
+                if (key >= r.hi || key + p.c.page_len <= r.lo) return -1;  // nothing visible: not loaded
+                const int page = row[col];
+                return page >= 0 && page < p.c.pages ? page : p.c.pages;  // out of the map: TMA fills zeros
+            };
+            auto scale = [&](const float* at, int page) {
+                return page >= 0 && page < p.c.pages ? at[page * p.c.scale_page_stride + walk.h] : 0.f;
+            };
+            int page = entry(base_col + lane), page1 = entry(base_col + 32 + lane), page2 = 0;
+            bool fresh = true;  // scales of the current batch not yet asked for
+            float ks = 0.f, vs = 0.f, ks1 = 0.f, vs1 = 0.f;
+            // The copies of tile j into stage `to`.
+            auto copy = [&](int j, int to) {
+                const int tile = walk.tile + j, i = base_col + lane - ((tile * kTile) >> shift);
+                if (i >= 0 && i < per_tile && page >= 0) {
+                    uint8_t* dst = ring + to * kStageBytes + i * box_bytes;
+                    const int prow = per_tile > 1 ? 0 : (tile * kTile) & (p.c.page_len - 1);
+                    tma_load_page(dst, &a.kmap, prow, walk.h, page, &s.full[to], policy);
+                    tma_load_page(dst + kHalfBytes, &a.vmap, prow, walk.h, page, &s.full[to], policy);
+                }
+            };
+            int copied = 0;  // tiles of this piece whose copies were issued
+            for (int j = 0; j < walk.n; ++j) {
+                const int col0 = ((walk.tile + j) * kTile) >> shift;
+                if (col0 >= base_col + 32) {
+                    base_col += 32;
+                    page = page1;
+                    ks = ks1;
+                    vs = vs1;
+                    page1 = page2;
+                    ks1 = scale(p.c.k_scale, page1);
+                    vs1 = scale(p.c.v_scale, page1);
+                    page2 = entry(base_col + 64 + lane);
+                }
+                if (j >= copied) {
+                    if (round > 0) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&s.empty[stg], (round - 1) & 1));
+                        if (!ok) break;
+                        copy(j, stg);
+                        copied = j + 1;
+                    } else {  // every stage that was never used, as far as the batch goes
+                        do copy(copied, stg + copied - j);
+                        while (++copied < walk.n && stg + copied - j < stages &&
+                               (((walk.tile + copied) * kTile) >> shift) < base_col + 32);
                     }
                 }
-                const int st = pos % stages;
-                if (pos >= stages) ok = mbar_wait(&s.empty[st], ((pos / stages) - 1) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const int i = lane + have - col0;  // this lane's page in the tile
+                if (fresh) {
+                    fresh = false;
+                    ks = scale(p.c.k_scale, page);
+                    vs = scale(p.c.v_scale, page);
+                    ks1 = scale(p.c.k_scale, page1);
+                    vs1 = scale(p.c.v_scale, page1);
+                    page2 = entry(base_col + 64 + lane);
+                }
+                // The pages' scales, and the stage's one arrival with the bytes to expect.
+                const int i = base_col + lane - col0;
                 const bool mine = i >= 0 && i < per_tile;
-                const bool load = mine && page >= 0;
                 if (mine) {
-                    s.scales[st][0][i] = ks;
-                    s.scales[st][1][i] = vs;
+                    s.scales[stg][0][i] = ks;
+                    s.scales[stg][1][i] = vs;
                 }
                 if (lane >= per_tile && lane < kPagesPerTile) {
-                    s.scales[st][0][lane] = 0.f;
-                    s.scales[st][1][lane] = 0.f;
+                    s.scales[stg][0][lane] = 0.f;
+                    s.scales[stg][1][lane] = 0.f;
                 }
-                const int boxes = __popc(__ballot_sync(0xffffffffu, load));
+                const int boxes = __popc(__ballot_sync(0xffffffffu, mine && page >= 0));
                 __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(&s.full[st], 2 * boxes * box_bytes);
-                __syncwarp();
-                if (load) {
-                    uint8_t* dst = ring + st * kStageBytes + i * box_bytes;
-                    const int prow = (tile * kTile) & (p.c.page_len - 1);  // 64 for the second half of a 128-token page
-                    tma_load_page(dst, &a.kmap, per_tile > 1 ? 0 : prow, walk.h, page, &s.full[st], policy);
-                    tma_load_page(dst + kHalfBytes, &a.vmap, per_tile > 1 ? 0 : prow, walk.h, page, &s.full[st], policy);
+                if (lane == 0) mbar_arrive_expect_tx(&s.full[stg], 2 * boxes * box_bytes);
+                if (++stg == stages) {
+                    stg = 0;
+                    ++round;
                 }
             }
-            if (!walk.next(index)) break;
+            if (!ok || !walk.next(index)) break;
         }
         if (!ok) {
             if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
             // Do not leave while copies into this CTA's shared memory are in flight.
-            for (int q = max(0, pos - stages); q < pos; ++q) mbar_wait(&s.full[q % stages], (q / stages) & 1);
+            for (int i = 0; i < stages; ++i) {
+                const int used = i < stg ? round + 1 : round;  // times the stage was filled
+                if (used > 0) mbar_wait(&s.full[i], (used - 1) & 1);
+            }
         }
         return;
     }
@@ -522,7 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                                          2 * (i % (kHeadDim / 2))) = 0u;
     }
     const int g = lane >> 2, t = lane & 3;
-    int pos = 0;   // ring position of the piece's first tile
+    int mine = warp;           // this warp's next tile, counted from the piece's first
+    int stg = warp, phase = 0; // its stage
     bool ok = true;  // after a wait that timed out: no more waits, but every barrier is kept
     for (int n = 0; walk.n > 0; ++n) {
         const int sl = n & 1;
@@ -551,17 +586,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         st.l = 0.f;
         st.vref = 0.f;
         st.vinv = 0.f;
-        // This warp's tiles: ring positions that are warp (mod kWarps).
-        for (int j = (warp - pos % kWarps + kWarps) % kWarps; j < walk.n; j += kWarps) {
-            const int q = pos + j, stg = q % stages;
-            if (ok) ok = mbar_wait(&s.full[stg], (q / stages) & 1);
+        // This warp's tiles: every kWarps-th of the CTA's.
+        for (; mine < walk.n; mine += kWarps) {
+            const int j = mine;
+            if (ok) ok = mbar_wait(&s.full[stg], phase);
             consume_tile<kCode, kCap, kBias>(st, ring + stg * kStageBytes, s.scales[stg], qf, factor, slope,
                                              p.cap * 1.4426950408889634f, (walk.tile + j) * kTile, lo, hi, m_pos,
                                              p.c.page_shift, lane);
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.empty[stg]);
+            stg += kWarps;
+            if (stg >= stages) {
+                stg -= stages;
+                phase ^= 1;
+            }
         }
-        pos += walk.n;
+        mine -= walk.n;
 
         // Merge the warps.
         float l = st.l;
@@ -604,42 +644,53 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             named_barrier_sync(1, kConsumers);  // s.acc is free again
         } else {
             // A piece of a unit: store it, and the unit's last CTA merges all.
-            // Tile x lies in the share of CTA ceil((x + 1) G / T) - 1; a share's
-            // first piece goes to its slot 0, its last to slot 1.
-            auto piece = [&](int64_t c) {
-                const int second = total * c / G < walk.unit_first ? 1 : 0;
-                return a.partials + ((c * 2 + second) * kGroup + hq) * kPartialFloats;
+            // Tile x lies in the share of CTA ceil((x + 1) G / T) - 1.  A share's
+            // first piece goes to its slot 0; its last, if another one, to slot 1:
+            // only the unit's first CTA can have begun before it.
+            const int c0 = (int)(((walk.unit_first + 1) * G + total - 1) / total) - 1;
+            const int pieces = (int)(((walk.unit_first + walk.unit_tiles) * G + total - 1) / total) - c0;
+            const int second = total * c0 / G < walk.unit_first ? 1 : 0;
+            auto piece = [&](int c, int head) {
+                return a.partials + (((c0 + c) * 2 + (c ? 0 : second)) * kGroup + head) * kPartialFloats;
             };
-            float* mine = piece(me);
-            *reinterpret_cast<float2*>(mine + d0) = make_float2(A0, A1);
-            if (d0 == 0) *reinterpret_cast<float2*>(mine + kHeadDim) = make_float2(M, L);
+            float* row = piece((int)me - c0, hq);
+            *reinterpret_cast<float2*>(row + d0) = make_float2(A0, A1);
+            if (d0 == 0) *reinterpret_cast<float2*>(row + kHeadDim) = make_float2(M, L);
             __threadfence();
             named_barrier_sync(1, kConsumers);
-            const int64_t c0 = ((walk.unit_first + 1) * G + total - 1) / total - 1;
-            const int64_t c1 = ((walk.unit_first + walk.unit_tiles) * G + total - 1) / total - 1;
             if (tid == 0) {
                 uint32_t* count = a.arrivals + walk.b * heads + walk.h;
-                const bool last = atomicAdd(count, 1u) == (uint32_t)(c1 - c0);
+                const bool last = atomicAdd(count, 1u) == (uint32_t)(pieces - 1);
                 if (last) *count = 0;
                 __threadfence();
                 s.last = last;
             }
             named_barrier_sync(1, kConsumers);
-            const bool last = s.last != 0;
-            if (last) {
+            if (s.last != 0) {
+                // Every load of a round at once: the pieces' (m, l) through shared memory, then 8 rows at a time.
+                float2* ml = reinterpret_cast<float2*>(&s.acc[0][0][0]);  // [head][piece]
                 M = -INFINITY;
-                for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(piece(c) + kHeadDim));
+                for (int i = tid; i < kGroup * pieces; i += kConsumers)
+                    ml[i] = __ldcg(reinterpret_cast<const float2*>(piece(i % pieces, i / pieces) + kHeadDim));
+                named_barrier_sync(1, kConsumers);
+                for (int c = 0; c < pieces; ++c) M = fmaxf(M, ml[hq * pieces + c].x);
                 const float use = M == -INFINITY ? 0.f : M;
                 L = A0 = A1 = 0.f;
-#pragma unroll 4
-                for (int64_t c = c0; c <= c1; ++c) {
-                    const float* x = piece(c);
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
-                    const float2 v = __ldcg(reinterpret_cast<const float2*>(x + d0));
-                    const float f = fast_exp2(ml.x - use);
-                    L = fmaf(f, ml.y, L);
-                    A0 = fmaf(f, v.x, A0);
-                    A1 = fmaf(f, v.y, A1);
+                for (int c = 0; c < pieces; c += 8) {
+                    float2 v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        v[e] = c + e < pieces ? __ldcg(reinterpret_cast<const float2*>(piece(c + e, hq) + d0))
+                                              : make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (c + e >= pieces) break;
+                        const float2 x = ml[hq * pieces + c + e];
+                        const float f = fast_exp2(x.x - use);
+                        L = fmaf(f, x.y, L);
+                        A0 = fmaf(f, v[e].x, A0);
+                        A1 = fmaf(f, v[e].y, A1);
+                    }
                 }
                 write(A0, A1, L);
             }
@@ -687,7 +738,7 @@ cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, in
     a.partials = reinterpret_cast<float*>(ws + kPagedPartialsOffset);
     a.stages = decode_stages(call.batch);
     const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (2 * (size_t)call.batch + 1) * 4;
-    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, smem, stream>>>(a);
+    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms < kMaxCtas ? sms : kMaxCtas, kThreads, smem, stream>>>(a);
     return cudaGetLastError();
 }
 
