@@ -415,13 +415,13 @@ int fill_args(gqa::DecodeArgs& a, const void* q, const void* k, const void* v, v
 
 int gqa::device_sms(int* sms) { return current_device(sms); }
 
-int gqa::paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c) {
+int gqa::paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c, int rows) {
     PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
     if (!encode) return GQA_ERR_CUDA;
     const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)c.page_len, (cuuint64_t)c.kv_heads,
                                 (cuuint64_t)c.pages};
     const cuuint64_t strides[3] = {(cuuint64_t)c.row_stride, (cuuint64_t)c.head_stride, (cuuint64_t)c.page_stride};
-    const cuuint32_t box[4] = {(cuuint32_t)kHeadDim, (cuuint32_t)(c.page_len < 64 ? c.page_len : 64), 1, 1};
+    const cuuint32_t box[4] = {(cuuint32_t)kHeadDim, (cuuint32_t)(c.page_len < rows ? c.page_len : rows), 1, 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box,
                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -539,7 +539,7 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
     call->q_rotated = (p->flags & GQA_FLAG_Q_ROTATED) != 0;
     // Key positions and tile counts are 32-bit.
     if ((int64_t)p->table_width * c->page_len > 0x7FFFFFFF ||
-        (int64_t)p->batch * p->table_width * (c->page_len / 64 + 1) > 0x7FFFFFFF)
+        (int64_t)p->batch * p->table_width * (c->page_len / 32 + 1) > 0x7FFFFFFF)
         return GQA_ERR_BATCH;
     return check_device_memory({q, out, c->k, c->v, c->k_scale, c->v_scale, p->block_table, p->seq_lens,
                                 call->query_positions, call->first_query, p->doc_starts, p->prefix_ends, p->slopes});
@@ -565,7 +565,7 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (!chunked) {
         CUtensorMap kmap, vmap;
-        if ((st = paged_map(&kmap, a.p.c.k, a.p.c)) != GQA_OK || (st = paged_map(&vmap, a.p.c.v, a.p.c)) != GQA_OK)
+        if ((st = paged_map(&kmap, a.p.c.k, a.p.c, paged_decode_tile())) != GQA_OK || (st = paged_map(&vmap, a.p.c.v, a.p.c, paged_decode_tile())) != GQA_OK)
             return st;
         return launch_paged_decode(a.p, a.rope, cache->code, kmap, vmap, sms, static_cast<uint8_t*>(workspace), s) ==
                        cudaSuccess

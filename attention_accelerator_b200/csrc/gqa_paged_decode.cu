@@ -40,15 +40,19 @@ namespace gqa {
 namespace {
 
 constexpr int kWarps = 8;                      // consumer warps
+constexpr int kLoaders = 2;                    // loader warps
 constexpr int kConsumers = kWarps * 32;
-constexpr int kLoaderWarp = kWarps, kQueryWarp = kWarps + 1;
-constexpr int kThreads = (kWarps + 2) * 32;
-constexpr int kTile = 64;                      // keys
+constexpr int kQueryWarp = kWarps + kLoaders;
+constexpr int kThreads = (kQueryWarp + 1) * 32;
+constexpr int kTile = 32;                      // keys
+constexpr int kTileShift = 5;
+constexpr int kSteps = kTile / 16;             // of 16 keys
 constexpr int kHalfBytes = kTile * kHeadDim;   // K or V of a tile
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 200 * 1024 / kStageBytes;
 constexpr int kPagesPerTile = kTile / kPagedMinPage;
-constexpr int kMaxCtas = kWarps * 66;          // pieces of a unit: their (m, l) fit where the warps' rows were
+constexpr int kOutThreads = kGroup * kHeadDim / 2;  // two outputs each
+static_assert(kConsumers >= kOutThreads, "a thread for every two outputs");
 constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
 
 // Shared memory behind the ring (bytes).
@@ -102,10 +106,10 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
     return d;
 }
 
-// The sequences' tiles, in shared memory: first[b] the running sum (per head),
-// base[b] the first visible tile.
+// The sequences' visible keys, lo[b] <= p < hi[b], and the running sum of their
+// tiles (per head), in shared memory.
 struct TileIndex {
-    const int *first, *base;
+    const int *first, *lo, *hi;
     int batch, heads;
 };
 
@@ -135,7 +139,7 @@ struct Walk {
     __device__ __forceinline__ void place(const TileIndex& t) {
         unit_first = (int64_t)t.first[b] * t.heads + (int64_t)h * unit_tiles;
         const int j = (int)(x - unit_first);
-        tile = t.base[b] + j;
+        tile = (t.lo[b] >> kTileShift) + j;
         n = (int)min((int64_t)(unit_tiles - j), end - x);
     }
     // To the next piece; false at the share's end.
@@ -199,14 +203,14 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                                              const uint32_t (&qf)[16], float factor, float slope, float cap2,
                                              int key0, int lo, int hi, int m_pos, int page_shift, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    // Pages of the tile: step i (16 keys) lies in page i >> sh of it (page_len 64 and 128: page 0).
-    const int sh = page_shift >= 6 ? 2 : page_shift - 4;
-    float z[4][2];
+    // Step i (16 keys) lies in page i >> sh of the tile.
+    const int sh = min(page_shift, kTileShift) - 4;
+    float z[kSteps][2];
     {
         const uint8_t* k = stage + g * kHeadDim;
         const int c0 = ((2 * t) ^ g) << 4, c1 = ((2 * t + 1) ^ g) << 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kSteps; ++i) {
             float s[4] = {0.f, 0.f, 0.f, 0.f};
             const uint4 a = lds128(k + (16 * i) * kHeadDim + c0), b = lds128(k + (16 * i + 8) * kHeadDim + c0);
             const uint4 c = lds128(k + (16 * i) * kHeadDim + c1), d = lds128(k + (16 * i + 8) * kHeadDim + c1);
@@ -226,13 +230,13 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     }
     if constexpr (kCap) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) z[i][e] = cap2 * tanh_fast(z[i][e]);
     }
     if constexpr (kBias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 z[i][e] = fmaf(-slope, fabsf((float)(m_pos - (key0 + 16 * i + 8 * e + g))), z[i][e]);
@@ -240,15 +244,16 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     const bool edge = key0 < lo || key0 + kTile > hi;  // of the whole warp
     if (edge) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = key0 + 16 * i + 8 * e + g;
                 if (key < lo || key >= hi) z[i][e] = -INFINITY;
             }
     }
-    float mx = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1])),
-                     fmaxf(fmaxf(z[2][0], z[2][1]), fmaxf(z[3][0], z[3][1])));
+    float mx = fmaxf(z[0][0], z[0][1]);
+#pragma unroll
+    for (int i = 1; i < kSteps; ++i) mx = fmaxf(mx, fmaxf(z[i][0], z[i][1]));
 #pragma unroll
     for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     const float m_new = fmaxf(st.m, mx);
@@ -281,7 +286,7 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     const uint8_t* v = stage + kHalfBytes;
     const int r0 = 2 * t * kHeadDim + ((g ^ (2 * t)) << 4), r1 = (2 * t + 1) * kHeadDim + ((g ^ (2 * t + 1)) << 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kSteps; ++i) {
         const float r = scales[1][i >> sh] * st.vinv;
         float w[2];
 #pragma unroll
@@ -326,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     uint8_t* ring = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);  // 128-byte swizzle atoms
     Shared& s = *reinterpret_cast<Shared*>(ring + a.stages * kStageBytes);
     int* first = reinterpret_cast<int*>(&s + 1);
-    int* base = first + (a.p.batch + 1);
+    int* los = first + (a.p.batch + 1);
+    int* his = los + a.p.batch;
     const PagedCall& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int batch = p.batch, heads = p.c.kv_heads, stages = a.stages;
@@ -345,18 +351,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         prefetch_tensormap(&a.vmap);
     }
     // Tiles of every sequence and their running sum.
-    auto range_of = [&](int b) {
-        const int64_t m = p.query_positions ? p.query_positions[b] : (int64_t)p.seq_lens[b] - 1;
-        return paged_range(p, b, m, paged_length(p, b));
-    };
     {
         const int per = (batch + kThreads - 1) / kThreads;
         const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
         int sum = 0;
         for (int b = b0; b < b1; ++b) {
-            const KeyRange r = range_of(b);
-            const int n = r.hi > r.lo ? (r.hi + kTile - 1) / kTile - r.lo / kTile : 0;
-            base[b] = r.lo / kTile;
+            const int64_t m = p.query_positions ? p.query_positions[b] : (int64_t)p.seq_lens[b] - 1;
+            const KeyRange r = paged_range(p, b, m, paged_length(p, b));
+            const int n = r.hi > r.lo ? ((r.hi + kTile - 1) >> kTileShift) - (r.lo >> kTileShift) : 0;
+            los[b] = r.lo;
+            his[b] = r.hi;
             first[b] = n;
             sum += n;
         }
@@ -378,22 +382,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         if (b0 < batch && b1 == batch) first[batch] = at;
         __syncthreads();
     }
-    const TileIndex index{first, base, batch, heads};
+    const TileIndex index{first, los, his, batch, heads};
     const int64_t total = (int64_t)first[batch] * heads;
     const int64_t G = min((int64_t)gridDim.x, total), me = blockIdx.x;  // CTAs with a share: one tile at least
     Walk walk;
     walk.start(index, me < G ? total * me / G : 0, me < G ? total * (me + 1) / G : 0);
 
-    if (warp == kLoaderWarp) {
+    if (warp >= kWarps && warp < kQueryWarp) {
         // ============================ loader ============================
         const uint64_t policy = l2_evict_first_policy();
         const int shift = p.c.page_shift;
         const int box_rows = min(p.c.page_len, kTile), box_bytes = box_rows * kHeadDim;
         const int per_tile = max(1, kTile >> shift);  // pages of a tile
-        int stg = 0, round = 0;                       // stage, times round the ring
+        int mine = warp - kWarps;                     // next tile, counted from the piece's first: every kLoaders-th
+        int stg = mine, round = 0;                    // its stage, times round the ring
         bool ok = true;
         for (; walk.n > 0 && ok;) {
-            const KeyRange r = range_of(walk.b);
+            const KeyRange r{los[walk.b], his[walk.b]};
             const int32_t* row = p.block_table + walk.b * p.table_stride;
             // Pages in batches of 32 columns, one a lane, each step a batch ahead of the next: table
             // entries two batches ahead, scales one, so that no load is waited for but a piece's first.
@@ -420,9 +425,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                     tma_load_page(dst + kHalfBytes, &a.vmap, prow, walk.h, page, &s.full[to], policy);
                 }
             };
-            int copied = 0;  // tiles of this piece whose copies were issued
-            for (int j = 0; j < walk.n; ++j) {
-                const int col0 = ((walk.tile + j) * kTile) >> shift;
+            int copied = 0;  // copies of the tiles before this one were issued
+            for (; mine < walk.n; mine += kLoaders) {
+                const int j = mine, col0 = ((walk.tile + j) * kTile) >> shift;
                 if (col0 >= base_col + 32) {
                     base_col += 32;
                     page = page1;
@@ -440,9 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                         copy(j, stg);
                         copied = j + 1;
                     } else {  // every stage that was never used, as far as the batch goes
-                        do copy(copied, stg + copied - j);
-                        while (++copied < walk.n && stg + copied - j < stages &&
-                               (((walk.tile + copied) * kTile) >> shift) < base_col + 32);
+                        copied = j;
+                        do {
+                            copy(copied, stg + copied - j);
+                            copied += kLoaders;
+                        } while (copied < walk.n && stg + copied - j < stages &&
+                                 (((walk.tile + copied) * kTile) >> shift) < base_col + 32);
                     }
                 }
                 if (fresh) {
@@ -455,8 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                 }
                 // The pages' scales, and the stage's one arrival with the bytes to expect.
                 const int i = base_col + lane - col0;
-                const bool mine = i >= 0 && i < per_tile;
-                if (mine) {
+                const bool here = i >= 0 && i < per_tile;
+                if (here) {
                     s.scales[stg][0][i] = ks;
                     s.scales[stg][1][i] = vs;
                 }
@@ -464,22 +472,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                     s.scales[stg][0][lane] = 0.f;
                     s.scales[stg][1][lane] = 0.f;
                 }
-                const int boxes = __popc(__ballot_sync(0xffffffffu, mine && page >= 0));
+                const int boxes = __popc(__ballot_sync(0xffffffffu, here && page >= 0));
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&s.full[stg], 2 * boxes * box_bytes);
-                if (++stg == stages) {
-                    stg = 0;
+                stg += kLoaders;
+                if (stg >= stages) {
+                    stg -= stages;
                     ++round;
                 }
             }
+            mine -= walk.n;
             if (!ok || !walk.next(index)) break;
         }
         if (!ok) {
             if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
             // Do not leave while copies into this CTA's shared memory are in flight.
-            for (int i = 0; i < stages; ++i) {
-                const int used = i < stg ? round + 1 : round;  // times the stage was filled
-                if (used > 0) mbar_wait(&s.full[i], (used - 1) & 1);
+            for (int i = 1; i <= stages / kLoaders && (round > 0 || stg >= i * kLoaders); ++i) {
+                const int at = stg - i * kLoaders;  // this warp's i-th stage back
+                mbar_wait(&s.full[at < 0 ? at + stages : at], (at < 0 ? round - 1 : round) & 1);
             }
         }
         return;
@@ -487,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     if (warp == kQueryWarp) {
         // ============================ queries ============================
         int n = 0;
+        const uint64_t step0 = a.rope.step[2 * lane], step1 = a.rope.step[2 * lane + 1];
         while (walk.n > 0) {
             const int sl = n & 1;
             if (n >= 2 && !mbar_wait(&s.qempty[sl], ((n >> 1) - 1) & 1)) {
@@ -495,45 +506,64 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             }
             __syncwarp();
             Slot& slot = s.slot[sl];
-            const int64_t m = p.query_positions ? p.query_positions[walk.b] : (int64_t)p.seq_lens[walk.b] - 1;
-            const KeyRange r = paged_range(p, walk.b, m, paged_length(p, walk.b));
-            float2 f0 = make_float2(1.f, 0.f), f1 = f0;
-            if (!p.q_rotated) {
-                f0 = rope_factor(a.rope.step[2 * lane], m);
-                f1 = rope_factor(a.rope.step[2 * lane + 1], m);
-            }
+            // Every load first.
+            const __nv_bfloat16* q = p.q + walk.b * p.q_row_stride + walk.h * kGroup * p.q_head_stride + 2 * lane;
+            uint32_t xw[kGroup], yw[kGroup];
 #pragma unroll
             for (int hq = 0; hq < kGroup; ++hq) {
-                const __nv_bfloat16* q = p.q + walk.b * p.q_row_stride + (walk.h * kGroup + hq) * p.q_head_stride;
-                const float2 x = bf16x2_to_float2(*reinterpret_cast<const uint32_t*>(q + 2 * lane));
-                const float2 y = bf16x2_to_float2(*reinterpret_cast<const uint32_t*>(q + kPairs + 2 * lane));
-                float v[4] = {x.x * f0.x - y.x * f0.y, x.y * f1.x - y.y * f1.y, x.x * f0.y + y.x * f0.x,
-                              x.y * f1.y + y.y * f1.x};
-                float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-                bool fine = most <= 3.402823466e38f && v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3];
+                xw[hq] = *reinterpret_cast<const uint32_t*>(q + hq * p.q_head_stride);
+                yw[hq] = *reinterpret_cast<const uint32_t*>(q + hq * p.q_head_stride + kPairs);
+            }
+            const int64_t m = p.query_positions ? p.query_positions[walk.b] : (int64_t)p.seq_lens[walk.b] - 1;
+            float slope = 0.f;
+            if (kBias && lane < kGroup) slope = p.slopes[walk.h * kGroup + lane] * 1.4426950408889634f;
+            float2 f0 = make_float2(1.f, 0.f), f1 = f0;
+            if (!p.q_rotated) {
+                f0 = rope_factor(step0, m);
+                f1 = rope_factor(step1, m);
+            }
+            float v[kGroup][4], most[kGroup];
+            bool fine[kGroup];
 #pragma unroll
-                for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                fine = __all_sync(0xffffffffu, fine);
+            for (int hq = 0; hq < kGroup; ++hq) {
+                const float2 x = bf16x2_to_float2(xw[hq]), y = bf16x2_to_float2(yw[hq]);
+                v[hq][0] = x.x * f0.x - y.x * f0.y;
+                v[hq][1] = x.y * f1.x - y.y * f1.y;
+                v[hq][2] = x.x * f0.y + y.x * f0.x;
+                v[hq][3] = x.y * f1.y + y.y * f1.x;
+                most[hq] = fmaxf(fmaxf(fabsf(v[hq][0]), fabsf(v[hq][1])), fmaxf(fabsf(v[hq][2]), fabsf(v[hq][3])));
+                fine[hq] = __all_sync(0xffffffffu, most[hq] <= 3.402823466e38f && v[hq][0] == v[hq][0] &&
+                                                       v[hq][1] == v[hq][1] && v[hq][2] == v[hq][2] &&
+                                                       v[hq][3] == v[hq][3]);
+            }
+            // (Magnitudes are non-negative: their bits order as integers.)
+#pragma unroll
+            for (int hq = 0; hq < kGroup; ++hq)
+                most[hq] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most[hq])));
+#pragma unroll
+            for (int hq = 0; hq < kGroup; ++hq) {
                 // 2^e just above the largest (2^-126 at least), e <= 127 so that its inverse is a normal number.
-                const int e = min(253, max(1, (__float_as_int(most) >> 23) + 1));
+                const int e = min(253, max(1, (__float_as_int(most[hq]) >> 23) + 1));
                 const float up = __int_as_float(e << 23), down = __int_as_float((254 - e) << 23);
                 float hp[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] *= down;
-                    hp[i] = __half2float(__float2half_rn(v[i]));
+                    v[hq][i] *= down;
+                    hp[i] = __half2float(__float2half_rn(v[hq][i]));
                 }
                 *reinterpret_cast<uint32_t*>(&slot.q[2 * hq][2 * lane]) = pack_half2(hp[0], hp[1]);
                 *reinterpret_cast<uint32_t*>(&slot.q[2 * hq][kPairs + 2 * lane]) = pack_half2(hp[2], hp[3]);
-                *reinterpret_cast<uint32_t*>(&slot.q[2 * hq + 1][2 * lane]) = pack_half2(v[0] - hp[0], v[1] - hp[1]);
+                *reinterpret_cast<uint32_t*>(&slot.q[2 * hq + 1][2 * lane]) =
+                    pack_half2(v[hq][0] - hp[0], v[hq][1] - hp[1]);
                 *reinterpret_cast<uint32_t*>(&slot.q[2 * hq + 1][kPairs + 2 * lane]) =
-                    pack_half2(v[2] - hp[2], v[3] - hp[3]);
-                if (lane == 0) {
+                    pack_half2(v[hq][2] - hp[2], v[hq][3] - hp[3]);
+                if (lane == hq) {
                     const float unit = kCap ? p.scale / p.cap : p.scale * 1.4426950408889634f;
-                    slot.factor[hq] = fine ? unit * up : __int_as_float(0x7fffffff);
-                    slot.slope[hq] = kBias ? p.slopes[walk.h * kGroup + hq] * 1.4426950408889634f : 0.f;
+                    slot.factor[hq] = fine[hq] ? unit * up : __int_as_float(0x7fffffff);
+                    slot.slope[hq] = slope;
                 }
             }
+            const KeyRange r{los[walk.b], his[walk.b]};
             if (lane == 0) {
                 slot.lo = r.lo;
                 slot.hi = r.hi;
@@ -618,21 +648,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             s.m[warp][t] = st.m;
             s.l[warp][t] = l;
         }
-        named_barrier_sync(1, kConsumers);
-        const int hq = tid >> 6, d0 = 2 * (tid & 63);
-        float M = -INFINITY;
+        const bool writer = tid < kOutThreads;
+        const int hq = (tid >> 6) & 3, d0 = 2 * (tid & 63);
+        float M, L, A0, A1;
+        auto merge_warps = [&] {  // of head hq, dims d0 and d0 + 1
+            named_barrier_sync(1, kConsumers);
+            M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s.m[w][hq]);
-        const float Mu = M == -INFINITY ? 0.f : M;
-        float L = 0.f, A0 = 0.f, A1 = 0.f;
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s.m[w][hq]);
+            const float Mu = M == -INFINITY ? 0.f : M;
+            L = A0 = A1 = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = fast_exp2(s.m[w][hq] - Mu);
-            const float2 x = *reinterpret_cast<const float2*>(&s.acc[w][hq][d0]);
-            L = fmaf(f, s.l[w][hq], L);
-            A0 = fmaf(f, x.x, A0);
-            A1 = fmaf(f, x.y, A1);
-        }
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = fast_exp2(s.m[w][hq] - Mu);
+                const float2 x = *reinterpret_cast<const float2*>(&s.acc[w][hq][d0]);
+                L = fmaf(f, s.l[w][hq], L);
+                A0 = fmaf(f, x.x, A0);
+                A1 = fmaf(f, x.y, A1);
+            }
+        };
+        merge_warps();
         uint32_t* out = reinterpret_cast<uint32_t*>(p.out + walk.b * p.out_row_stride +
                                                     (walk.h * kGroup + hq) * p.out_head_stride + d0);
         auto write = [&](float x, float y, float sum) {
@@ -640,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             *out = *reinterpret_cast<const uint32_t*>(&v);
         };
         if (walk.n == walk.unit_tiles) {
-            write(A0, A1, L);
+            if (writer) write(A0, A1, L);
             named_barrier_sync(1, kConsumers);  // s.acc is free again
         } else {
             // A piece of a unit: store it, and the unit's last CTA merges all.
@@ -654,45 +689,74 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                 return a.partials + (((c0 + c) * 2 + (c ? 0 : second)) * kGroup + head) * kPartialFloats;
             };
             float* row = piece((int)me - c0, hq);
-            *reinterpret_cast<float2*>(row + d0) = make_float2(A0, A1);
-            if (d0 == 0) *reinterpret_cast<float2*>(row + kHeadDim) = make_float2(M, L);
-            __threadfence();
+            if (writer) *reinterpret_cast<float2*>(row + d0) = make_float2(A0, A1);
+            if (writer && d0 == 0) *reinterpret_cast<float2*>(row + kHeadDim) = make_float2(M, L);
             named_barrier_sync(1, kConsumers);
             if (tid == 0) {
+                // Releases the CTA's rows (the barrier ordered them before it) and acquires the others'.
                 uint32_t* count = a.arrivals + walk.b * heads + walk.h;
-                const bool last = atomicAdd(count, 1u) == (uint32_t)(pieces - 1);
-                if (last) *count = 0;
-                __threadfence();
-                s.last = last;
+                uint32_t before;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+                s.last = before == (uint32_t)(pieces - 1);
+                if (s.last) *count = 0;
             }
             named_barrier_sync(1, kConsumers);
             if (s.last != 0) {
-                // Every load of a round at once: the pieces' (m, l) through shared memory, then 8 rows at a time.
-                float2* ml = reinterpret_cast<float2*>(&s.acc[0][0][0]);  // [head][piece]
-                M = -INFINITY;
-                for (int i = tid; i < kGroup * pieces; i += kConsumers)
-                    ml[i] = __ldcg(reinterpret_cast<const float2*>(piece(i % pieces, i / pieces) + kHeadDim));
-                named_barrier_sync(1, kConsumers);
-                for (int c = 0; c < pieces; ++c) M = fmaxf(M, ml[hq * pieces + c].x);
-                const float use = M == -INFINITY ? 0.f : M;
-                L = A0 = A1 = 0.f;
-                for (int c = 0; c < pieces; c += 8) {
-                    float2 v[8];
+                // Each warp merges every kWarps-th piece, a lane 4 dims of all heads; then the warps as above.
+                constexpr int kAtOnce = 4;
+                float4 acc[kGroup];
+                float m[kGroup], sum[kGroup];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        v[e] = c + e < pieces ? __ldcg(reinterpret_cast<const float2*>(piece(c + e, hq) + d0))
-                                              : make_float2(0.f, 0.f);
+                for (int h4 = 0; h4 < kGroup; ++h4) {
+                    acc[h4] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    m[h4] = -INFINITY;
+                    sum[h4] = 0.f;
+                }
+                for (int c = warp; c < pieces; c += kWarps * kAtOnce) {
+                    float4 v[kAtOnce][kGroup];
+                    float2 ml[kAtOnce][kGroup];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (c + e >= pieces) break;
-                        const float2 x = ml[hq * pieces + c + e];
-                        const float f = fast_exp2(x.x - use);
-                        L = fmaf(f, x.y, L);
-                        A0 = fmaf(f, v[e].x, A0);
-                        A1 = fmaf(f, v[e].y, A1);
+                    for (int e = 0; e < kAtOnce; ++e)
+#pragma unroll
+                        for (int h4 = 0; h4 < kGroup; ++h4) {
+                            const bool real = c + e * kWarps < pieces;
+                            const float* x = piece(real ? c + e * kWarps : c, h4);
+                            ml[e][h4] = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
+                            v[e][h4] = __ldcg(reinterpret_cast<const float4*>(x + 4 * lane));
+                            if (!real) ml[e][h4] = make_float2(-INFINITY, 0.f);
+                        }
+#pragma unroll
+                    for (int h4 = 0; h4 < kGroup; ++h4) {
+                        float now = m[h4];
+#pragma unroll
+                        for (int e = 0; e < kAtOnce; ++e) now = fmaxf(now, ml[e][h4].x);
+                        const float use = now == -INFINITY ? 0.f : now;
+                        const float f0 = fast_exp2(m[h4] - use);
+                        m[h4] = now;
+                        sum[h4] *= f0;
+                        acc[h4] = make_float4(acc[h4].x * f0, acc[h4].y * f0, acc[h4].z * f0, acc[h4].w * f0);
+#pragma unroll
+                        for (int e = 0; e < kAtOnce; ++e) {
+                            if (c + e * kWarps >= pieces) break;
+                            const float f = fast_exp2(ml[e][h4].x - use);
+                            sum[h4] = fmaf(f, ml[e][h4].y, sum[h4]);
+                            acc[h4].x = fmaf(f, v[e][h4].x, acc[h4].x);
+                            acc[h4].y = fmaf(f, v[e][h4].y, acc[h4].y);
+                            acc[h4].z = fmaf(f, v[e][h4].z, acc[h4].z);
+                            acc[h4].w = fmaf(f, v[e][h4].w, acc[h4].w);
+                        }
                     }
                 }
-                write(A0, A1, L);
+#pragma unroll
+                for (int h4 = 0; h4 < kGroup; ++h4) {
+                    *reinterpret_cast<float4*>(&s.acc[warp][h4][4 * lane]) = acc[h4];
+                    if (lane == h4) {
+                        s.m[warp][h4] = m[h4];
+                        s.l[warp][h4] = sum[h4];
+                    }
+                }
+                merge_warps();
+                if (writer) write(A0, A1, L);
             }
             named_barrier_sync(1, kConsumers);
         }
@@ -702,9 +766,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
 }
 
 int decode_stages(int batch) {
-    const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (2 * (int64_t)batch + 1) * 4;
+    static_assert(227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * GQA_PAGED_MAX_BATCH + 1) * 4 >=
+                      (int64_t)kStageBytes * (kWarps + kLoaders),
+                  "a stage for every warp");
+    const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * (int64_t)batch + 1) * 4;
     const int64_t n = room / kStageBytes;
-    return (int)(n < kMaxStages ? n : kMaxStages);
+    return (int)((n < kMaxStages ? n : kMaxStages) / kLoaders * kLoaders);  // a loader's stages are its own
 }
 
 using Kernel = void (*)(DecodePagedArgs);
@@ -719,6 +786,8 @@ Kernel kernel_for(int code, bool cap, bool bias) {
 }
 
 }  // namespace
+
+int paged_decode_tile() { return kTile; }
 
 // The counters come first, as many as any call can have: a region that moved with
 // the batch would meet another call's partial rows.
@@ -737,8 +806,8 @@ cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, in
     a.arrivals = reinterpret_cast<uint32_t*>(ws + kPagedArrivalsOffset);
     a.partials = reinterpret_cast<float*>(ws + kPagedPartialsOffset);
     a.stages = decode_stages(call.batch);
-    const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (2 * (size_t)call.batch + 1) * 4;
-    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms < kMaxCtas ? sms : kMaxCtas, kThreads, smem, stream>>>(a);
+    const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (3 * (size_t)call.batch + 1) * 4;
+    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, smem, stream>>>(a);
     return cudaGetLastError();
 }
 

@@ -6,8 +6,8 @@
 namespace gqa {
 
 // TMA map of K or V codes: (128, page_len, heads, pages) bytes, box (128,
-// min(page_len, 64), 1, 1), 128-byte swizzle.  A status.
-int paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c);
+// min(page_len, rows), 1, 1), 128-byte swizzle.  A status.
+int paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c, int rows);
 
 // Workspace of both attention calls: status word, one counter per (sequence, KV
 // head) -- zero between calls -- and partial rows.
@@ -16,6 +16,7 @@ constexpr size_t kPagedPartialsOffset =
     kPagedArrivalsOffset + (size_t)GQA_PAGED_MAX_BATCH * kNumKVHeads * sizeof(uint32_t);
 
 // One token a sequence.
+int paged_decode_tile();
 size_t paged_decode_workspace(int sms);
 cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream);
