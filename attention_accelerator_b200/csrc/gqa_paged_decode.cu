@@ -40,7 +40,8 @@ namespace gqa {
 namespace {
 
 constexpr int kWarps = 8;                      // consumer warps
-constexpr int kLoaders = 2;                    // loader warps
+constexpr int kLoaders = 1;                    // loader warps
+constexpr int kBurst = 4;                      // tiles that a loader warp handles at once
 constexpr int kConsumers = kWarps * 32;
 constexpr int kQueryWarp = kWarps + kLoaders;
 constexpr int kThreads = (kQueryWarp + 1) * 32;
@@ -52,6 +53,7 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kMaxStages = 200 * 1024 / kStageBytes;
 constexpr int kPagesPerTile = kTile / kPagedMinPage;
 constexpr int kOutThreads = kGroup * kHeadDim / 2;  // two outputs each
+static_assert(kSteps == 2 && kPagesPerTile == 2, "scales of two pages a tile");
 static_assert(kConsumers >= kOutThreads, "a thread for every two outputs");
 constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
 
@@ -65,8 +67,8 @@ struct alignas(16) Slot {            // one unit's queries (two slots)
 };
 struct alignas(16) Shared {
     uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2];
-    float scales[kMaxStages][2][kPagesPerTile];  // K, V
     Slot slot[2];
+    float4 scales[kMaxStages];  // K of the tile's two pages, V of them
     float acc[kWarps][kGroup][kRowF];
     float m[kWarps][kGroup], l[kWarps][kGroup];
     int last;
@@ -199,12 +201,13 @@ struct State {
 };
 
 template <int kCode, bool kCap, bool kBias>
-__device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float (*scales)[kPagesPerTile],
+__device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float4& scales,
                                              const uint32_t (&qf)[16], float factor, float slope, float cap2,
                                              int key0, int lo, int hi, int m_pos, int page_shift, int lane) {
     const int g = lane >> 2, t = lane & 3;
     // Step i (16 keys) lies in page i >> sh of the tile.
     const int sh = min(page_shift, kTileShift) - 4;
+    const float4 sc = scales;
     float z[kSteps][2];
     {
         const uint8_t* k = stage + g * kHeadDim;
@@ -223,7 +226,7 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                 to_half4<kCode>(dn[e], a1, a3);
                 mma_16x8x16(s, a0, a1, a2, a3, qf[2 * e], qf[2 * e + 1]);
             }
-            const float f = factor * scales[0][i >> sh];
+            const float f = factor * (i >> sh ? sc.y : sc.x);
             z[i][0] = (s[0] + s[1]) * f;
             z[i][1] = (s[2] + s[3]) * f;
         }
@@ -260,11 +263,8 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     // V scales: where a page's passes the running power of two, that grows.
     float vmax = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPagesPerTile; ++i) {
-        const float a = fabsf(scales[1][i]);  // zero where the tile has fewer pages
-        if (a <= 3.402823466e38f) vmax = fmaxf(vmax, a);
-    }
+    if (fabsf(sc.z) <= 3.402823466e38f) vmax = fabsf(sc.z);
+    if (fabsf(sc.w) <= 3.402823466e38f) vmax = fmaxf(vmax, fabsf(sc.w));
     float vscale = 1.f;
     if (vmax > 2.f * st.vref) {
         // The power of two below it, within the range where both vinv and its inverse are normal numbers.
@@ -287,7 +287,7 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     const int r0 = 2 * t * kHeadDim + ((g ^ (2 * t)) << 4), r1 = (2 * t + 1) * kHeadDim + ((g ^ (2 * t + 1)) << 4);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-        const float r = scales[1][i >> sh] * st.vinv;
+        const float r = (i >> sh ? sc.w : sc.z) * st.vinv;
         float w[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -390,106 +390,106 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
 
     if (warp >= kWarps && warp < kQueryWarp) {
         // ============================ loader ============================
+        // One warp's time per tile bounds the CTA's rate (one at a time: about 700
+        // cycles, as long as 16 KB take to arrive), so it works on kBurst tiles at
+        // once, a tile a lane.
         const uint64_t policy = l2_evict_first_policy();
         const int shift = p.c.page_shift;
-        const int box_rows = min(p.c.page_len, kTile), box_bytes = box_rows * kHeadDim;
-        const int per_tile = max(1, kTile >> shift);  // pages of a tile
-        int mine = warp - kWarps;                     // next tile, counted from the piece's first: every kLoaders-th
-        int stg = mine, round = 0;                    // its stage, times round the ring
+        const bool two = shift < kTileShift;  // two pages a tile (16 tokens each)
+        const int box_bytes = min(p.c.page_len, kTile) * kHeadDim;
+        int stg = 0, round = 0;  // next stage, times round the ring
         bool ok = true;
-        for (; walk.n > 0 && ok;) {
-            const KeyRange r{los[walk.b], his[walk.b]};
+        while (walk.n > 0 && ok) {
+            const int64_t lo = los[walk.b], hi = his[walk.b];
             const int32_t* row = p.block_table + walk.b * p.table_stride;
-            // Pages in batches of 32 columns, one a lane, each step a batch ahead of the next: table
-            // entries two batches ahead, scales one, so that no load is waited for but a piece's first.
-            int base_col = (walk.tile * kTile) >> shift;  // column of lane 0's page in the current batch
-            auto entry = [&](int col) {
-                const int64_t key = (int64_t)col << shift;
-                if (key >= r.hi || key + p.c.page_len <= r.lo) return -1;  // nothing visible: not loaded
-                const int page = row[col];
+            // Lane's tile of a batch of 32: its pages (-1: no visible key, not loaded) and their scales.
+            struct Pages {
+                int a, b;
+            };
+            auto entry = [&](int64_t key) {
+                if (key >= hi || key + min(p.c.page_len, kTile) <= lo) return -1;
+                const int page = row[key >> shift];
                 return page >= 0 && page < p.c.pages ? page : p.c.pages;  // out of the map: TMA fills zeros
+            };
+            auto pages = [&](int j) {
+                const int64_t key = (int64_t)(walk.tile + j + lane) << kTileShift;
+                return Pages{entry(key), two ? entry(key + kPagedMinPage) : -1};
             };
             auto scale = [&](const float* at, int page) {
                 return page >= 0 && page < p.c.pages ? at[page * p.c.scale_page_stride + walk.h] : 0.f;
             };
-            int page = entry(base_col + lane), page1 = entry(base_col + 32 + lane), page2 = 0;
-            bool fresh = true;  // scales of the current batch not yet asked for
-            float ks = 0.f, vs = 0.f, ks1 = 0.f, vs1 = 0.f;
-            // The copies of tile j into stage `to`.
-            auto copy = [&](int j, int to) {
-                const int tile = walk.tile + j, i = base_col + lane - ((tile * kTile) >> shift);
-                if (i >= 0 && i < per_tile && page >= 0) {
-                    uint8_t* dst = ring + to * kStageBytes + i * box_bytes;
-                    const int prow = per_tile > 1 ? 0 : (tile * kTile) & (p.c.page_len - 1);
-                    tma_load_page(dst, &a.kmap, prow, walk.h, page, &s.full[to], policy);
-                    tma_load_page(dst + kHalfBytes, &a.vmap, prow, walk.h, page, &s.full[to], policy);
+            auto scales = [&](Pages g) {
+                float4 f = make_float4(scale(p.c.k_scale, g.a), 0.f, scale(p.c.v_scale, g.a), 0.f);
+                if (two) {
+                    f.y = scale(p.c.k_scale, g.b);
+                    f.w = scale(p.c.v_scale, g.b);
                 }
+                return f;
             };
-            int copied = 0;  // copies of the tiles before this one were issued
-            for (; mine < walk.n; mine += kLoaders) {
-                const int j = mine, col0 = ((walk.tile + j) * kTile) >> shift;
-                if (col0 >= base_col + 32) {
-                    base_col += 32;
-                    page = page1;
-                    ks = ks1;
-                    vs = vs1;
-                    page1 = page2;
-                    ks1 = scale(p.c.k_scale, page1);
-                    vs1 = scale(p.c.v_scale, page1);
-                    page2 = entry(base_col + 64 + lane);
+            // Each step a batch ahead of the next (entries two batches ahead of their
+            // use, scales one), so that no load is waited for but a piece's first.
+            Pages now = pages(0), next = pages(32), later{-1, -1};
+            float4 f_now, f_next;
+            for (int j0 = 0; j0 < walk.n && ok; j0 += 32) {
+                if (j0 > 0) {
+                    now = next;
+                    f_now = f_next;
+                    next = later;
+                    f_next = scales(next);
+                    later = pages(j0 + 64);
                 }
-                if (j >= copied) {
-                    if (round > 0) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&s.empty[stg], (round - 1) & 1));
-                        if (!ok) break;
-                        copy(j, stg);
-                        copied = j + 1;
-                    } else {  // every stage that was never used, as far as the batch goes
-                        copied = j;
-                        do {
-                            copy(copied, stg + copied - j);
-                            copied += kLoaders;
-                        } while (copied < walk.n && stg + copied - j < stages &&
-                                 (((walk.tile + copied) * kTile) >> shift) < base_col + 32);
+                const int batch_n = min(32, walk.n - j0);
+                for (int k0 = 0; k0 < batch_n; k0 += kBurst) {
+                    const int n = min(kBurst, batch_n - k0);
+                    const bool mine = lane >= k0 && lane < k0 + n;
+                    int to = stg + lane - k0, turn = round;
+                    if (to >= stages) {
+                        to -= stages;
+                        ++turn;
+                    }
+                    if (mine && turn > 0) ok = mbar_wait(&s.empty[to], (turn - 1) & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (mine) {
+                        const int boxes = (now.a >= 0) + (now.b >= 0);
+                        if (j0 + k0 > 0) s.scales[to] = f_now;
+                        // (A piece's first burst: the copies before the scales, which are still on their way.)
+                        if (j0 + k0 > 0) mbar_arrive_expect_tx(&s.full[to], 2 * boxes * box_bytes);
+                        uint8_t* dst = ring + to * kStageBytes;
+                        const int prow = two ? 0 : ((walk.tile + j0 + lane) * kTile) & (p.c.page_len - 1);
+                        if (now.a >= 0) {
+                            tma_load_page(dst, &a.kmap, prow, walk.h, now.a, &s.full[to], policy);
+                            tma_load_page(dst + kHalfBytes, &a.vmap, prow, walk.h, now.a, &s.full[to], policy);
+                        }
+                        if (now.b >= 0) {
+                            tma_load_page(dst + box_bytes, &a.kmap, 0, walk.h, now.b, &s.full[to], policy);
+                            tma_load_page(dst + kHalfBytes + box_bytes, &a.vmap, 0, walk.h, now.b, &s.full[to], policy);
+                        }
+                        if (j0 + k0 == 0) {
+                            s.scales[to] = scales(now);
+                            mbar_arrive_expect_tx(&s.full[to], 2 * boxes * box_bytes);
+                        }
+                    }
+                    if (j0 + k0 == 0) {
+                        f_now = scales(now);
+                        f_next = scales(next);
+                        later = pages(64);
+                    }
+                    stg += n;
+                    if (stg >= stages) {
+                        stg -= stages;
+                        ++round;
                     }
                 }
-                if (fresh) {
-                    fresh = false;
-                    ks = scale(p.c.k_scale, page);
-                    vs = scale(p.c.v_scale, page);
-                    ks1 = scale(p.c.k_scale, page1);
-                    vs1 = scale(p.c.v_scale, page1);
-                    page2 = entry(base_col + 64 + lane);
-                }
-                // The pages' scales, and the stage's one arrival with the bytes to expect.
-                const int i = base_col + lane - col0;
-                const bool here = i >= 0 && i < per_tile;
-                if (here) {
-                    s.scales[stg][0][i] = ks;
-                    s.scales[stg][1][i] = vs;
-                }
-                if (lane >= per_tile && lane < kPagesPerTile) {
-                    s.scales[stg][0][lane] = 0.f;
-                    s.scales[stg][1][lane] = 0.f;
-                }
-                const int boxes = __popc(__ballot_sync(0xffffffffu, here && page >= 0));
-                __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(&s.full[stg], 2 * boxes * box_bytes);
-                stg += kLoaders;
-                if (stg >= stages) {
-                    stg -= stages;
-                    ++round;
-                }
             }
-            mine -= walk.n;
-            if (!ok || !walk.next(index)) break;
+            if (!walk.next(index)) break;
         }
         if (!ok) {
             if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
             // Do not leave while copies into this CTA's shared memory are in flight.
-            for (int i = 1; i <= stages / kLoaders && (round > 0 || stg >= i * kLoaders); ++i) {
-                const int at = stg - i * kLoaders;  // this warp's i-th stage back
-                mbar_wait(&s.full[at < 0 ? at + stages : at], (at < 0 ? round - 1 : round) & 1);
+            for (int i = 0; i < stages; ++i) {
+                const int filled = i < stg ? round + 1 : round;  // times stage i was
+                if (filled > 0) mbar_wait(&s.full[i], (filled - 1) & 1);
             }
         }
         return;
@@ -767,11 +767,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
 
 int decode_stages(int batch) {
     static_assert(227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * GQA_PAGED_MAX_BATCH + 1) * 4 >=
-                      (int64_t)kStageBytes * (kWarps + kLoaders),
+                      (int64_t)kStageBytes * (kWarps + kBurst),
                   "a stage for every warp");
     const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * (int64_t)batch + 1) * 4;
     const int64_t n = room / kStageBytes;
-    return (int)((n < kMaxStages ? n : kMaxStages) / kLoaders * kLoaders);  // a loader's stages are its own
+    return (int)((n < kMaxStages ? n : kMaxStages));
 }
 
 using Kernel = void (*)(DecodePagedArgs);
