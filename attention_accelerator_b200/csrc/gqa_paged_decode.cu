@@ -40,11 +40,10 @@ namespace gqa {
 namespace {
 
 constexpr int kWarps = 8;                      // consumer warps
-constexpr int kLoaders = 1;                    // loader warps
-constexpr int kBurst = 4;                      // tiles that a loader warp handles at once
-constexpr int kConsumers = kWarps * 32;
-constexpr int kQueryWarp = kWarps + kLoaders;
-constexpr int kThreads = (kQueryWarp + 1) * 32;
+constexpr int kBurst = 4;                      // tiles that the loader handles at once
+constexpr int kFinishers = kGroup;              // finisher warps, one a Q head
+constexpr int kLoaderWarp = kWarps, kQueryWarp = kWarps + 1, kFinishWarp = kWarps + 2;
+constexpr int kThreads = (kFinishWarp + kFinishers) * 32;
 constexpr int kTile = 32;                      // keys
 constexpr int kTileShift = 5;
 constexpr int kSteps = kTile / 16;             // of 16 keys
@@ -52,9 +51,7 @@ constexpr int kHalfBytes = kTile * kHeadDim;   // K or V of a tile
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kMaxStages = 200 * 1024 / kStageBytes;
 constexpr int kPagesPerTile = kTile / kPagedMinPage;
-constexpr int kOutThreads = kGroup * kHeadDim / 2;  // two outputs each
 static_assert(kSteps == 2 && kPagesPerTile == 2, "scales of two pages a tile");
-static_assert(kConsumers >= kOutThreads, "a thread for every two outputs");
 constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
 
 // Shared memory behind the ring (bytes).
@@ -66,12 +63,13 @@ struct alignas(16) Slot {            // one unit's queries (two slots)
     int lo, hi, m, pad;
 };
 struct alignas(16) Shared {
-    uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2];
+    uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2], rfull[2], rempty[2];
     Slot slot[2];
     float4 scales[kMaxStages];  // K of the tile's two pages, V of them
-    float acc[kWarps][kGroup][kRowF];
-    float m[kWarps][kGroup], l[kWarps][kGroup];
-    int last;
+    struct {  // what the consumer warps make of a piece (two of them)
+        float acc[kWarps][kGroup][kRowF];
+        float m[kWarps][kGroup], l[kWarps][kGroup];
+    } result[2];
     int sum[kThreads / 32];
 };
 
@@ -80,7 +78,7 @@ struct alignas(64) DecodePagedArgs {
     PagedCall p;
     RopeSteps rope;
     uint32_t* status;
-    uint32_t* arrivals;  // [batch * heads], zero between calls
+    uint32_t* arrivals;  // [batch * Q heads], zero between calls
     float* partials;     // [grid][2][4][132]
     int stages;
 };
@@ -345,6 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.qfull[i], 1);
             mbar_init(&s.qempty[i], kWarps);
+            mbar_init(&s.rfull[i], kWarps);
+            mbar_init(&s.rempty[i], kFinishers);
         }
         fence_barrier_init();
         prefetch_tensormap(&a.kmap);
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     Walk walk;
     walk.start(index, me < G ? total * me / G : 0, me < G ? total * (me + 1) / G : 0);
 
-    if (warp >= kWarps && warp < kQueryWarp) {
+    if (warp == kLoaderWarp) {
         // ============================ loader ============================
         // One warp's time per tile bounds the CTA's rate (one at a time: about 700
         // cycles, as long as 16 KB take to arrive), so it works on kBurst tiles at
@@ -577,14 +577,106 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         return;
     }
 
-    // ============================ consumers ============================
-    // Sequences that see nothing.
-    for (int b = blockIdx.x; b < batch; b += gridDim.x) {
-        if (first[b + 1] != first[b]) continue;
-        for (int i = tid; i < heads * kGroup * (kHeadDim / 2); i += kConsumers)
-            *reinterpret_cast<uint32_t*>(p.out + b * p.out_row_stride + (i / (kHeadDim / 2)) * p.out_head_stride +
-                                         2 * (i % (kHeadDim / 2))) = 0u;
+    if (warp >= kFinishWarp) {
+        // ============================ finishers ============================
+        // A warp a head: the consumers' parts of a piece to an output row, or, for a
+        // piece of a unit, to a partial row -- while the consumers go on.
+        const int hq = warp - kFinishWarp;
+        // Sequences that see nothing.
+        for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+            if (first[b + 1] != first[b]) continue;
+            for (int h = 0; h < heads; ++h)
+                *reinterpret_cast<uint2*>(p.out + b * p.out_row_stride + (h * kGroup + hq) * p.out_head_stride +
+                                          4 * lane) = make_uint2(0u, 0u);
+        }
+        bool ok = true;  // after a wait that timed out: no more waits, but the counters are kept
+        for (int n = 0; walk.n > 0; ++n) {
+            const int sl = n & 1;
+            if (ok) ok = mbar_wait(&s.rfull[sl], (n >> 1) & 1);
+            __syncwarp();
+            const auto& r = s.result[sl];
+            float M = -INFINITY, L = 0.f;
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto add = [&](float f, float l, float4 x) {
+                L = fmaf(f, l, L);
+                A.x = fmaf(f, x.x, A.x);
+                A.y = fmaf(f, x.y, A.y);
+                A.z = fmaf(f, x.z, A.z);
+                A.w = fmaf(f, x.w, A.w);
+            };
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, r.m[w][hq]);
+            const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                add(fast_exp2(r.m[w][hq] - Mu), r.l[w][hq], *reinterpret_cast<const float4*>(&r.acc[w][hq][4 * lane]));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.rempty[sl]);
+            bool done = walk.n == walk.unit_tiles;
+            if (!done) {
+                // A piece of a unit: store it, and the unit's last CTA merges all.
+                // Tile x lies in the share of CTA ceil((x + 1) G / T) - 1.  A share's
+                // first piece goes to its slot 0; its last, if another one, to slot 1:
+                // only the unit's first CTA can have begun before it.
+                const int c0 = (int)(((walk.unit_first + 1) * G + total - 1) / total) - 1;
+                const int pieces = (int)(((walk.unit_first + walk.unit_tiles) * G + total - 1) / total) - c0;
+                const int second = total * c0 / G < walk.unit_first ? 1 : 0;
+                auto piece = [&](int c) {
+                    return a.partials + (((c0 + c) * 2 + (c ? 0 : second)) * kGroup + hq) * kPartialFloats;
+                };
+                float* mine = piece((int)me - c0);
+                *reinterpret_cast<float4*>(mine + 4 * lane) = A;
+                if (lane == 0) *reinterpret_cast<float2*>(mine + kHeadDim) = make_float2(M, L);
+                __syncwarp();
+                uint32_t before = 0;
+                if (lane == 0) {
+                    // Releases the warp's row and acquires the others'.
+                    uint32_t* count = a.arrivals + (walk.b * heads + walk.h) * kGroup + hq;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+                    if (before == (uint32_t)(pieces - 1)) *count = 0;
+                }
+                done = __shfl_sync(0xffffffffu, before, 0) == (uint32_t)(pieces - 1);
+                if (done) {
+                    constexpr int kAtOnce = 10;
+                    M = -INFINITY;
+                    L = 0.f;
+                    A = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int c = 0; c < pieces; c += kAtOnce) {
+                        float4 v[kAtOnce];
+                        float2 ml[kAtOnce];
+                        float now = M;
+#pragma unroll
+                        for (int e = 0; e < kAtOnce; ++e) {
+                            const float* x = piece(min(c + e, pieces - 1));
+                            ml[e] = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
+                            v[e] = __ldcg(reinterpret_cast<const float4*>(x + 4 * lane));
+                        }
+#pragma unroll
+                        for (int e = 0; e < kAtOnce; ++e) now = fmaxf(now, ml[e].x);
+                        const float use = now == -INFINITY ? 0.f : now;
+                        const float f0 = fast_exp2(M - use);
+                        M = now;
+                        L *= f0;
+                        A = make_float4(A.x * f0, A.y * f0, A.z * f0, A.w * f0);
+#pragma unroll
+                        for (int e = 0; e < kAtOnce; ++e)
+                            if (c + e < pieces) add(fast_exp2(ml[e].x - use), ml[e].y, v[e]);
+                    }
+                }
+            }
+            if (done) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(A.x / L, A.y / L), y = __floats2bfloat162_rn(A.z / L, A.w / L);
+                *reinterpret_cast<uint2*>(p.out + walk.b * p.out_row_stride + (walk.h * kGroup + hq) * p.out_head_stride +
+                                          4 * lane) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            }
+            if (!walk.next(index)) break;
+        }
+        if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+        return;
     }
+
+    // ============================ consumers ============================
     const int g = lane >> 2, t = lane & 3;
     int mine = warp;           // this warp's next tile, counted from the piece's first
     int stg = warp, phase = 0; // its stage
@@ -633,133 +725,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         }
         mine -= walk.n;
 
-        // Merge the warps.
+        // This warp's part of the piece, for the finishers.
         float l = st.l;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
         const float back = st.vref * (1.f / kWeightScale);
+        if (ok && n >= 2) ok = mbar_wait(&s.rempty[sl], ((n >> 1) - 1) & 1);
+        auto& r = s.result[sl];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(&s.acc[warp][t][16 * g + 4 * i]) =
+            *reinterpret_cast<float4*>(&r.acc[warp][t][16 * g + 4 * i]) =
                 make_float4((st.o[2 * i][0] + st.o[2 * i][1]) * back, (st.o[2 * i][2] + st.o[2 * i][3]) * back,
                             (st.o[2 * i + 1][0] + st.o[2 * i + 1][1]) * back,
                             (st.o[2 * i + 1][2] + st.o[2 * i + 1][3]) * back);
         if (g == 0) {
-            s.m[warp][t] = st.m;
-            s.l[warp][t] = l;
+            r.m[warp][t] = st.m;
+            r.l[warp][t] = l;
         }
-        const bool writer = tid < kOutThreads;
-        const int hq = (tid >> 6) & 3, d0 = 2 * (tid & 63);
-        float M, L, A0, A1;
-        auto merge_warps = [&] {  // of head hq, dims d0 and d0 + 1
-            named_barrier_sync(1, kConsumers);
-            M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s.m[w][hq]);
-            const float Mu = M == -INFINITY ? 0.f : M;
-            L = A0 = A1 = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float f = fast_exp2(s.m[w][hq] - Mu);
-                const float2 x = *reinterpret_cast<const float2*>(&s.acc[w][hq][d0]);
-                L = fmaf(f, s.l[w][hq], L);
-                A0 = fmaf(f, x.x, A0);
-                A1 = fmaf(f, x.y, A1);
-            }
-        };
-        merge_warps();
-        uint32_t* out = reinterpret_cast<uint32_t*>(p.out + walk.b * p.out_row_stride +
-                                                    (walk.h * kGroup + hq) * p.out_head_stride + d0);
-        auto write = [&](float x, float y, float sum) {
-            const __nv_bfloat162 v = __floats2bfloat162_rn(x / sum, y / sum);
-            *out = *reinterpret_cast<const uint32_t*>(&v);
-        };
-        if (walk.n == walk.unit_tiles) {
-            if (writer) write(A0, A1, L);
-            named_barrier_sync(1, kConsumers);  // s.acc is free again
-        } else {
-            // A piece of a unit: store it, and the unit's last CTA merges all.
-            // Tile x lies in the share of CTA ceil((x + 1) G / T) - 1.  A share's
-            // first piece goes to its slot 0; its last, if another one, to slot 1:
-            // only the unit's first CTA can have begun before it.
-            const int c0 = (int)(((walk.unit_first + 1) * G + total - 1) / total) - 1;
-            const int pieces = (int)(((walk.unit_first + walk.unit_tiles) * G + total - 1) / total) - c0;
-            const int second = total * c0 / G < walk.unit_first ? 1 : 0;
-            auto piece = [&](int c, int head) {
-                return a.partials + (((c0 + c) * 2 + (c ? 0 : second)) * kGroup + head) * kPartialFloats;
-            };
-            float* row = piece((int)me - c0, hq);
-            if (writer) *reinterpret_cast<float2*>(row + d0) = make_float2(A0, A1);
-            if (writer && d0 == 0) *reinterpret_cast<float2*>(row + kHeadDim) = make_float2(M, L);
-            named_barrier_sync(1, kConsumers);
-            if (tid == 0) {
-                // Releases the CTA's rows (the barrier ordered them before it) and acquires the others'.
-                uint32_t* count = a.arrivals + walk.b * heads + walk.h;
-                uint32_t before;
-                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
-                s.last = before == (uint32_t)(pieces - 1);
-                if (s.last) *count = 0;
-            }
-            named_barrier_sync(1, kConsumers);
-            if (s.last != 0) {
-                // Each warp merges every kWarps-th piece, a lane 4 dims of all heads; then the warps as above.
-                constexpr int kAtOnce = 4;
-                float4 acc[kGroup];
-                float m[kGroup], sum[kGroup];
-#pragma unroll
-                for (int h4 = 0; h4 < kGroup; ++h4) {
-                    acc[h4] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    m[h4] = -INFINITY;
-                    sum[h4] = 0.f;
-                }
-                for (int c = warp; c < pieces; c += kWarps * kAtOnce) {
-                    float4 v[kAtOnce][kGroup];
-                    float2 ml[kAtOnce][kGroup];
-#pragma unroll
-                    for (int e = 0; e < kAtOnce; ++e)
-#pragma unroll
-                        for (int h4 = 0; h4 < kGroup; ++h4) {
-                            const bool real = c + e * kWarps < pieces;
-                            const float* x = piece(real ? c + e * kWarps : c, h4);
-                            ml[e][h4] = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
-                            v[e][h4] = __ldcg(reinterpret_cast<const float4*>(x + 4 * lane));
-                            if (!real) ml[e][h4] = make_float2(-INFINITY, 0.f);
-                        }
-#pragma unroll
-                    for (int h4 = 0; h4 < kGroup; ++h4) {
-                        float now = m[h4];
-#pragma unroll
-                        for (int e = 0; e < kAtOnce; ++e) now = fmaxf(now, ml[e][h4].x);
-                        const float use = now == -INFINITY ? 0.f : now;
-                        const float f0 = fast_exp2(m[h4] - use);
-                        m[h4] = now;
-                        sum[h4] *= f0;
-                        acc[h4] = make_float4(acc[h4].x * f0, acc[h4].y * f0, acc[h4].z * f0, acc[h4].w * f0);
-#pragma unroll
-                        for (int e = 0; e < kAtOnce; ++e) {
-                            if (c + e * kWarps >= pieces) break;
-                            const float f = fast_exp2(ml[e][h4].x - use);
-                            sum[h4] = fmaf(f, ml[e][h4].y, sum[h4]);
-                            acc[h4].x = fmaf(f, v[e][h4].x, acc[h4].x);
-                            acc[h4].y = fmaf(f, v[e][h4].y, acc[h4].y);
-                            acc[h4].z = fmaf(f, v[e][h4].z, acc[h4].z);
-                            acc[h4].w = fmaf(f, v[e][h4].w, acc[h4].w);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int h4 = 0; h4 < kGroup; ++h4) {
-                    *reinterpret_cast<float4*>(&s.acc[warp][h4][4 * lane]) = acc[h4];
-                    if (lane == h4) {
-                        s.m[warp][h4] = m[h4];
-                        s.l[warp][h4] = sum[h4];
-                    }
-                }
-                merge_warps();
-                if (writer) write(A0, A1, L);
-            }
-            named_barrier_sync(1, kConsumers);
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.rfull[sl]);
         if (!walk.next(index)) break;
     }
     if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
@@ -767,8 +751,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
 
 int decode_stages(int batch) {
     static_assert(227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * GQA_PAGED_MAX_BATCH + 1) * 4 >=
-                      (int64_t)kStageBytes * (kWarps + kBurst),
-                  "a stage for every warp");
+                      (int64_t)kStageBytes * kWarps,
+                  "a stage for every consumer warp");
     const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * (int64_t)batch + 1) * 4;
     const int64_t n = room / kStageBytes;
     return (int)((n < kMaxStages ? n : kMaxStages));

@@ -9,11 +9,11 @@ namespace gqa {
 // min(page_len, rows), 1, 1), 128-byte swizzle.  A status.
 int paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c, int rows);
 
-// Workspace of both attention calls: status word, one counter per (sequence, KV
+// Workspace of both attention calls: status word, one counter per (sequence, Q
 // head) -- zero between calls -- and partial rows.
 constexpr size_t kPagedArrivalsOffset = 256;
 constexpr size_t kPagedPartialsOffset =
-    kPagedArrivalsOffset + (size_t)GQA_PAGED_MAX_BATCH * kNumKVHeads * sizeof(uint32_t);
+    kPagedArrivalsOffset + (size_t)GQA_PAGED_MAX_BATCH * kNumQHeads * sizeof(uint32_t);
 
 // One token a sequence.
 int paged_decode_tile();
