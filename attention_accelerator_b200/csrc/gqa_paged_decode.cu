@@ -42,14 +42,15 @@ namespace {
 constexpr int kWarps = 8;                      // consumer warps
 constexpr int kBurst = 4;                      // tiles that the loader handles at once
 constexpr int kFinishers = kGroup;              // finisher warps, one a Q head
-constexpr int kLoaderWarp = kWarps, kQueryWarp = kWarps + 1, kFinishWarp = kWarps + 2;
+constexpr int kLoaders = 2;                    // loader warps
+constexpr int kLoaderWarp = kWarps, kQueryWarp = kLoaderWarp + kLoaders, kFinishWarp = kQueryWarp + 1;
 constexpr int kThreads = (kFinishWarp + kFinishers) * 32;
 constexpr int kTile = 32;                      // keys
 constexpr int kTileShift = 5;
 constexpr int kSteps = kTile / 16;             // of 16 keys
 constexpr int kHalfBytes = kTile * kHeadDim;   // K or V of a tile
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kMaxStages = 200 * 1024 / kStageBytes;
+constexpr int kMaxStages = 3 * kWarps;
 constexpr int kPagesPerTile = kTile / kPagedMinPage;
 static_assert(kSteps == 2 && kPagesPerTile == 2, "scales of two pages a tile");
 constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
@@ -63,13 +64,13 @@ struct alignas(16) Slot {            // one unit's queries (two slots)
     int lo, hi, m, pad;
 };
 struct alignas(16) Shared {
-    uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2], rfull[2], rempty[2];
+    uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2], rfull, rempty;
     Slot slot[2];
     float4 scales[kMaxStages];  // K of the tile's two pages, V of them
-    struct {  // what the consumer warps make of a piece (two of them)
+    struct {  // what the consumer warps make of a piece
         float acc[kWarps][kGroup][kRowF];
         float m[kWarps][kGroup], l[kWarps][kGroup];
-    } result[2];
+    } result;
     int sum[kThreads / 32];
 };
 
@@ -343,9 +344,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.qfull[i], 1);
             mbar_init(&s.qempty[i], kWarps);
-            mbar_init(&s.rfull[i], kWarps);
-            mbar_init(&s.rempty[i], kFinishers);
         }
+        mbar_init(&s.rfull, kWarps);
+        mbar_init(&s.rempty, kFinishers);
         fence_barrier_init();
         prefetch_tensormap(&a.kmap);
         prefetch_tensormap(&a.vmap);
@@ -388,11 +389,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     Walk walk;
     walk.start(index, me < G ? total * me / G : 0, me < G ? total * (me + 1) / G : 0);
 
-    if (warp == kLoaderWarp) {
+    if (warp >= kLoaderWarp && warp < kQueryWarp) {
         // ============================ loader ============================
-        // One warp's time per tile bounds the CTA's rate (one at a time: about 700
-        // cycles, as long as 16 KB take to arrive), so it works on kBurst tiles at
-        // once, a tile a lane.
+        // What a loader warp does per tile takes longer than the tile needs to arrive
+        // (about 700 cycles for one tile at a time, 355 in bursts, of which the copies'
+        // issue is the most; 8 KB arrive in 355), so each works on kBurst tiles at once,
+        // a tile a lane, and each group of kBurst stages has one of the warps.
         const uint64_t policy = l2_evict_first_policy();
         const int shift = p.c.page_shift;
         const bool two = shift < kTileShift;  // two pages a tile (16 tokens each)
@@ -439,15 +441,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                     later = pages(j0 + 64);
                 }
                 const int batch_n = min(32, walk.n - j0);
-                for (int k0 = 0; k0 < batch_n; k0 += kBurst) {
-                    const int n = min(kBurst, batch_n - k0);
-                    const bool mine = lane >= k0 && lane < k0 + n;
-                    int to = stg + lane - k0, turn = round;
-                    if (to >= stages) {
-                        to -= stages;
-                        ++turn;
-                    }
-                    if (mine && turn > 0) ok = mbar_wait(&s.empty[to], (turn - 1) & 1);
+                for (int k0 = 0, n; k0 < batch_n; k0 += n) {
+                    n = min(kBurst - stg % kBurst, batch_n - k0);  // to the end of the group
+                    const bool mine = stg / kBurst % kLoaders == warp - kLoaderWarp && lane >= k0 && lane < k0 + n;
+                    const int to = stg + lane - k0;
+                    if (mine && round > 0) ok = mbar_wait(&s.empty[to], (round - 1) & 1);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (mine) {
@@ -476,8 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                         later = pages(64);
                     }
                     stg += n;
-                    if (stg >= stages) {
-                        stg -= stages;
+                    if (stg == stages) {
+                        stg = 0;
                         ++round;
                     }
                 }
@@ -488,8 +486,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
             // Do not leave while copies into this CTA's shared memory are in flight.
             for (int i = 0; i < stages; ++i) {
-                const int filled = i < stg ? round + 1 : round;  // times stage i was
-                if (filled > 0) mbar_wait(&s.full[i], (filled - 1) & 1);
+                const int filled = i < stg ? round + 1 : round;  // times stage i was, its own group's
+                if (i / kBurst % kLoaders == warp - kLoaderWarp && filled > 0) mbar_wait(&s.full[i], (filled - 1) & 1);
             }
         }
         return;
@@ -591,10 +589,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         }
         bool ok = true;  // after a wait that timed out: no more waits, but the counters are kept
         for (int n = 0; walk.n > 0; ++n) {
-            const int sl = n & 1;
-            if (ok) ok = mbar_wait(&s.rfull[sl], (n >> 1) & 1);
+            if (ok) ok = mbar_wait(&s.rfull, n & 1);
             __syncwarp();
-            const auto& r = s.result[sl];
+            const auto& r = s.result;
             float M = -INFINITY, L = 0.f;
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
             auto add = [&](float f, float l, float4 x) {
@@ -611,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             for (int w = 0; w < kWarps; ++w)
                 add(fast_exp2(r.m[w][hq] - Mu), r.l[w][hq], *reinterpret_cast<const float4*>(&r.acc[w][hq][4 * lane]));
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s.rempty[sl]);
+            if (lane == 0) mbar_arrive(&s.rempty);
             bool done = walk.n == walk.unit_tiles;
             if (!done) {
                 // A piece of a unit: store it, and the unit's last CTA merges all.
@@ -730,8 +727,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
         const float back = st.vref * (1.f / kWeightScale);
-        if (ok && n >= 2) ok = mbar_wait(&s.rempty[sl], ((n >> 1) - 1) & 1);
-        auto& r = s.result[sl];
+        if (ok && n >= 1) ok = mbar_wait(&s.rempty, (n - 1) & 1);
+        auto& r = s.result;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             *reinterpret_cast<float4*>(&r.acc[warp][t][16 * g + 4 * i]) =
@@ -743,19 +740,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             r.l[warp][t] = l;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.rfull[sl]);
+        if (lane == 0) mbar_arrive(&s.rfull);
         if (!walk.next(index)) break;
     }
     if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
 }
 
+// A wait by parity is sound only for the phase after the last one that the same
+// warp saw complete, so each stage has one consumer warp and one loader warp: the
+// ring is a whole number of stages for each consumer warp, and of loader groups.
 int decode_stages(int batch) {
     static_assert(227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * GQA_PAGED_MAX_BATCH + 1) * 4 >=
                       (int64_t)kStageBytes * kWarps,
                   "a stage for every consumer warp");
+    static_assert(kWarps % kBurst == 0 && kMaxStages % kWarps == 0, "whole groups");
     const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * (int64_t)batch + 1) * 4;
     const int64_t n = room / kStageBytes;
-    return (int)((n < kMaxStages ? n : kMaxStages));
+    return (int)(n < kMaxStages ? n : kMaxStages) / kWarps * kWarps;
 }
 
 using Kernel = void (*)(DecodePagedArgs);
