@@ -448,11 +448,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                     if (mine && round > 0) ok = mbar_wait(&s.empty[to], (round - 1) & 1);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
+                    if (j0 + k0 == 0) {  // a piece's first scales: on their way while its first copies are issued
+                        f_now = scales(now);
+                        f_next = scales(next);
+                        later = pages(64);
+                    }
                     if (mine) {
-                        const int boxes = (now.a >= 0) + (now.b >= 0);
-                        if (j0 + k0 > 0) s.scales[to] = f_now;
-                        // (A piece's first burst: the copies before the scales, which are still on their way.)
-                        if (j0 + k0 > 0) mbar_arrive_expect_tx(&s.full[to], 2 * boxes * box_bytes);
                         uint8_t* dst = ring + to * kStageBytes;
                         const int prow = two ? 0 : ((walk.tile + j0 + lane) * kTile) & (p.c.page_len - 1);
                         if (now.a >= 0) {
@@ -463,15 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                             tma_load_page(dst + box_bytes, &a.kmap, 0, walk.h, now.b, &s.full[to], policy);
                             tma_load_page(dst + kHalfBytes + box_bytes, &a.vmap, 0, walk.h, now.b, &s.full[to], policy);
                         }
-                        if (j0 + k0 == 0) {
-                            s.scales[to] = scales(now);
-                            mbar_arrive_expect_tx(&s.full[to], 2 * boxes * box_bytes);
-                        }
-                    }
-                    if (j0 + k0 == 0) {
-                        f_now = scales(now);
-                        f_next = scales(next);
-                        later = pages(64);
+                        s.scales[to] = f_now;
+                        mbar_arrive_expect_tx(&s.full[to], 2 * ((now.a >= 0) + (now.b >= 0)) * box_bytes);
                     }
                     stg += n;
                     if (stg == stages) {
