@@ -22,6 +22,7 @@ int check_device_memory(std::initializer_list<const void*> ptrs);
 int device_sms(int* sms);
 
 cudaError_t paged_decode_prepare();
+cudaError_t paged_chunk_prepare();
 
 struct DecodeArgs;
 struct RopeTable;

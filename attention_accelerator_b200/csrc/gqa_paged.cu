@@ -360,97 +360,6 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 }
 
 // ---------------------------------------------------------------------------
-// Attention, one warp a Q head, one CTA a (query row, KV head): 32 keys at a
-// time, a key a lane for the scores, 4 dims a lane for the values.
-// ---------------------------------------------------------------------------
-struct SimpleArgs {
-    PagedCall p;
-    RopeSteps rope;
-};
-
-template <int kCode>
-__global__ void __launch_bounds__(kGroup * 32) paged_attention_kernel(const __grid_constant__ SimpleArgs a) {
-    __shared__ float s_q[kGroup][kHeadDim];
-    const PagedCall& p = a.p;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x, h = blockIdx.y, qh = h * kGroup + warp;
-    int b = row;
-    int64_t m;
-    if (p.first_query) {
-        if (row >= p.first_query[p.batch]) return;
-        b = 0;
-        while (p.first_query[b + 1] <= row) ++b;
-        m = (int64_t)p.seq_lens[b] - (p.first_query[b + 1] - p.first_query[b]) + (row - p.first_query[b]);
-    } else {
-        m = p.query_positions ? p.query_positions[b] : (int64_t)p.seq_lens[b] - 1;
-    }
-    const KeyRange range = paged_range(p, row, m, paged_length(p, b));
-    const __nv_bfloat16* q = p.q + row * p.q_row_stride + qh * p.q_head_stride;
-    for (int i = lane; i < kPairs; i += 32) {
-        float x = __bfloat162float(q[i]), y = __bfloat162float(q[i + kPairs]);
-        if (!p.q_rotated) {
-            const float2 f = rope_factor(a.rope.step[i], m);
-            const float re = x * f.x - y * f.y;
-            y = x * f.y + y * f.x;
-            x = re;
-        }
-        s_q[warp][i] = x * p.scale;
-        s_q[warp][i + kPairs] = y * p.scale;
-    }
-    __syncwarp();
-    float top = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = range.lo; k0 < range.hi; k0 += 32) {
-        const int key = k0 + lane;
-        const bool seen = key < range.hi;
-        int page = seen ? p.block_table[b * p.table_stride + (key >> p.c.page_shift)] : -1;
-        if (page >= p.c.pages) page = -1;
-        const int64_t at = page < 0 ? 0 : page * p.c.page_stride + (key & (p.c.page_len - 1)) * p.c.row_stride +
-                                              h * p.c.head_stride;
-        float z = 0.f;
-        if (page >= 0) {
-            for (int d = 0; d < kHeadDim; d += 16) {
-                const uint4 w = *reinterpret_cast<const uint4*>(p.c.k + at + d);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    z = fmaf(code_value<kCode>((uint8_t)(ws[e >> 2] >> (8 * (e & 3)))), s_q[warp][d + e], z);
-            }
-            z *= p.c.k_scale[page * p.c.scale_page_stride + h];
-        }
-        if (p.cap > 0.f) z = p.cap * tanhf(z / p.cap);
-        if (p.slopes) z -= p.slopes[qh] * (float)llabs(m - key);
-        if (!seen) z = -INFINITY;
-        float mx = z;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        const float now = fmaxf(top, mx);
-        const float use = now == -INFINITY ? 0.f : now;
-        const float alpha = expf(top - use);
-        const float w = seen ? expf(z - use) : 0.f;
-        total = total * alpha + w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] *= alpha;
-        top = now;
-        const float wv = page >= 0 ? w * p.c.v_scale[page * p.c.scale_page_stride + h] : 0.f;
-        const int n = min(32, range.hi - k0);
-        for (int i = 0; i < n; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, wv, i);
-            const int64_t ai = __shfl_sync(0xffffffffu, at, i);
-            if (__shfl_sync(0xffffffffu, page, i) < 0) continue;
-            const uint32_t c = *reinterpret_cast<const uint32_t*>(p.c.v + ai + 4 * lane);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = fmaf(wi, code_value<kCode>((uint8_t)(c >> (8 * e))), acc[e]);
-        }
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    __nv_bfloat16* out = p.out + row * p.out_row_stride + qh * p.out_head_stride + 4 * lane;
-    const bool any = range.hi > range.lo;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = __float2bfloat16_rn(any ? acc[e] / total : 0.f);
-}
-
-// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -547,36 +456,34 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
 
 int launched() { return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA; }
 
+size_t workspace_of(int batch, int rows, int heads, bool chunked, int sms) {
+    return chunked ? paged_chunk_workspace(batch, rows, heads, sms) : paged_decode_workspace(sms);
+}
+
 int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p, void* workspace,
            size_t workspace_bytes, void* stream, bool chunked) {
-    SimpleArgs a;
-    int st = check_call(q, out, cache, p, chunked, &a.p);
+    PagedCall call;
+    int st = check_call(q, out, cache, p, chunked, &call);
     if (st != GQA_OK) return st;
     if (!workspace || !aligned16(workspace)) return GQA_ERR_WORKSPACE;
     int sms = 0;
     st = device_sms(&sms);
     if (st != GQA_OK) return st;
-    if (workspace_bytes < paged_decode_workspace(sms)) return GQA_ERR_WORKSPACE;
+    if (workspace_bytes < workspace_of(p->batch, p->rows, cache->kv_heads, chunked, sms)) return GQA_ERR_WORKSPACE;
     st = check_device_memory({workspace});
     if (st != GQA_OK) return st;
     if (p->rows == 0) return GQA_OK;
-    a.rope = rope_steps_of(p->rope_theta);
-    const dim3 grid(p->rows, cache->kv_heads);
+    const RopeSteps& rope = rope_steps_of(p->rope_theta);
+    const int tile = chunked ? paged_chunk_tile() : paged_decode_tile();
+    CUtensorMap kmap, vmap;
+    if ((st = paged_map(&kmap, call.c.k, call.c, tile)) != GQA_OK ||
+        (st = paged_map(&vmap, call.c.v, call.c, tile)) != GQA_OK)
+        return st;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!chunked) {
-        CUtensorMap kmap, vmap;
-        if ((st = paged_map(&kmap, a.p.c.k, a.p.c, paged_decode_tile())) != GQA_OK || (st = paged_map(&vmap, a.p.c.v, a.p.c, paged_decode_tile())) != GQA_OK)
-            return st;
-        return launch_paged_decode(a.p, a.rope, cache->code, kmap, vmap, sms, static_cast<uint8_t*>(workspace), s) ==
-                       cudaSuccess
-                   ? GQA_OK
-                   : GQA_ERR_CUDA;
-    }
-    if (cache->code == GQA_CODE_INT8)
-        paged_attention_kernel<GQA_CODE_INT8><<<grid, kGroup * 32, 0, s>>>(a);
-    else
-        paged_attention_kernel<GQA_CODE_E4M3><<<grid, kGroup * 32, 0, s>>>(a);
-    return launched();
+    const cudaError_t e = chunked ? launch_paged_chunk(call, rope, cache->code, kmap, vmap, sms, ws, s)
+                                  : launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, s);
+    return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
 }  // namespace
@@ -708,7 +615,7 @@ size_t gqa_paged_workspace_bytes(const gqa_paged_cache* cache, const gqa_paged_p
         return 0;
     int sms = 0;
     if (device_sms(&sms) != GQA_OK) return 0;
-    return paged_decode_workspace(sms);
+    return workspace_of(p->batch, p->rows, cache->kv_heads, p->first_query != nullptr, sms);
 }
 
 int gqa_decode_paged(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,

@@ -1,0 +1,991 @@
+// gqa_paged_chunk.cu -- any number of queries a sequence over the paged 8-bit
+// cache, on the fifth-generation tensor cores.
+//
+// Work.  A unit is 64 consecutive queries of one sequence and one KV head: 256
+// rows (query, Q head), two M = 128 tiles.  Its keys are those that any of its
+// rows sees, in tiles of 128 on a grid of absolute positions.  plan_units_kernel
+// (one CTA) finds every unit's keys from the lengths and masks in device memory,
+// sums the tiles, and says where each CTA of paged_chunk_kernel begins: all tiles
+// of all units in order are dealt out evenly, as decode_paged does, so that causal
+// prompts, ragged batches and one long context alike fill the GPU.  A unit that
+// crosses shares leaves FP32 partial rows; its last CTA merges them in order.
+//
+// Precision.  Codes become FP16 exactly for S = Q K^T; Q is rotated in FP32,
+// divided by a power of two that brings the row's largest below 1, and rounded to
+// FP16 (2^-11 of a term: three more bits than the BF16 it came as).  K's scale
+// multiplies the FP32 scores.  V's scale, over a running power of two, multiplies
+// its codes in FP16, the weights 2^(z - m) round to FP16, and O accumulates in
+// FP32 in TMEM: together a few 2^-11 of the sum of |weight * value| at worst, for
+// an output that is rounded to 2^-8.
+//
+// Warps (one CTA per SM):
+//   0-3, 4-7   softmax of M tile 0, 1: a thread a row.  Per unit, 4 lanes rotate one
+//              query's 4 head rows (16 pairs each) into the swizzled A operand.  Per
+//              tile: maximum of the S row from TMEM (per 16 keys, then times their
+//              page's scale), weights back over S as FP16 (the A operand of O += P V).
+//              The reference m moves only when a maximum passes it by 2^8; then O is
+//              rescaled in TMEM, which the in-order tensor pipe leaves still.
+//   8-11       conversion: 16 KB of codes (TMA, 128-byte swizzle) to 32 KB of FP16 in
+//              the K-major (K) and MN-major (V) operand layout, which are the same
+//              bytes: rows of 64 dims, two blocks, 128-byte swizzle.
+//   12         MMA issuer: S0 S1 | PV0 S0' PV1 S1' | ..., so that one M tile's products
+//              run while the other's softmax does.
+//   13         loader: table entries, scales, TMA.
+//   14         zeros of units whose rows see nothing.
+#include "gqa_internal.h"
+#include "gqa_paged.cuh"
+#include "gqa_paged_internal.h"
+#include "gqa_tcgen05.cuh"
+
+namespace gqa {
+
+namespace {
+
+constexpr int kTile = 128;                 // keys
+constexpr int kTileShift = 7;
+constexpr int kTokens = 64;                // queries of a unit
+constexpr int kRowsM = 128;                // rows of an M tile
+constexpr int kRawBytes = kTile * kHeadDim;          // K or V codes of a tile
+constexpr int kBlockBytes = kTile * 128;             // 128 rows x 64 dims of FP16
+constexpr int kHalfTileBytes = 2 * kBlockBytes;      // K or V of a tile in FP16; an M tile of Q
+constexpr int kRaw = 3;                    // ring slots of codes
+constexpr int kConv = 3;                   // ring slots of FP16
+constexpr int kScaleSlots = 4;             // tiles whose scales are in flight
+constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
+constexpr int kThreads = (kLoadWarp + 2) * 32;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColO = 256;  // two of 128 columns each; P over the first 64 of its S
+constexpr float kHeadroom = 8.f;   // log2 by which a maximum may pass the reference
+constexpr float kLift = 7.f;       // weights are 2^(z - m + 7): up to 2^15, and FP16's 2^-24 is 2^-31 of the reference
+
+constexpr int kSlotFloats = kRowsM * 2 * (kHeadDim + 2);  // a partial: acc [32][256] float4, (m, l) [256]
+
+// kind::f16 with FP16 A and B, FP32 accumulators, M = 128, N = 128.
+constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);  // B (V) MN-major
+
+struct Unit {
+    int32_t b, row0, n, pos0;     // sequence, first query row, queries, position of the first
+    int32_t lo, hi, tiles, tile0; // keys that any row sees, their tiles
+    int64_t first;                // tiles of all units before it (per head)
+    int64_t pad;
+};
+struct Meta {
+    int64_t total;  // tiles of all units and heads
+    int32_t ctas;   // with a share
+    int32_t units;
+};
+
+struct TileScales {
+    float k[8], v[8];   // of each 16 keys: K's scale (NaN where V's is no number), V's over the reference
+    float fall, ref;    // what O is multiplied by before this tile; the reference
+    float pad[2];
+};
+
+struct alignas(16) Shared {
+    uint64_t raw_full[kRaw], raw_empty[kRaw], conv_full[kConv], conv_empty[kConv];
+    uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], group[2];
+    uint64_t pad;
+    TileScales scales[kScaleSlots];
+    uint32_t tmem;
+    int last[2];
+};
+
+struct alignas(64) ChunkPagedArgs {
+    CUtensorMap kmap, vmap;  // (128, page_len, heads, pages) bytes, box (128, page_len, 1, 1)
+    PagedCall p;
+    RopeSteps rope;
+    uint32_t* status;
+    const Meta* meta;
+    const Unit* units;
+    const int32_t* starts;  // [ctas] unit in which each share begins
+    uint32_t* arrivals;     // [units][heads][2]
+    float* partials;        // [ctas][2][kSlotFloats]
+};
+
+struct PlanUnitsArgs {
+    PagedCall p;
+    Meta* meta;
+    Unit* units;
+    int32_t* starts;
+    uint32_t* arrivals;
+    int32_t max_units, ctas;
+};
+
+// ---------------------------------------------------------------------------
+// Planning: units of every sequence, the keys each sees, running sums, shares.
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+
+// Exclusive running sum over the CTA of one value a thread; *all gets the total.
+__device__ __forceinline__ int64_t scan_exclusive(int64_t v, int64_t* warp_sum, int64_t* all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += x;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int64_t base = 0, total = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+        if (w < warp) base += warp_sum[w];
+        total += warp_sum[w];
+    }
+    *all = total;
+    return base + incl - v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_constant__ PlanUnitsArgs a) {
+    extern __shared__ int32_t offset[];  // first unit of each sequence
+    __shared__ int64_t warp_sum[kPlanThreads / 32];
+    const PagedCall& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, batch = p.batch;
+    // Rows of sequence b, kept within the call's whatever the device's numbers say.
+    auto rows_of = [&](int b, int& row0) {
+        row0 = min(max(p.first_query[b], 0), p.rows);
+        return max(0, min(p.first_query[b + 1], p.rows) - row0);
+    };
+    const int per = (batch + kPlanThreads - 1) / kPlanThreads;
+    const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
+    int64_t sum = 0, total = 0;
+    for (int b = b0; b < b1; ++b) {
+        int row0;
+        sum += (rows_of(b, row0) + kTokens - 1) / kTokens;
+    }
+    int64_t at = scan_exclusive(sum, warp_sum, &total);
+    for (int b = b0; b < b1; ++b) {
+        int row0;
+        offset[b] = (int)at;
+        at += (rows_of(b, row0) + kTokens - 1) / kTokens;
+    }
+    const int units = (int)min(total, (int64_t)a.max_units);
+    __syncthreads();
+    // A warp a unit: the keys that any of its rows sees.
+    for (int u = warp; u < units; u += kPlanThreads / 32) {
+        int lo_b = 0, hi_b = batch;
+        while (hi_b - lo_b > 1) {
+            const int mid = (lo_b + hi_b) >> 1;
+            if (offset[mid] <= u) lo_b = mid; else hi_b = mid;
+        }
+        const int b = lo_b;  // (of sequences that share an offset the last: the one with rows)
+        int row0;
+        const int rows = rows_of(b, row0), skip = (u - offset[b]) * kTokens;
+        const int n = min(kTokens, rows - skip), len = paged_length(p, b);
+        const int64_t pos0 = (int64_t)p.seq_lens[b] - rows + skip;
+        int lo = 0x7fffffff, hi = 0;
+        for (int i = lane; i < n; i += 32) {
+            const KeyRange r = paged_range(p, row0 + skip + i, pos0 + i, len);
+            if (r.hi > r.lo) {
+                lo = min(lo, r.lo);
+                hi = max(hi, r.hi);
+            }
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        if (lane == 0) {
+            Unit x;
+            x.b = b;
+            x.row0 = row0 + skip;
+            x.n = n;
+            x.pos0 = (int)pos0;
+            x.lo = lo;
+            x.hi = hi;
+            x.tile0 = hi > 0 ? lo >> kTileShift : 0;
+            x.tiles = hi > 0 ? ((hi + kTile - 1) >> kTileShift) - x.tile0 : 0;
+            x.first = 0;
+            x.pad = 0;
+            a.units[u] = x;
+        }
+    }
+    __syncthreads();
+    const int heads = p.c.kv_heads;
+    const int uper = (units + kPlanThreads - 1) / kPlanThreads;
+    const int u0 = min(units, tid * uper), u1 = min(units, u0 + uper);
+    sum = 0;
+    for (int u = u0; u < u1; ++u) sum += a.units[u].tiles;
+    at = scan_exclusive(sum, warp_sum, &total);
+    total *= heads;
+    const int64_t G = min((int64_t)a.ctas, total);
+    for (int u = u0; u < u1; ++u) {
+        const int tiles = a.units[u].tiles;
+        a.units[u].first = at;
+        // Shares i begin at tile total * i / G: those that begin in this unit.
+        const int64_t begin = at * heads, end = (at + tiles) * heads;
+        if (tiles > 0)
+            for (int64_t i = (begin * G + total - 1) / total; i < G && total * i / G < end; ++i)
+                if (total * i / G >= begin) a.starts[i] = u;
+        at += tiles;
+    }
+    for (int i = tid; i < units * heads * 2; i += kPlanThreads) a.arrivals[i] = 0;
+    if (tid == 0) *a.meta = Meta{total, (int32_t)G, units};
+}
+
+// ---------------------------------------------------------------------------
+// A CTA's walk through its share, one unit's piece at a time.
+// ---------------------------------------------------------------------------
+struct Walk {
+    int64_t x, end;
+    int u, h, j, n;  // unit, KV head, first tile within the unit and tiles of the piece
+    Unit unit;
+    __device__ __forceinline__ void start(const ChunkPagedArgs& a, const Meta& meta) {
+        n = 0;
+        const int64_t me = blockIdx.x, G = meta.ctas;
+        if (me >= G) return;
+        x = meta.total * me / G;
+        end = meta.total * (me + 1) / G;
+        u = a.starts[me];
+        unit = a.units[u];
+        const int64_t rem = x - unit.first * a.p.c.kv_heads;
+        h = (int)(rem / unit.tiles);
+        place(a);
+    }
+    __device__ __forceinline__ int64_t unit_first(const ChunkPagedArgs& a) const {
+        return unit.first * a.p.c.kv_heads + (int64_t)h * unit.tiles;
+    }
+    __device__ __forceinline__ void place(const ChunkPagedArgs& a) {
+        j = (int)(x - unit_first(a));
+        n = (int)min((int64_t)(unit.tiles - j), end - x);
+    }
+    __device__ __forceinline__ bool next(const ChunkPagedArgs& a) {
+        x += n;
+        if (x >= end) return false;
+        if (++h == a.p.c.kv_heads) {
+            h = 0;
+            do unit = a.units[++u];
+            while (unit.tiles == 0);
+        }
+        place(a);
+        return true;
+    }
+};
+
+__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int head, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(0), "r"(head), "r"(page), "r"(smem_addr(bar))
+        : "memory");
+}
+
+template <int kCode>
+__device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (kCode == GQA_CODE_INT8) {
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
+        const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
+        lo = *reinterpret_cast<const uint32_t*>(&a);
+        hi = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+// V's operand: codes times their scale.  A NaN code would reach, times a weight of
+// zero, the rows that do not see its key: the maximum with -448 makes it a number.
+template <int kCode>
+__device__ __forceinline__ uint32_t scale_half2(uint32_t a, __half2 b) {
+    __half2 v = *reinterpret_cast<const __half2*>(&a);
+    if constexpr (kCode == GQA_CODE_E4M3) v = __hmax2(v, __half2half2(__ushort_as_half(0xdf00)));
+    v = __hmul2(v, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float tanh_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * 2.8853900817779268f) + 1.f));
+    return fmaf(-2.f, r, 1.f);
+}
+
+__device__ __forceinline__ float finite_or(float x, float other) {
+    return fabsf(x) <= 3.402823466e38f ? x : other;
+}
+
+// The row of a softmax thread.
+struct Row {
+    float factor;      // scores of the row: S * page scale * factor, in log2 units (or over the cap)
+    float cap2;        // cap * log2(e)
+    float slope;       // times log2(e)
+    int lo, hi, pos;   // visible keys, position
+};
+
+// Scores of 32 keys from key k0 on, in log2 units; masked ones -inf where `edge`.
+template <bool kCap, bool kBias>
+__device__ __forceinline__ void scores(float (&z)[32], const uint32_t (&s)[32], const Row& row, const float* ks,
+                                       int k0, bool edge) {
+    const float f0 = row.factor * ks[0], f1 = row.factor * ks[1];
+    const float ahead = kBias ? (float)(k0 - row.pos) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        float x = __uint_as_float(s[e]) * (e < 16 ? f0 : f1);
+        if constexpr (kCap) x = row.cap2 * tanh_fast(x);
+        if constexpr (kBias) x = fmaf(-row.slope, fabsf(ahead + (float)e), x);
+        z[e] = x;
+    }
+    if (edge) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (k0 + e < row.lo || k0 + e >= row.hi) z[e] = -INFINITY;
+    }
+}
+
+template <int kCode, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkPagedArgs a) {
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    uint8_t* q_smem = smem;                                // two M tiles
+    uint8_t* conv = q_smem + 2 * kHalfTileBytes;           // kConv slots of FP16
+    uint8_t* raw = conv + kConv * kHalfTileBytes;          // kRaw slots of codes
+    Shared& s = *reinterpret_cast<Shared*>(raw + kRaw * kRawBytes);
+    const PagedCall& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < kRaw; ++i) {
+            mbar_init(&s.raw_full[i], 1);
+            mbar_init(&s.raw_empty[i], 4);
+        }
+        for (int i = 0; i < kConv; ++i) {
+            mbar_init(&s.conv_full[i], 4);
+            mbar_init(&s.conv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.q_full[i], kRowsM);
+            mbar_init(&s.s_full[i], 1);
+            mbar_init(&s.p_full[i], kRowsM);
+            mbar_init(&s.pv_done[i], 1);
+            mbar_init(&s.group[i], kRowsM);
+        }
+        fence_barrier_init();
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s.tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (lane == 0) {
+            prefetch_tensormap(&a.kmap);
+            prefetch_tensormap(&a.vmap);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s.tmem;
+    const Meta meta = *a.meta;
+    Walk walk;
+    walk.start(a, meta);
+    bool ok = true;
+
+    if (warp < kConvWarp) {
+        // ============================ softmax ============================
+        const int m = warp >> 2, r = tid & (kRowsM - 1);  // M tile, row: query 32 m + r / 4, head r % 4
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + kColS + m * 128 + lanes, t_o = tmem + kColO + m * 128 + lanes;
+        uint8_t* q_tile = q_smem + m * kHalfTileBytes;
+        int seen = 0;     // tiles of this M tile so far (phases of s_full)
+        int pieces = 0;   // of this M tile (phases of pv_done)
+        int syncs = 0;    // phases of group
+        int slot = 0;     // scales of the piece's first tile
+        auto group_sync = [&] {
+            mbar_arrive(&s.group[m]);
+            if (ok) ok = mbar_wait(&s.group[m], syncs & 1);
+            ++syncs;
+        };
+        while (walk.n > 0) {
+            const Unit& un = walk.unit;
+            const int token = 32 * m + (r >> 2), head = r & 3;
+            const bool active = un.n > 32 * m, real = token < un.n;
+            if (active && ok) {
+                Row row;
+                const int64_t pos = (int64_t)un.pos0 + token;
+                row.pos = (int)pos;
+                row.lo = 0;
+                row.hi = 0x7fffffff;  // rows of no query: nothing to mask, nothing written
+                if (real) {
+                    const KeyRange range = paged_range(p, un.row0 + token, pos, paged_length(p, un.b));
+                    row.lo = range.lo;
+                    row.hi = range.hi;
+                }
+                row.cap2 = p.cap * 1.4426950408889634f;
+                row.slope = kBias ? p.slopes[walk.h * kGroup + head] * 1.4426950408889634f : 0.f;
+                row.factor = 0.f;
+                // ---- Q: 16 pairs of this lane's query, 4 heads ----
+                {
+                    float2 f[16];
+                    const int pair0 = 16 * (lane & 3);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        f[i] = p.q_rotated || !real ? make_float2(1.f, 0.f) : rope_factor(a.rope.step[pair0 + i], pos);
+                    const float unit = kCap ? p.scale / p.cap : p.scale * 1.4426950408889634f;
+#pragma unroll 1
+                    for (int hq = 0; hq < kGroup; ++hq) {
+                        uint32_t xw[8], yw[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) xw[i] = yw[i] = 0u;
+                        if (real) {
+                            const uint4* q = reinterpret_cast<const uint4*>(
+                                p.q + (int64_t)(un.row0 + token) * p.q_row_stride +
+                                (walk.h * kGroup + hq) * p.q_head_stride + pair0);
+                            const uint4 x0 = q[0], x1 = q[1], y0 = q[8], y1 = q[9];
+                            xw[0] = x0.x; xw[1] = x0.y; xw[2] = x0.z; xw[3] = x0.w;
+                            xw[4] = x1.x; xw[5] = x1.y; xw[6] = x1.z; xw[7] = x1.w;
+                            yw[0] = y0.x; yw[1] = y0.y; yw[2] = y0.z; yw[3] = y0.w;
+                            yw[4] = y1.x; yw[5] = y1.y; yw[6] = y1.z; yw[7] = y1.w;
+                        }
+                        float x[16], y[16], most = 0.f;
+                        bool fine = true;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 xv = bf16x2_to_float2(xw[i >> 1]), yv = bf16x2_to_float2(yw[i >> 1]);
+                            const float re = i & 1 ? xv.y : xv.x, im = i & 1 ? yv.y : yv.x;
+                            x[i] = re * f[i].x - im * f[i].y;
+                            y[i] = re * f[i].y + im * f[i].x;
+                            fine &= fabsf(x[i]) <= 3.402823466e38f && fabsf(y[i]) <= 3.402823466e38f;
+                            most = fmaxf(most, fmaxf(fabsf(x[i]), fabsf(y[i])));
+                        }
+                        if (!fine) most = INFINITY;
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                        const int e = min(253, max(1, (__float_as_int(most) >> 23) + 1));
+                        const float up = __int_as_float(e << 23), down = __int_as_float((254 - e) << 23);
+                        if (hq == head) row.factor = most == INFINITY ? __int_as_float(0x7fffffff) : unit * up;
+                        const int qr = (r & ~3) + hq;  // row of the M tile
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                w[i] = half ? pack_half2(y[2 * i] * down, y[2 * i + 1] * down)
+                                            : pack_half2(x[2 * i] * down, x[2 * i + 1] * down);
+                            uint8_t* at = q_tile + half * kBlockBytes + qr * 128;
+                            const int c = 2 * (lane & 3);
+                            *reinterpret_cast<uint4*>(at + ((c ^ (qr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(at + (((c + 1) ^ (qr & 7)) << 4)) =
+                                make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    mbar_arrive(&s.q_full[m]);
+                }
+                float ref = -INFINITY;   // weights are 2^(z - ref)
+                float l = 0.f, vref = 0.f;
+                for (int j = 0; j < walk.n; ++j) {
+                    if (!warp_wait(&s.s_full[m], (seen + j) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const TileScales& sc = s.scales[(slot + j) & (kScaleSlots - 1)];
+                    const int k0 = (un.tile0 + walk.j + j) << kTileShift;
+                    const bool edge = __any_sync(0xffffffffu, row.lo > k0 || row.hi < k0 + kTile);
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(t_s + 32 * c, v);
+                        tmem_wait_ld();
+                        if constexpr (kBias) {
+                            float z[32];
+                            scores<kCap, kBias>(z, v, row, sc.k + 2 * c, k0 + 32 * c, edge);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, z[e]);
+                        } else {
+                            // The largest S of 16 keys, then their scale: it is not negative, and neither is the cap.
+                            if (edge) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (k0 + 32 * c + e < row.lo || k0 + 32 * c + e >= row.hi) v[e] = 0xff800000u;
+                            }
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                float top = __uint_as_float(v[16 * half]);
+#pragma unroll
+                                for (int e = 1; e < 16; ++e) top = fmaxf(top, __uint_as_float(v[16 * half + e]));
+                                float z = top * (row.factor * sc.k[2 * c + half]);
+                                if constexpr (kCap) z = top == -INFINITY ? top : row.cap2 * tanh_fast(z);
+                                mx = fmaxf(mx, z);
+                            }
+                        }
+                    }
+                    // The reference moves when the maximum passes it by 2^kHeadroom (at once from nothing).
+                    const float want = mx - kLift;
+                    const bool move = want > ref + kHeadroom || (ref == -INFINITY && want > ref);
+                    const float to = move ? want : ref;
+                    const float fall = j > 0 ? sc.fall : 1.f;
+                    if (__any_sync(0xffffffffu, move) || fall != 1.f) {
+                        const float alpha = move ? fast_exp2(ref - to) : 1.f;
+                        l *= alpha;
+                        ref = to;
+                        if (j > 0) {
+                            const float f = alpha * fall;
+#pragma unroll 1
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + 32 * c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st32(t_o + 32 * c, o);
+                            }
+                        }
+                    }
+                    vref = sc.ref;
+                    const float use = ref == -INFINITY ? 0.f : ref;
+                    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32], w[16];
+                        tmem_ld32(t_s + 32 * c, v);
+                        tmem_wait_ld();
+                        if constexpr (kCap || kBias) {
+                            float z[32];
+                            scores<kCap, kBias>(z, v, row, sc.k + 2 * c, k0 + 32 * c, edge);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float p0 = fast_exp2(z[e] - use), p1 = fast_exp2(z[e + 1] - use);
+                                sum0 += p0;
+                                sum1 += p1;
+                                w[e >> 1] = pack_half2(p0, p1);
+                            }
+                        } else {
+                            const float f0 = row.factor * sc.k[2 * c], f1 = row.factor * sc.k[2 * c + 1];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float f = e < 16 ? f0 : f1;
+                                float p0 = fast_exp2(fmaf(__uint_as_float(v[e]), f, -use));
+                                float p1 = fast_exp2(fmaf(__uint_as_float(v[e + 1]), f, -use));
+                                if (edge) {
+                                    const int key = k0 + 32 * c + e;
+                                    if (key < row.lo || key >= row.hi) p0 = 0.f;
+                                    if (key + 1 < row.lo || key + 1 >= row.hi) p1 = 0.f;
+                                }
+                                sum0 += p0;
+                                sum1 += p1;
+                                w[e >> 1] = pack_half2(p0, p1);
+                            }
+                        }
+                        tmem_st16(t_s + 16 * c, w);  // over columns that were read
+                    }
+                    l += sum0 + sum1;
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&s.p_full[m]);
+                }
+                // ---- the piece's rows ----
+                if (ok) ok = warp_wait(&s.pv_done[m], pieces & 1);
+                tc_fence_after();
+                __nv_bfloat16* out = p.out + (int64_t)(un.row0 + token) * p.out_row_stride +
+                                     (walk.h * kGroup + head) * p.out_head_stride;
+                auto write = [&](int c, const float (&x)[32]) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint4 w;
+                        uint32_t* wp = &w.x;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(x[e + 2 * i], x[e + 2 * i + 1]);
+                            wp[i] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                        *reinterpret_cast<uint4*>(out + 32 * c + e) = w;
+                    }
+                };
+                if (walk.n == un.tiles) {
+                    const float f = l == 0.f ? 0.f : vref / l;  // a row that sees nothing is 0
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        float x[32];
+                        tmem_ld32(t_o + 32 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * f;
+                        if (real) write(c, x);
+                    }
+                } else {
+                    // A piece of a unit: its slots as in decode_paged (a share's first piece 0, its last 1).
+                    const int64_t G = meta.ctas, total = meta.total, first = walk.unit_first(a);
+                    const int c0 = (int)(((first + 1) * G + total - 1) / total) - 1;
+                    const int parts = (int)(((first + un.tiles) * G + total - 1) / total) - c0;
+                    const int second = total * c0 / G < first ? 1 : 0;
+                    auto part = [&](int c) {
+                        return a.partials + (int64_t)((c0 + c) * 2 + (c ? 0 : second)) * kSlotFloats;
+                    };
+                    const int prow = m * kRowsM + r;
+                    {
+                        float* mine = part((int)blockIdx.x - c0);
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(t_o + 32 * c, o);
+                            tmem_wait_ld();
+                            if (real)
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    reinterpret_cast<float4*>(mine)[(8 * c + e) * 2 * kRowsM + prow] = make_float4(
+                                        __uint_as_float(o[4 * e]) * vref, __uint_as_float(o[4 * e + 1]) * vref,
+                                        __uint_as_float(o[4 * e + 2]) * vref, __uint_as_float(o[4 * e + 3]) * vref);
+                        }
+                        if (real)
+                            reinterpret_cast<float2*>(mine + 2 * kRowsM * kHeadDim)[prow] = make_float2(ref, l);
+                    }
+                    group_sync();
+                    if (r == 0) {
+                        uint32_t* count = a.arrivals + ((int64_t)walk.u * p.c.kv_heads + walk.h) * 2 + m;
+                        uint32_t before;
+                        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                                     : "=r"(before)
+                                     : "l"(count)
+                                     : "memory");
+                        s.last[m] = before == (uint32_t)(parts - 1);
+                    }
+                    group_sync();
+                    if (ok && s.last[m] && real) {
+                        float M = -INFINITY, L = 0.f;
+                        for (int c = 0; c < parts; ++c)
+                            M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part(c) + 2 * kRowsM * kHeadDim) + prow).x);
+                        const float mu = M == -INFINITY ? 0.f : M;
+                        for (int c = 0; c < parts; ++c) {
+                            const float2 v = __ldcg(reinterpret_cast<const float2*>(part(c) + 2 * kRowsM * kHeadDim) + prow);
+                            L = fmaf(fast_exp2(v.x - mu), v.y, L);
+                        }
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll 1
+                        for (int c4 = 0; c4 < 4; ++c4) {
+                            float x[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = 0.f;
+                            for (int c = 0; c < parts; ++c) {
+                                const float* at = part(c);
+                                const float f = inv * fast_exp2(
+                                    __ldcg(reinterpret_cast<const float2*>(at + 2 * kRowsM * kHeadDim) + prow).x - mu);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float4 v =
+                                        __ldcg(reinterpret_cast<const float4*>(at) + (8 * c4 + e) * 2 * kRowsM + prow);
+                                    x[4 * e] = fmaf(f, v.x, x[4 * e]);
+                                    x[4 * e + 1] = fmaf(f, v.y, x[4 * e + 1]);
+                                    x[4 * e + 2] = fmaf(f, v.z, x[4 * e + 2]);
+                                    x[4 * e + 3] = fmaf(f, v.w, x[4 * e + 3]);
+                                }
+                            }
+                            write(c4, x);
+                        }
+                    }
+                }
+                tc_fence_before();  // the next unit's products overwrite O after this thread's next arrival
+                seen += walk.n;
+                ++pieces;
+            }
+            slot = (slot + walk.n) & (kScaleSlots - 1);
+            if (!ok || !walk.next(a)) break;
+        }
+    } else if (warp < kMmaWarp) {
+        // ============================ conversion ============================
+        const int cw = warp - kConvWarp, t = lane & 3;
+        const int row0 = 32 * cw + (lane >> 2);  // this lane's rows: row0 + 8 i
+        int item = 0;  // K and V of the tiles in turn
+        int rs = 0, rphase = 0, cs = 0, cphase = 0, tile_count = 0;
+        while (walk.n > 0 && ok) {
+            for (int j = 0; j < walk.n && ok; ++j, ++tile_count) {
+                const TileScales& sc = s.scales[tile_count & (kScaleSlots - 1)];
+                const int k0 = (walk.unit.tile0 + walk.j + j) << kTileShift;
+                const int klo = walk.unit.lo - k0, khi = walk.unit.hi - k0;
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv, ++item) {
+                    ok = mbar_wait(&s.raw_full[rs], rphase) && (item < kConv || mbar_wait(&s.conv_empty[cs], cphase ^ 1));
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint8_t* src = raw + rs * kRawBytes;
+                    uint8_t* dst = conv + cs * kHalfTileBytes;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = row0 + 8 * i, sw = row & 7;
+                        const __half2 f = __float2half2_rn(kv ? sc.v[2 * cw + (i >> 1)] : 1.f);
+                        const bool gone = kv && (row < klo || row >= khi);  // no row sees it: its codes may be anything
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int c = 4 * half + t;  // dims 16 c .. 16 c + 15: block `half`
+                            const uint4 x = lds128(src + row * kHeadDim + ((c ^ sw) << 4));
+                            uint32_t w[8];
+                            to_half4<kCode>(x.x, w[0], w[1]);
+                            to_half4<kCode>(x.y, w[2], w[3]);
+                            to_half4<kCode>(x.z, w[4], w[5]);
+                            to_half4<kCode>(x.w, w[6], w[7]);
+                            if (kv) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) w[e] = gone ? 0u : scale_half2<kCode>(w[e], f);
+                            }
+                            uint8_t* at = dst + half * kBlockBytes + row * 128;
+                            *reinterpret_cast<uint4*>(at + (((2 * t) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(at + (((2 * t + 1) ^ sw) << 4)) =
+                                make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&s.conv_full[cs]);
+                        mbar_arrive(&s.raw_empty[rs]);
+                    }
+                    if (++rs == kRaw) {
+                        rs = 0;
+                        rphase ^= 1;
+                    }
+                    if (++cs == kConv) {
+                        cs = 0;
+                        cphase ^= 1;
+                    }
+                }
+            }
+            if (!ok || !walk.next(a)) break;
+        }
+    } else if (warp == kMmaWarp) {
+        // ============================ MMA issuer ============================
+        if (lane == 0) {
+            int cs = 0, cphase = 0;   // next slot of FP16
+            int seen[2] = {0, 0}, pieces[2] = {0, 0};
+            auto advance = [&] {
+                if (++cs == kConv) {
+                    cs = 0;
+                    cphase ^= 1;
+                }
+            };
+            auto issue_s = [&](int m, int slot) {
+                const uint32_t kaddr = smem_addr(conv + slot * kHalfTileBytes), qaddr = smem_addr(q_smem + m * kHalfTileBytes);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk) {
+                    const uint32_t off = (kk >> 2) * kBlockBytes + (kk & 3) * 32;
+                    mma_ss(tmem + kColS + m * 128, smem_desc_sw128(qaddr + off, 16, 1024),
+                           smem_desc_sw128(kaddr + off, 16, 1024), kIdescS, kk != 0);
+                }
+                tc_commit(&s.s_full[m]);
+            };
+            while (walk.n > 0 && ok) {
+                const int ms = walk.unit.n > 32 ? 2 : 1;
+                // S of the first tile.
+                ok = mbar_wait(&s.conv_full[cs], cphase);
+                for (int m = 0; m < ms && ok; ++m) {
+                    ok = mbar_wait(&s.q_full[m], pieces[m] & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(m, cs);
+                }
+                if (!ok) break;
+                tc_commit(&s.conv_empty[cs]);
+                advance();
+                for (int j = 0; j < walk.n && ok; ++j) {
+                    const int vs = cs, vphase = cphase;
+                    advance();
+                    const bool more = j + 1 < walk.n;
+                    const int ks = cs, kphase = cphase;
+                    for (int m = 0; m < ms; ++m) {
+                        ok = mbar_wait(&s.p_full[m], seen[m] & 1) && (m || mbar_wait(&s.conv_full[vs], vphase));
+                        if (!ok) break;
+                        ++seen[m];
+                        tc_fence_after();
+                        const uint32_t vaddr = smem_addr(conv + vs * kHalfTileBytes);
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma_ts(tmem + kColO + m * 128, tmem + kColS + m * 128 + 8 * kk,
+                                   smem_desc_sw128(vaddr + kk * 16 * 128, kBlockBytes, 1024), kIdescO,
+                                   (j > 0 || kk > 0) ? 1u : 0u);
+                        if (m == ms - 1) tc_commit(&s.conv_empty[vs]);
+                        if (more) {
+                            if (m == 0) ok = mbar_wait(&s.conv_full[ks], kphase);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_s(m, ks);
+                            if (m == ms - 1) tc_commit(&s.conv_empty[ks]);
+                        } else {
+                            tc_commit(&s.pv_done[m]);
+                        }
+                    }
+                    if (more) advance();
+                }
+                for (int m = 0; m < ms; ++m) ++pieces[m];
+                if (!ok || !walk.next(a)) break;
+            }
+        }
+    } else if (warp == kLoadWarp) {
+        // ============================ loader ============================
+        const int shift = p.c.page_shift, per_tile = kTile >> shift;  // pages of a tile
+        const int box_bytes = p.c.page_len * kHeadDim;
+        int rs = 0, rphase = 0, tile_count = 0, item = 0;
+        while (walk.n > 0 && ok) {
+            const int32_t* table = p.block_table + walk.unit.b * p.table_stride;
+            const int64_t lo = walk.unit.lo, hi = walk.unit.hi;
+            // Lane's page of tile j (-1: no visible key, not loaded).
+            auto entry = [&](int j) {
+                const int64_t key = ((int64_t)(walk.unit.tile0 + walk.j + j) << kTileShift) + ((int64_t)lane << shift);
+                if (lane >= per_tile || j >= walk.n || key >= hi || key + p.c.page_len <= lo) return -1;
+                const int page = table[key >> shift];
+                return page >= 0 && page < p.c.pages ? page : p.c.pages;  // out of the map: TMA fills zeros
+            };
+            auto scale = [&](const float* at, int page) {
+                return page >= 0 && page < p.c.pages ? at[page * p.c.scale_page_stride + walk.h] : 0.f;
+            };
+            int page = entry(0), page1 = entry(1);
+            float ks = scale(p.c.k_scale, page), vs = scale(p.c.v_scale, page);
+            float ref = 0.f;  // V's running power of two
+            for (int j = 0; j < walk.n; ++j, ++tile_count) {
+                const int page2 = entry(j + 2);
+                const float ks1 = scale(p.c.k_scale, page1), vs1 = scale(p.c.v_scale, page1);
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                for (int kv = 0; kv < 2; ++kv, ++item) {
+                    if (item >= kRaw) ok = __all_sync(0xffffffffu, mbar_wait(&s.raw_empty[rs], rphase ^ 1));
+                    if (!ok) break;
+                    if (kv == 0) {
+                        // Scales of the tile, a lane 16 keys.
+                        const float top = __uint_as_float(
+                            __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(finite_or(vs, 0.f)))));
+                        float fall = 1.f;
+                        if (top > 2.f * ref) {
+                            const float to = __int_as_float(min(253, max(13, __float_as_int(top) >> 23)) << 23);
+                            fall = ref / to;
+                            ref = to;
+                        }
+                        const int from = (lane & 7) >> (shift - 4);
+                        const float kg = __shfl_sync(0xffffffffu, ks, from), vg = __shfl_sync(0xffffffffu, vs, from);
+                        const bool fine = fabsf(vg) <= 3.402823466e38f;
+                        TileScales& sc = s.scales[tile_count & (kScaleSlots - 1)];
+                        if (lane < 8) {
+                            sc.k[lane] = fine ? kg : __int_as_float(0x7fffffff);
+                            sc.v[lane] = fine && ref > 0.f ? vg / ref : 0.f;
+                        }
+                        if (lane == 8) {
+                            sc.fall = fall;
+                            sc.ref = ref;
+                        }
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[rs], boxes * box_bytes);
+                    __syncwarp();
+                    if (page >= 0)
+                        tma_load_page(raw + rs * kRawBytes + lane * box_bytes, kv ? &a.vmap : &a.kmap, walk.h, page,
+                                      &s.raw_full[rs]);
+                    if (++rs == kRaw) {
+                        rs = 0;
+                        rphase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                page = page1;
+                page1 = page2;
+                ks = ks1;
+                vs = vs1;
+            }
+            if (!ok || !walk.next(a)) break;
+        }
+        if (!ok)  // do not leave while copies into this CTA's shared memory are in flight
+            for (int i = 1; i <= kRaw && i <= item; ++i) {
+                const int at = rs - i;
+                mbar_wait(&s.raw_full[at < 0 ? at + kRaw : at], at < 0 ? rphase ^ 1 : rphase);
+            }
+    } else {
+        // ============================ rows that see nothing ============================
+        for (int u = blockIdx.x; u < meta.units; u += gridDim.x) {
+            const Unit un = a.units[u];
+            if (un.tiles > 0) continue;
+            const int per_row = p.c.kv_heads * kGroup;
+            for (int i = 0; i < un.n * per_row; ++i)
+                *reinterpret_cast<uint2*>(p.out + (int64_t)(un.row0 + i / per_row) * p.out_row_stride +
+                                          (i % per_row) * p.out_head_stride + 4 * lane) = make_uint2(0u, 0u);
+        }
+    }
+    if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+}
+
+constexpr int kSmemBytes =
+    1024 + 2 * kHalfTileBytes + kConv * kHalfTileBytes + kRaw * kRawBytes + (int)sizeof(Shared);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+
+using Kernel = void (*)(ChunkPagedArgs);
+
+Kernel kernel_for(int code, bool cap, bool bias) {
+    if (code == GQA_CODE_INT8) {
+        if (cap) return bias ? paged_chunk_kernel<0, true, true> : paged_chunk_kernel<0, true, false>;
+        return bias ? paged_chunk_kernel<0, false, true> : paged_chunk_kernel<0, false, false>;
+    }
+    if (cap) return bias ? paged_chunk_kernel<1, true, true> : paged_chunk_kernel<1, true, false>;
+    return bias ? paged_chunk_kernel<1, false, true> : paged_chunk_kernel<1, false, false>;
+}
+
+// Layout behind the counters that the decode keeps; everything here is written by each call.
+struct Regions {
+    size_t starts, units, arrivals, partials, end;
+};
+Regions regions(int batch, int rows, int heads, int sms) {
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    const size_t units = (size_t)rows / kTokens + batch;
+    Regions r;
+    r.starts = kPagedPartialsOffset + 256;  // (Meta first)
+    r.units = r.starts + up((size_t)sms * sizeof(int32_t));
+    r.arrivals = r.units + up(units * sizeof(Unit));
+    r.partials = r.arrivals + up(units * heads * 2 * sizeof(uint32_t));
+    r.end = r.partials + (size_t)sms * 2 * kSlotFloats * sizeof(float);
+    return r;
+}
+
+}  // namespace
+
+int paged_chunk_tile() { return kTile; }
+
+size_t paged_chunk_workspace(int batch, int rows, int heads, int sms) { return regions(batch, rows, heads, sms).end; }
+
+cudaError_t paged_chunk_prepare() {
+    for (int i = 0; i < 8; ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4),
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
+                               const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
+    const Regions r = regions(call.batch, call.rows, call.c.kv_heads, sms);
+    PlanUnitsArgs pl;
+    pl.p = call;
+    pl.meta = reinterpret_cast<Meta*>(ws + kPagedPartialsOffset);
+    pl.units = reinterpret_cast<Unit*>(ws + r.units);
+    pl.starts = reinterpret_cast<int32_t*>(ws + r.starts);
+    pl.arrivals = reinterpret_cast<uint32_t*>(ws + r.arrivals);
+    pl.max_units = call.rows / kTokens + call.batch;
+    pl.ctas = sms;
+    plan_units_kernel<<<1, kPlanThreads, call.batch * sizeof(int32_t), stream>>>(pl);
+    ChunkPagedArgs a;
+    a.kmap = kmap;
+    a.vmap = vmap;
+    a.p = call;
+    a.rope = rope;
+    a.status = reinterpret_cast<uint32_t*>(ws);
+    a.meta = pl.meta;
+    a.units = pl.units;
+    a.starts = pl.starts;
+    a.arrivals = pl.arrivals;
+    a.partials = reinterpret_cast<float*>(ws + r.partials);
+    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, kSmemBytes, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace gqa

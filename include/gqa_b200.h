@@ -561,7 +561,9 @@ int gqa_read_paged(const gqa_paged_cache *cache, const int64_t *slots, int n, vo
  * and prefix_ends (prefix mask: keys below it are visible whatever the query's
  * position; default 0) are per query row, NULL for none.  Keys outside the
  * visible range never influence a result, whatever their codes; a block's NaN
- * scale reaches a row only through a visible key.  Page numbers outside
+ * scale reaches a row only through a visible key.  Scales are not negative, and
+ * visible codes are numbers (gqa_append_paged writes no e4m3 NaN; the value read
+ * for one is unspecified).  Page numbers outside
  * [0, pages) read as zeros, and no key at or past table_width * page_len is visible.
  */
 typedef struct gqa_paged_params {
