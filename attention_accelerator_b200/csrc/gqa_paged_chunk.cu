@@ -52,7 +52,10 @@ constexpr int kRaw = 3;                    // ring slots of codes
 constexpr int kConv = 3;                   // ring slots of FP16
 constexpr int kScaleSlots = 4;             // tiles whose scales are in flight
 constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
-constexpr int kThreads = (kLoadWarp + 2) * 32;
+constexpr int kThreads = 16 * 32;
+// Registers: launched with 128 a thread; each group of four warps takes its share.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 184, kConvRegs = 80, kRestRegs = 56;
+static_assert(2 * kSoftmaxRegs + kConvRegs + kRestRegs <= 4 * kLaunchRegs, "of what the CTA was launched with");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256;  // two of 128 columns each; P over the first 64 of its S
 constexpr float kHeadroom = 8.f;   // log2 by which a maximum may pass the reference
@@ -321,24 +324,12 @@ struct Row {
     int lo, hi, pos;   // visible keys, position
 };
 
-// Scores of 32 keys from key k0 on, in log2 units; masked ones -inf where `edge`.
-template <bool kCap, bool kBias>
-__device__ __forceinline__ void scores(float (&z)[32], const uint32_t (&s)[32], const Row& row, const float* ks,
-                                       int k0, bool edge) {
-    const float f0 = row.factor * ks[0], f1 = row.factor * ks[1];
-    const float ahead = kBias ? (float)(k0 - row.pos) : 0.f;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        float x = __uint_as_float(s[e]) * (e < 16 ? f0 : f1);
-        if constexpr (kCap) x = row.cap2 * tanh_fast(x);
-        if constexpr (kBias) x = fmaf(-row.slope, fabsf(ahead + (float)e), x);
-        z[e] = x;
-    }
-    if (edge) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (k0 + e < row.lo || k0 + e >= row.hi) z[e] = -INFINITY;
-    }
+template <int kRegs>
+__device__ __forceinline__ void take_registers() {
+    if constexpr (kRegs > kLaunchRegs)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+    else
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 template <int kCode, bool kCap, bool kBias>
@@ -391,6 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 
     if (warp < kConvWarp) {
         // ============================ softmax ============================
+        take_registers<kSoftmaxRegs>();
         const int m = warp >> 2, r = tid & (kRowsM - 1);  // M tile, row: query 32 m + r / 4, head r % 4
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + kColS + m * 128 + lanes, t_o = tmem + kColO + m * 128 + lanes;
@@ -491,34 +483,48 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     const TileScales& sc = s.scales[(slot + j) & (kScaleSlots - 1)];
                     const int k0 = (un.tile0 + walk.j + j) << kTileShift;
                     const bool edge = __any_sync(0xffffffffu, row.lo > k0 || row.hi < k0 + kTile);
+                    // The row's 128 scores, in the reference's units once kCap or kBias needs them so.
+                    float z[kTile];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t(&)[32]>(z[32 * c]));
+                    float f[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = row.factor * sc.k[i];
+                    tmem_wait_ld();
+                    if constexpr (kCap || kBias) {
+                        const float ahead = (float)(k0 - row.pos);
+#pragma unroll
+                        for (int e = 0; e < kTile; ++e) {
+                            z[e] *= f[e >> 4];
+                            if constexpr (kCap) z[e] = row.cap2 * tanh_fast(z[e]);
+                            if constexpr (kBias) z[e] = fmaf(-row.slope, fabsf(ahead + (float)e), z[e]);
+                        }
+                    }
+                    if (edge) {
+                        if constexpr (!kCap && !kBias) {  // scaled before the mask: -inf times a scale of 0 is none
+#pragma unroll
+                            for (int e = 0; e < kTile; ++e) z[e] *= f[e >> 4];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) f[i] = 1.f;
+                        }
+                        // Visible keys of the tile as bits: from row.lo - k0 on, below row.hi - k0.
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int from = min(32, max(0, row.lo - k0 - 32 * c)), to = min(32, max(0, row.hi - k0 - 32 * c));
+                            const uint32_t seen_bits = __funnelshift_lc(0xffffffffu, 0u, to) & ~__funnelshift_lc(0xffffffffu, 0u, from);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(seen_bits & (1u << e))) z[32 * c + e] = -INFINITY;
+                        }
+                    }
                     float mx = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(t_s + 32 * c, v);
-                        tmem_wait_ld();
-                        if constexpr (kBias) {
-                            float z[32];
-                            scores<kCap, kBias>(z, v, row, sc.k + 2 * c, k0 + 32 * c, edge);
+                    for (int i = 0; i < 8; ++i) {
+                        // The largest of 16 keys, then their scale: it is not negative.
+                        float top = fmaxf(z[16 * i], z[16 * i + 1]);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, z[e]);
-                        } else {
-                            // The largest S of 16 keys, then their scale: it is not negative, and neither is the cap.
-                            if (edge) {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (k0 + 32 * c + e < row.lo || k0 + 32 * c + e >= row.hi) v[e] = 0xff800000u;
-                            }
-#pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                float top = __uint_as_float(v[16 * half]);
-#pragma unroll
-                                for (int e = 1; e < 16; ++e) top = fmaxf(top, __uint_as_float(v[16 * half + e]));
-                                float z = top * (row.factor * sc.k[2 * c + half]);
-                                if constexpr (kCap) z = top == -INFINITY ? top : row.cap2 * tanh_fast(z);
-                                mx = fmaxf(mx, z);
-                            }
-                        }
+                        for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(top, z[16 * i + e]), z[16 * i + e + 1]);
+                        mx = fmaxf(mx, kCap || kBias ? top : top * f[i]);
                     }
                     // The reference moves when the maximum passes it by 2^kHeadroom (at once from nothing).
                     const float want = mx - kLift;
@@ -544,42 +550,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     }
                     vref = sc.ref;
                     const float use = ref == -INFINITY ? 0.f : ref;
-                    float sum0 = 0.f, sum1 = 0.f;
+                    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32], w[16];
-                        tmem_ld32(t_s + 32 * c, v);
-                        tmem_wait_ld();
-                        if constexpr (kCap || kBias) {
-                            float z[32];
-                            scores<kCap, kBias>(z, v, row, sc.k + 2 * c, k0 + 32 * c, edge);
+                        uint32_t w[16];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const float p0 = fast_exp2(z[e] - use), p1 = fast_exp2(z[e + 1] - use);
-                                sum0 += p0;
-                                sum1 += p1;
-                                w[e >> 1] = pack_half2(p0, p1);
+                        for (int e = 0; e < 32; e += 2) {
+                            float2 x = make_float2(z[32 * c + e], z[32 * c + e + 1]);
+                            const float2 less = make_float2(-use, -use);
+                            if constexpr (kCap || kBias) {
+                                x = __fadd2_rn(x, less);
+                            } else {
+                                const float g = f[2 * c + (e >> 4)];
+                                x = __ffma2_rn(x, make_float2(g, g), less);
                             }
-                        } else {
-                            const float f0 = row.factor * sc.k[2 * c], f1 = row.factor * sc.k[2 * c + 1];
-#pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const float f = e < 16 ? f0 : f1;
-                                float p0 = fast_exp2(fmaf(__uint_as_float(v[e]), f, -use));
-                                float p1 = fast_exp2(fmaf(__uint_as_float(v[e + 1]), f, -use));
-                                if (edge) {
-                                    const int key = k0 + 32 * c + e;
-                                    if (key < row.lo || key >= row.hi) p0 = 0.f;
-                                    if (key + 1 < row.lo || key + 1 >= row.hi) p1 = 0.f;
-                                }
-                                sum0 += p0;
-                                sum1 += p1;
-                                w[e >> 1] = pack_half2(p0, p1);
-                            }
+                            x = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                            sum = __fadd2_rn(sum, x);
+                            w[e >> 1] = pack_half2(x.x, x.y);
                         }
                         tmem_st16(t_s + 16 * c, w);  // over columns that were read
                     }
-                    l += sum0 + sum1;
+                    l += sum.x + sum.y;
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&s.p_full[m]);
@@ -694,6 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         }
     } else if (warp < kMmaWarp) {
         // ============================ conversion ============================
+        take_registers<kConvRegs>();
         const int cw = warp - kConvWarp, t = lane & 3;
         const int row0 = 32 * cw + (lane >> 2);  // this lane's rows: row0 + 8 i
         int item = 0;  // K and V of the tiles in turn
@@ -752,7 +744,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             }
             if (!ok || !walk.next(a)) break;
         }
-    } else if (warp == kMmaWarp) {
+    } else {
+    take_registers<kRestRegs>();
+    if (warp == kMmaWarp) {
         // ============================ MMA issuer ============================
         if (lane == 0) {
             int cs = 0, cphase = 0;   // next slot of FP16
@@ -764,12 +758,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 }
             };
             auto issue_s = [&](int m, int slot) {
-                const uint32_t kaddr = smem_addr(conv + slot * kHalfTileBytes), qaddr = smem_addr(q_smem + m * kHalfTileBytes);
-#pragma unroll
+                const uint64_t kd = smem_desc_sw128(smem_addr(conv + slot * kHalfTileBytes), 16, 1024);
+                const uint64_t qd = smem_desc_sw128(smem_addr(q_smem + m * kHalfTileBytes), 16, 1024);
+#pragma unroll 1
                 for (int kk = 0; kk < 8; ++kk) {
-                    const uint32_t off = (kk >> 2) * kBlockBytes + (kk & 3) * 32;
-                    mma_ss(tmem + kColS + m * 128, smem_desc_sw128(qaddr + off, 16, 1024),
-                           smem_desc_sw128(kaddr + off, 16, 1024), kIdescS, kk != 0);
+                    const uint32_t off = ((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;  // (in units of 16 bytes)
+                    mma_ss(tmem + kColS + m * 128, qd + off, kd + off, kIdescS, kk != 0);
                 }
                 tc_commit(&s.s_full[m]);
             };
@@ -796,12 +790,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         if (!ok) break;
                         ++seen[m];
                         tc_fence_after();
-                        const uint32_t vaddr = smem_addr(conv + vs * kHalfTileBytes);
-#pragma unroll
+                        const uint64_t vd = smem_desc_sw128(smem_addr(conv + vs * kHalfTileBytes), kBlockBytes, 1024);
+#pragma unroll 1
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ts(tmem + kColO + m * 128, tmem + kColS + m * 128 + 8 * kk,
-                                   smem_desc_sw128(vaddr + kk * 16 * 128, kBlockBytes, 1024), kIdescO,
-                                   (j > 0 || kk > 0) ? 1u : 0u);
+                            mma_ts(tmem + kColO + m * 128, tmem + kColS + m * 128 + 8 * kk, vd + kk * (16 * 128 >> 4),
+                                   kIdescO, (j > 0 || kk > 0) ? 1u : 0u);
                         if (m == ms - 1) tc_commit(&s.conv_empty[vs]);
                         if (more) {
                             if (m == 0) ok = mbar_wait(&s.conv_full[ks], kphase);
@@ -894,7 +887,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 const int at = rs - i;
                 mbar_wait(&s.raw_full[at < 0 ? at + kRaw : at], at < 0 ? rphase ^ 1 : rphase);
             }
-    } else {
+    } else if (warp == kLoadWarp + 1) {
         // ============================ rows that see nothing ============================
         for (int u = blockIdx.x; u < meta.units; u += gridDim.x) {
             const Unit un = a.units[u];
@@ -904,6 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 *reinterpret_cast<uint2*>(p.out + (int64_t)(un.row0 + i / per_row) * p.out_row_stride +
                                           (i % per_row) * p.out_head_stride + 4 * lane) = make_uint2(0u, 0u);
         }
+    }
     }
     if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
 
@@ -954,7 +948,12 @@ size_t paged_chunk_workspace(int batch, int rows, int heads, int sms) { return r
 
 cudaError_t paged_chunk_prepare() {
     for (int i = 0; i < 8; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4),
+        // The register shares are of kLaunchRegs a thread: with fewer at launch the kernel would wait for good.
+        cudaFuncAttributes at;
+        cudaError_t e = cudaFuncGetAttributes(&at, kernel_for(i & 1, i & 2, i & 4));
+        if (e != cudaSuccess) return e;
+        if (at.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+        e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4),
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
         if (e != cudaSuccess) return e;
     }
