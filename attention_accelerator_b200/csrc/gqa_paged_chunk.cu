@@ -748,7 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     take_registers<kRestRegs>();
     if (warp == kMmaWarp) {
         // ============================ MMA issuer ============================
-        if (lane == 0) {
+        {
+            const uint32_t leader = elect_lane();  // (the waits and the walk are the whole warp's)
             int cs = 0, cphase = 0;   // next slot of FP16
             int seen[2] = {0, 0}, pieces[2] = {0, 0};
             auto advance = [&] {
@@ -757,59 +758,60 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     cphase ^= 1;
                 }
             };
+            const uint32_t cols = uniform(tmem);
             auto issue_s = [&](int m, int slot) {
                 const uint64_t kd = smem_desc_sw128(smem_addr(conv + slot * kHalfTileBytes), 16, 1024);
                 const uint64_t qd = smem_desc_sw128(smem_addr(q_smem + m * kHalfTileBytes), 16, 1024);
-#pragma unroll 1
+#pragma unroll
                 for (int kk = 0; kk < 8; ++kk) {
                     const uint32_t off = ((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;  // (in units of 16 bytes)
-                    mma_ss(tmem + kColS + m * 128, qd + off, kd + off, kIdescS, kk != 0);
+                    mma_ss_by(leader, cols + kColS + m * 128, qd + off, kd + off, kIdescS, kk != 0);
                 }
-                tc_commit(&s.s_full[m]);
+                tc_commit_by(leader, &s.s_full[m]);
             };
-            while (walk.n > 0 && ok) {
-                const int ms = walk.unit.n > 32 ? 2 : 1;
+            while (uniform(walk.n) > 0 && ok) {
+                const int ms = uniform(walk.unit.n) > 32 ? 2 : 1, n = uniform(walk.n);
                 // S of the first tile.
-                ok = mbar_wait(&s.conv_full[cs], cphase);
+                ok = warp_wait(&s.conv_full[cs], cphase);
                 for (int m = 0; m < ms && ok; ++m) {
-                    ok = mbar_wait(&s.q_full[m], pieces[m] & 1);
+                    ok = warp_wait(&s.q_full[m], pieces[m] & 1);
                     if (!ok) break;
                     tc_fence_after();
                     issue_s(m, cs);
                 }
                 if (!ok) break;
-                tc_commit(&s.conv_empty[cs]);
+                tc_commit_by(leader, &s.conv_empty[cs]);
                 advance();
-                for (int j = 0; j < walk.n && ok; ++j) {
+                for (int j = 0; j < n && ok; ++j) {
                     const int vs = cs, vphase = cphase;
                     advance();
-                    const bool more = j + 1 < walk.n;
+                    const bool more = j + 1 < n;
                     const int ks = cs, kphase = cphase;
                     for (int m = 0; m < ms; ++m) {
-                        ok = mbar_wait(&s.p_full[m], seen[m] & 1) && (m || mbar_wait(&s.conv_full[vs], vphase));
+                        ok = warp_wait(&s.p_full[m], seen[m] & 1) && (m || warp_wait(&s.conv_full[vs], vphase));
                         if (!ok) break;
                         ++seen[m];
                         tc_fence_after();
                         const uint64_t vd = smem_desc_sw128(smem_addr(conv + vs * kHalfTileBytes), kBlockBytes, 1024);
-#pragma unroll 1
+#pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ts(tmem + kColO + m * 128, tmem + kColS + m * 128 + 8 * kk, vd + kk * (16 * 128 >> 4),
+                            mma_ts_by(leader, cols + kColO + m * 128, cols + kColS + m * 128 + 8 * kk, vd + kk * (16 * 128 >> 4),
                                    kIdescO, (j > 0 || kk > 0) ? 1u : 0u);
-                        if (m == ms - 1) tc_commit(&s.conv_empty[vs]);
+                        if (m == ms - 1) tc_commit_by(leader, &s.conv_empty[vs]);
                         if (more) {
-                            if (m == 0) ok = mbar_wait(&s.conv_full[ks], kphase);
+                            if (m == 0) ok = warp_wait(&s.conv_full[ks], kphase);
                             if (!ok) break;
                             tc_fence_after();
                             issue_s(m, ks);
-                            if (m == ms - 1) tc_commit(&s.conv_empty[ks]);
+                            if (m == ms - 1) tc_commit_by(leader, &s.conv_empty[ks]);
                         } else {
-                            tc_commit(&s.pv_done[m]);
+                            tc_commit_by(leader, &s.pv_done[m]);
                         }
                     }
                     if (more) advance();
                 }
                 for (int m = 0; m < ms; ++m) ++pieces[m];
-                if (!ok || !walk.next(a)) break;
+                if (!ok || !uniform(walk.next(a))) break;
             }
         }
     } else if (warp == kLoadWarp) {

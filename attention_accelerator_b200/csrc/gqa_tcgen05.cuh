@@ -100,6 +100,46 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t adesc, uint64_t bdes
         : "memory");
 }
 
+// The same instructions issued by one lane of a warp that runs together: the
+// operands stay warp-uniform, so that they are computed in uniform registers
+// (inside a branch of one lane each costs a move to them, and the issue of an
+// MMA takes twice its 64 cycles).
+// `x`, which every lane holds, known to the compiler to be the same in all.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void mma_ss_by(uint32_t leader, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, l;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 l, %5, 0;\n\t"
+        "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts_by(uint32_t leader, uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, l;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 l, %5, 0;\n\t"
+        "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_by(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred l;\n\t"
+        "setp.ne.b32 l, %1, 0;\n\t"
+        "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(leader)
+        : "memory");
+}
+
 // Bounded wait with one outcome for the whole warp, so that the warp-wide
 // tcgen05.ld / tcgen05.st that follow are never reached by part of it.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
