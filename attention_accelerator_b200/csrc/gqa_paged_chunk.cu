@@ -90,6 +90,7 @@ struct alignas(16) Shared {
     uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], group[2];
     uint64_t pad;
     TileScales scales[kScaleSlots];
+    uint64_t step[kPairs];  // turns per position of each pair
     uint32_t tmem;
     int last[2];
 };
@@ -316,6 +317,17 @@ __device__ __forceinline__ float finite_or(float x, float other) {
     return fabsf(x) <= 3.402823466e38f ? x : other;
 }
 
+// rope_factor from the top 32 bits of the phase: 2^-32 turns, a 128th of what FP32 leaves of it.
+__device__ __forceinline__ float2 rope_factor_fast(uint64_t step, int64_t pos) {
+    const int turns = (int)((step * (uint64_t)pos) >> 32);
+    float sn, cs;
+    sincospif(__int2float_rn(turns) * 0x1p-31f, &sn, &cs);
+    return make_float2(cs, sn);
+}
+
+// The larger magnitude of two BF16 codes, as FP32 bits (which order as integers).
+__device__ __forceinline__ uint32_t magnitudes(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
+
 // The row of a softmax thread.
 struct Row {
     float factor;      // scores of the row: S * page scale * factor, in log2 units (or over the cap)
@@ -361,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         }
         fence_barrier_init();
     }
+    if (tid < kPairs) s.step[tid] = a.rope.step[tid];
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s.tmem)),
                      "r"(kTmemCols)
@@ -391,6 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         int pieces = 0;   // of this M tile (phases of pv_done)
         int syncs = 0;    // phases of group
         int slot = 0;     // scales of the piece's first tile
+        int row_unit = -1;
+        Row row;
+        row.cap2 = p.cap * 1.4426950408889634f;
         auto group_sync = [&] {
             mbar_arrive(&s.group[m]);
             if (ok) ok = mbar_wait(&s.group[m], syncs & 1);
@@ -401,72 +417,71 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             const int token = 32 * m + (r >> 2), head = r & 3;
             const bool active = un.n > 32 * m, real = token < un.n;
             if (active && ok) {
-                Row row;
                 const int64_t pos = (int64_t)un.pos0 + token;
-                row.pos = (int)pos;
-                row.lo = 0;
-                row.hi = 0x7fffffff;  // rows of no query: nothing to mask, nothing written
-                if (real) {
-                    const KeyRange range = paged_range(p, un.row0 + token, pos, paged_length(p, un.b));
-                    row.lo = range.lo;
-                    row.hi = range.hi;
+                if (walk.u != row_unit) {  // (the heads of a unit follow one another)
+                    row_unit = walk.u;
+                    row.pos = (int)pos;
+                    row.lo = 0;
+                    row.hi = 0x7fffffff;  // rows of no query: nothing to mask, nothing written
+                    if (real) {
+                        const KeyRange range = paged_range(p, un.row0 + token, pos, paged_length(p, un.b));
+                        row.lo = range.lo;
+                        row.hi = range.hi;
+                    }
                 }
-                row.cap2 = p.cap * 1.4426950408889634f;
                 row.slope = kBias ? p.slopes[walk.h * kGroup + head] * 1.4426950408889634f : 0.f;
                 row.factor = 0.f;
                 // ---- Q: 16 pairs of this lane's query, 4 heads ----
                 {
-                    float2 f[16];
-                    const int pair0 = 16 * (lane & 3);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        f[i] = p.q_rotated || !real ? make_float2(1.f, 0.f) : rope_factor(a.rope.step[pair0 + i], pos);
+                    const int q4 = lane & 3;
                     const float unit = kCap ? p.scale / p.cap : p.scale * 1.4426950408889634f;
-#pragma unroll 1
+                    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+                    const uint4* q = reinterpret_cast<const uint4*>(
+                        p.q + (int64_t)(un.row0 + token) * p.q_row_stride + walk.h * kGroup * p.q_head_stride + 16 * q4);
+                    uint4 w[kGroup][4];  // pairs 0-7 and 8-15: first, then second elements
+#pragma unroll
+                    for (int hq = 0; hq < kGroup; ++hq)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[hq][i] = real ? q[hq * (p.q_head_stride / 8) + (i & 1) + 8 * (i >> 1)] : none;
+                    float down[kGroup];
+#pragma unroll
                     for (int hq = 0; hq < kGroup; ++hq) {
-                        uint32_t xw[8], yw[8];
+                        // A power of two above the row's largest: a rotated pair passes it by no more than sqrt(2).
+                        uint32_t top = 0;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) xw[i] = yw[i] = 0u;
-                        if (real) {
-                            const uint4* q = reinterpret_cast<const uint4*>(
-                                p.q + (int64_t)(un.row0 + token) * p.q_row_stride +
-                                (walk.h * kGroup + hq) * p.q_head_stride + pair0);
-                            const uint4 x0 = q[0], x1 = q[1], y0 = q[8], y1 = q[9];
-                            xw[0] = x0.x; xw[1] = x0.y; xw[2] = x0.z; xw[3] = x0.w;
-                            xw[4] = x1.x; xw[5] = x1.y; xw[6] = x1.z; xw[7] = x1.w;
-                            yw[0] = y0.x; yw[1] = y0.y; yw[2] = y0.z; yw[3] = y0.w;
-                            yw[4] = y1.x; yw[5] = y1.y; yw[6] = y1.z; yw[7] = y1.w;
-                        }
-                        float x[16], y[16], most = 0.f;
-                        bool fine = true;
+                        for (int i = 0; i < 4; ++i)
+                            top = max(top, max(max(magnitudes(w[hq][i].x), magnitudes(w[hq][i].y)),
+                                               max(magnitudes(w[hq][i].z), magnitudes(w[hq][i].w))));
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const int e = min(253, max(1, (int)(top >> 23) + 1));
+                        if (hq == head)
+                            row.factor = top < 0x7f800000u ? unit * __int_as_float(e << 23) : __int_as_float(0x7fffffff);
+                        down[hq] = __int_as_float((254 - e) << 23);
+                    }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 xv = bf16x2_to_float2(xw[i >> 1]), yv = bf16x2_to_float2(yw[i >> 1]);
-                            const float re = i & 1 ? xv.y : xv.x, im = i & 1 ? yv.y : yv.x;
-                            x[i] = re * f[i].x - im * f[i].y;
-                            y[i] = re * f[i].y + im * f[i].x;
-                            fine &= fabsf(x[i]) <= 3.402823466e38f && fabsf(y[i]) <= 3.402823466e38f;
-                            most = fmaxf(most, fmaxf(fabsf(x[i]), fabsf(y[i])));
-                        }
-                        if (!fine) most = INFINITY;
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                        const int e = min(253, max(1, (__float_as_int(most) >> 23) + 1));
-                        const float up = __int_as_float(e << 23), down = __int_as_float((254 - e) << 23);
-                        if (hq == head) row.factor = most == INFINITY ? __int_as_float(0x7fffffff) : unit * up;
-                        const int qr = (r & ~3) + hq;  // row of the M tile
+                    for (int c = 0; c < 2; ++c) {  // 8 pairs: 16 bytes of each block
+                        float2 f[8];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            uint32_t w[8];
+                        for (int i = 0; i < 8; ++i)
+                            f[i] = p.q_rotated ? make_float2(1.f, 0.f) : rope_factor_fast(s.step[16 * q4 + 8 * c + i], pos);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                w[i] = half ? pack_half2(y[2 * i] * down, y[2 * i + 1] * down)
-                                            : pack_half2(x[2 * i] * down, x[2 * i + 1] * down);
-                            uint8_t* at = q_tile + half * kBlockBytes + qr * 128;
-                            const int c = 2 * (lane & 3);
-                            *reinterpret_cast<uint4*>(at + ((c ^ (qr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4*>(at + (((c + 1) ^ (qr & 7)) << 4)) =
-                                make_uint4(w[4], w[5], w[6], w[7]);
+                        for (int hq = 0; hq < kGroup; ++hq) {
+                            const uint4 u4 = w[hq][c], v4 = w[hq][c + 2];
+                            const uint32_t uw[4] = {u4.x, u4.y, u4.z, u4.w}, vw[4] = {v4.x, v4.y, v4.z, v4.w};
+                            uint32_t x[4], y[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 u = bf16x2_to_float2(uw[i]), v = bf16x2_to_float2(vw[i]);
+                                const float2 f0 = f[2 * i], f1 = f[2 * i + 1];
+                                x[i] = pack_half2((u.x * f0.x - v.x * f0.y) * down[hq], (u.y * f1.x - v.y * f1.y) * down[hq]);
+                                y[i] = pack_half2((u.x * f0.y + v.x * f0.x) * down[hq], (u.y * f1.y + v.y * f1.x) * down[hq]);
+                            }
+                            const int qr = (r & ~3) + hq;  // row of the M tile
+                            uint8_t* to = q_tile + qr * 128 + (((2 * q4 + c) ^ (qr & 7)) << 4);
+                            *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+                            *reinterpret_cast<uint4*>(to + kBlockBytes) = make_uint4(y[0], y[1], y[2], y[3]);
                         }
                     }
                     fence_proxy_async_smem();
@@ -595,16 +610,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 };
                 if (walk.n == un.tiles) {
                     const float f = l == 0.f ? 0.f : vref / l;  // a row that sees nothing is 0
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        float x[32];
-                        tmem_ld32(t_o + 32 * c, o);
-                        tmem_wait_ld();
+                    float x[kHeadDim];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * f;
-                        if (real) write(c, x);
-                    }
+                    for (int c = 0; c < 4; ++c) tmem_ld32(t_o + 32 * c, reinterpret_cast<uint32_t(&)[32]>(x[32 * c]));
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < kHeadDim; ++e) x[e] *= f;
+                    if (real)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) write(c, reinterpret_cast<const float(&)[32]>(x[32 * c]));
                 } else {
                     // A piece of a unit: its slots as in decode_paged (a share's first piece 0, its last 1).
                     const int64_t G = meta.ctas, total = meta.total, first = walk.unit_first(a);
@@ -617,18 +631,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     const int prow = m * kRowsM + r;
                     {
                         float* mine = part((int)blockIdx.x - c0);
-#pragma unroll 1
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + 32 * c, o);
-                            tmem_wait_ld();
-                            if (real)
+                        float x[kHeadDim];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    reinterpret_cast<float4*>(mine)[(8 * c + e) * 2 * kRowsM + prow] = make_float4(
-                                        __uint_as_float(o[4 * e]) * vref, __uint_as_float(o[4 * e + 1]) * vref,
-                                        __uint_as_float(o[4 * e + 2]) * vref, __uint_as_float(o[4 * e + 3]) * vref);
-                        }
+                        for (int c = 0; c < 4; ++c) tmem_ld32(t_o + 32 * c, reinterpret_cast<uint32_t(&)[32]>(x[32 * c]));
+                        tmem_wait_ld();
+                        if (real)
+#pragma unroll
+                            for (int e = 0; e < kHeadDim / 4; ++e)
+                                reinterpret_cast<float4*>(mine)[e * 2 * kRowsM + prow] =
+                                    make_float4(x[4 * e] * vref, x[4 * e + 1] * vref, x[4 * e + 2] * vref, x[4 * e + 3] * vref);
                         if (real)
                             reinterpret_cast<float2*>(mine + 2 * kRowsM * kHeadDim)[prow] = make_float2(ref, l);
                     }
