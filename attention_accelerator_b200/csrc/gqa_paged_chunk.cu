@@ -6,7 +6,7 @@
 // rows sees, in tiles of 128 on a grid of absolute positions.  plan_units_kernel
 // (one CTA) finds every unit's keys from the lengths and masks in device memory,
 // sums the tiles, and says where each CTA of paged_chunk_kernel begins: all tiles
-// of all units in order are dealt out evenly, as decode_paged does, so that causal
+// of all units in order are dealt out at even cost, so that causal
 // prompts, ragged batches and one long context alike fill the GPU.  A unit that
 // crosses shares leaves FP32 partial rows; its last CTA merges them in order.
 //
@@ -78,6 +78,10 @@ struct Meta {
     int32_t ctas;   // with a share
     int32_t units;
 };
+// What a unit costs a CTA beside its tiles (queries, the pipeline's start and
+// end, its rows), in tiles: measured at 25-28 thousand cycles to a tile's 5.
+constexpr int kUnitCost = 5;
+constexpr int kMaxCtas = 255;
 
 struct TileScales {
     float k[8], v[8];   // of each 16 keys: K's scale (NaN where V's is no number), V's over the reference
@@ -91,6 +95,7 @@ struct alignas(16) Shared {
     uint64_t pad;
     TileScales scales[kScaleSlots];
     uint64_t step[kPairs];  // turns per position of each pair
+    int64_t cuts[kMaxCtas + 1];
     uint32_t tmem;
     int last[2];
 };
@@ -103,6 +108,7 @@ struct alignas(64) ChunkPagedArgs {
     const Meta* meta;
     const Unit* units;
     const int32_t* starts;  // [ctas] unit in which each share begins
+    const int64_t* cuts;    // [ctas + 1] tiles (of all units and heads, in order) where the shares begin
     uint32_t* arrivals;     // [units][heads][2]
     float* partials;        // [ctas][2][kSlotFloats]
 };
@@ -112,6 +118,7 @@ struct PlanUnitsArgs {
     Meta* meta;
     Unit* units;
     int32_t* starts;
+    int64_t* cuts;
     uint32_t* arrivals;
     int32_t max_units, ctas;
 };
@@ -208,21 +215,35 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     const int heads = p.c.kv_heads;
     const int uper = (units + kPlanThreads - 1) / kPlanThreads;
     const int u0 = min(units, tid * uper), u1 = min(units, u0 + uper);
+    // Shares are cut evenly in cost: a unit's cells are kUnitCost of its own, then one for each tile.
     sum = 0;
-    for (int u = u0; u < u1; ++u) sum += a.units[u].tiles;
+    int64_t cells = 0, cost = 0;
+    for (int u = u0; u < u1; ++u) {
+        const int tiles = a.units[u].tiles;
+        sum += tiles;
+        cells += tiles ? tiles + kUnitCost : 0;
+    }
     at = scan_exclusive(sum, warp_sum, &total);
+    int64_t cell = scan_exclusive(cells, warp_sum, &cost);
     total *= heads;
-    const int64_t G = min((int64_t)a.ctas, total);
+    cost *= heads;
+    // Shares longer than kUnitCost: each has a tile.
+    const int64_t G = min((int64_t)a.ctas, cost / (kUnitCost + 1));
     for (int u = u0; u < u1; ++u) {
         const int tiles = a.units[u].tiles;
         a.units[u].first = at;
-        // Shares i begin at tile total * i / G: those that begin in this unit.
-        const int64_t begin = at * heads, end = (at + tiles) * heads;
-        if (tiles > 0)
-            for (int64_t i = (begin * G + total - 1) / total; i < G && total * i / G < end; ++i)
-                if (total * i / G >= begin) a.starts[i] = u;
+        if (tiles > 0) {
+            const int64_t begin = cell * heads, each = tiles + kUnitCost, end = begin + each * heads;
+            for (int64_t i = (begin * G + cost - 1) / cost; i < G && cost * i / G < end; ++i) {
+                const int64_t off = cost * i / G - begin, h = off / each, t = off - h * each - kUnitCost;
+                a.starts[i] = u;
+                a.cuts[i] = at * heads + h * tiles + (t > 0 ? t : 0);
+            }
+            cell += each;
+        }
         at += tiles;
     }
+    if (tid == 0) a.cuts[G] = total;
     for (int i = tid; i < units * heads * 2; i += kPlanThreads) a.arrivals[i] = 0;
     if (tid == 0) *a.meta = Meta{total, (int32_t)G, units};
 }
@@ -236,10 +257,10 @@ struct Walk {
     Unit unit;
     __device__ __forceinline__ void start(const ChunkPagedArgs& a, const Meta& meta) {
         n = 0;
-        const int64_t me = blockIdx.x, G = meta.ctas;
-        if (me >= G) return;
-        x = meta.total * me / G;
-        end = meta.total * (me + 1) / G;
+        const int me = blockIdx.x;
+        if (me >= meta.ctas) return;
+        x = a.cuts[me];
+        end = a.cuts[me + 1];
         u = a.starts[me];
         unit = a.units[u];
         const int64_t rem = x - unit.first * a.p.c.kv_heads;
@@ -373,7 +394,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         }
         fence_barrier_init();
     }
+    const Meta meta = *a.meta;
     if (tid < kPairs) s.step[tid] = a.rope.step[tid];
+    if (tid <= meta.ctas) s.cuts[tid] = a.cuts[tid];
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s.tmem)),
                      "r"(kTmemCols)
@@ -388,7 +411,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    const Meta meta = *a.meta;
     Walk walk;
     walk.start(a, meta);
     bool ok = true;
@@ -621,10 +643,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         for (int c = 0; c < 4; ++c) write(c, reinterpret_cast<const float(&)[32]>(x[32 * c]));
                 } else {
                     // A piece of a unit: its slots as in decode_paged (a share's first piece 0, its last 1).
-                    const int64_t G = meta.ctas, total = meta.total, first = walk.unit_first(a);
-                    const int c0 = (int)(((first + 1) * G + total - 1) / total) - 1;
-                    const int parts = (int)(((first + un.tiles) * G + total - 1) / total) - c0;
-                    const int second = total * c0 / G < first ? 1 : 0;
+                    const int64_t first = walk.unit_first(a);
+                    auto share_of = [&](int64_t tile) {  // the last cut at or before it
+                        int lo = 0, hi = meta.ctas;
+                        while (hi - lo > 1) {
+                            const int mid = (lo + hi) >> 1;
+                            if (s.cuts[mid] <= tile) lo = mid; else hi = mid;
+                        }
+                        return lo;
+                    };
+                    const int c0 = share_of(first), parts = share_of(first + un.tiles - 1) - c0 + 1;
+                    const int second = s.cuts[c0] < first ? 1 : 0;
                     auto part = [&](int c) {
                         return a.partials + (int64_t)((c0 + c) * 2 + (c ? 0 : second)) * kSlotFloats;
                     };
@@ -939,14 +968,15 @@ Kernel kernel_for(int code, bool cap, bool bias) {
 
 // Layout behind the counters that the decode keeps; everything here is written by each call.
 struct Regions {
-    size_t starts, units, arrivals, partials, end;
+    size_t starts, cuts, units, arrivals, partials, end;
 };
 Regions regions(int batch, int rows, int heads, int sms) {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     const size_t units = (size_t)rows / kTokens + batch;
     Regions r;
     r.starts = kPagedPartialsOffset + 256;  // (Meta first)
-    r.units = r.starts + up((size_t)sms * sizeof(int32_t));
+    r.cuts = r.starts + up((size_t)sms * sizeof(int32_t));
+    r.units = r.cuts + up((size_t)(sms + 1) * sizeof(int64_t));
     r.arrivals = r.units + up(units * sizeof(Unit));
     r.partials = r.arrivals + up(units * heads * 2 * sizeof(uint32_t));
     r.end = r.partials + (size_t)sms * 2 * kSlotFloats * sizeof(float);
@@ -975,12 +1005,14 @@ cudaError_t paged_chunk_prepare() {
 
 cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
                                const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
+    if (sms > kMaxCtas) sms = kMaxCtas;
     const Regions r = regions(call.batch, call.rows, call.c.kv_heads, sms);
     PlanUnitsArgs pl;
     pl.p = call;
     pl.meta = reinterpret_cast<Meta*>(ws + kPagedPartialsOffset);
     pl.units = reinterpret_cast<Unit*>(ws + r.units);
     pl.starts = reinterpret_cast<int32_t*>(ws + r.starts);
+    pl.cuts = reinterpret_cast<int64_t*>(ws + r.cuts);
     pl.arrivals = reinterpret_cast<uint32_t*>(ws + r.arrivals);
     pl.max_units = call.rows / kTokens + call.batch;
     pl.ctas = sms;
@@ -994,6 +1026,7 @@ cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int
     a.meta = pl.meta;
     a.units = pl.units;
     a.starts = pl.starts;
+    a.cuts = pl.cuts;
     a.arrivals = pl.arrivals;
     a.partials = reinterpret_cast<float*>(ws + r.partials);
     kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, kSmemBytes, stream>>>(a);
