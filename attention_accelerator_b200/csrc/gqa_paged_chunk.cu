@@ -70,8 +70,7 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);  // B (V) MN-major
 struct Unit {
     int32_t b, row0, n, pos0;     // sequence, first query row, queries, position of the first
     int32_t lo, hi, tiles, tile0; // keys that any row sees, their tiles
-    int64_t first;                // tiles of all units before it (per head)
-    int64_t pad;
+    int64_t first, cell;          // tiles and cost of all units before it (per head)
 };
 struct Meta {
     int64_t total;  // tiles of all units and heads
@@ -128,30 +127,41 @@ struct PlanUnitsArgs {
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
-// Exclusive running sum over the CTA of one value a thread; *all gets the total.
-__device__ __forceinline__ int64_t scan_exclusive(int64_t v, int64_t* warp_sum, int64_t* all) {
+// Exclusive running sums over the CTA of two values a thread; `all` gets the totals.
+__device__ __forceinline__ longlong2 scan_exclusive(longlong2 v, longlong2* warp_sum, longlong2* all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t incl = v;
+    longlong2 incl = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += x;
+        const long long x = __shfl_up_sync(0xffffffffu, incl.x, d), y = __shfl_up_sync(0xffffffffu, incl.y, d);
+        if (lane >= d) {
+            incl.x += x;
+            incl.y += y;
+        }
     }
     __syncthreads();
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    int64_t base = 0, total = 0;
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-        if (w < warp) base += warp_sum[w];
-        total += warp_sum[w];
+    longlong2 mine = warp_sum[lane], base = make_longlong2(0, 0);
+    *all = mine;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        all->x += __shfl_xor_sync(0xffffffffu, all->x, d);
+        all->y += __shfl_xor_sync(0xffffffffu, all->y, d);
     }
-    *all = total;
-    return base + incl - v;
+    if (lane >= warp) mine = make_longlong2(0, 0);
+    base = mine;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        base.x += __shfl_xor_sync(0xffffffffu, base.x, d);
+        base.y += __shfl_xor_sync(0xffffffffu, base.y, d);
+    }
+    return make_longlong2(base.x + incl.x - v.x, base.y + incl.y - v.y);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_constant__ PlanUnitsArgs a) {
     extern __shared__ int32_t offset[];  // first unit of each sequence
-    __shared__ int64_t warp_sum[kPlanThreads / 32];
+    __shared__ longlong2 warp_sum[kPlanThreads / 32];
     const PagedCall& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, batch = p.batch;
     // Rows of sequence b, kept within the call's whatever the device's numbers say.
@@ -161,18 +171,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     };
     const int per = (batch + kPlanThreads - 1) / kPlanThreads;
     const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
-    int64_t sum = 0, total = 0;
+    longlong2 sum = make_longlong2(0, 0), all;
     for (int b = b0; b < b1; ++b) {
         int row0;
-        sum += (rows_of(b, row0) + kTokens - 1) / kTokens;
+        sum.x += (rows_of(b, row0) + kTokens - 1) / kTokens;
     }
-    int64_t at = scan_exclusive(sum, warp_sum, &total);
+    int64_t at = scan_exclusive(sum, warp_sum, &all).x;
     for (int b = b0; b < b1; ++b) {
         int row0;
         offset[b] = (int)at;
         at += (rows_of(b, row0) + kTokens - 1) / kTokens;
     }
-    const int units = (int)min(total, (int64_t)a.max_units);
+    const int units = (int)min((int64_t)all.x, (int64_t)a.max_units);
     __syncthreads();
     // A warp a unit: the keys that any of its rows sees.
     for (int u = warp; u < units; u += kPlanThreads / 32) {
@@ -206,8 +216,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
             x.hi = hi;
             x.tile0 = hi > 0 ? lo >> kTileShift : 0;
             x.tiles = hi > 0 ? ((hi + kTile - 1) >> kTileShift) - x.tile0 : 0;
-            x.first = 0;
-            x.pad = 0;
+            x.first = x.cell = 0;
             a.units[u] = x;
         }
     }
@@ -216,34 +225,40 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     const int uper = (units + kPlanThreads - 1) / kPlanThreads;
     const int u0 = min(units, tid * uper), u1 = min(units, u0 + uper);
     // Shares are cut evenly in cost: a unit's cells are kUnitCost of its own, then one for each tile.
-    sum = 0;
-    int64_t cells = 0, cost = 0;
+    sum = make_longlong2(0, 0);
     for (int u = u0; u < u1; ++u) {
         const int tiles = a.units[u].tiles;
-        sum += tiles;
-        cells += tiles ? tiles + kUnitCost : 0;
+        sum.x += tiles;
+        sum.y += tiles ? tiles + kUnitCost : 0;
     }
-    at = scan_exclusive(sum, warp_sum, &total);
-    int64_t cell = scan_exclusive(cells, warp_sum, &cost);
-    total *= heads;
-    cost *= heads;
+    longlong2 here = scan_exclusive(sum, warp_sum, &all);
+    const int64_t total = all.x * heads, cost = all.y * heads;
+    for (int u = u0; u < u1; ++u) {
+        const int tiles = a.units[u].tiles;
+        a.units[u].first = here.x;
+        a.units[u].cell = here.y;
+        here.x += tiles;
+        here.y += tiles ? tiles + kUnitCost : 0;
+    }
+    __syncthreads();
     // Shares longer than kUnitCost: each has a tile.
     const int64_t G = min((int64_t)a.ctas, cost / (kUnitCost + 1));
-    for (int u = u0; u < u1; ++u) {
-        const int tiles = a.units[u].tiles;
-        a.units[u].first = at;
-        if (tiles > 0) {
-            const int64_t begin = cell * heads, each = tiles + kUnitCost, end = begin + each * heads;
-            for (int64_t i = (begin * G + cost - 1) / cost; i < G && cost * i / G < end; ++i) {
-                const int64_t off = cost * i / G - begin, h = off / each, t = off - h * each - kUnitCost;
-                a.starts[i] = u;
-                a.cuts[i] = at * heads + h * tiles + (t > 0 ? t : 0);
+    if (tid <= G) {
+        int64_t cut = total;
+        if (tid < G) {
+            const int64_t c = cost * tid / G;
+            int lo = 0, hi = units;  // (of units that share a cell the last: the one with tiles)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.units[mid].cell * heads <= c) lo = mid; else hi = mid;
             }
-            cell += each;
+            const Unit x = a.units[lo];
+            const int64_t each = x.tiles + kUnitCost, off = c - x.cell * heads, h = off / each, t = off - h * each - kUnitCost;
+            a.starts[tid] = lo;
+            cut = x.first * heads + h * x.tiles + (t > 0 ? t : 0);
         }
-        at += tiles;
+        a.cuts[tid] = cut;
     }
-    if (tid == 0) a.cuts[G] = total;
     for (int i = tid; i < units * heads * 2; i += kPlanThreads) a.arrivals[i] = 0;
     if (tid == 0) *a.meta = Meta{total, (int32_t)G, units};
 }
@@ -327,6 +342,10 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+// tanh(x) / x = sum of kTanh[i] x^2i for |x| <= 1: interpolated at the Chebyshev points of x^2.
+__device__ constexpr float kTanh[6] = {0.999999463558197f,    -0.33329179883003235f, 0.13282513618469238f,
+                                       -0.05163545906543732f, 0.01677674594125271f,  -0.0030804092530161142f};
 
 __device__ __forceinline__ float tanh_fast(float x) {
     float r;
@@ -528,13 +547,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
                     for (int i = 0; i < 8; ++i) f[i] = row.factor * sc.k[i];
                     tmem_wait_ld();
-                    if constexpr (kCap || kBias) {
+                    if constexpr (kCap) {
+                        // tanh(x) / x as a polynomial of x^2 up to |x| = 1 (within 2^-20), on the FMA pipe: the
+                        // MUFU is busy with the weights.  A tile with a score past the cap takes the other way.
+                        float most = 0.f;
+#pragma unroll
+                        for (int e = 0; e < kTile; e += 2) {
+                            const float2 x = __fmul2_rn(make_float2(z[e], z[e + 1]), make_float2(f[e >> 4], f[e >> 4]));
+                            const float2 t = __fmul2_rn(x, x);
+                            most = fmaxf(fmaxf(most, t.x), t.y);
+                            float2 y = make_float2(kTanh[5], kTanh[5]);
+#pragma unroll
+                            for (int i = 4; i >= 0; --i) y = __ffma2_rn(y, t, make_float2(kTanh[i], kTanh[i]));
+                            y = __fmul2_rn(__fmul2_rn(x, make_float2(row.cap2, row.cap2)), y);
+                            z[e] = y.x;
+                            z[e + 1] = y.y;
+                        }
+                        if (__any_sync(0xffffffffu, most > 1.f)) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t(&)[32]>(z[32 * c]));
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < kTile; ++e) z[e] = row.cap2 * tanh_fast(z[e] * f[e >> 4]);
+                        }
+                    }
+                    if constexpr (kBias) {
                         const float ahead = (float)(k0 - row.pos);
 #pragma unroll
                         for (int e = 0; e < kTile; ++e) {
-                            z[e] *= f[e >> 4];
-                            if constexpr (kCap) z[e] = row.cap2 * tanh_fast(z[e]);
-                            if constexpr (kBias) z[e] = fmaf(-row.slope, fabsf(ahead + (float)e), z[e]);
+                            if constexpr (!kCap) z[e] *= f[e >> 4];
+                            z[e] = fmaf(-row.slope, fabsf(ahead + (float)e), z[e]);
                         }
                     }
                     if (edge) {
@@ -684,35 +727,50 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     }
                     group_sync();
                     if (ok && s.last[m] && real) {
-                        float M = -INFINITY, L = 0.f;
-                        for (int c = 0; c < parts; ++c)
-                            M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part(c) + 2 * kRowsM * kHeadDim) + prow).x);
+                        // The first few parts' (m, l) stay in registers; 16 loads of a row in flight.
+                        constexpr int kKept = 4;
+                        auto ml = [&](int c) {
+                            return __ldcg(reinterpret_cast<const float2*>(part(c) + 2 * kRowsM * kHeadDim) + prow);
+                        };
+                        float2 kept[kKept];
+#pragma unroll
+                        for (int i = 0; i < kKept; ++i) kept[i] = i < parts ? ml(i) : make_float2(-INFINITY, 0.f);
+                        float M = fmaxf(fmaxf(kept[0].x, kept[1].x), fmaxf(kept[2].x, kept[3].x)), L = 0.f;
+                        for (int c = kKept; c < parts; ++c) M = fmaxf(M, ml(c).x);
                         const float mu = M == -INFINITY ? 0.f : M;
-                        for (int c = 0; c < parts; ++c) {
-                            const float2 v = __ldcg(reinterpret_cast<const float2*>(part(c) + 2 * kRowsM * kHeadDim) + prow);
+#pragma unroll
+                        for (int i = 0; i < kKept; ++i) {
+                            kept[i].x = fast_exp2(kept[i].x - mu);
+                            L = fmaf(kept[i].x, kept[i].y, L);
+                        }
+                        for (int c = kKept; c < parts; ++c) {
+                            const float2 v = ml(c);
                             L = fmaf(fast_exp2(v.x - mu), v.y, L);
                         }
                         const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll 1
-                        for (int c4 = 0; c4 < 4; ++c4) {
-                            float x[32];
+                        for (int half = 0; half < 2; ++half) {
+                            float x[64];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) x[e] = 0.f;
+                            for (int e = 0; e < 64; ++e) x[e] = 0.f;
+#pragma unroll 1
                             for (int c = 0; c < parts; ++c) {
-                                const float* at = part(c);
-                                const float f = inv * fast_exp2(
-                                    __ldcg(reinterpret_cast<const float2*>(at + 2 * kRowsM * kHeadDim) + prow).x - mu);
+                                const float4* at = reinterpret_cast<const float4*>(part(c)) + half * 16 * 2 * kRowsM + prow;
+                                float4 v[16];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const float4 v =
-                                        __ldcg(reinterpret_cast<const float4*>(at) + (8 * c4 + e) * 2 * kRowsM + prow);
-                                    x[4 * e] = fmaf(f, v.x, x[4 * e]);
-                                    x[4 * e + 1] = fmaf(f, v.y, x[4 * e + 1]);
-                                    x[4 * e + 2] = fmaf(f, v.z, x[4 * e + 2]);
-                                    x[4 * e + 3] = fmaf(f, v.w, x[4 * e + 3]);
+                                for (int e = 0; e < 16; ++e) v[e] = __ldcg(at + e * 2 * kRowsM);
+                                const float f = inv * (c == 0 ? kept[0].x : c == 1 ? kept[1].x : c == 2 ? kept[2].x
+                                                       : c == 3 ? kept[3].x : fast_exp2(ml(c).x - mu));
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    x[4 * e] = fmaf(f, v[e].x, x[4 * e]);
+                                    x[4 * e + 1] = fmaf(f, v[e].y, x[4 * e + 1]);
+                                    x[4 * e + 2] = fmaf(f, v[e].z, x[4 * e + 2]);
+                                    x[4 * e + 3] = fmaf(f, v[e].w, x[4 * e + 3]);
                                 }
                             }
-                            write(c4, x);
+                            write(2 * half, reinterpret_cast<const float(&)[32]>(x[0]));
+                            write(2 * half + 1, reinterpret_cast<const float(&)[32]>(x[32]));
                         }
                     }
                 }
@@ -727,7 +785,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         // ============================ conversion ============================
         take_registers<kConvRegs>();
         const int cw = warp - kConvWarp, t = lane & 3;
-        const int row0 = 32 * cw + (lane >> 2);  // this lane's rows: row0 + 8 i
+        // This lane's rows: row0 + 8 i.  Eight lanes that access shared memory together take chunks 0-3
+        // of two rows whose numbers differ in bits 0 and 2: with the swizzle, all eight 16-byte columns
+        // of the codes' rows and of the operand's.
+        const int row0 = 32 * cw + ((lane >> 3) ^ (lane & 4 ? 5 : 0));
         int item = 0;  // K and V of the tiles in turn
         int rs = 0, rphase = 0, cs = 0, cphase = 0, tile_count = 0;
         while (walk.n > 0 && ok) {
