@@ -343,9 +343,10 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// tanh(x) / x = sum of kTanh[i] x^2i for |x| <= 1: interpolated at the Chebyshev points of x^2.
-__device__ constexpr float kTanh[6] = {0.999999463558197f,    -0.33329179883003235f, 0.13282513618469238f,
-                                       -0.05163545906543732f, 0.01677674594125271f,  -0.0030804092530161142f};
+// tanh(x) / x = sum of kTanh[i] x^2i for |x| <= 1/2, within 2^-15 of it (a quarter of
+// what a weight's rounding to FP16 moves at a score of 4): interpolated at the
+// Chebyshev points of x^2.
+__device__ constexpr float kTanh[3] = {0.99997777f, -0.33170217f, 0.11525216f};
 
 __device__ __forceinline__ float tanh_fast(float x) {
     float r;
@@ -548,28 +549,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     for (int i = 0; i < 8; ++i) f[i] = row.factor * sc.k[i];
                     tmem_wait_ld();
                     if constexpr (kCap) {
-                        // tanh(x) / x as a polynomial of x^2 up to |x| = 1 (within 2^-20), on the FMA pipe: the
-                        // MUFU is busy with the weights.  A tile with a score past the cap takes the other way.
+                        // cap tanh(x) as a polynomial up to |x| = 1/2, on the FMA pipe: the MUFU is busy with the
+                        // weights.  A tile with a score past half the cap takes the other way, through TMEM.
+                        const float2 c0 = make_float2(kTanh[0] * row.cap2, kTanh[0] * row.cap2),
+                                     c1 = make_float2(kTanh[1] * row.cap2, kTanh[1] * row.cap2),
+                                     c2 = make_float2(kTanh[2] * row.cap2, kTanh[2] * row.cap2);
                         float most = 0.f;
 #pragma unroll
                         for (int e = 0; e < kTile; e += 2) {
                             const float2 x = __fmul2_rn(make_float2(z[e], z[e + 1]), make_float2(f[e >> 4], f[e >> 4]));
                             const float2 t = __fmul2_rn(x, x);
                             most = fmaxf(fmaxf(most, t.x), t.y);
-                            float2 y = make_float2(kTanh[5], kTanh[5]);
-#pragma unroll
-                            for (int i = 4; i >= 0; --i) y = __ffma2_rn(y, t, make_float2(kTanh[i], kTanh[i]));
-                            y = __fmul2_rn(__fmul2_rn(x, make_float2(row.cap2, row.cap2)), y);
+                            const float2 y = __fmul2_rn(x, __ffma2_rn(__ffma2_rn(c2, t, c1), t, c0));
                             z[e] = y.x;
                             z[e + 1] = y.y;
                         }
-                        if (__any_sync(0xffffffffu, most > 1.f)) {
+                        if (__any_sync(0xffffffffu, most > 0.25f)) {
+#pragma unroll 1
+                            for (int i = 0; i < 8; ++i) {
+                                uint32_t v[16];
+                                tmem_ld16(t_s + 16 * i, v);
+                                const float g = row.factor * sc.k[i];
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e)
+                                    v[e] = __float_as_uint(row.cap2 * tanh_fast(__uint_as_float(v[e]) * g));
+                                tmem_st16(t_s + 16 * i, v);
+                            }
+                            tmem_wait_st();
 #pragma unroll
                             for (int c = 0; c < 4; ++c)
                                 tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t(&)[32]>(z[32 * c]));
                             tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < kTile; ++e) z[e] = row.cap2 * tanh_fast(z[e] * f[e >> 4]);
                         }
                     }
                     if constexpr (kBias) {
