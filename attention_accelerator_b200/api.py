@@ -106,7 +106,13 @@ def _workspace(device: torch.device, stream_ptr: int, nbytes: int) -> torch.Tens
         return buf
 
 
+# torch's own lookup of the current stream's handle, without the Stream object (2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -577,4 +583,9 @@ def read_device_status(device: torch.device | None = None) -> int:
     ws = _workspace(device, stream, 4096)
     st = ctypes.c_int(0)
     _check(_lib.load().gqa_read_status(ws.data_ptr(), stream, ctypes.byref(st)), "read_device_status")
+    paged = _ws.get((device.index, ("paged", stream)))
+    if st.value == _lib.GQA_OK and paged is not None:
+        _check(_lib.load().gqa_read_status(paged.data_ptr(), stream, ctypes.byref(st)), "read_device_status")
+        if st.value != _lib.GQA_OK:
+            paged.zero_()  # the paged calls' counters lie past the header
     return st.value

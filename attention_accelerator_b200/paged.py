@@ -118,7 +118,7 @@ def _need(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: 
     """Pointer of a contiguous tensor of a call, or of None."""
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -169,15 +169,14 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     _table(block_table, n, device)
     if free_pages.dim() != 1:
         raise ValueError("free_pages must be one-dimensional")
-    if lens_out is None:
-        lens_out = torch.empty_like(lens)
-    if n_free_out is None:
-        n_free_out = torch.empty_like(n_free)
+    if not 0 <= max_tokens <= 0x7FFFFFFF:
+        raise ValueError(f"max_tokens must be in [0, 2^31), got {max_tokens}")
     i32 = torch.int32
-    first = torch.empty(n + 1, dtype=i32, device=device)
     slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
-    positions = torch.empty(max_tokens, dtype=i32, device=device)
-    counts = torch.empty(4, dtype=i32, device=device)
+    room = [n if lens_out is None else 0, 1 if n_free_out is None else 0, n + 1, max_tokens, 4]  # in one allocation
+    new_lens_out, new_n_free, first, positions, counts = torch.empty(sum(room), dtype=i32, device=device).split(room)
+    lens_out = new_lens_out if lens_out is None else lens_out
+    n_free_out = new_n_free if n_free_out is None else n_free_out
     stream = _stream_ptr(device)
     ws = _paged_workspace(device, stream, _lib.CHUNKED_WORKSPACE_BYTES)
     _check(lib.gqa_plan_pages(
@@ -192,7 +191,7 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
 
 
 def _rows(name: str, t: torch.Tensor, heads: int, device: torch.device) -> None:
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or tuple(t.shape[1:]) != (heads, HEAD_DIM) or t.stride(-1) != 1 \
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (heads, HEAD_DIM) or t.stride(2) != 1 \
             or t.device != device:
         raise ValueError(f"{name} must be bfloat16 [rows, {heads}, {HEAD_DIM}] on {device} with a contiguous last dim")
 
@@ -274,14 +273,18 @@ def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_posit
         out_row_stride=out.stride(0), out_head_stride=out.stride(1))
     if rows == 0:
         return out
-    nbytes = lib.gqa_paged_workspace_bytes(ctypes.byref(cache.c), ctypes.byref(p))
-    if nbytes == 0:
-        raise GqaError(_lib.GQA_ERR_CUDA, f"{name}: workspace sizing failed (no supported GPU?)")
     stream = _stream_ptr(device)
-    ws = _paged_workspace(device, stream, nbytes)
     fn = lib.gqa_decode_paged if first_query is None else lib.gqa_decode_paged_chunked
-    _check(fn(q.data_ptr(), out.data_ptr(), ctypes.byref(cache.c), ctypes.byref(p), ws.data_ptr(), ws.numel(), stream),
-           name)
+    c = ctypes.byref(cache.c)
+    ws = _paged_workspace(device, stream, _lib.CHUNKED_WORKSPACE_BYTES)
+    status = fn(q.data_ptr(), out.data_ptr(), c, ctypes.byref(p), ws.data_ptr(), ws.numel(), stream)
+    if status == _lib.GQA_ERR_WORKSPACE:  # nothing was launched: the stream's first call, or a larger one
+        nbytes = lib.gqa_paged_workspace_bytes(c, ctypes.byref(p))
+        if nbytes == 0:
+            raise GqaError(_lib.GQA_ERR_CUDA, f"{name}: workspace sizing failed (no supported GPU?)")
+        ws = _paged_workspace(device, stream, nbytes)
+        status = fn(q.data_ptr(), out.data_ptr(), c, ctypes.byref(p), ws.data_ptr(), ws.numel(), stream)
+    _check(status, name)
     return out
 
 
