@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
     const int page_mask = (1 << a.page_shift) - 1;
     auto pages_of = [&](long long len) { return (int)((len + page_mask) >> a.page_shift); };
     if (tid == 0) s_bad = 0;
+    const int n_free = *a.n_free;
     __syncthreads();
 
     // Each thread sums a stretch of consecutive requests, then the block scans the stretches.
@@ -92,15 +93,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
         for (int i = 0; i < 3; ++i) warp_sum[i][warp] = incl[i];
     if (bad) s_bad = 1;
     __syncthreads();
-    long long total[3] = {0, 0, 0}, base[3] = {0, 0, 0};
-    for (int w = 0; w < 32; ++w) {
+    long long total[3], base[3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            if (w < warp) base[i] += warp_sum[i][w];
-            total[i] += warp_sum[i][w];
+    for (int i = 0; i < 3; ++i) {
+        total[i] = warp_sum[i][lane];
+        base[i] = lane < warp ? total[i] : 0;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            total[i] += __shfl_xor_sync(0xffffffffu, total[i], d);
+            base[i] += __shfl_xor_sync(0xffffffffu, base[i], d);
         }
     }
-    const int n_free = *a.n_free;
     // All or nothing.  (The sums in shared memory are 32-bit: with `ok` they fit.)
     const bool ok = !s_bad && n_free >= 0 && total[0] <= a.max_tokens && n_free + total[2] <= a.free_capacity &&
                     total[1] <= n_free + total[2];
@@ -186,10 +189,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // Append: RoPE of K, quantisation, and the rescale of a page's earlier codes.
 //
-// A CTA takes the runs that start in its window of tokens, for one head of K or
-// V (grid: windows x heads x {K, V}).  With 2 * page_len threads a run's rows fit
-// the registers (8 threads a row, each 8 rotate_half pairs; 4 rows a thread), so
-// that the rows are read once: amax over the block, then the codes.
+// A CTA takes the runs that start in its window of tokens, for `heads` heads of K
+// or V (grid: windows x head groups x {K, V}).  8 threads take a row, each 8
+// rotate_half pairs, and a thread two rows: with 4 * page_len threads a run's rows
+// stay in registers from the amax over the block to its codes.  A decode step's
+// runs of one row get 64 threads instead (16 rows), so that all CTAs of the step
+// are resident at once; a longer run is then read a second time.
+// K's rotation factors cost more than anything else here (one sine and cosine a
+// pair): a call of many tokens computes them once for all heads of a run.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     PagedCacheView c;
@@ -197,18 +204,17 @@ struct AppendArgs {
     int64_t k_tstride, k_hstride, v_tstride, v_hstride;
     const int64_t* slots;
     const int32_t* positions;
-    int n_tokens, window;
+    int n_tokens, window, heads;
     RopeSteps rope;
 };
 
+constexpr int kAppendRows = 2;  // of a run, per thread
 constexpr float kMinBlockScale = 0x1p-100f;  // keeps 1 / scale finite for a block of zeros
 
 template <int kCode>
-__device__ __forceinline__ uint64_t encode8(const float* x, float inv) {
-    uint64_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w |= (uint64_t)value_code<kCode>(x[e] * inv) << (8 * e);
-    return w;
+__device__ __forceinline__ uint2 encode8(const float* x, float inv) {
+    return make_uint2(value_codes4<kCode>(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv), __fmul_rn(x[2], inv), __fmul_rn(x[3], inv)),
+                      value_codes4<kCode>(__fmul_rn(x[4], inv), __fmul_rn(x[5], inv), __fmul_rn(x[6], inv), __fmul_rn(x[7], inv)));
 }
 
 __device__ __forceinline__ void unpack8(uint4 w, float* x) {
@@ -221,111 +227,178 @@ __device__ __forceinline__ void unpack8(uint4 w, float* x) {
     }
 }
 
-template <int kCode>
-__global__ void __launch_bounds__(2 * kPagedMaxPage) append_kernel(const __grid_constant__ AppendArgs a) {
-    __shared__ float s_max[2 * kPagedMaxPage / 32];
-    __shared__ int s_len[2 * kPagedMaxPage / 32];
+// kOnce: 4 * page_len threads, so that every run's rows stay in registers.
+template <int kCode, bool kOnce>
+__global__ void __launch_bounds__(kOnce ? 4 * kPagedMaxPage : 64) append_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ uint32_t s_max[4 * kPagedMaxPage / 32];
+    __shared__ int s_len[4 * kPagedMaxPage / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
-    const int head = blockIdx.y;
+    const int head0 = blockIdx.y * a.heads, head1 = min(a.c.kv_heads, head0 + a.heads);
     const bool is_k = blockIdx.z == 0;
     const int page_len = a.c.page_len, page_mask = page_len - 1;
     const int64_t n_slots = (int64_t)a.c.pages << a.c.page_shift;
-    const __nv_bfloat16* src = (is_k ? a.k : a.v) + head * (is_k ? a.k_hstride : a.v_hstride);
-    const int64_t tstride = is_k ? a.k_tstride : a.v_tstride;
-    uint8_t* codes = (is_k ? a.c.k : a.c.v) + head * a.c.head_stride;
-    float* scales = (is_k ? a.c.k_scale : a.c.v_scale) + head;
+    const int64_t tstride = is_k ? a.k_tstride : a.v_tstride, hstride = is_k ? a.k_hstride : a.v_hstride;
     const float qmax = kCode == GQA_CODE_INT8 ? 127.f : 448.f;
-    const int chunk = tid & 7, row0 = tid >> 3, rows_per_pass = blockDim.x >> 3;  // page_len / 4
+    const int chunk = tid & 7, row0 = tid >> 3, rows_per_pass = blockDim.x >> 3;  // page_len / 2
 
-    const int w0 = blockIdx.x * a.window, w1 = min(a.n_tokens, w0 + a.window);
-    for (int t0 = w0; t0 < w1; ++t0) {
+    // The tokens of the window that start a run: slots of the cache whose predecessor is not the token before.
+    const int w0 = blockIdx.x * a.window;
+    const int64_t first_slot = w0 + tid < a.n_tokens ? a.slots[w0 + tid] : -1;
+    unsigned starts;
+    {
+        const int t = w0 + lane;
+        int64_t slot = -1, before = -1;
+        if (lane < a.window && t < a.n_tokens) {
+            slot = a.slots[t];
+            if (t > 0) before = a.slots[t - 1];
+        }
+        starts = __ballot_sync(0xffffffffu, slot >= 0 && slot < n_slots && ((slot & page_mask) == 0 || before != slot - 1));
+    }
+    for (; starts; starts &= starts - 1) {
+        const int t0 = w0 + __ffs(starts) - 1;
         const int64_t slot = a.slots[t0];
-        if (slot < 0 || slot >= n_slots) continue;  // the whole CTA: slot is uniform
         const int r0 = (int)(slot & page_mask);
-        if (t0 > 0 && r0 != 0 && a.slots[t0 - 1] == slot - 1) continue;  // inside another run
         // Rows of the run: up to the page's end, the call's end or the first slot that does not follow.
-        const bool in = tid < page_len - r0 && t0 + tid < a.n_tokens && a.slots[t0 + tid] == slot + tid;
-        const unsigned miss = ~__ballot_sync(0xffffffffu, in);
-        if (lane == 0) s_len[warp] = miss ? __ffs(miss) - 1 : 32;
-        __syncthreads();
         int len = 0;
-        for (int w = 0; w < n_warps; ++w) {
-            len += s_len[w];
-            if (s_len[w] < 32) break;
+        for (int at = 0; at < page_len - r0; at += blockDim.x) {
+            const int i = at + tid;
+            const bool in = i < page_len - r0 && t0 + i < a.n_tokens &&
+                            (t0 == w0 && at == 0 ? first_slot : a.slots[t0 + i]) == slot + i;
+            const unsigned miss = ~__ballot_sync(0xffffffffu, in);
+            if (lane == 0) s_len[warp] = miss ? __ffs(miss) - 1 : 32;
+            __syncthreads();
+            int n = 0;
+            for (int w = 0; w < n_warps; ++w) {
+                n += s_len[w];
+                if (s_len[w] < 32) break;
+            }
+            len += n;
+            __syncthreads();
+            if (n < (int)blockDim.x) break;
         }
         const int64_t page = slot >> a.c.page_shift;
-        uint8_t* base = codes + page * a.c.page_stride;
-        float* scale_at = scales + page * a.c.scale_page_stride;
-        const float old = r0 ? *scale_at : 0.f;
-
-        // Rows row0, row0 + rows_per_pass, ...: dims 8 chunk .. and 64 + 8 chunk ..
-        float x[4][16];
-        float most = 0.f;
-        bool finite = true;
+        const bool turn = is_k && a.positions;
+        // Rows b0 + row0, b0 + row0 + rows_per_pass of the run: dims 8 chunk .. and 64 + 8 chunk ..
+        const int cap = rows_per_pass * kAppendRows;  // rows at once; a longer run is read twice
+        uint4 raw[kAppendRows][2];
+        float2 f[kAppendRows][8];
+        float x[kAppendRows][16];
+        auto load = [&](int head, int b0) {
+            const __nv_bfloat16* src = (is_k ? a.k : a.v) + head * hstride + 8 * chunk;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int r = row0 + p * rows_per_pass;
-            if (r >= len) continue;
-            const __nv_bfloat16* row = src + (int64_t)(t0 + r) * tstride;
-            unpack8(*reinterpret_cast<const uint4*>(row + 8 * chunk), x[p]);
-            unpack8(*reinterpret_cast<const uint4*>(row + 64 + 8 * chunk), x[p] + 8);
-            if (is_k && a.positions) {
+            for (int p = 0; p < kAppendRows; ++p) {
+                const int r = b0 + row0 + p * rows_per_pass;
+                if (r >= len) continue;
+                const __nv_bfloat16* row = src + (int64_t)(t0 + r) * tstride;
+                raw[p][0] = *reinterpret_cast<const uint4*>(row);
+                raw[p][1] = *reinterpret_cast<const uint4*>(row + 64);
+            }
+        };
+        auto factors = [&](int b0) {
+            if (!turn) return;
+#pragma unroll
+            for (int p = 0; p < kAppendRows; ++p) {
+                const int r = b0 + row0 + p * rows_per_pass;
+                if (r >= len) continue;
                 const int pos = a.positions[t0 + r];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 f = rope_factor(a.rope.step[8 * chunk + e], pos);
-                    const float re = x[p][e], im = x[p][8 + e];
-                    x[p][e] = re * f.x - im * f.y;
-                    x[p][8 + e] = re * f.y + im * f.x;
+                for (int e = 0; e < 8; ++e) f[p][e] = rope_factor_fast(a.rope.step[8 * chunk + e], pos);
+            }
+        };
+        // The rows' values, and the largest magnitude, as FP32 bits (which order as integers).
+        auto values = [&](int b0, uint32_t top) {
+#pragma unroll
+            for (int p = 0; p < kAppendRows; ++p) {
+                if (b0 + row0 + p * rows_per_pass >= len) continue;
+                unpack8(raw[p][0], x[p]);
+                unpack8(raw[p][1], x[p] + 8);
+                if (turn) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float re = x[p][e], im = x[p][8 + e];
+                        x[p][e] = re * f[p][e].x - im * f[p][e].y;
+                        x[p][8 + e] = re * f[p][e].y + im * f[p][e].x;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[p][e]) & 0x7fffffffu);
+            }
+            return top;
+        };
+        auto scale_of = [&](int head) {
+            return r0 ? (is_k ? a.c.k_scale : a.c.v_scale)[head + page * a.c.scale_page_stride] : 0.f;
+        };
+        load(head0, 0);
+        float next_old = scale_of(head0);
+        factors(0);
+#pragma unroll 1
+        for (int head = head0; head < head1; ++head) {
+            uint8_t* base = (is_k ? a.c.k : a.c.v) + head * a.c.head_stride + page * a.c.page_stride;
+            float* scale_at = (is_k ? a.c.k_scale : a.c.v_scale) + head + page * a.c.scale_page_stride;
+            const float old = next_old;
+            uint32_t top = values(0, 0u);
+            for (int b0 = cap; !kOnce && b0 < len; b0 += cap) {
+                load(head, b0);
+                factors(b0);
+                top = values(b0, top);
+            }
+            if ((kOnce || len <= cap) && head + 1 < head1) load(head + 1, 0);  // on its way while this block is reduced and written
+            if (head + 1 < head1) next_old = scale_of(head + 1);
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) s_max[warp] = top;
+            __syncthreads();
+            top = s_max[0];
+            for (int w = 1; w < n_warps; ++w) top = max(top, s_max[w]);
+            const float most = top < 0x7f800000u ? __uint_as_float(top) : INFINITY;
+            const float mine =
+                most == INFINITY ? __int_as_float(0x7fffffff) : fmaxf(__fdiv_rn(most, qmax), kMinBlockScale);
+            const float scale = mine > old || mine != mine ? mine : old;
+            const float inv = scale == scale ? __frcp_rn(scale) : 0.f;
+            for (int b0 = 0; b0 < len; b0 += cap) {
+                if (!kOnce && len > cap) {
+                    load(head, b0);
+                    factors(b0);
+                    values(b0, 0u);
+                }
+#pragma unroll
+                for (int p = 0; p < kAppendRows; ++p) {
+                    const int r = b0 + row0 + p * rows_per_pass;
+                    if (r >= len) continue;
+                    if (!(scale == scale))
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[p][e] = 0.f;
+                    uint8_t* row = base + (r0 + r) * a.c.row_stride;
+                    *reinterpret_cast<uint2*>(row + 8 * chunk) = encode8<kCode>(x[p], inv);
+                    *reinterpret_cast<uint2*>(row + 64 + 8 * chunk) = encode8<kCode>(x[p] + 8, inv);
+                }
+                if (kOnce) break;
+            }
+            if (mine > old) {
+                for (int r = row0; r < r0; r += rows_per_pass) {
+                    uint8_t* row = base + r * a.c.row_stride;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint2* at = reinterpret_cast<uint2*>(row + 64 * half + 8 * chunk);
+                        const uint2 w = *at;
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            y[e] = __fmul_rn(code_value<kCode>((uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)))), old);
+                        *at = encode8<kCode>(y, inv);
+                    }
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                most = fmaxf(most, fabsf(x[p][e]));
-                finite &= fabsf(x[p][e]) <= 3.402823466e38f;
+            if (!kOnce && len > cap && head + 1 < head1) {
+                load(head + 1, 0);
+                factors(0);
             }
+            __syncthreads();  // everyone has read the old scale, s_len and s_max
+            if (tid == 0) *scale_at = scale;
         }
-        if (!finite) most = INFINITY;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        if (lane == 0) s_max[warp] = most;
-        __syncthreads();
-        most = s_max[0];
-        for (int w = 1; w < n_warps; ++w) most = fmaxf(most, s_max[w]);
-        const float mine = most == INFINITY ? __int_as_float(0x7fffffff) : fmaxf(__fdiv_rn(most, qmax), kMinBlockScale);
-        const float scale = mine > old || mine != mine ? mine : old;
-        const float inv = scale == scale ? __frcp_rn(scale) : 0.f;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int r = row0 + p * rows_per_pass;
-            if (r >= len) continue;
-            if (!(scale == scale))
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[p][e] = 0.f;
-            uint8_t* row = base + (r0 + r) * a.c.row_stride;
-            *reinterpret_cast<uint64_t*>(row + 8 * chunk) = encode8<kCode>(x[p], inv);
-            *reinterpret_cast<uint64_t*>(row + 64 + 8 * chunk) = encode8<kCode>(x[p] + 8, inv);
-        }
-        if (mine > old) {
-            for (int r = row0; r < r0; r += rows_per_pass) {
-                uint8_t* row = base + r * a.c.row_stride;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint64_t* at = reinterpret_cast<uint64_t*>(row + 64 * half + 8 * chunk);
-                    const uint64_t w = *at;
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = code_value<kCode>((uint8_t)(w >> (8 * e))) * old;
-                    *at = encode8<kCode>(y, inv);
-                }
-            }
-        }
-        __syncthreads();  // everyone has read the old scale, s_len and s_max
-        if (tid == 0) *scale_at = scale;
     }
 }
 
-// Rows back to BF16: one warp a (row, K or V), 4 dims a lane and head.
+// Rows back to BF16: a thread 16 codes of one (row, head), of K or V.
 struct ReadArgs {
     PagedCacheView c;
     const int64_t* slots;
@@ -335,28 +408,32 @@ struct ReadArgs {
 
 template <int kCode>
 __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadArgs a) {
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int chunk = (int)(i & 7);
+    const int64_t at = i >> 3, row = at / a.c.kv_heads;
+    const int head = (int)(at - row * a.c.kv_heads);
     if (row >= a.n) return;
     const int64_t slot = a.slots[row];
-    const bool real = slot >= 0 && slot < ((int64_t)a.c.pages << a.c.page_shift);
-    const int64_t page = real ? slot >> a.c.page_shift : 0;
-    const int64_t at = page * a.c.page_stride + (real ? slot & (a.c.page_len - 1) : 0) * a.c.row_stride;
-    const uint8_t* codes = (blockIdx.y ? a.c.v : a.c.k) + at + 4 * lane;
-    const float* scales = (blockIdx.y ? a.c.v_scale : a.c.k_scale) + page * a.c.scale_page_stride;
-    __nv_bfloat16* out = (blockIdx.y ? a.out_v : a.out_k) + (int64_t)row * a.c.kv_heads * kHeadDim + 4 * lane;
-    for (int h = 0; h < a.c.kv_heads; ++h) {
-        uint2 o = make_uint2(0u, 0u);
-        if (real) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + h * a.c.head_stride);
-            const float s = scales[h];
-            float y[4];
+    uint4 o[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (slot >= 0 && slot < ((int64_t)a.c.pages << a.c.page_shift)) {
+        const int64_t page = slot >> a.c.page_shift;
+        const uint8_t* codes = (blockIdx.y ? a.c.v : a.c.k) + page * a.c.page_stride +
+                               (slot & (a.c.page_len - 1)) * a.c.row_stride + head * a.c.head_stride + 16 * chunk;
+        const float s = (blockIdx.y ? a.c.v_scale : a.c.k_scale)[page * a.c.scale_page_stride + head];
+        const uint4 w = *reinterpret_cast<const uint4*>(codes);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        uint32_t* to = &o[0].x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = code_value<kCode>((uint8_t)(w >> (8 * e))) * s;
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
-            o = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t pair = ws[e >> 1] >> (16 * (e & 1));
+            const __nv_bfloat162 v = __floats2bfloat162_rn(code_value<kCode>((uint8_t)pair) * s,
+                                                           code_value<kCode>((uint8_t)(pair >> 8)) * s);
+            to[e] = *reinterpret_cast<const uint32_t*>(&v);
         }
-        *reinterpret_cast<uint2*>(out + h * kHeadDim) = o;
     }
+    uint4* out = reinterpret_cast<uint4*>((blockIdx.y ? a.out_v : a.out_k) + at * kHeadDim + 16 * chunk);
+    out[0] = o[0];
+    out[1] = o[1];
 }
 
 // ---------------------------------------------------------------------------
@@ -572,14 +649,19 @@ int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token
     a.slots = slots;
     a.positions = positions;
     a.n_tokens = n_tokens;
-    a.window = n_tokens <= 2048 ? 1 : 16;
+    // A step's rows, one a request, want every CTA that they can have; prompts' fill pages, of which a window
+    // of 16 tokens begins one at most.
+    const bool step = n_tokens <= 1024;
+    a.window = step ? 1 : 16;
+    a.heads = step ? 1 : cache->kv_heads;
+    const int threads = step ? 64 : 4 * cache->page_len;
     a.rope = rope_steps_of(rope_theta);
-    const dim3 grid((n_tokens + a.window - 1) / a.window, cache->kv_heads, 2);
+    const dim3 grid((n_tokens + a.window - 1) / a.window, (cache->kv_heads + a.heads - 1) / a.heads, 2);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (cache->code == GQA_CODE_INT8)
-        append_kernel<GQA_CODE_INT8><<<grid, 2 * cache->page_len, 0, s>>>(a);
+        (step ? append_kernel<GQA_CODE_INT8, false> : append_kernel<GQA_CODE_INT8, true>)<<<grid, threads, 0, s>>>(a);
     else
-        append_kernel<GQA_CODE_E4M3><<<grid, 2 * cache->page_len, 0, s>>>(a);
+        (step ? append_kernel<GQA_CODE_E4M3, false> : append_kernel<GQA_CODE_E4M3, true>)<<<grid, threads, 0, s>>>(a);
     return launched();
 }
 
@@ -600,7 +682,7 @@ int gqa_read_paged(const gqa_paged_cache* cache, const int64_t* slots, int n, vo
     a.out_k = static_cast<__nv_bfloat16*>(out_k);
     a.out_v = static_cast<__nv_bfloat16*>(out_v);
     a.n = n;
-    const dim3 grid((n + 7) / 8, 2);
+    const dim3 grid((unsigned)(((int64_t)n * cache->kv_heads * 8 + 255) / 256), 2);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (cache->code == GQA_CODE_INT8)
         read_kernel<GQA_CODE_INT8><<<grid, 256, 0, s>>>(a);

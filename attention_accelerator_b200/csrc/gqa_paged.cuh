@@ -67,6 +67,14 @@ __device__ __forceinline__ KeyRange paged_range(const PagedCall& a, int row, int
     return KeyRange{lo, (int)hi};
 }
 
+// rope_factor from the top 32 bits of the phase: 2^-32 turns, a 128th of what FP32 leaves of it.
+__device__ __forceinline__ float2 rope_factor_fast(uint64_t step, int64_t pos) {
+    const int turns = (int)((step * (uint64_t)pos) >> 32);
+    float sn, cs;
+    sincospif(__int2float_rn(turns) * 0x1p-31f, &sn, &cs);
+    return make_float2(cs, sn);
+}
+
 // Value of one code.
 template <int kCode>
 __device__ __forceinline__ float code_value(uint8_t c) {
@@ -78,14 +86,19 @@ __device__ __forceinline__ float code_value(uint8_t c) {
     }
 }
 
-// Code of a value already divided by its scale: round to nearest even, saturating.
+// Codes of 4 values already divided by their scale, first in the low byte: round to
+// nearest even.  For int8 the caller keeps |y| below 127.5; the sum with 1.5 * 2^23
+// leaves the integer in the low bits.  e4m3 saturates.
 template <int kCode>
-__device__ __forceinline__ uint8_t value_code(float y) {
+__device__ __forceinline__ uint32_t value_codes4(float y0, float y1, float y2, float y3) {
     if constexpr (kCode == GQA_CODE_INT8) {
-        const int i = __float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
-        return (uint8_t)(int8_t)i;
+        const uint32_t a = __float_as_uint(__fadd_rn(y0, 12582912.f)), b = __float_as_uint(__fadd_rn(y1, 12582912.f));
+        const uint32_t c = __float_as_uint(__fadd_rn(y2, 12582912.f)), d = __float_as_uint(__fadd_rn(y3, 12582912.f));
+        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
     } else {
-        return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y2, y3), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
     }
 }
 

@@ -358,14 +358,6 @@ __device__ __forceinline__ float finite_or(float x, float other) {
     return fabsf(x) <= 3.402823466e38f ? x : other;
 }
 
-// rope_factor from the top 32 bits of the phase: 2^-32 turns, a 128th of what FP32 leaves of it.
-__device__ __forceinline__ float2 rope_factor_fast(uint64_t step, int64_t pos) {
-    const int turns = (int)((step * (uint64_t)pos) >> 32);
-    float sn, cs;
-    sincospif(__int2float_rn(turns) * 0x1p-31f, &sn, &cs);
-    return make_float2(cs, sn);
-}
-
 // The larger magnitude of two BF16 codes, as FP32 bits (which order as integers).
 __device__ __forceinline__ uint32_t magnitudes(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
 

@@ -190,6 +190,34 @@ def test_append_without_rope_is_exact(code, layout, page_len, heads):
         assert torch.equal(g.cpu(), torch.from_numpy(x).to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("page_len,code", [(16, "e4m3"), (32, "int8"), (64, "e4m3"), (128, "int8")])
+def test_append_of_many_tokens_is_exact(page_len, code):
+    """Prompts: more tokens than a step has, runs that fill pages and cross them."""
+    gen = torch.Generator("cuda").manual_seed(page_len)
+    lens, starts = [700, 1, page_len * 3, 331, 90], [5, page_len - 1, 0, page_len // 2, 3]
+    table, slots = list(range(200))[::-1], []
+    for n, a in zip(lens, starts):
+        pages = [table.pop() for _ in range(-(-(a + n) // page_len))]
+        slots += [pages[(a + i) // page_len] * page_len + (a + i) % page_len for i in range(n)]
+    cache = random_cache(gen, 200, page_len, code, "position_major", 3)
+    n = len(slots)
+    assert n > 1024
+    k, v = (torch.randn(n, 3, 128, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2))
+    k[::100] *= 30
+    want = {name: expect_append(rows_of(cache, t), s.cpu().numpy(), x.float().cpu().numpy(), slots, page_len, code)
+            for name, t, s, x in (("k", cache.k, cache.k_scale, k), ("v", cache.v, cache.v_scale, v))}
+    gqa.append_paged(cache, k, v, ints(slots, torch.int64))
+    for name, t, s in (("k", cache.k, cache.k_scale), ("v", cache.v, cache.v_scale)):
+        assert np.array_equal(s.cpu().numpy(), want[name][1]), name
+        assert np.array_equal(rows_of(cache, t), want[name][0]), name
+    # the same rows with rotation by zero, which is none: the same codes
+    again = random_cache(gen, 200, page_len, code, "position_major", 3)
+    again.k.view(torch.uint8).copy_(cache.k.view(torch.uint8))
+    again.k_scale.copy_(cache.k_scale)
+    gqa.append_paged(again, k, v, ints(slots, torch.int64), positions=torch.zeros(n, dtype=torch.int32, device="cuda"))
+    assert torch.equal(again.k_scale, cache.k_scale) and np.array_equal(words(again.k), words(cache.k))
+
+
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 def test_append_rotates_k(code):
     """Stored K is RoPE(k) to half a step of its scale; the rotation's own error (FP32, about 2^-22 of the pair's
