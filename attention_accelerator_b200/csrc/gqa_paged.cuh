@@ -75,6 +75,27 @@ __device__ __forceinline__ float2 rope_factor_fast(uint64_t step, int64_t pos) {
     return make_float2(cs, sn);
 }
 
+// Programmatic dependent launch: a kernel so launched starts before the one in
+// front of it in the stream has ended, and touches no memory before the wait.
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void allow_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename Args>
+inline cudaError_t launch_dependent(void (*kernel)(Args), int grid, int threads, size_t smem, cudaStream_t stream,
+                                    const Args& a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 // Value of one code.
 template <int kCode>
 __device__ __forceinline__ float code_value(uint8_t c) {

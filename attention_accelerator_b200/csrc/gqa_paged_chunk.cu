@@ -164,6 +164,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     __shared__ longlong2 warp_sum[kPlanThreads / 32];
     const PagedCall& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, batch = p.batch;
+    dependency_wait();
+    allow_dependents();
     // Rows of sequence b, kept within the call's whatever the device's numbers say.
     auto rows_of = [&](int b, int& row0) {
         row0 = min(max(p.first_query[b], 0), p.rows);
@@ -406,6 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         }
         fence_barrier_init();
     }
+    dependency_wait();
+    allow_dependents();
     const Meta meta = *a.meta;
     if (tid < kPairs) s.step[tid] = a.rope.step[tid];
     if (tid <= meta.ctas) s.cuts[tid] = a.cuts[tid];
@@ -1080,7 +1084,8 @@ cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int
     pl.arrivals = reinterpret_cast<uint32_t*>(ws + r.arrivals);
     pl.max_units = call.rows / kTokens + call.batch;
     pl.ctas = sms;
-    plan_units_kernel<<<1, kPlanThreads, call.batch * sizeof(int32_t), stream>>>(pl);
+    cudaError_t e = launch_dependent(plan_units_kernel, 1, kPlanThreads, call.batch * sizeof(int32_t), stream, pl);
+    if (e != cudaSuccess) return e;
     ChunkPagedArgs a;
     a.kmap = kmap;
     a.vmap = vmap;
@@ -1093,8 +1098,7 @@ cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int
     a.cuts = pl.cuts;
     a.arrivals = pl.arrivals;
     a.partials = reinterpret_cast<float*>(ws + r.partials);
-    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, kSmemBytes, stream>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), sms, kThreads, kSmemBytes, stream, a);
 }
 
 }  // namespace gqa

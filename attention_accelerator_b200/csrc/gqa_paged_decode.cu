@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         prefetch_tensormap(&a.kmap);
         prefetch_tensormap(&a.vmap);
     }
+    dependency_wait();
+    allow_dependents();
     // Tiles of every sequence and their running sum.
     {
         const int per = (batch + kThreads - 1) / kThreads;
@@ -786,8 +788,7 @@ cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, in
     a.partials = reinterpret_cast<float*>(ws + kPagedPartialsOffset);
     a.stages = decode_stages(call.batch);
     const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (3 * (size_t)call.batch + 1) * 4;
-    kernel_for(code, call.cap > 0.f, call.slopes != nullptr)<<<sms, kThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), sms, kThreads, smem, stream, a);
 }
 
 cudaError_t paged_decode_prepare() {
