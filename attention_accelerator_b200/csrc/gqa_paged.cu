@@ -523,8 +523,8 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
     call->scale = p->scale;
     call->cap = p->score_cap;
     call->q_rotated = (p->flags & GQA_FLAG_Q_ROTATED) != 0;
-    // Key positions and tile counts are 32-bit.
-    if ((int64_t)p->table_width * c->page_len > 0x7FFFFFFF ||
+    // Key positions, a tile past them, and tile counts are 32-bit.
+    if ((int64_t)p->table_width * c->page_len > 1 << 30 ||
         (int64_t)p->batch * p->table_width * (c->page_len / 32 + 1) > 0x7FFFFFFF)
         return GQA_ERR_BATCH;
     return check_device_memory({q, out, c->k, c->v, c->k_scale, c->v_scale, p->block_table, p->seq_lens,

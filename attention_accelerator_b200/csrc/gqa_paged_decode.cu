@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             if (lane == 0) {
                 slot.lo = r.lo;
                 slot.hi = r.hi;
-                slot.m = (int)m;
+                slot.m = (int)max(m, -(int64_t)(1 << 30));  // (distances stay 32-bit)
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.qfull[sl]);

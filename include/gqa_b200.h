@@ -564,7 +564,8 @@ int gqa_read_paged(const gqa_paged_cache *cache, const int64_t *slots, int n, vo
  * scale reaches a row only through a visible key.  Scales are not negative, and
  * visible codes are numbers (gqa_append_paged writes no e4m3 NaN; the value read
  * for one is unspecified).  Page numbers outside
- * [0, pages) read as zeros, and no key at or past table_width * page_len is visible.
+ * [0, pages) read as zeros, and no key at or past table_width * page_len (2^30 at
+ * most) is visible.
  */
 typedef struct gqa_paged_params {
     int32_t batch;               /* 1..GQA_PAGED_MAX_BATCH */
@@ -589,7 +590,9 @@ typedef struct gqa_paged_params {
 } gqa_paged_params;
 
 /* Device workspace of either call, on the current device (0 on invalid input):
- * zero at allocation, kept between calls, used by the paged calls of one stream only. */
+ * zero at allocation, kept between calls, used by the paged calls of one stream only.
+ * Its first word is the status word of gqa_read_status; after a timed-out wait set
+ * all of it to zero again. */
 size_t gqa_paged_workspace_bytes(const gqa_paged_cache *cache, const gqa_paged_params *p);
 
 /* One query a sequence: q, out [batch][4 * kv_heads][128]. */

@@ -112,7 +112,7 @@ def test_c_refuses_bad_caches(name, change, want):
 @pytest.mark.parametrize("change,want", [
     (dict(block_table=None), "NULL_POINTER"), (dict(seq_lens=None), "NULL_POINTER"), (dict(batch=0), "BATCH"),
     (dict(batch=8193, rows=8193), "BATCH"), (dict(rows=-1), "BATCH"), (dict(table_width=0), "BATCH"),
-    (dict(table_stride=2), "BATCH"), (dict(reserved=1), "BATCH"), (dict(flags=1), "FLAGS"), (dict(flags=2), "FLAGS"),
+    (dict(table_stride=2), "BATCH"), (dict(table_width=(1 << 26) + 1, table_stride=1 << 27), "BATCH"), (dict(reserved=1), "BATCH"), (dict(flags=1), "FLAGS"), (dict(flags=2), "FLAGS"),
     (dict(scale=0.0), "SCALE"), (dict(scale=math.nan), "SCALE"), (dict(score_cap=-1.0), "SCALE"),
     (dict(score_cap=math.inf), "SCALE"), (dict(rope_theta=0.0), "ROPE_THETA"), (dict(q_row_stride=4), "ALIGNMENT"),
     (dict(out_head_stride=-128), "ALIGNMENT")])

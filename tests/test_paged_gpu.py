@@ -645,6 +645,74 @@ def test_calls_of_different_sizes_share_a_workspace():
         check(got[pick], q[pick], s, pick, [s.lens[i] - 1 for i in pick], unit=DECODE_UNIT)
 
 
+def test_nothing_visible_at_all():
+    lens = [70, 0, 200]
+    s = Setup(lens, seed=41, page_len=16, code="e4m3")
+    q = s.queries(3)
+    out = torch.full((3, 32, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    gqa.decode_paged(q, s.cache, ints(s.table), ints(lens), doc_starts=ints([70, 0, 900]), out=out)
+    assert not out.any()
+    first = [0, 70, 70, 150]
+    q = s.queries(150)
+    out = torch.full((150, 32, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first), doc_starts=ints([300] * 150), out=out)
+    assert not out.any()
+    out = torch.full((150, 32, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints([0, 0, 0, 0]), out=out)
+    assert bool((out == 5.0).all())  # no sequence has a query
+
+
+def test_first_query_is_kept_within_the_rows():
+    """Numbers in first_query that name rows the call does not have are cut to those it has."""
+    lens = [100, 100]
+    s = Setup(lens, seed=42, page_len=32)
+    q = s.queries(10)
+    guard = torch.full((30, 32, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    for first in ([0, 4, 1 << 30], [-7, 4, 10], [0, 12, 11], [10, 4, 2]):
+        gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first), out=guard[10:20])
+        assert bool((guard[:10] == 5.0).all()) and bool((guard[20:] == 5.0).all())
+    assert gqa.read_device_status() == 0
+
+
+def test_two_streams_at_once():
+    """Calls on two streams have workspaces of their own."""
+    setups = [Setup(lens, seed=50 + i, page_len=64) for i, lens in enumerate(([5000, 300] * 8, [900, 2000, 40] * 6))]
+    work, want = [], []
+    for s in setups:
+        n = len(s.lens)
+        first = [0]
+        for length in s.lens:
+            first.append(first[-1] + min(length, 40))
+        work.append((s, s.queries(n), s.queries(first[-1]), ints(s.table), ints(s.lens), ints(first)))
+    run = lambda s, q, qc, t, n, f: (gqa.decode_paged(q, s.cache, t, n),  # noqa: E731
+                                     gqa.decode_paged_chunked(qc, s.cache, t, n, f))
+    want = [run(*w) for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[] for _ in work]
+    for _ in range(10):
+        for i, (w, st) in enumerate(zip(work, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(run(*w))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for pair in g:
+            for a, b in zip(pair, w):
+                assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_the_largest_batch():
+    lens = [(i * 53) % 40 for i in range(8192)]
+    s = Setup(lens, seed=31, page_len=16, heads=1)
+    q = s.queries(8192)
+    got = gqa.decode_paged(q, s.cache, ints(s.table), ints(lens))
+    pick = list(range(0, 8192, 409)) + [8191]
+    check(got[pick], q[pick], s, pick, [lens[i] - 1 for i in pick], unit=DECODE_UNIT)
+    rows = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(list(range(8193))))
+    check(rows[pick], q[pick], s, pick, [lens[i] - 1 for i in pick], unit=CHUNK_UNIT)
+    assert gqa.read_device_status() == 0
+
+
 def test_many_sequences():
     lens = [(i * 37) % 150 for i in range(1500)]
     s = Setup(lens, seed=30, page_len=16, code="e4m3", heads=2)
