@@ -22,6 +22,9 @@ namespace {
 // given back in this very call or from below them on the stack, so no CTA reads
 // what another writes.  lens_out and n_free_out may be the inputs: the last CTA
 // to have read those writes them.
+//
+// Bound by latency: two chains of loads, the sums' barriers and the search, 9 us
+// for 64 requests, 11 for 1024 with 66 thousand tokens (1.6 MB).
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -197,6 +200,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
 // are resident at once; a longer run is then read a second time.
 // K's rotation factors cost more than anything else here (one sine and cosine a
 // pair): a call of many tokens computes them once for all heads of a run.
+// Measured: 18000 rows in pages of 32 42 us (111 MB, 2.6 TB/s: the factors, the
+// maximum's barrier and the two passes' latency), in pages of 64, e4m3, 45 us, of 128
+// 60 us (fewer CTAs an SM); a step's 64 rows 3.8 us, bound by latency.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     PagedCacheView c;
@@ -398,7 +404,8 @@ __global__ void __launch_bounds__(kOnce ? 4 * kPagedMaxPage : 64) append_kernel(
     }
 }
 
-// Rows back to BF16: a thread 16 codes of one (row, head), of K or V.
+// Rows back to BF16: a thread 16 codes of one (row, head), of K or V.  18000 rows
+// 21 us (111 MB, 5.2 TB/s), 64 rows 4.5 us.
 struct ReadArgs {
     PagedCacheView c;
     const int64_t* slots;

@@ -123,4 +123,36 @@ __device__ __forceinline__ uint32_t value_codes4(float y0, float y1, float y2, f
     }
 }
 
+// Four codes of a word to two FP16 pairs, exactly.
+template <int kCode>
+__device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (kCode == GQA_CODE_INT8) {
+        // 1024 + (c + 128) is the FP16 number 0x6400 | byte; minus 1152 it is c.
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
+        const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
+        lo = *reinterpret_cast<const uint32_t*>(&a);
+        hi = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// tanh to about 2^-22: 1 - 2 / (e^2x + 1).
+__device__ __forceinline__ float tanh_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * 2.8853900817779268f) + 1.f));
+    return fmaf(-2.f, r, 1.f);
+}
+
 }  // namespace gqa

@@ -32,6 +32,18 @@
 //              run while the other's softmax does.
 //   13         loader: table entries, scales, TMA.
 //   14         zeros of units whose rows see nothing.
+//
+// Bound, for long contexts, by a tile's chain: the softmax of 2 x 128 rows (about
+// 2500 cycles), the conversion of K and V (1400 each) and the products (2000)
+// overlap to a period of 4700 cycles; the tensor pipe is 40 % busy.  For short
+// ones, by the 25 to 28 thousand cycles a unit costs beside its tiles; for a few
+// drafted tokens, by the same chain with most rows empty.  Measured (B200, e4m3):
+// 16 x 128 queries on 8192 keys 309 us (883 TFLOP/s, 55 % of the cuBLAS rate;
+// 350 us under the power limit), one prompt of 8192 597 us (922 TFLOP/s), 48 x 5
+// queries on 2000 to 4000 keys 230 us (409 MB).  Each took longer: Q prepared by the
+// conversion warps (371 us, spills), two passes over S at fewer registers (354), a
+// polynomial tanh (355, capped), both M tiles on alternate tiles of few queries
+// (281 against 237, and 9 % off the rest).
 #include "gqa_internal.h"
 #include "gqa_paged.cuh"
 #include "gqa_paged_internal.h"
@@ -312,24 +324,6 @@ __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map,
         : "memory");
 }
 
-template <int kCode>
-__device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if constexpr (kCode == GQA_CODE_INT8) {
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
-        const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
-        lo = *reinterpret_cast<const uint32_t*>(&a);
-        hi = *reinterpret_cast<const uint32_t*>(&b);
-    } else {
-        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-            : "=r"(lo), "=r"(hi)
-            : "r"(w));
-    }
-}
-
 // V's operand: codes times their scale.  A NaN code would reach, times a weight of
 // zero, the rows that do not see its key: the maximum with -448 makes it a number.
 template <int kCode>
@@ -340,21 +334,10 @@ __device__ __forceinline__ uint32_t scale_half2(uint32_t a, __half2 b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 // tanh(x) / x = sum of kTanh[i] x^2i for |x| <= 1/2, within 2^-15 of it (a quarter of
 // what a weight's rounding to FP16 moves at a score of 4): interpolated at the
 // Chebyshev points of x^2.
 __device__ constexpr float kTanh[3] = {0.99997777f, -0.33170217f, 0.11525216f};
-
-__device__ __forceinline__ float tanh_fast(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * 2.8853900817779268f) + 1.f));
-    return fmaf(-2.f, r, 1.f);
-}
 
 __device__ __forceinline__ float finite_or(float x, float other) {
     return fabsf(x) <= 3.402823466e38f ? x : other;

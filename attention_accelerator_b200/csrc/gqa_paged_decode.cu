@@ -1,7 +1,11 @@
 // gqa_paged_decode.cu -- one token a sequence over the paged 8-bit cache.
 //
+//   out[h] = sum_p softmax_p(z)[p] V[p],  z[p] = scale * (Q[h] . K[p]) * k_scale[page of p],
+// capped, biased and masked as gqa_b200.h says, in one pass over the visible keys
+// with a running maximum and sum a warp.
+//
 // Work.  A unit is one (sequence, KV head); its visible keys are cut into tiles
-// of 64 on a grid of absolute positions.  All tiles of all units, in order, are
+// of 32 on a grid of absolute positions.  All tiles of all units, in order, are
 // dealt out evenly: CTA i of G (one per SM) takes tiles [T i / G, T (i + 1) / G),
 // whatever the lengths -- which only the GPU knows, so every CTA first sums the
 // sequences' tiles itself.  A unit inside one CTA's share is written out by it; a
@@ -9,11 +13,14 @@
 // the last of its CTAs to finish merges them in CTA order, so that results do not
 // depend on which one that is.
 //
-// A CTA is 8 consumer warps, a loader warp and a query warp.
-//   loader   block-table entries and scales 32 pages at a time, one a lane; per
-//            tile one TMA box per page of K and of V (64 rows of 128 codes in
-//            all, 128-byte swizzle) into a ring of 16 KB stages, and the pages'
-//            scales beside them.  Pages with no visible key are not loaded.
+// A CTA is 8 consumer warps, 2 loader warps, a query warp and 4 finisher warps.
+//   loader   four tiles at a time, every second four each: the block-table
+//            entries and scales of their pages (two pages a tile at most), then
+//            a TMA box per page of K and of V (32 rows of 128 codes in all,
+//            128-byte swizzle) into a ring of 8 KB stages, 24 deep, and the
+//            pages' scales beside them.  Pages with no visible key are not
+//            loaded.  A stage belongs to one loader and one consumer warp, so
+//            that no one waits for a phase that another has passed.
 //   query    per unit, the 4 Q rows rotated in FP32, divided by a power of two
 //            that brings the row's largest below 1, and split into two FP16
 //            parts (22 bits): 8 columns, the N of an m16n8k16 product.
@@ -26,9 +33,21 @@
 //            FP16 parts again, and movmatrix turns them into the other product's
 //            operand: O^T = V^T P^T, M 16 dims, whose operand lanes build from
 //            the 16-byte pieces of 4 keys by byte permutes.
+//   finisher one a Q head: joins the consumers' rows of a unit and writes it, or
+//            its partial, while the consumers are at the next unit.
 // Why mma.sync and not tcgen05: with 4 queries a KV head there is nothing to
 // amortise a 16-bit copy of K and V in shared memory over; here a code goes from
 // its 8-bit stage through registers into the product once.
+//
+// Bound by HBM for long contexts, by the chain length -> table entry -> page ->
+// product -> merge for short ones.  Measured (B200, int8, page 16 to 64): 64
+// ragged sequences, 586 MB, 96 us: 6.1 TB/s, 94 % of the copy rate; 148 of 4096
+// keys 188 us (6.6 TB/s); one of 131072 keys 49 us (5.5 TB/s), of 4096 12.4 us,
+// of 30 5.9 us.  32 sequences read 294.8 MB of DRAM, the codes and no more, at
+// 18 % of the tensor pipe and 38 % of the issue slots.  Tiles of 64 keys, half as
+// many, left the ring too coarse for the short shares (one of 131072: 53 us); one
+// loader warp needed 700 cycles a tile, more than the consumers; 10 to 13 consumer
+// warps do not fit the registers.
 #include "gqa_internal.h"
 #include "gqa_paged.cuh"
 #include "gqa_paged_internal.h"
@@ -157,38 +176,6 @@ struct Walk {
         return true;
     }
 };
-
-// Four codes of a word to two FP16 pairs, exactly.
-template <int kCode>
-__device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if constexpr (kCode == GQA_CODE_INT8) {
-        // 1024 + (c + 128) is the FP16 number 0x6400 | byte; minus 1152 it is c.
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
-        const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
-        lo = *reinterpret_cast<const uint32_t*>(&a);
-        hi = *reinterpret_cast<const uint32_t*>(&b);
-    } else {
-        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-            : "=r"(lo), "=r"(hi)
-            : "r"(w));
-    }
-}
-
-// tanh to about 2^-22: 1 - 2 / (e^2x + 1).
-__device__ __forceinline__ float tanh_fast(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * 2.8853900817779268f) + 1.f));
-    return fmaf(-2.f, r, 1.f);
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 
 // Running state of a consumer warp for the current unit.  Lane (g, t) = (lane / 4,
 // lane % 4): head t's maximum and sum (the sum over this lane's keys only), and
