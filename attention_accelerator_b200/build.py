@@ -17,9 +17,9 @@ INCLUDE = ROOT / "include"
 LIB = PKG / "lib" / "libgqa_b200.so"
 SOURCES = [CSRC / "gqa_abi.cu", CSRC / "gqa_decode.cu", CSRC / "gqa_noalloc.cu", CSRC / "gqa_chunked.cu", CSRC / "gqa_peer.cu",
            CSRC / "gqa_memfile.cu", CSRC / "gqa_rtl.cu", CSRC / "gqa_paged.cu",
-           CSRC / "gqa_paged_decode.cu", CSRC / "gqa_paged_chunk.cu"]
+           CSRC / "gqa_paged_decode.cu", CSRC / "gqa_paged_chunk.cu", CSRC / "gqa_paged_few.cu"]
 HEADERS = [INCLUDE / "gqa_b200.h", CSRC / "gqa_device.cuh", CSRC / "gqa_internal.h", CSRC / "gqa_tcgen05.cuh", CSRC / "gqa_paged.cuh",
-           CSRC / "gqa_paged_internal.h"]
+           CSRC / "gqa_paged_internal.h", CSRC / "gqa_paged_units.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

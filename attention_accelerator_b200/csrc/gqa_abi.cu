@@ -82,7 +82,8 @@ int current_device(int* sms) {
         if (major != 10 || minor != 0) {
             di.status = GQA_ERR_UNSUPPORTED_DEVICE;
         } else if (gqa::decode_prepare(dev) != cudaSuccess || gqa::chunked_prepare() != cudaSuccess ||
-                   gqa::paged_decode_prepare() != cudaSuccess || gqa::paged_chunk_prepare() != cudaSuccess) {
+                   gqa::paged_decode_prepare() != cudaSuccess || gqa::paged_chunk_prepare() != cudaSuccess ||
+                   gqa::paged_few_prepare() != cudaSuccess) {
             di.status = GQA_ERR_CUDA;
         }
         di.sms = n;

@@ -23,6 +23,7 @@ int device_sms(int* sms);
 
 cudaError_t paged_decode_prepare();
 cudaError_t paged_chunk_prepare();
+cudaError_t paged_few_prepare();
 
 struct DecodeArgs;
 struct RopeTable;

@@ -4,6 +4,7 @@
 #include "gqa_internal.h"
 #include "gqa_paged_internal.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -541,7 +542,9 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
 int launched() { return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA; }
 
 size_t workspace_of(int batch, int rows, int heads, bool chunked, int sms) {
-    return chunked ? paged_chunk_workspace(batch, rows, heads, sms) : paged_decode_workspace(sms);
+    if (!chunked) return paged_decode_workspace(sms);
+    const size_t few = paged_few_takes(batch, rows) ? paged_few_workspace(batch, rows, sms) : 0;
+    return std::max(few, paged_chunk_workspace(batch, rows, heads, sms));
 }
 
 int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p, void* workspace,
@@ -558,15 +561,17 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     if (st != GQA_OK) return st;
     if (p->rows == 0) return GQA_OK;
     const RopeSteps& rope = rope_steps_of(p->rope_theta);
-    const int tile = chunked ? paged_chunk_tile() : paged_decode_tile();
+    const bool few = chunked && paged_few_takes(p->batch, p->rows);
+    const int tile = few ? paged_few_tile() : chunked ? paged_chunk_tile() : paged_decode_tile();
     CUtensorMap kmap, vmap;
     if ((st = paged_map(&kmap, call.c.k, call.c, tile)) != GQA_OK ||
         (st = paged_map(&vmap, call.c.v, call.c, tile)) != GQA_OK)
         return st;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = chunked ? launch_paged_chunk(call, rope, cache->code, kmap, vmap, sms, ws, s)
-                                  : launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, s);
+    const cudaError_t e = few       ? launch_paged_few(call, rope, cache->code, kmap, vmap, sms, ws, s)
+                          : chunked ? launch_paged_chunk(call, rope, cache->code, kmap, vmap, sms, ws, s)
+                                    : launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, s);
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 

@@ -47,6 +47,7 @@
 #include "gqa_internal.h"
 #include "gqa_paged.cuh"
 #include "gqa_paged_internal.h"
+#include "gqa_paged_units.cuh"
 #include "gqa_tcgen05.cuh"
 
 namespace gqa {
@@ -79,20 +80,9 @@ constexpr int kSlotFloats = kRowsM * 2 * (kHeadDim + 2);  // a partial: acc [32]
 constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescO = kIdescS | (1u << 16);  // B (V) MN-major
 
-struct Unit {
-    int32_t b, row0, n, pos0;     // sequence, first query row, queries, position of the first
-    int32_t lo, hi, tiles, tile0; // keys that any row sees, their tiles
-    int64_t first, cell;          // tiles and cost of all units before it (per head)
-};
-struct Meta {
-    int64_t total;  // tiles of all units and heads
-    int32_t ctas;   // with a share
-    int32_t units;
-};
 // What a unit costs a CTA beside its tiles (queries, the pipeline's start and
 // end, its rows), in tiles: measured at 25-28 thousand cycles to a tile's 5.
 constexpr int kUnitCost = 5;
-constexpr int kMaxCtas = 255;
 
 struct TileScales {
     float k[8], v[8];   // of each 16 keys: K's scale (NaN where V's is no number), V's over the reference
@@ -126,12 +116,9 @@ struct alignas(64) ChunkPagedArgs {
 
 struct PlanUnitsArgs {
     PagedCall p;
-    Meta* meta;
-    Unit* units;
-    int32_t* starts;
-    int64_t* cuts;
-    uint32_t* arrivals;
-    int32_t max_units, ctas;
+    UnitPlan to;
+    int32_t tokens, tile_shift, unit_cost;  // queries of a unit, keys of a tile (log2), what a unit costs in tiles
+    int32_t max_units, ctas, counters;      // counters to zero (0: two a unit and head)
 };
 
 // ---------------------------------------------------------------------------
@@ -188,13 +175,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     longlong2 sum = make_longlong2(0, 0), all;
     for (int b = b0; b < b1; ++b) {
         int row0;
-        sum.x += (rows_of(b, row0) + kTokens - 1) / kTokens;
+        sum.x += (rows_of(b, row0) + a.tokens - 1) / a.tokens;
     }
     int64_t at = scan_exclusive(sum, warp_sum, &all).x;
     for (int b = b0; b < b1; ++b) {
         int row0;
         offset[b] = (int)at;
-        at += (rows_of(b, row0) + kTokens - 1) / kTokens;
+        at += (rows_of(b, row0) + a.tokens - 1) / a.tokens;
     }
     const int units = (int)min((int64_t)all.x, (int64_t)a.max_units);
     __syncthreads();
@@ -207,8 +194,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
         }
         const int b = lo_b;  // (of sequences that share an offset the last: the one with rows)
         int row0;
-        const int rows = rows_of(b, row0), skip = (u - offset[b]) * kTokens;
-        const int n = min(kTokens, rows - skip), len = paged_length(p, b);
+        const int rows = rows_of(b, row0), skip = (u - offset[b]) * a.tokens;
+        const int n = min(a.tokens, rows - skip), len = paged_length(p, b);
         const int64_t pos0 = (int64_t)p.seq_lens[b] - rows + skip;
         int lo = 0x7fffffff, hi = 0;
         for (int i = lane; i < n; i += 32) {
@@ -228,35 +215,35 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
             x.pos0 = (int)pos0;
             x.lo = lo;
             x.hi = hi;
-            x.tile0 = hi > 0 ? lo >> kTileShift : 0;
-            x.tiles = hi > 0 ? ((hi + kTile - 1) >> kTileShift) - x.tile0 : 0;
+            x.tile0 = hi > 0 ? lo >> a.tile_shift : 0;
+            x.tiles = hi > 0 ? ((hi + (1 << a.tile_shift) - 1) >> a.tile_shift) - x.tile0 : 0;
             x.first = x.cell = 0;
-            a.units[u] = x;
+            a.to.units[u] = x;
         }
     }
     __syncthreads();
     const int heads = p.c.kv_heads;
     const int uper = (units + kPlanThreads - 1) / kPlanThreads;
     const int u0 = min(units, tid * uper), u1 = min(units, u0 + uper);
-    // Shares are cut evenly in cost: a unit's cells are kUnitCost of its own, then one for each tile.
+    // Shares are cut evenly in cost: a unit's cells are a.unit_cost of its own, then one for each tile.
     sum = make_longlong2(0, 0);
     for (int u = u0; u < u1; ++u) {
-        const int tiles = a.units[u].tiles;
+        const int tiles = a.to.units[u].tiles;
         sum.x += tiles;
-        sum.y += tiles ? tiles + kUnitCost : 0;
+        sum.y += tiles ? tiles + a.unit_cost : 0;
     }
     longlong2 here = scan_exclusive(sum, warp_sum, &all);
     const int64_t total = all.x * heads, cost = all.y * heads;
     for (int u = u0; u < u1; ++u) {
-        const int tiles = a.units[u].tiles;
-        a.units[u].first = here.x;
-        a.units[u].cell = here.y;
+        const int tiles = a.to.units[u].tiles;
+        a.to.units[u].first = here.x;
+        a.to.units[u].cell = here.y;
         here.x += tiles;
-        here.y += tiles ? tiles + kUnitCost : 0;
+        here.y += tiles ? tiles + a.unit_cost : 0;
     }
     __syncthreads();
-    // Shares longer than kUnitCost: each has a tile.
-    const int64_t G = min((int64_t)a.ctas, cost / (kUnitCost + 1));
+    // Shares longer than a.unit_cost: each has a tile.
+    const int64_t G = min((int64_t)a.ctas, cost / (a.unit_cost + 1));
     if (tid <= G) {
         int64_t cut = total;
         if (tid < G) {
@@ -264,57 +251,19 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
             int lo = 0, hi = units;  // (of units that share a cell the last: the one with tiles)
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (a.units[mid].cell * heads <= c) lo = mid; else hi = mid;
+                if (a.to.units[mid].cell * heads <= c) lo = mid; else hi = mid;
             }
-            const Unit x = a.units[lo];
-            const int64_t each = x.tiles + kUnitCost, off = c - x.cell * heads, h = off / each, t = off - h * each - kUnitCost;
-            a.starts[tid] = lo;
+            const Unit x = a.to.units[lo];
+            const int64_t each = x.tiles + a.unit_cost, off = c - x.cell * heads, h = off / each, t = off - h * each - a.unit_cost;
+            a.to.starts[tid] = lo;
             cut = x.first * heads + h * x.tiles + (t > 0 ? t : 0);
         }
-        a.cuts[tid] = cut;
+        a.to.cuts[tid] = cut;
     }
-    for (int i = tid; i < units * heads * 2; i += kPlanThreads) a.arrivals[i] = 0;
-    if (tid == 0) *a.meta = Meta{total, (int32_t)G, units};
+    const int counters = a.counters ? a.counters : units * heads * 2;
+    for (int i = tid; i < counters; i += kPlanThreads) a.to.arrivals[i] = 0;
+    if (tid == 0) *a.to.meta = Meta{total, (int32_t)G, units};
 }
-
-// ---------------------------------------------------------------------------
-// A CTA's walk through its share, one unit's piece at a time.
-// ---------------------------------------------------------------------------
-struct Walk {
-    int64_t x, end;
-    int u, h, j, n;  // unit, KV head, first tile within the unit and tiles of the piece
-    Unit unit;
-    __device__ __forceinline__ void start(const ChunkPagedArgs& a, const Meta& meta) {
-        n = 0;
-        const int me = blockIdx.x;
-        if (me >= meta.ctas) return;
-        x = a.cuts[me];
-        end = a.cuts[me + 1];
-        u = a.starts[me];
-        unit = a.units[u];
-        const int64_t rem = x - unit.first * a.p.c.kv_heads;
-        h = (int)(rem / unit.tiles);
-        place(a);
-    }
-    __device__ __forceinline__ int64_t unit_first(const ChunkPagedArgs& a) const {
-        return unit.first * a.p.c.kv_heads + (int64_t)h * unit.tiles;
-    }
-    __device__ __forceinline__ void place(const ChunkPagedArgs& a) {
-        j = (int)(x - unit_first(a));
-        n = (int)min((int64_t)(unit.tiles - j), end - x);
-    }
-    __device__ __forceinline__ bool next(const ChunkPagedArgs& a) {
-        x += n;
-        if (x >= end) return false;
-        if (++h == a.p.c.kv_heads) {
-            h = 0;
-            do unit = a.units[++u];
-            while (unit.tiles == 0);
-        }
-        place(a);
-        return true;
-    }
-};
 
 __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int head, int page, uint64_t* bar) {
     asm volatile(
@@ -1017,24 +966,17 @@ Kernel kernel_for(int code, bool cap, bool bias) {
     return bias ? paged_chunk_kernel<1, false, true> : paged_chunk_kernel<1, false, false>;
 }
 
-// Layout behind the counters that the decode keeps; everything here is written by each call.
-struct Regions {
-    size_t starts, cuts, units, arrivals, partials, end;
-};
-Regions regions(int batch, int rows, int heads, int sms) {
-    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    const size_t units = (size_t)rows / kTokens + batch;
-    Regions r;
-    r.starts = kPagedPartialsOffset + 256;  // (Meta first)
-    r.cuts = r.starts + up((size_t)sms * sizeof(int32_t));
-    r.units = r.cuts + up((size_t)(sms + 1) * sizeof(int64_t));
-    r.arrivals = r.units + up(units * sizeof(Unit));
-    r.partials = r.arrivals + up(units * heads * 2 * sizeof(uint32_t));
-    r.end = r.partials + (size_t)sms * 2 * kSlotFloats * sizeof(float);
-    return r;
+UnitRegions regions(int batch, int rows, int heads, int sms) {
+    return unit_regions(batch, rows, kTokens, (size_t)heads * 2, sms, (size_t)sms * 2 * kSlotFloats * sizeof(float));
 }
 
 }  // namespace
+
+cudaError_t launch_plan_units(const PagedCall& call, const UnitPlan& to, int tokens, int tile_shift, int unit_cost,
+                              int counters, int ctas, cudaStream_t stream) {
+    const PlanUnitsArgs a{call, to, tokens, tile_shift, unit_cost, call.rows / tokens + call.batch, ctas, counters};
+    return launch_dependent(plan_units_kernel, 1, kPlanThreads, call.batch * sizeof(int32_t), stream, a);
+}
 
 int paged_chunk_tile() { return kTile; }
 
@@ -1057,17 +999,9 @@ cudaError_t paged_chunk_prepare() {
 cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
                                const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
     if (sms > kMaxCtas) sms = kMaxCtas;
-    const Regions r = regions(call.batch, call.rows, call.c.kv_heads, sms);
-    PlanUnitsArgs pl;
-    pl.p = call;
-    pl.meta = reinterpret_cast<Meta*>(ws + kPagedPartialsOffset);
-    pl.units = reinterpret_cast<Unit*>(ws + r.units);
-    pl.starts = reinterpret_cast<int32_t*>(ws + r.starts);
-    pl.cuts = reinterpret_cast<int64_t*>(ws + r.cuts);
-    pl.arrivals = reinterpret_cast<uint32_t*>(ws + r.arrivals);
-    pl.max_units = call.rows / kTokens + call.batch;
-    pl.ctas = sms;
-    cudaError_t e = launch_dependent(plan_units_kernel, 1, kPlanThreads, call.batch * sizeof(int32_t), stream, pl);
+    const UnitRegions r = regions(call.batch, call.rows, call.c.kv_heads, sms);
+    const UnitPlan pl = unit_plan(r, ws);
+    const cudaError_t e = launch_plan_units(call, pl, kTokens, kTileShift, kUnitCost, 0, sms, stream);
     if (e != cudaSuccess) return e;
     ChunkPagedArgs a;
     a.kmap = kmap;
