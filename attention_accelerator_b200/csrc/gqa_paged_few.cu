@@ -41,7 +41,7 @@ constexpr int kSteps = kTile / 16;
 constexpr int kHalfBytes = kTile * kHeadDim;
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 2 * kWarps;
-constexpr int kUnitCost = 4;
+constexpr int kUnitCost = 16;
 constexpr int kRowF = kHeadDim + 4;    // padded row
 constexpr int kUnitRows = kTokens * kGroup;
 // Weights are 2^(z - m) with z up to 8 above the reference m, times a page's V scale
@@ -109,59 +109,83 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     const int sh = min(page_shift, kTileShift) - 4;
     float z[kN][kSteps][4];  // [key g or g + 8][query], as the product leaves them
     {
+        // Both steps' products side by side: each is a chain of eight.
         const uint8_t* k = stage + g * kHeadDim;
         const int c0 = ((2 * t) ^ g) << 4, c1 = ((2 * t + 1) ^ g) << 4;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int n = 0; n < kN; ++n)
+            for (int i = 0; i < kSteps; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[n][i][e] = 0.f;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int c = half ? c1 : c0;
-                const uint4 a = lds128(k + (16 * i) * kHeadDim + c), b = lds128(k + (16 * i + 8) * kHeadDim + c);
-                const uint32_t up[4] = {a.x, a.y, a.z, a.w}, dn[4] = {b.x, b.y, b.z, b.w};
+        for (int half = 0; half < 2; ++half) {
+            uint4 up[kSteps], dn[kSteps];
 #pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    uint32_t x[8];
-                    to_half4<kCode>(up[2 * f], x[0], x[2]);
-                    to_half4<kCode>(dn[2 * f], x[1], x[3]);
-                    to_half4<kCode>(up[2 * f + 1], x[4], x[6]);
-                    to_half4<kCode>(dn[2 * f + 1], x[5], x[7]);
+            for (int i = 0; i < kSteps; ++i) {
+                up[i] = lds128(k + (16 * i) * kHeadDim + (half ? c1 : c0));
+                dn[i] = lds128(k + (16 * i + 8) * kHeadDim + (half ? c1 : c0));
+            }
 #pragma unroll
-                    for (int n = 0; n < kN; ++n) {
-                        const uint4 q = lds128(&slot.q[n][2 * half + f][lane]);
-                        mma_16x8x16(z[n][i], x[0], x[1], x[2], x[3], q.x, q.y);
-                        mma_16x8x16(z[n][i], x[4], x[5], x[6], x[7], q.z, q.w);
+            for (int f = 0; f < 2; ++f) {
+                uint4 q[kN];
+#pragma unroll
+                for (int n = 0; n < kN; ++n) q[n] = lds128(&slot.q[n][2 * half + f][lane]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        uint32_t x[4];
+                        to_half4<kCode>(f ? e ? up[i].w : up[i].z : e ? up[i].y : up[i].x, x[0], x[2]);
+                        to_half4<kCode>(f ? e ? dn[i].w : dn[i].z : e ? dn[i].y : dn[i].x, x[1], x[3]);
+#pragma unroll
+                        for (int n = 0; n < kN; ++n)
+                            mma_16x8x16(z[n][i], x[0], x[1], x[2], x[3], e ? q[n].z : q[n].x, e ? q[n].w : q[n].y);
                     }
-                }
             }
         }
     }
     const bool edge = key0 < slot.lo_most || key0 + kTile > slot.hi_least;  // of the whole warp
-    bool above = false;
+    // Where a query does not see a key, in one branch of the whole warp.
+    auto blank = [&](float x) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int lo = slot.lo[2 * n + e] - key0 - g, hi = slot.hi[2 * n + e] - key0 - g;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (16 * i + 8 * u < lo || 16 * i + 8 * u >= hi) z[n][i][2 * u + e] = x;
+            }
+    };
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
         const float2 factor = *reinterpret_cast<const float2*>(&slot.factor[n][2 * t]);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const float f = i >> sh ? sc.y : sc.x;
+            const float f = i >> sh ? sc.y : sc.x, f0 = f * factor.x, f1 = f * factor.y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = z[n][i][e] * (f * (e & 1 ? factor.y : factor.x));
+                float x = z[n][i][e] * (e & 1 ? f1 : f0);
                 if constexpr (kCap) x = cap2 * tanh_fast(x);
                 if constexpr (kBias)
                     x = fmaf(-slot.slope[t], fabsf((float)(slot.m + 2 * n + (e & 1) - (key0 + 16 * i + 8 * (e >> 1) + g))), x);
-                if (edge) {
-                    const int key = key0 + 16 * i + 8 * (e >> 1) + g, q = 2 * n + (e & 1);
-                    if (key < slot.lo[q] || key >= slot.hi[q]) x = -INFINITY;
-                }
                 z[n][i][e] = x;
-                above |= x > st.m[n][e & 1] + kHeadroom;
             }
         }
     }
+    if (edge) blank(-INFINITY);
+    float mx[kN][2];  // of this lane's keys
+    bool above = false;
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            mx[n][e] = fmaxf(fmaxf(z[n][0][e], z[n][0][2 + e]), fmaxf(z[n][1][e], z[n][1][2 + e]));
+            above |= mx[n][e] > st.m[n][e] + kHeadroom;
+        }
     // V scales: where a page's passes the running power of two, that grows.
     float vmax = 0.f;
     if (fabsf(sc.z) <= 3.402823466e38f) vmax = fabsf(sc.z);
@@ -182,12 +206,9 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
             float f[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float mx = fmaxf(z[n][0][e], z[n][0][2 + e]);
+                float m_new = fmaxf(st.m[n][e], mx[n][e]);
 #pragma unroll
-                for (int i = 1; i < kSteps; ++i) mx = fmaxf(mx, fmaxf(z[n][i][e], z[n][i][2 + e]));
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                const float m_new = fmaxf(st.m[n][e], mx);
+                for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
                 const float alpha = fast_exp2(st.m[n][e] - (m_new == -INFINITY ? 0.f : m_new));
                 st.m[n][e] = m_new;
                 st.l[n][e] *= alpha;
@@ -199,52 +220,53 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                 for (int e = 0; e < 4; ++e) st.o[n][i][e] *= f[e & 1];
         }
     }
-    uint32_t w[kN][kSteps][2];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
         const float m0 = st.m[n][0] == -INFINITY ? 0.f : st.m[n][0], m1 = st.m[n][1] == -INFINITY ? 0.f : st.m[n][1];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const float r = (i >> sh ? sc.w : sc.z) * st.vinv;
-            float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float y = fast_exp2(z[n][i][e] - (e & 1 ? m1 : m0));
                 st.l[n][e & 1] += y;
-                x[e] = y * r;
-                if (edge && z[n][i][e] == -INFINITY) x[e] = 0.f;  // not NaN, whatever the page's scale
+                z[n][i][e] = y * r;
             }
-            w[n][i][0] = transpose_8x8(pack_half2(x[0], x[1]));
-            w[n][i][1] = transpose_8x8(pack_half2(x[2], x[3]));
         }
     }
+    if (edge) blank(0.f);  // not NaN, whatever the page's scale
+    uint32_t w[kN][kSteps][2];
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) w[n][i][u] = transpose_8x8(pack_half2(z[n][i][2 * u], z[n][i][2 * u + 1]));
     const uint8_t* v = stage + kHalfBytes;
     const int r0 = 2 * t * kHeadDim + ((g ^ (2 * t)) << 4), r1 = (2 * t + 1) * kHeadDim + ((g ^ (2 * t + 1)) << 4);
-    // A code that no query sees may be e4m3's NaN: -448 in its place.
-    auto number = [&](uint32_t x) {
-        if (kCode == GQA_CODE_E4M3 && edge) {
-            const __half2 y = __hmax2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(-448.f));
-            return *reinterpret_cast<const uint32_t*>(&y);
-        }
-        return x;
-    };
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
         const uint8_t* vi = v + 16 * i * kHeadDim;
         const uint4 x0 = lds128(vi + r0), x1 = lds128(vi + r1);
         const uint4 x2 = lds128(vi + 8 * kHeadDim + r0), x3 = lds128(vi + 8 * kHeadDim + r1);
-        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
-        const uint32_t w2[4] = {x2.x, x2.y, x2.z, x2.w}, w3[4] = {x3.x, x3.y, x3.z, x3.w};
+        uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+        uint32_t w2[4] = {x2.x, x2.y, x2.z, x2.w}, w3[4] = {x3.x, x3.y, x3.z, x3.w};
+        if (kCode == GQA_CODE_E4M3 && edge) {  // a code that no query sees may be NaN: 0 in its place
+            auto number = [](uint32_t& x) { x &= ~__vcmpeq4(x & 0x7f7f7f7fu, 0x7f7f7f7fu); };
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                number(w0[j]);
+                number(w1[j]);
+                number(w2[j]);
+                number(w3[j]);
+            }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
             uint32_t a0, a1, a2, a3;
             to_half4<kCode>(__byte_perm(w0[j >> 1], w1[j >> 1], sel), a0, a1);
             to_half4<kCode>(__byte_perm(w2[j >> 1], w3[j >> 1], sel), a2, a3);
-            a0 = number(a0);
-            a1 = number(a1);
-            a2 = number(a2);
-            a3 = number(a3);
 #pragma unroll
             for (int n = 0; n < kN; ++n) mma_16x8x16(st.o[n][j], a0, a1, a2, a3, w[n][i][0], w[n][i][1]);
         }
