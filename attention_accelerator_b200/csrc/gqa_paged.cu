@@ -3,8 +3,8 @@
 #include "gqa_paged.cuh"
 #include "gqa_internal.h"
 #include "gqa_paged_internal.h"
+#include "gqa_paged_units.cuh"
 
-#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -541,10 +541,20 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
 
 int launched() { return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA; }
 
+// A chunked call goes to the kernel for a few queries a sequence (gqa_paged_few.cu)
+// where its rows are 6 a sequence or less on average: 48 sequences of 5 queries take
+// 125 us there and 229 in the chunked kernel, of 2 86 and 228; 12 a sequence are two
+// of its units each and take as long as the one chunk.  One sequence may hold most
+// of the rows (a chunk of a prompt among single tokens), which only the GPU knows:
+// beyond kFewAlone rows both kernels are launched and the plan hands the call to
+// the one it is cheaper for.
+constexpr int kFewAverage = 6, kFewAlone = 12;
+bool few_queries(int batch, int rows) { return rows <= (int64_t)kFewAverage * batch; }
+
 size_t workspace_of(int batch, int rows, int heads, bool chunked, int sms) {
     if (!chunked) return paged_decode_workspace(sms);
-    const size_t few = paged_few_takes(batch, rows) ? paged_few_workspace(batch, rows, sms) : 0;
-    return std::max(few, paged_chunk_workspace(batch, rows, heads, sms));
+    return few_queries(batch, rows) ? paged_few_workspace(batch, rows, heads, sms)
+                                    : paged_chunk_workspace(batch, rows, heads, sms);
 }
 
 int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p, void* workspace,
@@ -561,17 +571,31 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     if (st != GQA_OK) return st;
     if (p->rows == 0) return GQA_OK;
     const RopeSteps& rope = rope_steps_of(p->rope_theta);
-    const bool few = chunked && paged_few_takes(p->batch, p->rows);
-    const int tile = few ? paged_few_tile() : chunked ? paged_chunk_tile() : paged_decode_tile();
-    CUtensorMap kmap, vmap;
-    if ((st = paged_map(&kmap, call.c.k, call.c, tile)) != GQA_OK ||
-        (st = paged_map(&vmap, call.c.v, call.c, tile)) != GQA_OK)
-        return st;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
+    uint32_t* status = reinterpret_cast<uint32_t*>(ws);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = few       ? launch_paged_few(call, rope, cache->code, kmap, vmap, sms, ws, s)
-                          : chunked ? launch_paged_chunk(call, rope, cache->code, kmap, vmap, sms, ws, s)
-                                    : launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, s);
+    CUtensorMap kmap, vmap;
+    auto maps = [&](int tile) {
+        const int k = paged_map(&kmap, call.c.k, call.c, tile);
+        return k != GQA_OK ? k : paged_map(&vmap, call.c.v, call.c, tile);
+    };
+    cudaError_t e = cudaSuccess;
+    if (!chunked) {
+        if ((st = maps(paged_decode_tile())) != GQA_OK) return st;
+        e = launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, s);
+    } else {
+        const bool few = few_queries(p->batch, p->rows), many = !few || p->rows > kFewAlone;
+        const UnitShape chunk = paged_chunk_shape(call, sms, ws), small = few ? paged_few_shape(call, sms, ws) : chunk;
+        e = launch_plan_units(call, small, few && many ? &chunk : nullptr, s);
+        if (e == cudaSuccess && few) {
+            if ((st = maps(paged_few_tile())) != GQA_OK) return st;
+            e = launch_paged_few(call, rope, cache->code, kmap, vmap, small, status, s);
+        }
+        if (e == cudaSuccess && many) {
+            if ((st = maps(paged_chunk_tile())) != GQA_OK) return st;
+            e = launch_paged_chunk(call, rope, cache->code, kmap, vmap, chunk, status, s);
+        }
+    }
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 

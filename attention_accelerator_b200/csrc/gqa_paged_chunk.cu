@@ -55,8 +55,8 @@ namespace gqa {
 namespace {
 
 constexpr int kTile = 128;                 // keys
-constexpr int kTileShift = 7;
-constexpr int kTokens = 64;                // queries of a unit
+constexpr int kTileShift = kChunkTileShift;
+constexpr int kTokens = kChunkTokens;      // queries of a unit
 constexpr int kRowsM = 128;                // rows of an M tile
 constexpr int kRawBytes = kTile * kHeadDim;          // K or V codes of a tile
 constexpr int kBlockBytes = kTile * 128;             // 128 rows x 64 dims of FP16
@@ -79,10 +79,6 @@ constexpr int kSlotFloats = kRowsM * 2 * (kHeadDim + 2);  // a partial: acc [32]
 // kind::f16 with FP16 A and B, FP32 accumulators, M = 128, N = 128.
 constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescO = kIdescS | (1u << 16);  // B (V) MN-major
-
-// What a unit costs a CTA beside its tiles (queries, the pipeline's start and
-// end, its rows), in tiles: measured at 25-28 thousand cycles to a tile's 5.
-constexpr int kUnitCost = 5;
 
 struct TileScales {
     float k[8], v[8];   // of each 16 keys: K's scale (NaN where V's is no number), V's over the reference
@@ -116,9 +112,7 @@ struct alignas(64) ChunkPagedArgs {
 
 struct PlanUnitsArgs {
     PagedCall p;
-    UnitPlan to;
-    int32_t tokens, tile_shift, unit_cost;  // queries of a unit, keys of a tile (log2), what a unit costs in tiles
-    int32_t max_units, ctas, counters;      // counters to zero (0: two a unit and head)
+    UnitShape first, other;
 };
 
 // ---------------------------------------------------------------------------
@@ -158,13 +152,14 @@ __device__ __forceinline__ longlong2 scan_exclusive(longlong2 v, longlong2* warp
     return make_longlong2(base.x + incl.x - v.x, base.y + incl.y - v.y);
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_constant__ PlanUnitsArgs a) {
-    extern __shared__ int32_t offset[];  // first unit of each sequence
-    __shared__ longlong2 warp_sum[kPlanThreads / 32];
-    const PagedCall& p = a.p;
+// False where a call cut into the chunked kernel's units would cost less (kChoice).
+template <bool kFew, bool kChoice>
+__device__ __forceinline__ bool plan_units(const PagedCall& p, const UnitShape& a, int32_t* offset, longlong2* warp_sum,
+                                           unsigned long long* chunked) {
+    constexpr int kQueries = kFew ? kFewTokens : kChunkTokens, kShift = kFew ? kFewTileShift : kChunkTileShift;
+    constexpr int kCost = kFew ? kFewUnitCost : kChunkUnitCost;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, batch = p.batch;
-    dependency_wait();
-    allow_dependents();
+    unsigned long long as_chunks = 0;  // cost, in the chunked kernel's tiles
     // Rows of sequence b, kept within the call's whatever the device's numbers say.
     auto rows_of = [&](int b, int& row0) {
         row0 = min(max(p.first_query[b], 0), p.rows);
@@ -175,13 +170,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     longlong2 sum = make_longlong2(0, 0), all;
     for (int b = b0; b < b1; ++b) {
         int row0;
-        sum.x += (rows_of(b, row0) + a.tokens - 1) / a.tokens;
+        sum.x += (rows_of(b, row0) + kQueries - 1) / kQueries;
     }
     int64_t at = scan_exclusive(sum, warp_sum, &all).x;
     for (int b = b0; b < b1; ++b) {
         int row0;
         offset[b] = (int)at;
-        at += (rows_of(b, row0) + a.tokens - 1) / a.tokens;
+        at += (rows_of(b, row0) + kQueries - 1) / kQueries;
     }
     const int units = (int)min((int64_t)all.x, (int64_t)a.max_units);
     __syncthreads();
@@ -194,8 +189,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
         }
         const int b = lo_b;  // (of sequences that share an offset the last: the one with rows)
         int row0;
-        const int rows = rows_of(b, row0), skip = (u - offset[b]) * a.tokens;
-        const int n = min(a.tokens, rows - skip), len = paged_length(p, b);
+        const int rows = rows_of(b, row0), skip = (u - offset[b]) * kQueries;
+        const int n = min(kQueries, rows - skip), len = paged_length(p, b);
         const int64_t pos0 = (int64_t)p.seq_lens[b] - rows + skip;
         int lo = 0x7fffffff, hi = 0;
         for (int i = lane; i < n; i += 32) {
@@ -215,35 +210,40 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
             x.pos0 = (int)pos0;
             x.lo = lo;
             x.hi = hi;
-            x.tile0 = hi > 0 ? lo >> a.tile_shift : 0;
-            x.tiles = hi > 0 ? ((hi + (1 << a.tile_shift) - 1) >> a.tile_shift) - x.tile0 : 0;
+            x.tile0 = hi > 0 ? lo >> kShift : 0;
+            x.tiles = hi > 0 ? ((hi + (1 << kShift) - 1) >> kShift) - x.tile0 : 0;
             x.first = x.cell = 0;
             a.to.units[u] = x;
+            // A unit of the chunked kernel that begins here sees much what this one does.
+            if (kChoice && x.tiles && skip / kChunkTokens * kChunkTokens + kQueries > skip)
+                as_chunks += (x.tiles >> (kChunkTileShift - kShift)) + 1 + kChunkUnitCost;
         }
     }
+    if (kChoice && lane == 0 && as_chunks) atomicAdd(chunked, as_chunks);
     __syncthreads();
     const int heads = p.c.kv_heads;
     const int uper = (units + kPlanThreads - 1) / kPlanThreads;
     const int u0 = min(units, tid * uper), u1 = min(units, u0 + uper);
-    // Shares are cut evenly in cost: a unit's cells are a.unit_cost of its own, then one for each tile.
+    // Shares are cut evenly in cost: a unit's cells are kCost of its own, then one for each tile.
     sum = make_longlong2(0, 0);
     for (int u = u0; u < u1; ++u) {
         const int tiles = a.to.units[u].tiles;
         sum.x += tiles;
-        sum.y += tiles ? tiles + a.unit_cost : 0;
+        sum.y += tiles ? tiles + kCost : 0;
     }
     longlong2 here = scan_exclusive(sum, warp_sum, &all);
     const int64_t total = all.x * heads, cost = all.y * heads;
+    if (kChoice && all.y > kChunkTileCost * (int64_t)*chunked) return false;
     for (int u = u0; u < u1; ++u) {
         const int tiles = a.to.units[u].tiles;
         a.to.units[u].first = here.x;
         a.to.units[u].cell = here.y;
         here.x += tiles;
-        here.y += tiles ? tiles + a.unit_cost : 0;
+        here.y += tiles ? tiles + kCost : 0;
     }
     __syncthreads();
-    // Shares longer than a.unit_cost: each has a tile.
-    const int64_t G = min((int64_t)a.ctas, cost / (a.unit_cost + 1));
+    // Shares longer than kCost: each has a tile.
+    const int64_t G = min((int64_t)a.ctas, cost / (kCost + 1));
     if (tid <= G) {
         int64_t cut = total;
         if (tid < G) {
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
                 if (a.to.units[mid].cell * heads <= c) lo = mid; else hi = mid;
             }
             const Unit x = a.to.units[lo];
-            const int64_t each = x.tiles + a.unit_cost, off = c - x.cell * heads, h = off / each, t = off - h * each - a.unit_cost;
+            const int64_t each = x.tiles + kCost, off = c - x.cell * heads, h = off / each, t = off - h * each - kCost;
             a.to.starts[tid] = lo;
             cut = x.first * heads + h * x.tiles + (t > 0 ? t : 0);
         }
@@ -263,6 +263,26 @@ __global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_c
     const int counters = a.counters ? a.counters : units * heads * 2;
     for (int i = tid; i < counters; i += kPlanThreads) a.to.arrivals[i] = 0;
     if (tid == 0) *a.to.meta = Meta{total, (int32_t)G, units};
+    return true;
+}
+
+template <bool kFew, bool kChoice>
+__global__ void __launch_bounds__(kPlanThreads) plan_units_kernel(const __grid_constant__ PlanUnitsArgs a) {
+    extern __shared__ int32_t offset[];  // first unit of each sequence
+    __shared__ longlong2 warp_sum[kPlanThreads / 32];
+    __shared__ unsigned long long chunked;
+    if (kChoice && threadIdx.x == 0) chunked = 0;
+    dependency_wait();
+    allow_dependents();
+    if (kChoice) __syncthreads();
+    const bool first = plan_units<kFew, kChoice>(a.p, a.first, offset, warp_sum, &chunked);
+    if constexpr (kChoice) {
+        if (!first) {
+            __syncthreads();
+            plan_units<false, false>(a.p, a.other, offset, warp_sum, &chunked);
+        }
+        if (threadIdx.x == 0) *(first ? a.other.to.meta : a.first.to.meta) = Meta{0, 0, 0};
+    }
 }
 
 __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int head, int page, uint64_t* bar) {
@@ -343,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     dependency_wait();
     allow_dependents();
     const Meta meta = *a.meta;
+    if (meta.units == 0) return;  // cut for the few-query kernel, or no rows
     if (tid < kPairs) s.step[tid] = a.rope.step[tid];
     if (tid <= meta.ctas) s.cuts[tid] = a.cuts[tid];
     if (warp == kMmaWarp) {
@@ -967,15 +988,19 @@ Kernel kernel_for(int code, bool cap, bool bias) {
 }
 
 UnitRegions regions(int batch, int rows, int heads, int sms) {
-    return unit_regions(batch, rows, kTokens, (size_t)heads * 2, sms, (size_t)sms * 2 * kSlotFloats * sizeof(float));
+    const size_t units = (size_t)rows / kTokens + batch;
+    return unit_regions(kPagedPartialsOffset, batch, rows, kTokens, units * heads * 2, sms,
+                        (size_t)sms * 2 * kSlotFloats * sizeof(float));
 }
 
 }  // namespace
 
-cudaError_t launch_plan_units(const PagedCall& call, const UnitPlan& to, int tokens, int tile_shift, int unit_cost,
-                              int counters, int ctas, cudaStream_t stream) {
-    const PlanUnitsArgs a{call, to, tokens, tile_shift, unit_cost, call.rows / tokens + call.batch, ctas, counters};
-    return launch_dependent(plan_units_kernel, 1, kPlanThreads, call.batch * sizeof(int32_t), stream, a);
+cudaError_t launch_plan_units(const PagedCall& call, const UnitShape& first, const UnitShape* other, cudaStream_t stream) {
+    const PlanUnitsArgs a{call, first, other ? *other : first};
+    const auto kernel = other       ? plan_units_kernel<true, true>
+                        : first.few ? plan_units_kernel<true, false>
+                                    : plan_units_kernel<false, false>;
+    return launch_dependent(kernel, 1, kPlanThreads, call.batch * sizeof(int32_t), stream, a);
 }
 
 int paged_chunk_tile() { return kTile; }
@@ -996,26 +1021,18 @@ cudaError_t paged_chunk_prepare() {
     return cudaSuccess;
 }
 
+UnitShape paged_chunk_shape(const PagedCall& call, int sms, uint8_t* ws) {
+    return unit_shape(regions(call.batch, call.rows, call.c.kv_heads, sms), ws, call.rows / kTokens + call.batch,
+                      sms < kMaxCtas ? sms : kMaxCtas, 0, false);
+}
+
 cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
-                               const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
-    if (sms > kMaxCtas) sms = kMaxCtas;
-    const UnitRegions r = regions(call.batch, call.rows, call.c.kv_heads, sms);
-    const UnitPlan pl = unit_plan(r, ws);
-    const cudaError_t e = launch_plan_units(call, pl, kTokens, kTileShift, kUnitCost, 0, sms, stream);
-    if (e != cudaSuccess) return e;
-    ChunkPagedArgs a;
-    a.kmap = kmap;
-    a.vmap = vmap;
-    a.p = call;
-    a.rope = rope;
-    a.status = reinterpret_cast<uint32_t*>(ws);
-    a.meta = pl.meta;
-    a.units = pl.units;
-    a.starts = pl.starts;
-    a.cuts = pl.cuts;
-    a.arrivals = pl.arrivals;
-    a.partials = reinterpret_cast<float*>(ws + r.partials);
-    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), sms, kThreads, kSmemBytes, stream, a);
+                               const CUtensorMap& vmap, const UnitShape& shape, uint32_t* status, cudaStream_t stream) {
+    const UnitPlan& pl = shape.to;
+    const ChunkPagedArgs a{kmap, vmap, call, rope, status, pl.meta, pl.units, pl.starts, pl.cuts, pl.arrivals,
+                           shape.partials};
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), shape.ctas, kThreads, kSmemBytes,
+                            stream, a);
 }
 
 }  // namespace gqa

@@ -34,14 +34,13 @@ constexpr int kThreads = (kZeroWarp + 1) * 32;
 // Registers: launched with 128 a thread; each group of four warps takes its share.
 constexpr int kLaunchRegs = 128, kConsumerRegs = 192, kRestRegs = 64;
 static_assert(kThreads == 512 && 2 * kConsumerRegs + 2 * kRestRegs <= 4 * kLaunchRegs, "of what the CTA was launched with");
-constexpr int kTokens = 6;         // queries of a unit
+constexpr int kTokens = kFewTokens;  // queries of a unit
 constexpr int kPairsQ = kTokens / 2;
-constexpr int kTile = 32, kTileShift = 5;
+constexpr int kTileShift = kFewTileShift, kTile = 1 << kTileShift;
 constexpr int kSteps = kTile / 16;
 constexpr int kHalfBytes = kTile * kHeadDim;
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 2 * kWarps;
-constexpr int kUnitCost = 16;
 constexpr int kRowF = kHeadDim + 4;    // padded row
 constexpr int kUnitRows = kTokens * kGroup;
 // Weights are 2^(z - m) with z up to 8 above the reference m, times a page's V scale
@@ -299,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
     dependency_wait();
     allow_dependents();
     const Meta meta = *a.meta;
+    if (meta.units == 0) return;  // cut for the chunked kernel, or no rows
     if (tid <= meta.ctas) s.cuts[tid] = a.cuts[tid];
     __syncthreads();
     bool ok = true;  // after a wait that timed out: no more waits, but every barrier and counter is kept
@@ -716,16 +716,22 @@ Kernel kernel_for(int code, bool cap, bool bias) {
     return bias ? paged_few_kernel<1, false, true> : paged_few_kernel<1, false, false>;
 }
 
-UnitRegions regions(int batch, int rows, int sms) {
-    return unit_regions(batch, rows, kTokens, 1, sms, ((size_t)sms * 2 * kUnitRows * kRowF) * sizeof(float) +
-                                                          (size_t)sms * kGroup * sizeof(uint32_t));
+UnitRegions regions(int batch, int rows, int heads, int sms) {  // behind the chunked kernel's
+    return unit_regions(paged_chunk_workspace(batch, rows, heads, sms), batch, rows, kTokens, (size_t)sms * kGroup, sms,
+                        (size_t)sms * 2 * kUnitRows * kRowF * sizeof(float));
 }
 
 }  // namespace
 
 int paged_few_tile() { return kTile; }
-bool paged_few_takes(int batch, int rows) { return rows <= (int64_t)kTokens * batch; }
-size_t paged_few_workspace(int batch, int rows, int sms) { return regions(batch, rows, sms).end; }
+
+size_t paged_few_workspace(int batch, int rows, int heads, int sms) { return regions(batch, rows, heads, sms).end; }
+
+UnitShape paged_few_shape(const PagedCall& call, int sms, uint8_t* ws) {
+    const int ctas = sms < kMaxCtas ? sms : kMaxCtas;
+    return unit_shape(regions(call.batch, call.rows, call.c.kv_heads, sms), ws, call.rows / kTokens + call.batch, ctas,
+                      ctas * kGroup, true);
+}
 
 cudaError_t paged_few_prepare() {
     for (int i = 0; i < 8; ++i) {
@@ -741,17 +747,11 @@ cudaError_t paged_few_prepare() {
 }
 
 cudaError_t launch_paged_few(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
-                             const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
-    if (sms > kMaxCtas) sms = kMaxCtas;
-    const UnitRegions r = regions(call.batch, call.rows, sms);
-    UnitPlan pl = unit_plan(r, ws);
-    // The counters are a share's, not a unit's: behind the partial rows.
-    pl.arrivals = reinterpret_cast<uint32_t*>(ws + r.partials + (size_t)sms * 2 * kUnitRows * kRowF * sizeof(float));
-    const cudaError_t e = launch_plan_units(call, pl, kTokens, kTileShift, kUnitCost, sms * kGroup, sms, stream);
-    if (e != cudaSuccess) return e;
-    const FewPagedArgs a{kmap, vmap, call, rope, reinterpret_cast<uint32_t*>(ws), pl.meta, pl.units, pl.starts, pl.cuts,
-                         pl.arrivals, reinterpret_cast<float*>(ws + r.partials)};
-    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), sms, kThreads, kSmemBytes, stream, a);
+                             const CUtensorMap& vmap, const UnitShape& shape, uint32_t* status, cudaStream_t stream) {
+    const UnitPlan& pl = shape.to;
+    const FewPagedArgs a{kmap, vmap, call, rope, status, pl.meta, pl.units, pl.starts, pl.cuts, pl.arrivals, shape.partials};
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), shape.ctas, kThreads, kSmemBytes,
+                            stream, a);
 }
 
 }  // namespace gqa

@@ -21,17 +21,11 @@ size_t paged_decode_workspace(int sms);
 cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream);
 
-// Any number of queries a sequence: two launches (units and shares, attention).
+// Any number of queries a sequence: units and shares, then the kernel for them
+// (gqa_paged_units.cuh).
 int paged_chunk_tile();
 size_t paged_chunk_workspace(int batch, int rows, int heads, int sms);
-cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
-                               const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream);
-
-// The same for a few queries a sequence.
 int paged_few_tile();
-bool paged_few_takes(int batch, int rows);
-size_t paged_few_workspace(int batch, int rows, int sms);
-cudaError_t launch_paged_few(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
-                             const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream);
+size_t paged_few_workspace(int batch, int rows, int heads, int sms);
 
 }  // namespace gqa

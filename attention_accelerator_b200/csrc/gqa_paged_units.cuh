@@ -27,26 +27,35 @@ struct UnitPlan {
     uint32_t* arrivals;  // counters, zeroed
 };
 
-// Layout behind the counters that the decode keeps; everything here is written by each call.
-struct UnitRegions {
-    size_t starts, cuts, units, arrivals, partials, end;
+// How a kernel wants a call cut, and where it reads that.
+struct UnitShape {
+    UnitPlan to;
+    float* partials;
+    int32_t max_units, ctas, counters;  // counters to zero (0: two a unit and head)
+    bool few;
 };
-inline UnitRegions unit_regions(int batch, int rows, int tokens, size_t counters_a_unit, int sms, size_t partials) {
+
+// Layout in the workspace, from `base` on; everything here is written by each call.
+struct UnitRegions {
+    size_t meta, starts, cuts, units, arrivals, partials, end;
+};
+inline UnitRegions unit_regions(size_t base, int batch, int rows, int tokens, size_t counters, int sms, size_t partials) {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    const size_t units = (size_t)rows / tokens + batch;
     UnitRegions r;
-    r.starts = kPagedPartialsOffset + 256;  // (Meta first)
+    r.meta = base;
+    r.starts = base + 256;
     r.cuts = r.starts + up((size_t)sms * sizeof(int32_t));
     r.units = r.cuts + up((size_t)(sms + 1) * sizeof(int64_t));
-    r.arrivals = r.units + up(units * sizeof(Unit));
-    r.partials = r.arrivals + up(units * counters_a_unit * sizeof(uint32_t));
-    r.end = r.partials + partials;
+    r.arrivals = r.units + up(((size_t)rows / tokens + batch) * sizeof(Unit));
+    r.partials = r.arrivals + up(counters * sizeof(uint32_t));
+    r.end = r.partials + up(partials);
     return r;
 }
-inline UnitPlan unit_plan(const UnitRegions& r, uint8_t* ws) {
-    return UnitPlan{reinterpret_cast<Meta*>(ws + kPagedPartialsOffset), reinterpret_cast<Unit*>(ws + r.units),
-                    reinterpret_cast<int32_t*>(ws + r.starts), reinterpret_cast<int64_t*>(ws + r.cuts),
-                    reinterpret_cast<uint32_t*>(ws + r.arrivals)};
+inline UnitShape unit_shape(const UnitRegions& r, uint8_t* ws, int max_units, int ctas, int counters, bool few) {
+    return UnitShape{UnitPlan{reinterpret_cast<Meta*>(ws + r.meta), reinterpret_cast<Unit*>(ws + r.units),
+                              reinterpret_cast<int32_t*>(ws + r.starts), reinterpret_cast<int64_t*>(ws + r.cuts),
+                              reinterpret_cast<uint32_t*>(ws + r.arrivals)},
+                     reinterpret_cast<float*>(ws + r.partials), max_units, ctas, counters, few};
 }
 
 // A CTA's walk through its share, one unit's piece at a time.
@@ -90,10 +99,23 @@ struct Walk {
     }
 };
 
-// One CTA: units of `tokens` queries, their keys in tiles of 2^tile_shift, shares
-// of even cost (a unit costs unit_cost tiles beside its own), `counters` zeroed (0:
-// two a unit and head).
-cudaError_t launch_plan_units(const PagedCall& call, const UnitPlan& to, int tokens, int tile_shift, int unit_cost,
-                              int counters, int ctas, cudaStream_t stream);
+// Queries of a unit, keys of a tile (log2) and what a unit costs beside its tiles, in
+// tiles: of the chunked kernel (measured: 25 to 28 thousand cycles to a tile's 5) and
+// of the one for few queries (48 x 5 drafted tokens: 147 us with 4, 128 with 12, 124
+// with 16 or 20).  And a tile of the former in tiles of the latter: 4700 cycles to 580.
+constexpr int kChunkTokens = 64, kChunkTileShift = 7, kChunkUnitCost = 5;
+constexpr int kFewTokens = 6, kFewTileShift = 5, kFewUnitCost = 16;
+constexpr int kChunkTileCost = 8;
+
+// One CTA: the call cut as `first` wants it or, where `other` is given and the
+// lengths in device memory make that cheaper, as that; the kernel of the one not
+// taken finds no units.
+cudaError_t launch_plan_units(const PagedCall& call, const UnitShape& first, const UnitShape* other, cudaStream_t stream);
+UnitShape paged_chunk_shape(const PagedCall& call, int sms, uint8_t* ws);
+UnitShape paged_few_shape(const PagedCall& call, int sms, uint8_t* ws);
+cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
+                               const CUtensorMap& vmap, const UnitShape& shape, uint32_t* status, cudaStream_t stream);
+cudaError_t launch_paged_few(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
+                             const CUtensorMap& vmap, const UnitShape& shape, uint32_t* status, cudaStream_t stream);
 
 }  // namespace gqa
