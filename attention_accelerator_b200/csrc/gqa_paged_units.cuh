@@ -104,7 +104,7 @@ struct Walk {
 // of the one for few queries (48 x 5 drafted tokens: 147 us with 4, 128 with 12, 124
 // with 16 or 20).  And a tile of the former in tiles of the latter: 4700 cycles to 580.
 constexpr int kChunkTokens = 64, kChunkTileShift = 7, kChunkUnitCost = 5;
-constexpr int kFewTokens = 6, kFewTileShift = 5, kFewUnitCost = 16;
+constexpr int kFewTokens = 6, kFewTileShift = 5, kFewUnitCost = 20;
 constexpr int kChunkTileCost = 8;
 
 // One CTA: the call cut as `first` wants it or, where `other` is given and the

@@ -723,3 +723,85 @@ def test_many_sequences():
     check(torch.stack(sub), q[pick], s, pick, [lens[i] - 1 for i in pick], unit=DECODE_UNIT)
     rows = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(list(range(1501))))
     check(rows[pick], q[pick], s, pick, [lens[i] - 1 for i in pick], unit=CHUNK_UNIT)
+
+
+# ---- a few queries a sequence: a kernel of its own, which keeps one FP16 part of Q and of the weights (so CHUNK_UNIT's
+# bound holds for it: it rounds a subset of what the chunked kernel does) --------------------------------------------
+@pytest.mark.parametrize("counts,lens", [
+    ([6], [6]), ([2], [31]), ([4], [33]), ([6], [20000]),             # one unit, cut by up to every CTA
+    ([1, 2, 3, 4, 5, 6], [1, 2, 300, 64, 5, 3000]),                   # every number of queries
+    ([7, 0, 5, 13, 1, 6, 0, 12], [7, 9, 1000, 13, 40, 700, 0, 65]),   # several units a sequence, and none
+    ([5] * 60, [5 + 37 * i for i in range(60)])])                     # many units a share
+@pytest.mark.parametrize("code,page_len,layout", [("int8", 16, "position_major"), ("e4m3", 64, "head_major"),
+                                                  ("int8", 128, "head_major"), ("e4m3", 32, "position_major")])
+def test_few_queries_a_sequence(counts, lens, code, page_len, layout):
+    assert sum(counts) <= 6 * len(counts)
+    s = Setup(lens, seed=sum(lens), page_len=page_len, code=code, layout=layout)
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    rows = first[-1]
+    q = s.queries(rows + 2)
+    owner = [b for b, n in enumerate(counts) for _ in range(n)]
+    pos = [lens[b] - n + i for b, n in enumerate(counts) for i in range(n)]
+    s.poison(lambda b, p: False)
+    out = torch.full((rows + 2, 32, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first), out=out)
+    assert bool((out[rows:] == 7.0).all())
+    pick = sorted(set(range(0, rows, max(1, rows // 40))) | {rows - 1})
+    check(got[pick], q[pick], s, [owner[i] for i in pick], [pos[i] for i in pick], unit=CHUNK_UNIT)
+    again = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first))
+    assert torch.equal(got[:rows].view(torch.int16), again[:rows].view(torch.int16))
+    assert gqa.read_device_status() == 0
+
+
+@pytest.mark.parametrize("what", MODS)
+@pytest.mark.parametrize("code,page_len", [("e4m3", 16), ("int8", 64)])
+def test_few_queries_masks_cap_and_bias(what, code, page_len):
+    counts, lens = [6, 5, 1, 11, 2, 0, 4], [6, 301, 77, 700, 1500, 8, 130]
+    s = Setup(lens, seed=7 * len(what), page_len=page_len, code=code)
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    owner = [b for b, n in enumerate(counts) for _ in range(n)]
+    pos = [lens[b] - n + i for b, n in enumerate(counts) for i in range(n)]
+    q = s.queries(first[-1])
+    call, chk = modifiers(s, what, owner, pos)
+    starts, ends = chk.get("starts", [0] * len(pos)), chk.get("ends", [0] * len(pos))
+    visible = [set() for _ in lens]
+    for i, b in enumerate(owner):
+        visible[b] |= set(range(max(0, starts[i]), min(lens[b], max(pos[i] + 1, ends[i]))))
+    s.poison(lambda b, p: p not in visible[b])
+    got = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first), **call)
+    check(got, q, s, owner, pos, unit=CHUNK_UNIT, **chk)
+    assert gqa.read_device_status() == 0
+
+
+@pytest.mark.parametrize("counts,lens", [
+    ([1] * 20 + [100], [40] * 20 + [3000]),        # the long one has the keys, too: cut as chunks
+    ([100] + [1] * 20, [130] + [2000] * 20),       # it has few of them: cut as few queries
+    ([0] * 20 + [120], [5] * 20 + [121]),
+    ([2] * 7, [0] * 7)])                           # more rows than keys: most of them see nothing
+def test_one_chunk_among_single_tokens(counts, lens):
+    s = Setup(lens, seed=5, page_len=32, code="int8")
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    owner = [b for b, n in enumerate(counts) for _ in range(n)]
+    pos = [lens[b] - n + i for b, n in enumerate(counts) for i in range(n)]
+    q = s.queries(first[-1])
+    s.poison(lambda b, p: False)
+    got = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first))
+    check(got, q, s, owner, pos, unit=CHUNK_UNIT)
+    assert gqa.read_device_status() == 0
+
+
+def test_few_queries_reach_every_page_and_head_shard():
+    """Table entries outside the cache are zeros, not reads; a shard's heads match the whole cache's."""
+    lens, counts = [200, 64, 33], [5, 6, 2]
+    s = Setup(lens, seed=9, page_len=16, code="e4m3", heads=3)
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    owner = [b for b, n in enumerate(counts) for _ in range(n)]
+    pos = [lens[b] - n + i for b, n in enumerate(counts) for i in range(n)]
+    q = s.queries(first[-1])
+    s.poison(lambda b, p: False)
+    got = gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first))
+    check(got, q, s, owner, pos, unit=CHUNK_UNIT)
+    table = [[-5 if c % 2 else 1 << 30 for c in range(len(row))] for row in s.table]
+    out = gqa.decode_paged_chunked(q, s.cache, ints(table), ints(lens), ints(first))
+    assert bool((out == 0).all())  # codes and scales of such pages count as 0
+    assert gqa.read_device_status() == 0
