@@ -553,8 +553,8 @@ bool few_queries(int batch, int rows) { return rows <= (int64_t)kFewAverage * ba
 
 size_t workspace_of(int batch, int rows, int heads, bool chunked, int sms) {
     if (!chunked) return paged_decode_workspace(sms);
-    return few_queries(batch, rows) ? paged_few_workspace(batch, rows, heads, sms)
-                                    : paged_chunk_workspace(batch, rows, heads, sms);
+    // Both kernels' regions whichever takes the call: a workspace for the largest call holds every smaller one.
+    return paged_few_workspace(batch, rows, heads, sms);
 }
 
 int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p, void* workspace,

@@ -726,7 +726,9 @@ Kernel kernel_for(int code, bool cap, bool bias) {
     return bias ? paged_few_kernel<1, false, true> : paged_few_kernel<1, false, false>;
 }
 
-UnitRegions regions(int batch, int rows, int heads, int sms) {  // behind the chunked kernel's
+// Behind the chunked kernel's.  Units enough for any split of the rows, so that a call
+// with more rows never needs less.
+UnitRegions regions(int batch, int rows, int heads, int sms) {
     return unit_regions(paged_chunk_workspace(batch, rows, heads, sms), batch, rows, kTokens, (size_t)sms * kGroup, sms,
                         (size_t)sms * 2 * kUnitRows * kRowF * sizeof(float));
 }

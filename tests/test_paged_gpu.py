@@ -805,3 +805,21 @@ def test_few_queries_reach_every_page_and_head_shard():
     out = gqa.decode_paged_chunked(q, s.cache, ints(table), ints(lens), ints(first))
     assert bool((out == 0).all())  # codes and scales of such pages count as 0
     assert gqa.read_device_status() == 0
+
+
+def test_a_workspace_for_the_largest_call_holds_every_smaller_one():
+    import ctypes
+
+    from attention_accelerator_b200 import _lib
+    cache = gqa.paged_cache(2, 16)
+    first = ints([0, 1])
+
+    def need(batch, rows):
+        p = _lib.GqaPagedParams()
+        p.batch, p.rows, p.first_query = batch, rows, first.data_ptr()
+        return _lib.load().gqa_paged_workspace_bytes(ctypes.byref(cache.c), ctypes.byref(p))
+
+    sizes = [[need(batch, rows) for rows in (1, 6, 12, 13, 64, 384, 385, 8192, 100000)] for batch in (1, 2, 63, 64, 1000, 8192)]
+    assert all(x > 0 for row in sizes for x in row)
+    assert all(row == sorted(row) for row in sizes)
+    assert all(list(col) == sorted(col) for col in zip(*sizes))
