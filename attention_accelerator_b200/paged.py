@@ -172,9 +172,9 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     if not 0 <= max_tokens <= 0x7FFFFFFF:
         raise ValueError(f"max_tokens must be in [0, 2^31), got {max_tokens}")
     i32 = torch.int32
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
+    slots = lens.new_empty(max_tokens, dtype=torch.int64)
     room = [n if lens_out is None else 0, 1 if n_free_out is None else 0, n + 1, max_tokens, 4]  # in one allocation
-    new_lens_out, new_n_free, first, positions, counts = torch.empty(sum(room), dtype=i32, device=device).split(room)
+    new_lens_out, new_n_free, first, positions, counts = lens.new_empty(sum(room), dtype=i32).split(room)
     lens_out = new_lens_out if lens_out is None else lens_out
     n_free_out = new_n_free if n_free_out is None else n_free_out
     stream = _stream_ptr(device)
@@ -229,7 +229,8 @@ def read_paged(cache: PagedCache, slots: torch.Tensor) -> tuple[torch.Tensor, to
         raise ValueError("read_paged takes CUDA tensors")
     n = slots.shape[0] if slots.dim() == 1 else -1
     ptr = _need("slots", slots, torch.int64, (n,), device)
-    k, v = (torch.empty((n, cache.kv_heads, HEAD_DIM), dtype=torch.bfloat16, device=device) for _ in range(2))
+    shape = (n, cache.kv_heads, HEAD_DIM)
+    k, v = slots.new_empty(shape, dtype=torch.bfloat16), slots.new_empty(shape, dtype=torch.bfloat16)
     if n:
         _check(lib.gqa_read_paged(ctypes.byref(cache.c), ptr, n, k.data_ptr(), v.data_ptr(), _stream_ptr(device)),
                "read_paged")
@@ -255,7 +256,7 @@ def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_posit
     if score_cap is not None and not (score_cap > 0.0 and math.isfinite(score_cap)):
         raise ValueError("score_cap must be positive and finite, or None")
     if out is None:
-        out = torch.empty((rows, heads, HEAD_DIM), dtype=torch.bfloat16, device=device)
+        out = q.new_empty((rows, heads, HEAD_DIM))
     else:
         _check_out(out, (rows, heads, HEAD_DIM), torch.bfloat16, device)
     i32 = torch.int32
