@@ -94,7 +94,7 @@ struct alignas(16) Shared {
 };
 
 struct alignas(64) DecodePagedArgs {
-    CUtensorMap kmap, vmap;  // (128, page_len, heads, pages) bytes, box (128, min(page_len, 64), 1, 1)
+    CUtensorMap kmap, vmap;  // (128, page_len, heads, pages) bytes, box (128, min(page_len, 32), 1, 1)
     PagedCall p;
     RopeSteps rope;
     uint32_t* status;
