@@ -67,6 +67,8 @@ class PagedCache:
         for name, t in (("k_scale", self.k_scale), ("v_scale", self.v_scale)):
             if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or t.stride(-1) != 1 and heads > 1:
                 raise ValueError(f"{name} must be float32 [{pages}, {heads}] with a contiguous last dim")
+            if pages > 1 and t.stride(0) < heads:  # (an expanded tensor: an append writes each page's own scale)
+                raise ValueError(f"{name}'s pages must not overlap (row stride {t.stride(0)} for {heads} heads)")
         if self.v_scale.stride(0) != self.k_scale.stride(0) and pages > 1:
             raise ValueError("k_scale and v_scale must have the same strides")
         for name, t in (("v", v), ("k_scale", self.k_scale), ("v_scale", self.v_scale)):

@@ -54,6 +54,22 @@ def test_cache_refuses_wrong_tensors():
         gqa.PagedCache(wide, wide, torch.zeros(4, 9), torch.zeros(4, 9))
 
 
+def test_cache_refuses_scales_whose_pages_overlap():
+    """An expanded scale tensor has fewer floats than pages times heads."""
+    for heads in (1, 8):
+        k = torch.zeros(4, heads, 16, 128, dtype=torch.int8)
+        whole, one = torch.zeros(4, heads), torch.zeros(1, heads).expand(4, heads)
+        for scales in (dict(k_scale=one, v_scale=one), dict(k_scale=one, v_scale=whole), dict(k_scale=whole, v_scale=one)):
+            with pytest.raises(ValueError, match="overlap|same strides"):
+                gqa.PagedCache(k, k.clone(), **scales)
+        skewed = torch.zeros(64).as_strided((4, heads), (max(1, heads - 1), 1))
+        if heads > 1:
+            with pytest.raises(ValueError, match="overlap"):
+                gqa.PagedCache(k, k.clone(), skewed, skewed)
+        one_page = torch.zeros(1, heads).expand(1, heads)
+        gqa.PagedCache(k[:1], k[:1].clone(), one_page, one_page.clone())
+
+
 def test_calls_refuse_host_tensors():
     c = host_cache()
     i32 = torch.zeros(2, dtype=torch.int32)
