@@ -236,7 +236,7 @@ __device__ __forceinline__ int run_length(const AppendArgs& a, int t0, int64_t s
     int len = 0;
     for (int at = 0; at < room; at += 32) {
         const int i = at + lane;
-        const bool in = i < room && t0 + i < a.n_tokens && a.slots[t0 + i] == slot + i;
+        const bool in = i < room && i < a.n_tokens - t0 && a.slots[t0 + i] == slot + i;
         const unsigned miss = ~__ballot_sync(0xffffffffu, in);
         len += miss ? __ffs(miss) - 1 : 32;
         if (miss) break;
@@ -397,9 +397,9 @@ __global__ void __launch_bounds__(256, 2) append_pages_kernel(const __grid_const
     const int w0 = blockIdx.x * kWindow;
     unsigned starts;
     {
-        const int t = w0 + lane;
         int64_t slot = -1, before = -1;
-        if (lane < kWindow && t < a.n_tokens) {
+        if (lane < kWindow && lane < a.n_tokens - w0) {
+            const int t = w0 + lane;
             slot = a.slots[t];
             if (t > 0) before = a.slots[t - 1];
         }
@@ -777,7 +777,7 @@ int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token
     // 33 us as prompts, whose runs fill pages, so that a window of 16 tokens begins one at most.
     const bool step = n_tokens <= 1024;
     a.rope = rope_steps_of(rope_theta);
-    const dim3 grid(step ? n_tokens : (n_tokens + kWindow - 1) / kWindow, step ? cache->kv_heads : 1, 2);
+    const dim3 grid(step ? n_tokens : (n_tokens - 1) / kWindow + 1, step ? cache->kv_heads : 1, 2);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool int8 = cache->code == GQA_CODE_INT8;
     if (step) {

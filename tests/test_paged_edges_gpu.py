@@ -25,3 +25,19 @@ def test_the_longest_slot_list():
         assert int((plan.positions[max(2, at):at + (1 << 28)] != -1).sum()) == 0
     del plan
     torch.cuda.empty_cache()
+
+
+def test_an_append_of_as_many_rows_as_an_int32_counts():
+    """Rows that are all one row; only the last two are stored, at the list's very end."""
+    n = 0x7FFFFFFF
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    cache = gqa.paged_cache(1, 64, dtype=torch.int8, kv_heads=1)
+    row = torch.full((1, 1, 128), 3.0, dtype=torch.bfloat16, device="cuda").expand(n, 1, 128)
+    slots = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    slots[n - 2], slots[n - 1] = 8, 9
+    gqa.append_paged(cache, row, row, slots)
+    k, _ = gqa.read_paged(cache, ints([7, 8, 9, 10], torch.int64))
+    assert k[:, 0, 0].tolist() == [0.0, 3.0, 3.0, 0.0]
+    del slots, row
+    torch.cuda.empty_cache()
