@@ -196,6 +196,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     return true;
 }
 
+// The same with one outcome for the whole warp, so that what follows warp-wide
+// (tcgen05.ld, shuffles, votes) is never reached by part of it.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
 // L2 policy for streamed-once K/V rows.
 __device__ __forceinline__ uint64_t l2_evict_first_policy() {
     uint64_t pol;

@@ -90,7 +90,7 @@ struct TileScales {
 struct alignas(16) Shared {
     uint64_t raw_full[kRaw], raw_empty[kRaw], conv_full[kConv], conv_empty[kConv];
     uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], group[2];
-    uint64_t pad;
+    uint64_t drain;  // products in flight when the issuer gives up
     TileScales scales[kScaleSlots];
     uint64_t step[kPairs];  // turns per position of each pair
     int64_t cuts[kMaxCtas + 1];
@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             mbar_init(&s.pv_done[i], 1);
             mbar_init(&s.group[i], kRowsM);
         }
+        mbar_init(&s.drain, 1);
         fence_barrier_init();
     }
     dependency_wait();
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         row.cap2 = p.cap * 1.4426950408889634f;
         auto group_sync = [&] {
             mbar_arrive(&s.group[m]);
-            if (ok) ok = mbar_wait(&s.group[m], syncs & 1);
+            if (ok) ok = warp_wait(&s.group[m], syncs & 1);
             ++syncs;
         };
         while (walk.n > 0) {
@@ -874,6 +875,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 }
                 for (int m = 0; m < ms; ++m) ++pieces[m];
                 if (!ok || !uniform(walk.next(a))) break;
+            }
+            if (!ok) {  // shared memory and TMEM are given back with no product under way
+                tc_commit_by(leader, &s.drain);
+                warp_wait(&s.drain, 0);
             }
         }
     } else if (warp == kLoadWarp) {

@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         const uint64_t step0 = a.rope.step[2 * lane], step1 = a.rope.step[2 * lane + 1];
         while (walk.n > 0) {
             const int sl = n & 1;
-            if (n >= 2 && !mbar_wait(&s.qempty[sl], ((n >> 1) - 1) & 1)) {
+            if (n >= 2 && !warp_wait(&s.qempty[sl], ((n >> 1) - 1) & 1)) {
                 if (lane == 0) atomicOr(a.status, kDevStatusTimeout);
                 break;
             }
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             }
             if (!walk.next(index)) break;
         }
-        if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+        if (!ok) atomicOr(a.status, kDevStatusTimeout);  // (any lane's)
         return;
     }
 
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         if (lane == 0) mbar_arrive(&s.rfull);
         if (!walk.next(index)) break;
     }
-    if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+    if (!ok) atomicOr(a.status, kDevStatusTimeout);
 }
 
 // A wait by parity is sound only for the phase after the last one that the same

@@ -322,7 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
         int passes = 0;             // pairs of queries handed over so far
         for (int n = 0; (int)blockIdx.x < meta.ctas; ++n) {
             const int sl = n & 1;
-            ok = ok && mbar_wait(&s.qfull[sl], (n >> 1) & 1);
+            // One outcome for the warp: a lane that left alone would leave the others in a vote.
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&s.qfull[sl], (n >> 1) & 1));
             if (!ok) break;  // (all that follow give up too)
             const Slot& slot = s.slot[sl];
             const int pairs = slot.pairs, tiles = slot.tiles, tile0 = slot.tile;
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             const uint64_t step0 = a.rope.step[2 * lane], step1 = a.rope.step[2 * lane + 1];
             for (int n = 0; walk.n > 0; ++n) {
                 const int sl = n & 1;
-                if (n >= 2 && !mbar_wait(&s.qempty[sl], ((n >> 1) - 1) & 1)) {
+                if (n >= 2 && !warp_wait(&s.qempty[sl], ((n >> 1) - 1) & 1)) {
                     ok = false;
                     break;
                 }
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             }
         }
     }
-    if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+    if (!ok) atomicOr(a.status, kDevStatusTimeout);  // (any lane's)
 }
 
 constexpr int kSmemBytes = 1024 + kStages * kStageBytes + (int)sizeof(Shared);

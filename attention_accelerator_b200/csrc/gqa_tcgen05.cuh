@@ -140,10 +140,4 @@ __device__ __forceinline__ void tc_commit_by(uint32_t leader, uint64_t* bar) {
         : "memory");
 }
 
-// Bounded wait with one outcome for the whole warp, so that the warp-wide
-// tcgen05.ld / tcgen05.st that follow are never reached by part of it.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
-
 }  // namespace gqa
