@@ -133,10 +133,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
     }
     __syncthreads();
 
-    // (64 bits: max_tokens and the stack may come within a step of 2^31.)
-    const int64_t stride = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
+    // (Unsigned: max_tokens and the stack may come within a step of 2^31.)
+    const uint32_t stride = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
     const int n_tokens = tokens[n], n_need = ok ? needs[n] : 0, n_give = ok ? gives[n] : 0;
-    for (int64_t r = first; r <= n; r += stride) a.first_token[r] = tokens[r];
+    for (uint32_t r = first; r <= (uint32_t)n; r += stride) a.first_token[r] = tokens[r];
     // Page given back number i: its request is the last whose sum is at most i
     // and which gives any (requests that give none repeat the next one's sum).
     auto given = [&](int i) {
@@ -145,10 +145,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
     };
     // Page popped number j: the top of the stack with this call's pages pushed on it.
     auto popped = [&](int j) { return j < n_give ? given(n_give - 1 - j) : a.free_pages[n_free - 1 - (j - n_give)]; };
-    for (int64_t t = first; t < a.max_tokens; t += stride) {
+    for (uint32_t t = first; t < (uint32_t)a.max_tokens; t += stride) {
         int64_t slot = -1;
         int pos = -1;
-        if (t < n_tokens) {
+        if (t < (uint32_t)n_tokens) {
             const int r = last_at_most(tokens, n, (int)t);
             const int len = a.lens[r], held = pages_of(len);
             pos = len + ((int)t - tokens[r]);
@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
         a.slots[t] = slot;
         a.positions[t] = pos;
     }
-    for (int64_t j = first; j < n_need; j += stride) {
+    for (uint32_t j = first; j < (uint32_t)n_need; j += stride) {
         const int r = last_at_most(needs, n, (int)j);
         a.block_table[r * a.table_stride + pages_of(a.lens[r]) + ((int)j - needs[r])] = popped((int)j);
     }
-    for (int64_t i = first; i < n_give; i += stride) a.free_pages[n_free + i] = given((int)i);
+    for (uint32_t i = first; i < (uint32_t)n_give; i += stride) a.free_pages[n_free + (int)i] = given((int)i);
     if (blockIdx.x == 0 && tid == 0) {
         a.counts[0] = n_tokens;
         a.counts[1] = n_need;
