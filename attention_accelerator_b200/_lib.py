@@ -43,6 +43,8 @@ GQA_FLAG_K_ROTATED = 0x2
 GQA_FLAG_Q_ROTATED = 0x4
 PARTIAL_FLOATS = 132
 
+GQA_CAPTURE_RELAXED = 2
+
 GQA_CODE_INT8 = 0
 GQA_CODE_E4M3 = 1
 PAGED_MAX_BATCH = 8192
@@ -149,6 +151,7 @@ _SIGNATURES = {
     "gqa_mem_decode": (ctypes.c_int, [_P, ctypes.c_size_t, ctypes.c_int, _P, ctypes.c_uint64, _P, _P,
                                       ctypes.c_size_t, _P]),
     "gqa_mem_encode_bytes": (ctypes.c_size_t, [ctypes.c_uint64, ctypes.c_int]),
+    "gqa_capture_mode": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
     "gqa_plan_pages": (ctypes.c_int, [_P, _P, ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int, _P,
                                       ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "gqa_append_paged": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,

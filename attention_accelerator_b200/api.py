@@ -101,9 +101,29 @@ def _workspace(device: torch.device, stream_ptr: int, nbytes: int) -> torch.Tens
         if buf is None or buf.numel() < nbytes:
             if buf is not None:
                 _ws_retired.append(buf)
-            buf = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
+            buf = _zeroed(max(nbytes, 4096), device)
             _ws[key] = buf
         return buf
+
+
+def _zeroed(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Zeros for the current stream's calls.  While that stream captures a CUDA graph its own allocations and memsets
+    belong to the graph, and the buffer would be zero only once that graph had run: then from another stream, by now."""
+    if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    lib, mode = _lib.load(), ctypes.c_int(0)
+    _check(lib.gqa_capture_mode(_lib.GQA_CAPTURE_RELAXED, ctypes.byref(mode)), "gqa_capture_mode")
+    try:
+        for _ in range(64):  # (streams come round: one that captures, this one among them, is passed over)
+            side = torch.cuda.Stream(device)
+            with torch.cuda.stream(side):
+                if not torch.cuda.is_current_stream_capturing():
+                    buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+                    side.synchronize()
+                    return buf
+    finally:
+        _check(lib.gqa_capture_mode(mode.value, ctypes.byref(mode)), "gqa_capture_mode")
+    raise GqaError(_lib.GQA_ERR_CUDA, "no stream to make a workspace on: every one is capturing")
 
 
 # torch's own lookup of the current stream's handle, without the Stream object (2 us a call).

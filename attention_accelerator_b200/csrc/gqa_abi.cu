@@ -882,4 +882,13 @@ int gqa_read_status(void* workspace, void* stream, int* device_status) {
     return GQA_OK;
 }
 
+int gqa_capture_mode(int mode, int* before) {
+    if (!before) return GQA_ERR_NULL_POINTER;
+    if (mode < cudaStreamCaptureModeGlobal || mode > cudaStreamCaptureModeRelaxed) return GQA_ERR_FLAGS;
+    cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(mode);
+    if (cudaThreadExchangeStreamCaptureMode(&m) != cudaSuccess) return GQA_ERR_CUDA;
+    *before = m;
+    return GQA_OK;
+}
+
 }  // extern "C"

@@ -9,7 +9,8 @@ The cache is a pool of pages of ``page_len`` tokens; every (page, KV head) block
     out = decode_paged_chunked(q, cache, block_table, plan.lens, plan.first_token)    # any number
 
 with every length in device memory: no call waits for the GPU, and a captured CUDA graph of the step follows the
-lengths.  K is rotated when it is appended (as :func:`rope_k_cache` does for a BF16 cache), Q when it is used.
+lengths.  A graph keeps the workspace of the stream that it was captured on: graphs captured on one stream, and that
+stream's own calls, are not to run at the same time.  K is rotated when it is appended (as :func:`rope_k_cache` does for a BF16 cache), Q when it is used.
 
 The geometry is the library's: 4 Q heads to each KV head and 128 dims; 1 to 8 KV heads (a head shard's cache holds
 only its own).  Everything runs in ``lib/libgqa_b200.so``; the C side is ``include/gqa_b200.h``.

@@ -417,6 +417,18 @@ int gqa_decode_exchange(const void *q, const void *k, const void *v, void *out, 
                         void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * Sets how far CUDA graph captures restrict this thread's calls (GQA_CAPTURE_*,
+ * cudaStreamCaptureMode's values) and returns in `before` what it was.  A workspace
+ * that a captured call is the first to use has to be zero before the graph runs: a
+ * memset on the capturing stream is a node of that graph.  In relaxed mode the
+ * thread may allocate it, set it to zero on a stream that captures nothing and wait.
+ */
+#define GQA_CAPTURE_GLOBAL 0
+#define GQA_CAPTURE_THREAD_LOCAL 1
+#define GQA_CAPTURE_RELAXED 2
+int gqa_capture_mode(int mode, int *before);
+
+/*
  * Read (and clear) the device status word a kernel leaves in `workspace`:
  * GQA_OK, or GQA_ERR_DEVICE_TIMEOUT if a bounded wait gave up.  Synchronises
  * `stream`.  Plays the part of ERROR_FLAGS/STATUS (axi_lite_regs.v:153-157,178).

@@ -150,6 +150,13 @@ def test_c_refuses_what_only_one_call_takes():
         assert lib.gqa_plan_pages(*args) == getattr(_lib, "GQA_ERR_" + want), (at, value)
 
 
+def test_capture_mode_refuses_what_is_no_mode():
+    lib, before = _lib.load(), ctypes.c_int(-1)
+    for mode in (-1, 3):
+        assert lib.gqa_capture_mode(mode, ctypes.byref(before)) == _lib.GQA_ERR_FLAGS and before.value == -1
+    assert lib.gqa_capture_mode(_lib.GQA_CAPTURE_RELAXED, None) == _lib.GQA_ERR_NULL_POINTER
+
+
 def test_oracle_plan_allocates_every_page_once():
     table, free = [[-1] * 4 for _ in range(3)], list(range(8))
     ok, lens, first, slots, positions, taken, given = ref.plan_step([0, 0, 0], [17, 0, 16], table, free, 16, 40, 8)

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import attention_accelerator_b200 as gqa
-from test_paged_gpu import ints
+from attention_accelerator_b200 import api
+from test_paged_gpu import Setup, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +42,73 @@ def test_an_append_of_as_many_rows_as_an_int32_counts():
     assert k[:, 0, 0].tolist() == [0.0, 3.0, 3.0, 0.0]
     del slots, row
     torch.cuda.empty_cache()
+
+
+def test_graphs_captured_without_a_warm_up(monkeypatch):
+    """Two steps captured on a stream that has run nothing: each replays first, in any order, whatever the memory
+    behind their workspaces held, and the stream's own calls beside them."""
+    page_len, lens = 64, [5000, 3]
+    side = torch.cuda.Stream()
+    graphs, steps = [], []
+    for seed in (81, 82):
+        s = Setup(lens, seed=seed, page_len=page_len, width=120, spare=40)
+        q, qc = s.queries(2), s.queries(70)
+        held, new, spare = ints(lens), ints([1500, 1]), ints(s.unused + [-1] * 100)
+        table, n_free = ints(s.table), ints([0])
+        state = dict(table=table, spare=spare, held=held)
+        start = {k: v.clone() for k, v in state.items()}
+        n_free.fill_(len(s.unused))
+        count = n_free.clone()
+
+        def step(s=s, q=q, qc=qc, state=state, new=new, n_free=n_free):
+            a = gqa.decode_paged(q, s.cache, state["table"], state["held"])
+            b = gqa.decode_paged_chunked(qc, s.cache, state["table"], state["held"], first)
+            plan = gqa.plan_pages(state["held"], new, state["table"], state["spare"], n_free, page_len=page_len,
+                                  max_tokens=1600)
+            return a, b, plan.lens, plan.n_free, plan.slots
+
+        first = ints([0, 67, 70])
+        steps.append((step, state, start, n_free, count))
+    torch.cuda.synchronize()
+
+    def restore(i):
+        _, state, start, n_free, count = steps[i]
+        for name, t in state.items():
+            t.copy_(start[name])
+        n_free.copy_(count)
+
+    want = []
+    for i in range(2):
+        want.append([t.clone() for t in steps[i][0]()])
+        restore(i)
+    zeros, nodes = torch.zeros, []
+
+    def spy(*args, **kw):
+        nodes.append(torch.cuda.is_current_stream_capturing())
+        return zeros(*args, **kw)
+
+    monkeypatch.setattr(torch, "zeros", spy)
+    torch.cuda.synchronize()
+    for key in [k for k in api._ws if k[1] in (side.cuda_stream, ("paged", side.cuda_stream))]:
+        api._ws_retired.append(api._ws.pop(key))  # (streams come round: another test's workspace is not this one's)
+    known = set(api._ws)
+    for step, *_ in steps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = step()
+        graphs.append((g, out))
+    made = set(api._ws) - known
+    assert nodes and not any(nodes)  # none is zeroed by a node of a graph
+    assert made and not any(bool(api._ws[key].any()) for key in made)  # zero before either graph has run
+    for i in (1, 0, 0, 1):
+        graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(graphs[i][1], want[i]):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        restore(i)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = steps[0][0]()
+    side.synchronize()
+    for a, b in zip(got, want[0]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
