@@ -735,9 +735,12 @@ int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, i
     a.free_capacity = free_capacity;
     a.page_shift = shift;
     a.max_tokens = max_tokens;
+    // The limit is the kernel's, not the call's: always the same, so that another thread's call does not lower it
+    // before this one's launch.
+    constexpr int kMostSmem = 3 * (GQA_PAGED_MAX_BATCH + 1) * (int)sizeof(int32_t);
     const size_t smem = 3 * (size_t)(requests + 1) * sizeof(int32_t);
     if (smem > 40 * 1024 && cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)smem) != cudaSuccess)
+                                                 kMostSmem) != cudaSuccess)
         return GQA_ERR_CUDA;
     const int64_t items = max_tokens > requests ? max_tokens : requests;
     int64_t grid = (items + kPlanThreads - 1) / kPlanThreads;

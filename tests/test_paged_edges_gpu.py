@@ -2,6 +2,8 @@
 call: one token a sequence, a few queries a sequence (at most 6 rows of one on average, 12 in all) and chunks."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -112,3 +114,27 @@ def test_graphs_captured_without_a_warm_up(monkeypatch):
     side.synchronize()
     for a, b in zip(got, want[0]):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_plans_of_different_sizes_from_two_threads():
+    """Each thread plans for its own number of requests on its own stream: none is refused for the other's sake."""
+    failed = []
+
+    def work(requests):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                zeros = torch.zeros(requests, dtype=torch.int32, device="cuda")
+                table = torch.zeros(requests, 1, dtype=torch.int32, device="cuda")
+                for _ in range(2000):
+                    plan = gqa.plan_pages(zeros, zeros, table, zeros, zeros[:1], page_len=16, max_tokens=1)
+                plan.check()
+        except Exception as e:  # noqa: BLE001 -- whatever it is, the test shows it
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(n,)) for n in (3500, 8192, 5000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
