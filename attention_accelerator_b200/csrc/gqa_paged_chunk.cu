@@ -427,7 +427,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 // ---- Q: 16 pairs of this lane's query, 4 heads ----
                 {
                     const int q4 = lane & 3;
-                    const float unit = kCap ? p.scale / p.cap : p.scale * 1.4426950408889634f;
+                    // The scale's sign goes into Q, so that a row's factor is not negative (nor are the pages' scales)
+                    // and the largest of 16 products is the largest of their scores.
+                    const float unit = fabsf(kCap ? p.scale / p.cap : p.scale * 1.4426950408889634f);
+                    const int sign = __float_as_int(p.scale) & (int)0x80000000;
                     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
                     const uint4* q = reinterpret_cast<const uint4*>(
                         p.q + (int64_t)(un.row0 + token) * p.q_row_stride + walk.h * kGroup * p.q_head_stride + 16 * q4);
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         const int e = min(253, max(1, (int)(top >> 23) + 1));
                         if (hq == head)
                             row.factor = top < 0x7f800000u ? unit * __int_as_float(e << 23) : __int_as_float(0x7fffffff);
-                        down[hq] = __int_as_float((254 - e) << 23);
+                        down[hq] = __int_as_float((254 - e) << 23 | sign);
                     }
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {  // 8 pairs: 16 bytes of each block
@@ -562,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     float mx = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        // The largest of 16 keys, then their scale: it is not negative.
+                        // The largest of 16 keys, then their factor: it is not negative.
                         float top = fmaxf(z[16 * i], z[16 * i + 1]);
 #pragma unroll
                         for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(top, z[16 * i + e]), z[16 * i + e + 1]);

@@ -2,16 +2,65 @@
 call: one token a sequence, a few queries a sequence (at most 6 rows of one on average, 12 in all) and chunks."""
 from __future__ import annotations
 
+import math
 import threading
 
+import numpy as np
 import pytest
 import torch
 
 import attention_accelerator_b200 as gqa
 from attention_accelerator_b200 import api
-from test_paged_gpu import Setup, ints
+from oracle import paged as ref
+from test_paged_gpu import CHUNK_UNIT, DECODE_UNIT, THETA, Setup, ints
 
 pytestmark = pytest.mark.gpu
+
+#: name -> queries of each of the two sequences of a call that the kernel of that name takes
+KERNELS = {"decode": [1, 1], "few": [5, 2], "chunk": [70, 65]}
+
+
+def unit_of(kernel):
+    return DECODE_UNIT if kernel == "decode" else CHUNK_UNIT
+
+
+def placed(kernel, lens):
+    """(first_query, owner, position) of a call's rows: the last tokens of each sequence."""
+    counts = KERNELS[kernel]
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    owner = [b for b, n in enumerate(counts) for _ in range(n)]
+    return first, owner, [lens[b] - n + i for b, n in enumerate(counts) for i in range(n)]
+
+
+def attend(kernel, q, cache, table, lens, first, **more):
+    if kernel == "decode":
+        return gqa.decode_paged(q, cache, table, lens, **more)
+    return gqa.decode_paged_chunked(q, cache, table, lens, ints(first), **more)
+
+
+def close(got, q, setup, owner, positions, *, unit, theta=THETA, q_rotated=False, cap=0.0, slopes=None, starts=None,
+          scale=1 / math.sqrt(128), floor=2.0 ** -22):
+    """Every output against 64 bits.  A score is off by 2 units of the sum of its terms' sizes (Q, and K's or the cap's
+    rounding), FP32's 2^-19 of that and 2^-22 of the bias -- nothing that grows with the cap alone; a weight by e to
+    twice that, 3 units and 2^-20; the output by its BF16 rounding, and by ``floor`` of its row's largest sum of
+    |weight * value|: weights below FP16's range (2^-31 of the largest weight times scale, a few hundred of them)."""
+    got = got.float().cpu().numpy().astype(np.float64)
+    x = q.float().cpu().numpy().astype(np.float64)
+    if not q_rotated:
+        x = ref.rope(x, np.array(positions), theta)
+    slopes = slopes.cpu().numpy().astype(np.float64) if slopes is not None else None
+    kv = {b: setup.values(b) for b in set(owner)}
+    for i, (b, m) in enumerate(zip(owner, positions)):
+        p = np.arange(setup.lens[b])
+        seen = (p >= (starts[i] if starts is not None else 0)) & (p <= m)
+        k, v = kv[b]
+        out, size, most = ref.attend(x[i], k, v, m, seen, scale=scale, cap=cap, slopes=slopes)
+        far = np.abs(m - p).max() * slopes.max() if slopes is not None and len(p) else 0.0
+        z = (2 * unit + 2.0 ** -19) * most + 2.0 ** -22 * far
+        tol = (2.0 ** -8 * np.abs(out) + (math.expm1(2 * z) + 3 * unit + 2.0 ** -20) * size * 1.01
+               + floor * size.max(-1, keepdims=True) + 1e-37)
+        bad = ~(np.abs(got[i] - out) <= tol)
+        assert not bad.any(), (i, b, m, int(bad.sum()), got[i][bad][:4], out[bad][:4])
 
 
 def test_the_longest_slot_list():
@@ -138,3 +187,18 @@ def test_plans_of_different_sizes_from_two_threads():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("scale,loud", [(-0.1, 1), (-0.3, 8), (0.3, 8)])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_scores_of_either_sign_of_the_scale(kernel, scale, loud, code):
+    """Softmax of -z is as good as that of z: over several whole tiles, with queries large enough for weights far apart."""
+    lens = [700, 641]
+    s = Setup(lens, seed=71, page_len=32, code=code)
+    first, owner, pos = placed(kernel, lens)
+    q = s.queries(first[-1]) * loud
+    got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, scale=scale)
+    close(got, q, s, owner, pos, unit=unit_of(kernel), scale=scale)
+    got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, scale=scale, score_cap=5.0)
+    close(got, q, s, owner, pos, unit=unit_of(kernel), scale=scale, cap=5.0)
