@@ -617,7 +617,9 @@ int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_pag
     call->rows = p->rows;
     call->table_width = p->table_width;
     call->scale = p->scale;
-    call->cap = p->score_cap;
+    // In FP32 a cap beyond 2^96 leaves the scores as they are and one below 2^-96 makes them 0, within 2^-96; in
+    // between the products with it are normal numbers.
+    call->cap = p->score_cap > 0x1p96f ? 0.f : p->score_cap > 0.f && p->score_cap < 0x1p-96f ? 0x1p-96f : p->score_cap;
     call->q_rotated = (p->flags & GQA_FLAG_Q_ROTATED) != 0;
     // Key positions, a tile past them, and tile counts are 32-bit.
     if ((int64_t)p->table_width * c->page_len > 1 << 30 ||

@@ -148,11 +148,39 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// tanh to about 2^-22: 1 - 2 / (e^2x + 1).
-__device__ __forceinline__ float tanh_fast(float x) {
+// tanh, to a few 2^-23 of itself however small it is: a cap far above the scores
+// multiplies it back, so that an absolute error would grow with the cap.
+// Up to |x| = 1/2 as x times a polynomial in t = x^2, interpolated at the Chebyshev
+// points of tanh(x) / x (2^-26 of it); beyond as 1 - 2 / (e^2x + 1).
+constexpr float kTanhNear = 0.25f;  // of t
+__device__ __forceinline__ float tanh_near(float x, float t) {
+    float p = fmaf(0.0171313453f, t, -0.0529842377f);
+    p = fmaf(p, t, 0.13324751f);
+    p = fmaf(p, t, -0.333330691f);
+    return x * fmaf(p, t, 1.f);
+}
+__device__ __forceinline__ float tanh_far(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * 2.8853900817779268f) + 1.f));
     return fmaf(-2.f, r, 1.f);
+}
+
+// cap2 * tanh of a warp's scores, kN a lane (a multiple of the cap in, log2 units out).
+template <int kN>
+__device__ __forceinline__ void cap_scores(float (&z)[kN], float cap2) {
+    float x[kN];
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        x[i] = z[i];
+        const float t = x[i] * x[i];
+        far |= t > kTanhNear;
+        z[i] = cap2 * tanh_near(x[i], t);
+    }
+    if (__any_sync(0xffffffffu, far))
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (x[i] * x[i] > kTanhNear) z[i] = cap2 * tanh_far(x[i]);
 }
 
 // Rows of a page from `row` on (as many as the map's box) of K or V of a head.

@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                             z[e] = y.x;
                             z[e + 1] = y.y;
                         }
-                        if (__any_sync(0xffffffffu, most > 0.25f)) {
+                        if (__any_sync(0xffffffffu, most > kTanhNear)) {
 #pragma unroll 1
                             for (int i = 0; i < 8; ++i) {
                                 uint32_t v[16];
@@ -526,8 +526,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                                 const float g = row.factor * sc.k[i];
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    v[e] = __float_as_uint(row.cap2 * tanh_fast(__uint_as_float(v[e]) * g));
+                                for (int e = 0; e < 16; ++e) {
+                                    const float x = __uint_as_float(v[e]) * g, t = x * x;
+                                    v[e] = __float_as_uint(row.cap2 * (t > kTanhNear ? tanh_far(x) : tanh_near(x, t)));
+                                }
                                 tmem_st16(t_s + 16 * i, v);
                             }
                             tmem_wait_st();

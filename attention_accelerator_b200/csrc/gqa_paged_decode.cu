@@ -194,12 +194,7 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
             z[i][1] = (s[2] + s[3]) * f;
         }
     }
-    if constexpr (kCap) {
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) z[i][e] = cap2 * tanh_fast(z[i][e]);
-    }
+    if constexpr (kCap) cap_scores(reinterpret_cast<float(&)[2 * kSteps]>(z), cap2);
     if constexpr (kBias) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)

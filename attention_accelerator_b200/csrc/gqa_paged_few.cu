@@ -176,13 +176,17 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
         for (int i = 0; i < kSteps; ++i) {
             const float f = i >> sh ? sc.y : sc.x, f0 = f * factor.x, f1 = f * factor.y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x = z[n][i][e] * (e & 1 ? f1 : f0);
-                if constexpr (kCap) x = cap2 * tanh_fast(x);
-                if constexpr (kBias)
-                    x = fmaf(-slot.slope[t], fabsf((float)(slot.m + 2 * n + (e & 1) - (key0 + 16 * i + 8 * (e >> 1) + g))), x);
-                z[n][i][e] = x;
-            }
+            for (int e = 0; e < 4; ++e) z[n][i][e] *= e & 1 ? f1 : f0;
+        }
+        if constexpr (kCap) cap_scores(reinterpret_cast<float(&)[4 * kSteps]>(z[n]), cap2);
+        if constexpr (kBias) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    z[n][i][e] = fmaf(-slot.slope[t],
+                                      fabsf((float)(slot.m + 2 * n + (e & 1) - (key0 + 16 * i + 8 * (e >> 1) + g))),
+                                      z[n][i][e]);
         }
     }
     if (edge) blank(-INFINITY);

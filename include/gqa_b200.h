@@ -566,6 +566,7 @@ int gqa_read_paged(const gqa_paged_cache *cache, const int64_t *slots, int n, vo
  * Attention over the paged cache.  Query row i (of sequence b, at position m,
  * rotated at m unless GQA_FLAG_Q_ROTATED) and Q head qh of KV head h = qh / 4:
  *   z_p = scale * <q, K_p>;  with score_cap > 0: z_p = cap * tanh(z_p / cap);
+ *   (any finite cap: beyond 2^96 it is none, below 2^-96 it is 2^-96);
  *   with slopes: z_p -= slopes[qh] * |m - p|;
  *   visible keys: max(0, doc_starts[i]) <= p < min(seq_lens[b], max(m + 1, prefix_ends[i]));
  *   out = softmax(z) V over the visible keys, BF16; a row that sees no key is 0.

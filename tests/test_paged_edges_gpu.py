@@ -202,3 +202,15 @@ def test_scores_of_either_sign_of_the_scale(kernel, scale, loud, code):
     close(got, q, s, owner, pos, unit=unit_of(kernel), scale=scale)
     got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, scale=scale, score_cap=5.0)
     close(got, q, s, owner, pos, unit=unit_of(kernel), scale=scale, cap=5.0)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("cap", [1e-38, 1e-30, 1.0, 50.0, 1e4, 1e6, 1e8, 1e20, 1e30, 3e38])
+def test_caps_of_every_size(kernel, cap):
+    """A cap far above the scores changes nothing, one far below them makes the weights equal."""
+    lens = [700, 150]
+    s = Setup(lens, seed=72, page_len=16, code="e4m3")
+    first, owner, pos = placed(kernel, lens)
+    q = s.queries(first[-1]) * 4
+    got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, score_cap=cap)
+    close(got, q, s, owner, pos, unit=unit_of(kernel), cap=float(np.float32(cap)))
