@@ -143,6 +143,29 @@ __device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi)
     }
 }
 
+// V's scales join the weights as exponents: the weights of a row for the product
+// with V's codes are 2^(z + log2(V scale) - m), m the row's reference for this sum,
+// so that what a row does not see, or gives no weight, takes no bits from what it
+// does; their sum, which divides, takes each page's scale out again in FP32 (1 /
+// scale is kept as kWeightUnit / scale: up to 2^121, the scale of BF16's largest
+// number, no part of it passes FP32's range).  A block of zeros has the smallest
+// scale that an append writes, 2^-100, and a page never written one of 0: such
+// blocks count as zeros, with 2^-60 in their scale's place, so that their keys'
+// weights stay in the sum beside pages of 2^-80 to 2^60.
+constexpr float kWeightUnit = 0x1p-12f, kNoVScale = 0x1p-100f;
+struct VScale {
+    float log2, inv;  // of a page's V scale; inv times kWeightUnit
+    bool some;        // not zeros
+};
+__device__ __forceinline__ VScale v_scale_of(float s) {
+    const bool some = s > kNoVScale;
+    // Exponent and fraction apart: the fraction's logarithm is good to 2^-22 of 1.
+    const uint32_t bits = __float_as_uint(some ? fminf(s, 0x1.fffffep121f) : 0x1p-60f);
+    const int e = (int)(bits >> 23) - 127;
+    const float f = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+    return VScale{(float)e + __log2f(f), __fdividef(kWeightUnit, f) * __uint_as_float((uint32_t)(127 - e) << 23), some};
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);

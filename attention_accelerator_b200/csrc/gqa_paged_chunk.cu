@@ -13,10 +13,10 @@
 // Precision.  Codes become FP16 exactly for S = Q K^T; Q is rotated in FP32,
 // divided by a power of two that brings the row's largest below 1, and rounded to
 // FP16 (2^-11 of a term: three more bits than the BF16 it came as).  K's scale
-// multiplies the FP32 scores.  V's scale, over a running power of two, multiplies
-// its codes in FP16, the weights 2^(z - m) round to FP16, and O accumulates in
-// FP32 in TMEM: together a few 2^-11 of the sum of |weight * value| at worst, for
-// an output that is rounded to 2^-8.
+// multiplies the FP32 scores.  V's codes are exact too: its scale joins the weights,
+// 2^(z + log2(V scale) - m), which round to FP16, and O accumulates in FP32 in TMEM:
+// together a few 2^-11 of the sum of |weight * value|, and 2^-31 of the row's largest
+// weight times scale for each key, for an output that is rounded to 2^-8.
 //
 // Warps (one CTA per SM):
 //   0-3, 4-7   softmax of M tile 0, 1: a thread a row.  Per unit, 4 lanes rotate one
@@ -73,7 +73,7 @@ static_assert(2 * kSoftmaxRegs + kConvRegs + kRestRegs <= 4 * kLaunchRegs, "of w
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256;  // two of 128 columns each; P over the first 64 of its S
 constexpr float kHeadroom = 8.f;   // log2 by which a maximum may pass the reference
-constexpr float kLift = 7.f;       // weights are 2^(z - m + 7): up to 2^15, and FP16's 2^-24 is 2^-31 of the reference
+constexpr float kLift = 7.f;       // weights are 2^(7 ..): up to 2^15, and FP16's 2^-24 is 2^-31 of the reference
 
 constexpr int kSlotFloats = kRowsM * 2 * (kHeadDim + 2);  // a partial: acc [32][256] float4, (m, l) [256]
 
@@ -82,9 +82,10 @@ constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 2
 constexpr uint32_t kIdescO = kIdescS | (1u << 16);  // B (V) MN-major
 
 struct TileScales {
-    float k[8], v[8];   // of each 16 keys: K's scale (NaN where V's is no number), V's over the reference
-    float fall, ref;    // what O is multiplied by before this tile; the reference
-    float pad[2];
+    float k[8];                 // of each 16 keys: K's scale (NaN where V's is no number)
+    float v_log2[8], v_inv[8];  // and V's, as VScale has it
+    uint32_t v_some;            // bits: V is not zeros
+    uint32_t pad[7];
 };
 
 struct alignas(16) Shared {
@@ -294,24 +295,21 @@ __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map,
         : "memory");
 }
 
-// V's operand: codes times their scale.  A NaN code would reach, times a weight of
-// zero, the rows that do not see its key: the maximum with -448 makes it a number.
+// V's operand.  A NaN code would reach, times a weight of zero, the rows that do not
+// see its key: the maximum with -448 makes it a number.
 template <int kCode>
-__device__ __forceinline__ uint32_t scale_half2(uint32_t a, __half2 b) {
-    __half2 v = *reinterpret_cast<const __half2*>(&a);
-    if constexpr (kCode == GQA_CODE_E4M3) v = __hmax2(v, __half2half2(__ushort_as_half(0xdf00)));
-    v = __hmul2(v, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint32_t numbers(uint32_t a) {
+    if constexpr (kCode == GQA_CODE_E4M3) {
+        const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0xdf00)));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return a;
 }
 
 // tanh(x) / x = sum of kTanh[i] x^2i for |x| <= 1/2, within 2^-15 of it (a quarter of
 // what a weight's rounding to FP16 moves at a score of 4): interpolated at the
 // Chebyshev points of x^2.
 __device__ constexpr float kTanh[3] = {0.99997777f, -0.33170217f, 0.11525216f};
-
-__device__ __forceinline__ float finite_or(float x, float other) {
-    return fabsf(x) <= 3.402823466e38f ? x : other;
-}
 
 // The larger magnitude of two BF16 codes, as FP32 bits (which order as integers).
 __device__ __forceinline__ uint32_t magnitudes(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
@@ -483,8 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     fence_proxy_async_smem();
                     mbar_arrive(&s.q_full[m]);
                 }
-                float ref = -INFINITY;   // weights are 2^(z - ref)
-                float l = 0.f, vref = 0.f;
+                float ref = -INFINITY;   // weights for O are 2^(z + log2(V scale) - ref)
+                float l = 0.f;           // their sum without that scale, times kWeightUnit
                 for (int j = 0; j < walk.n; ++j) {
                     if (!warp_wait(&s.s_full[m], (seen + j) & 1)) {
                         ok = false;
@@ -571,53 +569,52 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         float top = fmaxf(z[16 * i], z[16 * i + 1]);
 #pragma unroll
                         for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(top, z[16 * i + e]), z[16 * i + e + 1]);
-                        mx = fmaxf(mx, kCap || kBias ? top : top * f[i]);
+                        mx = fmaxf(mx, kCap || kBias ? top + sc.v_log2[i] : fmaf(top, f[i], sc.v_log2[i]));
                     }
                     // The reference moves when the maximum passes it by 2^kHeadroom (at once from nothing).
                     const float want = mx - kLift;
                     const bool move = want > ref + kHeadroom || (ref == -INFINITY && want > ref);
                     const float to = move ? want : ref;
-                    const float fall = j > 0 ? sc.fall : 1.f;
-                    if (__any_sync(0xffffffffu, move) || fall != 1.f) {
+                    if (__any_sync(0xffffffffu, move)) {
                         const float alpha = move ? fast_exp2(ref - to) : 1.f;
                         l *= alpha;
                         ref = to;
                         if (j > 0) {
-                            const float f = alpha * fall;
 #pragma unroll 1
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t o[32];
                                 tmem_ld32(t_o + 32 * c, o);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
                                 tmem_st32(t_o + 32 * c, o);
                             }
                         }
                     }
-                    vref = sc.ref;
                     const float use = ref == -INFINITY ? 0.f : ref;
-                    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t w[16];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float2 x = make_float2(z[32 * c + e], z[32 * c + e + 1]);
-                            const float2 less = make_float2(-use, -use);
-                            if constexpr (kCap || kBias) {
-                                x = __fadd2_rn(x, less);
-                            } else {
-                                const float g = f[2 * c + (e >> 4)];
-                                x = __ffma2_rn(x, make_float2(g, g), less);
+                        for (int half = 0; half < 2; ++half) {  // 16 keys of one page
+                            const int i = 2 * c + half;
+                            const float off = sc.v_log2[i] - use;
+                            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                float2 x = make_float2(z[16 * i + e], z[16 * i + e + 1]);
+                                if constexpr (kCap || kBias)
+                                    x = __fadd2_rn(x, make_float2(off, off));
+                                else
+                                    x = __ffma2_rn(x, make_float2(f[i], f[i]), make_float2(off, off));
+                                x = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                                sum = __fadd2_rn(sum, x);
+                                w[8 * half + (e >> 1)] = pack_half2(x.x, x.y);
                             }
-                            x = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-                            sum = __fadd2_rn(sum, x);
-                            w[e >> 1] = pack_half2(x.x, x.y);
+                            l = fmaf(sum.x + sum.y, sc.v_inv[i], l);
                         }
                         tmem_st16(t_s + 16 * c, w);  // over columns that were read
                     }
-                    l += sum.x + sum.y;
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&s.p_full[m]);
@@ -641,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     }
                 };
                 if (walk.n == un.tiles) {
-                    const float f = l == 0.f ? 0.f : vref / l;  // a row that sees nothing is 0
+                    const float f = l == 0.f ? 0.f : kWeightUnit / l;  // a row that sees nothing is 0
                     float x[kHeadDim];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) tmem_ld32(t_o + 32 * c, reinterpret_cast<uint32_t(&)[32]>(x[32 * c]));
@@ -678,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
                             for (int e = 0; e < kHeadDim / 4; ++e)
                                 reinterpret_cast<float4*>(mine)[e * 2 * kRowsM + prow] =
-                                    make_float4(x[4 * e] * vref, x[4 * e + 1] * vref, x[4 * e + 2] * vref, x[4 * e + 3] * vref);
+                                    make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
                         if (real)
                             reinterpret_cast<float2*>(mine + 2 * kRowsM * kHeadDim)[prow] = make_float2(ref, l);
                     }
@@ -714,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                             const float2 v = ml(c);
                             L = fmaf(fast_exp2(v.x - mu), v.y, L);
                         }
-                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        const float inv = L == 0.f ? 0.f : kWeightUnit / L;
 #pragma unroll 1
                         for (int half = 0; half < 2; ++half) {
                             float x[64];
@@ -773,8 +770,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int row = row0 + 8 * i, sw = row & 7;
-                        const __half2 f = __float2half2_rn(kv ? sc.v[2 * cw + (i >> 1)] : 1.f);
-                        const bool gone = kv && (row < klo || row >= khi);  // no row sees it: its codes may be anything
+                        // Where no row sees the key, its codes may be anything.
+                        const bool gone = kv && (row < klo || row >= khi || !(sc.v_some >> (2 * cw + (i >> 1)) & 1));
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const int c = 4 * half + t;  // dims 16 c .. 16 c + 15: block `half`
@@ -786,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                             to_half4<kCode>(x.w, w[6], w[7]);
                             if (kv) {
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) w[e] = gone ? 0u : scale_half2<kCode>(w[e], f);
+                                for (int e = 0; e < 8; ++e) w[e] = gone ? 0u : numbers<kCode>(w[e]);
                             }
                             uint8_t* at = dst + half * kBlockBytes + row * 128;
                             *reinterpret_cast<uint4*>(at + (((2 * t) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -906,7 +903,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             };
             int page = entry(0), page1 = entry(1);
             float ks = scale(p.c.k_scale, page), vs = scale(p.c.v_scale, page);
-            float ref = 0.f;  // V's running power of two
             for (int j = 0; j < walk.n; ++j, ++tile_count) {
                 const int page2 = entry(j + 2);
                 const float ks1 = scale(p.c.k_scale, page1), vs1 = scale(p.c.v_scale, page1);
@@ -916,25 +912,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     if (!ok) break;
                     if (kv == 0) {
                         // Scales of the tile, a lane 16 keys.
-                        const float top = __uint_as_float(
-                            __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(finite_or(vs, 0.f)))));
-                        float fall = 1.f;
-                        if (top > 2.f * ref) {
-                            const float to = __int_as_float(min(253, max(13, __float_as_int(top) >> 23)) << 23);
-                            fall = ref / to;
-                            ref = to;
-                        }
                         const int from = (lane & 7) >> (shift - 4);
                         const float kg = __shfl_sync(0xffffffffu, ks, from), vg = __shfl_sync(0xffffffffu, vs, from);
                         const bool fine = fabsf(vg) <= 3.402823466e38f;
+                        const VScale v = v_scale_of(vg);
+                        const uint32_t some = __ballot_sync(0xffffffffu, lane < 8 && v.some);
                         TileScales& sc = s.scales[tile_count & (kScaleSlots - 1)];
+                        if (lane == 0) sc.v_some = some;
                         if (lane < 8) {
                             sc.k[lane] = fine ? kg : __int_as_float(0x7fffffff);
-                            sc.v[lane] = fine && ref > 0.f ? vg / ref : 0.f;
-                        }
-                        if (lane == 8) {
-                            sc.fall = fall;
-                            sc.ref = ref;
+                            sc.v_log2[lane] = v.log2;
+                            sc.v_inv[lane] = v.inv;
                         }
                         __syncwarp();
                     }

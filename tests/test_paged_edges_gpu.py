@@ -214,3 +214,68 @@ def test_caps_of_every_size(kernel, cap):
     q = s.queries(first[-1]) * 4
     got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, score_cap=cap)
     close(got, q, s, owner, pos, unit=unit_of(kernel), cap=float(np.float32(cap)))
+
+
+def spread(s, scales, owner=0):
+    """V scales of a sequence's pages, first to last (a list, or a function of the page's number)."""
+    for col in range(-(-s.lens[owner] // s.page_len)):
+        s.cache.v_scale[s.table[owner][col]] = scales(col) / (127 if s.code == "int8" else 448)
+
+
+SPREAD = ["chunk"]  # whose V scales may lie far apart
+RATIOS = [2.0 ** -10, 2.0 ** -20, 2.0 ** -24, 2.0 ** -30, 2.0 ** -60]
+
+
+@pytest.mark.parametrize("kernel", SPREAD)
+@pytest.mark.parametrize("ratio", RATIOS)
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("loud_first", [True, False])
+def test_quiet_pages_beside_loud_ones_that_a_row_does_not_see(kernel, ratio, code, loud_first):
+    """Every second row sees none of the loud pages: its output is the quiet pages' to full precision."""
+    lens = [700, 640]
+    s = Setup(lens, seed=73, page_len=16, code=code)
+    first, owner, pos = placed(kernel, lens)
+    cut = 320
+    for b in (0, 1):
+        spread(s, lambda col: (1.0 if (col * 16 < cut) == loud_first else ratio), b)
+    q = s.queries(first[-1])
+    starts = [cut if i % 2 else 0 for i in range(first[-1])]
+    got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, doc_starts=ints(starts))
+    close(got, q, s, owner, pos, unit=unit_of(kernel), starts=starts)
+
+
+@pytest.mark.parametrize("kernel", SPREAD)
+@pytest.mark.parametrize("ratio", RATIOS)
+def test_quiet_pages_beside_loud_ones_of_no_weight(kernel, ratio):
+    """The bias takes the weight of the loud pages, 400 keys away, below 2^-144: what is left is the quiet pages'."""
+    lens = [700, 640]
+    # (One token: among others, so that a warp has several tiles of a sequence.)
+    s = Setup(lens + ([700] * 30 if kernel == "decode" else []), seed=74, page_len=64, code="int8")
+    first, owner, pos = placed(kernel, lens)
+    for b in (0, 1):
+        spread(s, lambda col: 1.0 if col < 3 else ratio, b)
+    q = s.queries(first[-1] if kernel != "decode" else len(s.lens))
+    slopes = torch.full((32,), 0.25, device="cuda")
+    got = attend(kernel, q, s.cache, ints(s.table), ints(s.lens), first, distance_slopes=slopes, q_rotated=True)
+    close(got, q, s, owner, pos, unit=unit_of(kernel), slopes=slopes, q_rotated=True)
+
+
+@pytest.mark.parametrize("kernel", SPREAD)
+@pytest.mark.parametrize("size", [1e18, 1.0, 1e-18])
+@pytest.mark.parametrize("quiet", [0.0, 2.0 ** -100])
+def test_pages_of_zeros_beside_others(kernel, size, quiet):
+    """Blocks of zeros have the smallest scale that an append writes, pages never written one of 0: their keys keep
+    their weights, and the others their values, wherever in the sequence they are."""
+    lens = [700, 640]
+    for places in (lambda col: col == 0, lambda col: col < 9, lambda col: col % 3 == 1, lambda col: col > 5):
+        s = Setup(lens, seed=75, page_len=64, code="e4m3")
+        first, owner, pos = placed(kernel, lens)
+        v = s.cache.v.view(torch.uint8)
+        for b in (0, 1):
+            spread(s, lambda col: quiet * 448 if places(col) else size, b)
+            for col, page in enumerate(s.table[b]):
+                if places(col) and page >= 0:
+                    v[page] = 0
+        q = s.queries(first[-1])
+        got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first)
+        close(got, q, s, owner, pos, unit=unit_of(kernel))
