@@ -16,9 +16,9 @@
 // takes 96 registers of a lane.
 //
 // Precision.  Q, divided by a power of two that brings the row's largest below 1,
-// and the weights, 2^(z - m) times their page's V scale over a running power of two,
-// round to FP16 (2^-11 of a term: three bits more than the BF16 that Q came as and
-// the output becomes); codes are exact, sums and scores FP32.
+// and the weights, 2^(z + log2(V scale) - m), round to FP16 (2^-11 of a term: three
+// bits more than the BF16 that Q came as and the output becomes; 2^-31 of the row's
+// largest weight times scale for each key); codes are exact, sums and scores FP32.
 //
 // Bound by the consumers' instructions: of a tile's 3600 cycles in a warp the products
 // with K take 1280, those with V 1250, the softmax 1080, with the tensor pipe about a
@@ -53,10 +53,9 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 2 * kWarps;
 constexpr int kRowF = kHeadDim + 4;    // padded row
 constexpr int kUnitRows = kTokens * kGroup;
-// Weights are 2^(z - m) with z up to 8 above the reference m, times a page's V scale
-// over a power of two (below 4): up to 2^15 with this lift, and FP16's 2^-24 is 2^-29
-// of a weight at the reference.
-constexpr float kHeadroom = 8.f, kLift = 32.f;
+// Weights are lifted by 2^7 and may pass the reference by 2^8: up to 2^15, and FP16's
+// 2^-24 is 2^-31 of a weight at the reference.
+constexpr float kHeadroom = 8.f, kLift = 7.f;
 
 struct alignas(16) Slot {  // one unit's queries (two slots)
     uint4 q[kPairsQ][4][32];       // the lanes' operands: column 2 head + query % 2, 8 of the lane's 32 dims
@@ -70,7 +69,8 @@ struct alignas(16) Slot {  // one unit's queries (two slots)
 struct alignas(16) Shared {
     uint64_t full[kStages], empty[kStages], qfull[2], qempty[2], rfull, rempty;
     Slot slot[2];
-    float4 scales[kStages];  // K of the tile's two pages, V of them
+    float4 scales[kStages];  // K of the tile's two pages (NaN where V's is no number), log2 of V's
+    float4 v_inv[kStages];   // V's, as VScale has them; 0 where V is zeros, else 1
     struct {  // what the consumer warps make of two queries of a piece
         float acc[kWarps][2 * kGroup][kRowF];
         float m[kWarps][2 * kGroup], l[kWarps][2 * kGroup];
@@ -100,19 +100,18 @@ __device__ __forceinline__ void take_registers() {
 }
 
 // Running state of a consumer warp for the current unit.  Lane (g, t) = (lane / 4,
-// lane % 4): head t's reference and sum (over this lane's keys only) for each query,
+// lane % 4): head t's reference and sum (over this lane's keys only, times kWeightUnit) for each query,
 // and O for head t, dims 16 g + 2 i (o[][i][0] the pair's first query, [1] its second)
 // and + 1 ([2], [3]).
 struct State {
     float o[kPairsQ][8][4];
     float m[kPairsQ][2], l[kPairsQ][2];
-    float vref, vinv;  // a power of two no page's V scale so far reaches twice, and kLift over it
 };
 
 // Tiles of a unit with kN pairs of queries.
 template <int kCode, bool kCap, bool kBias, int kN>
-__device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float4& sc, const Slot& slot,
-                                             float cap2, int key0, int page_shift, int lane) {
+__device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float4& sc, const float4& vi,
+                                             const Slot& slot, float cap2, int key0, int page_shift, int lane) {
     const int g = lane >> 2, t = lane & 3;
     // Step i (16 keys) lies in page i >> sh of the tile.
     const int sh = min(page_shift, kTileShift) - 4;
@@ -155,30 +154,23 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
         }
     }
     const bool edge = key0 < slot.lo_most || key0 + kTile > slot.hi_least;  // of the whole warp
-    // Where a query does not see a key, in one branch of the whole warp.
-    auto blank = [&](float x) {
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int lo = slot.lo[2 * n + e] - key0 - g, hi = slot.hi[2 * n + e] - key0 - g;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        if (16 * i + 8 * u < lo || 16 * i + 8 * u >= hi) z[n][i][2 * u + e] = x;
-            }
-    };
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
         const float2 factor = *reinterpret_cast<const float2*>(&slot.factor[n][2 * t]);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const float f = i >> sh ? sc.y : sc.x, f0 = f * factor.x, f1 = f * factor.y;
+            const float lv = kCap ? 0.f : i >> sh ? sc.w : sc.z;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[n][i][e] *= e & 1 ? f1 : f0;
+            for (int e = 0; e < 4; ++e) z[n][i][e] = fmaf(z[n][i][e], e & 1 ? f1 : f0, lv);
         }
-        if constexpr (kCap) cap_scores(reinterpret_cast<float(&)[4 * kSteps]>(z[n]), cap2);
+        if constexpr (kCap) {
+            cap_scores(reinterpret_cast<float(&)[4 * kSteps]>(z[n]), cap2);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[n][i][e] += i >> sh ? sc.w : sc.z;
+        }
         if constexpr (kBias) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
@@ -189,31 +181,30 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                                       z[n][i][e]);
         }
     }
-    if (edge) blank(-INFINITY);
+    if (edge) {  // where a query does not see a key, in one branch of the whole warp
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int lo = slot.lo[2 * n + e] - key0 - g, hi = slot.hi[2 * n + e] - key0 - g;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (16 * i + 8 * u < lo || 16 * i + 8 * u >= hi) z[n][i][2 * u + e] = -INFINITY;
+            }
+    }
     float mx[kN][2];  // of this lane's keys
     bool above = false;
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            mx[n][e] = fmaxf(fmaxf(z[n][0][e], z[n][0][2 + e]), fmaxf(z[n][1][e], z[n][1][2 + e]));
+            mx[n][e] = fmaxf(fmaxf(z[n][0][e], z[n][0][2 + e]), fmaxf(z[n][1][e], z[n][1][2 + e])) - kLift;
             above |= mx[n][e] > st.m[n][e] + kHeadroom;
         }
-    // V scales: where a page's passes the running power of two, that grows.
-    float vmax = 0.f;
-    if (fabsf(sc.z) <= 3.402823466e38f) vmax = fabsf(sc.z);
-    if (fabsf(sc.w) <= 3.402823466e38f) vmax = fmaxf(vmax, fabsf(sc.w));
-    const bool louder = vmax >= 2.f * st.vref && vmax > 0.f;
     // The references move only when a score passes one by kHeadroom.
-    if (__any_sync(0xffffffffu, above) || louder) {
-        float vscale = 1.f;
-        if (louder) {
-            // The power of two below it, within the range where both vinv and its inverse are normal numbers.
-            const float ref = __int_as_float(min(253, max(13, __float_as_int(vmax) >> 23)) << 23);
-            vscale = st.vref / ref;
-            st.vref = ref;
-            st.vinv = kLift / ref;
-        }
+    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
             float f[2];
@@ -222,10 +213,9 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                 float m_new = fmaxf(st.m[n][e], mx[n][e]);
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
-                const float alpha = fast_exp2(st.m[n][e] - (m_new == -INFINITY ? 0.f : m_new));
+                f[e] = fast_exp2(st.m[n][e] - (m_new == -INFINITY ? 0.f : m_new));
                 st.m[n][e] = m_new;
-                st.l[n][e] *= alpha;
-                f[e] = alpha * vscale;
+                st.l[n][e] *= f[e];
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -238,16 +228,15 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
         const float m0 = st.m[n][0] == -INFINITY ? 0.f : st.m[n][0], m1 = st.m[n][1] == -INFINITY ? 0.f : st.m[n][1];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const float r = (i >> sh ? sc.w : sc.z) * st.vinv;
+            const float inv = i >> sh ? vi.y : vi.x, some = i >> sh ? vi.w : vi.z;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float y = fast_exp2(z[n][i][e] - (e & 1 ? m1 : m0));
-                st.l[n][e & 1] += y;
-                z[n][i][e] = y * r;
+                st.l[n][e & 1] = fmaf(y, inv, st.l[n][e & 1]);
+                z[n][i][e] = y * some;
             }
         }
     }
-    if (edge) blank(0.f);  // not NaN, whatever the page's scale
     uint32_t w[kN][kSteps][2];
 #pragma unroll
     for (int n = 0; n < kN; ++n)
@@ -345,21 +334,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                     st.l[q][e] = 0.f;
                 }
             }
-            st.vref = 0.f;
-            st.vinv = 0.f;
             // This warp's tiles: every kWarps-th of the CTA's.
             for (; mine < tiles; mine += kWarps) {
                 if (ok) ok = mbar_wait(&s.full[stg], phase);
                 const uint8_t* stage = ring + stg * kStageBytes;
                 const int key0 = (tile0 + mine) * kTile;
                 const float cap2 = p.cap * 1.4426950408889634f;
-                const float4 sc = s.scales[stg];
+                const float4 sc = s.scales[stg], vi = s.v_inv[stg];
                 if (pairs == 1)
-                    consume_tile<kCode, kCap, kBias, 1>(st, stage, sc, slot, cap2, key0, p.c.page_shift, lane);
+                    consume_tile<kCode, kCap, kBias, 1>(st, stage, sc, vi, slot, cap2, key0, p.c.page_shift, lane);
                 else if (pairs == 2)
-                    consume_tile<kCode, kCap, kBias, 2>(st, stage, sc, slot, cap2, key0, p.c.page_shift, lane);
+                    consume_tile<kCode, kCap, kBias, 2>(st, stage, sc, vi, slot, cap2, key0, p.c.page_shift, lane);
                 else
-                    consume_tile<kCode, kCap, kBias, 3>(st, stage, sc, slot, cap2, key0, p.c.page_shift, lane);
+                    consume_tile<kCode, kCap, kBias, 3>(st, stage, sc, vi, slot, cap2, key0, p.c.page_shift, lane);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.empty[stg]);
                 stg += kWarps;
@@ -373,7 +360,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             if (lane == 0) mbar_arrive(&s.qempty[sl]);
 
             // This warp's part of the piece, for the finishers, two queries at a time.
-            const float back = st.vref * (1.f / kLift);
             auto& r = s.result;
 #pragma unroll
             for (int q = 0; q < kPairsQ; ++q) {
@@ -390,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         *reinterpret_cast<float4*>(&r.acc[warp][2 * t + e][16 * g + 4 * i]) =
-                            make_float4(st.o[q][2 * i][e] * back, st.o[q][2 * i][2 + e] * back,
-                                        st.o[q][2 * i + 1][e] * back, st.o[q][2 * i + 1][2 + e] * back);
+                            make_float4(st.o[q][2 * i][e], st.o[q][2 * i][2 + e], st.o[q][2 * i + 1][e],
+                                        st.o[q][2 * i + 1][2 + e]);
                 if (g == 0) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -441,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             auto write = [&](int q, int e, float4 x, float l) {
                 const int token = 2 * q + e;
                 if (token >= un.n) return;
-                const float inv = l == 0.f ? 0.f : 1.f / l;  // 0 for a row that sees nothing
+                const float inv = l == 0.f ? 0.f : kWeightUnit / l;  // 0 for a row that sees nothing
                 const __nv_bfloat162 u = __floats2bfloat162_rn(x.x * inv, x.y * inv), v = __floats2bfloat162_rn(x.z * inv, x.w * inv);
                 *reinterpret_cast<uint2*>(p.out + (int64_t)(un.row0 + token) * p.out_row_stride +
                                           (walk.h * kGroup + hq) * p.out_head_stride + 4 * lane) =
@@ -592,7 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                                 tma_load_page(dst + box_bytes, &a.kmap, 0, walk.h, now.b, &s.full[to], policy);
                                 tma_load_page(dst + kHalfBytes + box_bytes, &a.vmap, 0, walk.h, now.b, &s.full[to], policy);
                             }
-                            s.scales[to] = f_now;
+                            const VScale va = v_scale_of(f_now.z), vb = v_scale_of(f_now.w);
+                            const float nan = __int_as_float(0x7fffffff);
+                            s.scales[to] = make_float4(fabsf(f_now.z) <= 3.402823466e38f ? f_now.x : nan,
+                                                       fabsf(f_now.w) <= 3.402823466e38f ? f_now.y : nan, va.log2, vb.log2);
+                            s.v_inv[to] = make_float4(va.inv, vb.inv, va.some ? 1.f : 0.f, vb.some ? 1.f : 0.f);
                             mbar_arrive_expect_tx(&s.full[to], 2 * ((now.a >= 0) + (now.b >= 0)) * box_bytes);
                         }
                         stg += n;

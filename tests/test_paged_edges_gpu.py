@@ -222,7 +222,7 @@ def spread(s, scales, owner=0):
         s.cache.v_scale[s.table[owner][col]] = scales(col) / (127 if s.code == "int8" else 448)
 
 
-SPREAD = ["chunk"]  # whose V scales may lie far apart
+SPREAD = ["few", "chunk"]  # whose V scales may lie far apart
 RATIOS = [2.0 ** -10, 2.0 ** -20, 2.0 ** -24, 2.0 ** -30, 2.0 ** -60]
 
 
