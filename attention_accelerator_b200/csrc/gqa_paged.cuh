@@ -154,16 +154,26 @@ __device__ __forceinline__ void to_half4(uint32_t w, uint32_t& lo, uint32_t& hi)
 // weights stay in the sum beside pages of 2^-80 to 2^60.
 constexpr float kWeightUnit = 0x1p-12f, kNoVScale = 0x1p-100f;
 struct VScale {
-    float log2, inv;  // of a page's V scale; inv times kWeightUnit
-    bool some;        // not zeros
+    float exponent, fraction;  // of a page's V scale; the fraction in [1, 2), 0 where V is zeros
+    float inv;                 // kWeightUnit / 2^exponent
 };
 __device__ __forceinline__ VScale v_scale_of(float s) {
     const bool some = s > kNoVScale;
-    // Exponent and fraction apart: the fraction's logarithm is good to 2^-22 of 1.
     const uint32_t bits = __float_as_uint(some ? fminf(s, 0x1.fffffep121f) : 0x1p-60f);
     const int e = (int)(bits >> 23) - 127;
-    const float f = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
-    return VScale{(float)e + __log2f(f), __fdividef(kWeightUnit, f) * __uint_as_float((uint32_t)(127 - e) << 23), some};
+    return VScale{(float)e, some ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : 0.f,
+                  kWeightUnit * __uint_as_float((uint32_t)(127 - e) << 23)};
+}
+// The fraction joined to the exponent (its logarithm is good to 2^-22 of 1).
+struct VLog2 {
+    float log2, inv;  // inv: kWeightUnit / scale
+    bool some;        // V is not zeros
+};
+__device__ __forceinline__ VLog2 v_log2_of(float s) {
+    const VScale v = v_scale_of(s);
+    const bool some = v.fraction > 0.f;
+    const float f = some ? v.fraction : 1.f;
+    return VLog2{v.exponent + __log2f(f), __fdividef(v.inv, f), some};
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {

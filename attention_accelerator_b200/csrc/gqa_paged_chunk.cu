@@ -83,7 +83,7 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);  // B (V) MN-major
 
 struct TileScales {
     float k[8];                 // of each 16 keys: K's scale (NaN where V's is no number)
-    float v_log2[8], v_inv[8];  // and V's, as VScale has it
+    float v_log2[8], v_inv[8];  // and V's, as VLog2 has it
     uint32_t v_some;            // bits: V is not zeros
     uint32_t pad[7];
 };
@@ -915,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         const int from = (lane & 7) >> (shift - 4);
                         const float kg = __shfl_sync(0xffffffffu, ks, from), vg = __shfl_sync(0xffffffffu, vs, from);
                         const bool fine = fabsf(vg) <= 3.402823466e38f;
-                        const VScale v = v_scale_of(vg);
+                        const VLog2 v = v_log2_of(vg);
                         const uint32_t some = __ballot_sync(0xffffffffu, lane < 8 && v.some);
                         TileScales& sc = s.scales[tile_count & (kScaleSlots - 1)];
                         if (lane == 0) sc.v_some = some;

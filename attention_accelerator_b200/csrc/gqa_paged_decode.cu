@@ -29,8 +29,8 @@
 //            deep; codes become FP16 exactly, so a score carries FP32's error
 //            only.  Softmax runs in the result's layout (lane: 2 keys of one
 //            head) without a shuffle but for the maximum.  The weights, times
-//            their page's V scale over a running power of two, split into two
-//            FP16 parts again, and movmatrix turns them into the other product's
+//            their page's V scale (its power of two joins the score, against the
+//            row's largest such sum), split into two FP16 parts again, and movmatrix turns them into the other product's
 //            operand: O^T = V^T P^T, M 16 dims, whose operand lanes build from
 //            the 16-byte pieces of 4 keys by byte permutes.
 //   finisher one a Q head: joins the consumers' rows of a unit and writes it, or
@@ -72,7 +72,7 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kMaxStages = 3 * kWarps;
 constexpr int kPagesPerTile = kTile / kPagedMinPage;
 static_assert(kSteps == 2 && kPagesPerTile == 2, "scales of two pages a tile");
-constexpr float kWeightScale = 4096.f;         // keeps FP16's subnormal step, 2^-24, 2^-36 of a weight of 1
+constexpr float kLift = 12.f;                  // weights up to 2^13: FP16's subnormal step, 2^-24, is 2^-36 of the largest
 
 // Shared memory behind the ring (bytes).
 constexpr int kRowF = kHeadDim + 4;  // padded partial row
@@ -85,7 +85,8 @@ struct alignas(16) Slot {            // one unit's queries (two slots)
 struct alignas(16) Shared {
     uint64_t full[kMaxStages], empty[kMaxStages], qfull[2], qempty[2], rfull, rempty;
     Slot slot[2];
-    float4 scales[kMaxStages];  // K of the tile's two pages, V of them
+    float4 scales[kMaxStages];  // K of the tile's two pages (NaN where V's is no number), V's exponents
+    float4 v_rest[kMaxStages];  // V's fractions and inverses, as VScale has them
     struct {  // what the consumer warps make of a piece
         float acc[kWarps][kGroup][kRowF];
         float m[kWarps][kGroup], l[kWarps][kGroup];
@@ -155,17 +156,17 @@ struct Walk {
 };
 
 // Running state of a consumer warp for the current unit.  Lane (g, t) = (lane / 4,
-// lane % 4): head t's maximum and sum (the sum over this lane's keys only), and
-// O for head t, dims 16 g + 2 i (o[i][0] high parts, [1] low) and + 1 ([2], [3]).
+// lane % 4): head t's maximum of z + V's exponent, the sum of weights (over this
+// lane's keys only, without V's scale, times kWeightUnit), and O for head t, dims 16 g
+// + 2 i (o[i][0] high parts, [1] low) and + 1 ([2], [3]).
 struct State {
     float o[8][4];
     float m, l;
-    float vref, vinv;  // a power of two no page's V scale so far exceeds twice, and kWeightScale over it
 };
 
 template <int kCode, bool kCap, bool kBias>
 __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float4& scales,
-                                             const uint32_t (&qf)[16], float factor, float slope, float cap2,
+                                             const float4& v_rest, const uint32_t (&qf)[16], float factor, float slope, float cap2,
                                              int key0, int lo, int hi, int m_pos, int page_shift, int lane) {
     const int g = lane >> 2, t = lane & 3;
     // Step i (16 keys) lies in page i >> sh of the tile.
@@ -190,11 +191,18 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                 mma_16x8x16(s, a0, a1, a2, a3, qf[2 * e], qf[2 * e + 1]);
             }
             const float f = factor * (i >> sh ? sc.y : sc.x);
-            z[i][0] = (s[0] + s[1]) * f;
-            z[i][1] = (s[2] + s[3]) * f;
+            const float ve = kCap ? 0.f : i >> sh ? sc.w : sc.z;
+            z[i][0] = fmaf(s[0] + s[1], f, ve);
+            z[i][1] = fmaf(s[2] + s[3], f, ve);
         }
     }
-    if constexpr (kCap) cap_scores(reinterpret_cast<float(&)[2 * kSteps]>(z), cap2);
+    if constexpr (kCap) {
+        cap_scores(reinterpret_cast<float(&)[2 * kSteps]>(z), cap2);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) z[i][e] += i >> sh ? sc.w : sc.z;
+    }
     if constexpr (kBias) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
@@ -219,40 +227,27 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     const float m_new = fmaxf(st.m, mx);
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    // V scales: where a page's passes the running power of two, that grows.
-    float vmax = 0.f;
-    if (fabsf(sc.z) <= 3.402823466e38f) vmax = fabsf(sc.z);
-    if (fabsf(sc.w) <= 3.402823466e38f) vmax = fmaxf(vmax, fabsf(sc.w));
-    float vscale = 1.f;
-    if (vmax > 2.f * st.vref) {
-        // The power of two below it, within the range where both vinv and its inverse are normal numbers.
-        const float ref = __int_as_float(min(253, max(13, __float_as_int(vmax) >> 23)) << 23);
-        vscale = st.vref / ref;
-        st.vref = ref;
-        st.vinv = kWeightScale / ref;
-    }
-    if (__any_sync(0xffffffffu, m_new != st.m) || vscale != 1.f) {
+    if (__any_sync(0xffffffffu, m_new != st.m)) {
         const float alpha = fast_exp2(st.m - m_use);
-        const float f = alpha * vscale;
         st.l *= alpha;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[i][e] *= f;
+            for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
         st.m = m_new;
     }
+    const float m_low = m_use - kLift;
     const uint8_t* v = stage + kHalfBytes;
     const int r0 = 2 * t * kHeadDim + ((g ^ (2 * t)) << 4), r1 = (2 * t + 1) * kHeadDim + ((g ^ (2 * t + 1)) << 4);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-        const float r = (i >> sh ? sc.w : sc.z) * st.vinv;
+        const float r = i >> sh ? v_rest.y : v_rest.x, inv = i >> sh ? v_rest.w : v_rest.z;
         float w[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float p = fast_exp2(z[i][e] - m_use);
-            st.l += p;
+            const float p = fast_exp2(z[i][e] - m_low);
+            st.l = fmaf(p, inv, st.l);
             w[e] = p * r;
-            if (edge && z[i][e] == -INFINITY) w[e] = 0.f;  // not NaN, whatever the page's scale
         }
         const float h0 = __half2float(__float2half_rn(w[0])), h1 = __half2float(__float2half_rn(w[1]));
         const uint32_t b0 = transpose_8x8(pack_half2(h0, w[0] - h0));
@@ -425,7 +420,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                             tma_load_page(dst + box_bytes, &a.kmap, 0, walk.h, now.b, &s.full[to], policy);
                             tma_load_page(dst + kHalfBytes + box_bytes, &a.vmap, 0, walk.h, now.b, &s.full[to], policy);
                         }
-                        s.scales[to] = f_now;
+                        const VScale va = v_scale_of(f_now.z), vb = v_scale_of(f_now.w);
+                        const float nan = __int_as_float(0x7fffffff);
+                        s.scales[to] = make_float4(fabsf(f_now.z) <= 3.402823466e38f ? f_now.x : nan,
+                                                   fabsf(f_now.w) <= 3.402823466e38f ? f_now.y : nan, va.exponent,
+                                                   vb.exponent);
+                        s.v_rest[to] = make_float4(va.fraction, vb.fraction, va.inv, vb.inv);
                         mbar_arrive_expect_tx(&s.full[to], 2 * ((now.a >= 0) + (now.b >= 0)) * box_bytes);
                     }
                     stg += n;
@@ -658,13 +658,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
             for (int e = 0; e < 4; ++e) st.o[i][e] = 0.f;
         st.m = -INFINITY;
         st.l = 0.f;
-        st.vref = 0.f;
-        st.vinv = 0.f;
         // This warp's tiles: every kWarps-th of the CTA's.
         for (; mine < walk.n; mine += kWarps) {
             const int j = mine;
             if (ok) ok = mbar_wait(&s.full[stg], phase);
-            consume_tile<kCode, kCap, kBias>(st, ring + stg * kStageBytes, s.scales[stg], qf, factor, slope,
+            consume_tile<kCode, kCap, kBias>(st, ring + stg * kStageBytes, s.scales[stg], s.v_rest[stg], qf, factor, slope,
                                              p.cap * 1.4426950408889634f, (walk.tile + j) * kTile, lo, hi, m_pos,
                                              p.c.page_shift, lane);
             __syncwarp();
@@ -681,15 +679,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         float l = st.l;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-        const float back = st.vref * (1.f / kWeightScale);
         if (ok && n >= 1) ok = mbar_wait(&s.rempty, (n - 1) & 1);
         auto& r = s.result;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             *reinterpret_cast<float4*>(&r.acc[warp][t][16 * g + 4 * i]) =
-                make_float4((st.o[2 * i][0] + st.o[2 * i][1]) * back, (st.o[2 * i][2] + st.o[2 * i][3]) * back,
-                            (st.o[2 * i + 1][0] + st.o[2 * i + 1][1]) * back,
-                            (st.o[2 * i + 1][2] + st.o[2 * i + 1][3]) * back);
+                make_float4((st.o[2 * i][0] + st.o[2 * i][1]) * kWeightUnit, (st.o[2 * i][2] + st.o[2 * i][3]) * kWeightUnit,
+                            (st.o[2 * i + 1][0] + st.o[2 * i + 1][1]) * kWeightUnit,
+                            (st.o[2 * i + 1][2] + st.o[2 * i + 1][3]) * kWeightUnit);
         if (g == 0) {
             r.m[warp][t] = st.m;
             r.l[warp][t] = l;

@@ -70,7 +70,7 @@ struct alignas(16) Shared {
     uint64_t full[kStages], empty[kStages], qfull[2], qempty[2], rfull, rempty;
     Slot slot[2];
     float4 scales[kStages];  // K of the tile's two pages (NaN where V's is no number), log2 of V's
-    float4 v_inv[kStages];   // V's, as VScale has them; 0 where V is zeros, else 1
+    float4 v_inv[kStages];   // V's, as VLog2 has them; 0 where V is zeros, else 1
     struct {  // what the consumer warps make of two queries of a piece
         float acc[kWarps][2 * kGroup][kRowF];
         float m[kWarps][2 * kGroup], l[kWarps][2 * kGroup];
@@ -100,9 +100,9 @@ __device__ __forceinline__ void take_registers() {
 }
 
 // Running state of a consumer warp for the current unit.  Lane (g, t) = (lane / 4,
-// lane % 4): head t's reference and sum (over this lane's keys only, times kWeightUnit) for each query,
-// and O for head t, dims 16 g + 2 i (o[][i][0] the pair's first query, [1] its second)
-// and + 1 ([2], [3]).
+// lane % 4): head t's reference and sum (over this lane's keys only, times
+// kWeightUnit) for each query, and O for head t, dims 16 g + 2 i (o[][i][0] the
+// pair's first query, [1] its second) and + 1 ([2], [3]).
 struct State {
     float o[kPairsQ][8][4];
     float m[kPairsQ][2], l[kPairsQ][2];
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                                 tma_load_page(dst + box_bytes, &a.kmap, 0, walk.h, now.b, &s.full[to], policy);
                                 tma_load_page(dst + kHalfBytes + box_bytes, &a.vmap, 0, walk.h, now.b, &s.full[to], policy);
                             }
-                            const VScale va = v_scale_of(f_now.z), vb = v_scale_of(f_now.w);
+                            const VLog2 va = v_log2_of(f_now.z), vb = v_log2_of(f_now.w);
                             const float nan = __int_as_float(0x7fffffff);
                             s.scales[to] = make_float4(fabsf(f_now.z) <= 3.402823466e38f ? f_now.x : nan,
                                                        fabsf(f_now.w) <= 3.402823466e38f ? f_now.y : nan, va.log2, vb.log2);

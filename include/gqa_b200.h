@@ -574,7 +574,10 @@ int gqa_read_paged(const gqa_paged_cache *cache, const int64_t *slots, int n, vo
  * and prefix_ends (prefix mask: keys below it are visible whatever the query's
  * position; default 0) are per query row, NULL for none.  Keys outside the
  * visible range never influence a result, whatever their codes; a block's NaN
- * scale reaches a row only through a visible key.  Scales are not negative, and
+ * scale reaches a row only through a visible key.  V's scales may lie far apart:
+ * pages that a row does not see, or gives no weight, do not reach its others'
+ * precision.  A V scale of 2^-100 (what an append of zeros writes) or less says
+ * that the block is zeros.  Scales are not negative, and
  * visible codes are numbers (gqa_append_paged writes no e4m3 NaN; the value read
  * for one is unspecified).  Page numbers outside
  * [0, pages) read as zeros, and no key at or past table_width * page_len (2^30 at

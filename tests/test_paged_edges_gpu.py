@@ -222,11 +222,10 @@ def spread(s, scales, owner=0):
         s.cache.v_scale[s.table[owner][col]] = scales(col) / (127 if s.code == "int8" else 448)
 
 
-SPREAD = ["few", "chunk"]  # whose V scales may lie far apart
 RATIOS = [2.0 ** -10, 2.0 ** -20, 2.0 ** -24, 2.0 ** -30, 2.0 ** -60]
 
 
-@pytest.mark.parametrize("kernel", SPREAD)
+@pytest.mark.parametrize("kernel", ["few", "chunk"])
 @pytest.mark.parametrize("ratio", RATIOS)
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("loud_first", [True, False])
@@ -244,7 +243,7 @@ def test_quiet_pages_beside_loud_ones_that_a_row_does_not_see(kernel, ratio, cod
     close(got, q, s, owner, pos, unit=unit_of(kernel), starts=starts)
 
 
-@pytest.mark.parametrize("kernel", SPREAD)
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("ratio", RATIOS)
 def test_quiet_pages_beside_loud_ones_of_no_weight(kernel, ratio):
     """The bias takes the weight of the loud pages, 400 keys away, below 2^-144: what is left is the quiet pages'."""
@@ -260,7 +259,7 @@ def test_quiet_pages_beside_loud_ones_of_no_weight(kernel, ratio):
     close(got, q, s, owner, pos, unit=unit_of(kernel), slopes=slopes, q_rotated=True)
 
 
-@pytest.mark.parametrize("kernel", SPREAD)
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("size", [1e18, 1.0, 1e-18])
 @pytest.mark.parametrize("quiet", [0.0, 2.0 ** -100])
 def test_pages_of_zeros_beside_others(kernel, size, quiet):
