@@ -349,11 +349,9 @@ Plan make_plan(const gqa::SeqDesc* d, int batch, int sms, bool allow_cluster = f
 }
 
 void rope_steps(double theta, uint64_t* step, float2* rot_step, float2* rot_tile, int tile_keys) {
-    const double two_pi = 2.0 * M_PI;
     for (int i = 0; i < gqa::kPairs; ++i) {
         const double inv = std::pow(theta, -2.0 * i / (double)gqa::kHeadDim);
-        const double turns_q64 = inv / two_pi * 18446744073709551616.0;  // < 2^62
-        step[i] = (uint64_t)std::llround(turns_q64);
+        step[i] = gqa::rope_step(theta, i, gqa::kHeadDim);
         if (rot_step) rot_step[i] = make_float2((float)std::cos(4.0 * inv), (float)std::sin(4.0 * inv));
         if (rot_tile)
             rot_tile[i] = make_float2((float)std::cos(tile_keys * inv), (float)std::sin(tile_keys * inv));

@@ -6,6 +6,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <cmath>
 #include <initializer_list>
 
 namespace gqa {
@@ -24,6 +25,14 @@ int device_sms(int* sms);
 cudaError_t paged_decode_prepare();
 cudaError_t paged_chunk_prepare();
 cudaError_t paged_few_prepare();
+
+// Turns per position of rotate_half pair i, theta^(-2i/128) / 2 pi, as a Q0.64
+// fraction.  A base below 1 turns a pair by more than a turn: whole ones fall away.
+inline uint64_t rope_step(double theta, int pair, int head_dim) {
+    const double turns = std::pow(theta, -2.0 * pair / (double)head_dim) / (2.0 * M_PI);
+    const double q64 = (turns - std::floor(turns)) * 18446744073709551616.0;
+    return q64 < 9223372036854775808.0 ? (uint64_t)std::llround(q64) : (uint64_t)q64;  // (an integer from 2^53 on)
+}
 
 struct DecodeArgs;
 struct RopeTable;

@@ -542,10 +542,7 @@ const RopeSteps& rope_steps_of(float theta) {
     static thread_local float last = 0.f;
     static thread_local RopeSteps steps;
     if (last != theta) {
-        for (int i = 0; i < kPairs; ++i) {
-            const double inv = std::pow((double)theta, -2.0 * i / (double)kHeadDim);
-            steps.step[i] = (uint64_t)std::llround(inv / (2.0 * M_PI) * 18446744073709551616.0);
-        }
+        for (int i = 0; i < kPairs; ++i) steps.step[i] = rope_step(theta, i, kHeadDim);
         last = theta;
     }
     return steps;

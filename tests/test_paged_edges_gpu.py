@@ -12,7 +12,7 @@ import torch
 import attention_accelerator_b200 as gqa
 from attention_accelerator_b200 import api
 from oracle import paged as ref
-from test_paged_gpu import CHUNK_UNIT, DECODE_UNIT, THETA, Setup, ints
+from test_paged_gpu import CHUNK_UNIT, DECODE_UNIT, THETA, Setup, ints, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -278,3 +278,26 @@ def test_pages_of_zeros_beside_others(kernel, size, quiet):
         q = s.queries(first[-1])
         got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first)
         close(got, q, s, owner, pos, unit=unit_of(kernel))
+
+
+@pytest.mark.parametrize("theta", [0.05, 0.3, 1.0, 10.0])
+def test_small_rope_bases(theta):
+    """Bases below 1 turn a pair by more than a radian a position, up to several turns: only their fraction counts."""
+    lens = [300, 200]
+    s = Setup(lens, seed=76, page_len=32, code="int8")
+    for kernel in KERNELS:
+        first, owner, pos = placed(kernel, lens)
+        q = s.queries(first[-1])
+        got = attend(kernel, q, s.cache, ints(s.table), ints(lens), first, rope_theta=theta)
+        close(got, q, s, owner, pos, unit=unit_of(kernel), theta=float(np.float32(theta)))
+    cache = gqa.paged_cache(2, 64, dtype=torch.int8)
+    k = torch.randn(70, 8, 128, generator=s.gen, device="cuda").to(torch.bfloat16)
+    at = torch.arange(70, device="cuda")
+    gqa.append_paged(cache, k, k, at, positions=at.int() * 3, rope_theta=theta)
+    want = ref.rope(k.float().cpu().numpy(), np.arange(70) * 3, float(np.float32(theta)))
+    scale = cache.k_scale.cpu().numpy().astype(np.float64)[np.arange(70) // 64][..., None]
+    got = ref.code_values(rows_of(cache, cache.k).reshape(128, 8, 128)[:70], "int8") * scale
+    assert (np.abs(got - want) <= scale * (0.5 + 2.0 ** -6)).all()
+    # The BF16 cache's rotation, by the same table: one BF16 rounding, and FP32's.
+    got = gqa.rope_k_cache(k, at.int() * 3, rope_theta=theta).float().cpu().numpy()
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -18).all()
