@@ -61,6 +61,8 @@ struct DeviceInfo {
     int sms = 0;
     int cluster_cap[17] = {};  // decode clusters of n CTAs the device holds at once
     bool cluster_asked[17] = {};  // cluster_cap[n] is known
+    bool paged_init = false;
+    int paged_status = GQA_OK;
 };
 
 std::mutex g_mu;
@@ -81,9 +83,7 @@ int current_device(int* sms) {
         }
         if (major != 10 || minor != 0) {
             di.status = GQA_ERR_UNSUPPORTED_DEVICE;
-        } else if (gqa::decode_prepare(dev) != cudaSuccess || gqa::chunked_prepare() != cudaSuccess ||
-                   gqa::paged_decode_prepare() != cudaSuccess || gqa::paged_chunk_prepare() != cudaSuccess ||
-                   gqa::paged_few_prepare() != cudaSuccess) {
+        } else if (gqa::decode_prepare(dev) != cudaSuccess || gqa::chunked_prepare() != cudaSuccess) {
             di.status = GQA_ERR_CUDA;
         }
         di.sms = n;
@@ -413,6 +413,24 @@ int fill_args(gqa::DecodeArgs& a, const void* q, const void* k, const void* v, v
 }  // namespace
 
 int gqa::device_sms(int* sms) { return current_device(sms); }
+
+// The paged attention's 24 kernels are loaded and prepared by its own first call, not by the BF16 calls'
+// (a first BF16 decode took 13 ms for it, 5 without), which go on should a paged kernel's register shares not fit what it was built with.
+int gqa::paged_attention_sms(int* sms) {
+    const int st = current_device(sms);
+    int dev = 0;
+    if (st != GQA_OK) return st;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return GQA_ERR_CUDA;
+    std::lock_guard<std::mutex> lock(g_mu);
+    DeviceInfo& di = g_dev[dev];
+    if (!di.paged_init) {
+        if (gqa::paged_decode_prepare() != cudaSuccess || gqa::paged_chunk_prepare() != cudaSuccess ||
+            gqa::paged_few_prepare() != cudaSuccess)
+            di.paged_status = GQA_ERR_CUDA;
+        di.paged_init = true;
+    }
+    return di.paged_status;
+}
 
 int gqa::paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c, int rows) {
     PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();

@@ -21,6 +21,8 @@ int check_device_memory(std::initializer_list<const void*> ptrs);
 // SM count of the current device; prepares the kernels on first use.  A status
 // (GQA_ERR_UNSUPPORTED_DEVICE where it is not an sm_100 GPU).
 int device_sms(int* sms);
+// The same for the paged attention calls, whose kernels it prepares.
+int paged_attention_sms(int* sms);
 
 cudaError_t paged_decode_prepare();
 cudaError_t paged_chunk_prepare();

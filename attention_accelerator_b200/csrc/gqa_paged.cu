@@ -651,7 +651,7 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     if (st != GQA_OK) return st;
     if (!workspace || !aligned16(workspace)) return GQA_ERR_WORKSPACE;
     int sms = 0;
-    st = device_sms(&sms);
+    st = paged_attention_sms(&sms);
     if (st != GQA_OK) return st;
     if (workspace_bytes < workspace_of(p->batch, p->rows, cache->kv_heads, chunked, sms)) return GQA_ERR_WORKSPACE;
     st = check_device_memory({workspace});

@@ -301,3 +301,38 @@ def test_small_rope_bases(theta):
     # The BF16 cache's rotation, by the same table: one BF16 rounding, and FP32's.
     got = gqa.rope_k_cache(k, at.int() * 3, rope_theta=theta).float().cpu().numpy()
     assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("order", ["paged first", "others first", "captured first"])
+def test_the_first_call_of_a_process(order):
+    """Kernels are prepared by the first call that needs them, whichever call of the library that is."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys, torch
+import attention_accelerator_b200 as gqa
+q = torch.randn(1, 32, 128, device="cuda").bfloat16()
+k = torch.randn(64, 8, 128, device="cuda").bfloat16()
+table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([64], dtype=torch.int32, device="cuda")
+cache = gqa.paged_cache(1, 64, dtype=torch.int8)
+gqa.append_paged(cache, k, k, torch.arange(64, device="cuda"), positions=torch.arange(64, device="cuda").int())
+def paged(): return gqa.decode_paged(q, cache, table, lens)
+def others(): return gqa.decode(q[0], k, k, seq_len=64, query_position=63, kv_block_len=16, layout="position_major")
+if sys.argv[1] == "captured first":
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        a = paged()
+    graph.replay()
+    torch.cuda.synchronize()
+    b = others()
+elif sys.argv[1] == "paged first":
+    a, b = paged(), others()
+else:
+    b, a = others(), paged()
+assert float((a[0].float() - b.float()).abs().max()) < 0.1, (a, b)
+"""
+    run = subprocess.run([sys.executable, "-c", code, order], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0, run.stderr[-2000:]
