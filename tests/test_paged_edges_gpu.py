@@ -40,7 +40,7 @@ def attend(kernel, q, cache, table, lens, first, **more):
 
 def close(got, q, setup, owner, positions, *, unit, theta=THETA, q_rotated=False, cap=0.0, slopes=None, starts=None,
           scale=1 / math.sqrt(128), floor=2.0 ** -22):
-    """Every output against 64 bits.  A score is off by 2 units of the sum of its terms' sizes (Q, and K's or the cap's
+    """Outputs (27 rows of a chunk, every row of less) against 64 bits.  A score is off by 2 units of the sum of its terms' sizes (Q, and K's or the cap's
     rounding), FP32's 2^-19 of that and 2^-22 of the bias -- nothing that grows with the cap alone; a weight by e to
     twice that, 3 units and 2^-20; the output by its BF16 rounding, and by ``floor`` of its row's largest sum of
     |weight * value|: weights below FP16's range (2^-31 of the largest weight times scale, a few hundred of them)."""
@@ -50,7 +50,9 @@ def close(got, q, setup, owner, positions, *, unit, theta=THETA, q_rotated=False
         x = ref.rope(x, np.array(positions), theta)
     slopes = slopes.cpu().numpy().astype(np.float64) if slopes is not None else None
     kv = {b: setup.values(b) for b in set(owner)}
-    for i, (b, m) in enumerate(zip(owner, positions)):
+    rows = len(owner)
+    for i in sorted(set(range(0, rows, max(1, rows // 27))) | {rows - 1}):
+        b, m = owner[i], positions[i]
         p = np.arange(setup.lens[b])
         seen = (p >= (starts[i] if starts is not None else 0)) & (p <= m)
         k, v = kv[b]
@@ -336,3 +338,112 @@ assert float((a[0].float() - b.float()).abs().max()) < 0.1, (a, b)
     run = subprocess.run([sys.executable, "-c", code, order], capture_output=True, text=True, timeout=300,
                          cwd=Path(__file__).resolve().parents[1])
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_chunks_of_pages_outside_the_cache():
+    """Table entries that name no page read as zeros, in a chunk as in the other calls."""
+    lens = [200, 640]
+    s = Setup(lens, seed=77, page_len=32, code="e4m3")
+    first, owner, pos = placed("chunk", lens)
+    q = s.queries(first[-1])
+    s.poison(lambda b, p: False)
+    v, k = s.cache.v.view(torch.uint8), s.cache.k.view(torch.uint8)
+    for page in (-5, s.cache.pages, 1 << 30, -(1 << 31)):
+        table = [list(row) for row in s.table]
+        table[0][2], table[1][0] = page, page
+        got = gqa.decode_paged_chunked(q, s.cache, ints(table), ints(lens), ints(first))
+        zero = Setup(lens, seed=77, page_len=32, code="e4m3")
+        for b, col in ((0, 2), (1, 0)):
+            zero.cache.k.view(torch.uint8)[zero.table[b][col]] = 0
+            zero.cache.v.view(torch.uint8)[zero.table[b][col]] = 0
+        close(got, q, zero, owner, pos, unit=CHUNK_UNIT)
+    table = [[-1 if c % 2 else 1 << 30 for c in range(len(row))] for row in s.table]
+    assert not gqa.decode_paged_chunked(q, s.cache, ints(table), ints(lens), ints(first)).any()
+    assert k.shape == v.shape and gqa.read_device_status() == 0
+
+
+def test_chunks_of_pages_past_32_bits():
+    pages = 36000
+    k, v = (torch.empty(pages, 8, 128, 128, dtype=torch.uint8, device="cuda").view(torch.int8) for _ in range(2))
+    ks, vs = (torch.empty(pages, 8, dtype=torch.float32, device="cuda") for _ in range(2))
+    cache = gqa.PagedCache(k, v, ks, vs)
+    lens = [300, 140]
+    s = Setup(lens, seed=78, page_len=128, spare=0)
+    table, far = [[-1] * 3 for _ in lens], [35999, 17, 35000, 34000, 33000]
+    for b, n in enumerate((3, 2)):
+        for col in range(n):
+            src, dst = s.table[b][col], far.pop()
+            k[dst], v[dst], ks[dst], vs[dst] = s.cache.k[src], s.cache.v[src], s.cache.k_scale[src], s.cache.v_scale[src]
+            table[b][col] = dst
+    first, owner, pos = placed("chunk", lens)
+    q = s.queries(first[-1])
+    close(gqa.decode_paged_chunked(q, cache, ints(table), ints(lens), ints(first)), q, s, owner, pos, unit=CHUNK_UNIT)
+
+
+def test_a_visible_nan_in_a_chunk_reaches_its_rows_only():
+    lens = [200, 300]
+    s = Setup(lens, seed=79, page_len=16, code="int8")
+    first, owner, pos = placed("chunk", lens)
+    q = s.queries(first[-1])
+    s.cache.v_scale[s.table[0][10], 2] = math.nan   # keys 160 to 175
+    s.cache.k_scale[s.table[1][16], 5] = math.nan   # keys 256 to 271
+    nan = torch.isnan(gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first))).any(-1)
+    want = torch.zeros_like(nan)
+    for i, (b, m) in enumerate(zip(owner, pos)):
+        if b == 0 and m >= 160:
+            want[i, 8:12] = True
+        if b == 1 and m >= 256:
+            want[i, 20:24] = True
+    assert torch.equal(nan, want)
+
+
+def test_first_query_of_a_chunk_is_kept_within_the_rows():
+    lens = [300, 300, 300]
+    s = Setup(lens, seed=80, page_len=32)
+    q = s.queries(100)
+    guard = torch.full((300, 32, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    for first in ([0, 70, 100, 1 << 30], [-7, 70, 90, 100], [0, 120, 90, 100], [90, 70, 0, 100], [-(1 << 31), 0, 99, 100]):
+        gqa.decode_paged_chunked(q, s.cache, ints(s.table), ints(lens), ints(first), out=guard[100:200])
+        assert bool((guard[:100] == 5.0).all()) and bool((guard[200:] == 5.0).all())
+    assert gqa.read_device_status() == 0
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_strided_rows_of_each_kernel(kernel):
+    lens = [90, 200]
+    s = Setup(lens, seed=83, page_len=16)
+    first, owner, pos = placed(kernel, lens)
+    n = first[-1]
+    wide = torch.zeros(n, 40, 256, dtype=torch.bfloat16, device="cuda")
+    q = wide[:, 3:35, 64:192]
+    q.copy_(s.queries(n))
+    out = torch.zeros(n, 34, 136, dtype=torch.bfloat16, device="cuda")
+    table = torch.full((2, 50), 9999, dtype=torch.int32, device="cuda")
+    table[:, :len(s.table[0])] = ints(s.table)
+    got = attend(kernel, q, s.cache, table[:, :len(s.table[0])], ints(lens), first, out=out[:, 1:33, :128], scale=0.3)
+    close(got, q, s, owner, pos, unit=unit_of(kernel), scale=0.3)
+    assert not out[:, 0].any() and not out[:, 33].any() and not out[..., 128:].any()
+
+
+@pytest.mark.parametrize("kernel", ["few", "chunk"])
+def test_chunked_calls_in_a_graph_follow_the_lengths(kernel):
+    lens, counts = [700, 640], KERNELS[kernel]
+    s = Setup(lens, seed=84, page_len=64, code="e4m3")
+    first, owner, _ = placed(kernel, lens)
+    q, table, held = s.queries(first[-1]), ints(s.table), ints(lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    at = ints(first)
+    with torch.cuda.stream(side):
+        gqa.decode_paged_chunked(q, s.cache, table, held, at)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = gqa.decode_paged_chunked(q, s.cache, table, held, at)
+    for now in ([700, 640], [counts[0], 333], [512, 640]):
+        held.copy_(ints(now))
+        graph.replay()
+        torch.cuda.synchronize()
+        s.lens = now
+        pos = [now[b] - n + i for b, n in enumerate(counts) for i in range(n)]
+        close(out, q, s, owner, pos, unit=CHUNK_UNIT)
