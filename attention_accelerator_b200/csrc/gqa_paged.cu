@@ -24,8 +24,8 @@ namespace {
 // what another writes.  lens_out and n_free_out may be the inputs: the last CTA
 // to have read those writes them.
 //
-// Bound by latency: two chains of loads, the sums' barriers and the search, 9 us
-// for 64 requests, 11 for 1024 with 66 thousand tokens (1.6 MB).
+// Bound by latency: two chains of loads, the sums' barriers and the search, 6.5 us
+// for 64 requests, 9.7 for 1024 with 66 thousand tokens (1.6 MB), in a replayed graph.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -194,8 +194,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // Append: RoPE of K, quantisation, and the rescale of a page's earlier codes.
 //
-// Two kernels: a step's rows, and prompts.  Measured: a step's 64 rows 3.8 us, bound by
-// latency; 18000 rows in pages of 32 33 us (111 MB, 3.3 TB/s), of 64, e4m3, 34, of 128
+// Two kernels: a step's rows, and prompts.  Measured: a step's 64 rows 3.5 us, bound by
+// latency (6.0 in pages of 64, 8.9 in pages of 128, where every block's scale grows and
+// its rows are rounded again, one after the other); 18000 rows in pages of 32 33 us (111 MB, 3.3 TB/s), of 64, e4m3, 34, of 128
 // 40, of 16 39, bound by the latency of a run's steps at 16 warps an SM.  With a head
 // after the other in a CTA, a barrier each and the rows in 256-byte pieces, they took 42,
 // 45, 60 and 46.
@@ -630,8 +631,8 @@ int launched() { return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUD
 
 // A chunked call goes to the kernel for a few queries a sequence (gqa_paged_few.cu)
 // where its rows are 6 a sequence or less on average: 48 sequences of 5 queries take
-// 125 us there and 229 in the chunked kernel, of 2 86 and 228; 12 a sequence are two
-// of its units each and take as long as the one chunk.  One sequence may hold most
+// 117 us there and 214 in the chunked kernel, of 2 85 and 212; 12 a sequence are two
+// of its units each and take as long as the one chunk (211 and 215).  One sequence may hold most
 // of the rows (a chunk of a prompt among single tokens), which only the GPU knows:
 // beyond kFewAlone rows both kernels are launched and the plan hands the call to
 // the one it is cheaper for.
@@ -775,8 +776,10 @@ int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token
     a.slots = slots;
     a.positions = positions;
     a.n_tokens = n_tokens;
-    // Measured on either side of this: 64 rows 3.8 us as a step (a CTA a token and head); 18000 rows in pages of 32
-    // 33 us as prompts, whose runs fill pages, so that a window of 16 tokens begins one at most.
+    // A step's rows are runs of one, prompts' runs fill pages, so that a window of 16 tokens begins one at most; the
+    // count of rows stands for which it is.  Measured at the change, pages of 64: 1024 runs of one row 24 us as a step
+    // (93 with every scale grown), 1025 as prompts, 16 runs after one another in a CTA, 32 us (203), 8192 122 us; 18000
+    // rows of prompts in pages of 32 33 us.
     const bool step = n_tokens <= 1024;
     a.rope = rope_steps_of(rope_theta);
     const dim3 grid(step ? n_tokens : (n_tokens - 1) / kWindow + 1, step ? cache->kv_heads : 1, 2);

@@ -34,14 +34,15 @@
 //   14         zeros of units whose rows see nothing.
 //
 // Bound, for long contexts, by a tile's chain: the softmax of 2 x 128 rows (about
-// 2500 cycles), the conversion of K and V (1400 each) and the products (2000)
-// overlap to a period of 4700 cycles; the tensor pipe is 40 % busy.  For short
+// 2300 cycles), the conversion of K and V (1350 each) and the products (2000)
+// overlap to a period of 4500 cycles; the tensor pipe is 43 % busy.  For short
 // ones, by the 25 to 28 thousand cycles a unit costs beside its tiles; for a dozen
 // queries, by the same chain with most rows empty.  Measured (B200, e4m3):
-// 16 x 128 queries on 8192 keys 309 us (883 TFLOP/s, 55 % of the cuBLAS rate;
-// 350 us under the power limit), one prompt of 8192 597 us (922 TFLOP/s), 48 x 5
-// queries on up to 8191 keys 229 us (int8, 409 MB; 127 in gqa_paged_few.cu).  Each of
-// these took longer: Q prepared by the conversion warps (371 us, spills), two passes
+// 16 x 128 queries on 8192 keys 294 us (928 TFLOP/s, 57 % of the cuBLAS rate;
+// 336 us under the power limit), one prompt of 8192 564 us (977 TFLOP/s), 48 x 5
+// queries on up to 8191 keys 214 us (int8, 409 MB; 122 in gqa_paged_few.cu).  V's scale
+// multiplied into its codes in the conversion took 308 us.  Each of these took longer
+// when it was tried: Q prepared by the conversion warps (371 us, spills), two passes
 // over S at fewer registers (354), tanh as a polynomial up to 1 instead of 1/2 (355
 // against 300, capped prompts), both M tiles on alternate tiles of few queries (281
 // against 237, and 9 % off the rest).

@@ -40,11 +40,11 @@
 // its 8-bit stage through registers into the product once.
 //
 // Bound by HBM for long contexts, by the chain length -> table entry -> page ->
-// product -> merge for short ones.  Measured (B200, int8, page 16 to 64): 64
-// ragged sequences, 586 MB, 96 us: 6.1 TB/s, 94 % of the copy rate; 148 of 4096
-// keys 188 us (6.6 TB/s); one of 131072 keys 49 us (5.5 TB/s), of 4096 12.4 us,
-// of 30 5.9 us.  32 sequences read 294.8 MB of DRAM, the codes and no more, at
-// 18 % of the tensor pipe and 38 % of the issue slots.  Tiles of 64 keys, half as
+// product -> merge for short ones.  Measured (B200, in a replayed graph): 64 ragged
+// sequences, 586 MB, e4m3 98 us (6.0 TB/s, 91 % of the copy rate; 104 us as a call),
+// int8 103; 148 of 4096 keys 190 us (6.5 TB/s); one of 131072 keys 50 us (5.4 TB/s),
+// of 4096 11.5 us, of 30 5.1 us.  32 sequences read 294.8 MB of DRAM, the codes and no
+// more, at 17 % of the tensor pipe and 45 % of the issue slots.  Tiles of 64 keys, half as
 // many, left the ring too coarse for the short shares (one of 131072: 53 us); one
 // loader warp needed 700 cycles a tile, more than the consumers; 10 to 13 consumer
 // warps do not fit the registers.

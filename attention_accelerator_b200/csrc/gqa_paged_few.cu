@@ -20,12 +20,12 @@
 // bits more than the BF16 that Q came as and the output becomes; 2^-31 of the row's
 // largest weight times scale for each key); codes are exact, sums and scores FP32.
 //
-// Bound by the consumers' instructions: of a tile's 3600 cycles in a warp the products
-// with K take 1280, those with V 1250, the softmax 1080, with the tensor pipe about a
-// third busy and 2 warps a scheduler (O's registers leave no room for more).  Measured
-// (B200, int8, page 64, 48 sequences of up to 8191 keys, 409 MB): 5 queries each 127 us
-// (3.2 TB/s; the chunked kernel 229), 4 101, 2 88 (4.6 TB/s), e4m3 118.  One sequence of 5
-// queries 35 us, a third of it the merge of its 18 shares.  Masks tested score by
+// Bound by the consumers' instructions: of a tile's 3300 cycles in a warp the products
+// with K take 1280, those with V 1120, the softmax 860, with the tensor pipe 28 % busy
+// and 2 warps a scheduler (O's registers leave no room for more).  Measured (B200,
+// int8, page 64, 48 sequences of up to 8191 keys, 409 MB): 5 queries each 122 us (3.4
+// TB/s; the chunked kernel 214), 4 101, 2 89 (4.6 TB/s), 5 of e4m3 116, with cap 132.
+// One sequence of 5 queries 32 us, a third of it the merge of its 18 shares.  Masks tested score by
 // score, a branch each, took 164 us; two result buffers and a second query warp
 // gained nothing (short contexts lost 13 %).
 #include "gqa_paged_units.cuh"

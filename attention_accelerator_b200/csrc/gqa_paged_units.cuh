@@ -102,7 +102,7 @@ struct Walk {
 // Queries of a unit, keys of a tile (log2) and what a unit costs beside its tiles, in
 // tiles: of the chunked kernel (measured: 25 to 28 thousand cycles to a tile's 5) and
 // of the one for few queries (48 x 5 drafted tokens: 147 us with 4, 128 with 12, 124
-// with 16 or 20).  And a tile of the former in tiles of the latter: 4700 cycles to 580.
+// with 16 or 20).  And a tile of the former in tiles of the latter: 4500 cycles to 540.
 constexpr int kChunkTokens = 64, kChunkTileShift = 7, kChunkUnitCost = 5;
 constexpr int kFewTokens = 6, kFewTileShift = 5, kFewUnitCost = 20;
 constexpr int kChunkTileCost = 8;
