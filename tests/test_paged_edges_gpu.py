@@ -40,10 +40,11 @@ def attend(kernel, q, cache, table, lens, first, **more):
 
 def close(got, q, setup, owner, positions, *, unit, theta=THETA, q_rotated=False, cap=0.0, slopes=None, starts=None,
           scale=1 / math.sqrt(128), floor=2.0 ** -22):
-    """Outputs (27 rows of a chunk, every row of less) against 64 bits.  A score is off by 2 units of the sum of its terms' sizes (Q, and K's or the cap's
-    rounding), FP32's 2^-19 of that and 2^-22 of the bias -- nothing that grows with the cap alone; a weight by e to
-    twice that, 3 units and 2^-20; the output by its BF16 rounding, and by ``floor`` of its row's largest sum of
-    |weight * value|: weights below FP16's range (2^-31 of the largest weight times scale, a few hundred of them)."""
+    """Outputs (27 rows of a chunk, every row of less) against 64 bits.  A score is off by 2 units of the sum of its
+    terms' sizes (Q, and K's or the cap's rounding), FP32's 2^-19 of that and 2^-22 of the bias -- nothing that grows
+    with the cap alone; a weight by e to twice that, 3 units and 2^-20; the output by its BF16 rounding, and by
+    ``floor`` of its row's largest sum of |weight * value|: weights below FP16's range (2^-31 of the largest weight
+    times scale, a few hundred of them)."""
     got = got.float().cpu().numpy().astype(np.float64)
     x = q.float().cpu().numpy().astype(np.float64)
     if not q_rotated:
