@@ -102,6 +102,18 @@ class GqaPagedParams(ctypes.Structure):
                 ("out_row_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64)]
 
 
+class GqaPagedDiff(ctypes.Structure):
+    """Mirror of ``struct gqa_paged_diff``."""
+    _fields_ = [("lambdas", ctypes.c_void_p), ("lambda_row_stride", ctypes.c_int64), ("norm_weight", ctypes.c_void_p),
+                ("norm_eps", ctypes.c_float), ("out_scale", ctypes.c_float)]
+
+
+class GqaKeyWeights(ctypes.Structure):
+    """Mirror of ``struct gqa_key_weights``."""
+    _fields_ = [("weight", ctypes.c_void_p), ("position", ctypes.c_void_p), ("evicted", ctypes.c_void_p),
+                ("capacity", ctypes.c_int64)]
+
+
 CHUNKED_WORKSPACE_BYTES = 256
 PEER_HANDLE_BYTES = 64
 CHUNKED_MAX_QUERIES = 128
@@ -162,6 +174,23 @@ _SIGNATURES = {
                                         ctypes.c_size_t, _P]),
     "gqa_decode_paged_chunked": (ctypes.c_int, [_P, _P, ctypes.POINTER(GqaPagedCache),
                                                 ctypes.POINTER(GqaPagedParams), _P, ctypes.c_size_t, _P]),
+    "gqa_decode_paged_diff": (ctypes.c_int, [_P, _P, ctypes.POINTER(GqaPagedCache), ctypes.POINTER(GqaPagedParams),
+                                             ctypes.POINTER(GqaPagedDiff), _P, ctypes.c_size_t, _P]),
+    "gqa_decode_paged_chunked_diff": (ctypes.c_int, [_P, _P, ctypes.POINTER(GqaPagedCache),
+                                                     ctypes.POINTER(GqaPagedParams), ctypes.POINTER(GqaPagedDiff), _P,
+                                                     ctypes.c_size_t, _P]),
+    "gqa_key_weights_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(GqaPagedCache),
+                                                          ctypes.POINTER(GqaPagedParams)]),
+    "gqa_decode_paged_weights": (ctypes.c_int, [_P, _P, ctypes.POINTER(GqaPagedCache), ctypes.POINTER(GqaPagedParams),
+                                                ctypes.POINTER(GqaKeyWeights), _P, ctypes.c_size_t, _P]),
+    "gqa_add_key_weights": (ctypes.c_int, [_P, ctypes.POINTER(GqaPagedCache), ctypes.POINTER(GqaPagedParams),
+                                           ctypes.POINTER(GqaKeyWeights), _P, _P, ctypes.c_size_t, _P]),
+    "gqa_plan_eviction_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "gqa_plan_eviction": (ctypes.c_int, [ctypes.POINTER(GqaKeyWeights), ctypes.c_int, _P, _P, ctypes.c_int, _P,
+                                         ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int, ctypes.c_int,
+                                         ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "gqa_evict_paged": (ctypes.c_int, [ctypes.POINTER(GqaPagedCache), _P, ctypes.c_int64, ctypes.c_int,
+                                       ctypes.POINTER(GqaKeyWeights), _P, _P, ctypes.c_int, ctypes.c_int, _P]),
     "gqa_mem_encode": (ctypes.c_int, [_P, ctypes.c_uint64, ctypes.c_int, _P, _P]),
 }
 

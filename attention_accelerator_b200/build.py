@@ -17,7 +17,8 @@ INCLUDE = ROOT / "include"
 LIB = PKG / "lib" / "libgqa_b200.so"
 SOURCES = [CSRC / "gqa_abi.cu", CSRC / "gqa_decode.cu", CSRC / "gqa_noalloc.cu", CSRC / "gqa_chunked.cu", CSRC / "gqa_peer.cu",
            CSRC / "gqa_memfile.cu", CSRC / "gqa_rtl.cu", CSRC / "gqa_paged.cu",
-           CSRC / "gqa_paged_decode.cu", CSRC / "gqa_paged_chunk.cu", CSRC / "gqa_paged_few.cu"]
+           CSRC / "gqa_paged_decode.cu", CSRC / "gqa_paged_chunk.cu", CSRC / "gqa_paged_few.cu", CSRC / "gqa_paged_weigh.cu",
+           CSRC / "gqa_paged_evict.cu"]
 HEADERS = [INCLUDE / "gqa_b200.h", CSRC / "gqa_device.cuh", CSRC / "gqa_internal.h", CSRC / "gqa_tcgen05.cuh", CSRC / "gqa_paged.cuh",
            CSRC / "gqa_paged_internal.h", CSRC / "gqa_paged_units.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -58,7 +59,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
 
 def _compile(verbose: bool) -> Path:
     tmp = LIB.with_suffix(f".so.tmp{os.getpid()}")
-    cmd = [nvcc_path(), "-shared", "-Xcompiler", "-fPIC", "-O3", "-std=c++17", *ARCH_FLAGS, "-lineinfo",
+    cmd = [nvcc_path(), "-shared", "-Xcompiler", "-fPIC", "-O3", "-std=c++17", "--threads=0", *ARCH_FLAGS, "-lineinfo",
            f"-I{INCLUDE}", f"-I{CSRC}", "-o", str(tmp), *map(str, SOURCES)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

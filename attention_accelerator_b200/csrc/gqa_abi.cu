@@ -61,8 +61,8 @@ struct DeviceInfo {
     int sms = 0;
     int cluster_cap[17] = {};  // decode clusters of n CTAs the device holds at once
     bool cluster_asked[17] = {};  // cluster_cap[n] is known
-    bool paged_init = false;
-    int paged_status = GQA_OK;
+    bool paged_init[3] = {};  // per kind of paged call
+    int paged_status[3] = {};
 };
 
 std::mutex g_mu;
@@ -416,20 +416,24 @@ int gqa::device_sms(int* sms) { return current_device(sms); }
 
 // The paged attention's 24 kernels are loaded and prepared by its own first call, not by the BF16 calls'
 // (a first BF16 decode took 13 ms for it, 5 without), which go on should a paged kernel's register shares not fit what it was built with.
-int gqa::paged_attention_sms(int* sms) {
+// So are those of its differential form and of the calls that add up the keys' weights.
+int gqa::paged_attention_sms(int* sms, PagedKernels which) {
     const int st = current_device(sms);
     int dev = 0;
     if (st != GQA_OK) return st;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return GQA_ERR_CUDA;
     std::lock_guard<std::mutex> lock(g_mu);
     DeviceInfo& di = g_dev[dev];
-    if (!di.paged_init) {
-        if (gqa::paged_decode_prepare() != cudaSuccess || gqa::paged_chunk_prepare() != cudaSuccess ||
-            gqa::paged_few_prepare() != cudaSuccess)
-            di.paged_status = GQA_ERR_CUDA;
-        di.paged_init = true;
+    const int kind = (int)which;
+    if (!di.paged_init[kind]) {
+        const bool weights = which == PagedKernels::kWeights;
+        if (gqa::paged_decode_prepare(which) != cudaSuccess ||
+            (weights ? gqa::paged_weigh_prepare() != cudaSuccess
+                     : gqa::paged_chunk_prepare(which) != cudaSuccess || gqa::paged_few_prepare(which) != cudaSuccess))
+            di.paged_status[kind] = GQA_ERR_CUDA;
+        di.paged_init[kind] = true;
     }
-    return di.paged_status;
+    return di.paged_status[kind];
 }
 
 int gqa::paged_map(CUtensorMap* map, const uint8_t* base, const PagedCacheView& c, int rows) {

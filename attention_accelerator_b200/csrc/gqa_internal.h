@@ -21,12 +21,14 @@ int check_device_memory(std::initializer_list<const void*> ptrs);
 // SM count of the current device; prepares the kernels on first use.  A status
 // (GQA_ERR_UNSUPPORTED_DEVICE where it is not an sm_100 GPU).
 int device_sms(int* sms);
-// The same for the paged attention calls, whose kernels it prepares.
-int paged_attention_sms(int* sms);
+// The same for the paged attention calls, whose kernels it prepares: each kind of call its own.
+enum class PagedKernels { kPlain, kDiff, kWeights };
+int paged_attention_sms(int* sms, PagedKernels which);
 
-cudaError_t paged_decode_prepare();
-cudaError_t paged_chunk_prepare();
-cudaError_t paged_few_prepare();
+cudaError_t paged_decode_prepare(PagedKernels which);
+cudaError_t paged_chunk_prepare(PagedKernels which);
+cudaError_t paged_few_prepare(PagedKernels which);
+cudaError_t paged_weigh_prepare();
 
 // Turns per position of rotate_half pair i, theta^(-2i/128) / 2 pi, as a Q0.64
 // fraction.  A base below 1 turns a pair by more than a turn: whole ones fall away.

@@ -212,7 +212,6 @@ struct AppendArgs {
 };
 
 constexpr int kWindow = 16;  // tokens of a prompt in which a CTA looks for runs
-constexpr float kMinBlockScale = 0x1p-100f;  // keeps 1 / scale finite for a block of zeros
 
 template <int kCode>
 __device__ __forceinline__ uint2 encode8(const float* x, float inv) {
@@ -243,19 +242,6 @@ __device__ __forceinline__ int run_length(const AppendArgs& a, int t0, int64_t s
         if (miss) break;
     }
     return len;
-}
-
-// A block's scale from the largest magnitude of its new rows (FP32 bits) and the
-// scale that its earlier rows have.
-struct BlockScale {
-    float value, inv;
-    bool grew;
-};
-__device__ __forceinline__ BlockScale block_scale(uint32_t top, float qmax, float old) {
-    const float most = top < 0x7f800000u ? __uint_as_float(top) : INFINITY;
-    const float mine = most == INFINITY ? __int_as_float(0x7fffffff) : fmaxf(__fdiv_rn(most, qmax), kMinBlockScale);
-    const float value = mine > old || mine != mine ? mine : old;
-    return BlockScale{value, value == value ? __frcp_rn(value) : 0.f, mine > old};
 }
 
 // A lane's dims 0..7 and 64..71 of a row, from `row` on.
@@ -549,7 +535,9 @@ const RopeSteps& rope_steps_of(float theta) {
     return steps;
 }
 
-int check_cache(const gqa_paged_cache* c, PagedCacheView* v) {
+}  // namespace
+
+int check_paged_cache(const gqa_paged_cache* c, PagedCacheView* v) {
     if (!c->k || !c->v || !c->k_scale || !c->v_scale) return GQA_ERR_NULL_POINTER;
     if (c->kv_heads < 1 || c->kv_heads > kNumKVHeads) return GQA_ERR_KV_HEADS;
     if (c->code != GQA_CODE_INT8 && c->code != GQA_CODE_E4M3) return GQA_ERR_FLAGS;
@@ -578,13 +566,37 @@ int check_cache(const gqa_paged_cache* c, PagedCacheView* v) {
     return GQA_OK;
 }
 
+namespace {
+
+// The differential form's own arguments; fills `call->diff`.
+int check_diff(const gqa_paged_diff* d, PagedCall* call) {
+    if (!d || !d->lambdas) return GQA_ERR_NULL_POINTER;
+    if (((uintptr_t)d->lambdas & 3) || !aligned16(d->norm_weight) || d->lambda_row_stride < 0) return GQA_ERR_ALIGNMENT;
+    if (!std::isfinite(d->out_scale) || (d->norm_weight && (!(d->norm_eps > 0.f) || !std::isfinite(d->norm_eps))))
+        return GQA_ERR_SCALE;
+    call->diff = DiffCall{d->lambdas, d->norm_weight, d->lambda_row_stride, d->norm_eps, d->out_scale};
+    return check_device_memory({d->lambdas, d->norm_weight});
+}
+
+// The keys' weights that a call adds to.
+int check_weights(const gqa_key_weights* w, const PagedCall& call, KeyWeightsView* v) {
+    if (!w || !w->weight || !w->position || !w->evicted) return GQA_ERR_NULL_POINTER;
+    if (((uintptr_t)w->weight & 3) || ((uintptr_t)w->position & 3) || ((uintptr_t)w->evicted & 3)) return GQA_ERR_ALIGNMENT;
+    // A row of the table names no more keys than there is room for.
+    if (w->capacity < ((int64_t)call.table_width << call.c.page_shift) || w->capacity > 1 << 30) return GQA_ERR_KV_RANGE;
+    // A key has a row, which need not be its position: no bias, documents or prefixes.
+    if (call.slopes || call.doc_starts || call.prefix_ends || call.query_positions) return GQA_ERR_FLAGS;
+    *v = KeyWeightsView{w->weight, w->position, w->evicted, w->capacity};
+    return check_device_memory({w->weight, w->position, w->evicted});
+}
+
 // Checks both attention calls share; fills `call`.
 int check_call(const void* q, void* out, const gqa_paged_cache* c, const gqa_paged_params* p, bool chunked,
                PagedCall* call) {
     if (!q || !out || !c || !p || !p->block_table || !p->seq_lens || (chunked && !p->first_query))
         return GQA_ERR_NULL_POINTER;
     std::memset(call, 0, sizeof(*call));
-    const int st = check_cache(c, &call->c);
+    const int st = check_paged_cache(c, &call->c);
     if (st != GQA_OK) return st;
     if (p->batch < 1 || p->batch > GQA_PAGED_MAX_BATCH || p->rows < 0 || (!chunked && p->rows != p->batch) ||
         p->table_width < 1 || p->reserved != 0)
@@ -645,14 +657,15 @@ size_t workspace_of(int batch, int rows, int heads, bool chunked, int sms) {
     return paged_few_workspace(batch, rows, heads, sms);
 }
 
-int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p, void* workspace,
-           size_t workspace_bytes, void* stream, bool chunked) {
+int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
+           const gqa_paged_diff* diff, bool is_diff, void* workspace, size_t workspace_bytes, void* stream, bool chunked) {
     PagedCall call;
     int st = check_call(q, out, cache, p, chunked, &call);
+    if (st == GQA_OK && is_diff) st = check_diff(diff, &call);
     if (st != GQA_OK) return st;
     if (!workspace || !aligned16(workspace)) return GQA_ERR_WORKSPACE;
     int sms = 0;
-    st = paged_attention_sms(&sms);
+    st = paged_attention_sms(&sms, is_diff ? PagedKernels::kDiff : PagedKernels::kPlain);
     if (st != GQA_OK) return st;
     if (workspace_bytes < workspace_of(p->batch, p->rows, cache->kv_heads, chunked, sms)) return GQA_ERR_WORKSPACE;
     st = check_device_memory({workspace});
@@ -670,7 +683,7 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     cudaError_t e = cudaSuccess;
     if (!chunked) {
         if ((st = maps(paged_decode_tile())) != GQA_OK) return st;
-        e = launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, s);
+        e = launch_paged_decode(call, rope, cache->code, kmap, vmap, sms, ws, PagedScores{}, s);
     } else {
         const bool few = few_queries(p->batch, p->rows), many = !few || p->rows > kFewAlone;
         const UnitShape chunk = paged_chunk_shape(call, sms, ws), small = few ? paged_few_shape(call, sms, ws) : chunk;
@@ -754,7 +767,7 @@ int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token
                      float rope_theta, const gqa_paged_cache* cache, void* stream) {
     if (!k || !v || !slots || !cache) return GQA_ERR_NULL_POINTER;
     AppendArgs a;
-    int st = check_cache(cache, &a.c);
+    int st = check_paged_cache(cache, &a.c);
     if (st != GQA_OK) return st;
     if (n_tokens < 0) return GQA_ERR_BATCH;
     if (!(rope_theta > 0.f) || !std::isfinite(rope_theta)) return GQA_ERR_ROPE_THETA;
@@ -801,7 +814,7 @@ int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token
 int gqa_read_paged(const gqa_paged_cache* cache, const int64_t* slots, int n, void* out_k, void* out_v, void* stream) {
     if (!cache || !slots || !out_k || !out_v) return GQA_ERR_NULL_POINTER;
     ReadArgs a;
-    int st = check_cache(cache, &a.c);
+    int st = check_paged_cache(cache, &a.c);
     if (st != GQA_OK) return st;
     if (n < 0) return GQA_ERR_BATCH;
     if (!aligned16(out_k) || !aligned16(out_v)) return GQA_ERR_ALIGNMENT;
@@ -835,12 +848,87 @@ size_t gqa_paged_workspace_bytes(const gqa_paged_cache* cache, const gqa_paged_p
 
 int gqa_decode_paged(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
                      void* workspace, size_t workspace_bytes, void* stream) {
-    return attend(q, out, cache, p, workspace, workspace_bytes, stream, false);
+    return attend(q, out, cache, p, nullptr, false, workspace, workspace_bytes, stream, false);
 }
 
 int gqa_decode_paged_chunked(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
                              void* workspace, size_t workspace_bytes, void* stream) {
-    return attend(q, out, cache, p, workspace, workspace_bytes, stream, true);
+    return attend(q, out, cache, p, nullptr, false, workspace, workspace_bytes, stream, true);
+}
+
+int gqa_decode_paged_diff(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
+                          const gqa_paged_diff* diff, void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(q, out, cache, p, diff, true, workspace, workspace_bytes, stream, false);
+}
+
+int gqa_decode_paged_chunked_diff(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
+                                  const gqa_paged_diff* diff, void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(q, out, cache, p, diff, true, workspace, workspace_bytes, stream, true);
+}
+
+size_t gqa_key_weights_workspace_bytes(const gqa_paged_cache* cache, const gqa_paged_params* p) {
+    if (!cache || !p || p->batch < 1 || p->batch > GQA_PAGED_MAX_BATCH || p->rows < 0 || p->table_width < 1 ||
+        cache->kv_heads < 1 || cache->kv_heads > kNumKVHeads || cache->page_len < 1 || cache->page_len > kPagedMaxPage ||
+        (int64_t)p->table_width * cache->page_len > 1 << 30)
+        return 0;
+    int sms = 0;
+    if (device_sms(&sms) != GQA_OK) return 0;
+    return p->first_query ? paged_weigh_workspace(p->batch, p->rows, cache->kv_heads, sms)
+                          : score_regions(p->batch, cache->kv_heads, (int64_t)p->table_width * cache->page_len, sms).end;
+}
+
+int gqa_decode_paged_weights(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
+                             const gqa_key_weights* weights, void* workspace, size_t workspace_bytes, void* stream) {
+    PagedCall call;
+    KeyWeightsView kw;
+    int st = check_call(q, out, cache, p, false, &call);
+    if (st == GQA_OK) st = check_weights(weights, call, &kw);
+    if (st != GQA_OK) return st;
+    if (!workspace || !aligned16(workspace)) return GQA_ERR_WORKSPACE;
+    int sms = 0;
+    st = paged_attention_sms(&sms, PagedKernels::kWeights);
+    if (st != GQA_OK) return st;
+    const int64_t keys = (int64_t)call.table_width << call.c.page_shift;
+    const ScoreRegions r = score_regions(call.batch, call.c.kv_heads, keys, sms);
+    if (workspace_bytes < r.end) return GQA_ERR_WORKSPACE;
+    st = check_device_memory({workspace});
+    if (st != GQA_OK) return st;
+    CUtensorMap kmap, vmap;
+    if ((st = paged_map(&kmap, call.c.k, call.c, paged_decode_tile())) != GQA_OK) return st;
+    if ((st = paged_map(&vmap, call.c.v, call.c, paged_decode_tile())) != GQA_OK) return st;
+    call.evicted = kw.evicted;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const PagedScores scores{reinterpret_cast<float*>(ws + r.scores), reinterpret_cast<float*>(ws + r.row_log2), keys};
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = launch_paged_decode(call, rope_steps_of(p->rope_theta), cache->code, kmap, vmap, sms, ws, scores, s);
+    if (e == cudaSuccess) e = launch_score_weights(call, scores, kw, sms, s);
+    return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+}
+
+int gqa_add_key_weights(const void* q, const gqa_paged_cache* cache, const gqa_paged_params* p,
+                        const gqa_key_weights* weights, const int32_t* known, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+    PagedCall call;
+    KeyWeightsView kw;
+    int st = check_call(q, const_cast<void*>(q), cache, p, true, &call);  // (no output rows)
+    if (st == GQA_OK) st = check_weights(weights, call, &kw);
+    if (st == GQA_OK) st = check_device_memory({known});
+    if (st != GQA_OK) return st;
+    if ((uintptr_t)known & 3) return GQA_ERR_ALIGNMENT;
+    if (!workspace || !aligned16(workspace)) return GQA_ERR_WORKSPACE;
+    int sms = 0;
+    st = paged_attention_sms(&sms, PagedKernels::kWeights);
+    if (st != GQA_OK) return st;
+    if (workspace_bytes < paged_weigh_workspace(call.batch, call.rows, call.c.kv_heads, sms)) return GQA_ERR_WORKSPACE;
+    st = check_device_memory({workspace});
+    if (st != GQA_OK) return st;
+    if (call.rows == 0) return GQA_OK;
+    CUtensorMap kmap;
+    if ((st = paged_map(&kmap, call.c.k, call.c, paged_weigh_box())) != GQA_OK) return st;
+    call.evicted = kw.evicted;
+    const cudaError_t e = launch_paged_weigh(call, rope_steps_of(p->rope_theta), cache->code, kmap, kw, known, sms,
+                                             static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
 }  // extern "C"

@@ -25,6 +25,13 @@ struct PagedCacheView {
     int64_t page_stride, row_stride, head_stride, scale_page_stride;
 };
 
+// Differential attention (gqa_paged_diff): Q heads 2 j and 2 j + 1 are the two maps of head j.
+struct DiffCall {
+    const float *lambdas, *gain;  // gain null: no norm
+    int64_t lambda_stride;        // of a query row
+    float eps, out_scale;
+};
+
 // One attention call over the cache (gqa_paged_params, checked).
 struct PagedCall {
     PagedCacheView c;
@@ -32,6 +39,7 @@ struct PagedCall {
     __nv_bfloat16* out;
     const int32_t* block_table;
     const int32_t *seq_lens, *query_positions, *first_query;
+    const int32_t* evicted;  // tokens that a sequence's rows are fewer than, or null
     const int32_t *doc_starts, *prefix_ends;
     const float* slopes;
     int64_t table_stride;
@@ -39,6 +47,7 @@ struct PagedCall {
     int32_t batch, rows, table_width;
     float scale, cap;
     int32_t q_rotated;
+    DiffCall diff;
 };
 
 // Keys of sequence b that can be visible at all: its length, cut to what its
@@ -48,6 +57,9 @@ __device__ __forceinline__ int paged_length(const PagedCall& a, int b) {
     const int n = a.seq_lens[b];
     return n < 0 ? 0 : (int)(n < room ? n : room);
 }
+
+// Tokens evicted from sequence b so far.
+__device__ __forceinline__ int paged_evicted(const PagedCall& a, int b) { return min(max(a.evicted[b], 0), 1 << 30); }
 
 struct KeyRange {
     int lo, hi;  // visible keys lo <= p < hi (none where hi <= lo)
@@ -81,10 +93,10 @@ __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol
 __device__ __forceinline__ void allow_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename Args>
-inline cudaError_t launch_dependent(void (*kernel)(Args), int grid, int threads, size_t smem, cudaStream_t stream,
+inline cudaError_t launch_dependent(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream,
                                     const Args& a) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -121,6 +133,53 @@ __device__ __forceinline__ uint32_t value_codes4(float y0, float y1, float y2, f
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y2, y3), __NV_SATFINITE, __NV_E4M3);
         return lo | hi << 16;
     }
+}
+
+// The difference of a row's two maps to the output row (BF16): with a gain over the
+// RMS of its 128 values, then times out_scale.  A sum of squares past FP32's range is
+// taken again of the values over 2^70, beside which eps is nothing.
+constexpr float kDiffDown = 0x1p-70f;
+__device__ __forceinline__ float diff_factor(const DiffCall& d, float sum, float eps) {
+    return d.out_scale * rsqrtf(fmaf(sum, 1.f / kHeadDim, eps));
+}
+// By a warp, 4 dims a lane.
+__device__ __forceinline__ void write_diff_row(const DiffCall& d, float4 x, __nv_bfloat16* out, int lane) {
+    float f = d.out_scale;
+    float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+    if (d.gain) {
+        g = *reinterpret_cast<const float4*>(d.gain + 4 * lane);
+        float sum = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, x.w * x.w)));
+#pragma unroll
+        for (int e = 16; e; e >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+        float eps = d.eps;
+        if (sum == INFINITY) {
+            eps = 0.f;
+            x = make_float4(x.x * kDiffDown, x.y * kDiffDown, x.z * kDiffDown, x.w * kDiffDown);
+            sum = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, x.w * x.w)));
+#pragma unroll
+            for (int e = 16; e; e >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+        }
+        f = diff_factor(d, sum, eps);
+    }
+    const __nv_bfloat162 u = __floats2bfloat162_rn(x.x * f * g.x, x.y * f * g.y);
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x.z * f * g.z, x.w * f * g.w);
+    *reinterpret_cast<uint2*>(out + 4 * lane) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+}
+
+constexpr float kMinBlockScale = 0x1p-100f;  // keeps 1 / scale finite for a block of zeros
+
+// A block's scale from the largest magnitude of its new rows (FP32 bits) and the
+// scale that its earlier rows have.
+struct BlockScale {
+    float value, inv;
+    bool grew;
+};
+__device__ __forceinline__ BlockScale block_scale(uint32_t top, float qmax, float old) {
+    const float most = top < 0x7f800000u ? __uint_as_float(top) : INFINITY;
+    const float mine = most == INFINITY ? __int_as_float(0x7fffffff) : fmaxf(__fdiv_rn(most, qmax), kMinBlockScale);
+    const float value = mine > old || mine != mine ? mine : old;
+    return BlockScale{value, value == value ? __frcp_rn(value) : 0.f, mine > old};
 }
 
 // Four codes of a word to two FP16 pairs, exactly.

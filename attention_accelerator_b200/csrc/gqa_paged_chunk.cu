@@ -331,7 +331,68 @@ __device__ __forceinline__ void take_registers() {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-template <int kCode, bool kCap, bool kBias>
+// A row of two maps' difference, kept by the two lanes of its heads (0: the first map's,
+// 1: the second's): of each half of the 128 dims the first lane has the first 32.
+struct DiffRow {
+    float d[64];
+    // The lanes' rows, dims 64 half .. of them, x times f.
+    template <int kHalf>
+    __device__ __forceinline__ void take(const float (&x)[64], float f, int lane) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const float lo = x[e] * f, hi = x[32 + e] * f;
+            const float got = __shfl_xor_sync(0xffffffffu, lane ? lo : hi, 1);
+            d[32 * kHalf + e] = lane ? got - hi : lo - got;
+        }
+    }
+    __device__ __forceinline__ void write(const DiffCall& c, __nv_bfloat16* out, int lane, bool real) {
+        float f = c.out_scale;
+        if (c.gain) {
+            float eps = c.eps;
+            auto squares = [&] {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 64; ++e) sum = fmaf(d[e], d[e], sum);
+                return sum + __shfl_xor_sync(0xffffffffu, sum, 1);
+            };
+            float sum = squares();
+            if (__any_sync(0xffffffffu, sum == INFINITY)) {
+                const float down = sum == INFINITY ? kDiffDown : 1.f;
+                eps = sum == INFINITY ? 0.f : eps;
+#pragma unroll
+                for (int e = 0; e < 64; ++e) d[e] *= down;
+                sum = squares();
+            }
+            f = diff_factor(c, sum, eps);
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+                const float4 g = __ldg(reinterpret_cast<const float4*>(c.gain + 64 * (e >> 5) + 32 * lane + (e & 31)));
+                d[e] *= f * g.x;
+                d[e + 1] *= f * g.y;
+                d[e + 2] *= f * g.z;
+                d[e + 3] *= f * g.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) d[e] *= f;
+        }
+        if (!real) return;
+#pragma unroll
+        for (int e = 0; e < 64; e += 8) {
+            uint4 w;
+            uint32_t* wp = &w.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 v = __floats2bfloat162_rn(d[e + 2 * i], d[e + 2 * i + 1]);
+                wp[i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            *reinterpret_cast<uint4*>(out + 64 * (e >> 5) + 32 * lane + (e & 31)) = w;
+        }
+    }
+};
+
+// kDiff: Q heads 2 j and 2 j + 1 are joined to one output row.
+template <int kCode, bool kCap, bool kBias, bool kDiff>
 __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkPagedArgs a) {
     extern __shared__ uint8_t raw_smem[];
     uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
@@ -624,7 +685,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 if (ok) ok = warp_wait(&s.pv_done[m], pieces & 1);
                 tc_fence_after();
                 __nv_bfloat16* out = p.out + (int64_t)(un.row0 + token) * p.out_row_stride +
-                                     (walk.h * kGroup + head) * p.out_head_stride;
+                                     (kDiff ? walk.h * (kGroup / 2) + (head >> 1) : walk.h * kGroup + head) * p.out_head_stride;
+                DiffRow joined;
+                float map_factor = 1.f;  // kDiff: of this head's map
+                if (kDiff && real && (head & 1))
+                    map_factor = p.diff.lambdas[(int64_t)(un.row0 + token) * p.diff.lambda_stride +
+                                                walk.h * (kGroup / 2) + (head >> 1)];
                 auto write = [&](int c, const float (&x)[32]) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
@@ -640,6 +706,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 };
                 if (walk.n == un.tiles) {
                     const float f = l == 0.f ? 0.f : kWeightUnit / l;  // a row that sees nothing is 0
+                    if constexpr (kDiff) {
+                        float x[64];
+                        tmem_ld32(t_o, reinterpret_cast<uint32_t(&)[32]>(x[0]));
+                        tmem_ld32(t_o + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
+                        tmem_wait_ld();
+                        joined.take<0>(x, f * map_factor, head & 1);
+                        tmem_ld32(t_o + 64, reinterpret_cast<uint32_t(&)[32]>(x[0]));
+                        tmem_ld32(t_o + 96, reinterpret_cast<uint32_t(&)[32]>(x[32]));
+                        tmem_wait_ld();
+                        joined.take<1>(x, f * map_factor, head & 1);
+                        joined.write(p.diff, out, head & 1, real);
+                    } else {
                     float x[kHeadDim];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) tmem_ld32(t_o + 32 * c, reinterpret_cast<uint32_t(&)[32]>(x[32 * c]));
@@ -649,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     if (real)
 #pragma unroll
                         for (int c = 0; c < 4; ++c) write(c, reinterpret_cast<const float(&)[32]>(x[32 * c]));
+                    }
                 } else {
                     // A piece of a unit: its slots as in decode_paged (a share's first piece 0, its last 1).
                     const int64_t first = walk.unit_first(a);
@@ -691,7 +770,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         s.last[m] = before == (uint32_t)(parts - 1);
                     }
                     group_sync();
-                    if (ok && s.last[m] && real) {
+                    // (kDiff: every lane of the warp, for the exchange between the two heads' lanes.)
+                    if (ok && s.last[m] && (kDiff || real)) {
                         // The first few parts' (m, l) stay in registers; 16 loads of a row in flight.
                         constexpr int kKept = 4;
                         auto ml = [&](int c) {
@@ -712,8 +792,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                             const float2 v = ml(c);
                             L = fmaf(fast_exp2(v.x - mu), v.y, L);
                         }
-                        const float inv = L == 0.f ? 0.f : kWeightUnit / L;
-#pragma unroll 1
+                        const float inv = (L == 0.f ? 0.f : kWeightUnit / L) * map_factor;
+#pragma unroll(kDiff ? 2 : 1)
                         for (int half = 0; half < 2; ++half) {
                             float x[64];
 #pragma unroll
@@ -734,9 +814,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                                     x[4 * e + 3] = fmaf(f, v[e].w, x[4 * e + 3]);
                                 }
                             }
-                            write(2 * half, reinterpret_cast<const float(&)[32]>(x[0]));
-                            write(2 * half + 1, reinterpret_cast<const float(&)[32]>(x[32]));
+                            if constexpr (kDiff) {
+                                if (half)
+                                    joined.take<1>(x, 1.f, head & 1);
+                                else
+                                    joined.take<0>(x, 1.f, head & 1);
+                            } else {
+                                write(2 * half, reinterpret_cast<const float(&)[32]>(x[0]));
+                                write(2 * half + 1, reinterpret_cast<const float(&)[32]>(x[32]));
+                            }
                         }
+                        if constexpr (kDiff) joined.write(p.diff, out, head & 1, real);
                     }
                 }
                 tc_fence_before();  // the next unit's products overwrite O after this thread's next arrival
@@ -955,7 +1043,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         for (int u = blockIdx.x; u < meta.units; u += gridDim.x) {
             const Unit un = a.units[u];
             if (un.tiles > 0) continue;
-            const int per_row = p.c.kv_heads * kGroup;
+            const int per_row = p.c.kv_heads * (kDiff ? kGroup / 2 : kGroup);
             for (int i = 0; i < un.n * per_row; ++i)
                 *reinterpret_cast<uint2*>(p.out + (int64_t)(un.row0 + i / per_row) * p.out_row_stride +
                                           (i % per_row) * p.out_head_stride + 4 * lane) = make_uint2(0u, 0u);
@@ -978,13 +1066,17 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
 using Kernel = void (*)(ChunkPagedArgs);
 
-Kernel kernel_for(int code, bool cap, bool bias) {
+template <bool kDiff>
+Kernel kernel_of(int code, bool cap, bool bias) {
     if (code == GQA_CODE_INT8) {
-        if (cap) return bias ? paged_chunk_kernel<0, true, true> : paged_chunk_kernel<0, true, false>;
-        return bias ? paged_chunk_kernel<0, false, true> : paged_chunk_kernel<0, false, false>;
+        if (cap) return bias ? paged_chunk_kernel<0, true, true, kDiff> : paged_chunk_kernel<0, true, false, kDiff>;
+        return bias ? paged_chunk_kernel<0, false, true, kDiff> : paged_chunk_kernel<0, false, false, kDiff>;
     }
-    if (cap) return bias ? paged_chunk_kernel<1, true, true> : paged_chunk_kernel<1, true, false>;
-    return bias ? paged_chunk_kernel<1, false, true> : paged_chunk_kernel<1, false, false>;
+    if (cap) return bias ? paged_chunk_kernel<1, true, true, kDiff> : paged_chunk_kernel<1, true, false, kDiff>;
+    return bias ? paged_chunk_kernel<1, false, true, kDiff> : paged_chunk_kernel<1, false, false, kDiff>;
+}
+Kernel kernel_for(int code, bool cap, bool bias, bool diff) {
+    return diff ? kernel_of<true>(code, cap, bias) : kernel_of<false>(code, cap, bias);
 }
 
 UnitRegions regions(int batch, int rows, int heads, int sms) {
@@ -1007,14 +1099,15 @@ int paged_chunk_tile() { return kTile; }
 
 size_t paged_chunk_workspace(int batch, int rows, int heads, int sms) { return regions(batch, rows, heads, sms).end; }
 
-cudaError_t paged_chunk_prepare() {
+cudaError_t paged_chunk_prepare(PagedKernels which) {
+    const bool diff = which == PagedKernels::kDiff;
     for (int i = 0; i < 8; ++i) {
         // The register shares are of kLaunchRegs a thread: with fewer at launch the kernel would wait for good.
         cudaFuncAttributes at;
-        cudaError_t e = cudaFuncGetAttributes(&at, kernel_for(i & 1, i & 2, i & 4));
+        cudaError_t e = cudaFuncGetAttributes(&at, kernel_for(i & 1, i & 2, i & 4, diff));
         if (e != cudaSuccess) return e;
         if (at.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
-        e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4),
+        e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4, diff),
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
         if (e != cudaSuccess) return e;
     }
@@ -1031,7 +1124,7 @@ cudaError_t launch_paged_chunk(const PagedCall& call, const RopeSteps& rope, int
     const UnitPlan& pl = shape.to;
     const ChunkPagedArgs a{kmap, vmap, call, rope, status, pl.meta, pl.units, pl.starts, pl.cuts, pl.arrivals,
                            shape.partials};
-    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), shape.ctas, kThreads, kSmemBytes,
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr, call.diff.lambdas != nullptr), shape.ctas, kThreads, kSmemBytes,
                             stream, a);
 }
 

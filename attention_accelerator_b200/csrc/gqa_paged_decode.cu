@@ -94,6 +94,10 @@ struct alignas(16) Shared {
     int sum[kThreads / 32];
 };
 
+// What a kernel does beside the plain call: kDiff joins Q heads 2 j and 2 j + 1 to one
+// row; kScores leaves every score (log2 units) and the rows' sums for the keys' weights.
+enum Mode { kPlain, kDiff, kScores };
+
 struct alignas(64) DecodePagedArgs {
     CUtensorMap kmap, vmap;  // (128, page_len, heads, pages) bytes, box (128, min(page_len, 32), 1, 1)
     PagedCall p;
@@ -101,6 +105,9 @@ struct alignas(64) DecodePagedArgs {
     uint32_t* status;
     uint32_t* arrivals;  // [batch * Q heads], zero between calls
     float* partials;     // [grid][2][4][132]
+    float* scores;       // kScores: [batch][heads][score_keys][4]
+    float* row_log2;     // kScores: [batch][Q heads], log2 of the sum of 2^score
+    int64_t score_keys;
     int stages;
 };
 
@@ -164,10 +171,11 @@ struct State {
     float m, l;
 };
 
-template <int kCode, bool kCap, bool kBias>
+template <int kCode, bool kCap, bool kBias, Mode kMode>
 __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, const float4& scales,
                                              const float4& v_rest, const uint32_t (&qf)[16], float factor, float slope, float cap2,
-                                             int key0, int lo, int hi, int m_pos, int page_shift, int lane) {
+                                             int key0, int lo, int hi, int m_pos, int page_shift, int lane,
+                                             float* scores) {
     const int g = lane >> 2, t = lane & 3;
     // Step i (16 keys) lies in page i >> sh of the tile.
     const int sh = min(page_shift, kTileShift) - 4;
@@ -191,13 +199,22 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
                 mma_16x8x16(s, a0, a1, a2, a3, qf[2 * e], qf[2 * e + 1]);
             }
             const float f = factor * (i >> sh ? sc.y : sc.x);
-            const float ve = kCap ? 0.f : i >> sh ? sc.w : sc.z;
+            const float ve = kCap || kMode == kScores ? 0.f : i >> sh ? sc.w : sc.z;
             z[i][0] = fmaf(s[0] + s[1], f, ve);
             z[i][1] = fmaf(s[2] + s[3], f, ve);
         }
     }
-    if constexpr (kCap) {
-        cap_scores(reinterpret_cast<float(&)[2 * kSteps]>(z), cap2);
+    if constexpr (kCap) cap_scores(reinterpret_cast<float(&)[2 * kSteps]>(z), cap2);
+    if constexpr (kMode == kScores) {  // 8 keys' scores of 4 heads, 128 bytes of a warp, at a time
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 16 * i + 8 * e + g;
+                if (key < hi) scores[(int64_t)key * kGroup + t] = z[i][e];  // (lo is 0 in these calls)
+            }
+    }
+    if constexpr (kCap || kMode == kScores) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
@@ -278,7 +295,7 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     }
 }
 
-template <int kCode, bool kCap, bool kBias>
+template <int kCode, bool kCap, bool kBias, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_constant__ DecodePagedArgs a) {
     extern __shared__ uint8_t raw[];
     uint8_t* ring = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);  // 128-byte swizzle atoms
@@ -286,6 +303,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     int* first = reinterpret_cast<int*>(&s + 1);
     int* los = first + (a.p.batch + 1);
     int* his = los + a.p.batch;
+    // kDiff: the second head's rows of a pair, for its first head's finisher (two turns of each pair).
+    float(*pair_row)[2][kHeadDim] = reinterpret_cast<float(*)[2][kHeadDim]>(his + a.p.batch + (3 - 3 * a.p.batch & 3));
     const PagedCall& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int batch = p.batch, heads = p.c.kv_heads, stages = a.stages;
@@ -307,13 +326,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     }
     dependency_wait();
     allow_dependents();
+    auto position_of = [&](int b) {
+        const int64_t last = (int64_t)p.seq_lens[b] - 1;
+        if constexpr (kMode == kScores) return last > 0 ? last + paged_evicted(p, b) : last;
+        return p.query_positions ? p.query_positions[b] : last;
+    };
     // Tiles of every sequence and their running sum.
     {
         const int per = (batch + kThreads - 1) / kThreads;
         const int b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
         int sum = 0;
         for (int b = b0; b < b1; ++b) {
-            const int64_t m = p.query_positions ? p.query_positions[b] : (int64_t)p.seq_lens[b] - 1;
+            const int64_t m = position_of(b);
             const KeyRange r = paged_range(p, b, m, paged_length(p, b));
             const int n = r.hi > r.lo ? ((r.hi + kTile - 1) >> kTileShift) - (r.lo >> kTileShift) : 0;
             los[b] = r.lo;
@@ -467,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                 xw[hq] = *reinterpret_cast<const uint32_t*>(q + hq * p.q_head_stride);
                 yw[hq] = *reinterpret_cast<const uint32_t*>(q + hq * p.q_head_stride + kPairs);
             }
-            const int64_t m = p.query_positions ? p.query_positions[walk.b] : (int64_t)p.seq_lens[walk.b] - 1;
+            const int64_t m = position_of(walk.b);
             float slope = 0.f;
             if (kBias && lane < kGroup) slope = p.slopes[walk.h * kGroup + lane] * 1.4426950408889634f;
             float2 f0 = make_float2(1.f, 0.f), f1 = f0;
@@ -536,12 +560,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         // piece of a unit, to a partial row -- while the consumers go on.
         const int hq = warp - kFinishWarp;
         // Sequences that see nothing.
-        for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+        constexpr int kOuts = kMode == kDiff ? kGroup / 2 : kGroup;  // output heads of a KV head
+        for (int b = blockIdx.x; b < batch && hq < kOuts; b += gridDim.x) {
             if (first[b + 1] != first[b]) continue;
             for (int h = 0; h < heads; ++h)
-                *reinterpret_cast<uint2*>(p.out + b * p.out_row_stride + (h * kGroup + hq) * p.out_head_stride +
+                *reinterpret_cast<uint2*>(p.out + b * p.out_row_stride + (h * kOuts + hq) * p.out_head_stride +
                                           4 * lane) = make_uint2(0u, 0u);
         }
+        int turn = 0;  // kDiff: of pair_row
         bool ok = true;  // after a wait that timed out: no more waits, but the counters are kept
         for (int n = 0; walk.n > 0; ++n) {
             if (ok) ok = mbar_wait(&s.rfull, n & 1);
@@ -564,7 +590,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                 add(fast_exp2(r.m[w][hq] - Mu), r.l[w][hq], *reinterpret_cast<const float4*>(&r.acc[w][hq][4 * lane]));
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.rempty);
-            bool done = walk.n == walk.unit_tiles;
+            const bool whole = walk.n == walk.unit_tiles;
+            bool done = whole;
             if (!done) {
                 // A piece of a unit: store it, and the unit's last CTA merges all.
                 // Tile x lies in the share of CTA ceil((x + 1) G / T) - 1.  A share's
@@ -573,22 +600,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                 const int c0 = (int)(((walk.unit_first + 1) * G + total - 1) / total) - 1;
                 const int pieces = (int)(((walk.unit_first + walk.unit_tiles) * G + total - 1) / total) - c0;
                 const int second = total * c0 / G < walk.unit_first ? 1 : 0;
-                auto piece = [&](int c) {
-                    return a.partials + (((c0 + c) * 2 + (c ? 0 : second)) * kGroup + hq) * kPartialFloats;
+                auto piece = [&](int c, int head) {
+                    return a.partials + (((c0 + c) * 2 + (c ? 0 : second)) * kGroup + head) * kPartialFloats;
                 };
-                float* mine = piece((int)me - c0);
+                float* mine = piece((int)me - c0, hq);
                 *reinterpret_cast<float4*>(mine + 4 * lane) = A;
                 if (lane == 0) *reinterpret_cast<float2*>(mine + kHeadDim) = make_float2(M, L);
                 __syncwarp();
                 uint32_t before = 0;
+                // kDiff: both heads of a pair arrive at its first one's counter, and the last warp merges both.
+                const uint32_t all = (uint32_t)(kMode == kDiff ? 2 * pieces : pieces);
                 if (lane == 0) {
                     // Releases the warp's row and acquires the others'.
-                    uint32_t* count = a.arrivals + (walk.b * heads + walk.h) * kGroup + hq;
+                    uint32_t* count = a.arrivals + (walk.b * heads + walk.h) * kGroup + (kMode == kDiff ? hq & ~1 : hq);
                     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
-                    if (before == (uint32_t)(pieces - 1)) *count = 0;
+                    if (before == all - 1) *count = 0;
                 }
-                done = __shfl_sync(0xffffffffu, before, 0) == (uint32_t)(pieces - 1);
-                if (done) {
+                done = __shfl_sync(0xffffffffu, before, 0) == all - 1;
+                auto merge = [&](int head) {
                     constexpr int kAtOnce = 10;
                     M = -INFINITY;
                     L = 0.f;
@@ -599,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                         float now = M;
 #pragma unroll
                         for (int e = 0; e < kAtOnce; ++e) {
-                            const float* x = piece(min(c + e, pieces - 1));
+                            const float* x = piece(min(c + e, pieces - 1), head);
                             ml[e] = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
                             v[e] = __ldcg(reinterpret_cast<const float4*>(x + 4 * lane));
                         }
@@ -614,9 +643,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
                         for (int e = 0; e < kAtOnce; ++e)
                             if (c + e < pieces) add(fast_exp2(ml[e].x - use), ml[e].y, v[e]);
                     }
+                };
+                if (done) {
+                    if constexpr (kMode == kDiff) {
+                        merge(hq | 1);
+                        const float f = p.diff.lambdas[walk.b * p.diff.lambda_stride + walk.h * (kGroup / 2) + (hq >> 1)];
+                        const float4 b = make_float4(f * (A.x / L), f * (A.y / L), f * (A.z / L), f * (A.w / L));
+                        merge(hq & ~1);
+                        write_diff_row(p.diff, make_float4(A.x / L - b.x, A.y / L - b.y, A.z / L - b.z, A.w / L - b.w),
+                                       p.out + walk.b * p.out_row_stride +
+                                           (walk.h * (kGroup / 2) + (hq >> 1)) * p.out_head_stride,
+                                       lane);
+                    } else {
+                        merge(hq);
+                    }
                 }
             }
-            if (done) {
+            if constexpr (kMode == kDiff) {
+                if (whole) {
+                    const int j = hq >> 1;
+                    float* row = pair_row[j][turn];
+                    turn ^= 1;  // (the pair is at most one turn apart: what is read now is not written before the next barrier)
+                    if (hq & 1) {
+                        const float f = p.diff.lambdas[walk.b * p.diff.lambda_stride + walk.h * (kGroup / 2) + j];
+                        *reinterpret_cast<float4*>(row + 4 * lane) =
+                            make_float4(f * (A.x / L), f * (A.y / L), f * (A.z / L), f * (A.w / L));
+                    }
+                    named_barrier_sync(1 + j, 64);  // both warps of the pair
+                    if (!(hq & 1)) {
+                        const float4 b = *reinterpret_cast<const float4*>(row + 4 * lane);
+                        write_diff_row(p.diff, make_float4(A.x / L - b.x, A.y / L - b.y, A.z / L - b.z, A.w / L - b.w),
+                                       p.out + walk.b * p.out_row_stride + (walk.h * (kGroup / 2) + j) * p.out_head_stride,
+                                       lane);
+                    }
+                }
+            } else if (done) {
+                if (kMode == kScores && lane == 0)
+                    a.row_log2[(walk.b * heads + walk.h) * kGroup + hq] = M + log2f(L);
                 const __nv_bfloat162 x = __floats2bfloat162_rn(A.x / L, A.y / L), y = __floats2bfloat162_rn(A.z / L, A.w / L);
                 *reinterpret_cast<uint2*>(p.out + walk.b * p.out_row_stride + (walk.h * kGroup + hq) * p.out_head_stride +
                                           4 * lane) =
@@ -648,6 +711,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         }
         const float factor = slot.factor[t], slope = slot.slope[t];
         const int lo = slot.lo, hi = slot.hi, m_pos = slot.m;
+        float* unit_scores = nullptr;
+        if constexpr (kMode == kScores)
+            unit_scores = a.scores + (int64_t)(walk.b * heads + walk.h) * a.score_keys * kGroup;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.qempty[sl]);
 
@@ -662,9 +728,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         for (; mine < walk.n; mine += kWarps) {
             const int j = mine;
             if (ok) ok = mbar_wait(&s.full[stg], phase);
-            consume_tile<kCode, kCap, kBias>(st, ring + stg * kStageBytes, s.scales[stg], s.v_rest[stg], qf, factor, slope,
-                                             p.cap * 1.4426950408889634f, (walk.tile + j) * kTile, lo, hi, m_pos,
-                                             p.c.page_shift, lane);
+            consume_tile<kCode, kCap, kBias, kMode>(st, ring + stg * kStageBytes, s.scales[stg], s.v_rest[stg], qf, factor,
+                                                    slope, p.cap * 1.4426950408889634f, (walk.tile + j) * kTile, lo, hi,
+                                                    m_pos, p.c.page_shift, lane, unit_scores);
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.empty[stg]);
             stg += kWarps;
@@ -701,25 +767,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
 // A wait by parity is sound only for the phase after the last one that the same
 // warp saw complete, so each stage has one consumer warp and one loader warp: the
 // ring is a whole number of stages for each consumer warp, and of loader groups.
-int decode_stages(int batch) {
-    static_assert(227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * GQA_PAGED_MAX_BATCH + 1) * 4 >=
+constexpr int kPairRowBytes = 16 + 2 * 2 * kHeadDim * (int)sizeof(float);  // (and its alignment)
+int decode_stages(int batch, Mode mode) {
+    static_assert(227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * GQA_PAGED_MAX_BATCH + 1) * 4 - kPairRowBytes >=
                       (int64_t)kStageBytes * kWarps,
                   "a stage for every consumer warp");
     static_assert(kWarps % kBurst == 0 && kMaxStages % kWarps == 0, "whole groups");
-    const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * (int64_t)batch + 1) * 4;
+    const int64_t room = 227 * 1024 - 1024 - (int64_t)sizeof(Shared) - (3 * (int64_t)batch + 1) * 4 -
+                         (mode == kDiff ? kPairRowBytes : 0);
     const int64_t n = room / kStageBytes;
     return (int)(n < kMaxStages ? n : kMaxStages) / kWarps * kWarps;
 }
 
 using Kernel = void (*)(DecodePagedArgs);
 
-Kernel kernel_for(int code, bool cap, bool bias) {
-    if (code == GQA_CODE_INT8) {
-        if (cap) return bias ? paged_decode_kernel<0, true, true> : paged_decode_kernel<0, true, false>;
-        return bias ? paged_decode_kernel<0, false, true> : paged_decode_kernel<0, false, false>;
+template <Mode kMode>
+Kernel kernel_of(int code, bool cap, bool bias) {
+    if constexpr (kMode == kScores) {  // without bias: a key's row is not its position
+        if (code == GQA_CODE_INT8)
+            return cap ? paged_decode_kernel<0, true, false, kMode> : paged_decode_kernel<0, false, false, kMode>;
+        return cap ? paged_decode_kernel<1, true, false, kMode> : paged_decode_kernel<1, false, false, kMode>;
+    } else {
+        if (code == GQA_CODE_INT8) {
+            if (cap) return bias ? paged_decode_kernel<0, true, true, kMode> : paged_decode_kernel<0, true, false, kMode>;
+            return bias ? paged_decode_kernel<0, false, true, kMode> : paged_decode_kernel<0, false, false, kMode>;
+        }
+        if (cap) return bias ? paged_decode_kernel<1, true, true, kMode> : paged_decode_kernel<1, true, false, kMode>;
+        return bias ? paged_decode_kernel<1, false, true, kMode> : paged_decode_kernel<1, false, false, kMode>;
     }
-    if (cap) return bias ? paged_decode_kernel<1, true, true> : paged_decode_kernel<1, true, false>;
-    return bias ? paged_decode_kernel<1, false, true> : paged_decode_kernel<1, false, false>;
+}
+
+Kernel kernel_for(int code, bool cap, bool bias, Mode mode) {
+    return mode == kDiff     ? kernel_of<kDiff>(code, cap, bias)
+           : mode == kScores ? kernel_of<kScores>(code, cap, bias)
+                             : kernel_of<kPlain>(code, cap, bias);
 }
 
 }  // namespace
@@ -733,7 +814,9 @@ size_t paged_decode_workspace(int sms) {
 }
 
 cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
-                                const CUtensorMap& vmap, int sms, uint8_t* ws, cudaStream_t stream) {
+                                const CUtensorMap& vmap, int sms, uint8_t* ws, const PagedScores& scores,
+                                cudaStream_t stream) {
+    const Mode mode = scores.scores ? kScores : call.diff.lambdas ? kDiff : kPlain;
     DecodePagedArgs a;
     a.kmap = kmap;
     a.vmap = vmap;
@@ -742,14 +825,19 @@ cudaError_t launch_paged_decode(const PagedCall& call, const RopeSteps& rope, in
     a.status = reinterpret_cast<uint32_t*>(ws);
     a.arrivals = reinterpret_cast<uint32_t*>(ws + kPagedArrivalsOffset);
     a.partials = reinterpret_cast<float*>(ws + kPagedPartialsOffset);
-    a.stages = decode_stages(call.batch);
-    const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (3 * (size_t)call.batch + 1) * 4;
-    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), sms, kThreads, smem, stream, a);
+    a.scores = scores.scores;
+    a.row_log2 = scores.row_log2;
+    a.score_keys = scores.keys;
+    a.stages = decode_stages(call.batch, mode);
+    const size_t smem = 1024 + (size_t)a.stages * kStageBytes + sizeof(Shared) + (3 * (size_t)call.batch + 1) * 4 +
+                        (mode == kDiff ? kPairRowBytes : 0);
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr, mode), sms, kThreads, smem, stream, a);
 }
 
-cudaError_t paged_decode_prepare() {
-    for (int i = 0; i < 8; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4),
+cudaError_t paged_decode_prepare(PagedKernels which) {
+    const Mode mode = which == PagedKernels::kDiff ? kDiff : which == PagedKernels::kWeights ? kScores : kPlain;
+    for (int i = 0; i < (mode == kScores ? 4 : 8); ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4, mode),
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
         if (e != cudaSuccess) return e;
     }

@@ -28,6 +28,7 @@
 // One sequence of 5 queries 32 us, a third of it the merge of its 18 shares.  Masks tested score by
 // score, a branch each, took 164 us; two result buffers and a second query warp
 // gained nothing (short contexts lost 13 %).
+#include "gqa_internal.h"
 #include "gqa_paged_units.cuh"
 
 namespace gqa {
@@ -76,6 +77,7 @@ struct alignas(16) Shared {
         float m[kWarps][2 * kGroup], l[kWarps][2 * kGroup];
     } result;
     int64_t cuts[kMaxCtas + 1];
+    float pair_row[2][2][2][kHeadDim];  // kDiff: [turn][pair][query]: the second head's rows, for the first's finisher
 };
 
 struct alignas(64) FewPagedArgs {
@@ -275,7 +277,8 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
     }
 }
 
-template <int kCode, bool kCap, bool kBias>
+// kDiff: Q heads 2 j and 2 j + 1 are joined to one output row.
+template <int kCode, bool kCap, bool kBias, bool kDiff>
 __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_constant__ FewPagedArgs a) {
     extern __shared__ uint8_t raw[];
     uint8_t* ring = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);  // 128-byte swizzle atoms
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
         Walk walk;
         walk.start(a, meta);
         const int hq = warp - kFinishWarp;
-        int passes = 0;
+        int passes = 0, turn = 0;
         for (; walk.n > 0;) {
             const Unit& un = walk.unit;
             const int pairs = (un.n + 1) >> 1;
@@ -421,8 +424,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                 pieces = share_of(first + un.tiles - 1) - c0 + 1;
                 second = s.cuts[c0] < first ? 1 : 0;
             }
-            auto piece = [&](int c, int q, int e) {
-                return a.partials + ((int64_t)(((c0 + c) * 2 + (c ? 0 : second)) * kUnitRows) + (2 * q + e) * kGroup + hq) * kRowF;
+            auto piece = [&](int c, int q, int e, int head) {
+                return a.partials + ((int64_t)(((c0 + c) * 2 + (c ? 0 : second)) * kUnitRows) + (2 * q + e) * kGroup + head) * kRowF;
+            };
+            // kDiff: a row's values times f, and the joined row's output.
+            auto times = [&](float4 x, float l, float f) {
+                f *= l == 0.f ? 0.f : kWeightUnit / l;
+                return make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+            };
+            auto lambda_of = [&](int token) {
+                return token < un.n ? p.diff.lambdas[(int64_t)(un.row0 + token) * p.diff.lambda_stride +
+                                                     walk.h * (kGroup / 2) + (hq >> 1)]
+                                    : 0.f;
+            };
+            auto write_diff = [&](int token, float4 x, float4 y) {
+                if (token < un.n)
+                    write_diff_row(p.diff, make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w),
+                                   p.out + (int64_t)(un.row0 + token) * p.out_row_stride +
+                                       (walk.h * (kGroup / 2) + (hq >> 1)) * p.out_head_stride,
+                                   lane);
             };
             auto write = [&](int q, int e, float4 x, float l) {
                 const int token = 2 * q + e;
@@ -458,12 +478,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.rempty);
+                if constexpr (kDiff) {
+                    if (whole) {
+                        const int j = hq >> 1;
+                        auto& rows = s.pair_row[turn][j];
+                        turn ^= 1;  // (the pair is at most one turn apart: these are not written before the next barrier)
+                        if (hq & 1)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                *reinterpret_cast<float4*>(&rows[e][4 * lane]) = times(A[e], L[e], lambda_of(2 * q + e));
+                        named_barrier_sync(1 + j, 64);  // both warps of the pair
+                        if (!(hq & 1))
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                write_diff(2 * q + e, times(A[e], L[e], 1.f),
+                                           *reinterpret_cast<const float4*>(&rows[e][4 * lane]));
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     if (whole) {
-                        write(q, e, A[e], L[e]);
+                        if constexpr (!kDiff) write(q, e, A[e], L[e]);
                     } else {
-                        float* mine = piece((int)blockIdx.x - c0, q, e);
+                        float* mine = piece((int)blockIdx.x - c0, q, e, hq);
                         *reinterpret_cast<float4*>(mine + 4 * lane) = A[e];
                         if (lane == 0) *reinterpret_cast<float2*>(mine + kHeadDim) = make_float2(M[e], L[e]);
                     }
@@ -475,21 +512,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                 if (lane == 0)  // releases the warp's rows and acquires the others'
                     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
                                  : "=r"(before)
-                                 : "l"(a.arrivals + c0 * kGroup + hq)
+                                 : "l"(a.arrivals + c0 * kGroup + (kDiff ? hq & ~1 : hq))
                                  : "memory");
-                if (__shfl_sync(0xffffffffu, before, 0) == (uint32_t)(pieces - 1)) {
+                // (kDiff: both heads of a pair arrive at its first one's counter, and the last warp merges both.)
+                if (__shfl_sync(0xffffffffu, before, 0) == (uint32_t)((kDiff ? 2 * pieces : pieces) - 1)) {
                     constexpr int kAtOnce = 6;
                     for (int token = 0; token < un.n; ++token) {
                         const int q = token >> 1, e = token & 1;
-                        float M = -INFINITY, L = 0.f;
-                        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+                        float M, L;
+                        float4 A;
+                        auto merge = [&](int head) {
+                        M = -INFINITY;
+                        L = 0.f;
+                        A = make_float4(0.f, 0.f, 0.f, 0.f);
                         for (int c = 0; c < pieces; c += kAtOnce) {
                             float4 v[kAtOnce];
                             float2 ml[kAtOnce];
                             float now = M;
 #pragma unroll
                             for (int i = 0; i < kAtOnce; ++i) {
-                                const float* x = piece(min(c + i, pieces - 1), q, e);
+                                const float* x = piece(min(c + i, pieces - 1), q, e, head);
                                 ml[i] = __ldcg(reinterpret_cast<const float2*>(x + kHeadDim));
                                 v[i] = __ldcg(reinterpret_cast<const float4*>(x + 4 * lane));
                             }
@@ -508,7 +550,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                                     A = make_float4(fmaf(f, v[i].x, A.x), fmaf(f, v[i].y, A.y), fmaf(f, v[i].z, A.z), fmaf(f, v[i].w, A.w));
                                 }
                         }
-                        write(q, e, A, L);
+                        };
+                        if constexpr (kDiff) {
+                            merge(hq | 1);
+                            const float4 second_map = times(A, L, lambda_of(token));
+                            merge(hq & ~1);
+                            write_diff(token, times(A, L, 1.f), second_map);
+                        } else {
+                            merge(hq);
+                            write(q, e, A, L);
+                        }
                     }
                 }
             }
@@ -692,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             }
         } else {
             // Units whose rows see nothing.
-            const int per_row = p.c.kv_heads * kGroup;
+            const int per_row = p.c.kv_heads * (kDiff ? kGroup / 2 : kGroup);
             for (int u = blockIdx.x; u < meta.units; u += gridDim.x) {
                 const Unit un = a.units[u];
                 if (un.tiles > 0) continue;
@@ -712,13 +763,17 @@ static_assert(kWarps % kBurst == 0 && kStages % (kBurst * kLoaders) == 0 && kSta
 
 using Kernel = void (*)(FewPagedArgs);
 
-Kernel kernel_for(int code, bool cap, bool bias) {
+template <bool kDiff>
+Kernel kernel_of(int code, bool cap, bool bias) {
     if (code == GQA_CODE_INT8) {
-        if (cap) return bias ? paged_few_kernel<0, true, true> : paged_few_kernel<0, true, false>;
-        return bias ? paged_few_kernel<0, false, true> : paged_few_kernel<0, false, false>;
+        if (cap) return bias ? paged_few_kernel<0, true, true, kDiff> : paged_few_kernel<0, true, false, kDiff>;
+        return bias ? paged_few_kernel<0, false, true, kDiff> : paged_few_kernel<0, false, false, kDiff>;
     }
-    if (cap) return bias ? paged_few_kernel<1, true, true> : paged_few_kernel<1, true, false>;
-    return bias ? paged_few_kernel<1, false, true> : paged_few_kernel<1, false, false>;
+    if (cap) return bias ? paged_few_kernel<1, true, true, kDiff> : paged_few_kernel<1, true, false, kDiff>;
+    return bias ? paged_few_kernel<1, false, true, kDiff> : paged_few_kernel<1, false, false, kDiff>;
+}
+Kernel kernel_for(int code, bool cap, bool bias, bool diff) {
+    return diff ? kernel_of<true>(code, cap, bias) : kernel_of<false>(code, cap, bias);
 }
 
 // Behind the chunked kernel's.  Units enough for any split of the rows, so that a call
@@ -740,14 +795,15 @@ UnitShape paged_few_shape(const PagedCall& call, int sms, uint8_t* ws) {
                       ctas * kGroup, true);
 }
 
-cudaError_t paged_few_prepare() {
+cudaError_t paged_few_prepare(PagedKernels which) {
+    const bool diff = which == PagedKernels::kDiff;
     for (int i = 0; i < 8; ++i) {
         // The register shares are of kLaunchRegs a thread: with fewer at launch the kernel would wait for good.
         cudaFuncAttributes at;
-        cudaError_t e = cudaFuncGetAttributes(&at, kernel_for(i & 1, i & 2, i & 4));
+        cudaError_t e = cudaFuncGetAttributes(&at, kernel_for(i & 1, i & 2, i & 4, diff));
         if (e != cudaSuccess) return e;
         if (at.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
-        e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        e = cudaFuncSetAttribute(kernel_for(i & 1, i & 2, i & 4, diff), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -757,7 +813,7 @@ cudaError_t launch_paged_few(const PagedCall& call, const RopeSteps& rope, int c
                              const CUtensorMap& vmap, const UnitShape& shape, uint32_t* status, cudaStream_t stream) {
     const UnitPlan& pl = shape.to;
     const FewPagedArgs a{kmap, vmap, call, rope, status, pl.meta, pl.units, pl.starts, pl.cuts, pl.arrivals, shape.partials};
-    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr), shape.ctas, kThreads, kSmemBytes,
+    return launch_dependent(kernel_for(code, call.cap > 0.f, call.slopes != nullptr, call.diff.lambdas != nullptr), shape.ctas, kThreads, kSmemBytes,
                             stream, a);
 }
 

@@ -1,0 +1,949 @@
+// gqa_paged_weigh.cu -- the attention weight that keys of the paged 8-bit cache get,
+// summed over queries and over the Q heads of a KV head's group.
+//
+//   weight[b][h][k] += sum over queries i that see k, Q heads g of h:  2^(z_igk - log2 sum_k' 2^z_igk')
+//
+// One token a sequence: paged_decode_kernel leaves its scores (16 bytes a key and KV
+// head) and the rows' sums; score_weights_kernel turns them into weights.
+//
+// Any number of queries, in three kernels on the fifth-generation tensor cores:
+//   weigh_queries_kernel  rotates the queries of a unit (64 consecutive queries of a
+//                         sequence, one KV head: 256 rows) and leaves them as two FP16
+//                         parts in the operand layout, so that no later pass rotates again.
+//   weigh_kernel, rows    S = Q K^T, a thread a row: running maximum and sum over the keys.
+//   weigh_kernel, keys    S^T = K Q^T, a thread a key: the sum of 2^(z - row's log2) over
+//                         the rows needs no exchange between threads, and a tile's keys
+//                         have one CTA, which adds the units' sums in order: no atomics.
+// The sums of a row are known only once all its keys were seen, so the product is
+// computed twice; keeping it (1 KB a key and KV head for 64 queries) would move eight
+// times the bytes that the codes have.
+//
+// Precision.  The weights are FP32 results: Q, divided by a power of two that brings a
+// row's largest below 1, is split into two FP16 parts (22 bits), both products
+// accumulate in the same FP32 columns; codes are exact.
+//
+// Warps of weigh_kernel (one CTA per SM; shares of even cost, from the lengths in device
+// memory, which every CTA sums itself):
+//   0-7    a thread a row (rows) or a key and half of the columns (keys)
+//   8-11   codes (TMA, 64 keys at a time) to FP16 operands
+//   12     MMA issuer, two tiles of accumulators in TMEM
+//   13, 14 loaders of codes and of queries
+#include "gqa_internal.h"
+#include "gqa_paged.cuh"
+#include "gqa_paged_internal.h"
+#include "gqa_tcgen05.cuh"
+
+namespace gqa {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// One token a sequence: scores to weights.
+// ---------------------------------------------------------------------------
+struct ScoreArgs {
+    PagedCall p;
+    PagedScores s;
+    KeyWeightsView w;
+};
+
+constexpr int kScoreThreads = 256, kScoreKeys = 4;  // keys a thread at a time
+
+__global__ void __launch_bounds__(kScoreThreads) score_weights_kernel(const __grid_constant__ ScoreArgs a) {
+    dependency_wait();
+    allow_dependents();
+    const int heads = a.p.c.kv_heads, b = blockIdx.x / heads;
+    const int len = paged_length(a.p, b), last = a.p.seq_lens[b] - 1;
+    if (len == 0) return;
+    const int64_t at = (int64_t)blockIdx.x * a.w.capacity;
+    const float4* scores = reinterpret_cast<const float4*>(a.s.scores) + (int64_t)blockIdx.x * a.s.keys;
+    const float4 sum = *reinterpret_cast<const float4*>(a.s.row_log2 + (int64_t)blockIdx.x * kGroup);
+    constexpr int kBlock = kScoreThreads * kScoreKeys;
+    for (int64_t k0 = (int64_t)blockIdx.y * kBlock + threadIdx.x; k0 < len; k0 += (int64_t)gridDim.y * kBlock) {
+        float4 z[kScoreKeys];
+        float old[kScoreKeys];
+#pragma unroll
+        for (int i = 0; i < kScoreKeys; ++i) {
+            const int64_t k = k0 + i * kScoreThreads;
+            if (k >= len) break;
+            z[i] = __ldcg(scores + k);
+            old[i] = k < last ? a.w.weight[at + k] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kScoreKeys; ++i) {
+            const int64_t k = k0 + i * kScoreThreads;
+            if (k >= len) break;
+            const float w = (fast_exp2(z[i].x - sum.x) + fast_exp2(z[i].y - sum.y)) +
+                            (fast_exp2(z[i].z - sum.z) + fast_exp2(z[i].w - sum.w));
+            a.w.weight[at + k] = old[i] + w;
+            if (k == last) a.w.position[at + k] = last + (last > 0 ? paged_evicted(a.p, b) : 0);
+        }
+    }
+    if (last == 0 && blockIdx.x == b * heads && blockIdx.y == 0 && threadIdx.x == 0) a.w.evicted[b] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Any number of queries.
+// ---------------------------------------------------------------------------
+constexpr int kTokens = 64;                        // queries of a unit
+constexpr int kRows = kTokens * kGroup;            // its rows
+constexpr int kTile = 128, kTileShift = 7;         // keys
+constexpr int kHalfKeys = 64;                      // of a TMA slot
+constexpr int kRawBytes = kHalfKeys * kHeadDim;
+constexpr int kBlockBytes = kTile * 128;           // 64 dims of a tile in FP16
+constexpr int kTileBytes = 2 * kBlockBytes;
+constexpr int kQBlockBytes = kRows * 128;          // 64 dims of a part of the rows
+constexpr int kQBytes = 4 * kQBlockBytes;          // [part][64 dims][row]
+constexpr int kRaw = 3, kConv = 2, kScaleSlots = 8;
+constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kQueryWarp = 14;
+constexpr int kThreads = 16 * 32, kSumThreads = 8 * 32;
+constexpr uint32_t kTmemCols = 512;                // two tiles of 256 columns
+// What a unit costs beside its tiles when the shares of the rows' pass are cut, in tiles.
+constexpr int kUnitCost = 2;
+constexpr float kHeadroom = 8.f;                   // log2 by which a maximum may pass the reference
+
+// kind::f16, FP16 A and B (both K-major), FP32 accumulators, M = 128.
+constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 4) << 24);
+__device__ __forceinline__ constexpr uint32_t idesc_n(uint32_t n) { return kIdesc | ((n >> 3) << 17); }
+
+struct alignas(64) WeighArgs {
+    CUtensorMap kmap;  // (128, page_len, heads, pages) bytes, box (128, min(page_len, 64), 1, 1)
+    PagedCall p;
+    RopeSteps rope;
+    KeyWeightsView w;
+    const int32_t* known;
+    uint32_t* status;
+    uint8_t* queries;    // [units * heads][kQBytes]
+    float* factor;       // [units * heads][kRows]: z of a row is its product times the page's scale times this
+    float* row_log2;     // [units * heads][kRows]: log2 of the sum of 2^z
+    uint32_t* arrivals;  // [units * heads]
+    float2* partials;    // [ctas][2][kRows]: reference and sum
+    int max_units;
+};
+
+// A sequence's queries and keys.  Queries at negative positions see nothing and are left out.
+struct Seq {
+    int row0, n, pos0, len;  // first query row, queries, the first one's row of the cache, keys
+    int tiles, units, id0;   // tiles of keys, units of queries, number of the first unit in the call
+    int c;                   // ceil(pos0 / 64)
+    __device__ __forceinline__ Seq() {}
+    __device__ __forceinline__ Seq(const PagedCall& p, int b) {
+        const int first = min(max(p.first_query[b], 0), p.rows);
+        const int all = max(0, min(p.first_query[b + 1], p.rows) - first), keys = max(0, p.seq_lens[b]);
+        n = min(all, keys);
+        row0 = first + all - n;
+        pos0 = keys - n;
+        len = paged_length(p, b);
+        tiles = (len + kTile - 1) >> kTileShift;
+        units = (n + kTokens - 1) / kTokens;
+        // A number for each unit that needs no sum over the sequences: it grows by one from unit to unit and by
+        // one at least from sequence to sequence.
+        id0 = row0 / kTokens + b;
+        c = (pos0 + kTokens - 1) / kTokens;
+    }
+    // Tiles that unit u sees: of the keys up to its last query, ceil((pos0 + 64 (u + 1)) / 128) = floor((c + u + 2) / 2).
+    __device__ __forceinline__ int unit_tiles(int u) const {
+        return min(tiles, u < units - 1 ? (c + u + 2) >> 1 : (int)(((int64_t)pos0 + n + kTile - 1) >> kTileShift));
+    }
+    // Cells of units before u, a unit's own cost and one a tile: the sum of floor(i / 2) up to i < k is floor((k - 1)^2 / 4).
+    __device__ __forceinline__ int64_t unit_cells(int u) const {
+        const int v = min(u, units - 1);
+        const int whole = min(v, max(0, 2 * tiles - c - 2));  // units that do not see all tiles
+        auto f = [](int64_t k) { return (k - 1) * (k - 1) / 4; };
+        int64_t cells = f((int64_t)c + 2 + whole) - f((int64_t)c + 2) + (int64_t)(v - whole) * tiles;
+        if (u == units && units > 0) cells += unit_tiles(units - 1);
+        return cells + (int64_t)u * kUnitCost;
+    }
+    // The first unit that sees tile i: those before end below it.
+    __device__ __forceinline__ int first_unit(int i) const { return max(0, 2 * i - c); }
+    // Cells of tiles before i: one for each unit that sees them.
+    __device__ __forceinline__ int64_t tile_cells(int i) const {
+        const int i0 = (c + 1) >> 1;
+        const int64_t gone = i > i0 ? (int64_t)(i - i0) * (i + i0 - 1 - c) : 0;
+        return (int64_t)units * i - gone;
+    }
+    template <bool kKeys>
+    __device__ __forceinline__ int64_t cells() const {
+        return units == 0 ? 0 : kKeys ? tile_cells(tiles) : unit_cells(units);
+    }
+};
+
+// A CTA's share, run by run: consecutive tiles for one unit of queries and one head.
+template <bool kKeys>
+struct Walk {
+    const PagedCall& p;
+    Seq q;
+    int b, h, u;             // sequence, head, unit
+    int tile0, count;        // of the run
+    int j0, j1;              // kKeys: the piece's tiles, for which units follow one another
+    int64_t cell, base, end; // cell of the run's first tile (rows) or of the piece's (keys); of the sequence's first; the share's end
+    __device__ __forceinline__ Walk(const PagedCall& call) : p(call) {}
+
+    __device__ __forceinline__ int id() const { return q.id0 + u; }
+    __device__ __forceinline__ int queries() const { return min(kTokens, q.n - u * kTokens); }
+    __device__ __forceinline__ int pos() const { return q.pos0 + u * kTokens; }
+
+    // From cell x (of sequence `seq`, whose first cell is `first`) to `stop`.
+    __device__ __forceinline__ void start(int seq, int64_t first, int64_t x, int64_t stop) {
+        count = 0;
+        end = stop;
+        if (x >= stop) return;
+        b = seq;
+        base = first;
+        q = Seq(p, b);
+        const int64_t each = q.cells<kKeys>();
+        h = (int)((x - base) / each);
+        const int64_t rem = x - base - h * each;
+        // The last unit, or the first tile, at or before (after) the cell.
+        int lo = 0, hi = kKeys ? q.tiles : q.units;
+        if constexpr (kKeys) {
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (q.tile_cells(mid) >= rem) hi = mid; else lo = mid + 1;
+            }
+            j0 = lo;
+            if (j0 == q.tiles) {
+                j0 = 0;
+                if (!next_head()) return;
+            }
+            piece();
+        } else {
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (q.unit_cells(mid) <= rem) lo = mid; else hi = mid;
+            }
+            u = lo;
+            tile0 = (int)max((int64_t)0, rem - q.unit_cells(u) - kUnitCost);
+            run();
+        }
+    }
+    // To the next run; false at the share's end.
+    __device__ __forceinline__ bool next() {
+        if constexpr (kKeys) {
+            if (++u < q.units) {
+                unit_run();
+                return true;
+            }
+            j0 = j1;
+            if (j0 == q.tiles) {
+                j0 = 0;
+                if (!next_head()) return false;
+            }
+            piece();
+            return count > 0;
+        } else {
+            tile0 = 0;
+            if (++u == q.units) {
+                u = 0;
+                if (!next_head()) return false;
+            }
+            run();
+            return count > 0;
+        }
+    }
+
+private:
+    __device__ __forceinline__ bool next_head() {
+        if (++h < p.c.kv_heads) return true;
+        h = 0;
+        base += q.cells<kKeys>() * p.c.kv_heads;
+        do {
+            if (++b >= p.batch || base >= end) {
+                count = 0;
+                return false;
+            }
+            q = Seq(p, b);
+        } while (q.units == 0);
+        return true;
+    }
+    __device__ __forceinline__ void run() {  // rows: unit u from tile0 on
+        cell = base + h * q.cells<kKeys>() + q.unit_cells(u) + kUnitCost + tile0;
+        count = (int)max((int64_t)0, min((int64_t)(q.unit_tiles(u) - tile0), end - cell));
+    }
+    __device__ __forceinline__ void piece() {  // keys: tiles from j0 on that begin within the share
+        const int64_t from = base + h * q.cells<kKeys>();
+        int lo = j0, hi = q.tiles;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (from + q.tile_cells(mid) >= end) hi = mid; else lo = mid + 1;
+        }
+        j1 = lo;
+        count = 0;
+        if (j1 <= j0) return;
+        u = q.first_unit(j0);
+        unit_run();
+    }
+    __device__ __forceinline__ void unit_run() {
+        tile0 = j0;
+        count = min(j1, q.unit_tiles(u)) - j0;
+    }
+};
+
+struct alignas(16) Shared {
+    uint64_t raw_full[kRaw], raw_empty[kRaw], conv_full[kConv], conv_empty[kConv];
+    uint64_t q_full, q_empty, s_full[2], s_empty[2];
+    uint64_t drain;  // products in flight when the issuer gives up
+    float scales[kScaleSlots][8];
+    float4 columns[2][kRows / 2];  // keys: factors and -log2 of two columns, of a run and the next
+    float half[2][kTile];          // keys: the second half of the columns' sums
+    long long warp_sum[kThreads / 32];
+    long long start_base;
+    int start_b;
+    uint32_t tmem;
+    int last;
+};
+
+// Rotation and split of a unit's queries, and the row's factors.  Lane = (query, 16 pairs).
+struct PrepArgs {
+    PagedCall p;
+    RopeSteps rope;
+    const int32_t* known;
+    uint8_t* queries;
+    float* factor;
+    uint32_t* arrivals;
+};
+
+__device__ __forceinline__ uint32_t bf16_magnitudes(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
+
+// A sequence without rows before these is a new one: nothing was evicted from it.
+__device__ __forceinline__ int known_of(const int32_t* known, int b, const Seq& q) { return known ? known[b] : q.pos0; }
+
+__global__ void __launch_bounds__(kSumThreads) weigh_queries_kernel(const __grid_constant__ PrepArgs a) {
+    const PagedCall& p = a.p;
+    const int id = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, token = tid >> 2, q4 = tid & 3;
+    __shared__ uint64_t step[kPairs];
+    if (tid < kPairs) step[tid] = a.rope.step[tid];
+    dependency_wait();
+    allow_dependents();
+    // The last sequence whose first unit has this number or a lower one.
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (Seq(p, mid).id0 <= id) lo = mid; else hi = mid;
+    }
+    const Seq q(p, lo);
+    const int u = id - q.id0;
+    if (u < 0 || u >= q.units) return;
+    const int64_t cell = (int64_t)id * p.c.kv_heads + h;
+    if (tid == 0) a.arrivals[cell] = 0;
+    __syncthreads();
+    const int n = min(kTokens, q.n - u * kTokens);
+    if (token >= ((n + 7) & ~7)) return;  // whole steps of 32 rows are read
+    const bool real = token < n;
+    const int64_t pos = (int64_t)q.pos0 + u * kTokens + token +
+                        (known_of(a.known, lo, q) > 0 ? paged_evicted(p, lo) : 0);
+    const float unit = p.cap > 0.f ? p.scale / p.cap : p.scale * 1.4426950408889634f;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(q.row0 + u * kTokens + token) * p.q_row_stride +
+                                                      h * kGroup * p.q_head_stride + 16 * q4);
+    float2 f[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        f[i] = p.q_rotated ? make_float2(1.f, 0.f) : rope_factor(step[16 * q4 + i], pos);
+    uint8_t* out = a.queries + cell * kQBytes;
+#pragma unroll 1
+    for (int hq = 0; hq < kGroup; ++hq) {
+        uint4 w[4];  // pairs 0-7 and 8-15: first, then second elements
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = real ? src[hq * (p.q_head_stride / 8) + (i & 1) + 8 * (i >> 1)] : none;
+        // A power of two above the row's largest: a rotated pair passes it by no more than sqrt(2).
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            top = max(top, max(max(bf16_magnitudes(w[i].x), bf16_magnitudes(w[i].y)),
+                               max(bf16_magnitudes(w[i].z), bf16_magnitudes(w[i].w))));
+        const unsigned quad = 0xfu << (tid & 28);
+        top = max(top, __shfl_xor_sync(quad, top, 1));
+        top = max(top, __shfl_xor_sync(quad, top, 2));
+        const int e = min(253, max(1, (int)(top >> 23) + 1));
+        const float down = __int_as_float((254 - e) << 23);
+        const int row = token * kGroup + hq;
+        if (q4 == 0)
+            a.factor[cell * kRows + row] =
+                !real ? 0.f : top < 0x7f800000u ? unit * __int_as_float(e << 23) : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // 8 pairs: 16 bytes of each block of 64 dims, and of each part
+            const uint4 u4 = w[c], v4 = w[c + 2];
+            const uint32_t uw[4] = {u4.x, u4.y, u4.z, u4.w}, vw[4] = {v4.x, v4.y, v4.z, v4.w};
+            uint32_t xh[4], xl[4], yh[4], yl[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 s = bf16x2_to_float2(uw[i]), t = bf16x2_to_float2(vw[i]);
+                const float2 f0 = f[8 * c + 2 * i], f1 = f[8 * c + 2 * i + 1];
+                const float x0 = (s.x * f0.x - t.x * f0.y) * down, x1 = (s.y * f1.x - t.y * f1.y) * down;
+                const float y0 = (s.x * f0.y + t.x * f0.x) * down, y1 = (s.y * f1.y + t.y * f1.x) * down;
+                const float hx0 = __half2float(__float2half_rn(x0)), hx1 = __half2float(__float2half_rn(x1));
+                const float hy0 = __half2float(__float2half_rn(y0)), hy1 = __half2float(__float2half_rn(y1));
+                xh[i] = pack_half2(hx0, hx1);
+                xl[i] = pack_half2(x0 - hx0, x1 - hx1);
+                yh[i] = pack_half2(hy0, hy1);
+                yl[i] = pack_half2(y0 - hy0, y1 - hy1);
+            }
+            uint8_t* to = out + row * 128 + (((2 * q4 + c) ^ (row & 7)) << 4);
+            *reinterpret_cast<uint4*>(to) = make_uint4(xh[0], xh[1], xh[2], xh[3]);
+            *reinterpret_cast<uint4*>(to + kQBlockBytes) = make_uint4(yh[0], yh[1], yh[2], yh[3]);
+            *reinterpret_cast<uint4*>(to + 2 * kQBlockBytes) = make_uint4(xl[0], xl[1], xl[2], xl[3]);
+            *reinterpret_cast<uint4*>(to + 3 * kQBlockBytes) = make_uint4(yl[0], yl[1], yl[2], yl[3]);
+        }
+    }
+}
+
+__device__ __forceinline__ void sums_sync() { named_barrier_sync(1, kSumThreads); }
+
+// Rows of a unit as the MMA takes them: whole steps of 32 columns.
+__device__ __forceinline__ int columns_of(int n) { return (n * kGroup + 31) & ~31; }
+
+// A copy that stays in L2 as others do: the unit's tiles are dealt to several CTAs.
+__device__ __forceinline__ void bulk_load_queries(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)),
+        "l"(src), "r"(bytes), "r"(smem_addr(bar))
+        : "memory");
+}
+
+template <int kCode, bool kCap, bool kKeys>
+__global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constant__ WeighArgs a) {
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    uint8_t* q_smem = smem;
+    uint8_t* conv = q_smem + kQBytes;
+    uint8_t* raw = conv + kConv * kTileBytes;
+    Shared& s = *reinterpret_cast<Shared*>(raw + kRaw * kRawBytes);
+    const PagedCall& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = p.c.kv_heads;
+
+    if (tid == 0) {
+        for (int i = 0; i < kRaw; ++i) {
+            mbar_init(&s.raw_full[i], 1);
+            mbar_init(&s.raw_empty[i], 4);
+        }
+        for (int i = 0; i < kConv; ++i) {
+            mbar_init(&s.conv_full[i], 8);
+            mbar_init(&s.conv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.s_full[i], 1);
+            mbar_init(&s.s_empty[i], kSumThreads / 32);
+        }
+        mbar_init(&s.q_full, 1);
+        mbar_init(&s.q_empty, 1);
+        mbar_init(&s.drain, 1);
+        fence_barrier_init();
+        prefetch_tensormap(&a.kmap);
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s.tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    dependency_wait();
+    allow_dependents();
+    // Cells of all sequences, and the one that this share begins in.
+    int64_t total, from, to;
+    int64_t shares;
+    {
+        const int per = (p.batch + kThreads - 1) / kThreads;
+        const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+        long long sum = 0;
+        for (int b = b0; b < b1; ++b) sum += Seq(p, b).cells<kKeys>() * heads;
+        long long incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += x;
+        }
+        if (lane == 31) s.warp_sum[warp] = incl;
+        __syncthreads();
+        long long at = incl - sum;
+        total = 0;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) at += s.warp_sum[w];
+            total += s.warp_sum[w];
+        }
+        shares = max((int64_t)1, min((int64_t)gridDim.x, total / (kUnitCost + 1)));
+        const int64_t me = blockIdx.x;
+        from = me < shares ? total * me / shares : total;
+        to = me < shares ? total * (me + 1) / shares : total;
+        if (from < to && at <= from && from < at + sum)
+            for (int b = b0; b < b1; ++b) {
+                const int64_t each = Seq(p, b).cells<kKeys>() * heads;
+                if (from < at + each) {
+                    s.start_b = b;
+                    s.start_base = at;
+                    break;
+                }
+                at += each;
+            }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s.tmem;
+    Walk<kKeys> walk(p);
+    walk.start(s.start_b, s.start_base, from, to);
+    bool ok = true;
+
+    if (warp < kConvWarp) {
+        // ============================ sums ============================
+        const int g = warp >> 2, r = tid & (kTile - 1);
+        const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const float cap2 = p.cap * 1.4426950408889634f;
+        int buf = 0, phase = 0, slot = 0, runs = 0;
+        auto wait_tile = [&] {
+            if (ok) ok = warp_wait(&s.s_full[buf], phase);
+            tc_fence_after();
+        };
+        auto free_tile = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+            slot = (slot + 1) & (kScaleSlots - 1);
+            if (++buf == 2) {
+                buf = 0;
+                phase ^= 1;
+            }
+        };
+        if constexpr (!kKeys) {
+            while (walk.count > 0) {
+                const int n = walk.queries(), token = 32 * g + (r >> 2);
+                const bool active = n > 32 * g, real = token < n;
+                const int64_t cell = (int64_t)walk.id() * heads + walk.h;
+                const float factor = real ? a.factor[cell * kRows + g * kTile + r] : 0.f;
+                const int hi = real ? (int)min((int64_t)walk.pos() + token + 1, (int64_t)walk.q.len) : 0x7fffffff;
+                float ref = -INFINITY, l = 0.f;
+                for (int t = 0; t < walk.count; ++t) {
+                    wait_tile();
+                    if (active) {
+                        const int k0 = (walk.tile0 + t) << kTileShift;
+                        const bool edge = __any_sync(0xffffffffu, hi < k0 + kTile);
+                        const uint32_t cols = t_s + buf * 256 + g * kTile;
+                        float v[2][32];
+                        tmem_ld32(cols, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float(&z)[32] = v[c & 1];
+                            tmem_wait_ld();
+                            if (c < 3) tmem_ld32(cols + 32 * (c + 1), reinterpret_cast<uint32_t(&)[32]>(v[(c + 1) & 1]));
+                            const float f0 = factor * s.scales[slot][2 * c], f1 = factor * s.scales[slot][2 * c + 1];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float f = e < 16 ? f0 : f1;
+                                const float2 x = __fmul2_rn(make_float2(z[e], z[e + 1]), make_float2(f, f));
+                                z[e] = x.x;
+                                z[e + 1] = x.y;
+                            }
+                            if constexpr (kCap) cap_scores(z, cap2);
+                            if (edge) {
+                                const int left = hi - k0 - 32 * c;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (e >= left) z[e] = -INFINITY;
+                            }
+                            float mx = fmaxf(z[0], z[1]);
+#pragma unroll
+                            for (int e = 2; e < 32; e += 2) mx = fmaxf(fmaxf(mx, z[e]), z[e + 1]);
+                            if (mx > ref + kHeadroom) {  // (at once from nothing)
+                                l *= fast_exp2(ref - mx);
+                                ref = mx;
+                            }
+                            const float use = ref == -INFINITY ? 0.f : ref;
+                            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float2 x = __fadd2_rn(make_float2(z[e], z[e + 1]), make_float2(-use, -use));
+                                sum = __fadd2_rn(sum, make_float2(fast_exp2(x.x), fast_exp2(x.y)));
+                            }
+                            l += sum.x + sum.y;
+                        }
+                    }
+                    free_tile();
+                }
+                // ---- the run's rows ----
+                const int tiles = walk.q.unit_tiles(walk.u);
+                float* out = a.row_log2 + cell * kRows + g * kTile + r;
+                auto log2_of = [&](float m, float sum) { return !real ? INFINITY : sum == 0.f ? -INFINITY : m + log2f(sum); };
+                if (walk.count == tiles) {
+                    if (active) *out = log2_of(ref, l);
+                } else {
+                    // A piece of a unit.  A share's first piece goes to its slot 0; its last, if another one, to slot
+                    // 1: only the unit's first share can have begun before it.
+                    const int64_t first = walk.cell - walk.tile0;  // the cell of the unit's first tile
+                    auto share_of = [&](int64_t x) { return (int)(((x + 1) * shares + total - 1) / total) - 1; };
+                    const int c0 = share_of(first), parts = share_of(first + tiles - 1) - c0 + 1;
+                    const int second = total * c0 / shares < first - kUnitCost ? 1 : 0;
+                    auto part = [&](int c) {
+                        return a.partials + (int64_t)((c0 + c) * 2 + (c ? 0 : second)) * kRows + g * kTile + r;
+                    };
+                    if (active) *part((int)blockIdx.x - c0) = make_float2(ref, l);
+                    sums_sync();
+                    if (tid == 0) {
+                        uint32_t before;
+                        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                                     : "=r"(before)
+                                     : "l"(a.arrivals + cell)
+                                     : "memory");
+                        s.last = before == (uint32_t)(parts - 1);
+                    }
+                    sums_sync();
+                    if (s.last && active) {
+                        float M = -INFINITY, L = 0.f;
+                        for (int c = 0; c < parts; ++c) {
+                            const float2 x = __ldcg(part(c));
+                            const float now = fmaxf(M, x.x), use = now == -INFINITY ? 0.f : now;
+                            L = L * fast_exp2(M - use) + x.y * fast_exp2(x.x - use);
+                            M = now;
+                        }
+                        *out = log2_of(M, L);
+                    }
+                    sums_sync();  // s.last is read
+                }
+                if (!walk.next()) break;
+            }
+        } else {
+            int tiles = 0;
+            while (walk.count > 0) {
+                const int n = walk.queries(), columns = columns_of(n), half = columns >> 1;
+                const int64_t cell = (int64_t)walk.id() * heads + walk.h;
+                {
+                    float* to = reinterpret_cast<float*>(s.columns[runs & 1]) + (tid >> 1) * 4 + (tid & 1);
+                    if (tid < columns) {
+                        to[0] = a.factor[cell * kRows + tid];
+                        to[2] = -a.row_log2[cell * kRows + tid];
+                    }
+                    sums_sync();
+                }
+                const float4* column = s.columns[runs & 1] + g * (half >> 1);
+                ++runs;
+                const int known = known_of(a.known, walk.b, walk.q);
+                const int evicted = known > 0 ? paged_evicted(p, walk.b) : 0;
+                const int64_t at = ((int64_t)walk.b * heads + walk.h) * a.w.capacity;
+                for (int t = 0; t < walk.count; ++t, ++tiles) {
+                    const int tile = walk.tile0 + t, key = (tile << kTileShift) + r;
+                    const bool fresh = walk.u == walk.q.first_unit(tile), held = g == 0 && key < walk.q.len;
+                    float weight = 0.f;
+                    if (held && (!fresh || key < known)) weight = a.w.weight[at + key];
+                    wait_tile();
+                    // Rows that see the key: from this column on.
+                    const int from_col = (key - walk.pos()) * kGroup - g * half;
+                    const bool edge = __any_sync(0xffffffffu, from_col > 0);
+                    const float ks = s.scales[slot][r >> 4];
+                    const uint32_t cols = t_s + buf * 256 + g * half;
+                    float2 sum = make_float2(0.f, 0.f);
+                    auto add = [&](float (&v)[16], int c) {
+                        float2 off[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 k = column[8 * c + i];
+                            const float2 f = __fmul2_rn(make_float2(k.x, k.y), make_float2(ks, ks));
+                            off[i] = make_float2(k.z, k.w);
+                            float2 x = make_float2(v[2 * i], v[2 * i + 1]);
+                            x = kCap ? __fmul2_rn(x, f) : __ffma2_rn(x, f, off[i]);
+                            v[2 * i] = x.x;
+                            v[2 * i + 1] = x.y;
+                        }
+                        if constexpr (kCap) {
+                            cap_scores(v, cap2);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                v[2 * i] += off[i].x;
+                                v[2 * i + 1] += off[i].y;
+                            }
+                        }
+                        if (edge) {
+                            const int skip = from_col - 16 * c;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (i < skip) v[i] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2)
+                            sum = __fadd2_rn(sum, make_float2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
+                    };
+                    const int steps = half >> 4;
+                    float x[16], y[16];
+                    tmem_ld16(cols, reinterpret_cast<uint32_t(&)[16]>(x));
+                    for (int c = 0; c < steps; c += 2) {
+                        tmem_wait_ld();
+                        if (c + 1 < steps) tmem_ld16(cols + 16 * (c + 1), reinterpret_cast<uint32_t(&)[16]>(y));
+                        add(x, c);
+                        if (c + 1 < steps) {
+                            tmem_wait_ld();
+                            if (c + 2 < steps) tmem_ld16(cols + 16 * (c + 2), reinterpret_cast<uint32_t(&)[16]>(x));
+                            add(y, c + 1);
+                        }
+                    }
+                    free_tile();
+                    const float mine = sum.x + sum.y;
+                    if (g) s.half[tiles & 1][r] = mine;
+                    sums_sync();
+                    if (held) {
+                        a.w.weight[at + key] = weight + (mine + s.half[tiles & 1][r]);
+                        if (fresh && key >= known) a.w.position[at + key] = key + evicted;
+                        if (fresh && key == 0 && known <= 0 && walk.h == 0) a.w.evicted[walk.b] = 0;
+                    }
+                }
+                if (!walk.next()) break;
+            }
+        }
+    } else if (warp < kMmaWarp) {
+        // ============================ conversion ============================
+        const int cw = warp - kConvWarp, t = lane & 3;
+        // As in the chunked attention kernel: eight lanes that access shared memory together have all eight 16-byte
+        // columns of the codes' rows and of the operand's.
+        const int row0 = 16 * cw + ((lane >> 3) ^ (lane & 4 ? 5 : 0));
+        int rs = 0, rphase = 0, cs = 0, cphase = 0, items = 0;
+        while (walk.count > 0 && ok) {
+            for (int j = 0; j < walk.count && ok; ++j, ++items) {
+                uint8_t* dst = conv + cs * kTileBytes;
+                for (int part = 0; part < 2; ++part) {
+                    ok = mbar_wait(&s.raw_full[rs], rphase) &&
+                         (part || items < kConv || mbar_wait(&s.conv_empty[cs], cphase ^ 1));
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint8_t* src = raw + rs * kRawBytes;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = row0 + 8 * i, sw = row & 7, to = row + kHalfKeys * part;
+#pragma unroll
+                        for (int block = 0; block < 2; ++block) {
+                            const uint4 x = lds128(src + row * kHeadDim + (((4 * block + t) ^ sw) << 4));
+                            uint32_t w[8];
+                            to_half4<kCode>(x.x, w[0], w[1]);
+                            to_half4<kCode>(x.y, w[2], w[3]);
+                            to_half4<kCode>(x.z, w[4], w[5]);
+                            to_half4<kCode>(x.w, w[6], w[7]);
+                            uint8_t* at = dst + block * kBlockBytes + to * 128;
+                            *reinterpret_cast<uint4*>(at + (((2 * t) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(at + (((2 * t + 1) ^ sw) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&s.conv_full[cs]);
+                        mbar_arrive(&s.raw_empty[rs]);
+                    }
+                    if (++rs == kRaw) {
+                        rs = 0;
+                        rphase ^= 1;
+                    }
+                }
+                if (++cs == kConv) {
+                    cs = 0;
+                    cphase ^= 1;
+                }
+            }
+            if (!ok || !walk.next()) break;
+        }
+    } else if (warp == kMmaWarp) {
+        // ============================ MMA issuer ============================
+        const uint32_t leader = elect_lane(), cols = uniform(tmem);
+        int cs = 0, cphase = 0, buf = 0, phase = 0, items = 0, runs = 0;
+        while (uniform(walk.count) > 0 && ok) {
+            const int n = uniform(walk.queries()), count = uniform(walk.count);
+            ok = warp_wait(&s.q_full, runs & 1);
+            ++runs;
+            for (int j = 0; j < count && ok; ++j, ++items) {
+                ok = warp_wait(&s.conv_full[cs], cphase) && (items < 2 || warp_wait(&s.s_empty[buf], phase ^ 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t kd = smem_desc_sw128(smem_addr(conv + cs * kTileBytes), 16, 1024);
+                const uint64_t qd = smem_desc_sw128(smem_addr(q_smem), 16, 1024);
+                const int products = kKeys || n <= 32 ? 1 : 2;
+                const uint32_t idesc = idesc_n(kKeys ? columns_of(n) : kTile);
+                for (int m = 0; m < products; ++m)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint64_t k = kd + (((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4);
+                            const uint64_t q = qd + (((2 * part + (kk >> 2)) * kQBlockBytes + m * kTile * 128 + (kk & 3) * 32) >> 4);
+                            mma_ss_by(leader, cols + buf * 256 + m * kTile, kKeys ? k : q, kKeys ? q : k, idesc,
+                                      part || kk ? 1u : 0u);
+                        }
+                tc_commit_by(leader, &s.s_full[buf]);
+                tc_commit_by(leader, &s.conv_empty[cs]);
+                if (j + 1 == count) tc_commit_by(leader, &s.q_empty);
+                if (++cs == kConv) {
+                    cs = 0;
+                    cphase ^= 1;
+                }
+                if (++buf == 2) {
+                    buf = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok || !uniform(walk.next())) break;
+        }
+        if (!ok) {  // shared memory and TMEM are given back with no product under way
+            tc_commit_by(leader, &s.drain);
+            warp_wait(&s.drain, 0);
+        }
+    } else if (warp == kLoadWarp) {
+        // ============================ codes ============================
+        const int shift = p.c.page_shift, per_tile = kTile >> shift;  // pages of a tile
+        const int box = min(p.c.page_len, kHalfKeys), box_bytes = box * kHeadDim;
+        const uint64_t policy = l2_evict_first_policy();
+        int rs = 0, rphase = 0, items = 0, slot = 0;
+        while (walk.count > 0 && ok) {
+            const int32_t* table = p.block_table + walk.b * p.table_stride;
+            const int64_t hi = walk.q.len;
+            // Lane's page of tile j of the run (-1: past the sequence's keys, not loaded).
+            auto entry = [&](int j) {
+                const int64_t key = ((int64_t)(walk.tile0 + j) << kTileShift) + ((int64_t)lane << shift);
+                if (lane >= per_tile || j >= walk.count || key >= hi) return -1;
+                const int page = table[key >> shift];
+                return page >= 0 && page < p.c.pages ? page : p.c.pages;  // out of the map: TMA fills zeros
+            };
+            auto scale = [&](int page) {
+                return page >= 0 && page < p.c.pages ? p.c.k_scale[page * p.c.scale_page_stride + walk.h] : 0.f;
+            };
+            int page = entry(0), page1 = entry(1);
+            float ks = scale(page);
+            for (int j = 0; j < walk.count && ok; ++j) {
+                const int page2 = entry(j + 2);
+                const float ks1 = scale(page1);
+                for (int part = 0; part < 2; ++part, ++items) {
+                    if (items >= kRaw) ok = __all_sync(0xffffffffu, mbar_wait(&s.raw_empty[rs], rphase ^ 1));
+                    if (!ok) break;
+                    if (part == 0) {
+                        const float x = __shfl_sync(0xffffffffu, ks, (lane & 7) >> (shift - 4));  // a lane 16 keys
+                        if (lane < 8) s.scales[slot][lane] = x;
+                        __syncwarp();
+                        slot = (slot + 1) & (kScaleSlots - 1);
+                    }
+                    // This half's pages: a page of 128 keys has a box in each.
+                    const bool mine = page >= 0 && (shift == kTileShift || (lane << shift) / kHalfKeys == part) &&
+                                      ((int64_t)(walk.tile0 + j) << kTileShift) + part * kHalfKeys < hi;
+                    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
+                    if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[rs], boxes * box_bytes);
+                    __syncwarp();
+                    if (mine)
+                        tma_load_page(raw + rs * kRawBytes + (shift == kTileShift ? 0 : (lane << shift) % kHalfKeys) * kHeadDim,
+                                      &a.kmap, shift == kTileShift ? part * kHalfKeys : 0, walk.h, page, &s.raw_full[rs],
+                                      policy);
+                    if (++rs == kRaw) {
+                        rs = 0;
+                        rphase ^= 1;
+                    }
+                }
+                page = page1;
+                page1 = page2;
+                ks = ks1;
+            }
+            if (!ok || !walk.next()) break;
+        }
+        if (!ok)  // do not leave while copies into this CTA's shared memory are in flight
+            for (int i = 1; i <= kRaw && i <= items; ++i) {
+                const int at = rs - i;
+                mbar_wait(&s.raw_full[at < 0 ? at + kRaw : at], at < 0 ? rphase ^ 1 : rphase);
+            }
+    } else if (warp == kQueryWarp) {
+        // ============================ queries ============================
+        int runs = 0;
+        while (walk.count > 0) {
+            if (runs > 0 && !warp_wait(&s.q_empty, (runs - 1) & 1)) {
+                ok = false;  // (the last copies have landed: their products were waited for)
+                break;
+            }
+            const uint32_t bytes = (walk.queries() > 32 ? kRows : kTile) * 128;
+            const uint8_t* src = a.queries + ((int64_t)walk.id() * heads + walk.h) * kQBytes;
+            if (lane == 0) mbar_arrive_expect_tx(&s.q_full, 4 * bytes);
+            __syncwarp();
+            if (lane < 4) bulk_load_queries(q_smem + lane * kQBlockBytes, src + lane * kQBlockBytes, bytes, &s.q_full);
+            ++runs;
+            if (!walk.next()) break;
+        }
+        if (runs > 0) warp_wait(&s.q_full, (runs - 1) & 1);  // no copy in flight when the CTA leaves
+    }
+    if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+}
+
+constexpr int kSmemBytes = 1024 + kQBytes + kConv * kTileBytes + kRaw * kRawBytes + (int)sizeof(Shared);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+
+using Kernel = void (*)(WeighArgs);
+
+template <bool kKeys>
+Kernel kernel_for(int code, bool cap) {
+    if (code == GQA_CODE_INT8) return cap ? weigh_kernel<0, true, kKeys> : weigh_kernel<0, false, kKeys>;
+    return cap ? weigh_kernel<1, true, kKeys> : weigh_kernel<1, false, kKeys>;
+}
+
+struct Regions {
+    size_t partials, arrivals, factor, row_log2, queries, end;
+};
+// Units: their numbers (Seq) are below this.
+int units_of(int batch, int rows) { return rows / kTokens + batch + 1; }
+Regions regions(int batch, int rows, int heads, int sms) {
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    const size_t units = (size_t)units_of(batch, rows) * heads;
+    Regions r;
+    r.partials = up(kPagedPartialsOffset);
+    r.arrivals = r.partials + up((size_t)sms * 2 * kRows * sizeof(float2));
+    r.factor = r.arrivals + up(units * sizeof(uint32_t));
+    r.row_log2 = r.factor + units * kRows * sizeof(float);
+    r.queries = r.row_log2 + units * kRows * sizeof(float);
+    r.end = r.queries + units * kQBytes;
+    return r;
+}
+
+}  // namespace
+
+int paged_weigh_box() { return kHalfKeys; }
+
+size_t paged_weigh_workspace(int batch, int rows, int heads, int sms) { return regions(batch, rows, heads, sms).end; }
+
+cudaError_t paged_weigh_prepare() {
+    for (int i = 0; i < 8; ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(i & 4 ? kernel_for<true>(i & 1, i & 2) : kernel_for<false>(i & 1, i & 2),
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+cudaError_t launch_score_weights(const PagedCall& call, const PagedScores& scores, const KeyWeightsView& weights, int sms,
+                                 cudaStream_t stream) {
+    const ScoreArgs a{call, scores, weights};
+    const int units = call.batch * call.c.kv_heads;
+    const int64_t most = (scores.keys + kScoreThreads * kScoreKeys - 1) / (kScoreThreads * kScoreKeys);
+    const int64_t want = ((int64_t)sms * 16 + units - 1) / units;
+    return launch_dependent(score_weights_kernel, dim3(units, (unsigned)(want < most ? want : most)), kScoreThreads, 0,
+                            stream, a);
+}
+
+cudaError_t launch_paged_weigh(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
+                               const KeyWeightsView& weights, const int32_t* known, int sms, uint8_t* ws,
+                               cudaStream_t stream) {
+    const Regions r = regions(call.batch, call.rows, call.c.kv_heads, sms);
+    WeighArgs a;
+    a.kmap = kmap;
+    a.p = call;
+    a.rope = rope;
+    a.w = weights;
+    a.known = known;
+    a.status = reinterpret_cast<uint32_t*>(ws);
+    a.queries = ws + r.queries;
+    a.factor = reinterpret_cast<float*>(ws + r.factor);
+    a.row_log2 = reinterpret_cast<float*>(ws + r.row_log2);
+    a.arrivals = reinterpret_cast<uint32_t*>(ws + r.arrivals);
+    a.partials = reinterpret_cast<float2*>(ws + r.partials);
+    a.max_units = units_of(call.batch, call.rows);
+    const PrepArgs prep{call, rope, known, a.queries, a.factor, a.arrivals};
+    cudaError_t e = launch_dependent(weigh_queries_kernel, dim3(a.max_units, call.c.kv_heads), kSumThreads, 0, stream, prep);
+    if (e == cudaSuccess)
+        e = launch_dependent(kernel_for<false>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes, stream, a);
+    if (e == cudaSuccess)
+        e = launch_dependent(kernel_for<true>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes, stream, a);
+    return e;
+}
+
+}  // namespace gqa

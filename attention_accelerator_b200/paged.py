@@ -241,7 +241,9 @@ def read_paged(cache: PagedCache, slots: torch.Tensor) -> tuple[torch.Tensor, to
 
 
 def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_positions, scale, rope_theta, q_rotated,
-            score_cap, distance_slopes, doc_starts, prefix_ends, out):
+            score_cap, distance_slopes, doc_starts, prefix_ends, out, out_heads=None, extra=(), entry=None, sizes=None):
+    """An attention call.  ``out_heads``: its output heads (default: the Q heads; 0: it has no output); ``entry``: its
+    entry point, which takes the C arguments ``extra`` behind the call's own; ``sizes``: that of its workspace."""
     lib = _lib.load()
     device = q.device
     if device.type != "cuda":
@@ -258,10 +260,12 @@ def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_posit
     _table(block_table, batch, device)
     if score_cap is not None and not (score_cap > 0.0 and math.isfinite(score_cap)):
         raise ValueError("score_cap must be positive and finite, or None")
+    if out_heads is None:
+        out_heads = heads
     if out is None:
-        out = q.new_empty((rows, heads, HEAD_DIM))
+        out = q.new_empty((rows, out_heads, HEAD_DIM)) if out_heads else q
     else:
-        _check_out(out, (rows, heads, HEAD_DIM), torch.bfloat16, device)
+        _check_out(out, (rows, out_heads, HEAD_DIM), torch.bfloat16, device)
     i32 = torch.int32
     p = GqaPagedParams(
         batch=batch, rows=rows, block_table=block_table.data_ptr(), table_stride=block_table.stride(0),
@@ -278,16 +282,17 @@ def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_posit
     if rows == 0:
         return out
     stream = _stream_ptr(device)
-    fn = lib.gqa_decode_paged if first_query is None else lib.gqa_decode_paged_chunked
+    fn = entry or (lib.gqa_decode_paged if first_query is None else lib.gqa_decode_paged_chunked)
     c = ctypes.byref(cache.c)
+    tensors = (q.data_ptr(), out.data_ptr()) if out_heads else (q.data_ptr(),)
     ws = _paged_workspace(device, stream, _lib.CHUNKED_WORKSPACE_BYTES)
-    status = fn(q.data_ptr(), out.data_ptr(), c, ctypes.byref(p), ws.data_ptr(), ws.numel(), stream)
+    status = fn(*tensors, c, ctypes.byref(p), *extra, ws.data_ptr(), ws.numel(), stream)
     if status == _lib.GQA_ERR_WORKSPACE:  # nothing was launched: the stream's first call, or a larger one
-        nbytes = lib.gqa_paged_workspace_bytes(c, ctypes.byref(p))
+        nbytes = (sizes or lib.gqa_paged_workspace_bytes)(c, ctypes.byref(p))
         if nbytes == 0:
             raise GqaError(_lib.GQA_ERR_CUDA, f"{name}: workspace sizing failed (no supported GPU?)")
         ws = _paged_workspace(device, stream, nbytes)
-        status = fn(q.data_ptr(), out.data_ptr(), c, ctypes.byref(p), ws.data_ptr(), ws.numel(), stream)
+        status = fn(*tensors, c, ctypes.byref(p), *extra, ws.data_ptr(), ws.numel(), stream)
     _check(status, name)
     return out
 
@@ -323,3 +328,58 @@ def decode_paged_chunked(q: torch.Tensor, cache: PagedCache, block_table: torch.
     :func:`decode_paged`.  Rows at or past ``first_query[batch]`` are not written."""
     return _attend("decode_paged_chunked", q, cache, block_table, seq_lens, first_query, None, scale, rope_theta,
                    q_rotated, score_cap, distance_slopes, doc_starts, prefix_ends, out)
+
+
+def _attend_diff(name: str, q, cache, block_table, seq_lens, first_query, lambdas, norm_weight, norm_eps, out_scale, **call):
+    lib = _lib.load()
+    heads, device = cache.kv_heads * GROUP_SIZE // 2, q.device
+    rows = q.shape[0] if q.dim() else 0
+    f32 = torch.float32
+    if lambdas.dtype is not f32 or lambdas.device != device or lambdas.shape not in ((heads,), (rows, heads)) \
+            or lambdas.stride(-1) != 1 and heads > 1 or lambdas.dim() == 2 and rows > 1 and lambdas.stride(0) < 0:
+        raise ValueError(f"lambdas must be float32 [{heads}] or [{rows}, {heads}] on {device} with a contiguous last dim")
+    gain = _need("norm_weight", norm_weight, f32, (HEAD_DIM,), device)
+    if not math.isfinite(out_scale):
+        raise ValueError("out_scale must be finite")
+    if gain is not None and not (norm_eps > 0.0 and math.isfinite(norm_eps)):
+        raise ValueError("norm_eps must be positive and finite")
+    d = _lib.GqaPagedDiff(lambdas=lambdas.data_ptr(), norm_weight=gain, norm_eps=norm_eps, out_scale=out_scale,
+                          lambda_row_stride=lambdas.stride(0) if lambdas.dim() == 2 and rows > 1 else 0)
+    return _attend(name, q, cache, block_table, seq_lens, first_query, out_heads=heads, extra=(ctypes.byref(d),),
+                   entry=lib.gqa_decode_paged_diff if first_query is None else lib.gqa_decode_paged_chunked_diff, **call)
+
+
+def decode_paged_diff(q: torch.Tensor, cache: PagedCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                      lambdas: torch.Tensor, *, norm_weight: torch.Tensor | None = None, norm_eps: float = 1e-5,
+                      out_scale: float = 1.0, query_positions: torch.Tensor | None = None, scale: float | None = None,
+                      rope_theta: float = ROPE_THETA, q_rotated: bool = False, score_cap: float | None = None,
+                      distance_slopes: torch.Tensor | None = None, doc_starts: torch.Tensor | None = None,
+                      prefix_ends: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Differential attention, one token a sequence: the difference of two softmax maps of one KV head.
+
+    Q heads ``2 j`` and ``2 j + 1`` are the maps of output head j, ``a_j = softmax(z_2j) V - lambda_j softmax(z_2j+1) V``
+    with the scores, masks and arguments of :func:`decode_paged`; returns BF16 ``[batch, 2 * heads, 128]``.
+    ``lambdas``: float32 ``[2 * heads]``, or ``[batch, 2 * heads]`` where they come from the tokens.  With
+    ``norm_weight`` (float32 ``[128]``) each head's row is divided by its root mean square,
+    ``a / sqrt(mean(a^2) + norm_eps) * norm_weight``; ``out_scale`` multiplies the row (``1 - lambda_init`` in a
+    differential transformer's layer).  A row that sees no key is 0.
+    """
+    return _attend_diff("decode_paged_diff", q, cache, block_table, seq_lens, None, lambdas, norm_weight, norm_eps,
+                        out_scale, query_positions=query_positions, scale=scale, rope_theta=rope_theta,
+                        q_rotated=q_rotated, score_cap=score_cap, distance_slopes=distance_slopes,
+                        doc_starts=doc_starts, prefix_ends=prefix_ends, out=out)
+
+
+def decode_paged_diff_chunked(q: torch.Tensor, cache: PagedCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                              first_query: torch.Tensor, lambdas: torch.Tensor, *,
+                              norm_weight: torch.Tensor | None = None, norm_eps: float = 1e-5, out_scale: float = 1.0,
+                              scale: float | None = None, rope_theta: float = ROPE_THETA, q_rotated: bool = False,
+                              score_cap: float | None = None, distance_slopes: torch.Tensor | None = None,
+                              doc_starts: torch.Tensor | None = None, prefix_ends: torch.Tensor | None = None,
+                              out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`decode_paged_diff` of any number of queries a sequence, packed as for :func:`decode_paged_chunked`;
+    ``lambdas`` float32 ``[2 * heads]`` or ``[rows, 2 * heads]``.  Returns BF16 ``[rows, 2 * heads, 128]``."""
+    return _attend_diff("decode_paged_diff_chunked", q, cache, block_table, seq_lens, first_query, lambdas, norm_weight,
+                        norm_eps, out_scale, query_positions=None, scale=scale, rope_theta=rope_theta,
+                        q_rotated=q_rotated, score_cap=score_cap, distance_slopes=distance_slopes,
+                        doc_starts=doc_starts, prefix_ends=prefix_ends, out=out)

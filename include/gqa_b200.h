@@ -620,6 +620,121 @@ int gqa_decode_paged(const void *q, void *out, const gqa_paged_cache *cache, con
 int gqa_decode_paged_chunked(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
                              void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Differential attention over the paged cache: the difference of two softmax
+ * maps of one KV head.  Q heads 2 j and 2 j + 1 (j = 0 .. 2 * kv_heads - 1) of a
+ * query row i are the maps of output head j:
+ *   a_j = softmax(z(Q head 2 j)) V - lambda(i, j) * softmax(z(Q head 2 j + 1)) V
+ *   out_j = out_scale * a_j, or with norm_weight
+ *   out_j = out_scale * norm_weight * a_j / sqrt(mean(a_j^2) + norm_eps)   (mean over the 128 dims)
+ * with z and the visible keys as for gqa_decode_paged; a row that sees no key is
+ * 0.  `out` is BF16 [rows][2 * kv_heads][128], rounded once; both maps, their
+ * difference and the norm are FP32.  Workspace: gqa_paged_workspace_bytes.
+ * No reference counterpart.
+ * ------------------------------------------------------------------------- */
+typedef struct gqa_paged_diff {
+    const float *lambdas;       /* lambda(i, j) at lambdas[i * lambda_row_stride + j] */
+    int64_t lambda_row_stride;  /* floats; 0: the same for every row */
+    const float *norm_weight;   /* [128], 16-byte aligned, or NULL: no norm */
+    float   norm_eps;           /* positive and finite where there is a norm */
+    float   out_scale;          /* finite */
+} gqa_paged_diff;
+
+int gqa_decode_paged_diff(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
+                          const gqa_paged_diff *diff, void *workspace, size_t workspace_bytes, void *stream);
+int gqa_decode_paged_chunked_diff(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
+                                  const gqa_paged_diff *diff, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Eviction by accumulated attention weight.
+ *
+ * Beside the cache a program keeps, for every row (held key) of every request and
+ * KV head, the attention weight that its queries have given it so far and the
+ * position of its token.  When a request holds more rows than its budget, those of
+ * the least weight go: gqa_plan_eviction chooses, gqa_evict_paged moves.  K was
+ * rotated at its token's position when it was appended, so a row may move: the rows
+ * that stay but lie past the new length fill the holes below it.  Afterwards a row's
+ * number is no longer its position: query and append positions are row + evicted[r]
+ * (GQA_FLAG_Q_ROTATED, positions of gqa_append_paged), and distance bias, document
+ * and prefix masks no longer apply.  No reference counterpart.
+ * ------------------------------------------------------------------------- */
+typedef struct gqa_key_weights {
+    float   *weight;    /* [batch][kv_heads][capacity] */
+    int32_t *position;  /* [batch][kv_heads][capacity] */
+    int32_t *evicted;   /* [batch]: tokens evicted so far */
+    int64_t capacity;   /* rows: at least table_width * page_len, at most 2^30 */
+} gqa_key_weights;
+
+/* Device workspace of either call below (0 on invalid input), as gqa_paged_workspace_bytes's: it serves those
+ * calls as well.  One token a sequence: 16 bytes for each key that the table could name and KV head. */
+size_t gqa_key_weights_workspace_bytes(const gqa_paged_cache *cache, const gqa_paged_params *p);
+
+/*
+ * gqa_decode_paged that adds, for each row k < seq_lens[b] of sequence b and each KV
+ * head, the softmax weights that the 4 Q heads of its group give it:
+ *   weight[b][h][k] = (k is the last row ? 0 : weight[b][h][k]) + sum of 4 weights.
+ * The last row is the query's own token: position[b][h][seq_len - 1] = seq_len - 1 +
+ * evicted[b], where the query stands too (query_positions is NULL; a sequence of one
+ * row is a new one, its evicted[b] becomes 0).  doc_starts, prefix_ends and slopes
+ * are NULL.  FP32 throughout, no atomics: results do not depend on timing.
+ */
+int gqa_decode_paged_weights(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
+                             const gqa_key_weights *weights, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The same sums over any number of queries a sequence, packed as for
+ * gqa_decode_paged_chunked, without attention's output: a prompt's tokens, or the
+ * last of them.  Query i of n of sequence b has row seq_lens[b] - n + i, sees the rows
+ * up to it and stands at row + evicted[b].  Rows from known[b] on (NULL: from the
+ * first query's row on) are new: their weight starts at 0 and their position is row +
+ * evicted[b]; where known[b] is 0 or less the sequence is a new one, and evicted[b]
+ * becomes 0.  Sequences without queries are left as they are.  `out` strides of `p`
+ * are not used.
+ */
+int gqa_add_key_weights(const void *q, const gqa_paged_cache *cache, const gqa_paged_params *p,
+                        const gqa_key_weights *weights, const int32_t *known, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/*
+ * What stays of each request, on the GPU.  Request r with lens[r] rows and keep =
+ * min(keep[r], max_keep): where 0 < keep < lens[r], every KV head keeps its `keep`
+ * rows of the highest weight, first of those to be spared (position < sinks, or among
+ * the last `recent` of the lens[r] + evicted[r] tokens so far), then of the others;
+ * equal weights: the lower row.  (Weights are not negative: what is counts as 0, NaN as the
+ * highest.)  Other requests are left as they are.
+ *  - take[r][h][i], i < max_keep: the row that moves to row i, -1 where none does: the
+ *    rows that stay at or past `keep`, in order, to those below it that do not, in order.
+ *  - lens_out, evicted_out: rows held and tokens evicted after the step; may be lens and
+ *    weights->evicted themselves.
+ *  - pages past the new length are pushed on the stack free_pages (entries [0, *n_free)
+ *    valid, n_free_out may be n_free), in the order of requests, then columns; the block
+ *    table keeps its entries, which gqa_evict_paged reads: call it before any call that
+ *    pops pages.
+ *  - counts[4]: requests cut, rows evicted a head, pages given back, status.
+ * All or nothing: a negative length, one past the table's row or weights->capacity, or a
+ * stack that would pass free_capacity: counts[3] is GQA_ERR_PAGES and nothing changes (take is -1).
+ * Workspace: gqa_plan_eviction_workspace_bytes, used by no other call at the same time;
+ * its first 256 bytes zero at allocation.
+ */
+size_t gqa_plan_eviction_workspace_bytes(int requests, int kv_heads, int max_keep);
+int gqa_plan_eviction(const gqa_key_weights *weights, int kv_heads, const int32_t *lens, const int32_t *keep, int requests,
+                      const int32_t *block_table, int64_t table_stride, int table_width, int32_t *free_pages,
+                      int free_capacity, const int32_t *n_free, int page_len, int max_keep, int sinks, int recent,
+                      int32_t *take, int32_t *lens_out, int32_t *evicted_out, int32_t *n_free_out, int32_t *counts,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Move the rows that gqa_plan_eviction chose: K and V codes, weights and positions.
+ * lens: its lens_out.  For each block (page and head, of K and of V) that rows move into:
+ *   scale = max(old scale, amax of the rows that move in / Qmax, 2^-100)
+ *   code = RNE(c * its old scale / scale) of those rows; if the scale grew, of all others too.
+ * A block that gets a row of a NaN scale has one itself (and codes of 0).  The pages of a
+ * request whose rows move must be its own.
+ */
+int gqa_evict_paged(const gqa_paged_cache *cache, const int32_t *block_table, int64_t table_stride, int table_width,
+                    const gqa_key_weights *weights, const int32_t *lens, const int32_t *take, int requests, int max_keep,
+                    void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -79,3 +79,83 @@ def attend(q, k, v, m, seen, *, scale, cap=0.0, slopes=None):
         out[h], size[h] = w @ vh, w @ np.abs(vh)
         most = max(most, abs(scale) * (np.abs(kh) @ np.abs(q[h])).max())
     return out, size, most
+
+
+def attend_diff(q, k, v, m, seen, lambdas, *, norm_weight=None, eps=1e-5, out_scale=1.0, **scores):
+    """Differential attention of one query row: Q heads 2 j and 2 j + 1 are the maps of head j.  Returns the output
+    [heads / 2, 128], the bound of what errors of the two maps' products would be a unit of, and :func:`attend`'s terms."""
+    maps, size, most = attend(q, k, v, m, seen, **scores)
+    lam = np.asarray(lambdas, np.float64)[:, None]
+    out, size = maps[0::2] - lam * maps[1::2], size[0::2] + np.abs(lam) * size[1::2]
+    if norm_weight is not None:
+        rms = np.sqrt((out * out).mean(-1, keepdims=True) + eps)
+        w = np.abs(norm_weight)
+        # A change d of the row moves the result by d / rms, and by out / rms times that of the root mean square.
+        size = w * (size / rms + np.abs(out) / rms ** 2 * np.sqrt((size * size).mean(-1, keepdims=True)))
+        out = out / rms * norm_weight
+    return out_scale * out, abs(out_scale) * size, most
+
+
+def plan_eviction(weight, position, lens, evicted, keep, table, free, page_len, capacity, *, max_keep, sinks, recent):
+    """The choice of what stays, on arrays and Python lists (``free``, the stack, grows unless the step is refused).
+    Returns (ok, take, lens, evicted, requests cut, rows evicted, pages given back)."""
+    requests, heads, room = weight.shape
+    take = np.full((requests, heads, max_keep), -1, np.int64)
+    ceil = lambda n: -(-n // page_len)  # noqa: E731
+    after = [min(k, max_keep) if 0 < min(k, max_keep) < n else n for n, k in zip(lens, keep)]
+    given = [p for r in range(requests) for p in table[r][ceil(after[r]):ceil(max(0, lens[r]))]]
+    if any(n < 0 or ceil(n) > len(table[0]) or n > room for n in lens) or len(free) + len(given) > capacity:
+        return False, take, list(lens), list(evicted), 0, 0, 0
+    free.extend(given)
+    for r in range(requests):
+        n, k = lens[r], after[r]
+        if k == n:
+            continue
+        for h in range(heads):
+            def mark(i):
+                w = float(weight[r, h, i])
+                p = int(position[r, h, i])
+                spared = p < sinks or p >= n + max(evicted[r], 0) - recent
+                return (not spared, math.isfinite(w) or not math.isnan(w), -max(w, 0.0) if not math.isnan(w) else 0.0, i)
+            stays = set(sorted(range(n), key=mark)[:k])
+            holes = [i for i in range(k) if i not in stays]
+            fills = [i for i in range(k, n) if i in stays]
+            take[r, h, holes] = fills
+    gone = [n - k for n, k in zip(lens, after)]
+    return (True, take, after, [e + g for e, g in zip(evicted, gone)], sum(g > 0 for g in gone), sum(gone), len(given))
+
+
+def evict(codes, scale, take, lens, table, page_len, code):
+    """The move in one of K and V: ``codes`` [pages, heads, page_len, 128] (values in 64 bits) and ``scale`` [pages,
+    heads], changed in place."""
+    before, held = codes.copy(), scale.copy()
+    top = CODE_MAX[code]
+    requests, heads, max_keep = take.shape
+    for r in range(requests):
+        for column in range(-(-min(max_keep, lens[r]) // page_len)):
+            to = table[r][column]
+            for h in range(heads):
+                rows = [(i, take[r, h, column * page_len + i]) for i in range(page_len)
+                        if column * page_len + i < max_keep and take[r, h, column * page_len + i] >= 0]
+                if not rows:
+                    continue
+                moves = {i: (table[r][s // page_len], s % page_len) for i, s in rows}
+                values = {i: before[p, h, s] * np.float64(held[p, h]) for i, (p, s) in moves.items()}
+                most = max(np.abs(x).max() for x in values.values())
+                now = np.float64(np.float32(max(held[to, h], most / top, MIN_SCALE)))
+                if now > held[to, h]:
+                    codes[to, h] = round_code(before[to, h] * np.float64(held[to, h]) / now, code)
+                for i, x in values.items():
+                    codes[to, h, i] = round_code(x / now, code)
+                scale[to, h] = now
+
+
+def round_code(y, code):
+    """The nearest code's value; of two as near the even one."""
+    if code == "int8":
+        return np.clip(np.rint(y), -127, 127)
+    grid = np.unique(E4M3[np.isfinite(E4M3)])
+    at = np.clip(np.searchsorted(grid, y), 1, len(grid) - 1)
+    lo, hi = grid[at - 1], grid[at]
+    even = lambda x: (np.abs(x) / 2.0 ** np.maximum(np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -9))) - 3, -9)) % 2 == 0  # noqa: E731
+    return np.where(y - lo < hi - y, lo, np.where(y - lo > hi - y, hi, np.where(even(lo), lo, hi)))
