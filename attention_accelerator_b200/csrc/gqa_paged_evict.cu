@@ -253,6 +253,16 @@ struct EvictArgs {
     bool last_pages;
 };
 
+// A block's scale from the largest magnitude of what moves in (FP32 bits, and what rounding to them took):
+// their sum over qmax, rounded once, so that a row of the largest code and the block's own scale leaves it.
+__device__ __forceinline__ BlockScale moved_scale(uint32_t top, float rest, float qmax, float old) {
+    if (top >= 0x7f800000u) return BlockScale{__int_as_float(0x7fffffff), 0.f, false};
+    const float most = __uint_as_float(top), y = __fdiv_rn(most, qmax);
+    const float mine = fmaxf(__fmaf_rn(__fadd_rn(__fmaf_rn(-y, qmax, most), rest), 1.f / qmax, y), kMinBlockScale);
+    const float value = mine > old ? mine : old;
+    return BlockScale{value, value == value ? __frcp_rn(value) : 0.f, mine > old};
+}
+
 // c s / scale, rounded to FP32 but for the last half of a thousandth of a unit.  The scales of a block and of
 // what moves into it are often in the ratio of two codes, so that the quotient lies half way between two
 // others: products rounded one after the other would take either (outputs twice as far from the rounded
@@ -325,13 +335,17 @@ __global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ Evic
         const uint32_t x = e < 4 ? w.x : e < 8 ? w.y : e < 12 ? w.z : w.w;
         return code_value<kCode>((uint8_t)(x >> (8 * (e & 3))));
     };
-    float most = 0.f;
+    float most = 0.f, most_rest = 0.f;  // the largest magnitude, and what rounding it to FP32 took
     bool fine = true;
     auto measure = [&](const Row& x) {
         float m = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(code(x.w, e)));
-        most = fmaxf(most, __fmul_rn(m, x.scale));
+        const float v = __fmul_rn(m, x.scale);
+        if (v > most) {
+            most = v;
+            most_rest = __fmaf_rn(m, x.scale, -v);
+        }
         fine &= x.scale <= 3.402823466e38f;  // (a block of NaN scale)
     };
     Row held[kHeldRows];
@@ -345,7 +359,10 @@ __global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ Evic
         if (4 * i + sub < n) measure(held[i]);
     for (int i = 4 * kHeldRows + sub; i < n; i += 4) measure(load(i));
     const uint32_t top = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(most) : 0x7f800000u);
-    const BlockScale scale = block_scale(top, qmax, old);
+    if (__float_as_uint(most) != top) most_rest = -INFINITY;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) most_rest = fmaxf(most_rest, __shfl_xor_sync(0xffffffffu, most_rest, d));
+    const BlockScale scale = moved_scale(top, most_rest, qmax, old);
     const bool number = scale.value == scale.value;
     auto codes16 = [&](const uint4& w, float s) {
         uint32_t o[4];
