@@ -4,6 +4,8 @@
 #include "gqa_paged.cuh"
 #include "gqa_paged_internal.h"
 
+#include <algorithm>
+
 namespace gqa {
 
 namespace {
@@ -11,16 +13,18 @@ namespace {
 // ---------------------------------------------------------------------------
 // The choice.
 //
-// A CTA a (request, KV head).  A row's rank is that of a 32-bit number: the bits of its
-// weight, which order as the weights do (they are not negative), and above them whether
-// it is spared.  Three passes over histograms of 11, 11 and 10 bits, from the top, find
-// the number of the last row that stays and how many rows of that very number stay; one
-// more pass, in the order of rows, marks them, counts holes below `keep` and rows that
-// stay past it, and pairs them off.  One more CTA gives the pages back.
+// A cluster of 1 to 8 CTAs a (request, KV head), each with a stretch of its rows.  A
+// row's rank is that of a 32-bit number: the bits of its weight, which order as the
+// weights do (they are not negative), and above them whether it is spared; the
+// numbers are computed once and kept in shared memory.  Three passes over histograms
+// of 11, 11 and 10 bits, from the top, find the number of the last row that stays and
+// how many rows of that very number stay.  Two more count, a warp a stretch of rows,
+// what is equal to it and then the holes below `keep` and the rows past it that stay;
+// the last lists both in order, and they are paired off.  One more CTA gives the pages
+// back.
 // ---------------------------------------------------------------------------
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kEach = 4;  // rows of a thread at a time
-constexpr int kBins = 2048;
+constexpr int kBins = 2048, kMaxCluster = 8;
+constexpr int kMaxRows = 48 * 1024;  // of a CTA in shared memory; numbers of rows past that are computed again
 
 struct EvictPlanArgs {
     KeyWeightsView w;
@@ -33,6 +37,8 @@ struct EvictPlanArgs {
     uint32_t* ticket;
     int32_t* lists;  // [requests * heads][2][max_keep]: holes and rows that fill them
     int requests, heads, table_width, free_capacity, page_shift, max_keep, sinks, recent;
+    int held_rows;   // of a CTA in shared memory
+    bool vectors;    // weights and positions of a head are 16-byte aligned
 };
 
 struct Cut {
@@ -43,161 +49,287 @@ __device__ __forceinline__ Cut cut_of(const EvictPlanArgs& a, int r) {
     return Cut{len, keep > 0 && keep < len ? keep : len};
 }
 
-// The sum over the CTA of values a thread, and of those before it.
-struct Sum {
-    int before, all;
-};
-__device__ __forceinline__ Sum block_sum(int v, int* warp_sum) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int incl = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += x;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sum[warp] = incl;
-    __syncthreads();
-    Sum s{incl - v, 0};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const int x = warp_sum[w];
-        s.all += x;
-        if (w < warp) s.before += x;
-    }
-    return s;
-}
-
 __device__ __forceinline__ uint32_t rank_of(const EvictPlanArgs& a, float weight, int position, int64_t recent_from) {
     const uint32_t bits = __float_as_uint(weight);
     const uint32_t w = weight != weight ? 0x7fffffffu : bits & 0x80000000u ? 0u : bits;
     return w | (position < a.sinks || position >= recent_from ? 0x80000000u : 0u);
 }
 
-__device__ void choose(const EvictPlanArgs& a, int r, int h, const Cut& cut, int* hist, int* warp_sum) {
-    __shared__ uint32_t s_bin, s_left;
-    const int tid = threadIdx.x;
-    const int64_t unit = (int64_t)r * a.heads + h;
-    const float* weight = a.w.weight + unit * a.w.capacity;
-    const int32_t* position = a.w.position + unit * a.w.capacity;
-    const int64_t recent_from = (int64_t)cut.len + min(max(a.w.evicted[r], 0), 1 << 30) - a.recent;
-    const int len = cut.len, keep = cut.keep;
-    auto number = [&](int i) { return rank_of(a, weight[i], position[i], recent_from); };
+// The sum over a warp, and of the lanes before.
+__device__ __forceinline__ int warp_before(int v) {
+    const int lane = threadIdx.x & 31;
+    int incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += x;
+    }
+    return incl - v;
+}
 
-    uint32_t found = 0, known = 0;  // the number's upper bits, and which these are
-    uint32_t left = (uint32_t)keep; // rows that stay among those which agree with it so far
-    constexpr int kShift[3] = {21, 10, 0};
+struct alignas(16) PlanShared {
+    int hist[3][kBins];
+    int warp_sum[32];
+    int2 warp_marks[32];
+    int equal;            // rows of the last one's number in this CTA
+    int2 marks;           // holes, and rows that fill them, in this CTA
+    uint32_t bin, left;
+    int bad, give, cuts, rows;
+    bool last;
+};
+
+template <typename T>
+__device__ __forceinline__ T of_rank(const T& x, uint32_t rank) {  // a value in the shared memory of a CTA of the cluster
+    static_assert(sizeof(T) % 4 == 0, "words");
+    T out;
+    const uint32_t at = cluster_map(&x, rank);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 4; ++i)
+        reinterpret_cast<float*>(&out)[i] = ld_cluster_f32(at + 4 * i);
+    return out;
+}
+
+template <int kThreads, bool kCluster>
+__device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared& s, uint32_t* ranks, int unit, const Cut& cut,
+                                       uint32_t rank, uint32_t ctas) {
+    constexpr int kWarps = kThreads / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = unit / a.heads;
+    const float* weight = a.w.weight + (int64_t)unit * a.w.capacity;
+    const int32_t* position = a.w.position + (int64_t)unit * a.w.capacity;
+    const int64_t recent_from = (int64_t)cut.len + min(max(a.w.evicted[r], 0), 1 << 30) - a.recent;
+    const int keep = cut.keep;
+    // This CTA's rows: whole steps of 32 for each of its warps.
+    const int each = ((cut.len + (int)ctas - 1) / (int)ctas + 32 * kWarps - 1) / (32 * kWarps) * (32 * kWarps);
+    const int row0 = min((int64_t)cut.len, (int64_t)each * rank), n = min(each, cut.len - row0);
+    auto number = [&](int i) { return rank_of(a, weight[i], position[i], recent_from); };
+    auto rank_at = [&](int i) { return i < a.held_rows ? ranks[i] : number(row0 + i); };  // (i: of this CTA)
+    auto all_arrive = [&] {
+        if constexpr (kCluster) cluster_sync_all(); else __syncthreads();
+    };
+
+    for (int i = tid; i < 3 * kBins; i += kThreads) s.hist[0][i] = 0;
+    __syncthreads();
+    auto count_in = [&](int* hist, uint32_t bin, bool in) {
+        // A warp of equal numbers counts as one.
+        const uint32_t first = __shfl_sync(0xffffffffu, bin, 0);
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (__all_sync(0xffffffffu, !in || bin == first) && (who & 1)) {
+            if (lane == 0) atomicAdd(&hist[first], __popc(who));
+        } else if (in) {
+            atomicAdd(&hist[bin], 1);
+        }
+    };
+    // The numbers, four rows a thread at a time where they lie so, and the first histogram.
+    {
+        constexpr int kAtOnce = 4;
+        const int held = min(n, a.held_rows);
+        const int whole = a.vectors ? held / (4 * kThreads * kAtOnce) * (4 * kThreads * kAtOnce) : 0;
+        for (int i0 = 0; i0 < whole; i0 += 4 * kThreads * kAtOnce) {
+            float4 w[kAtOnce];
+            int4 p[kAtOnce];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + 4 * (e * kThreads + tid);
+                w[e] = *reinterpret_cast<const float4*>(weight + row0 + i);
+                p[e] = *reinterpret_cast<const int4*>(position + row0 + i);
+            }
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + 4 * (e * kThreads + tid);
+                const uint4 x = make_uint4(rank_of(a, w[e].x, p[e].x, recent_from), rank_of(a, w[e].y, p[e].y, recent_from),
+                                           rank_of(a, w[e].z, p[e].z, recent_from), rank_of(a, w[e].w, p[e].w, recent_from));
+                *reinterpret_cast<uint4*>(ranks + i) = x;
+                count_in(s.hist[0], x.x >> 21, true);
+                count_in(s.hist[0], x.y >> 21, true);
+                count_in(s.hist[0], x.z >> 21, true);
+                count_in(s.hist[0], x.w >> 21, true);
+            }
+        }
+        for (int i0 = whole; i0 < n; i0 += kThreads * kAtOnce) {
+            uint32_t x[kAtOnce];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + e * kThreads + tid;
+                x[e] = i < n ? number(row0 + i) : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + e * kThreads + tid;
+                if (i < held) ranks[i] = x[e];
+                count_in(s.hist[0], x[e] >> 21, i < n);
+            }
+        }
+    }
+    uint32_t found = 0, known = 0;   // the number's upper bits, and which these are
+    uint32_t left = (uint32_t)keep;  // rows that stay among those which agree with it so far
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = kShift[pass];
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t mask = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < len; i += kThreads) {
-            const uint32_t x = number(i);
-            if ((x & known) == found) atomicAdd(&hist[x >> shift & mask], 1);
-        }
-        __syncthreads();
+        int* hist = s.hist[pass];
+        if (pass > 0)
+            for (int i0 = 0; i0 < n; i0 += kThreads) {
+                const int i = i0 + tid;
+                const uint32_t x = i < n ? rank_at(i) : 0u;
+                const bool in = i < n && (x & known) == found;
+                if (__any_sync(0xffffffffu, in)) count_in(hist, x >> shift & mask, in);
+            }
+        all_arrive();
         // From the highest bin down: the one in which the count passes what is left.
         constexpr int kOf = kBins / kThreads;
         int count[kOf], sum = 0;
 #pragma unroll
         for (int i = 0; i < kOf; ++i) {
-            count[i] = hist[kBins - 1 - (tid * kOf + i)];
+            const int bin = kBins - 1 - (tid * kOf + i);
+            if constexpr (kCluster) {
+                count[i] = 0;
+                for (uint32_t c = 0; c < ctas; ++c) count[i] += of_rank(hist[bin], c);
+            } else {
+                count[i] = hist[bin];
+            }
             sum += count[i];
         }
-        uint32_t before = (uint32_t)block_sum(sum, warp_sum).before;
+        const int in_warp = warp_before(sum);
+        if (lane == 31) s.warp_sum[warp] = in_warp + sum;
+        __syncthreads();
+        uint32_t before = (uint32_t)(in_warp + __reduce_add_sync(0xffffffffu, lane < warp ? s.warp_sum[lane] : 0));
 #pragma unroll
         for (int i = 0; i < kOf; ++i) {
             if (before < left && left <= before + count[i]) {
-                s_bin = (uint32_t)(kBins - 1 - (tid * kOf + i));
-                s_left = left - before;
+                s.bin = (uint32_t)(kBins - 1 - (tid * kOf + i));
+                s.left = left - before;
             }
             before += count[i];
         }
         __syncthreads();
-        found |= s_bin << shift;
+        found |= s.bin << shift;
         known |= mask << shift;
-        left = s_left;
+        left = s.left;
     }
-
-    int32_t* holes = a.lists + unit * 2 * a.max_keep;
-    int32_t* fills = holes + a.max_keep;
-    int32_t* take = a.take + unit * a.max_keep;
-    int equal = 0, n_holes = 0, n_fills = 0;  // of all rows before: of the very number, holes, rows that fill them
-    for (int i0 = 0; i0 < len; i0 += kThreads * kEach) {
-        const int first = i0 + tid * kEach;
-        uint32_t x[kEach];
-        int same = 0;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            x[e] = first + e < len ? number(first + e) : 0u;
-            same += first + e < len && x[e] == found;
-        }
-        const Sum ties = block_sum(same, warp_sum);
-        int tie = equal + ties.before;
-        equal += ties.all;
-        bool mark[kEach];
-        int marks = 0;  // holes, and from bit 16 on rows that fill them
-        static_assert(kThreads * kEach < 32768, "15 bits of each");
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = first + e;
-            bool stays = i < len && x[e] > found;
-            if (i < len && x[e] == found) stays = (uint32_t)tie++ < left;
-            mark[e] = i < len && stays == (i >= keep);
-            if (mark[e]) marks += i < keep ? 1 : 1 << 16;
-        }
-        const Sum both = block_sum(marks, warp_sum);
-        int at_hole = n_holes + (both.before & 0xffff), at_fill = n_fills + (both.before >> 16);
-        n_holes += both.all & 0xffff;
-        n_fills += both.all >> 16;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = first + e;
-            if (i < keep) take[i] = -1;
-            if (mark[e]) {
-                if (i < keep) holes[at_hole++] = i; else fills[at_fill++] = i;
-            }
-        }
-    }
-    for (int i = keep + tid; i < a.max_keep; i += kThreads) take[i] = -1;
+    // A warp's stretch of the CTA's rows.
+    const int per_warp = each / kWarps, w0 = warp * per_warp, w1 = min(n, w0 + per_warp);
+    // Rows of the very number before this warp's.
+    int equal = 0;
+    for (int i0 = w0; i0 < w1; i0 += 32) equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < w1 && rank_at(i0 + lane) == found));
+    if (lane == 0) s.warp_sum[warp] = equal;
     __syncthreads();
-    for (int i = tid; i < n_holes; i += kThreads) take[holes[i]] = fills[i];
+    const int of_warp = lane < kWarps ? s.warp_sum[lane] : 0;
+    if (tid == 0) s.equal = 0;
+    if (warp == 0) {
+        const int all = __reduce_add_sync(0xffffffffu, of_warp);
+        if (lane == 0) s.equal = all;
+    }
+    int tie = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
+    all_arrive();
+    if constexpr (kCluster)
+        tie += __reduce_add_sync(0xffffffffu, lane < (int)rank ? of_rank(s.equal, min((uint32_t)lane, ctas - 1)) : 0);
+    const int tie0 = tie;
+    // Whether row i (of this CTA, below w1) is a hole or fills one; ties are counted in order.
+    auto mark_of = [&](int i) {
+        const uint32_t x = i < w1 ? rank_at(i) : 0u;
+        const bool same = i < w1 && x == found;
+        const uint32_t ties = __ballot_sync(0xffffffffu, same);
+        const bool stays = i < w1 && (x > found || (same && (uint32_t)(tie + __popc(ties & ((1u << lane) - 1))) < left));
+        tie += __popc(ties);
+        return i < w1 && stays == (row0 + i >= keep);
+    };
+    int2 marks = make_int2(0, 0);
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        const uint32_t m = __ballot_sync(0xffffffffu, mark_of(i0 + lane));
+        const int split = min(32, max(0, keep - row0 - i0));  // rows of the step below keep
+        const uint32_t low = split == 32 ? 0xffffffffu : (1u << split) - 1;
+        marks.x += __popc(m & low);
+        marks.y += __popc(m & ~low);
+    }
+    if (lane == 0) s.warp_marks[warp] = marks;
+    __syncthreads();
+    const int2 wm = lane < kWarps ? s.warp_marks[lane] : make_int2(0, 0);
+    if (warp == 0) {
+        const int2 all = make_int2(__reduce_add_sync(0xffffffffu, wm.x), __reduce_add_sync(0xffffffffu, wm.y));
+        if (lane == 0) s.marks = all;
+    }
+    int at_hole = __reduce_add_sync(0xffffffffu, lane < warp ? wm.x : 0);
+    int at_fill = __reduce_add_sync(0xffffffffu, lane < warp ? wm.y : 0);
+    all_arrive();
+    int holes_all = 0;
+    {
+        int2 x = make_int2(0, 0);
+        if constexpr (kCluster) {
+            if (lane < (int)ctas) x = of_rank(s.marks, (uint32_t)lane);
+        } else if (lane == 0) {
+            x = s.marks;
+        }
+        holes_all = __reduce_add_sync(0xffffffffu, x.x);
+        at_hole += __reduce_add_sync(0xffffffffu, lane < (int)rank ? x.x : 0);
+        at_fill += __reduce_add_sync(0xffffffffu, lane < (int)rank ? x.y : 0);
+    }
+    int32_t* holes = a.lists + (int64_t)unit * 2 * a.max_keep;
+    int32_t* fills = holes + a.max_keep;
+    int32_t* take = a.take + (int64_t)unit * a.max_keep;
+    tie = tie0;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        const int i = row0 + i0 + lane;
+        const bool mark = mark_of(i0 + lane);
+        const uint32_t m = __ballot_sync(0xffffffffu, mark);
+        const int split = min(32, max(0, keep - row0 - i0));
+        const uint32_t low = split == 32 ? 0xffffffffu : (1u << split) - 1, before = (1u << lane) - 1;
+        if (lane < split && i0 + lane < w1) take[i] = -1;
+        if (mark) {
+            if (lane < split) holes[at_hole + __popc(m & low & before)] = i;
+            else fills[at_fill + __popc(m & ~low & before)] = i;
+        }
+        at_hole += __popc(m & low);
+        at_fill += __popc(m & ~low);
+    }
+    for (int i = keep + (int)rank * kThreads + tid; i < a.max_keep; i += (int)ctas * kThreads) take[i] = -1;
+    if constexpr (kCluster) __threadfence();
+    all_arrive();
+    for (int i = (int)rank * kThreads + tid; i < holes_all; i += (int)ctas * kThreads) take[__ldcg(holes + i)] = __ldcg(fills + i);
 }
 
+template <int kThreads, bool kCluster>
 __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_constant__ EvictPlanArgs a) {
-    __shared__ int hist[kBins];
-    __shared__ int warp_sum[kWarps];
-    __shared__ bool s_last;
+    extern __shared__ uint32_t ranks[];
+    __shared__ PlanShared s;
     const int tid = threadIdx.x, n = a.requests;
+    uint32_t rank = 0, ctas = 1;
+    if constexpr (kCluster) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+    }
+    const int unit = blockIdx.x / ctas;
     const int page_mask = (1 << a.page_shift) - 1;
     auto pages_of = [&](int len) { return (int)(((int64_t)len + page_mask) >> a.page_shift); };
+    if (tid == 0) s.bad = s.give = s.cuts = s.rows = 0;
     const int n_free = *a.n_free;
+    __syncthreads();
     // All or nothing: every CTA looks at all requests.
     const int per = (n + kThreads - 1) / kThreads, r0 = min(n, tid * per), r1 = min(n, r0 + per);
     bool bad = false;
-    int give = 0;
+    int64_t give = 0;
     for (int r = r0; r < r1; ++r) {
         const Cut c = cut_of(a, r);
         bad |= c.len < 0 || pages_of(c.len) > a.table_width || c.len > a.w.capacity;
         if (!bad) give += pages_of(c.len) - pages_of(c.keep);
     }
+    if (give > 0) atomicAdd(&s.give, (int)min(give, (int64_t)0x7fffffff / kThreads));  // (past any stack all the same)
     bad = __syncthreads_or(bad);
-    const Sum gives = block_sum(bad ? 0 : give, warp_sum);
-    const bool ok = !bad && n_free >= 0 && (int64_t)n_free + gives.all <= a.free_capacity;
+    const bool ok = !bad && n_free >= 0 && (int64_t)n_free + s.give <= a.free_capacity;
 
-    if ((int)blockIdx.x < n * a.heads) {
-        const int r = blockIdx.x / a.heads, h = blockIdx.x - r * a.heads;
-        const Cut cut = cut_of(a, r);
+    if (unit < n * a.heads) {
+        const Cut cut = cut_of(a, unit / a.heads);
         if (ok && cut.keep < cut.len) {
-            choose(a, r, h, cut, hist, warp_sum);
+            choose<kThreads, kCluster>(a, s, ranks, unit, cut, rank, ctas);
         } else {
-            int32_t* take = a.take + (int64_t)blockIdx.x * a.max_keep;
-            for (int i = tid; i < a.max_keep; i += kThreads) take[i] = -1;
+            int32_t* take = a.take + (int64_t)unit * a.max_keep;
+            for (int i = (int)rank * kThreads + tid; i < a.max_keep; i += (int)ctas * kThreads) take[i] = -1;
         }
-    } else {
-        int at = gives.before, cuts = 0, rows = 0;
+    } else if (rank == 0) {
+        // Pages that each thread's requests give, and what those before them give.
+        const int lane = tid & 31, warp = tid >> 5, mine = ok ? (int)give : 0, in_warp = warp_before(mine);
+        if (lane == 31) s.warp_sum[warp] = in_warp + mine;
+        __syncthreads();
+        int at = in_warp + __reduce_add_sync(0xffffffffu, lane < warp ? s.warp_sum[lane] : 0), cuts = 0, rows = 0;
         for (int r = r0; r < r1 && ok; ++r) {
             const Cut c = cut_of(a, r);
             cuts += c.keep < c.len;
@@ -205,12 +337,13 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
             const int32_t* row = a.block_table + r * a.table_stride;
             for (int j = pages_of(c.keep); j < pages_of(c.len); ++j) a.free_pages[n_free + at++] = row[j];
         }
-        cuts = block_sum(cuts, warp_sum).all;
-        rows = block_sum(rows, warp_sum).all;
+        atomicAdd(&s.cuts, cuts);
+        atomicAdd(&s.rows, rows);
+        __syncthreads();
         if (tid == 0) {
-            a.counts[0] = cuts;
-            a.counts[1] = rows;
-            a.counts[2] = ok ? gives.all : 0;
+            a.counts[0] = s.cuts;
+            a.counts[1] = s.rows;
+            a.counts[2] = ok ? s.give : 0;
             a.counts[3] = ok ? GQA_OK : GQA_ERR_PAGES;
         }
     }
@@ -218,19 +351,19 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
     __syncthreads();
     if (tid == 0) {
         __threadfence();
-        s_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+        s.last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
         __threadfence();
-        if (s_last) *a.ticket = 0;
+        if (s.last) *a.ticket = 0;
     }
-    __syncthreads();
-    if (!s_last) return;
+    if constexpr (kCluster) cluster_sync_all(); else __syncthreads();  // (none leaves while another reads its counts)
+    if (!s.last) return;
     for (int r = tid; r < n; r += kThreads) {
         const Cut c = cut_of(a, r);
         const int evicted = a.w.evicted[r];
         a.lens_out[r] = ok ? c.keep : c.len;
         a.evicted_out[r] = ok ? evicted + (c.len - c.keep) : evicted;
     }
-    if (tid == 0) *a.n_free_out = ok ? n_free + gives.all : n_free;
+    if (tid == 0) *a.n_free_out = ok ? n_free + s.give : n_free;
 }
 
 // ---------------------------------------------------------------------------
@@ -263,14 +396,36 @@ __device__ __forceinline__ BlockScale moved_scale(uint32_t top, float rest, floa
     return BlockScale{value, value == value ? __frcp_rn(value) : 0.f, mine > old};
 }
 
-// c s / scale, rounded to FP32 but for the last half of a thousandth of a unit.  The scales of a block and of
-// what moves into it are often in the ratio of two codes, so that the quotient lies half way between two
-// others: products rounded one after the other would take either (outputs twice as far from the rounded
-// values of e4m3).
-__device__ __forceinline__ float over_scale(float c, float s, const BlockScale& scale) {
-    const float x = __fmul_rn(c, s), x_rest = __fmaf_rn(c, s, -x);
-    const float y = __fmul_rn(x, scale.inv);
-    return __fmaf_rn(__fadd_rn(__fmaf_rn(-y, scale.value, x), x_rest), scale.inv, y);
+// s / scale in two parts: c times both, added in one step, is c s / scale rounded to FP32 but for the last
+// thousandth of a unit.  The scales of a block and of what moves into it are often in the ratio of two codes, so
+// that the quotient lies half way between two others: products rounded one after the other would take either
+// (e4m3 values 0.0044 of their norm from the rounded ones instead of 0.0017).
+struct Ratio {
+    float hi, lo;
+};
+__device__ __forceinline__ Ratio ratio_of(float s, const BlockScale& scale) {
+    const float hi = __fmul_rn(s, scale.inv);
+    return Ratio{hi, __fmul_rn(__fmaf_rn(-hi, scale.value, s), scale.inv)};
+}
+__device__ __forceinline__ float times(float c, const Ratio& r) { return __fmaf_rn(c, r.hi, __fmul_rn(c, r.lo)); }
+
+// Four codes of a word as values.
+template <int kCode>
+__device__ __forceinline__ void values4(uint32_t w, float (&x)[4]) {
+    if constexpr (kCode == GQA_CODE_INT8) {
+        const uint32_t u = w ^ 0x80808080u;  // 2^23 + (c + 128) as FP32
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + e)) - 8388736.f;
+    } else {
+        uint32_t lo, hi;
+        to_half4<kCode>(w, lo, hi);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        x[0] = a.x;
+        x[1] = a.y;
+        x[2] = b.x;
+        x[3] = b.y;
+    }
 }
 
 constexpr int kHeldRows = 8;  // rows of a lane that stay in registers between the two passes
@@ -331,16 +486,19 @@ __global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ Evic
                                                    (from & (page_len - 1)) * a.c.row_stride),
                    scales[at * a.c.scale_page_stride]};
     };
-    auto code = [](const uint4& w, int e) {
-        const uint32_t x = e < 4 ? w.x : e < 8 ? w.y : e < 12 ? w.z : w.w;
-        return code_value<kCode>((uint8_t)(x >> (8 * (e & 3))));
-    };
     float most = 0.f, most_rest = 0.f;  // the largest magnitude, and what rounding it to FP32 took
     bool fine = true;
     auto measure = [&](const Row& x) {
-        float m = 0.f;
+        const uint32_t ws[4] = {x.w.x, x.w.y, x.w.z, x.w.w};
+        __half2 top = __half2half2(__ushort_as_half(0));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(code(x.w, e)));
+        for (int i = 0; i < 4; ++i) {
+            uint32_t lo, hi;
+            to_half4<kCode>(ws[i], lo, hi);
+            top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&lo)));
+            top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&hi)));
+        }
+        const float m = __half2float(__hmax(__low2half(top), __high2half(top)));
         const float v = __fmul_rn(m, x.scale);
         if (v > most) {
             most = v;
@@ -365,12 +523,17 @@ __global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ Evic
     const BlockScale scale = moved_scale(top, most_rest, qmax, old);
     const bool number = scale.value == scale.value;
     auto codes16 = [&](const uint4& w, float s) {
+        if (!number) return make_uint4(0u, 0u, 0u, 0u);
+        if (s == scale.value) return w;
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        const Ratio ratio = ratio_of(s, scale);
         uint32_t o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float y[4];
+            values4<kCode>(ws[i], y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = number ? over_scale(code(w, 4 * i + e), s, scale) : 0.f;
+            for (int e = 0; e < 4; ++e) y[e] = times(y[e], ratio);
             o[i] = value_codes4<kCode>(y[0], y[1], y[2], y[3]);
         }
         return make_uint4(o[0], o[1], o[2], o[3]);
@@ -391,6 +554,44 @@ __global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ Evic
             *at = codes16(*at, old);
         }
     if (lane == 0) scales[page * a.c.scale_page_stride] = scale.value;
+}
+
+// How many CTAs a (request, head) gets goes by the rows that it may hold (its lengths are in device memory): stretches
+// of 4096 and more fill a CTA's time beside what a cluster's barriers cost, as long as there are SMs for them.
+template <int kThreads, bool kCluster>
+cudaError_t launch_plan(const EvictPlanArgs& a, int ctas, size_t smem, cudaStream_t stream) {
+    const auto kernel = plan_eviction_kernel<kThreads, kCluster>;
+    // The limit is the kernel's, not the call's: always the same, so that another thread's call does not lower it.
+    if (smem > 16 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRows * (int)sizeof(uint32_t));
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.requests * a.heads + 1) * ctas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = kCluster ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+cudaError_t launch_plan_eviction(EvictPlanArgs& a, int sms, cudaStream_t stream) {
+    const int64_t most = std::min<int64_t>(a.w.capacity, (int64_t)a.table_width << a.page_shift);
+    const int units = a.requests * a.heads;
+    int ctas = 1;
+    while (ctas < kMaxCluster && most >= 8192 * (int64_t)ctas && units * ctas * 2 <= 2 * sms) ctas *= 2;
+    const bool small = most <= 2048;
+    const int step = small ? 128 : 512;
+    const int64_t rows = ((most + ctas - 1) / ctas + step - 1) / step * step;
+    a.held_rows = (int)std::min<int64_t>(rows, kMaxRows);
+    const size_t smem = a.held_rows * sizeof(uint32_t);
+    if (small) return launch_plan<128, false>(a, 1, smem, stream);
+    return ctas > 1 ? launch_plan<512, true>(a, ctas, smem, stream) : launch_plan<512, false>(a, 1, smem, stream);
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -466,8 +667,8 @@ int gqa_plan_eviction(const gqa_key_weights* weights, int kv_heads, const int32_
     a.max_keep = max_keep;
     a.sinks = sinks;
     a.recent = recent;
-    plan_eviction_kernel<<<requests * kv_heads + 1, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return cudaGetLastError() == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+    a.vectors = weights->capacity % 4 == 0 && !((reinterpret_cast<uintptr_t>(a.w.weight) | reinterpret_cast<uintptr_t>(a.w.position)) & 15u);
+    return launch_plan_eviction(a, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
 int gqa_evict_paged(const gqa_paged_cache* cache, const int32_t* block_table, int64_t table_stride, int table_width,

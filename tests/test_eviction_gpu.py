@@ -547,3 +547,43 @@ def test_refusals():
         gqa.evict_paged(s.cache, table, w, gqa.EvictionPlan(plan.take[:, :4], plan.lens, None, None, None))
     with pytest.raises(ValueError, match="hold 47 rows"):
         gqa.evict_paged(s.cache, table, small, plan)
+
+
+@pytest.mark.parametrize("requests,heads,longest,keep", [(1, 8, 131072, 4000), (1, 1, 40000, 39000), (3, 8, 20000, 1),
+                                                         (40, 8, 50500, 700), (70, 8, 8200, 4096)])
+@pytest.mark.parametrize("kind", ["spread", "equal", "two"])
+def test_plan_of_long_requests(requests, heads, longest, keep, kind):
+    """Requests whose rows several thread blocks share, and more rows than one keeps on chip, against a stable sort."""
+    gen = torch.Generator("cuda").manual_seed(longest)
+    page_len = 64
+    width = -(-longest // page_len)
+    w = gqa.key_weights(requests, width * page_len, kv_heads=heads)
+    if kind == "spread":
+        w.weight.copy_(torch.exp(3 * torch.randn(w.weight.shape, generator=gen, device="cuda")))
+        w.weight[..., ::3] = 1.0
+    elif kind == "two":
+        w.weight.copy_(torch.randint(0, 2, w.weight.shape, generator=gen, device="cuda"))
+    w.position.copy_(torch.arange(width * page_len, device="cuda").flip(0).expand_as(w.position))
+    lens = [longest - (r * 977) % (longest // 2) for r in range(requests)]
+    free, n_free = torch.full((requests * width,), -1, dtype=torch.int32, device="cuda"), ints([0])
+    table = torch.arange(requests * width, dtype=torch.int32, device="cuda").view(requests, width)
+    ln = ints(lens)
+    plan = gqa.plan_eviction(w, ln, ints([keep] * requests), table, free, n_free, page_len=page_len, max_keep=keep, sinks=3,
+                             recent=5)
+    plan.check()
+    row = torch.arange(width * page_len, device="cuda")
+    safe = (w.position < 3) | (w.position >= (ln - 5)[:, None, None])
+    mark = w.weight.view(torch.int32).long() + (safe.long() << 32)
+    mark = torch.where(row < ln[:, None, None], mark, -1)
+    order = torch.sort(mark, dim=-1, descending=True, stable=True).indices[..., :keep]
+    stays = torch.zeros_like(mark, dtype=torch.bool).scatter_(-1, order, True)
+    stays &= (ln > keep)[:, None, None] | (row < ln[:, None, None])
+    for r in range(requests):
+        for h in range(0, heads, 3):
+            if lens[r] <= keep:
+                assert bool((plan.take[r, h] == -1).all())
+                continue
+            holes, fills = torch.nonzero(~stays[r, h, :keep])[:, 0], torch.nonzero(stays[r, h, keep:])[:, 0] + keep
+            want = torch.full((keep,), -1, dtype=torch.int32, device="cuda")
+            want[holes] = fills.int()
+            assert torch.equal(plan.take[r, h], want), (r, h)
