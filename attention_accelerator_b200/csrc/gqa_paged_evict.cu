@@ -16,14 +16,14 @@ namespace {
 // A cluster of 1 to 8 CTAs a (request, KV head), each with a stretch of its rows.  A
 // row's rank is that of a 32-bit number: the bits of its weight, which order as the
 // weights do (they are not negative), and above them whether it is spared; the
-// numbers are computed once and kept in shared memory.  Three passes over histograms
-// of 11, 11 and 10 bits, from the top, find the number of the last row that stays and
-// how many rows of that very number stay.  Two more count, a warp a stretch of rows,
-// what is equal to it and then the holes below `keep` and the rows past it that stay;
-// the last lists both in order, and they are paired off.  One more CTA gives the pages
-// back.
+// numbers are computed once and kept in shared memory.  Passes over histograms, from
+// the top bits down (11, 11 and 10; 4 times 8 for short requests, whose time is the
+// bins'), find the number of the last row that stays and how many rows of that very
+// number stay.  Two more count, a warp a stretch of rows, a lane four rows, what is equal
+// to it and then the holes below `keep` and the rows past it that stay; the last lists
+// both in order, and they are paired off.  One more CTA gives the pages back.
 // ---------------------------------------------------------------------------
-constexpr int kBins = 2048, kMaxCluster = 8;
+constexpr int kMaxCluster = 8;
 constexpr int kMaxRows = 48 * 1024;  // of a CTA in shared memory; numbers of rows past that are computed again
 
 struct EvictPlanArgs {
@@ -39,6 +39,7 @@ struct EvictPlanArgs {
     int requests, heads, table_width, free_capacity, page_shift, max_keep, sinks, recent;
     int held_rows;   // of a CTA in shared memory
     bool vectors;    // weights and positions of a head are 16-byte aligned
+    bool in_place;   // lens_out, evicted_out or n_free_out may be what is read
 };
 
 struct Cut {
@@ -67,14 +68,24 @@ __device__ __forceinline__ int warp_before(int v) {
     return incl - v;
 }
 
+template <int kThreads>
+struct Radix {
+    static constexpr int kBits = kThreads == 128 ? 8 : 11, kPasses = kThreads == 128 ? 4 : 3, kBins = 1 << kBits;
+    static __device__ __forceinline__ constexpr int shift(int pass) { return pass + 1 == kPasses ? 0 : 32 - kBits * (pass + 1); }
+    static __device__ __forceinline__ constexpr uint32_t mask(int pass) {
+        return pass + 1 == kPasses ? (1u << (32 - kBits * (kPasses - 1))) - 1 : (1u << kBits) - 1;
+    }
+};
+
+template <int kThreads>
 struct alignas(16) PlanShared {
-    int hist[3][kBins];
+    int hist[Radix<kThreads>::kPasses][Radix<kThreads>::kBins];
     int warp_sum[32];
     int2 warp_marks[32];
     int equal;            // rows of the last one's number in this CTA
     int2 marks;           // holes, and rows that fill them, in this CTA
     uint32_t bin, left;
-    int bad, give, cuts, rows;
+    int give, cuts, rows;
     bool last;
 };
 
@@ -90,97 +101,107 @@ __device__ __forceinline__ T of_rank(const T& x, uint32_t rank) {  // a value in
 }
 
 template <int kThreads, bool kCluster>
-__device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared& s, uint32_t* ranks, int unit, const Cut& cut,
+__device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThreads>& s, uint32_t* ranks, int unit, const Cut& cut,
                                        uint32_t rank, uint32_t ctas) {
-    constexpr int kWarps = kThreads / 32;
+    using R = Radix<kThreads>;
+    constexpr int kWarps = kThreads / 32, kStep = 128 * kWarps;  // four rows a lane
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = unit / a.heads;
     const float* weight = a.w.weight + (int64_t)unit * a.w.capacity;
     const int32_t* position = a.w.position + (int64_t)unit * a.w.capacity;
     const int64_t recent_from = (int64_t)cut.len + min(max(a.w.evicted[r], 0), 1 << 30) - a.recent;
     const int keep = cut.keep;
-    // This CTA's rows: whole steps of 32 for each of its warps.
-    const int each = ((cut.len + (int)ctas - 1) / (int)ctas + 32 * kWarps - 1) / (32 * kWarps) * (32 * kWarps);
-    const int row0 = min((int64_t)cut.len, (int64_t)each * rank), n = min(each, cut.len - row0);
+    // This CTA's rows: whole steps of 128 for each of its warps.
+    const int each = ((cut.len + (int)ctas - 1) / (int)ctas + kStep - 1) / kStep * kStep;
+    const int row0 = (int)min((int64_t)cut.len, (int64_t)each * rank), n = min(each, cut.len - row0);
     auto number = [&](int i) { return rank_of(a, weight[i], position[i], recent_from); };
-    auto rank_at = [&](int i) { return i < a.held_rows ? ranks[i] : number(row0 + i); };  // (i: of this CTA)
+    // Rows i to i + 3 of this CTA (0 past its last).
+    auto four = [&](int i) {
+        if (i < a.held_rows) return *reinterpret_cast<const uint4*>(ranks + i);
+        uint4 x;
+        x.x = i < n ? number(row0 + i) : 0u;
+        x.y = i + 1 < n ? number(row0 + i + 1) : 0u;
+        x.z = i + 2 < n ? number(row0 + i + 2) : 0u;
+        x.w = i + 3 < n ? number(row0 + i + 3) : 0u;
+        return x;
+    };
     auto all_arrive = [&] {
         if constexpr (kCluster) cluster_sync_all(); else __syncthreads();
     };
 
-    for (int i = tid; i < 3 * kBins; i += kThreads) s.hist[0][i] = 0;
+    for (int i = tid; i < R::kPasses * R::kBins; i += kThreads) s.hist[0][i] = 0;
     __syncthreads();
     auto count_in = [&](int* hist, uint32_t bin, bool in) {
         // A warp of equal numbers counts as one.
         const uint32_t first = __shfl_sync(0xffffffffu, bin, 0);
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (__all_sync(0xffffffffu, !in || bin == first) && (who & 1)) {
-            if (lane == 0) atomicAdd(&hist[first], __popc(who));
+        if (__all_sync(0xffffffffu, in && bin == first)) {
+            if (lane == 0) atomicAdd(&hist[bin], 32);
         } else if (in) {
             atomicAdd(&hist[bin], 1);
         }
     };
-    // The numbers, four rows a thread at a time where they lie so, and the first histogram.
+    // The numbers, and the first histogram.
+    auto keep_four = [&](int i, const uint4& x) {  // (i < each)
+        if (i < a.held_rows) *reinterpret_cast<uint4*>(ranks + i) = x;
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) count_in(s.hist[0], xs[e] >> R::shift(0), i + e < n);
+    };
     {
         constexpr int kAtOnce = 4;
-        const int held = min(n, a.held_rows);
-        const int whole = a.vectors ? held / (4 * kThreads * kAtOnce) * (4 * kThreads * kAtOnce) : 0;
-        for (int i0 = 0; i0 < whole; i0 += 4 * kThreads * kAtOnce) {
-            float4 w[kAtOnce];
-            int4 p[kAtOnce];
+        int i0 = 0;
+        if (a.vectors)
+            for (; i0 + kStep * kAtOnce <= n; i0 += kStep * kAtOnce) {
+                float4 w[kAtOnce];
+                int4 p[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-                const int i = i0 + 4 * (e * kThreads + tid);
-                w[e] = *reinterpret_cast<const float4*>(weight + row0 + i);
-                p[e] = *reinterpret_cast<const int4*>(position + row0 + i);
+                for (int e = 0; e < kAtOnce; ++e) {
+                    const int i = row0 + i0 + e * kStep + 4 * tid;
+                    w[e] = *reinterpret_cast<const float4*>(weight + i);
+                    p[e] = *reinterpret_cast<const int4*>(position + i);
+                }
+#pragma unroll
+                for (int e = 0; e < kAtOnce; ++e)
+                    keep_four(i0 + e * kStep + 4 * tid,
+                              make_uint4(rank_of(a, w[e].x, p[e].x, recent_from), rank_of(a, w[e].y, p[e].y, recent_from),
+                                         rank_of(a, w[e].z, p[e].z, recent_from), rank_of(a, w[e].w, p[e].w, recent_from)));
             }
+        for (; i0 < n; i0 += 2 * kStep) {
+            uint32_t x[8];
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-                const int i = i0 + 4 * (e * kThreads + tid);
-                const uint4 x = make_uint4(rank_of(a, w[e].x, p[e].x, recent_from), rank_of(a, w[e].y, p[e].y, recent_from),
-                                           rank_of(a, w[e].z, p[e].z, recent_from), rank_of(a, w[e].w, p[e].w, recent_from));
-                *reinterpret_cast<uint4*>(ranks + i) = x;
-                count_in(s.hist[0], x.x >> 21, true);
-                count_in(s.hist[0], x.y >> 21, true);
-                count_in(s.hist[0], x.z >> 21, true);
-                count_in(s.hist[0], x.w >> 21, true);
-            }
-        }
-        for (int i0 = whole; i0 < n; i0 += kThreads * kAtOnce) {
-            uint32_t x[kAtOnce];
-#pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-                const int i = i0 + e * kThreads + tid;
+            for (int e = 0; e < 8; ++e) {
+                const int i = i0 + (e >> 2) * kStep + 4 * tid + (e & 3);
                 x[e] = i < n ? number(row0 + i) : 0u;
             }
-#pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-                const int i = i0 + e * kThreads + tid;
-                if (i < held) ranks[i] = x[e];
-                count_in(s.hist[0], x[e] >> 21, i < n);
-            }
+            keep_four(i0 + 4 * tid, make_uint4(x[0], x[1], x[2], x[3]));
+            if (i0 + kStep < each) keep_four(i0 + kStep + 4 * tid, make_uint4(x[4], x[5], x[6], x[7]));
         }
     }
     uint32_t found = 0, known = 0;   // the number's upper bits, and which these are
     uint32_t left = (uint32_t)keep;  // rows that stay among those which agree with it so far
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    for (int pass = 0; pass < R::kPasses; ++pass) {
+        const int shift = R::shift(pass);
+        const uint32_t mask = R::mask(pass);
         int* hist = s.hist[pass];
         if (pass > 0)
-            for (int i0 = 0; i0 < n; i0 += kThreads) {
-                const int i = i0 + tid;
-                const uint32_t x = i < n ? rank_at(i) : 0u;
-                const bool in = i < n && (x & known) == found;
-                if (__any_sync(0xffffffffu, in)) count_in(hist, x >> shift & mask, in);
+            for (int i0 = 0; i0 < n; i0 += kStep) {
+                const int i = i0 + 4 * tid;
+                const uint4 x = four(i);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                bool in[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) in[e] = i + e < n && (xs[e] & known) == found;
+                if (__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3]))
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) count_in(hist, xs[e] >> shift & mask, in[e]);
             }
         all_arrive();
         // From the highest bin down: the one in which the count passes what is left.
-        constexpr int kOf = kBins / kThreads;
+        constexpr int kOf = R::kBins / kThreads;
         int count[kOf], sum = 0;
 #pragma unroll
         for (int i = 0; i < kOf; ++i) {
-            const int bin = kBins - 1 - (tid * kOf + i);
+            const int bin = R::kBins - 1 - (tid * kOf + i);
             if constexpr (kCluster) {
                 count[i] = 0;
                 for (uint32_t c = 0; c < ctas; ++c) count[i] += of_rank(hist[bin], c);
@@ -196,7 +217,7 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared& s, ui
 #pragma unroll
         for (int i = 0; i < kOf; ++i) {
             if (before < left && left <= before + count[i]) {
-                s.bin = (uint32_t)(kBins - 1 - (tid * kOf + i));
+                s.bin = (uint32_t)(R::kBins - 1 - (tid * kOf + i));
                 s.left = left - before;
             }
             before += count[i];
@@ -210,56 +231,63 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared& s, ui
     const int per_warp = each / kWarps, w0 = warp * per_warp, w1 = min(n, w0 + per_warp);
     // Rows of the very number before this warp's.
     int equal = 0;
-    for (int i0 = w0; i0 < w1; i0 += 32) equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < w1 && rank_at(i0 + lane) == found));
+    for (int i = w0 + 4 * lane; i < w1; i += 128) {
+        const uint4 x = four(i);
+        equal += (x.x == found) + (i + 1 < w1 && x.y == found) + (i + 2 < w1 && x.z == found) + (i + 3 < w1 && x.w == found);
+    }
+    equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) s.warp_sum[warp] = equal;
     __syncthreads();
     const int of_warp = lane < kWarps ? s.warp_sum[lane] : 0;
-    if (tid == 0) s.equal = 0;
     if (warp == 0) {
         const int all = __reduce_add_sync(0xffffffffu, of_warp);
         if (lane == 0) s.equal = all;
     }
     int tie = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0);
-    all_arrive();
-    if constexpr (kCluster)
+    if constexpr (kCluster) {
+        cluster_sync_all();
         tie += __reduce_add_sync(0xffffffffu, lane < (int)rank ? of_rank(s.equal, min((uint32_t)lane, ctas - 1)) : 0);
+    }
     const int tie0 = tie;
-    // Whether row i (of this CTA, below w1) is a hole or fills one; ties are counted in order.
-    auto mark_of = [&](int i) {
-        const uint32_t x = i < w1 ? rank_at(i) : 0u;
-        const bool same = i < w1 && x == found;
-        const uint32_t ties = __ballot_sync(0xffffffffu, same);
-        const bool stays = i < w1 && (x > found || (same && (uint32_t)(tie + __popc(ties & ((1u << lane) - 1))) < left));
-        tie += __popc(ties);
-        return i < w1 && stays == (row0 + i >= keep);
+    // Which of rows i to i + 3 (of this CTA; a lane's, by whole warps) are holes or fill one, as bits; ties are counted in order.
+    auto marks_of = [&](int i) {
+        const uint4 x = i < w1 ? four(i) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+        uint32_t same = 0, stays = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            same |= (i + e < w1 && xs[e] == found) << e;
+            stays |= (xs[e] > found) << e;
+        }
+        if (__any_sync(0xffffffffu, same)) {
+            int at = tie + warp_before(__popc(same));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (same >> e & 1) stays |= ((uint32_t)at++ < left) << e;
+            tie += __reduce_add_sync(0xffffffffu, __popc(same));
+        }
+        const uint32_t low = (1u << min(4, max(0, keep - row0 - i))) - 1, rows = (1u << min(4, max(0, w1 - i))) - 1;
+        return ((stays & ~low) | (~stays & low)) & rows;
     };
+    auto low_of = [&](int i) { return (1u << min(4, max(0, keep - row0 - i))) - 1; };  // rows below keep
     int2 marks = make_int2(0, 0);
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const uint32_t m = __ballot_sync(0xffffffffu, mark_of(i0 + lane));
-        const int split = min(32, max(0, keep - row0 - i0));  // rows of the step below keep
-        const uint32_t low = split == 32 ? 0xffffffffu : (1u << split) - 1;
+    for (int i0 = w0; i0 < w1; i0 += 128) {
+        const uint32_t m = marks_of(i0 + 4 * lane), low = low_of(i0 + 4 * lane);
         marks.x += __popc(m & low);
         marks.y += __popc(m & ~low);
     }
+    marks = make_int2(__reduce_add_sync(0xffffffffu, marks.x), __reduce_add_sync(0xffffffffu, marks.y));
     if (lane == 0) s.warp_marks[warp] = marks;
     __syncthreads();
     const int2 wm = lane < kWarps ? s.warp_marks[lane] : make_int2(0, 0);
-    if (warp == 0) {
-        const int2 all = make_int2(__reduce_add_sync(0xffffffffu, wm.x), __reduce_add_sync(0xffffffffu, wm.y));
-        if (lane == 0) s.marks = all;
-    }
+    int2 all = make_int2(__reduce_add_sync(0xffffffffu, wm.x), __reduce_add_sync(0xffffffffu, wm.y));
     int at_hole = __reduce_add_sync(0xffffffffu, lane < warp ? wm.x : 0);
     int at_fill = __reduce_add_sync(0xffffffffu, lane < warp ? wm.y : 0);
-    all_arrive();
-    int holes_all = 0;
-    {
-        int2 x = make_int2(0, 0);
-        if constexpr (kCluster) {
-            if (lane < (int)ctas) x = of_rank(s.marks, (uint32_t)lane);
-        } else if (lane == 0) {
-            x = s.marks;
-        }
-        holes_all = __reduce_add_sync(0xffffffffu, x.x);
+    if constexpr (kCluster) {
+        if (tid == 0) s.marks = all;
+        cluster_sync_all();
+        const int2 x = lane < (int)ctas ? of_rank(s.marks, (uint32_t)lane) : make_int2(0, 0);
+        all.x = __reduce_add_sync(0xffffffffu, x.x);
         at_hole += __reduce_add_sync(0xffffffffu, lane < (int)rank ? x.x : 0);
         at_fill += __reduce_add_sync(0xffffffffu, lane < (int)rank ? x.y : 0);
     }
@@ -267,30 +295,33 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared& s, ui
     int32_t* fills = holes + a.max_keep;
     int32_t* take = a.take + (int64_t)unit * a.max_keep;
     tie = tie0;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = row0 + i0 + lane;
-        const bool mark = mark_of(i0 + lane);
-        const uint32_t m = __ballot_sync(0xffffffffu, mark);
-        const int split = min(32, max(0, keep - row0 - i0));
-        const uint32_t low = split == 32 ? 0xffffffffu : (1u << split) - 1, before = (1u << lane) - 1;
-        if (lane < split && i0 + lane < w1) take[i] = -1;
-        if (mark) {
-            if (lane < split) holes[at_hole + __popc(m & low & before)] = i;
-            else fills[at_fill + __popc(m & ~low & before)] = i;
-        }
-        at_hole += __popc(m & low);
-        at_fill += __popc(m & ~low);
+    for (int i0 = w0; i0 < w1; i0 += 128) {
+        const int i = i0 + 4 * lane;
+        const uint32_t m = marks_of(i), low = low_of(i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (low >> e & 1 && i + e < w1) take[row0 + i + e] = -1;
+        if (!__any_sync(0xffffffffu, m)) continue;
+        const int n_low = __popc(m & low), n_high = __popc(m & ~low);
+        int hole = at_hole + warp_before(n_low), fill = at_fill + warp_before(n_high);
+        at_hole += __reduce_add_sync(0xffffffffu, n_low);
+        at_fill += __reduce_add_sync(0xffffffffu, n_high);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (m >> e & 1) {
+                if (low >> e & 1) holes[hole++] = row0 + i + e; else fills[fill++] = row0 + i + e;
+            }
     }
     for (int i = keep + (int)rank * kThreads + tid; i < a.max_keep; i += (int)ctas * kThreads) take[i] = -1;
     if constexpr (kCluster) __threadfence();
     all_arrive();
-    for (int i = (int)rank * kThreads + tid; i < holes_all; i += (int)ctas * kThreads) take[__ldcg(holes + i)] = __ldcg(fills + i);
+    for (int i = (int)rank * kThreads + tid; i < all.x; i += (int)ctas * kThreads) take[__ldcg(holes + i)] = __ldcg(fills + i);
 }
 
 template <int kThreads, bool kCluster>
 __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_constant__ EvictPlanArgs a) {
     extern __shared__ uint32_t ranks[];
-    __shared__ PlanShared s;
+    __shared__ PlanShared<kThreads> s;
     const int tid = threadIdx.x, n = a.requests;
     uint32_t rank = 0, ctas = 1;
     if constexpr (kCluster) {
@@ -300,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
     const int unit = blockIdx.x / ctas;
     const int page_mask = (1 << a.page_shift) - 1;
     auto pages_of = [&](int len) { return (int)(((int64_t)len + page_mask) >> a.page_shift); };
-    if (tid == 0) s.bad = s.give = s.cuts = s.rows = 0;
+    if (tid == 0) s.give = s.cuts = s.rows = 0;
     const int n_free = *a.n_free;
     __syncthreads();
     // All or nothing: every CTA looks at all requests.
@@ -348,15 +379,20 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
         }
     }
     // Every CTA has read lens, evicted and n_free once all have arrived here: the outputs may be these.
-    __syncthreads();
-    if (tid == 0) {
-        __threadfence();
-        s.last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
-        __threadfence();
-        if (s.last) *a.ticket = 0;
+    bool last = unit == n * a.heads && rank == 0;
+    if (a.in_place) {
+        __syncthreads();
+        if (tid == 0) {
+            __threadfence();
+            s.last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+            __threadfence();
+            if (s.last) *a.ticket = 0;
+        }
+        __syncthreads();
+        last = s.last;
     }
-    if constexpr (kCluster) cluster_sync_all(); else __syncthreads();  // (none leaves while another reads its counts)
-    if (!s.last) return;
+    if constexpr (kCluster) cluster_sync_all();  // none leaves while another reads its counts
+    if (!last) return;
     for (int r = tid; r < n; r += kThreads) {
         const Cut c = cut_of(a, r);
         const int evicted = a.w.evicted[r];
@@ -431,7 +467,7 @@ __device__ __forceinline__ void values4(uint32_t w, float (&x)[4]) {
 constexpr int kHeldRows = 8;  // rows of a lane that stay in registers between the two passes
 
 template <int kCode>
-__global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ EvictArgs a) {
+__global__ void __launch_bounds__(256, 4) evict_kernel(const __grid_constant__ EvictArgs a) {
     __shared__ int2 s_moves[kNumKVHeads][kPagedMaxPage];
     dependency_wait();
     allow_dependents();
@@ -586,7 +622,7 @@ cudaError_t launch_plan_eviction(EvictPlanArgs& a, int sms, cudaStream_t stream)
     int ctas = 1;
     while (ctas < kMaxCluster && most >= 8192 * (int64_t)ctas && units * ctas * 2 <= 2 * sms) ctas *= 2;
     const bool small = most <= 2048;
-    const int step = small ? 128 : 512;
+    const int step = small ? 512 : 2048;  // whole steps of a CTA's warps
     const int64_t rows = ((most + ctas - 1) / ctas + step - 1) / step * step;
     a.held_rows = (int)std::min<int64_t>(rows, kMaxRows);
     const size_t smem = a.held_rows * sizeof(uint32_t);
@@ -667,6 +703,13 @@ int gqa_plan_eviction(const gqa_key_weights* weights, int kv_heads, const int32_
     a.max_keep = max_keep;
     a.sinks = sinks;
     a.recent = recent;
+    auto overlap = [](const int32_t* x, int64_t nx, const int32_t* y, int64_t ny) { return x < y + ny && y < x + nx; };
+    a.in_place = false;
+    for (const int32_t* out : {lens_out, evicted_out})
+        a.in_place |= overlap(out, requests, lens, requests) || overlap(out, requests, keep, requests) ||
+                      overlap(out, requests, weights->evicted, requests) || overlap(out, requests, n_free, 1);
+    a.in_place |= overlap(n_free_out, 1, n_free, 1) || overlap(n_free_out, 1, lens, requests) ||
+                  overlap(n_free_out, 1, keep, requests) || overlap(n_free_out, 1, weights->evicted, requests);
     a.vectors = weights->capacity % 4 == 0 && !((reinterpret_cast<uintptr_t>(a.w.weight) | reinterpret_cast<uintptr_t>(a.w.position)) & 15u);
     return launch_plan_eviction(a, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
