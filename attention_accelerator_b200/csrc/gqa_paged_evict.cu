@@ -89,26 +89,35 @@ struct alignas(16) PlanShared {
     bool last;
 };
 
-template <typename T>
-__device__ __forceinline__ T of_rank(const T& x, uint32_t rank) {  // a value in the shared memory of a CTA of the cluster
-    static_assert(sizeof(T) % 4 == 0, "words");
-    T out;
-    const uint32_t at = cluster_map(&x, rank);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 4; ++i)
-        reinterpret_cast<float*>(&out)[i] = ld_cluster_f32(at + 4 * i);
-    return out;
+// Values in the shared memory of a CTA of the cluster.  (Volatile, but not ordered with other memory: several are
+// on their way at once, behind the cluster's barrier.)
+__device__ __forceinline__ int of_rank(const int& x, uint32_t rank) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(cluster_map(&x, rank)));
+    return v;
+}
+__device__ __forceinline__ int2 of_rank(const int2& x, uint32_t rank) {
+    int2 v;
+    asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(cluster_map(&x, rank)));
+    return v;
+}
+__device__ __forceinline__ int4 of_rank(const int4& x, uint32_t rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(cluster_map(&x, rank)));
+    return v;
 }
 
 template <int kThreads, bool kCluster>
 __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThreads>& s, uint32_t* ranks, int unit, const Cut& cut,
-                                       uint32_t rank, uint32_t ctas) {
+                                       int evicted, uint32_t rank, uint32_t ctas) {
     using R = Radix<kThreads>;
     constexpr int kWarps = kThreads / 32, kStep = 128 * kWarps;  // four rows a lane
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = unit / a.heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float* weight = a.w.weight + (int64_t)unit * a.w.capacity;
     const int32_t* position = a.w.position + (int64_t)unit * a.w.capacity;
-    const int64_t recent_from = (int64_t)cut.len + min(max(a.w.evicted[r], 0), 1 << 30) - a.recent;
+    const int64_t recent_from = (int64_t)cut.len + min(max(evicted, 0), 1 << 30) - a.recent;
     const int keep = cut.keep;
     // This CTA's rows: whole steps of 128 for each of its warps.
     const int each = ((cut.len + (int)ctas - 1) / (int)ctas + kStep - 1) / kStep * kStep;
@@ -199,17 +208,27 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThrea
         // From the highest bin down: the one in which the count passes what is left.
         constexpr int kOf = R::kBins / kThreads;
         int count[kOf], sum = 0;
+        if constexpr (kCluster) {
+            static_assert(!kCluster || kOf == 4, "a vector of bins a thread");
+            int4 of[kMaxCluster];
 #pragma unroll
-        for (int i = 0; i < kOf; ++i) {
-            const int bin = R::kBins - 1 - (tid * kOf + i);
-            if constexpr (kCluster) {
-                count[i] = 0;
-                for (uint32_t c = 0; c < ctas; ++c) count[i] += of_rank(hist[bin], c);
-            } else {
-                count[i] = hist[bin];
-            }
-            sum += count[i];
+            for (uint32_t c = 0; c < kMaxCluster; ++c)
+                of[c] = c < ctas ? of_rank(*reinterpret_cast<const int4*>(&hist[R::kBins - 4 * (tid + 1)]), c)
+                                 : make_int4(0, 0, 0, 0);
+            int4 all = of[0];
+#pragma unroll
+            for (uint32_t c = 1; c < kMaxCluster; ++c)
+                all = make_int4(all.x + of[c].x, all.y + of[c].y, all.z + of[c].z, all.w + of[c].w);
+            count[0] = all.w;
+            count[1] = all.z;
+            count[2] = all.y;
+            count[3] = all.x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kOf; ++i) count[i] = hist[R::kBins - 1 - (tid * kOf + i)];
         }
+#pragma unroll
+        for (int i = 0; i < kOf; ++i) sum += count[i];
         const int in_warp = warp_before(sum);
         if (lane == 31) s.warp_sum[warp] = in_warp + sum;
         __syncthreads();
@@ -332,7 +351,9 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
     const int page_mask = (1 << a.page_shift) - 1;
     auto pages_of = [&](int len) { return (int)(((int64_t)len + page_mask) >> a.page_shift); };
     if (tid == 0) s.give = s.cuts = s.rows = 0;
-    const int n_free = *a.n_free;
+    // Every load that waits for nothing first.
+    const int n_free = *a.n_free, mine = min(unit / a.heads, n - 1), evicted = a.w.evicted[mine];
+    const Cut cut = cut_of(a, mine);
     __syncthreads();
     // All or nothing: every CTA looks at all requests.
     const int per = (n + kThreads - 1) / kThreads, r0 = min(n, tid * per), r1 = min(n, r0 + per);
@@ -348,25 +369,32 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
     const bool ok = !bad && n_free >= 0 && (int64_t)n_free + s.give <= a.free_capacity;
 
     if (unit < n * a.heads) {
-        const Cut cut = cut_of(a, unit / a.heads);
         if (ok && cut.keep < cut.len) {
-            choose<kThreads, kCluster>(a, s, ranks, unit, cut, rank, ctas);
+            choose<kThreads, kCluster>(a, s, ranks, unit, cut, evicted, rank, ctas);
         } else {
             int32_t* take = a.take + (int64_t)unit * a.max_keep;
             for (int i = (int)rank * kThreads + tid; i < a.max_keep; i += (int)ctas * kThreads) take[i] = -1;
         }
     } else if (rank == 0) {
         // Pages that each thread's requests give, and what those before them give.
-        const int lane = tid & 31, warp = tid >> 5, mine = ok ? (int)give : 0, in_warp = warp_before(mine);
-        if (lane == 31) s.warp_sum[warp] = in_warp + mine;
+        const int lane = tid & 31, warp = tid >> 5, gives = ok ? (int)give : 0, in_warp = warp_before(gives);
+        if (lane == 31) s.warp_sum[warp] = in_warp + gives;
         __syncthreads();
         int at = in_warp + __reduce_add_sync(0xffffffffu, lane < warp ? s.warp_sum[lane] : 0), cuts = 0, rows = 0;
-        for (int r = r0; r < r1 && ok; ++r) {
-            const Cut c = cut_of(a, r);
+        for (int i = 0; i < per && ok; ++i) {
+            const int r = r0 + i;
+            const Cut c = r < r1 ? cut_of(a, r) : Cut{0, 0};
             cuts += c.keep < c.len;
             rows += c.len - c.keep;
-            const int32_t* row = a.block_table + r * a.table_stride;
-            for (int j = pages_of(c.keep); j < pages_of(c.len); ++j) a.free_pages[n_free + at++] = row[j];
+            // A request's pages by the whole warp, one lane's request after another's.
+            const int from = pages_of(c.keep), n_pages = pages_of(c.len) - from;
+            for (uint32_t left = __ballot_sync(0xffffffffu, n_pages > 0); left; left &= left - 1) {
+                const int who = __ffs(left) - 1, w_at = __shfl_sync(0xffffffffu, at, who);
+                const int w_n = __shfl_sync(0xffffffffu, n_pages, who), w_from = __shfl_sync(0xffffffffu, from, who);
+                const int32_t* row = a.block_table + __shfl_sync(0xffffffffu, r, who) * a.table_stride + w_from;
+                for (int j = lane; j < w_n; j += 32) a.free_pages[n_free + w_at + j] = row[j];
+            }
+            at += n_pages;
         }
         atomicAdd(&s.cuts, cuts);
         atomicAdd(&s.rows, rows);
