@@ -24,10 +24,16 @@
 //
 // Warps of weigh_kernel (one CTA per SM; shares of even cost, from the lengths in device
 // memory, which every CTA sums itself):
-//   0-7    a thread a row (rows) or a key and half of the columns (keys)
-//   8-11   codes (TMA, 64 keys at a time) to FP16 operands
-//   12     MMA issuer, two tiles of accumulators in TMEM
-//   13, 14 loaders of codes and of queries
+//   0-3, 4-7  a thread a row (rows: of M tile 0, 1) or a key (keys: the first and the second
+//             half of the columns)
+//   8-11      codes to FP16: to the B operand in shared memory (rows), or a thread a key to
+//             the A operand in TMEM (keys)
+//   12        MMA issuer
+//   13, 14    loaders of codes and of queries
+// The A operand is in TMEM in both passes -- the unit's queries, written by the rows'
+// threads, or the tile's keys -- because two operands of 128 x 16 in shared memory are
+// read at half the rate of the products; so are the operands' other users, 1700 of a
+// tile's cycles in all.
 #include "gqa_internal.h"
 #include "gqa_paged.cuh"
 #include "gqa_paged_internal.h"
@@ -87,26 +93,36 @@ __global__ void __launch_bounds__(kScoreThreads) score_weights_kernel(const __gr
 constexpr int kTokens = 64;                        // queries of a unit
 constexpr int kRows = kTokens * kGroup;            // its rows
 constexpr int kTile = 128, kTileShift = 7;         // keys
-constexpr int kHalfKeys = 64;                      // of a TMA slot
-constexpr int kRawBytes = kHalfKeys * kHeadDim;
+constexpr int kRawBytes = kTile * kHeadDim;
 constexpr int kBlockBytes = kTile * 128;           // 64 dims of a tile in FP16
 constexpr int kTileBytes = 2 * kBlockBytes;
 constexpr int kQBlockBytes = kRows * 128;          // 64 dims of a part of the rows
 constexpr int kQBytes = 4 * kQBlockBytes;          // [part][64 dims][row]
-constexpr int kRaw = 3, kConv = 2, kScaleSlots = 8;
+constexpr int kScaleSlots = 16;
 constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kQueryWarp = 14;
 constexpr int kThreads = 16 * 32, kSumThreads = 8 * 32;
-constexpr uint32_t kTmemCols = 512;                // two tiles of 256 columns
+// TMEM.  Rows: S of each M tile, then its queries' two parts.  Keys: three S of up to 128 columns, two tiles of keys.
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColQ = 256, kColK = 384;
+constexpr int kSums = 3;  // S of the keys' pass
 // What a unit costs beside its tiles when the shares of the rows' pass are cut, in tiles.
 constexpr int kUnitCost = 2;
-constexpr float kHeadroom = 8.f;                   // log2 by which a maximum may pass the reference
+// The rows' reference is the largest of the first keys; a sum of weights past 2^kOverflow moves it.
+constexpr float kOverflow = 0x1p90f;
+
+// Shared memory of a pass: rings of codes and of FP16 tiles, or of codes beside the queries.
+template <bool kKeys>
+struct Rings {
+    static constexpr int kRaw = kKeys ? 4 : 3, kConv = kKeys ? 2 : 4;
+    static constexpr int kBytes = kRaw * kRawBytes + (kKeys ? kQBytes : kConv * kTileBytes);
+};
 
 // kind::f16, FP16 A and B (both K-major), FP32 accumulators, M = 128.
 constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 4) << 24);
 __device__ __forceinline__ constexpr uint32_t idesc_n(uint32_t n) { return kIdesc | ((n >> 3) << 17); }
 
 struct alignas(64) WeighArgs {
-    CUtensorMap kmap;  // (128, page_len, heads, pages) bytes, box (128, min(page_len, 64), 1, 1)
+    CUtensorMap kmap;  // (128, page_len, heads, pages) bytes, box (128, page_len, 1, 1)
     PagedCall p;
     RopeSteps rope;
     KeyWeightsView w;
@@ -279,12 +295,12 @@ private:
 };
 
 struct alignas(16) Shared {
-    uint64_t raw_full[kRaw], raw_empty[kRaw], conv_full[kConv], conv_empty[kConv];
-    uint64_t q_full, q_empty, s_full[2], s_empty[2];
+    uint64_t raw_full[4], raw_empty[4], conv_full[4], conv_empty[4];
+    uint64_t q_full[2], q_empty, s_full[4], s_empty[kSums], half_full[2];  // s_full, keys: [half][tile % 2]
     uint64_t drain;  // products in flight when the issuer gives up
     float scales[kScaleSlots][8];
-    float4 columns[2][kRows / 2];  // keys: factors and -log2 of two columns, of a run and the next
-    float half[2][kTile];          // keys: the second half of the columns' sums
+    float4 columns[2][2][kRows / 4];  // keys: factors and -log2 of two columns, of a half's run and the next
+    float half[2][kTile];             // keys: the second half of the columns' sums
     long long warp_sum[kThreads / 32];
     long long start_base;
     int start_b;
@@ -402,12 +418,14 @@ __device__ __forceinline__ void bulk_load_queries(void* dst, const void* src, ui
 
 template <int kCode, bool kCap, bool kKeys>
 __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constant__ WeighArgs a) {
+    using R = Rings<kKeys>;
+    constexpr int kRaw = R::kRaw, kConv = R::kConv;
     extern __shared__ uint8_t raw_smem[];
     uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
-    uint8_t* q_smem = smem;
-    uint8_t* conv = q_smem + kQBytes;
-    uint8_t* raw = conv + kConv * kTileBytes;
-    Shared& s = *reinterpret_cast<Shared*>(raw + kRaw * kRawBytes);
+    uint8_t* raw = smem;
+    uint8_t* conv = raw + kRaw * kRawBytes;    // rows: the tiles in FP16
+    uint8_t* q_smem = raw + kRaw * kRawBytes;  // keys: the unit's queries
+    Shared& s = *reinterpret_cast<Shared*>(smem + R::kBytes);
     const PagedCall& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = p.c.kv_heads;
 
@@ -417,14 +435,15 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
             mbar_init(&s.raw_empty[i], 4);
         }
         for (int i = 0; i < kConv; ++i) {
-            mbar_init(&s.conv_full[i], 8);
+            mbar_init(&s.conv_full[i], 4);
             mbar_init(&s.conv_empty[i], 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(&s.s_full[i], 1);
+        for (int i = 0; i < kSums; ++i) mbar_init(&s.s_empty[i], 4);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.s_empty[i], kSumThreads / 32);
+            mbar_init(&s.q_full[i], kKeys ? 1 : 4);
+            mbar_init(&s.half_full[i], 4);
         }
-        mbar_init(&s.q_full, 1);
         mbar_init(&s.q_empty, 1);
         mbar_init(&s.drain, 1);
         fence_barrier_init();
@@ -486,24 +505,14 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     if (warp < kConvWarp) {
         // ============================ sums ============================
         const int g = warp >> 2, r = tid & (kTile - 1);
-        const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float cap2 = p.cap * 1.4426950408889634f;
-        int buf = 0, phase = 0, slot = 0, runs = 0;
-        auto wait_tile = [&] {
-            if (ok) ok = warp_wait(&s.s_full[buf], phase);
-            tc_fence_after();
-        };
-        auto free_tile = [&] {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.s_empty[buf]);
-            slot = (slot + 1) & (kScaleSlots - 1);
-            if (++buf == 2) {
-                buf = 0;
-                phase ^= 1;
-            }
-        };
+        int slot = 0;  // scales of the tile
+        auto next_slot = [&] { slot = (slot + 1) & (kScaleSlots - 1); };
         if constexpr (!kKeys) {
+            // A thread a row of M tile g, whose S and queries no other four warps use.
+            const uint32_t t_s = tmem + lanes + g * kTile, t_q = tmem + lanes + kColQ + g * kTile;
+            int phase = 0;
             while (walk.count > 0) {
                 const int n = walk.queries(), token = 32 * g + (r >> 2);
                 const bool active = n > 32 * g, real = token < n;
@@ -511,52 +520,86 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 const float factor = real ? a.factor[cell * kRows + g * kTile + r] : 0.f;
                 const int hi = real ? (int)min((int64_t)walk.pos() + token + 1, (int64_t)walk.q.len) : 0x7fffffff;
                 float ref = -INFINITY, l = 0.f;
-                for (int t = 0; t < walk.count; ++t) {
-                    wait_tile();
-                    if (active) {
-                        const int k0 = (walk.tile0 + t) << kTileShift;
-                        const bool edge = __any_sync(0xffffffffu, hi < k0 + kTile);
-                        const uint32_t cols = t_s + buf * 256 + g * kTile;
-                        float v[2][32];
-                        tmem_ld32(cols, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                if (active) {
+                    // The row's queries to TMEM (the products that read the last ones were waited for).
+                    const uint8_t* src = a.queries + cell * kQBytes + (g * kTile + r) * 128;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float(&z)[32] = v[c & 1];
-                            tmem_wait_ld();
-                            if (c < 3) tmem_ld32(cols + 32 * (c + 1), reinterpret_cast<uint32_t(&)[32]>(v[(c + 1) & 1]));
-                            const float f0 = factor * s.scales[slot][2 * c], f1 = factor * s.scales[slot][2 * c + 1];
+                    for (int b = 0; b < 4; ++b) {
+                        uint32_t w[32];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const float f = e < 16 ? f0 : f1;
-                                const float2 x = __fmul2_rn(make_float2(z[e], z[e + 1]), make_float2(f, f));
-                                z[e] = x.x;
-                                z[e + 1] = x.y;
-                            }
-                            if constexpr (kCap) cap_scores(z, cap2);
-                            if (edge) {
-                                const int left = hi - k0 - 32 * c;
+                        for (int c = 0; c < 8; ++c)
+                            reinterpret_cast<uint4*>(w)[c] =
+                                real ? *reinterpret_cast<const uint4*>(src + b * kQBlockBytes + ((c ^ (r & 7)) << 4))
+                                     : make_uint4(0u, 0u, 0u, 0u);
+                        tmem_st32(t_q + 32 * b, w);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s.q_full[g]);
+                }
+                for (int t = 0; t < walk.count; ++t, next_slot()) {
+                    if (!active) continue;
+                    if (ok) ok = warp_wait(&s.s_full[g], phase);
+                    phase ^= 1;
+                    tc_fence_after();
+                    const int k0 = (walk.tile0 + t) << kTileShift;
+                    const bool edge = __any_sync(0xffffffffu, hi < k0 + kTile);
+                    float v[2][32];
+                    tmem_ld32(t_s, reinterpret_cast<uint32_t(&)[32]>(v[0]));
 #pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (e >= left) z[e] = -INFINITY;
-                            }
-                            float mx = fmaxf(z[0], z[1]);
+                    for (int c = 0; c < 4; ++c) {
+                        float(&z)[32] = v[c & 1];
+                        tmem_wait_ld();
+                        if (c < 3) {
+                            tmem_ld32(t_s + 32 * (c + 1), reinterpret_cast<uint32_t(&)[32]>(v[(c + 1) & 1]));
+                        } else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&s.s_empty[g]);
+                        }
+                        float f0 = factor * s.scales[slot][2 * c], f1 = factor * s.scales[slot][2 * c + 1];
+                        if (kCap || edge) {  // scaled before the mask: -inf times a scale of 0 is none
 #pragma unroll
-                            for (int e = 2; e < 32; e += 2) mx = fmaxf(fmaxf(mx, z[e]), z[e + 1]);
-                            if (mx > ref + kHeadroom) {  // (at once from nothing)
-                                l *= fast_exp2(ref - mx);
-                                ref = mx;
-                            }
-                            const float use = ref == -INFINITY ? 0.f : ref;
+                            for (int e = 0; e < 32; ++e) z[e] *= e < 16 ? f0 : f1;
+                            f0 = f1 = 1.f;
+                        }
+                        if constexpr (kCap) {
+                            cap_scores(reinterpret_cast<float(&)[16]>(z[0]), cap2);
+                            cap_scores(reinterpret_cast<float(&)[16]>(z[16]), cap2);
+                        }
+                        if (edge) {
+                            const int left = hi - k0 - 32 * c;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (e >= left) z[e] = -INFINITY;
+                        }
+                        // Sum of 2^(z - ref) over the chunk, z times its factor.
+                        auto chunk = [&](float use) {
                             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
-                                const float2 x = __fadd2_rn(make_float2(z[e], z[e + 1]), make_float2(-use, -use));
+                                const float f = e < 16 ? f0 : f1;
+                                float2 x = make_float2(z[e], z[e + 1]);
+                                x = kCap ? __fadd2_rn(x, make_float2(-use, -use))
+                                         : __ffma2_rn(x, make_float2(f, f), make_float2(-use, -use));
                                 sum = __fadd2_rn(sum, make_float2(fast_exp2(x.x), fast_exp2(x.y)));
                             }
-                            l += sum.x + sum.y;
+                            return sum.x + sum.y;
+                        };
+                        float sum = ref == -INFINITY ? INFINITY : chunk(ref);
+                        if (!(sum < kOverflow)) {  // the row's first keys, or larger ones by far
+                            float mx = -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, z[e] * (e < 16 ? f0 : f1));
+                            const float now = fmaxf(ref, mx);
+                            l *= fast_exp2(ref - (now == -INFINITY ? 0.f : now));
+                            ref = now;
+                            sum = chunk(now == -INFINITY ? 0.f : now);
                         }
+                        l += sum;
+                        __syncwarp();
                     }
-                    free_tile();
                 }
                 // ---- the run's rows ----
                 const int tiles = walk.q.unit_tiles(walk.u);
@@ -600,34 +643,35 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 if (!walk.next()) break;
             }
         } else {
-            int tiles = 0;
+            // A thread a key and half g of the columns; S of a tile's halves follow one another.
+            // (A half has full barriers of its own: a wait by parity tells only one phase from the next.)
+            int buf = g, tiles = 0, runs = 0;
             while (walk.count > 0) {
-                const int n = walk.queries(), columns = columns_of(n), half = columns >> 1;
+                const int n = walk.queries(), half = columns_of(n) >> 1;
                 const int64_t cell = (int64_t)walk.id() * heads + walk.h;
-                {
-                    float* to = reinterpret_cast<float*>(s.columns[runs & 1]) + (tid >> 1) * 4 + (tid & 1);
-                    if (tid < columns) {
-                        to[0] = a.factor[cell * kRows + tid];
-                        to[2] = -a.row_log2[cell * kRows + tid];
-                    }
-                    sums_sync();
-                }
-                const float4* column = s.columns[runs & 1] + g * (half >> 1);
+                float4* column = s.columns[g][runs & 1];
                 ++runs;
+                if (r < half) {
+                    float* to = reinterpret_cast<float*>(column) + (r >> 1) * 4 + (r & 1);
+                    to[0] = a.factor[cell * kRows + g * half + r];
+                    to[2] = -a.row_log2[cell * kRows + g * half + r];
+                }
+                named_barrier_sync(2 + g, kTile);
                 const int known = known_of(a.known, walk.b, walk.q);
                 const int evicted = known > 0 ? paged_evicted(p, walk.b) : 0;
                 const int64_t at = ((int64_t)walk.b * heads + walk.h) * a.w.capacity;
-                for (int t = 0; t < walk.count; ++t, ++tiles) {
+                for (int t = 0; t < walk.count; ++t, ++tiles, next_slot()) {
                     const int tile = walk.tile0 + t, key = (tile << kTileShift) + r;
                     const bool fresh = walk.u == walk.q.first_unit(tile), held = g == 0 && key < walk.q.len;
                     float weight = 0.f;
                     if (held && (!fresh || key < known)) weight = a.w.weight[at + key];
-                    wait_tile();
+                    if (ok) ok = warp_wait(&s.s_full[2 * g + (tiles & 1)], (tiles >> 1) & 1);
+                    tc_fence_after();
                     // Rows that see the key: from this column on.
                     const int from_col = (key - walk.pos()) * kGroup - g * half;
                     const bool edge = __any_sync(0xffffffffu, from_col > 0);
                     const float ks = s.scales[slot][r >> 4];
-                    const uint32_t cols = t_s + buf * 256 + g * half;
+                    const uint32_t cols = tmem + lanes + buf * kTile;
                     float2 sum = make_float2(0.f, 0.f);
                     auto add = [&](float (&v)[16], int c) {
                         float2 off[8];
@@ -660,26 +704,38 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                             sum = __fadd2_rn(sum, make_float2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
                     };
                     const int steps = half >> 4;
+                    auto free_sums = [&] {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+                    };
                     float x[16], y[16];
                     tmem_ld16(cols, reinterpret_cast<uint32_t(&)[16]>(x));
                     for (int c = 0; c < steps; c += 2) {
                         tmem_wait_ld();
-                        if (c + 1 < steps) tmem_ld16(cols + 16 * (c + 1), reinterpret_cast<uint32_t(&)[16]>(y));
+                        if (c + 1 < steps) tmem_ld16(cols + 16 * (c + 1), reinterpret_cast<uint32_t(&)[16]>(y)); else free_sums();
                         add(x, c);
                         if (c + 1 < steps) {
                             tmem_wait_ld();
-                            if (c + 2 < steps) tmem_ld16(cols + 16 * (c + 2), reinterpret_cast<uint32_t(&)[16]>(x));
+                            if (c + 2 < steps) tmem_ld16(cols + 16 * (c + 2), reinterpret_cast<uint32_t(&)[16]>(x)); else free_sums();
                             add(y, c + 1);
                         }
                     }
-                    free_tile();
+                    buf += 2;  // (the other half's S lies between)
+                    if (buf >= kSums) buf -= kSums;
                     const float mine = sum.x + sum.y;
-                    if (g) s.half[tiles & 1][r] = mine;
-                    sums_sync();
-                    if (held) {
-                        a.w.weight[at + key] = weight + (mine + s.half[tiles & 1][r]);
-                        if (fresh && key >= known) a.w.position[at + key] = key + evicted;
-                        if (fresh && key == 0 && known <= 0 && walk.h == 0) a.w.evicted[walk.b] = 0;
+                    if (g) {
+                        // (The first half is at most a tile behind: S of this tile could not have been written before.)
+                        s.half[tiles & 1][r] = mine;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&s.half_full[tiles & 1]);
+                    } else {
+                        if (ok) ok = warp_wait(&s.half_full[tiles & 1], (tiles >> 1) & 1);
+                        if (held) {
+                            a.w.weight[at + key] = weight + (mine + s.half[tiles & 1][r]);
+                            if (fresh && key >= known) a.w.position[at + key] = key + evicted;
+                            if (fresh && key == 0 && known <= 0 && walk.h == 0) a.w.evicted[walk.b] = 0;
+                        }
                     }
                 }
                 if (!walk.next()) break;
@@ -688,22 +744,42 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     } else if (warp < kMmaWarp) {
         // ============================ conversion ============================
         const int cw = warp - kConvWarp, t = lane & 3;
-        // As in the chunked attention kernel: eight lanes that access shared memory together have all eight 16-byte
-        // columns of the codes' rows and of the operand's.
-        const int row0 = 16 * cw + ((lane >> 3) ^ (lane & 4 ? 5 : 0));
+        // Rows: as in the chunked attention kernel, eight lanes that access shared memory together have all eight
+        // 16-byte columns of the codes' rows and of the operand's.  Keys: a lane a key, whose eight neighbours' rows
+        // hold a chunk in eight different columns.
+        const int row0 = 32 * cw + ((lane >> 3) ^ (lane & 4 ? 5 : 0)), key = 32 * cw + lane;
         int rs = 0, rphase = 0, cs = 0, cphase = 0, items = 0;
         while (walk.count > 0 && ok) {
             for (int j = 0; j < walk.count && ok; ++j, ++items) {
-                uint8_t* dst = conv + cs * kTileBytes;
-                for (int part = 0; part < 2; ++part) {
-                    ok = mbar_wait(&s.raw_full[rs], rphase) &&
-                         (part || items < kConv || mbar_wait(&s.conv_empty[cs], cphase ^ 1));
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const uint8_t* src = raw + rs * kRawBytes;
+                ok = mbar_wait(&s.raw_full[rs], rphase) && (items < kConv || mbar_wait(&s.conv_empty[cs], cphase ^ 1));
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint8_t* src = raw + rs * kRawBytes;
+                if constexpr (kKeys) {
+                    uint32_t w[64];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int row = row0 + 8 * i, sw = row & 7, to = row + kHalfKeys * part;
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 x = lds128(src + key * kHeadDim + ((c ^ (key & 7)) << 4));
+                        to_half4<kCode>(x.x, w[8 * c], w[8 * c + 1]);
+                        to_half4<kCode>(x.y, w[8 * c + 2], w[8 * c + 3]);
+                        to_half4<kCode>(x.z, w[8 * c + 4], w[8 * c + 5]);
+                        to_half4<kCode>(x.w, w[8 * c + 6], w[8 * c + 7]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s.raw_empty[rs]);
+                    tc_fence_after();  // the products that read this tile's place are done
+                    const uint32_t to = tmem + ((uint32_t)(32 * cw) << 16) + kColK + cs * 64;
+                    tmem_st32(to, reinterpret_cast<const uint32_t(&)[32]>(w[0]));
+                    tmem_st32(to + 32, reinterpret_cast<const uint32_t(&)[32]>(w[32]));
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s.conv_full[cs]);
+                } else {
+                    uint8_t* dst = conv + cs * kTileBytes;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = row0 + 8 * i, sw = row & 7;
 #pragma unroll
                         for (int block = 0; block < 2; ++block) {
                             const uint4 x = lds128(src + row * kHeadDim + (((4 * block + t) ^ sw) << 4));
@@ -712,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                             to_half4<kCode>(x.y, w[2], w[3]);
                             to_half4<kCode>(x.z, w[4], w[5]);
                             to_half4<kCode>(x.w, w[6], w[7]);
-                            uint8_t* at = dst + block * kBlockBytes + to * 128;
+                            uint8_t* at = dst + block * kBlockBytes + row * 128;
                             *reinterpret_cast<uint4*>(at + (((2 * t) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                             *reinterpret_cast<uint4*>(at + (((2 * t + 1) ^ sw) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
                         }
@@ -723,10 +799,10 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         mbar_arrive(&s.conv_full[cs]);
                         mbar_arrive(&s.raw_empty[rs]);
                     }
-                    if (++rs == kRaw) {
-                        rs = 0;
-                        rphase ^= 1;
-                    }
+                }
+                if (++rs == kRaw) {
+                    rs = 0;
+                    rphase ^= 1;
                 }
                 if (++cs == kConv) {
                     cs = 0;
@@ -738,39 +814,73 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     } else if (warp == kMmaWarp) {
         // ============================ MMA issuer ============================
         const uint32_t leader = elect_lane(), cols = uniform(tmem);
-        int cs = 0, cphase = 0, buf = 0, phase = 0, items = 0, runs = 0;
+        int cs = 0, cphase = 0, runs = 0;
+        int used[2] = {0, 0}, q_runs[2] = {0, 0};  // rows: tiles and runs of each M tile
+        int buf = 0, phase = 0, sums = 0, items = 0;  // keys
+        auto next_tile = [&] {
+            if (++cs == kConv) {
+                cs = 0;
+                cphase ^= 1;
+            }
+        };
         while (uniform(walk.count) > 0 && ok) {
             const int n = uniform(walk.queries()), count = uniform(walk.count);
-            ok = warp_wait(&s.q_full, runs & 1);
-            ++runs;
-            for (int j = 0; j < count && ok; ++j, ++items) {
-                ok = warp_wait(&s.conv_full[cs], cphase) && (items < 2 || warp_wait(&s.s_empty[buf], phase ^ 1));
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t kd = smem_desc_sw128(smem_addr(conv + cs * kTileBytes), 16, 1024);
+            if constexpr (kKeys) {
+                const int half = columns_of(n) >> 1;
+                const uint32_t idesc = idesc_n(half);
+                ok = warp_wait(&s.q_full[0], runs & 1);
+                ++runs;
                 const uint64_t qd = smem_desc_sw128(smem_addr(q_smem), 16, 1024);
-                const int products = kKeys || n <= 32 ? 1 : 2;
-                const uint32_t idesc = idesc_n(kKeys ? columns_of(n) : kTile);
-                for (int m = 0; m < products; ++m)
+                for (int j = 0; j < count && ok; ++j, ++items) {
+                    ok = warp_wait(&s.conv_full[cs], cphase);
+                    for (int h = 0; h < 2 && ok; ++h, ++sums) {
+                        ok = sums < kSums || warp_wait(&s.s_empty[buf], phase ^ 1);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
+                        for (int part = 0; part < 2; ++part)
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            const uint64_t k = kd + (((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4);
-                            const uint64_t q = qd + (((2 * part + (kk >> 2)) * kQBlockBytes + m * kTile * 128 + (kk & 3) * 32) >> 4);
-                            mma_ss_by(leader, cols + buf * 256 + m * kTile, kKeys ? k : q, kKeys ? q : k, idesc,
-                                      part || kk ? 1u : 0u);
+                            for (int kk = 0; kk < 8; ++kk)
+                                mma_ts_by(leader, cols + buf * kTile, cols + kColK + cs * 64 + 8 * kk,
+                                          qd + (((2 * part + (kk >> 2)) * kQBlockBytes + h * half * 128 + (kk & 3) * 32) >> 4),
+                                          idesc, part || kk ? 1u : 0u);
+                        tc_commit_by(leader, &s.s_full[2 * h + (items & 1)]);
+                        if (++buf == kSums) {
+                            buf = 0;
+                            phase ^= 1;
                         }
-                tc_commit_by(leader, &s.s_full[buf]);
-                tc_commit_by(leader, &s.conv_empty[cs]);
-                if (j + 1 == count) tc_commit_by(leader, &s.q_empty);
-                if (++cs == kConv) {
-                    cs = 0;
-                    cphase ^= 1;
+                    }
+                    if (!ok) break;
+                    tc_commit_by(leader, &s.conv_empty[cs]);
+                    if (j + 1 == count) tc_commit_by(leader, &s.q_empty);
+                    next_tile();
                 }
-                if (++buf == 2) {
-                    buf = 0;
-                    phase ^= 1;
+            } else {
+                const int products = n <= 32 ? 1 : 2;
+                for (int j = 0; j < count && ok; ++j) {
+                    ok = warp_wait(&s.conv_full[cs], cphase);
+                    const uint64_t kd = smem_desc_sw128(smem_addr(conv + cs * kTileBytes), 16, 1024);
+                    for (int m = 0; m < products && ok; ++m) {
+                        if (j == 0) {
+                            ok = warp_wait(&s.q_full[m], q_runs[m] & 1);
+                            ++q_runs[m];
+                        }
+                        ok = ok && (used[m] == 0 || warp_wait(&s.s_empty[m], (used[m] - 1) & 1));
+                        if (!ok) break;
+                        ++used[m];
+                        tc_fence_after();
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk)
+                                mma_ts_by(leader, cols + m * kTile, cols + kColQ + m * kTile + 64 * part + 8 * kk,
+                                          kd + (((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4), idesc_n(kTile),
+                                          part || kk ? 1u : 0u);
+                        tc_commit_by(leader, &s.s_full[m]);
+                    }
+                    if (!ok) break;
+                    tc_commit_by(leader, &s.conv_empty[cs]);
+                    next_tile();
                 }
             }
             if (!ok || !uniform(walk.next())) break;
@@ -782,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     } else if (warp == kLoadWarp) {
         // ============================ codes ============================
         const int shift = p.c.page_shift, per_tile = kTile >> shift;  // pages of a tile
-        const int box = min(p.c.page_len, kHalfKeys), box_bytes = box * kHeadDim;
+        const int box_bytes = p.c.page_len * kHeadDim;
         const uint64_t policy = l2_evict_first_policy();
         int rs = 0, rphase = 0, items = 0, slot = 0;
         while (walk.count > 0 && ok) {
@@ -800,32 +910,23 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
             };
             int page = entry(0), page1 = entry(1);
             float ks = scale(page);
-            for (int j = 0; j < walk.count && ok; ++j) {
+            for (int j = 0; j < walk.count; ++j, ++items) {
                 const int page2 = entry(j + 2);
                 const float ks1 = scale(page1);
-                for (int part = 0; part < 2; ++part, ++items) {
-                    if (items >= kRaw) ok = __all_sync(0xffffffffu, mbar_wait(&s.raw_empty[rs], rphase ^ 1));
-                    if (!ok) break;
-                    if (part == 0) {
-                        const float x = __shfl_sync(0xffffffffu, ks, (lane & 7) >> (shift - 4));  // a lane 16 keys
-                        if (lane < 8) s.scales[slot][lane] = x;
-                        __syncwarp();
-                        slot = (slot + 1) & (kScaleSlots - 1);
-                    }
-                    // This half's pages: a page of 128 keys has a box in each.
-                    const bool mine = page >= 0 && (shift == kTileShift || (lane << shift) / kHalfKeys == part) &&
-                                      ((int64_t)(walk.tile0 + j) << kTileShift) + part * kHalfKeys < hi;
-                    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-                    if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[rs], boxes * box_bytes);
-                    __syncwarp();
-                    if (mine)
-                        tma_load_page(raw + rs * kRawBytes + (shift == kTileShift ? 0 : (lane << shift) % kHalfKeys) * kHeadDim,
-                                      &a.kmap, shift == kTileShift ? part * kHalfKeys : 0, walk.h, page, &s.raw_full[rs],
-                                      policy);
-                    if (++rs == kRaw) {
-                        rs = 0;
-                        rphase ^= 1;
-                    }
+                if (items >= kRaw) ok = __all_sync(0xffffffffu, mbar_wait(&s.raw_empty[rs], rphase ^ 1));
+                if (!ok) break;
+                const float x = __shfl_sync(0xffffffffu, ks, (lane & 7) >> (shift - 4));  // a lane 16 keys
+                if (lane < 8) s.scales[slot][lane] = x;
+                __syncwarp();
+                slot = (slot + 1) & (kScaleSlots - 1);
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[rs], boxes * box_bytes);
+                __syncwarp();
+                if (page >= 0)
+                    tma_load_page(raw + rs * kRawBytes + lane * box_bytes, &a.kmap, 0, walk.h, page, &s.raw_full[rs], policy);
+                if (++rs == kRaw) {
+                    rs = 0;
+                    rphase ^= 1;
                 }
                 page = page1;
                 page1 = page2;
@@ -838,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 const int at = rs - i;
                 mbar_wait(&s.raw_full[at < 0 ? at + kRaw : at], at < 0 ? rphase ^ 1 : rphase);
             }
-    } else if (warp == kQueryWarp) {
+    } else if (kKeys && warp == kQueryWarp) {
         // ============================ queries ============================
         int runs = 0;
         while (walk.count > 0) {
@@ -846,15 +947,15 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 ok = false;  // (the last copies have landed: their products were waited for)
                 break;
             }
-            const uint32_t bytes = (walk.queries() > 32 ? kRows : kTile) * 128;
+            const uint32_t bytes = columns_of(walk.queries()) * 128;
             const uint8_t* src = a.queries + ((int64_t)walk.id() * heads + walk.h) * kQBytes;
-            if (lane == 0) mbar_arrive_expect_tx(&s.q_full, 4 * bytes);
+            if (lane == 0) mbar_arrive_expect_tx(&s.q_full[0], 4 * bytes);
             __syncwarp();
-            if (lane < 4) bulk_load_queries(q_smem + lane * kQBlockBytes, src + lane * kQBlockBytes, bytes, &s.q_full);
+            if (lane < 4) bulk_load_queries(q_smem + lane * kQBlockBytes, src + lane * kQBlockBytes, bytes, &s.q_full[0]);
             ++runs;
             if (!walk.next()) break;
         }
-        if (runs > 0) warp_wait(&s.q_full, (runs - 1) & 1);  // no copy in flight when the CTA leaves
+        if (runs > 0) warp_wait(&s.q_full[0], (runs - 1) & 1);  // no copy in flight when the CTA leaves
     }
     if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
 
@@ -866,8 +967,9 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     }
 }
 
-constexpr int kSmemBytes = 1024 + kQBytes + kConv * kTileBytes + kRaw * kRawBytes + (int)sizeof(Shared);
-static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+template <bool kKeys>
+constexpr int kSmemBytes = 1024 + Rings<kKeys>::kBytes + (int)sizeof(Shared);
+static_assert(kSmemBytes<false> <= 227 * 1024 && kSmemBytes<true> <= 227 * 1024, "shared memory of one CTA");
 
 using Kernel = void (*)(WeighArgs);
 
@@ -897,14 +999,15 @@ Regions regions(int batch, int rows, int heads, int sms) {
 
 }  // namespace
 
-int paged_weigh_box() { return kHalfKeys; }
+int paged_weigh_box() { return kTile; }
 
 size_t paged_weigh_workspace(int batch, int rows, int heads, int sms) { return regions(batch, rows, heads, sms).end; }
 
 cudaError_t paged_weigh_prepare() {
     for (int i = 0; i < 8; ++i) {
         const cudaError_t e = cudaFuncSetAttribute(i & 4 ? kernel_for<true>(i & 1, i & 2) : kernel_for<false>(i & 1, i & 2),
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   i & 4 ? kSmemBytes<true> : kSmemBytes<false>);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -940,9 +1043,9 @@ cudaError_t launch_paged_weigh(const PagedCall& call, const RopeSteps& rope, int
     const PrepArgs prep{call, rope, known, a.queries, a.factor, a.arrivals};
     cudaError_t e = launch_dependent(weigh_queries_kernel, dim3(a.max_units, call.c.kv_heads), kSumThreads, 0, stream, prep);
     if (e == cudaSuccess)
-        e = launch_dependent(kernel_for<false>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes, stream, a);
+        e = launch_dependent(kernel_for<false>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes<false>, stream, a);
     if (e == cudaSuccess)
-        e = launch_dependent(kernel_for<true>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes, stream, a);
+        e = launch_dependent(kernel_for<true>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes<true>, stream, a);
     return e;
 }
 
