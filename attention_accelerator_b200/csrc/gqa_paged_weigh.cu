@@ -24,12 +24,12 @@
 //
 // Warps of weigh_kernel (one CTA per SM; shares of even cost, from the lengths in device
 // memory, which every CTA sums itself):
-//   0-3, 4-7  a thread a row (rows: of M tile 0, 1) or a key (keys: the first and the second
-//             half of the columns)
-//   8-11      codes to FP16: to the B operand in shared memory (rows), or a thread a key to
+//   0-15      sums, four groups of four: a thread a row and half of the tile's keys (rows: two
+//             groups each M tile), or a key and a quarter of the columns (keys)
+//   16-19     codes to FP16: to the B operand in shared memory (rows), or a thread a key to
 //             the A operand in TMEM (keys)
-//   12        MMA issuer
-//   13, 14    loaders of codes and of queries
+//   20        MMA issuer
+//   21, 22    loaders of codes and of queries
 // The A operand is in TMEM in both passes -- the unit's queries, written by the rows'
 // threads, or the tile's keys -- because two operands of 128 x 16 in shared memory are
 // read at half the rate of the products; so are the operands' other users, 1700 of a
@@ -99,12 +99,16 @@ constexpr int kTileBytes = 2 * kBlockBytes;
 constexpr int kQBlockBytes = kRows * 128;          // 64 dims of a part of the rows
 constexpr int kQBytes = 4 * kQBlockBytes;          // [part][64 dims][row]
 constexpr int kScaleSlots = 16;
-constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kQueryWarp = 14;
-constexpr int kThreads = 16 * 32, kSumThreads = 8 * 32;
+constexpr int kConvWarp = 16, kMmaWarp = 20, kLoadWarp = 21, kQueryWarp = 22;
+constexpr int kThreads = 24 * 32, kPrepThreads = 8 * 32;
+// Registers: launched with 80 a thread; each group of four warps takes its share.
+constexpr int kLaunchRegs = 80, kSumRegs = 88, kConvRegs = 64, kRestRegs = 64;
+static_assert(4 * kSumRegs + kConvRegs + kRestRegs <= 6 * kLaunchRegs, "of what the CTA was launched with");
 // TMEM.  Rows: S of each M tile, then its queries' two parts.  Keys: three S of up to 128 columns, two tiles of keys.
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColQ = 256, kColK = 384;
 constexpr int kSums = 3;  // S of the keys' pass
+constexpr int kParts = 4; // tiles whose quarters' sums wait to be joined
 // What a unit costs beside its tiles when the shares of the rows' pass are cut, in tiles.
 constexpr int kUnitCost = 2;
 // The rows' reference is the largest of the first keys; a sum of weights past 2^kOverflow moves it.
@@ -296,11 +300,13 @@ private:
 
 struct alignas(16) Shared {
     uint64_t raw_full[4], raw_empty[4], conv_full[4], conv_empty[4];
-    uint64_t q_full[2], q_empty, s_full[4], s_empty[kSums], half_full[2];  // s_full, keys: [half][tile % 2]
+    uint64_t q_full[2], q_empty, s_full[4], s_empty[kSums];  // s_full, keys: [half][tile % 2]
+    uint64_t part_full[kParts];
     uint64_t drain;  // products in flight when the issuer gives up
     float scales[kScaleSlots][8];
-    float4 columns[2][2][kRows / 4];  // keys: factors and -log2 of two columns, of a half's run and the next
-    float half[2][kTile];             // keys: the second half of the columns' sums
+    float4 columns[4][2][kRows / 8];  // keys: factors and -log2 of two columns, of a quarter's run and the next
+    float part[kParts][3][kTile];     // keys: sums of the quarters but the first
+    float2 other[2][2][kTile];        // rows: references and sums of the second half of the keys
     long long warp_sum[kThreads / 32];
     long long start_base;
     int start_b;
@@ -323,7 +329,7 @@ __device__ __forceinline__ uint32_t bf16_magnitudes(uint32_t w) { return max(w <
 // A sequence without rows before these is a new one: nothing was evicted from it.
 __device__ __forceinline__ int known_of(const int32_t* known, int b, const Seq& q) { return known ? known[b] : q.pos0; }
 
-__global__ void __launch_bounds__(kSumThreads) weigh_queries_kernel(const __grid_constant__ PrepArgs a) {
+__global__ void __launch_bounds__(kPrepThreads) weigh_queries_kernel(const __grid_constant__ PrepArgs a) {
     const PagedCall& p = a.p;
     const int id = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, token = tid >> 2, q4 = tid & 3;
     __shared__ uint64_t step[kPairs];
@@ -343,7 +349,7 @@ __global__ void __launch_bounds__(kSumThreads) weigh_queries_kernel(const __grid
     if (tid == 0) a.arrivals[cell] = 0;
     __syncthreads();
     const int n = min(kTokens, q.n - u * kTokens);
-    if (token >= ((n + 7) & ~7)) return;  // whole steps of 32 rows are read
+    if (token >= ((n + 15) & ~15)) return;  // whole steps of 64 rows are read
     const bool real = token < n;
     const int64_t pos = (int64_t)q.pos0 + u * kTokens + token +
                         (known_of(a.known, lo, q) > 0 ? paged_evicted(p, lo) : 0);
@@ -403,10 +409,8 @@ __global__ void __launch_bounds__(kSumThreads) weigh_queries_kernel(const __grid
     }
 }
 
-__device__ __forceinline__ void sums_sync() { named_barrier_sync(1, kSumThreads); }
-
-// Rows of a unit as the MMA takes them: whole steps of 32 columns.
-__device__ __forceinline__ int columns_of(int n) { return (n * kGroup + 31) & ~31; }
+// Rows of a unit as the MMA takes them: whole steps of 64 columns.
+__device__ __forceinline__ int columns_of(int n) { return (n * kGroup + 63) & ~63; }
 
 // A copy that stays in L2 as others do: the unit's tiles are dealt to several CTAs.
 __device__ __forceinline__ void bulk_load_queries(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -414,6 +418,14 @@ __device__ __forceinline__ void bulk_load_queries(void* dst, const void* src, ui
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)),
         "l"(src), "r"(bytes), "r"(smem_addr(bar))
         : "memory");
+}
+
+template <int kRegs>
+__device__ __forceinline__ void take_registers() {
+    if constexpr (kRegs > kLaunchRegs)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+    else
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 template <int kCode, bool kCap, bool kKeys>
@@ -439,11 +451,9 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
             mbar_init(&s.conv_empty[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&s.s_full[i], 1);
-        for (int i = 0; i < kSums; ++i) mbar_init(&s.s_empty[i], 4);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&s.q_full[i], kKeys ? 1 : 4);
-            mbar_init(&s.half_full[i], 4);
-        }
+        for (int i = 0; i < kSums; ++i) mbar_init(&s.s_empty[i], 8);
+        for (int i = 0; i < kParts; ++i) mbar_init(&s.part_full[i], 12);
+        for (int i = 0; i < 2; ++i) mbar_init(&s.q_full[i], kKeys ? 1 : 8);
         mbar_init(&s.q_empty, 1);
         mbar_init(&s.drain, 1);
         fence_barrier_init();
@@ -504,15 +514,16 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
 
     if (warp < kConvWarp) {
         // ============================ sums ============================
-        const int g = warp >> 2, r = tid & (kTile - 1);
+        take_registers<kSumRegs>();
+        const int g = warp >> 3, part = warp >> 2 & 1, r = tid & (kTile - 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float cap2 = p.cap * 1.4426950408889634f;
         int slot = 0;  // scales of the tile
         auto next_slot = [&] { slot = (slot + 1) & (kScaleSlots - 1); };
         if constexpr (!kKeys) {
-            // A thread a row of M tile g, whose S and queries no other four warps use.
-            const uint32_t t_s = tmem + lanes + g * kTile, t_q = tmem + lanes + kColQ + g * kTile;
-            int phase = 0;
+            // A thread a row of M tile g and half of a tile's keys; S and queries of the M tile are these eight warps'.
+            const uint32_t t_s = tmem + lanes + g * kTile + 64 * part, t_q = tmem + lanes + kColQ + g * kTile + 64 * part;
+            int phase = 0, runs = 0;
             while (walk.count > 0) {
                 const int n = walk.queries(), token = 32 * g + (r >> 2);
                 const bool active = n > 32 * g, real = token < n;
@@ -521,10 +532,10 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 const int hi = real ? (int)min((int64_t)walk.pos() + token + 1, (int64_t)walk.q.len) : 0x7fffffff;
                 float ref = -INFINITY, l = 0.f;
                 if (active) {
-                    // The row's queries to TMEM (the products that read the last ones were waited for).
-                    const uint8_t* src = a.queries + cell * kQBytes + (g * kTile + r) * 128;
+                    // One part of the row's queries to TMEM (the products that read the last ones were waited for).
+                    const uint8_t* src = a.queries + cell * kQBytes + (g * kTile + r) * 128 + 2 * part * kQBlockBytes;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 0; b < 2; ++b) {
                         uint32_t w[32];
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
@@ -543,22 +554,19 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     if (ok) ok = warp_wait(&s.s_full[g], phase);
                     phase ^= 1;
                     tc_fence_after();
-                    const int k0 = (walk.tile0 + t) << kTileShift;
-                    const bool edge = __any_sync(0xffffffffu, hi < k0 + kTile);
-                    float v[2][32];
-                    tmem_ld32(t_s, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                    const int k0 = ((walk.tile0 + t) << kTileShift) + 64 * part;
+                    const bool edge = __any_sync(0xffffffffu, hi < k0 + 64);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float(&z)[32] = v[c & 1];
+                    for (int c = 0; c < 2; ++c) {
+                        float z[32];
+                        tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t(&)[32]>(z));
+                        float f0 = factor * s.scales[slot][4 * part + 2 * c], f1 = factor * s.scales[slot][4 * part + 2 * c + 1];
                         tmem_wait_ld();
-                        if (c < 3) {
-                            tmem_ld32(t_s + 32 * (c + 1), reinterpret_cast<uint32_t(&)[32]>(v[(c + 1) & 1]));
-                        } else {
+                        if (c == 1) {
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&s.s_empty[g]);
                         }
-                        float f0 = factor * s.scales[slot][2 * c], f1 = factor * s.scales[slot][2 * c + 1];
                         if (kCap || edge) {  // scaled before the mask: -inf times a scale of 0 is none
 #pragma unroll
                             for (int e = 0; e < 32; ++e) z[e] *= e < 16 ? f0 : f1;
@@ -576,16 +584,16 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         }
                         // Sum of 2^(z - ref) over the chunk, z times its factor.
                         auto chunk = [&](float use) {
-                            float2 sum = make_float2(0.f, 0.f);
+                            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
                                 const float f = e < 16 ? f0 : f1;
                                 float2 x = make_float2(z[e], z[e + 1]);
                                 x = kCap ? __fadd2_rn(x, make_float2(-use, -use))
                                          : __ffma2_rn(x, make_float2(f, f), make_float2(-use, -use));
-                                sum = __fadd2_rn(sum, make_float2(fast_exp2(x.x), fast_exp2(x.y)));
+                                sum[e >> 1 & 1] = __fadd2_rn(sum[e >> 1 & 1], make_float2(fast_exp2(x.x), fast_exp2(x.y)));
                             }
-                            return sum.x + sum.y;
+                            return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                         };
                         float sum = ref == -INFINITY ? INFINITY : chunk(ref);
                         if (!(sum < kOverflow)) {  // the row's first keys, or larger ones by far
@@ -601,87 +609,102 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         __syncwarp();
                     }
                 }
-                // ---- the run's rows ----
-                const int tiles = walk.q.unit_tiles(walk.u);
-                float* out = a.row_log2 + cell * kRows + g * kTile + r;
-                auto log2_of = [&](float m, float sum) { return !real ? INFINITY : sum == 0.f ? -INFINITY : m + log2f(sum); };
-                if (walk.count == tiles) {
-                    if (active) *out = log2_of(ref, l);
-                } else {
-                    // A piece of a unit.  A share's first piece goes to its slot 0; its last, if another one, to slot
-                    // 1: only the unit's first share can have begun before it.
-                    const int64_t first = walk.cell - walk.tile0;  // the cell of the unit's first tile
-                    auto share_of = [&](int64_t x) { return (int)(((x + 1) * shares + total - 1) / total) - 1; };
-                    const int c0 = share_of(first), parts = share_of(first + tiles - 1) - c0 + 1;
-                    const int second = total * c0 / shares < first - kUnitCost ? 1 : 0;
-                    auto part = [&](int c) {
-                        return a.partials + (int64_t)((c0 + c) * 2 + (c ? 0 : second)) * kRows + g * kTile + r;
-                    };
-                    if (active) *part((int)blockIdx.x - c0) = make_float2(ref, l);
-                    sums_sync();
-                    if (tid == 0) {
-                        uint32_t before;
-                        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
-                                     : "=r"(before)
-                                     : "l"(a.arrivals + cell)
-                                     : "memory");
-                        s.last = before == (uint32_t)(parts - 1);
-                    }
-                    sums_sync();
-                    if (s.last && active) {
-                        float M = -INFINITY, L = 0.f;
-                        for (int c = 0; c < parts; ++c) {
-                            const float2 x = __ldcg(part(c));
-                            const float now = fmaxf(M, x.x), use = now == -INFINITY ? 0.f : now;
-                            L = L * fast_exp2(M - use) + x.y * fast_exp2(x.x - use);
-                            M = now;
+                // ---- the run's rows: both halves of the keys ----
+                float2& other = s.other[runs & 1][g][r];
+                ++runs;
+                if (part) other = make_float2(ref, l);
+                named_barrier_sync(2 + g, 2 * kTile);
+                if (!part) {
+                    const float now = fmaxf(ref, other.x), use = now == -INFINITY ? 0.f : now;
+                    l = l * fast_exp2(ref - use) + other.y * fast_exp2(other.x - use);
+                    ref = now;
+                    const int tiles = walk.q.unit_tiles(walk.u);
+                    float* out = a.row_log2 + cell * kRows + g * kTile + r;
+                    auto log2_of = [&](float m, float sum) { return !real ? INFINITY : sum == 0.f ? -INFINITY : m + log2f(sum); };
+                    if (walk.count == tiles) {
+                        if (active) *out = log2_of(ref, l);
+                    } else {
+                        // A piece of a unit.  A share's first piece goes to its slot 0; its last, if another one, to slot
+                        // 1: only the unit's first share can have begun before it.
+                        const int64_t first = walk.cell - walk.tile0;  // the cell of the unit's first tile
+                        auto share_of = [&](int64_t x) { return (int)(((x + 1) * shares + total - 1) / total) - 1; };
+                        const int c0 = share_of(first), parts = share_of(first + tiles - 1) - c0 + 1;
+                        const int second = total * c0 / shares < first - kUnitCost ? 1 : 0;
+                        auto piece = [&](int c) {
+                            return a.partials + (int64_t)((c0 + c) * 2 + (c ? 0 : second)) * kRows + g * kTile + r;
+                        };
+                        if (active) *piece((int)blockIdx.x - c0) = make_float2(ref, l);
+                        named_barrier_sync(1, 2 * kTile);
+                        if (tid == 0) {
+                            uint32_t before;
+                            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                                         : "=r"(before)
+                                         : "l"(a.arrivals + cell)
+                                         : "memory");
+                            s.last = before == (uint32_t)(parts - 1);
                         }
-                        *out = log2_of(M, L);
+                        named_barrier_sync(1, 2 * kTile);
+                        if (s.last && active) {
+                            float M = -INFINITY, L = 0.f;
+                            for (int c = 0; c < parts; ++c) {
+                                const float2 x = __ldcg(piece(c));
+                                const float top = fmaxf(M, x.x), by = top == -INFINITY ? 0.f : top;
+                                L = L * fast_exp2(M - by) + x.y * fast_exp2(x.x - by);
+                                M = top;
+                            }
+                            *out = log2_of(M, L);
+                        }
+                        named_barrier_sync(1, 2 * kTile);  // s.last is read
                     }
-                    sums_sync();  // s.last is read
                 }
                 if (!walk.next()) break;
             }
         } else {
-            // A thread a key and half g of the columns; S of a tile's halves follow one another.
+            // A thread a key and a quarter of the columns; S of a tile's halves follow one another.
             // (A half has full barriers of its own: a wait by parity tells only one phase from the next.)
             int buf = g, tiles = 0, runs = 0;
             while (walk.count > 0) {
-                const int n = walk.queries(), half = columns_of(n) >> 1;
+                const int n = walk.queries(), half = columns_of(n) >> 1, mine = half >> 1, col0 = g * half + part * mine;
                 const int64_t cell = (int64_t)walk.id() * heads + walk.h;
-                float4* column = s.columns[g][runs & 1];
+                float4* column = s.columns[2 * g + part][runs & 1];
                 ++runs;
-                if (r < half) {
+                if (r < mine) {
                     float* to = reinterpret_cast<float*>(column) + (r >> 1) * 4 + (r & 1);
-                    to[0] = a.factor[cell * kRows + g * half + r];
-                    to[2] = -a.row_log2[cell * kRows + g * half + r];
+                    to[0] = a.factor[cell * kRows + col0 + r];
+                    to[2] = -a.row_log2[cell * kRows + col0 + r];
                 }
-                named_barrier_sync(2 + g, kTile);
+                named_barrier_sync(2 + 2 * g + part, kTile);
                 const int known = known_of(a.known, walk.b, walk.q);
                 const int evicted = known > 0 ? paged_evicted(p, walk.b) : 0;
                 const int64_t at = ((int64_t)walk.b * heads + walk.h) * a.w.capacity;
                 for (int t = 0; t < walk.count; ++t, ++tiles, next_slot()) {
                     const int tile = walk.tile0 + t, key = (tile << kTileShift) + r;
-                    const bool fresh = walk.u == walk.q.first_unit(tile), held = g == 0 && key < walk.q.len;
+                    const bool fresh = walk.u == walk.q.first_unit(tile), held = warp < 4 && key < walk.q.len;
                     float weight = 0.f;
                     if (held && (!fresh || key < known)) weight = a.w.weight[at + key];
                     if (ok) ok = warp_wait(&s.s_full[2 * g + (tiles & 1)], (tiles >> 1) & 1);
                     tc_fence_after();
                     // Rows that see the key: from this column on.
-                    const int from_col = (key - walk.pos()) * kGroup - g * half;
+                    const int from_col = (key - walk.pos()) * kGroup - col0;
                     const bool edge = __any_sync(0xffffffffu, from_col > 0);
                     const float ks = s.scales[slot][r >> 4];
-                    const uint32_t cols = tmem + lanes + buf * kTile;
-                    float2 sum = make_float2(0.f, 0.f);
-                    auto add = [&](float (&v)[16], int c) {
-                        float2 off[8];
+                    const uint32_t cols = tmem + lanes + buf * kTile + part * mine;
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    for (int c = 0; c < mine >> 4; ++c) {  // 16 columns
+                        float v[16];
+                        tmem_ld16(cols + 16 * c, reinterpret_cast<uint32_t(&)[16]>(v));
+                        tmem_wait_ld();
+                        if (c + 1 == mine >> 4) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float4 k = column[8 * c + i];
                             const float2 f = __fmul2_rn(make_float2(k.x, k.y), make_float2(ks, ks));
-                            off[i] = make_float2(k.z, k.w);
                             float2 x = make_float2(v[2 * i], v[2 * i + 1]);
-                            x = kCap ? __fmul2_rn(x, f) : __ffma2_rn(x, f, off[i]);
+                            x = kCap ? __fmul2_rn(x, f) : __ffma2_rn(x, f, make_float2(k.z, k.w));
                             v[2 * i] = x.x;
                             v[2 * i + 1] = x.y;
                         }
@@ -689,8 +712,8 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                             cap_scores(v, cap2);
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                v[2 * i] += off[i].x;
-                                v[2 * i + 1] += off[i].y;
+                                v[2 * i] += column[8 * c + i].z;
+                                v[2 * i + 1] += column[8 * c + i].w;
                             }
                         }
                         if (edge) {
@@ -701,38 +724,23 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         }
 #pragma unroll
                         for (int i = 0; i < 16; i += 2)
-                            sum = __fadd2_rn(sum, make_float2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
-                    };
-                    const int steps = half >> 4;
-                    auto free_sums = [&] {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&s.s_empty[buf]);
-                    };
-                    float x[16], y[16];
-                    tmem_ld16(cols, reinterpret_cast<uint32_t(&)[16]>(x));
-                    for (int c = 0; c < steps; c += 2) {
-                        tmem_wait_ld();
-                        if (c + 1 < steps) tmem_ld16(cols + 16 * (c + 1), reinterpret_cast<uint32_t(&)[16]>(y)); else free_sums();
-                        add(x, c);
-                        if (c + 1 < steps) {
-                            tmem_wait_ld();
-                            if (c + 2 < steps) tmem_ld16(cols + 16 * (c + 2), reinterpret_cast<uint32_t(&)[16]>(x)); else free_sums();
-                            add(y, c + 1);
-                        }
+                            sum[i >> 1 & 1] = __fadd2_rn(sum[i >> 1 & 1], make_float2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
                     }
                     buf += 2;  // (the other half's S lies between)
                     if (buf >= kSums) buf -= kSums;
-                    const float mine = sum.x + sum.y;
-                    if (g) {
-                        // (The first half is at most a tile behind: S of this tile could not have been written before.)
-                        s.half[tiles & 1][r] = mine;
+                    const float total_mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    const int ring = tiles & (kParts - 1);
+                    if (warp >= 4) {
+                        // (The first quarter is at most two tiles behind: S of the third would take the place of one
+                        // that it has not read.)
+                        s.part[ring][2 * g + part - 1][r] = total_mine;
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&s.half_full[tiles & 1]);
+                        if (lane == 0) mbar_arrive(&s.part_full[ring]);
                     } else {
-                        if (ok) ok = warp_wait(&s.half_full[tiles & 1], (tiles >> 1) & 1);
+                        if (ok) ok = warp_wait(&s.part_full[ring], tiles / kParts & 1);
                         if (held) {
-                            a.w.weight[at + key] = weight + (mine + s.half[tiles & 1][r]);
+                            a.w.weight[at + key] =
+                                weight + ((total_mine + s.part[ring][0][r]) + (s.part[ring][1][r] + s.part[ring][2][r]));
                             if (fresh && key >= known) a.w.position[at + key] = key + evicted;
                             if (fresh && key == 0 && known <= 0 && walk.h == 0) a.w.evicted[walk.b] = 0;
                         }
@@ -743,6 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
         }
     } else if (warp < kMmaWarp) {
         // ============================ conversion ============================
+        take_registers<kConvRegs>();
         const int cw = warp - kConvWarp, t = lane & 3;
         // Rows: as in the chunked attention kernel, eight lanes that access shared memory together have all eight
         // 16-byte columns of the codes' rows and of the operand's.  Keys: a lane a key, whose eight neighbours' rows
@@ -756,21 +765,23 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 if (!ok) break;
                 const uint8_t* src = raw + rs * kRawBytes;
                 if constexpr (kKeys) {
-                    uint32_t w[64];
+                    tc_fence_after();  // the products that read this tile's place are done
+                    const uint32_t to = tmem + ((uint32_t)(32 * cw) << 16) + kColK + cs * 64;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const uint4 x = lds128(src + key * kHeadDim + ((c ^ (key & 7)) << 4));
-                        to_half4<kCode>(x.x, w[8 * c], w[8 * c + 1]);
-                        to_half4<kCode>(x.y, w[8 * c + 2], w[8 * c + 3]);
-                        to_half4<kCode>(x.z, w[8 * c + 4], w[8 * c + 5]);
-                        to_half4<kCode>(x.w, w[8 * c + 6], w[8 * c + 7]);
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint4 x = lds128(src + key * kHeadDim + (((4 * half + c) ^ (key & 7)) << 4));
+                            to_half4<kCode>(x.x, w[8 * c], w[8 * c + 1]);
+                            to_half4<kCode>(x.y, w[8 * c + 2], w[8 * c + 3]);
+                            to_half4<kCode>(x.z, w[8 * c + 4], w[8 * c + 5]);
+                            to_half4<kCode>(x.w, w[8 * c + 6], w[8 * c + 7]);
+                        }
+                        tmem_st32(to + 32 * half, w);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s.raw_empty[rs]);
-                    tc_fence_after();  // the products that read this tile's place are done
-                    const uint32_t to = tmem + ((uint32_t)(32 * cw) << 16) + kColK + cs * 64;
-                    tmem_st32(to, reinterpret_cast<const uint32_t(&)[32]>(w[0]));
-                    tmem_st32(to + 32, reinterpret_cast<const uint32_t(&)[32]>(w[32]));
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -811,7 +822,9 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
             }
             if (!ok || !walk.next()) break;
         }
-    } else if (warp == kMmaWarp) {
+    } else {
+    take_registers<kRestRegs>();
+    if (warp == kMmaWarp) {
         // ============================ MMA issuer ============================
         const uint32_t leader = elect_lane(), cols = uniform(tmem);
         int cs = 0, cphase = 0, runs = 0;
@@ -957,6 +970,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
         }
         if (runs > 0) warp_wait(&s.q_full[0], (runs - 1) & 1);  // no copy in flight when the CTA leaves
     }
+    }
     if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
 
     tc_fence_before();
@@ -1005,7 +1019,12 @@ size_t paged_weigh_workspace(int batch, int rows, int heads, int sms) { return r
 
 cudaError_t paged_weigh_prepare() {
     for (int i = 0; i < 8; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(i & 4 ? kernel_for<true>(i & 1, i & 2) : kernel_for<false>(i & 1, i & 2),
+        // The register shares are of kLaunchRegs a thread: with fewer at launch the kernel would wait for good.
+        cudaFuncAttributes at;
+        cudaError_t e = cudaFuncGetAttributes(&at, i & 4 ? kernel_for<true>(i & 1, i & 2) : kernel_for<false>(i & 1, i & 2));
+        if (e != cudaSuccess) return e;
+        if (at.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+        e = cudaFuncSetAttribute(i & 4 ? kernel_for<true>(i & 1, i & 2) : kernel_for<false>(i & 1, i & 2),
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    i & 4 ? kSmemBytes<true> : kSmemBytes<false>);
         if (e != cudaSuccess) return e;
@@ -1041,7 +1060,7 @@ cudaError_t launch_paged_weigh(const PagedCall& call, const RopeSteps& rope, int
     a.partials = reinterpret_cast<float2*>(ws + r.partials);
     a.max_units = units_of(call.batch, call.rows);
     const PrepArgs prep{call, rope, known, a.queries, a.factor, a.arrivals};
-    cudaError_t e = launch_dependent(weigh_queries_kernel, dim3(a.max_units, call.c.kv_heads), kSumThreads, 0, stream, prep);
+    cudaError_t e = launch_dependent(weigh_queries_kernel, dim3(a.max_units, call.c.kv_heads), kPrepThreads, 0, stream, prep);
     if (e == cudaSuccess)
         e = launch_dependent(kernel_for<false>(code, call.cap > 0.f), dim3(sms), kThreads, kSmemBytes<false>, stream, a);
     if (e == cudaSuccess)
