@@ -201,6 +201,8 @@ _lib = None
 def load() -> ctypes.CDLL:
     """Load the CUDA library (once); raises if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIB_PATH.is_file():

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass, field
+from typing import NamedTuple
 
 import torch
 
@@ -84,13 +85,13 @@ def key_weights(requests: int, capacity: int, *, kv_heads: int = N_KV_HEADS,
 
 
 def _check_weights(weights: KeyWeights, cache: PagedCache, block_table: torch.Tensor, requests: int) -> None:
-    if weights.device != cache.device:
+    rows, heads, capacity = weights.weight.shape
+    if weights.weight.device != cache.k.device:
         raise ValueError(f"weights are on {weights.device}; every tensor of this call must be on {cache.device}")
-    if weights.requests != requests or weights.kv_heads != cache.kv_heads:
-        raise ValueError(f"weights are of {weights.requests} requests and {weights.kv_heads} heads, the call of "
-                         f"{requests} and {cache.kv_heads}")
-    if block_table.dim() == 2 and weights.capacity < block_table.shape[1] * cache.page_len:
-        raise ValueError(f"weights hold {weights.capacity} rows a request, a row of block_table names "
+    if rows != requests or heads != cache.c.kv_heads:
+        raise ValueError(f"weights are of {rows} requests and {heads} heads, the call of {requests} and {cache.kv_heads}")
+    if block_table.dim() == 2 and capacity < block_table.shape[1] * cache.c.page_len:
+        raise ValueError(f"weights hold {capacity} rows a request, a row of block_table names "
                          f"{block_table.shape[1] * cache.page_len}")
 
 
@@ -129,8 +130,7 @@ def add_key_weights(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
             sizes=lib.gqa_key_weights_workspace_bytes)
 
 
-@dataclass(frozen=True)
-class EvictionPlan:
+class EvictionPlan(NamedTuple):
     """What :func:`plan_eviction` chose, all in device memory."""
     take: torch.Tensor     # int32 [requests, heads, max_keep]: the row that moves to row i, -1 where none does
     lens: torch.Tensor     # int32 [requests]: rows held after the step
@@ -166,7 +166,8 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
     n = lens.shape[0] if lens.dim() == 1 else 0
     if not 1 <= n <= _lib.PAGED_MAX_BATCH:
         raise ValueError(f"lens must be [requests] with 1 to {_lib.PAGED_MAX_BATCH} requests")
-    if weights.requests != n or weights.device != device:
+    requests, heads, _ = weights.weight.shape
+    if requests != n or weights.weight.device != device:
         raise ValueError(f"weights are of {weights.requests} requests on {weights.device}, lens of {n} on {device}")
     _table(block_table, n, device)
     if free_pages.dim() != 1:
@@ -178,17 +179,17 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
     i32 = torch.int32
     if evicted_out is None and lens_out is lens:
         evicted_out = weights.evicted
-    take = lens.new_empty((n, weights.kv_heads, max_keep), dtype=i32)
+    take = lens.new_empty((n, heads, max_keep), dtype=i32)
     room = [n if lens_out is None else 0, n if evicted_out is None else 0, 1 if n_free_out is None else 0, 4]
-    new_lens, new_evicted, new_n_free, counts = lens.new_empty(sum(room), dtype=i32).split(room)
+    new_lens, new_evicted, new_n_free, counts = lens.new_empty(sum(room), dtype=i32).split_with_sizes(room)
     lens_out = new_lens if lens_out is None else lens_out
     evicted_out = new_evicted if evicted_out is None else evicted_out
     n_free_out = new_n_free if n_free_out is None else n_free_out
     stream = _stream_ptr(device)
-    nbytes = lib.gqa_plan_eviction_workspace_bytes(n, weights.kv_heads, max_keep)
+    nbytes = lib.gqa_plan_eviction_workspace_bytes(n, heads, max_keep)
     ws = api._workspace(device, ("eviction", stream), nbytes)
     _check(lib.gqa_plan_eviction(
-        ctypes.byref(weights.c), weights.kv_heads, _need("lens", lens, i32, (n,), device),
+        ctypes.byref(weights.c), heads, _need("lens", lens, i32, (n,), device),
         _need("keep", keep, i32, (n,), device), n, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
         _need("free_pages", free_pages, i32, tuple(free_pages.shape), device), free_pages.shape[0],
         _need("n_free", n_free, i32, (1,), device), page_len, max_keep, sinks, recent, take.data_ptr(),

@@ -28,6 +28,7 @@ from ._lib import GqaPagedCache, GqaPagedParams
 from .api import GROUP_SIZE, HEAD_DIM, N_KV_HEADS, ROPE_THETA, GqaError, _check, _check_cuda, _check_out, _stream_ptr
 
 PAGE_LENS = (16, 32, 64, 128)
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _CODES = {torch.int8: _lib.GQA_CODE_INT8, torch.float8_e4m3fn: _lib.GQA_CODE_E4M3}
 
 
@@ -256,7 +257,8 @@ def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_posit
         raise ValueError(f"seq_lens must be [batch] with 1 to {_lib.PAGED_MAX_BATCH} sequences")
     if first_query is None and rows != batch:
         raise ValueError(f"{rows} query rows for {batch} sequences")
-    _check_cuda(device, cache=cache.k)
+    if cache.k.device != device:
+        _check_cuda(device, cache=cache.k)
     _table(block_table, batch, device)
     if score_cap is not None and not (score_cap > 0.0 and math.isfinite(score_cap)):
         raise ValueError("score_cap must be positive and finite, or None")
@@ -267,18 +269,17 @@ def _attend(name: str, q, cache, block_table, seq_lens, first_query, query_posit
     else:
         _check_out(out, (rows, out_heads, HEAD_DIM), torch.bfloat16, device)
     i32 = torch.int32
+    # (In the structure's order: naming the fields takes as long again.)
     p = GqaPagedParams(
-        batch=batch, rows=rows, block_table=block_table.data_ptr(), table_stride=block_table.stride(0),
-        table_width=block_table.shape[1], flags=_lib.GQA_FLAG_Q_ROTATED if q_rotated else 0,
-        seq_lens=_need("seq_lens", seq_lens, i32, (batch,), device),
-        query_positions=_need("query_positions", query_positions, i32, (batch,), device),
-        first_query=_need("first_query", first_query, i32, (batch + 1,), device),
-        doc_starts=_need("doc_starts", doc_starts, i32, (rows,), device),
-        prefix_ends=_need("prefix_ends", prefix_ends, i32, (rows,), device),
-        slopes=_need("distance_slopes", distance_slopes, torch.float32, (heads,), device),
-        scale=1.0 / math.sqrt(HEAD_DIM) if scale is None else scale, score_cap=score_cap or 0.0,
-        rope_theta=rope_theta, reserved=0, q_row_stride=q.stride(0), q_head_stride=q.stride(1),
-        out_row_stride=out.stride(0), out_head_stride=out.stride(1))
+        batch, rows, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        _lib.GQA_FLAG_Q_ROTATED if q_rotated else 0,
+        _need("seq_lens", seq_lens, i32, (batch,), device),
+        _need("query_positions", query_positions, i32, (batch,), device) if query_positions is not None else None,
+        _need("first_query", first_query, i32, (batch + 1,), device) if first_query is not None else None,
+        _need("doc_starts", doc_starts, i32, (rows,), device) if doc_starts is not None else None,
+        _need("prefix_ends", prefix_ends, i32, (rows,), device) if prefix_ends is not None else None,
+        _need("distance_slopes", distance_slopes, torch.float32, (heads,), device) if distance_slopes is not None else None,
+        _SCALE if scale is None else scale, score_cap or 0.0, rope_theta, 0, *q.stride()[:2], *out.stride()[:2])
     if rows == 0:
         return out
     stream = _stream_ptr(device)
@@ -332,19 +333,20 @@ def decode_paged_chunked(q: torch.Tensor, cache: PagedCache, block_table: torch.
 
 def _attend_diff(name: str, q, cache, block_table, seq_lens, first_query, lambdas, norm_weight, norm_eps, out_scale, **call):
     lib = _lib.load()
-    heads, device = cache.kv_heads * GROUP_SIZE // 2, q.device
+    heads, device = cache.c.kv_heads * GROUP_SIZE // 2, q.device
     rows = q.shape[0] if q.dim() else 0
     f32 = torch.float32
-    if lambdas.dtype is not f32 or lambdas.device != device or lambdas.shape not in ((heads,), (rows, heads)) \
-            or lambdas.stride(-1) != 1 and heads > 1 or lambdas.dim() == 2 and rows > 1 and lambdas.stride(0) < 0:
+    shape = lambdas.shape
+    if lambdas.dtype is not f32 or lambdas.device != device or shape != (heads,) and shape != (rows, heads) \
+            or lambdas.stride(-1) != 1:
         raise ValueError(f"lambdas must be float32 [{heads}] or [{rows}, {heads}] on {device} with a contiguous last dim")
-    gain = _need("norm_weight", norm_weight, f32, (HEAD_DIM,), device)
+    gain = _need("norm_weight", norm_weight, f32, (HEAD_DIM,), device) if norm_weight is not None else None
     if not math.isfinite(out_scale):
         raise ValueError("out_scale must be finite")
     if gain is not None and not (norm_eps > 0.0 and math.isfinite(norm_eps)):
         raise ValueError("norm_eps must be positive and finite")
-    d = _lib.GqaPagedDiff(lambdas=lambdas.data_ptr(), norm_weight=gain, norm_eps=norm_eps, out_scale=out_scale,
-                          lambda_row_stride=lambdas.stride(0) if lambdas.dim() == 2 and rows > 1 else 0)
+    d = _lib.GqaPagedDiff(lambdas.data_ptr(), lambdas.stride(0) if len(shape) == 2 and rows > 1 else 0, gain, norm_eps,
+                          out_scale)
     return _attend(name, q, cache, block_table, seq_lens, first_query, out_heads=heads, extra=(ctypes.byref(d),),
                    entry=lib.gqa_decode_paged_diff if first_query is None else lib.gqa_decode_paged_chunked_diff, **call)
 
