@@ -30,6 +30,7 @@
 //             the A operand in TMEM (keys)
 //   20        MMA issuer
 //   21, 22    loaders of codes and of queries
+//   23        finds the share's runs, ahead of all others
 // The A operand is in TMEM in both passes -- the unit's queries, written by the rows'
 // threads, or the tile's keys -- because two operands of 128 x 16 in shared memory are
 // read at half the rate of the products; so are the operands' other users, 1700 of a
@@ -99,7 +100,7 @@ constexpr int kTileBytes = 2 * kBlockBytes;
 constexpr int kQBlockBytes = kRows * 128;          // 64 dims of a part of the rows
 constexpr int kQBytes = 4 * kQBlockBytes;          // [part][64 dims][row]
 constexpr int kScaleSlots = 16;
-constexpr int kConvWarp = 16, kMmaWarp = 20, kLoadWarp = 21, kQueryWarp = 22;
+constexpr int kConvWarp = 16, kMmaWarp = 20, kLoadWarp = 21, kQueryWarp = 22, kWalkWarp = 23;
 constexpr int kThreads = 24 * 32, kPrepThreads = 8 * 32;
 // Registers: launched with 80 a thread; each group of four warps takes its share.
 constexpr int kLaunchRegs = 80, kSumRegs = 88, kConvRegs = 64, kRestRegs = 64;
@@ -109,6 +110,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColQ = 256, kColK = 384;
 constexpr int kSums = 3;  // S of the keys' pass
 constexpr int kParts = 4; // tiles whose quarters' sums wait to be joined
+constexpr int kRuns = 4;  // runs found ahead
 // What a unit costs beside its tiles when the shares of the rows' pass are cut, in tiles.
 constexpr int kUnitCost = 2;
 // The rows' reference is the largest of the first keys; a sum of weights past 2^kOverflow moves it.
@@ -298,7 +300,19 @@ private:
     }
 };
 
+// A run as the warps of a CTA take it.
+struct Run {
+    int b, h, u, count;       // sequence, head, unit, tiles (0: the share's end)
+    int tile0, n, pos, len;   // first tile, queries, the first one's row, keys of the sequence
+    int c;                    // as Seq has it
+    int known, evicted;       // keys
+    int tiles, c0, parts, second;  // rows: the unit's tiles; its first share, its shares, the first one's slot
+    int64_t cell;             // unit and head
+};
+
 struct alignas(16) Shared {
+    Run runs[kRuns];
+    uint64_t run_full[kRuns], run_empty[kRuns];
     uint64_t raw_full[4], raw_empty[4], conv_full[4], conv_empty[4];
     uint64_t q_full[2], q_empty, s_full[4], s_empty[kSums];  // s_full, keys: [half][tile % 2]
     uint64_t part_full[kParts];
@@ -409,6 +423,31 @@ __global__ void __launch_bounds__(kPrepThreads) weigh_queries_kernel(const __gri
     }
 }
 
+// cap2 * tanh of a thread's scores (multiples of the cap in, log2 units out), as cap_scores, two at a time.
+template <int kN>
+__device__ __forceinline__ void cap_pairs(float (&z)[kN], float cap2) {
+    auto both = [](float v) { return make_float2(v, v); };
+    float x[kN], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < kN; i += 2) {
+        const float2 v = make_float2(z[i], z[i + 1]), t = __fmul2_rn(v, v);
+        x[i] = v.x;
+        x[i + 1] = v.y;
+        most = fmaxf(fmaxf(most, t.x), t.y);
+        float2 y = __ffma2_rn(both(0.0171313453f), t, both(-0.0529842377f));
+        y = __ffma2_rn(y, t, both(0.13324751f));
+        y = __ffma2_rn(y, t, both(-0.333330691f));
+        y = __fmul2_rn(__ffma2_rn(y, t, both(1.f)), __fmul2_rn(v, both(cap2)));
+        z[i] = y.x;
+        z[i + 1] = y.y;
+    }
+    if (most > kTanhNear)
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (x[i] * x[i] > kTanhNear) z[i] = cap2 * tanh_far(x[i]);
+    __syncwarp();
+}
+
 // Rows of a unit as the MMA takes them: whole steps of 64 columns.
 __device__ __forceinline__ int columns_of(int n) { return (n * kGroup + 63) & ~63; }
 
@@ -454,6 +493,10 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
         for (int i = 0; i < kSums; ++i) mbar_init(&s.s_empty[i], 8);
         for (int i = 0; i < kParts; ++i) mbar_init(&s.part_full[i], 12);
         for (int i = 0; i < 2; ++i) mbar_init(&s.q_full[i], kKeys ? 1 : 8);
+        for (int i = 0; i < kRuns; ++i) {
+            mbar_init(&s.run_full[i], 1);
+            mbar_init(&s.run_empty[i], kKeys ? kWalkWarp : kWalkWarp - 1);  // all other warps (rows: but the queries' loader)
+        }
         mbar_init(&s.q_empty, 1);
         mbar_init(&s.drain, 1);
         fence_barrier_init();
@@ -508,9 +551,24 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    Walk<kKeys> walk(p);
-    walk.start(s.start_b, s.start_base, from, to);
     bool ok = true;
+    // The runs, in the order in which kWalkWarp finds them.  A warp that gave up goes through the others without work;
+    // the waits here last longer than all that can be waited for in between.
+    int run_i = 0;
+    auto next_run = [&](Run& r) {
+        const int at = run_i & (kRuns - 1);
+        bool got = false;
+        for (int i = 0; i < 16 && !got; ++i) got = warp_wait(&s.run_full[at], run_i / kRuns & 1);
+        r = s.runs[at];
+        if (!got) ok = false;
+        return got && r.count > 0;
+    };
+    auto end_run = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.run_empty[run_i & (kRuns - 1)]);
+        ++run_i;
+    };
+    Run run;
 
     if (warp < kConvWarp) {
         // ============================ sums ============================
@@ -524,12 +582,12 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
             // A thread a row of M tile g and half of a tile's keys; S and queries of the M tile are these eight warps'.
             const uint32_t t_s = tmem + lanes + g * kTile + 64 * part, t_q = tmem + lanes + kColQ + g * kTile + 64 * part;
             int phase = 0, runs = 0;
-            while (walk.count > 0) {
-                const int n = walk.queries(), token = 32 * g + (r >> 2);
+            for (; next_run(run); end_run()) {
+                const int n = run.n, token = 32 * g + (r >> 2);
                 const bool active = n > 32 * g, real = token < n;
-                const int64_t cell = (int64_t)walk.id() * heads + walk.h;
+                const int64_t cell = run.cell;
                 const float factor = real ? a.factor[cell * kRows + g * kTile + r] : 0.f;
-                const int hi = real ? (int)min((int64_t)walk.pos() + token + 1, (int64_t)walk.q.len) : 0x7fffffff;
+                const int hi = real ? min(run.pos + token + 1, run.len) : 0x7fffffff;
                 float ref = -INFINITY, l = 0.f;
                 if (active) {
                     // One part of the row's queries to TMEM (the products that read the last ones were waited for).
@@ -549,12 +607,12 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s.q_full[g]);
                 }
-                for (int t = 0; t < walk.count; ++t, next_slot()) {
+                for (int t = 0; t < run.count; ++t, next_slot()) {
                     if (!active) continue;
                     if (ok) ok = warp_wait(&s.s_full[g], phase);
                     phase ^= 1;
                     tc_fence_after();
-                    const int k0 = ((walk.tile0 + t) << kTileShift) + 64 * part;
+                    const int k0 = ((run.tile0 + t) << kTileShift) + 64 * part;
                     const bool edge = __any_sync(0xffffffffu, hi < k0 + 64);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -573,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                             f0 = f1 = 1.f;
                         }
                         if constexpr (kCap) {
-                            cap_scores(reinterpret_cast<float(&)[16]>(z[0]), cap2);
-                            cap_scores(reinterpret_cast<float(&)[16]>(z[16]), cap2);
+                            cap_pairs(reinterpret_cast<float(&)[16]>(z[0]), cap2);
+                            cap_pairs(reinterpret_cast<float(&)[16]>(z[16]), cap2);
                         }
                         if (edge) {
                             const int left = hi - k0 - 32 * c;
@@ -618,18 +676,13 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     const float now = fmaxf(ref, other.x), use = now == -INFINITY ? 0.f : now;
                     l = l * fast_exp2(ref - use) + other.y * fast_exp2(other.x - use);
                     ref = now;
-                    const int tiles = walk.q.unit_tiles(walk.u);
                     float* out = a.row_log2 + cell * kRows + g * kTile + r;
                     auto log2_of = [&](float m, float sum) { return !real ? INFINITY : sum == 0.f ? -INFINITY : m + log2f(sum); };
-                    if (walk.count == tiles) {
+                    if (run.count == run.tiles) {
                         if (active) *out = log2_of(ref, l);
                     } else {
-                        // A piece of a unit.  A share's first piece goes to its slot 0; its last, if another one, to slot
-                        // 1: only the unit's first share can have begun before it.
-                        const int64_t first = walk.cell - walk.tile0;  // the cell of the unit's first tile
-                        auto share_of = [&](int64_t x) { return (int)(((x + 1) * shares + total - 1) / total) - 1; };
-                        const int c0 = share_of(first), parts = share_of(first + tiles - 1) - c0 + 1;
-                        const int second = total * c0 / shares < first - kUnitCost ? 1 : 0;
+                        // A piece of a unit.
+                        const int c0 = run.c0, parts = run.parts, second = run.second;
                         auto piece = [&](int c) {
                             return a.partials + (int64_t)((c0 + c) * 2 + (c ? 0 : second)) * kRows + g * kTile + r;
                         };
@@ -657,15 +710,14 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         named_barrier_sync(1, 2 * kTile);  // s.last is read
                     }
                 }
-                if (!walk.next()) break;
             }
         } else {
             // A thread a key and a quarter of the columns; S of a tile's halves follow one another.
             // (A half has full barriers of its own: a wait by parity tells only one phase from the next.)
             int buf = g, tiles = 0, runs = 0;
-            while (walk.count > 0) {
-                const int n = walk.queries(), half = columns_of(n) >> 1, mine = half >> 1, col0 = g * half + part * mine;
-                const int64_t cell = (int64_t)walk.id() * heads + walk.h;
+            for (; next_run(run); end_run()) {
+                const int half = columns_of(run.n) >> 1, mine = half >> 1, col0 = g * half + part * mine;
+                const int64_t cell = run.cell;
                 float4* column = s.columns[2 * g + part][runs & 1];
                 ++runs;
                 if (r < mine) {
@@ -674,18 +726,17 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     to[2] = -a.row_log2[cell * kRows + col0 + r];
                 }
                 named_barrier_sync(2 + 2 * g + part, kTile);
-                const int known = known_of(a.known, walk.b, walk.q);
-                const int evicted = known > 0 ? paged_evicted(p, walk.b) : 0;
-                const int64_t at = ((int64_t)walk.b * heads + walk.h) * a.w.capacity;
-                for (int t = 0; t < walk.count; ++t, ++tiles, next_slot()) {
-                    const int tile = walk.tile0 + t, key = (tile << kTileShift) + r;
-                    const bool fresh = walk.u == walk.q.first_unit(tile), held = warp < 4 && key < walk.q.len;
+                const int known = run.known, len = run.len;
+                const int64_t at = ((int64_t)run.b * heads + run.h) * a.w.capacity;
+                for (int t = 0; t < run.count; ++t, ++tiles, next_slot()) {
+                    const int tile = run.tile0 + t, key = (tile << kTileShift) + r;
+                    const bool fresh = run.u == max(0, 2 * tile - run.c), held = warp < 4 && key < len;
                     float weight = 0.f;
                     if (held && (!fresh || key < known)) weight = a.w.weight[at + key];
                     if (ok) ok = warp_wait(&s.s_full[2 * g + (tiles & 1)], (tiles >> 1) & 1);
                     tc_fence_after();
                     // Rows that see the key: from this column on.
-                    const int from_col = (key - walk.pos()) * kGroup - col0;
+                    const int from_col = (key - run.pos) * kGroup - col0;
                     const bool edge = __any_sync(0xffffffffu, from_col > 0);
                     const float ks = s.scales[slot][r >> 4];
                     const uint32_t cols = tmem + lanes + buf * kTile + part * mine;
@@ -709,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                             v[2 * i + 1] = x.y;
                         }
                         if constexpr (kCap) {
-                            cap_scores(v, cap2);
+                            cap_pairs(v, cap2);
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 v[2 * i] += column[8 * c + i].z;
@@ -741,12 +792,11 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         if (held) {
                             a.w.weight[at + key] =
                                 weight + ((total_mine + s.part[ring][0][r]) + (s.part[ring][1][r] + s.part[ring][2][r]));
-                            if (fresh && key >= known) a.w.position[at + key] = key + evicted;
-                            if (fresh && key == 0 && known <= 0 && walk.h == 0) a.w.evicted[walk.b] = 0;
+                            if (fresh && key >= known) a.w.position[at + key] = key + run.evicted;
+                            if (fresh && key == 0 && known <= 0 && run.h == 0) a.w.evicted[run.b] = 0;
                         }
                     }
                 }
-                if (!walk.next()) break;
             }
         }
     } else if (warp < kMmaWarp) {
@@ -758,8 +808,8 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
         // hold a chunk in eight different columns.
         const int row0 = 32 * cw + ((lane >> 3) ^ (lane & 4 ? 5 : 0)), key = 32 * cw + lane;
         int rs = 0, rphase = 0, cs = 0, cphase = 0, items = 0;
-        while (walk.count > 0 && ok) {
-            for (int j = 0; j < walk.count && ok; ++j, ++items) {
+        for (; next_run(run); end_run()) {
+            for (int j = 0; j < run.count && ok; ++j, ++items) {
                 ok = mbar_wait(&s.raw_full[rs], rphase) && (items < kConv || mbar_wait(&s.conv_empty[cs], cphase ^ 1));
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -820,7 +870,6 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     cphase ^= 1;
                 }
             }
-            if (!ok || !walk.next()) break;
         }
     } else {
     take_registers<kRestRegs>();
@@ -836,8 +885,9 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 cphase ^= 1;
             }
         };
-        while (uniform(walk.count) > 0 && ok) {
-            const int n = uniform(walk.queries()), count = uniform(walk.count);
+        for (; next_run(run); end_run()) {
+            if (!ok) continue;
+            const int n = uniform(run.n), count = uniform(run.count);
             if constexpr (kKeys) {
                 const int half = columns_of(n) >> 1;
                 const uint32_t idesc = idesc_n(half);
@@ -896,7 +946,6 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     next_tile();
                 }
             }
-            if (!ok || !uniform(walk.next())) break;
         }
         if (!ok) {  // shared memory and TMEM are given back with no product under way
             tc_commit_by(leader, &s.drain);
@@ -908,22 +957,23 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
         const int box_bytes = p.c.page_len * kHeadDim;
         const uint64_t policy = l2_evict_first_policy();
         int rs = 0, rphase = 0, items = 0, slot = 0;
-        while (walk.count > 0 && ok) {
-            const int32_t* table = p.block_table + walk.b * p.table_stride;
-            const int64_t hi = walk.q.len;
+        for (; next_run(run); end_run()) {
+            if (!ok) continue;
+            const int32_t* table = p.block_table + run.b * p.table_stride;
+            const int64_t hi = run.len;
             // Lane's page of tile j of the run (-1: past the sequence's keys, not loaded).
             auto entry = [&](int j) {
-                const int64_t key = ((int64_t)(walk.tile0 + j) << kTileShift) + ((int64_t)lane << shift);
-                if (lane >= per_tile || j >= walk.count || key >= hi) return -1;
+                const int64_t key = ((int64_t)(run.tile0 + j) << kTileShift) + ((int64_t)lane << shift);
+                if (lane >= per_tile || j >= run.count || key >= hi) return -1;
                 const int page = table[key >> shift];
                 return page >= 0 && page < p.c.pages ? page : p.c.pages;  // out of the map: TMA fills zeros
             };
             auto scale = [&](int page) {
-                return page >= 0 && page < p.c.pages ? p.c.k_scale[page * p.c.scale_page_stride + walk.h] : 0.f;
+                return page >= 0 && page < p.c.pages ? p.c.k_scale[page * p.c.scale_page_stride + run.h] : 0.f;
             };
             int page = entry(0), page1 = entry(1);
             float ks = scale(page);
-            for (int j = 0; j < walk.count; ++j, ++items) {
+            for (int j = 0; j < run.count; ++j, ++items) {
                 const int page2 = entry(j + 2);
                 const float ks1 = scale(page1);
                 if (items >= kRaw) ok = __all_sync(0xffffffffu, mbar_wait(&s.raw_empty[rs], rphase ^ 1));
@@ -936,7 +986,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[rs], boxes * box_bytes);
                 __syncwarp();
                 if (page >= 0)
-                    tma_load_page(raw + rs * kRawBytes + lane * box_bytes, &a.kmap, 0, walk.h, page, &s.raw_full[rs], policy);
+                    tma_load_page(raw + rs * kRawBytes + lane * box_bytes, &a.kmap, 0, run.h, page, &s.raw_full[rs], policy);
                 if (++rs == kRaw) {
                     rs = 0;
                     rphase ^= 1;
@@ -945,7 +995,6 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                 page1 = page2;
                 ks = ks1;
             }
-            if (!ok || !walk.next()) break;
         }
         if (!ok)  // do not leave while copies into this CTA's shared memory are in flight
             for (int i = 1; i <= kRaw && i <= items; ++i) {
@@ -955,20 +1004,62 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     } else if (kKeys && warp == kQueryWarp) {
         // ============================ queries ============================
         int runs = 0;
-        while (walk.count > 0) {
-            if (runs > 0 && !warp_wait(&s.q_empty, (runs - 1) & 1)) {
-                ok = false;  // (the last copies have landed: their products were waited for)
-                break;
-            }
-            const uint32_t bytes = columns_of(walk.queries()) * 128;
-            const uint8_t* src = a.queries + ((int64_t)walk.id() * heads + walk.h) * kQBytes;
+        for (; next_run(run); end_run()) {
+            if (!ok) continue;
+            if (runs > 0) ok = warp_wait(&s.q_empty, (runs - 1) & 1);
+            if (!ok) continue;  // (the last copies have landed: their products were waited for)
+            const uint32_t bytes = columns_of(run.n) * 128;
+            const uint8_t* src = a.queries + run.cell * kQBytes;
             if (lane == 0) mbar_arrive_expect_tx(&s.q_full[0], 4 * bytes);
             __syncwarp();
             if (lane < 4) bulk_load_queries(q_smem + lane * kQBlockBytes, src + lane * kQBlockBytes, bytes, &s.q_full[0]);
             ++runs;
-            if (!walk.next()) break;
         }
         if (runs > 0) warp_wait(&s.q_full[0], (runs - 1) & 1);  // no copy in flight when the CTA leaves
+    } else if (warp == kWalkWarp && lane == 0) {
+        // ============================ runs ============================
+        Walk<kKeys> walk(p);
+        walk.start(s.start_b, s.start_base, from, to);
+        for (int i = 0;; ++i) {
+            const int at = i & (kRuns - 1);
+            if (i >= kRuns) {
+                ok = false;
+                for (int k = 0; k < 8 && !ok; ++k) ok = mbar_wait(&s.run_empty[at], (i / kRuns - 1) & 1);
+            }
+            const bool more = ok && walk.count > 0;
+            Run& r = s.runs[at];
+            r.count = more ? walk.count : 0;
+            if (more) {
+                const Seq& q = walk.q;
+                r.b = walk.b;
+                r.h = walk.h;
+                r.u = walk.u;
+                r.tile0 = walk.tile0;
+                r.n = walk.queries();
+                r.pos = walk.pos();
+                r.len = q.len;
+                r.c = q.c;
+                r.cell = (int64_t)walk.id() * heads + walk.h;
+                if constexpr (kKeys) {
+                    r.known = known_of(a.known, walk.b, q);
+                    r.evicted = r.known > 0 ? paged_evicted(p, walk.b) : 0;
+                } else {
+                    r.tiles = q.unit_tiles(walk.u);
+                    if (walk.count != r.tiles) {
+                        // A share's first piece goes to its slot 0; its last, if another one, to slot 1: only the
+                        // unit's first share can have begun before it.
+                        const int64_t first = walk.cell - walk.tile0;  // the cell of the unit's first tile
+                        auto share_of = [&](int64_t x) { return (int)(((x + 1) * shares + total - 1) / total) - 1; };
+                        r.c0 = share_of(first);
+                        r.parts = share_of(first + r.tiles - 1) - r.c0 + 1;
+                        r.second = total * r.c0 / shares < first - kUnitCost ? 1 : 0;
+                    }
+                }
+            }
+            mbar_arrive(&s.run_full[at]);
+            if (!more) break;
+            walk.next();
+        }
     }
     }
     if (!ok && lane == 0) atomicOr(a.status, kDevStatusTimeout);
