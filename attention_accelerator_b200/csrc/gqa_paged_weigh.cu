@@ -343,25 +343,28 @@ __device__ __forceinline__ uint32_t bf16_magnitudes(uint32_t w) { return max(w <
 // A sequence without rows before these is a new one: nothing was evicted from it.
 __device__ __forceinline__ int known_of(const int32_t* known, int b, const Seq& q) { return known ? known[b] : q.pos0; }
 
-__global__ void __launch_bounds__(kPrepThreads) weigh_queries_kernel(const __grid_constant__ PrepArgs a) {
+__global__ void __launch_bounds__(kPrepThreads, 2) weigh_queries_kernel(const __grid_constant__ PrepArgs a) {
     const PagedCall& p = a.p;
     const int id = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, token = tid >> 2, q4 = tid & 3;
     __shared__ uint64_t step[kPairs];
     if (tid < kPairs) step[tid] = a.rope.step[tid];
     dependency_wait();
     allow_dependents();
-    // The last sequence whose first unit has this number or a lower one.
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (Seq(p, mid).id0 <= id) lo = mid; else hi = mid;
+    // The last sequence whose first unit has this number or a lower one: a thread a candidate, of stretches and then of
+    // the one that it lies in (the numbers grow).
+    int lo = 0;
+    for (int room = p.batch; room > 1;) {
+        const int stride = (room + kPrepThreads - 1) / kPrepThreads, at = lo + tid * stride;
+        const int below = __syncthreads_count(tid * stride < room && Seq(p, at).id0 <= id);
+        lo += max(0, below - 1) * stride;
+        room = min(stride, p.batch - lo);
     }
     const Seq q(p, lo);
     const int u = id - q.id0;
     if (u < 0 || u >= q.units) return;
     const int64_t cell = (int64_t)id * p.c.kv_heads + h;
     if (tid == 0) a.arrivals[cell] = 0;
-    __syncthreads();
+    __syncthreads();  // (the steps)
     const int n = min(kTokens, q.n - u * kTokens);
     if (token >= ((n + 15) & ~15)) return;  // whole steps of 64 rows are read
     const bool real = token < n;
@@ -371,6 +374,11 @@ __global__ void __launch_bounds__(kPrepThreads) weigh_queries_kernel(const __gri
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(q.row0 + u * kTokens + token) * p.q_row_stride +
                                                       h * kGroup * p.q_head_stride + 16 * q4);
+    // A head's pairs 0-7 and 8-15, first and then second elements, asked for a head ahead.
+    auto load = [&](int hq, int i) { return real ? src[hq * (p.q_head_stride / 8) + (i & 1) + 8 * (i >> 1)] : none; };
+    uint4 next[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next[i] = load(0, i);
     float2 f[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -378,9 +386,12 @@ __global__ void __launch_bounds__(kPrepThreads) weigh_queries_kernel(const __gri
     uint8_t* out = a.queries + cell * kQBytes;
 #pragma unroll 1
     for (int hq = 0; hq < kGroup; ++hq) {
-        uint4 w[4];  // pairs 0-7 and 8-15: first, then second elements
+        uint4 w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = real ? src[hq * (p.q_head_stride / 8) + (i & 1) + 8 * (i >> 1)] : none;
+        for (int i = 0; i < 4; ++i) {
+            w[i] = next[i];
+            if (hq + 1 < kGroup) next[i] = load(hq + 1, i);
+        }
         // A power of two above the row's largest: a rotated pair passes it by no more than sqrt(2).
         uint32_t top = 0;
 #pragma unroll
