@@ -587,3 +587,187 @@ def test_plan_of_long_requests(requests, heads, longest, keep, kind):
             want = torch.full((keep,), -1, dtype=torch.int32, device="cuda")
             want[holes] = fills.int()
             assert torch.equal(plan.take[r, h], want), (r, h)
+
+
+# ---- edges -------------------------------------------------------------------------------------------------------
+def test_rows_far_into_large_tensors():
+    """Weights and positions past 2^31 elements and 4 GB: the last request and head of a wide state."""
+    lens = [70, 130]
+    s = Setup(lens, seed=2, page_len=64, code="int8")
+    room = 1 << 28
+    w = gqa.KeyWeights(torch.empty(2, 8, room, device="cuda"), torch.empty(2, 8, room, dtype=torch.int32, device="cuda"),
+                       ints([0, 5]))
+    for b, n in enumerate(lens):
+        w.weight[b, :, :n] = torch.rand(8, n, generator=s.gen, device="cuda")
+        w.position[b, :, :n] = torch.arange(n, device="cuda")
+    near = gqa.key_weights(2, 192)
+    near.weight[:, :, :130], near.position[:, :, :130] = w.weight[:, :, :130], w.position[:, :, :130]
+    near.evicted.copy_(w.evicted)
+    q, table, ln = s.queries(6), ints(s.table), ints(lens)
+    state = [t.clone() for t in (s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale)]
+    results = []
+    for x in (w, near):
+        for t, before in zip((s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale), state):
+            t.copy_(before)
+        out = gqa.decode_paged_weights(q[:2], s.cache, table, ln, x)
+        gqa.add_key_weights(q, s.cache, table, ln, ints([0, 4, 6]), x)
+        plan = gqa.plan_eviction(x, ln, ints([40, 100]), table, torch.zeros(9, dtype=torch.int32, device="cuda"), ints([0]),
+                                 page_len=64, max_keep=100)
+        gqa.evict_paged(s.cache, table, x, plan)
+        results.append([out, plan.take, x.evicted.clone(), s.cache.k.clone(), s.cache.v_scale.clone()] +
+                       [t[b, :, :n].clone() for t in (x.weight, x.position) for b, n in enumerate(lens)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_scores_past_4_gb():
+    """A table that could name 2^26 keys: the scores of a step's last heads lie past 4 GB of its workspace."""
+    lens = [300]
+    s = Setup(lens, seed=6, page_len=128, code="e4m3")
+    wide = torch.full((1, (1 << 26) // 128), -1, dtype=torch.int32, device="cuda")
+    wide[0, :3] = ints(s.table)[0]
+    q = s.queries(1)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        big = gqa.key_weights(1, 1 << 26)
+        a = gqa.decode_paged_weights(q, s.cache, wide, ints(lens), big)
+        small = gqa.key_weights(1, 384)
+        b = gqa.decode_paged_weights(q, s.cache, ints(s.table), ints(lens), small)
+        assert torch.equal(a, b) and torch.equal(big.weight[:, :, :384], small.weight)
+        torch.cuda.current_stream().synchronize()
+
+
+def test_calls_without_queries_or_keys():
+    lens = [0, 40, 0]
+    s = Setup(lens, seed=2, page_len=16)
+    w, q = some_weights(s, [4, 4, 4]), s.queries(3)
+    before = [t.clone() for t in (w.weight, w.position, w.evicted)]
+    table, ln = ints(s.table), ints(lens)
+    gqa.add_key_weights(q, s.cache, table, ln, ints([0, 0, 0, 0]), w)
+    gqa.add_key_weights(q[:0], s.cache, table, ln, ints([0, 0, 0, 0]), w)
+    gqa.add_key_weights(q, s.cache, table, ln, ints([0, 2, 2, 3]), w)  # queries of sequences without keys
+    for t, x in zip((w.weight, w.position, w.evicted), before):
+        assert torch.equal(t.nan_to_num(), x.nan_to_num())
+    none = ints([0, 0, 0])
+    assert not gqa.decode_paged_weights(q, s.cache, table, none, w).any()
+    for t, x in zip((w.weight, w.position, w.evicted), before):
+        assert torch.equal(t.nan_to_num(), x.nan_to_num())
+    plan = gqa.plan_eviction(w, none, ints([8, 8, 8]), table, ints([0] * 8), ints([0]), page_len=16, max_keep=8)
+    assert plan.counts.tolist() == [0, 0, 0, 0] and bool((plan.take == -1).all())
+    gqa.evict_paged(s.cache, table, w, plan)
+
+
+def test_lengths_and_queries_that_are_out_of_range():
+    """More queries than keys, a length past what the table names, rows of first_query out of order: nothing outside is
+    read or written, and what is in range is right."""
+    lens = [40, 48, 5]
+    s = Setup(lens, seed=8, page_len=16)
+    w, q = some_weights(s), s.queries(60)
+    before = w.weight.clone(), w.position.clone()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints(lens), ints([0, 3, 5, 60]), w)   # 55 queries of 5 keys
+    want = exact_weights(s, torch.cat([q[:5], q[55:60]]), [3, 2, 5], [0, 0, 0])
+    check_weights(s, w, before, want, [37, 46, 0], [0, 0, 0])
+    marked = w.weight.clone()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints([1000, 48, -7]), ints([0, 3, 5, 9]), w)
+    assert torch.equal(w.weight[2].nan_to_num(), marked[2].nan_to_num()) and bool((w.weight[0, :, :40] >= marked[0, :, :40]).all())
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints(lens), ints([70, -4, 50, 20]), w)
+    assert gqa.read_device_status() == 0
+
+
+def test_the_largest_batch():
+    lens = [1 + (b * 7) % 40 for b in range(8192)]
+    s = Setup(lens, seed=1, page_len=32, code="e4m3", heads=1)
+    w, q = some_weights(s), s.queries(8192)
+    before = w.weight.clone(), w.position.clone()
+    table, ln = ints(s.table), ints(lens)
+    gqa.decode_paged_weights(q, s.cache, table, ln, w)
+    other = some_weights(s)
+    other.weight.copy_(before[0]), other.position.copy_(before[1])
+    gqa.add_key_weights(q, s.cache, table, ln, ints(list(range(8193))), other)
+    assert torch.allclose(w.weight.nan_to_num(), other.weight.nan_to_num(), rtol=2.0 ** -14, atol=0)
+    pick = [0, 1, 4095, 8190, 8191]
+    for b in pick:
+        assert torch.allclose((w.weight[b, 0, :lens[b]] - torch.where(torch.arange(lens[b], device="cuda") < lens[b] - 1,
+                                                                       before[0][b, 0, :lens[b]], 0.0)).sum(),
+                              torch.tensor(4.0, device="cuda"), rtol=1e-4)
+    free = torch.zeros(20000, dtype=torch.int32, device="cuda")
+    plan = gqa.plan_eviction(w, ln, ints([8] * 8192), table, free, ints([0]), page_len=32, max_keep=8, sinks=1, recent=2)
+    plan.check()
+    assert plan.lens.tolist() == [min(n, 8) for n in lens]
+    assert plan.counts.tolist() == [sum(n > 8 for n in lens), sum(max(0, n - 8) for n in lens), sum(n > 32 for n in lens), 0]
+    gave = [s.table[b][1] for b in range(8192) if lens[b] > 32]
+    assert free[:len(gave)].tolist() == gave
+    gqa.evict_paged(s.cache, table, w, plan)
+    assert gqa.read_device_status() == 0
+
+
+def test_some_of_the_requests():
+    """Rows 1 and 2 of a state of 4 requests: a slice of it, of the table and of the lengths."""
+    lens = [50, 60, 70, 80]
+    s = Setup(lens, seed=7, page_len=16)
+    w, q = some_weights(s, [1, 2, 3, 4]), s.queries(2)
+    before = w.weight.clone(), w.position.clone()
+    gqa.decode_paged_weights(q, s.cache, ints(s.table)[1:3], ints(lens)[1:3], w[1:3])
+    for b in (0, 3):
+        assert torch.equal(w.weight[b].nan_to_num(), before[0][b].nan_to_num()) and torch.equal(w.position[b], before[1][b])
+    alone = gqa.KeyWeights(before[0][1:3].contiguous(), before[1][1:3].contiguous(), ints([2, 3]))
+    gqa.decode_paged_weights(q, s.cache, ints(s.table)[1:3], ints(lens)[1:3], alone)
+    assert torch.equal(alone.weight.nan_to_num(), w.weight[1:3].nan_to_num()) and torch.equal(alone.position, w.position[1:3])
+
+
+def test_two_streams_at_once():
+    """Calls on two streams have workspaces of their own."""
+    setups = [Setup([3000, 200], seed=i, page_len=64, code="int8") for i in (1, 2)]
+    states = [(s, some_weights(s), s.queries(80)) for s in setups]
+    want = []
+    for s, w, q in states:
+        copy = gqa.KeyWeights(w.weight.clone(), w.position.clone(), w.evicted.clone())
+        table, ln = ints(s.table), ints(s.lens)
+        for _ in range(5):
+            gqa.add_key_weights(q, s.cache, table, ln, ints([0, 64, 80]), copy)
+            out = gqa.decode_paged_weights(q[:2], s.cache, table, ln, copy)
+            plan = gqa.plan_eviction(copy, ln, ints([1000, 100]), table, torch.zeros(99, dtype=torch.int32, device="cuda"),
+                                     ints([0]), page_len=64, max_keep=1000)
+        want.append((copy.weight, out, plan.take))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    got = [None, None]
+    for step in range(5):
+        for i, ((s, w, q), st) in enumerate(zip(states, streams)):
+            with torch.cuda.stream(st):
+                table, ln = ints(s.table), ints(s.lens)
+                gqa.add_key_weights(q, s.cache, table, ln, ints([0, 64, 80]), w)
+                out = gqa.decode_paged_weights(q[:2], s.cache, table, ln, w)
+                plan = gqa.plan_eviction(w, ln, ints([1000, 100]), table, torch.zeros(99, dtype=torch.int32, device="cuda"),
+                                         ints([0]), page_len=64, max_keep=1000)
+                got[i] = (w.weight, out, plan.take)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x.nan_to_num(), y.nan_to_num())
+
+
+def test_c_refuses_masks_and_small_workspaces():
+    """What the Python calls do not offer: bias, documents, prefixes and positions with the keys' weights."""
+    import ctypes
+    lens = [20, 30]
+    s = Setup(lens, seed=1, page_len=16)
+    w, q = some_weights(s), s.queries(2)
+    lib, table, ln, out, first = _lib.load(), ints(s.table), ints(lens), torch.empty_like(q), ints([0, 1, 2])
+    base = dict(batch=2, rows=2, block_table=table.data_ptr(), table_stride=2, table_width=2, seq_lens=ln.data_ptr(),
+                scale=0.1, rope_theta=5e5, q_row_stride=4096, q_head_stride=128, out_row_stride=4096, out_head_stride=128)
+
+    def status(name, **change):
+        p = _lib.GqaPagedParams(**{**base, "first_query": first.data_ptr() if name == "add" else None, **change})
+        args = (q.data_ptr(), ctypes.byref(s.cache.c), ctypes.byref(p), ctypes.byref(w.c), None, None, 0, None)
+        if name == "add":
+            return lib.gqa_add_key_weights(*args)
+        return lib.gqa_decode_paged_weights(q.data_ptr(), out.data_ptr(), *args[1:4], None, 0, None)
+
+    zeros = ints([0, 0])
+    for name in ("add", "decode"):
+        for field in ("doc_starts", "prefix_ends", "slopes"):
+            assert status(name, **{field: torch.zeros(64, device="cuda").data_ptr() if field == "slopes" else zeros.data_ptr()}) \
+                == _lib.GQA_ERR_FLAGS
+        assert status(name) == _lib.GQA_ERR_WORKSPACE
+        assert status(name, table_width=3, table_stride=3) == _lib.GQA_ERR_KV_RANGE  # more keys than weights
+    assert status("decode", query_positions=zeros.data_ptr()) == _lib.GQA_ERR_FLAGS
