@@ -376,28 +376,57 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
             for (int i = (int)rank * kThreads + tid; i < a.max_keep; i += (int)ctas * kThreads) take[i] = -1;
         }
     } else if (rank == 0) {
-        // Pages that each thread's requests give, and what those before them give.
-        const int lane = tid & 31, warp = tid >> 5, gives = ok ? (int)give : 0, in_warp = warp_before(gives);
-        if (lane == 31) s.warp_sum[warp] = in_warp + gives;
-        __syncthreads();
-        int at = in_warp + __reduce_add_sync(0xffffffffu, lane < warp ? s.warp_sum[lane] : 0), cuts = 0, rows = 0;
-        for (int i = 0; i < per && ok; ++i) {
-            const int r = r0 + i;
-            const Cut c = r < r1 ? cut_of(a, r) : Cut{0, 0};
+        // As many requests at a time as there are threads: each thread its own one's first pages, the warps in turn
+        // what is left of the others.
+        constexpr int kOwn = 2;
+        const int lane = tid & 31, warp = tid >> 5;
+        int *at_of = s.hist[0], *from_of = at_of + kThreads, *left_of = from_of + kThreads;
+        static_assert(Radix<kThreads>::kBins * Radix<kThreads>::kPasses >= 3 * kThreads, "room in the histograms' place");
+        int base = n_free, cuts = 0, rows = 0;
+        for (int c0 = 0; c0 < n && ok; c0 += kThreads) {
+            const int r = c0 + tid;
+            const Cut c = r < n ? cut_of(a, r) : Cut{0, 0};
             cuts += c.keep < c.len;
             rows += c.len - c.keep;
-            // A request's pages by the whole warp, one lane's request after another's.
-            const int from = pages_of(c.keep), n_pages = pages_of(c.len) - from;
-            for (uint32_t left = __ballot_sync(0xffffffffu, n_pages > 0); left; left &= left - 1) {
-                const int who = __ffs(left) - 1, w_at = __shfl_sync(0xffffffffu, at, who);
-                const int w_n = __shfl_sync(0xffffffffu, n_pages, who), w_from = __shfl_sync(0xffffffffu, from, who);
-                const int32_t* row = a.block_table + __shfl_sync(0xffffffffu, r, who) * a.table_stride + w_from;
-                for (int j = lane; j < w_n; j += 32) a.free_pages[n_free + w_at + j] = row[j];
+            const int from = pages_of(c.keep), n_pages = pages_of(c.len) - from, in_warp = warp_before(n_pages);
+            __syncthreads();  // (the warps have read the last requests' numbers)
+            if (lane == 31) s.warp_sum[warp] = in_warp + n_pages;
+            __syncthreads();
+            int at = base + in_warp, all = 0;
+            for (int w = 0; w < kThreads / 32; ++w) {
+                const int x = s.warp_sum[w];
+                all += x;
+                if (w < warp) at += x;
             }
-            at += n_pages;
+            base += all;
+            const int32_t* row = a.block_table + r * a.table_stride + from;
+            int own[kOwn];
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) own[j] = j < n_pages ? __ldg(row + j) : 0;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j)
+                if (j < n_pages) a.free_pages[at + j] = own[j];
+            at_of[tid] = at;
+            from_of[tid] = from;
+            left_of[tid] = n_pages;
+            if (!__syncthreads_or(n_pages > kOwn)) continue;
+            for (int i = warp; i < min(kThreads, n - c0); i += kThreads / 32) {
+                const int32_t* of = a.block_table + (c0 + i) * a.table_stride + from_of[i];
+                int32_t* to = a.free_pages + at_of[i];
+                const int end = left_of[i];
+                constexpr int kAtOnce = 4;
+                for (int j0 = kOwn + lane; j0 < end; j0 += 32 * kAtOnce) {
+                    int32_t page[kAtOnce];
+#pragma unroll
+                    for (int e = 0; e < kAtOnce; ++e) page[e] = j0 + 32 * e < end ? __ldg(of + j0 + 32 * e) : 0;
+#pragma unroll
+                    for (int e = 0; e < kAtOnce; ++e)
+                        if (j0 + 32 * e < end) to[j0 + 32 * e] = page[e];
+                }
+            }
         }
-        atomicAdd(&s.cuts, cuts);
-        atomicAdd(&s.rows, rows);
+        if (cuts) atomicAdd(&s.cuts, cuts);
+        if (rows) atomicAdd(&s.rows, rows);
         __syncthreads();
         if (tid == 0) {
             a.counts[0] = s.cuts;
