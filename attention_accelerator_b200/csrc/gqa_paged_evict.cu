@@ -139,50 +139,64 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThrea
 
     for (int i = tid; i < R::kPasses * R::kBins; i += kThreads) s.hist[0][i] = 0;
     __syncthreads();
-    auto count_in = [&](int* hist, uint32_t bin, bool in) {
-        // A warp of equal numbers counts as one.
-        const uint32_t first = __shfl_sync(0xffffffffu, bin, 0);
-        if (__all_sync(0xffffffffu, in && bin == first)) {
-            if (lane == 0) atomicAdd(&hist[bin], 32);
-        } else if (in) {
-            atomicAdd(&hist[bin], 1);
+    auto count_four = [&](int* hist, const uint32_t (&bin)[4], const bool (&in)[4]) {
+        // A warp whose rows all have the same counts them as one.
+        const uint32_t first = __shfl_sync(0xffffffffu, bin[0], 0);
+        bool same = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) same &= in[e] && bin[e] == first;
+        if (__all_sync(0xffffffffu, same)) {
+            if (lane == 0) atomicAdd(&hist[first], 128);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (in[e]) atomicAdd(&hist[bin[e]], 1);
         }
     };
-    // The numbers, and the first histogram.
-    auto keep_four = [&](int i, const uint4& x) {  // (i < each)
-        if (i < a.held_rows) *reinterpret_cast<uint4*>(ranks + i) = x;
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) count_in(s.hist[0], xs[e] >> R::shift(0), i + e < n);
-    };
+    // The numbers, and the first histogram: four steps of the CTA's rows at a time, every load first.
     {
         constexpr int kAtOnce = 4;
-        int i0 = 0;
-        if (a.vectors)
-            for (; i0 + kStep * kAtOnce <= n; i0 += kStep * kAtOnce) {
-                float4 w[kAtOnce];
-                int4 p[kAtOnce];
+        const int room = (int)min(a.w.capacity - row0, (int64_t)each);  // rows that may be read
+        for (int i0 = 0; i0 < n; i0 += kStep * kAtOnce) {
+            float4 w[kAtOnce];
+            int4 p[kAtOnce];
 #pragma unroll
-                for (int e = 0; e < kAtOnce; ++e) {
-                    const int i = row0 + i0 + e * kStep + 4 * tid;
-                    w[e] = *reinterpret_cast<const float4*>(weight + i);
-                    p[e] = *reinterpret_cast<const int4*>(position + i);
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + e * kStep + 4 * tid;
+                w[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                p[e] = make_int4(0, 0, 0, 0);
+                if (i >= n) continue;
+                if (a.vectors && i + 4 <= room) {
+                    w[e] = *reinterpret_cast<const float4*>(weight + row0 + i);
+                    p[e] = *reinterpret_cast<const int4*>(position + row0 + i);
+                } else {
+                    float* we = &w[e].x;
+                    int* pe = &p[e].x;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (i + k < n) {
+                            we[k] = weight[row0 + i + k];
+                            pe[k] = position[row0 + i + k];
+                        }
                 }
-#pragma unroll
-                for (int e = 0; e < kAtOnce; ++e)
-                    keep_four(i0 + e * kStep + 4 * tid,
-                              make_uint4(rank_of(a, w[e].x, p[e].x, recent_from), rank_of(a, w[e].y, p[e].y, recent_from),
-                                         rank_of(a, w[e].z, p[e].z, recent_from), rank_of(a, w[e].w, p[e].w, recent_from)));
             }
-        for (; i0 < n; i0 += 2 * kStep) {
-            uint32_t x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = i0 + (e >> 2) * kStep + 4 * tid + (e & 3);
-                x[e] = i < n ? number(row0 + i) : 0u;
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + e * kStep + 4 * tid;
+                if (i0 + e * kStep >= n) break;
+                const float we[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+                const int pe[4] = {p[e].x, p[e].y, p[e].z, p[e].w};
+                uint32_t x[4], bin[4];
+                bool in[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    in[k] = i + k < n;
+                    x[k] = in[k] ? rank_of(a, we[k], pe[k], recent_from) : 0u;
+                    bin[k] = x[k] >> R::shift(0);
+                }
+                if (i < a.held_rows) *reinterpret_cast<uint4*>(ranks + i) = make_uint4(x[0], x[1], x[2], x[3]);
+                count_four(s.hist[0], bin, in);
             }
-            keep_four(i0 + 4 * tid, make_uint4(x[0], x[1], x[2], x[3]));
-            if (i0 + kStep < each) keep_four(i0 + kStep + 4 * tid, make_uint4(x[4], x[5], x[6], x[7]));
         }
     }
     uint32_t found = 0, known = 0;   // the number's upper bits, and which these are
@@ -197,12 +211,14 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThrea
                 const int i = i0 + 4 * tid;
                 const uint4 x = four(i);
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                uint32_t bin[4];
                 bool in[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) in[e] = i + e < n && (xs[e] & known) == found;
-                if (__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3]))
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) count_in(hist, xs[e] >> shift & mask, in[e]);
+                for (int e = 0; e < 4; ++e) {
+                    in[e] = i + e < n && (xs[e] & known) == found;
+                    bin[e] = xs[e] >> shift & mask;
+                }
+                if (__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) count_four(hist, bin, in);
             }
         all_arrive();
         // From the highest bin down: the one in which the count passes what is left.
@@ -279,11 +295,12 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThrea
             stays |= (xs[e] > found) << e;
         }
         if (__any_sync(0xffffffffu, same)) {
-            int at = tie + warp_before(__popc(same));
+            const int mine = __popc(same);
+            int at = tie + warp_before(mine);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (same >> e & 1) stays |= ((uint32_t)at++ < left) << e;
-            tie += __reduce_add_sync(0xffffffffu, __popc(same));
+            tie += __reduce_add_sync(0xffffffffu, mine);
         }
         const uint32_t low = (1u << min(4, max(0, keep - row0 - i))) - 1, rows = (1u << min(4, max(0, w1 - i))) - 1;
         return ((stays & ~low) | (~stays & low)) & rows;
@@ -321,10 +338,11 @@ __device__ __forceinline__ void choose(const EvictPlanArgs& a, PlanShared<kThrea
         for (int e = 0; e < 4; ++e)
             if (low >> e & 1 && i + e < w1) take[row0 + i + e] = -1;
         if (!__any_sync(0xffffffffu, m)) continue;
-        const int n_low = __popc(m & low), n_high = __popc(m & ~low);
-        int hole = at_hole + warp_before(n_low), fill = at_fill + warp_before(n_high);
-        at_hole += __reduce_add_sync(0xffffffffu, n_low);
-        at_fill += __reduce_add_sync(0xffffffffu, n_high);
+        const int both = __popc(m & low) | __popc(m & ~low) << 16, before = warp_before(both);  // (128 of each at most)
+        int hole = at_hole + (before & 0xffff), fill = at_fill + (before >> 16);
+        const int all_of = __reduce_add_sync(0xffffffffu, both);
+        at_hole += all_of & 0xffff;
+        at_fill += all_of >> 16;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (m >> e & 1) {
