@@ -480,12 +480,12 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
 // ---------------------------------------------------------------------------
 // The move.
 //
-// A warp a block (page and head, of K or of V) that rows move into: their largest
-// magnitude, the block's new scale, their codes, and where the scale grew the other
-// rows' codes again.  Rows come from past the new length and go below it, so that
-// blocks are independent -- but for the page in which the new length ends, which
-// rows leave and enter: the blocks of these pages are a launch of their own, behind
-// the others.
+// A warp 32 rows of a block (page and head, of K or of V) that rows move into, eight
+// warps a CTA: what moves in stays in registers between its largest magnitude and its
+// new codes; where the block's scale grew the other rows' codes are rounded again.
+// Rows come from past the new length and go below it, so that blocks are independent
+// -- but for the page in which the new length ends, which rows leave and enter: the
+// blocks of these pages are a launch of their own, behind the others.
 // ---------------------------------------------------------------------------
 struct EvictArgs {
     PagedCacheView c;
@@ -539,48 +539,53 @@ __device__ __forceinline__ void values4(uint32_t w, float (&x)[4]) {
     }
 }
 
-constexpr int kHeldRows = 8;  // rows of a lane that stay in registers between the two passes
+constexpr int kEvictWarps = 8, kWarpRows = 32, kHeldRows = kWarpRows / 4;  // (rows of a lane)
 
 template <int kCode>
-__global__ void __launch_bounds__(256, 4) evict_kernel(const __grid_constant__ EvictArgs a) {
-    __shared__ int2 s_moves[kNumKVHeads][kPagedMaxPage];
+__global__ void __launch_bounds__(32 * kEvictWarps, 4) evict_kernel(const __grid_constant__ EvictArgs a) {
+    __shared__ int2 s_moves[kEvictWarps][kWarpRows];
+    __shared__ uint2 s_top[kEvictWarps];
     dependency_wait();
     allow_dependents();
-    const int lane = threadIdx.x & 31, h = threadIdx.x >> 5, r = blockIdx.y, sub = lane >> 3, chunk = lane & 7;
-    const bool is_k = blockIdx.z == 0;
-    const int shift = a.c.page_shift, page_len = a.c.page_len, len = a.lens[r], end = len >> shift;
-    const int column = a.last_pages ? end : blockIdx.x;
-    if (len <= 0 || column >= a.table_width || (a.last_pages ? (len & (page_len - 1)) == 0 : column >= end)) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y, sub = lane >> 3, chunk = lane & 7;
+    const int shift = a.c.page_shift, page_len = a.c.page_len;
+    // Warps of a block, and this one's head and rows.
+    const int split = max(1, page_len / kWarpRows), group = warp / split, row0 = (warp - group * split) * kWarpRows;
+    const int h = (blockIdx.z >> 1) * (kEvictWarps / split) + group;
+    const bool is_k = (blockIdx.z & 1) == 0;
+    if (h >= a.c.kv_heads) return;
+    // Length, page and rows are asked for together where the column is known before the length.
+    const int len = a.lens[r], end = len >> shift;
+    const int column = a.last_pages ? max(end, 0) : blockIdx.x;
+    if (a.last_pages && (len <= 0 || column >= a.table_width || (len & (page_len - 1)) == 0)) return;
     const int32_t* table = a.block_table + r * a.table_stride;
     const int page = table[column];
-    if (page < 0 || page >= a.c.pages) return;
     const int64_t unit = (int64_t)r * a.c.kv_heads + h;
     const int32_t* take = a.take + unit * a.max_keep;
-    int2* moves = s_moves[h];  // (row of this page, row of the request)
-    int n = 0;
-    uint32_t moved[kPagedMaxPage / 32];
-#pragma unroll
-    for (int i = 0; i < kPagedMaxPage / 32; ++i) {
-        const int row = 32 * i + lane;
+    int2* moves = s_moves[warp];  // (row of this page, row of the request)
+    uint32_t moved;
+    {
+        const int row = row0 + lane;
         const int64_t to = ((int64_t)column << shift) + row;
         int from = -1;
-        if (row < page_len && to < a.max_keep && to < len) from = take[to];
+        if (row < page_len && to < a.max_keep) from = take[to];
+        if (len <= 0 || (!a.last_pages && column >= end) || page < 0 || page >= a.c.pages || to >= len) from = -1;
         if (from < len || from >= (int64_t)a.table_width << shift) from = -1;
-        moved[i] = __ballot_sync(0xffffffffu, from >= 0);
-        if (from >= 0) moves[n + __popc(moved[i] & ((1u << lane) - 1))] = make_int2(row, from);
-        n += __popc(moved[i]);
+        moved = __ballot_sync(0xffffffffu, from >= 0);
+        if (from >= 0) moves[__popc(moved & ((1u << lane) - 1))] = make_int2(row, from);
     }
-    if (n == 0) return;
+    const int n = __popc(moved);
+    // The block's warps go on together, if a row moves into any of them.
+    if (!(split > 1 ? named_barrier_or(1 + group, 32 * split, n > 0) : n > 0)) return;
     __syncwarp();
-    if (is_k)
-        for (int i = lane; i < n; i += 32) {
-            const int64_t to = unit * a.w.capacity + ((int64_t)column << shift) + moves[i].x;
-            const int64_t from = unit * a.w.capacity + moves[i].y;
-            if (moves[i].y < a.w.capacity) {
-                a.w.weight[to] = a.w.weight[from];
-                a.w.position[to] = a.w.position[from];
-            }
+    if (is_k && lane < n) {
+        const int64_t to = unit * a.w.capacity + ((int64_t)column << shift) + moves[lane].x;
+        const int64_t from = unit * a.w.capacity + moves[lane].y;
+        if (moves[lane].y < a.w.capacity) {
+            a.w.weight[to] = a.w.weight[from];
+            a.w.position[to] = a.w.position[from];
         }
+    }
     uint8_t* codes = (is_k ? a.c.k : a.c.v) + h * a.c.head_stride + 16 * chunk;
     float* scales = (is_k ? a.c.k_scale : a.c.v_scale) + h;
     const float qmax = kCode == GQA_CODE_INT8 ? 127.f : 448.f;
@@ -626,11 +631,22 @@ __global__ void __launch_bounds__(256, 4) evict_kernel(const __grid_constant__ E
 #pragma unroll
     for (int i = 0; i < kHeldRows; ++i)
         if (4 * i + sub < n) measure(held[i]);
-    for (int i = 4 * kHeldRows + sub; i < n; i += 4) measure(load(i));
-    const uint32_t top = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(most) : 0x7f800000u);
+    uint32_t top = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(most) : 0x7f800000u);
     if (__float_as_uint(most) != top) most_rest = -INFINITY;
 #pragma unroll
     for (int d = 16; d; d >>= 1) most_rest = fmaxf(most_rest, __shfl_xor_sync(0xffffffffu, most_rest, d));
+    if (split > 1) {
+        if (lane == 0) s_top[warp] = make_uint2(top, __float_as_uint(most_rest));
+        // (Also: every warp of the block has read its rows, wherever they come from, and the old scale.)
+        named_barrier_sync(1 + group, 32 * split);
+        for (int w = group * split; w < (group + 1) * split; ++w) {
+            const uint2 x = s_top[w];
+            if (x.x > top || (x.x == top && __uint_as_float(x.y) > most_rest)) {
+                top = x.x;
+                most_rest = __uint_as_float(x.y);
+            }
+        }
+    }
     const BlockScale scale = moved_scale(top, most_rest, qmax, old);
     const bool number = scale.value == scale.value;
     auto codes16 = [&](const uint4& w, float s) {
@@ -656,15 +672,14 @@ __global__ void __launch_bounds__(256, 4) evict_kernel(const __grid_constant__ E
 #pragma unroll
     for (int i = 0; i < kHeldRows; ++i)
         if (4 * i + sub < n) store(4 * i + sub, held[i]);
-    for (int i = 4 * kHeldRows + sub; i < n; i += 4) store(i, load(i));
     __syncwarp();  // rows of this very page have been read, and the old scale
     if (scale.grew)
-        for (int row = sub; row < page_len; row += 4) {
-            if (moved[row >> 5] >> (row & 31) & 1) continue;
+        for (int row = row0 + sub; row < min(page_len, row0 + kWarpRows); row += 4) {
+            if (moved >> (row - row0) & 1) continue;
             uint4* at = reinterpret_cast<uint4*>(block + row * a.c.row_stride);
             *at = codes16(*at, old);
         }
-    if (lane == 0) scales[page * a.c.scale_page_stride] = scale.value;
+    if (lane == 0 && row0 == 0) scales[page * a.c.scale_page_stride] = scale.value;
 }
 
 // How many CTAs a (request, head) gets goes by the rows that it may hold (its lengths are in device memory): stretches
@@ -813,12 +828,14 @@ int gqa_evict_paged(const gqa_paged_cache* cache, const int32_t* block_table, in
     a.table_width = table_width;
     a.max_keep = max_keep;
     const int columns = (max_keep + cache->page_len - 1) / cache->page_len;
+    const int heads = kEvictWarps / (cache->page_len > kWarpRows ? cache->page_len / kWarpRows : 1);  // of a CTA
+    const int groups = (cache->kv_heads + heads - 1) / heads;
     const auto kernel = cache->code == GQA_CODE_INT8 ? evict_kernel<GQA_CODE_INT8> : evict_kernel<GQA_CODE_E4M3>;
     cudaError_t e = cudaSuccess;
     for (int last = 0; last < 2 && e == cudaSuccess; ++last) {
         a.last_pages = last != 0;
-        e = launch_dependent(kernel, dim3(last ? 1 : columns < table_width ? columns : table_width, requests, 2),
-                             32 * cache->kv_heads, 0, static_cast<cudaStream_t>(stream), a);
+        e = launch_dependent(kernel, dim3(last ? 1 : columns < table_width ? columns : table_width, requests, 2 * groups),
+                             32 * kEvictWarps, 0, static_cast<cudaStream_t>(stream), a);
     }
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
