@@ -474,7 +474,7 @@ const char* gqa_status_string(int status) {
         case GQA_ERR_FLAGS: return "gqa_params.flags holds a bit this entry point does not support";
         case GQA_ERR_MEMORY: return "a tensor, table or workspace pointer is not memory of the current GPU";
         case GQA_ERR_KV_HEADS: return "KV-head range is empty or outside [0, 8)";
-        case GQA_ERR_PAGES: return "page planning refused: too few free pages, a block-table row too short, more new tokens than max_tokens, or a length out of range";
+        case GQA_ERR_PAGES: return "page planning refused: too few free pages, a block-table row too short, more new tokens than max_tokens, no room on the stack of free pages, or a length out of range";
         default: return "unknown status";
     }
 }

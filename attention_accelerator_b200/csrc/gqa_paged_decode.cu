@@ -94,8 +94,13 @@ struct alignas(16) Shared {
     int sum[kThreads / 32];
 };
 
-// What a kernel does beside the plain call: kDiff joins Q heads 2 j and 2 j + 1 to one
-// row; kScores leaves every score (log2 units) and the rows' sums for the keys' weights.
+// What a kernel does beside the plain call.
+// kDiff joins Q heads 2 j and 2 j + 1 to one row: the second head's finisher hands its
+// normalised row over in shared memory (a unit within the share), or the last warp of
+// both heads to arrive merges both (a unit that crosses shares).  64 ragged sequences
+// 97 to 99 us, one of 30 keys 5.8 us: as without it.
+// kScores leaves every score (log2 units, 16 bytes a key and KV head) and the rows' sums
+// for the keys' weights: 64 ragged sequences (int8) 99 -> 107 us.
 enum Mode { kPlain, kDiff, kScores };
 
 struct alignas(64) DecodePagedArgs {

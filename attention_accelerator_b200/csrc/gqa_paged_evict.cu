@@ -22,6 +22,10 @@ namespace {
 // number stay.  Two more count, a warp a stretch of rows, a lane four rows, what is equal
 // to it and then the holes below `keep` and the rows past it that stay; the last lists
 // both in order, and they are paired off.  One more CTA gives the pages back.
+//
+// Bound by the chain of loads, votes and barriers between the passes, not by the 8 bytes
+// a row: 64 requests of 1025 rows and 8 heads 11.5 us, 8 of up to 32768 26 us (64 clusters
+// of 4), one of 131072 28 us, 64 of up to 8192 35 us (replayed graph).
 // ---------------------------------------------------------------------------
 constexpr int kMaxCluster = 8;
 constexpr int kMaxRows = 48 * 1024;  // of a CTA in shared memory; numbers of rows past that are computed again
@@ -486,6 +490,10 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
 // Rows come from past the new length and go below it, so that blocks are independent
 // -- but for the page in which the new length ends, which rows leave and enter: the
 // blocks of these pages are a launch of their own, behind the others.
+//
+// Bound by the latency of take -> table -> codes and scale -> store: 8 prompts of up to
+// 16384 rows to 2000 (57 MB) 20.7 us in pages of 32, 21 of 64, 26 of 128 (int8); 64
+// requests of 272 rows to 257 11.8 us, two launches.
 // ---------------------------------------------------------------------------
 struct EvictArgs {
     PagedCacheView c;

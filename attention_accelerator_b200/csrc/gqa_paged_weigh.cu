@@ -22,6 +22,16 @@
 // row's largest below 1, is split into two FP16 parts (22 bits), both products
 // accumulate in the same FP32 columns; codes are exact.
 //
+// Bound: a tile of 128 keys for a unit takes 2048 cycles of the tensor pipe (two parts of
+// Q) and 2048 of the special-function unit in each pass; overlapped they come to 3100
+// (rows: S has one place for each M tile, the queries' parts take the other half of TMEM)
+// and 3900 (keys).  Measured (B200): the last 64 queries of 8 prompts of up to 16384 keys,
+// e4m3, 193 to 213 us (10 + 93 + 110 for the three kernels), 32 queries 138, 5 queries
+// 119; 6 ragged prompts of up to 2051 tokens, every query, int8, cap 50, 407 us (43 + 148
+// + 235: in the keys' pass a run has few tiles, and the queries' 128 KB are loaded for
+// each).  score_weights_kernel: 64 ragged sequences (2.3 M keys and heads, 90 MB, mostly
+// from L2) 11 us.
+//
 // Warps of weigh_kernel (one CTA per SM; shares of even cost, from the lengths in device
 // memory, which every CTA sums itself):
 //   0-15      sums, four groups of four: a thread a row and half of the tile's keys (rows: two
