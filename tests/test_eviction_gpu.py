@@ -771,3 +771,89 @@ def test_c_refuses_masks_and_small_workspaces():
         assert status(name) == _lib.GQA_ERR_WORKSPACE
         assert status(name, table_width=3, table_stride=3) == _lib.GQA_ERR_KV_RANGE  # more keys than weights
     assert status("decode", query_positions=zeros.data_ptr()) == _lib.GQA_ERR_FLAGS
+
+
+@pytest.mark.parametrize("counts,lens,known", [([200, 130, 70], [500, 130, 300], [0, 0, 0]), ([200, 130, 70], [500, 130, 300], [100, 60, 300])])
+def test_known_rows_of_many_units(counts, lens, known):
+    s = Setup(lens, seed=4, page_len=16, code="e4m3")
+    w, q = some_weights(s, [9, 9, 9]), s.queries(sum(counts))
+    before = w.weight.clone(), w.position.clone()
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints(lens), ints(first), w, known=ints(known))
+    now = [0 if k <= 0 else 9 for k in known]
+    assert w.evicted.tolist() == now
+    check_weights(s, w, before, exact_weights(s, q, counts, now), known, now)
+
+
+@pytest.mark.parametrize("cap", [1e-38, 1e-3, 30.0, 1e5, 3e38])
+@pytest.mark.parametrize("rotated", [False, True])
+def test_caps_of_any_size(cap, rotated):
+    """Far below the scores every visible key weighs the same; far above them the cap changes nothing."""
+    lens, counts = [130, 64], [70, 1]
+    s = Setup(lens, seed=4, page_len=64, code="int8")
+    q = s.queries(71)
+    # (Of a cap of 1e5 and more the scores' own rounding is all there is: the bound's cap is what is left of it.)
+    near = cap if 1e-3 < cap < 1e4 else 0.0
+    for call in ("add", "decode"):
+        w = some_weights(s)
+        before = w.weight.clone(), w.position.clone()
+        rows, n = (q, counts) if call == "add" else (q[:2], [1, 1])
+        more = dict(score_cap=cap, q_rotated=rotated)
+        if call == "add":
+            gqa.add_key_weights(rows, s.cache, ints(s.table), ints(lens), ints([0, 70, 71]), w, **more)
+        else:
+            gqa.decode_paged_weights(rows, s.cache, ints(s.table), ints(lens), w, **more)
+        if cap <= 1e-3:   # tanh is 1 or -1 for all scores but the smallest; all weights within 2 cap of one another
+            for b, (length, c) in enumerate(zip(lens, n)):
+                vis = (torch.arange(length - c, length)[:, None] >= torch.arange(length)[None]).double()
+                want = 4 * (vis / vis.sum(-1, keepdim=True)).sum(0).cuda()
+                start = torch.where(torch.arange(length, device="cuda") < length - c, before[0][b, :, :length].double(), 0.0)
+                assert bool(((w.weight[b, :, :length].double() - start - want).abs() <= (math.expm1(2 * cap) + 2.0 ** -18) * want
+                             + 2.0 ** -23 * (start + want)).all())
+        else:
+            check_weights(s, w, before, exact_weights(s, rows, n, [0, 0], near, q_rotated=rotated),
+                          [x - c for x, c in zip(lens, n)], [0, 0])
+
+
+FRESH = """
+import torch, attention_accelerator_b200 as gqa
+dev = torch.device("cuda", 0)
+i32 = dict(dtype=torch.int32, device=dev)
+cache = gqa.paged_cache(20, 32, dtype=torch.int8)
+cache.k.random_(-127, 127), cache.v.random_(-127, 127), cache.k_scale.fill_(0.01), cache.v_scale.fill_(0.01)
+table, lens = torch.arange(20, **i32).view(2, 10), torch.tensor([300, 200], **i32)
+w = gqa.key_weights(2, 320)
+q, first, keep = torch.randn(40, 32, 128, device=dev).bfloat16(), torch.tensor([0, 30, 40], **i32), torch.tensor([100, 150], **i32)
+free, n_free, lam = torch.zeros(20, **i32), torch.zeros(1, **i32), torch.rand(16, device=dev)
+def step():
+    gqa.add_key_weights(q, cache, table, lens, first, w)
+    out = gqa.decode_paged_weights(q[:2], cache, table, lens, w)
+    d = gqa.decode_paged_diff(q[:2], cache, table, lens, lam)
+    c = gqa.decode_paged_diff_chunked(q, cache, table, lens, first, lam)
+    plan = gqa.plan_eviction(w, lens, keep, table, free, n_free, page_len=32, max_keep=150)
+    gqa.evict_paged(cache, table, w, plan)
+    return out, d, c, plan.take
+state = [cache.k, cache.v, cache.k_scale, cache.v_scale, w.weight, w.position, w.evicted]
+start = [t.clone() for t in state]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+for t, x in zip(state, start):
+    t.copy_(x)
+for a, b in zip(got, step()):
+    assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+print("equal")
+"""
+
+
+def test_a_fresh_process_captures_without_a_warm_up():
+    """Every kernel's first launch is a capture's."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    res = subprocess.run([sys.executable, "-c", FRESH], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "equal" in res.stdout, res.stdout + res.stderr
