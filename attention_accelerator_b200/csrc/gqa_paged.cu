@@ -873,8 +873,9 @@ size_t gqa_key_weights_workspace_bytes(const gqa_paged_cache* cache, const gqa_p
         return 0;
     int sms = 0;
     if (device_sms(&sms) != GQA_OK) return 0;
-    return p->first_query ? paged_weigh_workspace(p->batch, p->rows, cache->kv_heads, sms)
-                          : score_regions(p->batch, cache->kv_heads, (int64_t)p->table_width * cache->page_len, sms).end;
+    const int64_t keys = (int64_t)p->table_width * cache->page_len;
+    return p->first_query ? paged_weigh_workspace(p->batch, p->rows, cache->kv_heads, keys, sms)
+                          : score_regions(p->batch, cache->kv_heads, keys, sms).end;
 }
 
 int gqa_decode_paged_weights(const void* q, void* out, const gqa_paged_cache* cache, const gqa_paged_params* p,
@@ -919,7 +920,9 @@ int gqa_add_key_weights(const void* q, const gqa_paged_cache* cache, const gqa_p
     int sms = 0;
     st = paged_attention_sms(&sms, PagedKernels::kWeights);
     if (st != GQA_OK) return st;
-    if (workspace_bytes < paged_weigh_workspace(call.batch, call.rows, call.c.kv_heads, sms)) return GQA_ERR_WORKSPACE;
+    if (workspace_bytes < paged_weigh_workspace(call.batch, call.rows, call.c.kv_heads,
+                                                (int64_t)call.table_width << call.c.page_shift, sms))
+        return GQA_ERR_WORKSPACE;
     st = check_device_memory({workspace});
     if (st != GQA_OK) return st;
     if (call.rows == 0) return GQA_OK;

@@ -55,7 +55,7 @@ cudaError_t launch_score_weights(const PagedCall& call, const PagedScores& score
 
 // The weights of any number of queries (gqa_paged_weigh.cu).
 int paged_weigh_box();
-size_t paged_weigh_workspace(int batch, int rows, int heads, int sms);
+size_t paged_weigh_workspace(int batch, int rows, int heads, int64_t keys, int sms);
 cudaError_t launch_paged_weigh(const PagedCall& call, const RopeSteps& rope, int code, const CUtensorMap& kmap,
                                const KeyWeightsView& weights, const int32_t* known, int sms, uint8_t* ws,
                                cudaStream_t stream);

@@ -785,6 +785,39 @@ def test_known_rows_of_many_units(counts, lens, known):
     check_weights(s, w, before, exact_weights(s, q, counts, now), known, now)
 
 
+@pytest.mark.parametrize("lens,counts,heads", [([2600, 700, 64, 1, 129], [2600, 700, 64, 1, 129], 8),
+                                               ([3000, 40000], [65, 70], 1), ([300] * 40, [300] * 40, 2)])
+def test_units_of_many_shares(lens, counts, heads):
+    """Sums of several units share by share, in both of their layouts, beside sequences of one unit."""
+    s = Setup(lens, seed=6, page_len=64, code="int8", heads=heads)
+    w, q = some_weights(s), s.queries(sum(counts))
+    before = w.weight.clone(), w.position.clone()
+    first = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    for turn in range(2):   # the second finds the first's sums in the workspace
+        for t, x in zip((w.weight, w.position), before):
+            t.copy_(x)
+        gqa.add_key_weights(q, s.cache, ints(s.table), ints(lens), ints(first), w)
+        check_weights(s, w, before, exact_weights(s, q, counts, [0] * len(lens)), [n - c for n, c in zip(lens, counts)],
+                      [0] * len(lens))
+
+
+def test_queries_that_several_sequences_claim():
+    """Numbers of first queries that fall: the weights are anything, the call ends, and the next one is right."""
+    lens = [700, 800, 900, 700, 800, 900]
+    s = Setup(lens, seed=8, page_len=16, code="e4m3")
+    w, q = some_weights(s), s.queries(600)
+    guard = w.weight.clone()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints(lens), ints([0, 600, 0, 600, -5, 700, 600]), w)
+    assert gqa.read_device_status() == 0
+    for b, n in enumerate(lens):
+        assert torch.equal(w.weight[b, :, n:].nan_to_num(), guard[b, :, n:].nan_to_num())
+    counts = [100] * 6
+    w = some_weights(s)
+    before = w.weight.clone(), w.position.clone()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints(lens), ints(range(0, 601, 100)), w)
+    check_weights(s, w, before, exact_weights(s, q, counts, [0] * 6), [n - 100 for n in lens], [0] * 6)
+
+
 @pytest.mark.parametrize("cap", [1e-38, 1e-3, 30.0, 1e5, 3e38])
 @pytest.mark.parametrize("rotated", [False, True])
 def test_caps_of_any_size(cap, rotated):
