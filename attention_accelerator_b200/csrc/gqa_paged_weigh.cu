@@ -1097,10 +1097,8 @@ struct JoinArgs {
 
 constexpr int kJoined = 4;  // shares at a time
 
-__global__ void __launch_bounds__(kScoreThreads) join_sums_kernel(const __grid_constant__ JoinArgs a) {
-    dependency_wait();
-    allow_dependents();
-    const int heads = a.p.c.kv_heads, unit = blockIdx.x, b = unit / heads;
+__device__ __forceinline__ void join_sums(const JoinArgs& a, int unit) {
+    const int heads = a.p.c.kv_heads, b = unit / heads;
     const Seq q(a.p, b);
     if (q.units < 2) return;
     const int known = known_of(a.known, b, q), evicted = known > 0 ? paged_evicted(a.p, b) : 0;
@@ -1109,7 +1107,7 @@ __global__ void __launch_bounds__(kScoreThreads) join_sums_kernel(const __grid_c
     for (int64_t key = (int64_t)blockIdx.y * kScoreThreads + threadIdx.x; key < q.len; key += (int64_t)gridDim.y * kScoreThreads) {
         const int tile = (int)(key >> kTileShift);
         float w = key < known ? a.w.weight[at + key] : 0.f;
-        // (Loads of several shares at a time: 10.8 us without, for 6 prompts of up to 2051 keys, 8 heads.)
+        // (Several shares' loads at a time: 7.3 us for 6 prompts of up to 2051 keys and 8 heads, one by one 10.8.)
         for (int c0 = shares.x; c0 <= shares.y; c0 += kJoined) {
             Piece piece[kJoined];
             float2 part[kJoined];
@@ -1134,6 +1132,19 @@ __global__ void __launch_bounds__(kScoreThreads) join_sums_kernel(const __grid_c
         a.w.weight[at + key] = w;
         if (key >= known) a.w.position[at + key] = (int)key + evicted;
         if (key == 0 && known <= 0 && unit == b * heads) a.w.evicted[b] = 0;
+    }
+}
+
+// A block's units are every gridDim.x-th.
+__global__ void __launch_bounds__(kScoreThreads) join_sums_kernel(const __grid_constant__ JoinArgs a) {
+    dependency_wait();
+    allow_dependents();
+    const int all = a.p.batch * a.p.c.kv_heads, step = gridDim.x;
+    for (int first = blockIdx.x; first < all; first += step * kScoreThreads) {
+        const int end = min(all, first + step * kScoreThreads), mine = first + (int)threadIdx.x * step;
+        // Where there are many, mostly of one query, the threads look at one each first.
+        if (all > step && !__syncthreads_or(mine < end && Seq(a.p, mine / a.p.c.kv_heads).units > 1)) continue;
+        for (int unit = first; unit < end; unit += step) join_sums(a, unit);
     }
 }
 
@@ -1244,7 +1255,7 @@ cudaError_t launch_paged_weigh(const PagedCall& call, const RopeSteps& rope, int
         const JoinArgs join{call, weights, known, a.pieces, a.shares_of, a.sums, a.sum_rows};
         const int heads = call.batch * call.c.kv_heads;
         const int64_t most = (keys + kScoreThreads - 1) / kScoreThreads, want = ((int64_t)sms * 8 + heads - 1) / heads;
-        e = launch_dependent(join_sums_kernel, dim3(heads, (unsigned)(want < most ? want : most)), kScoreThreads, 0, stream, join);
+        e = launch_dependent(join_sums_kernel, dim3(heads < 8 * sms ? heads : 8 * sms, (unsigned)(want < most ? want : most)), kScoreThreads, 0, stream, join);
     }
     return e;
 }
