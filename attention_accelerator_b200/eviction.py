@@ -16,7 +16,8 @@ next token has row ``lens[r]`` and position ``lens[r] + weights.evicted[r]``: ap
 (``append_paged(..., positions=...)``); ``decode_paged_weights`` and ``add_key_weights`` place their queries so by
 themselves, ``decode_paged`` takes ``query_positions``, and ``decode_paged_chunked`` queries that were rotated before
 (``q_rotated``).  Distance bias, document and prefix masks go by rows and no longer apply.  The pages of a request that is
-cut must be its own.  As with the other paged calls every length is in device memory and no call waits for the GPU.
+cut must be its own.  As with the other paged calls every length is in device memory, no call waits for the GPU, and a
+captured graph keeps the workspace of the stream that it was captured on.
 """
 from __future__ import annotations
 

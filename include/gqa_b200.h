@@ -665,8 +665,11 @@ typedef struct gqa_key_weights {
     int64_t capacity;   /* rows: at least table_width * page_len, at most 2^30 */
 } gqa_key_weights;
 
-/* Device workspace of either call below (0 on invalid input), as gqa_paged_workspace_bytes's: it serves those
- * calls as well.  One token a sequence: 16 bytes for each key that the table could name and KV head. */
+/* Device workspace of either call below (0 on invalid input), under the rules of gqa_paged_workspace_bytes's; one
+ * that is as large as both ask serves those calls as well.  One token a sequence (first_query NULL): 16 bytes for
+ * each key that the table could name and KV head.  Else 136 KB for 64 queries and KV head, and with more than 64
+ * rows in all the sums that thread blocks leave: at most 8 bytes for each key that the table could name, KV head
+ * and sequence, and 1.2 KB for each key of one sequence. */
 size_t gqa_key_weights_workspace_bytes(const gqa_paged_cache *cache, const gqa_paged_params *p);
 
 /*
@@ -676,7 +679,9 @@ size_t gqa_key_weights_workspace_bytes(const gqa_paged_cache *cache, const gqa_p
  * The last row is the query's own token: position[b][h][seq_len - 1] = seq_len - 1 +
  * evicted[b], where the query stands too (query_positions is NULL; a sequence of one
  * row is a new one, its evicted[b] becomes 0).  doc_starts, prefix_ends and slopes
- * are NULL.  FP32 throughout, no atomics: results do not depend on timing.
+ * are NULL.  FP32 throughout, no atomics: results do not depend on timing.  A Q head
+ * that is no number, or sees a page whose scale (K's or V's) is none, gives every key
+ * that it sees a weight of NaN, which stays until the row is evicted or new.
  */
 int gqa_decode_paged_weights(const void *q, void *out, const gqa_paged_cache *cache, const gqa_paged_params *p,
                              const gqa_key_weights *weights, void *workspace, size_t workspace_bytes, void *stream);
@@ -689,7 +694,7 @@ int gqa_decode_paged_weights(const void *q, void *out, const gqa_paged_cache *ca
  * first query's row on) are new: their weight starts at 0 and their position is row +
  * evicted[b]; where known[b] is 0 or less the sequence is a new one, and evicted[b]
  * becomes 0.  Sequences without queries are left as they are.  `out` strides of `p`
- * are not used.
+ * are not used.  What is no number spreads as above (V is not read).
  */
 int gqa_add_key_weights(const void *q, const gqa_paged_cache *cache, const gqa_paged_params *p,
                         const gqa_key_weights *weights, const int32_t *known, void *workspace, size_t workspace_bytes,

@@ -191,6 +191,35 @@ def test_a_page_scale_or_query_that_is_no_number_stays_with_its_own():
     assert bool(w.weight[1, 5, 199].isfinite()) and bool(w.weight[1, 5, :199].isnan().all())
 
 
+@pytest.mark.parametrize("which", ["k_scale", "v_scale", "query"])
+def test_a_decode_step_of_what_is_no_number(which):
+    """Every key of that sequence and head has a weight of NaN, no other one has; the plan takes them in order."""
+    lens = [300, 200, 7]
+    s = Setup(lens, seed=3, page_len=64, code="e4m3")
+    q = s.queries(3)
+    clean, w = some_weights(s), some_weights(s)
+    w.weight.copy_(clean.weight)
+    gqa.decode_paged_weights(q, s.cache, ints(s.table), ints(lens), clean)
+    if which == "query":
+        q[0, 4 * 2 + 3, 70] = math.nan
+    else:
+        getattr(s.cache, which)[s.table[0][1], 2] = math.nan
+    gqa.decode_paged_weights(q, s.cache, ints(s.table), ints(lens), w)
+    for b, n in enumerate(lens):
+        for h in range(8):
+            if (b, h) == (0, 2):
+                assert bool(w.weight[b, h, :n].isnan().all())
+            else:
+                assert torch.equal(w.weight[b, h, :n], clean.weight[b, h, :n]), (b, h)
+    free = torch.zeros(64, dtype=torch.int32, device="cuda")
+    plan = gqa.plan_eviction(w, ints(lens), ints([50, 0, 0]), ints(s.table), free, ints([0]), page_len=64, max_keep=50, sinks=0,
+                             recent=0)
+    plan.check()
+    take = ref.plan_eviction(w.weight.cpu().numpy(), w.position.cpu().numpy(), lens, [0, 0, 0], [50, 0, 0], s.table, [], 64, 64,
+                             max_keep=50, sinks=0, recent=0)[1]
+    assert np.array_equal(plan.take.cpu().numpy(), take) and plan.lens.tolist() == [50, 200, 7]
+
+
 def test_a_huge_query_costs_its_neighbours_nothing():
     """Rows of one unit have factors of their own: one of 2^60 beside ordinary ones."""
     lens = [200]
