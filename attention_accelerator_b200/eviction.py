@@ -180,9 +180,12 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
     i32 = torch.int32
     if evicted_out is None and lens_out is lens:
         evicted_out = weights.evicted
-    take = lens.new_empty((n, heads, max_keep), dtype=i32)
+    lens_ptr = _need("lens", lens, i32, (n,), device)
+    given = [_need("lens_out", lens_out, i32, (n,), device), _need("evicted_out", evicted_out, i32, (n,), device),
+             _need("n_free_out", n_free_out, i32, (1,), device)]
+    take = lens.new_empty((n, heads, max_keep))
     room = [n if lens_out is None else 0, n if evicted_out is None else 0, 1 if n_free_out is None else 0, 4]
-    new_lens, new_evicted, new_n_free, counts = lens.new_empty(sum(room), dtype=i32).split_with_sizes(room)
+    new_lens, new_evicted, new_n_free, counts = lens.new_empty(sum(room)).split_with_sizes(room)
     lens_out = new_lens if lens_out is None else lens_out
     evicted_out = new_evicted if evicted_out is None else evicted_out
     n_free_out = new_n_free if n_free_out is None else n_free_out
@@ -190,12 +193,12 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
     nbytes = lib.gqa_plan_eviction_workspace_bytes(n, heads, max_keep)
     ws = api._workspace(device, ("eviction", stream), nbytes)
     _check(lib.gqa_plan_eviction(
-        ctypes.byref(weights.c), heads, _need("lens", lens, i32, (n,), device),
-        _need("keep", keep, i32, (n,), device), n, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        _need("free_pages", free_pages, i32, tuple(free_pages.shape), device), free_pages.shape[0],
+        ctypes.byref(weights.c), heads, lens_ptr, _need("keep", keep, i32, (n,), device), n, block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1],
+        _need("free_pages", free_pages, i32, free_pages.shape, device), free_pages.shape[0],
         _need("n_free", n_free, i32, (1,), device), page_len, max_keep, sinks, recent, take.data_ptr(),
-        _need("lens_out", lens_out, i32, (n,), device), _need("evicted_out", evicted_out, i32, (n,), device),
-        _need("n_free_out", n_free_out, i32, (1,), device), counts.data_ptr(), ws.data_ptr(), ws.numel(), stream),
+        given[0] or lens_out.data_ptr(), given[1] or evicted_out.data_ptr(), given[2] or n_free_out.data_ptr(),
+        counts.data_ptr(), ws.data_ptr(), ws.numel(), stream),
         "plan_eviction")
     return EvictionPlan(take, lens_out, evicted_out, n_free_out, counts)
 
