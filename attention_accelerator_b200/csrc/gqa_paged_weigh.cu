@@ -29,7 +29,7 @@
 // (rows: S has one place for each M tile, the queries' parts take the other half of TMEM)
 // and 3900 (keys).  Measured (B200): the last 64 queries of 8 prompts of up to 16384 keys,
 // e4m3, 193 to 213 us (10 + 93 + 110 for the three kernels), 32 queries 138, 5 queries
-// 120; 6 ragged prompts of up to 2051 tokens, every query, int8, cap 50, 336 to 360 us (43 +
+// 120; 6 ragged prompts of up to 2051 tokens, every query, int8, cap 50, 322 to 345 us (33 +
 // 147 + 160 + 7).  The keys' pass goes unit by unit: with a thread block for each key's
 // tile, which needs no joining, a run has few tiles, the queries' 128 KB are loaded for
 // each, and the pass took 235 (for one unit a sequence the join costs 2, for two 9 of 348).
@@ -349,16 +349,18 @@ __global__ void __launch_bounds__(kPrepThreads, 2) weigh_queries_kernel(const __
     const float unit = p.cap > 0.f ? p.scale / p.cap : p.scale * 1.4426950408889634f;
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(q.row0 + u * kTokens + token) * p.q_row_stride +
-                                                      h * kGroup * p.q_head_stride + 16 * q4);
-    // A head's pairs 0-7 and 8-15, first and then second elements, asked for a head ahead.
-    auto load = [&](int hq, int i) { return real ? src[hq * (p.q_head_stride / 8) + (i & 1) + 8 * (i >> 1)] : none; };
+                                                      h * kGroup * p.q_head_stride + 8 * q4);
+    // Of a head's pairs 8 q4 to 8 q4 + 7 and those 32 further on, first and then second elements, asked for a head
+    // ahead.  (Four lanes write 64 bytes in a row, whole sectors; with 16 pairs in a row a lane, halves of them, the
+    // kernel took 44 us instead of 33 for 6700 tokens of 8 heads.)
+    auto load = [&](int hq, int i) { return real ? src[hq * (p.q_head_stride / 8) + 4 * i] : none; };
     uint4 next[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) next[i] = load(0, i);
     float2 f[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        f[i] = p.q_rotated ? make_float2(1.f, 0.f) : rope_factor(step[16 * q4 + i], pos);
+        f[i] = p.q_rotated ? make_float2(1.f, 0.f) : rope_factor(step[8 * q4 + (i & 7) + 4 * (i & 8)], pos);
     uint8_t* out = a.queries + cell * kQBytes;
 #pragma unroll 1
     for (int hq = 0; hq < kGroup; ++hq) {
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kPrepThreads, 2) weigh_queries_kernel(const __
                 yh[i] = pack_half2(hy0, hy1);
                 yl[i] = pack_half2(y0 - hy0, y1 - hy1);
             }
-            uint8_t* to = out + row * 128 + (((2 * q4 + c) ^ (row & 7)) << 4);
+            uint8_t* to = out + row * 128 + (((q4 + 4 * c) ^ (row & 7)) << 4);
             *reinterpret_cast<uint4*>(to) = make_uint4(xh[0], xh[1], xh[2], xh[3]);
             *reinterpret_cast<uint4*>(to + kQBlockBytes) = make_uint4(yh[0], yh[1], yh[2], yh[3]);
             *reinterpret_cast<uint4*>(to + 2 * kQBlockBytes) = make_uint4(xl[0], xl[1], xl[2], xl[3]);
