@@ -89,7 +89,8 @@ struct alignas(16) PlanShared {
     int equal;            // rows of the last one's number in this CTA
     int2 marks;           // holes, and rows that fill them, in this CTA
     uint32_t bin, left;
-    int give, cuts, rows;
+    unsigned long long give, rows;  // of all requests: a table may name more than 2^31 rows, a request millions of pages
+    int cuts;
     bool last;
 };
 
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
     const int unit = blockIdx.x / ctas;
     const int page_mask = (1 << a.page_shift) - 1;
     auto pages_of = [&](int len) { return (int)(((int64_t)len + page_mask) >> a.page_shift); };
-    if (tid == 0) s.give = s.cuts = s.rows = 0;
+    if (tid == 0) s.give = s.rows = s.cuts = 0;
     // Every load that waits for nothing first.
     const int n_free = *a.n_free, mine = min(unit / a.heads, n - 1), evicted = a.w.evicted[mine];
     const Cut cut = cut_of(a, mine);
@@ -386,9 +387,9 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
         bad |= c.len < 0 || pages_of(c.len) > a.table_width || c.len > a.w.capacity;
         if (!bad) give += pages_of(c.len) - pages_of(c.keep);
     }
-    if (give > 0) atomicAdd(&s.give, (int)min(give, (int64_t)0x7fffffff / kThreads));  // (past any stack all the same)
+    if (give > 0) atomicAdd(&s.give, (unsigned long long)give);
     bad = __syncthreads_or(bad);
-    const bool ok = !bad && n_free >= 0 && (int64_t)n_free + s.give <= a.free_capacity;
+    const bool ok = !bad && n_free >= 0 && (int64_t)n_free + (int64_t)s.give <= a.free_capacity;
 
     if (unit < n * a.heads) {
         if (ok && cut.keep < cut.len) {
@@ -404,7 +405,8 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
         const int lane = tid & 31, warp = tid >> 5;
         int *at_of = s.hist[0], *from_of = at_of + kThreads, *left_of = from_of + kThreads;
         static_assert(Radix<kThreads>::kBins * Radix<kThreads>::kPasses >= 3 * kThreads, "room in the histograms' place");
-        int base = n_free, cuts = 0, rows = 0;
+        int base = n_free, cuts = 0;
+        int64_t rows = 0;
         for (int c0 = 0; c0 < n && ok; c0 += kThreads) {
             const int r = c0 + tid;
             const Cut c = r < n ? cut_of(a, r) : Cut{0, 0};
@@ -448,12 +450,12 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
             }
         }
         if (cuts) atomicAdd(&s.cuts, cuts);
-        if (rows) atomicAdd(&s.rows, rows);
+        if (rows) atomicAdd(&s.rows, (unsigned long long)rows);
         __syncthreads();
         if (tid == 0) {
             a.counts[0] = s.cuts;
-            a.counts[1] = s.rows;
-            a.counts[2] = ok ? s.give : 0;
+            a.counts[1] = (int)min(s.rows, 0x7fffffffull);
+            a.counts[2] = ok ? (int)s.give : 0;
             a.counts[3] = ok ? GQA_OK : GQA_ERR_PAGES;
         }
     }
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) plan_eviction_kernel(const __grid_co
         a.lens_out[r] = ok ? c.keep : c.len;
         a.evicted_out[r] = ok ? evicted + (c.len - c.keep) : evicted;
     }
-    if (tid == 0) *a.n_free_out = ok ? n_free + s.give : n_free;
+    if (tid == 0) *a.n_free_out = ok ? n_free + (int)s.give : n_free;
 }
 
 // ---------------------------------------------------------------------------

@@ -715,7 +715,7 @@ int gqa_add_key_weights(const void *q, const gqa_paged_cache *cache, const gqa_p
  *    valid, n_free_out may be n_free), in the order of requests, then columns; the block
  *    table keeps its entries, which gqa_evict_paged reads: call it before any call that
  *    pops pages.
- *  - counts[4]: requests cut, rows evicted a head, pages given back, status.
+ *  - counts[4]: requests cut, rows evicted a head (2^31 - 1 where they are more), pages given back, status.
  * All or nothing: a negative length, one past the table's row or weights->capacity, or a
  * stack that would pass free_capacity: counts[3] is GQA_ERR_PAGES and nothing changes (take is -1).
  * Workspace: gqa_plan_eviction_workspace_bytes, used by no other call at the same time;

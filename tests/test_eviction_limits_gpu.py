@@ -1,0 +1,51 @@
+"""GPU tests of the keys' weights and of eviction where numbers are largest: tables, lengths, positions, scores."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import attention_accelerator_b200 as gqa
+from attention_accelerator_b200 import _lib
+from test_paged_gpu import ints
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_request_that_gives_back_millions_of_pages():
+    """4.3 million pages of one request: refused by a stack that lacks room for a few of them, else all given back."""
+    page_len, pages, keep = 16, 4_300_000, 40
+    length = pages * page_len - 5
+    w = gqa.key_weights(1, pages * page_len, kv_heads=1)
+    w.weight[0, 0, length - keep:length] = 1.0
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    given = table[0, -(-keep // page_len):]
+    for room in (given.numel() - 1, given.numel()):
+        stack = torch.full((given.numel() + 8,), -7, dtype=torch.int32, device="cuda")
+        plan = gqa.plan_eviction(w, ints([length]), ints([keep]), table, stack[:room], ints([0]), page_len=page_len,
+                                 max_keep=keep, sinks=0, recent=0)
+        if room < given.numel():
+            assert plan.counts.tolist() == [0, 0, 0, _lib.GQA_ERR_PAGES] and plan.n_free.tolist() == [0]
+            assert plan.lens.tolist() == [length] and bool((stack == -7).all()) and bool((plan.take == -1).all())
+        else:
+            assert plan.counts.tolist() == [1, length - keep, room, 0] and plan.n_free.tolist() == [room]
+            assert torch.equal(stack[:room], given) and bool((stack[room:] == -7).all())
+            assert plan.take.flatten().tolist() == list(range(length - keep, length))
+            assert plan.lens.tolist() == [keep] and plan.evicted.tolist() == [length - keep]
+
+
+def test_requests_that_lose_more_than_2_31_rows():
+    """The count of evicted rows stops at 2^31 - 1; lengths, tokens evicted and pages are whole."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    requests, length, page_len = 2100, 1 << 20, 128
+    w = gqa.key_weights(requests, length, kv_heads=1)
+    width = length // page_len
+    table = torch.arange(requests * width, dtype=torch.int32, device="cuda").view(requests, width)
+    stack = torch.full((requests * width,), -7, dtype=torch.int32, device="cuda")
+    plan = gqa.plan_eviction(w, ints([length] * requests), ints([8] * requests), table, stack, ints([0]), page_len=page_len,
+                             max_keep=8, sinks=0, recent=0)
+    given = requests * (width - 1)
+    assert plan.counts.tolist() == [requests, 0x7FFFFFFF, given, 0] and plan.n_free.tolist() == [given]
+    assert torch.equal(stack[:given], table[:, 1:].flatten()) and bool((stack[given:] == -7).all())
+    assert plan.lens.tolist() == [8] * requests and plan.evicted.tolist() == [length - 8] * requests
+    assert bool((plan.take == -1).all())  # equal weights: the lower rows stay
