@@ -728,8 +728,8 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     if (held && (only ? key < known : tile < run.add_below)) weight = out[key];
                     if (ok) ok = warp_wait(&s.s_full[2 * g + (tiles & 1)], (tiles >> 1) & 1);
                     tc_fence_after();
-                    // Rows that see the key: from this column on.
-                    const int from_col = (key - run.pos) * kGroup - col0;
+                    // Rows that see the key: from this column on.  (All do that stand 64 rows and more behind it; up to 2^31.)
+                    const int from_col = max(key - run.pos, -kTokens) * kGroup - col0;
                     const bool edge = __any_sync(0xffffffffu, from_col > 0);
                     const float ks = s.scales[slot][r >> 4];
                     const uint32_t cols = tmem + lanes + buf * kTile + part * mine;

@@ -1,12 +1,15 @@
 """GPU tests of the keys' weights and of eviction where numbers are largest: tables, lengths, positions, scores."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 import attention_accelerator_b200 as gqa
 from attention_accelerator_b200 import _lib
-from test_paged_gpu import ints
+from test_eviction_gpu import some_weights
+from test_paged_gpu import Setup, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +52,29 @@ def test_requests_that_lose_more_than_2_31_rows():
     assert torch.equal(stack[:given], table[:, 1:].flatten()) and bool((stack[given:] == -7).all())
     assert plan.lens.tolist() == [8] * requests and plan.evicted.tolist() == [length - 8] * requests
     assert bool((plan.take == -1).all())  # equal weights: the lower rows stay
+
+
+@pytest.mark.parametrize("length", [(1 << 29) + 50, 1 << 30, 0x7FFFFFFF])
+@pytest.mark.parametrize("counts", [[3, 64], [200, 1]])
+def test_queries_far_behind_the_keys(length, counts):
+    """Lengths past what the table names: the queries stand up to 2^31 rows behind its keys and see them all.  Bounds as
+    in :func:`test_eviction_gpu.exact_weights`."""
+    held = 320
+    s = Setup([held] * 2, seed=counts[0], page_len=64, code="int8", heads=2)
+    w, q = some_weights(s), s.queries(sum(counts))
+    before = w.weight.double(), w.position.clone()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints([length] * 2), ints([0, counts[0], sum(counts)]), w, q_rotated=True)
+    assert torch.equal(w.position, before[1]) and gqa.read_device_status() == 0
+    for b, n in enumerate(counts):
+        rows = q[sum(counts[:b]):][:n].double()
+        k = torch.from_numpy(s.values(b)[0]).cuda()
+        for h in range(2):
+            want, bound = before[0][b, h].clone(), 0.0
+            for g in range(4):
+                x = rows[:, 4 * h + g]
+                weight = torch.softmax(x @ k[:, h].T / math.sqrt(128), -1).sum(0)
+                most = float(x.abs().max()) * float(k[:, h].abs().sum(-1).max()) / math.sqrt(128)
+                want += weight
+                bound = bound + weight * (math.expm1(2 * 2.0 ** -18 * most) + 2.0 ** -20)
+            error = (w.weight[b, h].double() - want).abs()
+            assert bool((error <= bound + 2.0 ** -23 * want).all()), (b, h, float((error / want).max()))
