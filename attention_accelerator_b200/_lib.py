@@ -166,6 +166,9 @@ _SIGNATURES = {
     "gqa_capture_mode": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
     "gqa_plan_pages": (ctypes.c_int, [_P, _P, ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int, _P,
                                       ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "gqa_plan_pages_evicted": (ctypes.c_int, [_P, _P, ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int, _P, ctypes.c_int,
+                                              _P, ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P,
+                                              ctypes.c_size_t, _P]),
     "gqa_append_paged": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                         ctypes.c_int64, _P, _P, ctypes.c_float, ctypes.POINTER(GqaPagedCache), _P]),
     "gqa_read_paged": (ctypes.c_int, [ctypes.POINTER(GqaPagedCache), _P, ctypes.c_int, _P, _P, _P]),

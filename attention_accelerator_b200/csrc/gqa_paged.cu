@@ -38,6 +38,7 @@ struct PlanArgs {
     int32_t *lens_out, *n_free_out, *first_token;
     int64_t* slots;
     int32_t *positions, *counts;
+    int32_t* evicted;  // tokens evicted from each request, or null
     uint32_t* ticket;
     int32_t requests, table_width, free_capacity, page_shift, max_tokens;
 };
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
     for (int r = tid; r < n; r += kPlanThreads) {
         const int len = a.lens[r], add = a.new_lens[r];
         a.lens_out[r] = !ok ? len : add < 0 ? 0 : len + add;
+        if (ok && a.evicted && (add < 0 || len == 0)) a.evicted[r] = 0;  // the request ends, or is a new one
     }
     if (tid == 0) *a.n_free_out = ok ? n_free + n_give - n_need : n_free;
 }
@@ -700,19 +702,11 @@ int attend(const void* q, void* out, const gqa_paged_cache* cache, const gqa_pag
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
-}  // namespace
-
-}  // namespace gqa
-
-using namespace gqa;
-
-extern "C" {
-
-int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, int32_t* block_table,
-                   int64_t table_stride, int table_width, int32_t* free_pages, int free_capacity,
-                   const int32_t* n_free, int page_len, int max_tokens, int32_t* lens_out, int32_t* n_free_out,
-                   int32_t* first_token, int64_t* slots, int32_t* positions, int32_t* counts, void* workspace,
-                   size_t workspace_bytes, void* stream) {
+int plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, int32_t* block_table, int64_t table_stride,
+               int table_width, int32_t* free_pages, int free_capacity, const int32_t* n_free, int page_len,
+               int max_tokens, int32_t* lens_out, int32_t* n_free_out, int32_t* first_token, int64_t* slots,
+               int32_t* positions, int32_t* evicted, int32_t* counts, void* workspace, size_t workspace_bytes,
+               void* stream) {
     if (!lens || !new_lens || !block_table || !free_pages || !n_free || !lens_out || !n_free_out || !first_token ||
         !counts || (max_tokens > 0 && (!slots || !positions)))
         return GQA_ERR_NULL_POINTER;
@@ -727,7 +721,7 @@ int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, i
     int st = device_sms(&sms);
     if (st != GQA_OK) return st;
     st = check_device_memory({lens, new_lens, block_table, free_pages, n_free, lens_out, n_free_out, first_token,
-                                  slots, positions, counts, workspace});
+                              slots, positions, evicted, counts, workspace});
     if (st != GQA_OK) return st;
     PlanArgs a;
     a.lens = lens;
@@ -741,6 +735,7 @@ int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, i
     a.first_token = first_token;
     a.slots = slots;
     a.positions = positions;
+    a.evicted = evicted;
     a.counts = counts;
     a.ticket = static_cast<uint32_t*>(workspace) + 1;
     a.requests = requests;
@@ -760,6 +755,36 @@ int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, i
     if (grid > 128) grid = 128;
     plan_pages_kernel<<<(int)grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
     return launched();
+}
+
+}  // namespace
+
+}  // namespace gqa
+
+using namespace gqa;
+
+extern "C" {
+
+int gqa_plan_pages(const int32_t* lens, const int32_t* new_lens, int requests, int32_t* block_table,
+                   int64_t table_stride, int table_width, int32_t* free_pages, int free_capacity,
+                   const int32_t* n_free, int page_len, int max_tokens, int32_t* lens_out, int32_t* n_free_out,
+                   int32_t* first_token, int64_t* slots, int32_t* positions, int32_t* counts, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    return plan_pages(lens, new_lens, requests, block_table, table_stride, table_width, free_pages, free_capacity, n_free,
+                      page_len, max_tokens, lens_out, n_free_out, first_token, slots, positions, nullptr, counts, workspace,
+                      workspace_bytes, stream);
+}
+
+int gqa_plan_pages_evicted(const int32_t* lens, const int32_t* new_lens, int requests, int32_t* block_table,
+                           int64_t table_stride, int table_width, int32_t* free_pages, int free_capacity,
+                           const int32_t* n_free, int page_len, int max_tokens, int32_t* lens_out, int32_t* n_free_out,
+                           int32_t* first_token, int64_t* slots, int32_t* positions, int32_t* evicted, int32_t* counts,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    if (!evicted) return GQA_ERR_NULL_POINTER;
+    if ((uintptr_t)evicted & 3) return GQA_ERR_ALIGNMENT;
+    return plan_pages(lens, new_lens, requests, block_table, table_stride, table_width, free_pages, free_capacity, n_free,
+                      page_len, max_tokens, lens_out, n_free_out, first_token, slots, positions, evicted, counts, workspace,
+                      workspace_bytes, stream);
 }
 
 int gqa_append_paged(const void* k, const void* v, int n_tokens, int64_t k_token_stride, int64_t k_head_stride,

@@ -13,7 +13,9 @@ least weight:
 K was rotated at its token's position when it was appended, so that a row may move: the rows that stay but lie past the
 new length fill the holes below it, each head its own.  Afterwards a row's number is no longer its position.  A request's
 next token has row ``lens[r]`` and position ``lens[r] + weights.evicted[r]``: append it with that position
-(``append_paged(..., positions=...)``); ``decode_paged_weights`` and ``add_key_weights`` place their queries so by
+(``append_paged(..., positions=...)``) behind ``plan_pages(..., weights=weights)``, which sets ``evicted`` of a request that
+ends, or holds no rows yet, to 0 (a program that ends requests in another way does so before the first append of the next
+one in that row); ``decode_paged_weights`` and ``add_key_weights`` place their queries so by
 themselves, ``decode_paged`` takes ``query_positions``, and ``decode_paged_chunked`` queries that were rotated before
 (``q_rotated``).  Distance bias, document and prefix masks go by rows and no longer apply.  The pages of a request that is
 cut must be its own.  As with the other paged calls every length is in device memory, no call waits for the GPU, and a

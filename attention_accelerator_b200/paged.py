@@ -20,12 +20,16 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass, field
+from typing import TYPE_CHECKING
 
 import torch
 
 from . import _lib, api
 from ._lib import GqaPagedCache, GqaPagedParams
 from .api import GROUP_SIZE, HEAD_DIM, N_KV_HEADS, ROPE_THETA, GqaError, _check, _check_cuda, _check_out, _stream_ptr
+
+if TYPE_CHECKING:
+    from .eviction import KeyWeights
 
 PAGE_LENS = (16, 32, 64, 128)
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
@@ -151,7 +155,7 @@ class PagePlan:
 
 def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                n_free: torch.Tensor, *, page_len: int, max_tokens: int, lens_out: torch.Tensor | None = None,
-               n_free_out: torch.Tensor | None = None) -> PagePlan:
+               n_free_out: torch.Tensor | None = None, weights: "KeyWeights | None" = None) -> PagePlan:
     """Pages, slots and positions of a step's new tokens, from lengths in device memory.
 
     ``lens``/``new_lens``: int32 ``[requests]``; ``new_lens[r] < 0`` ends request r: its pages go back to the free
@@ -160,6 +164,10 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     ``n_free_out`` may be ``lens`` and ``n_free``.  A step that cannot be met (too few free pages, a row of the table
     too short, more than ``max_tokens`` new tokens) changes nothing and says so in ``counts[3]``
     (:meth:`PagePlan.check`).
+
+    ``weights``: the keys' weights of these requests, where some are cut to a budget (see ``eviction``): what was evicted
+    from a request that ends in this step, or that held no rows before it, becomes 0.  Without it the next request in an
+    ended one's row would stand behind the other's tokens.
     """
     lib = _lib.load()
     device = lens.device
@@ -183,13 +191,14 @@ def plan_pages(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     n_free_out = new_n_free if n_free_out is None else n_free_out
     stream = _stream_ptr(device)
     ws = _paged_workspace(device, stream, _lib.CHUNKED_WORKSPACE_BYTES)
-    _check(lib.gqa_plan_pages(
+    evicted = () if weights is None else (_need("weights.evicted", weights.evicted, i32, (n,), device),)
+    _check((lib.gqa_plan_pages_evicted if evicted else lib.gqa_plan_pages)(
         _need("lens", lens, i32, (n,), device), _need("new_lens", new_lens, i32, (n,), device), n,
         block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
         _need("free_pages", free_pages, i32, tuple(free_pages.shape), device), free_pages.shape[0],
         _need("n_free", n_free, i32, (1,), device), page_len, max_tokens,
         _need("lens_out", lens_out, i32, (n,), device), _need("n_free_out", n_free_out, i32, (1,), device),
-        first.data_ptr(), slots.data_ptr(), positions.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(),
+        first.data_ptr(), slots.data_ptr(), positions.data_ptr(), *evicted, counts.data_ptr(), ws.data_ptr(), ws.numel(),
         stream), "plan_pages")
     return PagePlan(lens_out, n_free_out, first, slots, positions, counts)
 

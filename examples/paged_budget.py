@@ -54,7 +54,7 @@ def main(argv=None) -> dict:
         """``new[r]`` tokens join request r, at the positions behind all it has had; returns the plan and their queries."""
         total = sum(new)
         plan = gqa.plan_pages(lens, torch.tensor(new, **i32), table, free, n_free, page_len=page_len, max_tokens=total,
-                              lens_out=lens, n_free_out=n_free)
+                              lens_out=lens, n_free_out=n_free, weights=weights)
         owner = torch.searchsorted(plan.first_token[1:], torch.arange(total, **i32), right=True)
         gqa.append_paged(cache, rows(total, KV_HEADS), rows(total, KV_HEADS), plan.slots,
                          positions=plan.positions + weights.evicted[owner])

@@ -541,6 +541,17 @@ int gqa_plan_pages(const int32_t *lens, const int32_t *new_lens, int requests, i
                    size_t workspace_bytes, void *stream);
 
 /*
+ * The same for requests that are cut to a budget (gqa_key_weights): evicted[r] of a request that ends in this step, or
+ * that held no rows before it, becomes 0, so that the next request in its row starts at position 0.  `evicted` is
+ * 4-byte aligned; nothing of it changes in a step that is refused.
+ */
+int gqa_plan_pages_evicted(const int32_t *lens, const int32_t *new_lens, int requests, int32_t *block_table,
+                           int64_t table_stride, int table_width, int32_t *free_pages, int free_capacity,
+                           const int32_t *n_free, int page_len, int max_tokens, int32_t *lens_out, int32_t *n_free_out,
+                           int32_t *first_token, int64_t *slots, int32_t *positions, int32_t *evicted, int32_t *counts,
+                           void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Append n_tokens K and V rows (BF16, token t head h at k + t*k_token_stride +
  * h*k_head_stride elements) to the cache at slots[t] (-1: skipped, as is a slot
  * outside the cache).  With `positions`, K is rotated at positions[t] first, in
@@ -656,7 +667,8 @@ int gqa_decode_paged_chunked_diff(const void *q, void *out, const gqa_paged_cach
  * that stay but lie past the new length fill the holes below it.  Afterwards a row's
  * number is no longer its position: query and append positions are row + evicted[r]
  * (GQA_FLAG_Q_ROTATED, positions of gqa_append_paged), and distance bias, document
- * and prefix masks no longer apply.  No reference counterpart.
+ * and prefix masks no longer apply.  A row of the batch that is used again starts with
+ * evicted[r] = 0 before its first append: gqa_plan_pages_evicted sees to that.  No reference counterpart.
  * ------------------------------------------------------------------------- */
 typedef struct gqa_key_weights {
     float   *weight;    /* [batch][kv_heads][capacity] */

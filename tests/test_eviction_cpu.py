@@ -74,6 +74,16 @@ def weights(**change):
     return _lib.GqaKeyWeights(**{**dict(weight=4096, position=4096, evicted=4096, capacity=48), **change})
 
 
+def test_c_refuses_bad_planning_with_weights():
+    lib = _lib.load()
+    ok = [4096, 4096, 2, 4096, 3, 3, 4096, 10, 4096, 16, 4, 4096, 4096, 4096, 4096, 4096, 4096, 4096, None, 0, None]
+    for at, value, want in [(0, None, "NULL_POINTER"), (16, None, "NULL_POINTER"), (16, 4098, "ALIGNMENT"),
+                            (17, None, "NULL_POINTER"), (2, 0, "BATCH"), (9, 24, "KV_BLOCK_LEN"), (18, None, "WORKSPACE")]:
+        args = list(ok)
+        args[at] = value
+        assert lib.gqa_plan_pages_evicted(*args) == getattr(_lib, "GQA_ERR_" + want), (at, value)
+
+
 def test_c_refuses_bad_evictions():
     lib = _lib.load()
     w = weights()
