@@ -156,7 +156,8 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
 
     Pages past the new lengths are pushed on ``free_pages`` (int32 ``[capacity]``, entries below ``n_free``, int32
     ``[1]``, valid).  ``lens_out``, ``evicted_out`` and ``n_free_out`` may be ``lens``, ``weights.evicted`` and
-    ``n_free``; where ``evicted_out`` is not given it is ``weights.evicted`` if ``lens_out`` is ``lens``, else new.  A step
+    ``n_free``; where ``evicted_out`` is not given it is ``weights.evicted`` if ``lens_out`` is ``lens`` (the same memory),
+    else new.  A step
     that cannot be met (a length past the table's row, no room on the stack) changes nothing and says so in ``counts[3]``
     (:meth:`EvictionPlan.check`).  Follow it with :func:`evict_paged` before anything takes pages or changes the lengths.
     """
@@ -180,7 +181,7 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
     if not (0 <= sinks <= 0x7FFFFFFF and 0 <= recent <= 0x7FFFFFFF):
         raise ValueError("sinks and recent must not be negative")
     i32 = torch.int32
-    if evicted_out is None and lens_out is lens:
+    if evicted_out is None and lens_out is not None and lens_out.data_ptr() == lens.data_ptr():
         evicted_out = weights.evicted
     lens_ptr = _need("lens", lens, i32, (n,), device)
     given = [_need("lens_out", lens_out, i32, (n,), device), _need("evicted_out", evicted_out, i32, (n,), device),

@@ -10,6 +10,7 @@ import torch
 import attention_accelerator_b200 as gqa
 from attention_accelerator_b200 import _lib
 from oracle import paged as ref
+from test_eviction_gpu import random_state
 from test_paged_gpu import THETA, ints, rows_of
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +114,20 @@ def test_the_next_request_in_a_row_that_was_cut(code):
     out = got[0][0][0].float().cpu().numpy()
     assert np.all(np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + (math.expm1(2 * 2.0 ** -18 * most) + 2.0 ** -17) * size)
     assert bool((got[0][2] == torch.arange(101, device="cuda", dtype=torch.int32)).all())
+
+
+# ---- parts of a batch ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lo,hi", [(0, 4), (1, 3)])
+def test_lens_out_of_the_same_memory(lo, hi):
+    """``lens_out`` that is ``lens`` by its memory, as slices of one tensor are: the tokens evicted join the weights' own."""
+    lens, keep = [50, 60, 70, 80], [20, 30, 0, 25]
+    weight, position, evicted = random_state(0, lens, 2, 96)
+    w = gqa.KeyWeights(torch.from_numpy(weight).cuda(), torch.from_numpy(position).cuda(), ints(evicted))
+    ln, table = ints(lens), torch.arange(24, dtype=torch.int32, device="cuda").view(4, 6)
+    stack, n_free = torch.zeros(24, dtype=torch.int32, device="cuda"), ints([0])
+    plan = gqa.plan_eviction(w[lo:hi], ln[lo:hi], ints(keep[lo:hi]), table[lo:hi], stack, n_free, page_len=16, max_keep=32,
+                             lens_out=ln[lo:hi], n_free_out=n_free)
+    plan.check()
+    after = [min(n, k) if k and lo <= r < hi else n for r, (n, k) in enumerate(zip(lens, keep))]
+    assert ln.tolist() == after
+    assert w.evicted.tolist() == [e + n - a for e, n, a in zip(evicted, lens, after)]
