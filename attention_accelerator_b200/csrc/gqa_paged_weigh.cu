@@ -22,7 +22,9 @@
 //
 // Precision.  The weights are FP32 results: Q, divided by a power of two that brings a
 // row's largest below 1, is split into two FP16 parts (22 bits), both products
-// accumulate in the same FP32 columns; codes are exact.
+// accumulate in the same FP32 columns; codes are exact.  Scores past kFar are rounded to
+// FP32 before a row's reference is taken from them, and the reference before its sum's
+// logarithm: in one step the rounding of a large product would be left in the exponent.
 //
 // Bound: a tile of 128 keys for a unit takes 2048 cycles of the tensor pipe (two parts of
 // Q) and 2048 of the special-function unit in each pass; overlapped they come to 3100
@@ -129,6 +131,9 @@ constexpr int kRuns = 4;  // runs found ahead
 constexpr int kUnitCost = 2;
 // The rows' reference is the largest of the first keys; a sum of weights past 2^kOverflow moves it.
 constexpr float kOverflow = 0x1p90f;
+// From such references on a score is rounded before they are taken from it: the test of it costs both passes 2 %
+// (a window of 64 queries on 8 x 16384 keys 217 -> 220 us).
+constexpr float kFar = 0x1p10f;
 
 // Shared memory of a pass: rings of codes and of FP16 tiles, or of codes beside the queries.
 template <bool kKeys>
@@ -158,7 +163,7 @@ struct alignas(64) WeighArgs {
     uint32_t* status;
     uint8_t* queries;    // [units * heads][kQBytes]
     float* factor;       // [units * heads][kRows]: z of a row is its product times the page's scale times this
-    float* row_log2;     // [units * heads][kRows]: log2 of the sum of 2^z
+    float2* row_sums;    // [units * heads][kRows]: reference, and log2 of the sum of 2^(z - reference)
     uint32_t* arrivals;  // [units * heads]
     float2* partials;    // [ctas][2][kRows]: reference and sum
     Piece* pieces;       // [batch * heads + ctas]
@@ -286,6 +291,7 @@ struct alignas(16) Shared {
     uint64_t drain;  // products in flight when the issuer gives up
     float scales[kScaleSlots][8];
     float4 columns[4][2][kRows / 8];  // keys: factors and -log2 of two columns, of a quarter's run and the next
+    float4 far[4][2][kRows / 8];      // and of those past kFar, whose -log2 is 0 there, reference and logarithm
     float part[kParts][3][kTile];     // keys: sums of the quarters but the first
     float2 other[2][2][kTile];        // rows: references and sums of the second half of the keys
     long long warp_sum[kThreads / 32];
@@ -603,9 +609,10 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     phase ^= 1;
                     tc_fence_after();
                     const int k0 = ((run.tile0 + t) << kTileShift) + 64 * part;
-                    const bool edge = __any_sync(0xffffffffu, hi < k0 + 64);
+                    const bool masked = __any_sync(0xffffffffu, hi < k0 + 64);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
+                        const bool edge = kCap ? masked : __any_sync(0xffffffffu, masked || fabsf(ref) >= kFar);  // (or -inf)
                         float z[32];
                         tmem_ld32(t_s + 32 * c, reinterpret_cast<uint32_t(&)[32]>(z));
                         float f0 = factor * s.scales[slot][4 * part + 2 * c], f1 = factor * s.scales[slot][4 * part + 2 * c + 1];
@@ -647,7 +654,11 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                         if (!(sum < kOverflow)) {  // the row's first keys, or larger ones by far
                             float mx = -INFINITY;
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, z[e] * (e < 16 ? f0 : f1));
+                            for (int e = 0; e < 32; ++e) {
+                                if constexpr (!kCap) z[e] *= e < 16 ? f0 : f1;
+                                mx = fmaxf(mx, z[e]);
+                            }
+                            f0 = f1 = 1.f;
                             const float now = fmaxf(ref, mx);
                             l *= fast_exp2(ref - (now == -INFINITY ? 0.f : now));
                             ref = now;
@@ -666,10 +677,12 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                     const float now = fmaxf(ref, other.x), use = now == -INFINITY ? 0.f : now;
                     l = l * fast_exp2(ref - use) + other.y * fast_exp2(other.x - use);
                     ref = now;
-                    float* out = a.row_log2 + cell * kRows + g * kTile + r;
-                    auto log2_of = [&](float m, float sum) { return !real ? INFINITY : sum == 0.f ? -INFINITY : m + log2f(sum); };
+                    float2* out = a.row_sums + cell * kRows + g * kTile + r;
+                    auto row_of = [&](float m, float sum) {
+                        return !real ? make_float2(INFINITY, 0.f) : sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m, log2f(sum));
+                    };
                     if (run.count == run.tiles) {
-                        if (active) *out = log2_of(ref, l);
+                        if (active) *out = row_of(ref, l);
                     } else {
                         // A piece of a unit.
                         const int c0 = run.c0, parts = run.parts, second = run.second;
@@ -695,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                                 L = L * fast_exp2(M - by) + x.y * fast_exp2(x.x - by);
                                 M = top;
                             }
-                            *out = log2_of(M, L);
+                            *out = row_of(M, L);
                         }
                         named_barrier_sync(1, 2 * kTile);  // s.last is read
                     }
@@ -708,14 +721,20 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
             for (; next_run(run); end_run()) {
                 const int half = columns_of(run.n) >> 1, mine = half >> 1, col0 = g * half + part * mine;
                 const int64_t cell = run.cell;
-                float4* column = s.columns[2 * g + part][runs & 1];
+                float4 *column = s.columns[2 * g + part][runs & 1], *far_column = s.far[2 * g + part][runs & 1];
                 ++runs;
+                bool mine_far = false;
                 if (r < mine) {
-                    float* to = reinterpret_cast<float*>(column) + (r >> 1) * 4 + (r & 1);
+                    const int at = (r >> 1) * 4 + (r & 1);
+                    float *to = reinterpret_cast<float*>(column) + at, *far_to = reinterpret_cast<float*>(far_column) + at;
+                    const float2 row = a.row_sums[cell * kRows + col0 + r];
+                    mine_far = fabsf(row.x) >= kFar && fabsf(row.x) < INFINITY;
                     to[0] = a.factor[cell * kRows + col0 + r];
-                    to[2] = -a.row_log2[cell * kRows + col0 + r];
+                    to[2] = mine_far ? 0.f : -(row.x + row.y);
+                    far_to[0] = mine_far ? -row.x : 0.f;
+                    far_to[2] = mine_far ? -row.y : 0.f;
                 }
-                named_barrier_sync(2 + 2 * g + part, kTile);
+                const bool far = named_barrier_or(2 + 2 * g + part, kTile, mine_far);
                 // The only unit's sums are added to the weights; those of several units are joined behind this kernel.
                 const bool only = run.add_below < 0;
                 const int known = run.known, len = run.len;
@@ -758,6 +777,14 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
                             for (int i = 0; i < 8; ++i) {
                                 v[2 * i] += column[8 * c + i].z;
                                 v[2 * i + 1] += column[8 * c + i].w;
+                            }
+                        }
+                        if (far) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 k = far_column[8 * c + i];
+                                v[2 * i] = (v[2 * i] + k.x) + k.z;
+                                v[2 * i + 1] = (v[2 * i + 1] + k.y) + k.w;
                             }
                         }
                         if (edge) {
@@ -1163,7 +1190,7 @@ Kernel kernel_for(int code, bool cap) {
 }
 
 struct Regions {
-    size_t partials, pieces, shares_of, arrivals, factor, row_log2, queries, sums, end;
+    size_t partials, pieces, shares_of, arrivals, factor, row_sums, queries, sums, end;
     int64_t sum_rows, max_cells;
     int n_pieces;
 };
@@ -1180,8 +1207,8 @@ Regions regions(int batch, int rows, int heads, int64_t keys, int sms) {
     r.shares_of = r.pieces + up((size_t)r.n_pieces * sizeof(Piece));
     r.arrivals = r.shares_of + up((size_t)batch * heads * sizeof(int2));
     r.factor = r.arrivals + up(units * sizeof(uint32_t));
-    r.row_log2 = r.factor + units * kRows * sizeof(float);
-    r.queries = r.row_log2 + units * kRows * sizeof(float);
+    r.row_sums = r.factor + units * kRows * sizeof(float);
+    r.queries = r.row_sums + units * kRows * sizeof(float2);
     r.sums = r.queries + units * kQBytes;
     const size_t tiles = (size_t)((keys + kTile - 1) / kTile);
     const size_t by_cell = units * (tiles + kUnitCost) * kTile, by_row = 2 * (size_t)r.n_pieces * tiles * kTile;
@@ -1238,7 +1265,7 @@ cudaError_t launch_paged_weigh(const PagedCall& call, const RopeSteps& rope, int
     a.status = reinterpret_cast<uint32_t*>(ws);
     a.queries = ws + r.queries;
     a.factor = reinterpret_cast<float*>(ws + r.factor);
-    a.row_log2 = reinterpret_cast<float*>(ws + r.row_log2);
+    a.row_sums = reinterpret_cast<float2*>(ws + r.row_sums);
     a.arrivals = reinterpret_cast<uint32_t*>(ws + r.arrivals);
     a.partials = reinterpret_cast<float2*>(ws + r.partials);
     a.pieces = reinterpret_cast<Piece*>(ws + r.pieces);

@@ -8,7 +8,7 @@ import torch
 
 import attention_accelerator_b200 as gqa
 from attention_accelerator_b200 import _lib
-from test_eviction_gpu import some_weights
+from test_eviction_gpu import exact_weights, some_weights
 from test_paged_gpu import Setup, ints
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +78,47 @@ def test_queries_far_behind_the_keys(length, counts):
                 bound = bound + weight * (math.expm1(2 * 2.0 ** -18 * most) + 2.0 ** -20)
             error = (w.weight[b, h].double() - want).abs()
             assert bool((error <= bound + 2.0 ** -23 * want).all()), (b, h, float((error / want).max()))
+
+
+@pytest.mark.parametrize("power,cap", [(4, 0.0), (14, 0.0), (18, 0.0), (24, 0.0), (28, 0.0), (32, 0.0), (40, 0.0), (60, 0.0),
+                                       (118, 0.0), (126, 0.0), (60, 1e6), (126, 1e30)])
+@pytest.mark.parametrize("n", [1, 40, 100])
+def test_queries_of_any_size_beside_ordinary_ones(power, cap, n):
+    """Rows of up to BF16's largest numbers, each the value of one key: it gets their whole weight (with a cap that they
+    pass, all keys of a positive score share it; one beyond 2^96 is none, as the call's arguments say), and the other rows
+    of their unit give what they give without them."""
+    exact_cap = cap if cap <= 2.0 ** 96 else 0.0
+    length = 700
+    s = Setup([length], seed=power, page_len=64, code="int8", heads=2)
+    s.cache.k_scale.fill_(2.0 ** -17)  # scores of 2^126 times a key stay within FP32
+    q = (s.queries(n).float() * 2.0 ** 10).to(torch.bfloat16)
+    plain, k = q.clone(), torch.from_numpy(s.values(0)[0]).cuda()
+    picks = [(row, head, 17 * row % (length - n + row + 1)) for row in {n // 10, n - 1} for head in (1, 6)]
+    for row, head, key in picks:
+        x = k[key, head // 4]
+        q[row, head] = (x / x.abs().max() * 2.0 ** power).to(torch.bfloat16)
+        plain[row, head] = 0.0
+    w = some_weights(s)
+    before = w.weight.clone()
+    gqa.add_key_weights(q, s.cache, ints(s.table), ints([length]), ints([0, n]), w, q_rotated=True, score_cap=cap or None)
+    total, bound = exact_weights(s, plain, [n], [0], cap=exact_cap, q_rotated=True)[0]
+    for row, head, key in picks:
+        seen = length - n + row + 1
+        total[head // 4, :seen] -= 1.0 / seen  # a row of zeros gives every key as much
+        x = q[row, head].double()
+        z = k[:seen, head // 4] @ x / math.sqrt(128)
+        if exact_cap:
+            z = exact_cap * torch.tanh(z / exact_cap)
+        p = torch.softmax(z, -1)
+        total[head // 4, :seen] += p
+        if power >= 24:  # no two scores are near each other but those at the cap, which are the same
+            assert float(p.max() - p[p > 0].min()) < 1e-12 and abs(float((p > 0).sum() * p.max()) - 1) < 1e-12
+            bound[head // 4, :seen] += 2.0 ** -20 * p
+        else:
+            most = float(x.abs().max()) * float(k[:, head // 4].abs().sum(-1).max()) / math.sqrt(128)
+            bound[head // 4, :seen] += p * (math.expm1(2 * 2.0 ** -18 * most) + 2.0 ** -20)
+    start = before[0, :, :length].double()
+    start[:, length - n:] = 0.0
+    error = (w.weight[0, :, :length].double() - start - total).abs()
+    # (2^-40: the rows of zeros that were taken out again.)
+    assert bool((error <= bound + 2.0 ** -23 * (start + total) + 2.0 ** -40).all()), float(error.max())
