@@ -71,6 +71,32 @@ struct ScoreArgs {
 
 constexpr int kScoreThreads = 256, kScoreKeys = 4;  // keys a thread at a time
 
+// From such scores on a row's sum has to stand beside its largest score, not in one number with it: a number of that
+// size has no room for the logarithm.
+constexpr float kFar = 0x1p10f;
+
+// A row's largest score and log2 of the sum of 2^(score - it), over `len` keys, by the block: for the head `head` of
+// the scores.  (Seldom: each block goes through the row.)
+__device__ __noinline__ float2 row_of_scores(const float* scores, int head, int len) {
+    __shared__ float part[kScoreThreads / 32];
+    auto over_block = [&](float v, bool largest) {
+        auto join = [&](float x, float y) { return largest ? fmaxf(x, y) : x + y; };
+#pragma unroll
+        for (int d = 16; d; d >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, d));
+        __syncthreads();  // (what stood there has been read)
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = part[0];
+        for (int w = 1; w < kScoreThreads / 32; ++w) v = join(v, part[w]);
+        return v;
+    };
+    float most = -INFINITY, sum = 0.f;
+    for (int64_t k = threadIdx.x; k < len; k += kScoreThreads) most = fmaxf(most, __ldcg(scores + k * kGroup + head));
+    most = over_block(most, true);
+    for (int64_t k = threadIdx.x; k < len; k += kScoreThreads) sum += fast_exp2(__ldcg(scores + k * kGroup + head) - most);
+    return make_float2(most, log2f(over_block(sum, false)));
+}
+
 __global__ void __launch_bounds__(kScoreThreads) score_weights_kernel(const __grid_constant__ ScoreArgs a) {
     dependency_wait();
     allow_dependents();
@@ -79,7 +105,16 @@ __global__ void __launch_bounds__(kScoreThreads) score_weights_kernel(const __gr
     if (len == 0) return;
     const int64_t at = (int64_t)blockIdx.x * a.w.capacity;
     const float4* scores = reinterpret_cast<const float4*>(a.s.scores) + (int64_t)blockIdx.x * a.s.keys;
-    const float4 sum = *reinterpret_cast<const float4*>(a.s.row_log2 + (int64_t)blockIdx.x * kGroup);
+    float4 sum = *reinterpret_cast<const float4*>(a.s.row_log2 + (int64_t)blockIdx.x * kGroup), most = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) {
+        float &log2 = (&sum.x)[g], &top = (&most.x)[g];
+        if (fabsf(log2) >= kFar) {
+            const float2 row = row_of_scores(reinterpret_cast<const float*>(scores), g, len);
+            top = row.x;
+            log2 = row.y;
+        }
+    }
     constexpr int kBlock = kScoreThreads * kScoreKeys;
     for (int64_t k0 = (int64_t)blockIdx.y * kBlock + threadIdx.x; k0 < len; k0 += (int64_t)gridDim.y * kBlock) {
         float4 z[kScoreKeys];
@@ -95,8 +130,8 @@ __global__ void __launch_bounds__(kScoreThreads) score_weights_kernel(const __gr
         for (int i = 0; i < kScoreKeys; ++i) {
             const int64_t k = k0 + i * kScoreThreads;
             if (k >= len) break;
-            const float w = (fast_exp2(z[i].x - sum.x) + fast_exp2(z[i].y - sum.y)) +
-                            (fast_exp2(z[i].z - sum.z) + fast_exp2(z[i].w - sum.w));
+            const float w = (fast_exp2((z[i].x - most.x) - sum.x) + fast_exp2((z[i].y - most.y) - sum.y)) +
+                            (fast_exp2((z[i].z - most.z) - sum.z) + fast_exp2((z[i].w - most.w) - sum.w));
             a.w.weight[at + k] = old[i] + w;
             if (k == last) a.w.position[at + k] = last + (last > 0 ? paged_evicted(a.p, b) : 0);
         }
@@ -131,9 +166,8 @@ constexpr int kRuns = 4;  // runs found ahead
 constexpr int kUnitCost = 2;
 // The rows' reference is the largest of the first keys; a sum of weights past 2^kOverflow moves it.
 constexpr float kOverflow = 0x1p90f;
-// From such references on a score is rounded before they are taken from it: the test of it costs both passes 2 %
-// (a window of 64 queries on 8 x 16384 keys 217 -> 220 us).
-constexpr float kFar = 0x1p10f;
+// (kFar: from such references on a score is rounded before they are taken from it.  The test of it costs both passes 2 %:
+// a window of 64 queries on 8 x 16384 keys 217 -> 220 us.)
 
 // Shared memory of a pass: rings of codes and of FP16 tiles, or of codes beside the queries.
 template <bool kKeys>

@@ -122,3 +122,38 @@ def test_queries_of_any_size_beside_ordinary_ones(power, cap, n):
     error = (w.weight[0, :, :length].double() - start - total).abs()
     # (2^-40: the rows of zeros that were taken out again.)
     assert bool((error <= bound + 2.0 ** -23 * (start + total) + 2.0 ** -40).all()), float(error.max())
+
+
+@pytest.mark.parametrize("v_scale", [1 / 127, 2.0 ** -4, 2.0 ** -40, 2.0 ** 30])
+@pytest.mark.parametrize("power", [8, 20, 24, 28, 30, 31, 32, 33, 34, 35, 36, 37, 38, 60, 118])
+def test_decode_steps_of_queries_of_any_size(power, v_scale):
+    """One token a sequence: the scores' rounding takes no part in the sums, whatever V's scales add to the exponents."""
+    lens = [300] * 15 + [5000]
+    s = Setup(lens, seed=power, page_len=64, code="int8", heads=2)
+    s.cache.k_scale.fill_(2.0 ** -17)
+    s.cache.v_scale.fill_(v_scale)
+    k = [torch.from_numpy(s.values(b)[0]).cuda() for b in range(len(lens))]
+    q = torch.zeros(len(lens), 8, 128, dtype=torch.bfloat16, device="cuda")
+    for b in range(len(lens)):
+        for head in range(8):
+            x = k[b][(7 * b + head) % 300, head // 4]
+            q[b, head] = (x / x.abs().max() * 2.0 ** (power + (b % 8) / 8)).to(torch.bfloat16)
+    w = some_weights(s)
+    before = w.weight.double()
+    gqa.decode_paged_weights(q, s.cache, ints(s.table), ints(lens), w, q_rotated=True)
+    for b, n in enumerate(lens):
+        for h in range(2):
+            want, bound = before[b, h, :n].clone(), 0.0
+            want[n - 1] = 0.0
+            for g in range(4):
+                x = q[b, 4 * h + g].double()
+                p = torch.softmax(k[b][:, h] @ x / math.sqrt(128), -1)
+                want += p
+                if power >= 24:  # one key stands out
+                    assert float(p.max()) > 1 - 1e-12
+                    bound = bound + 2.0 ** -20 * p
+                else:
+                    most = float(x.abs().max()) * float(k[b][:, h].abs().sum(-1).max()) / math.sqrt(128)
+                    bound = bound + p * (math.expm1(2 * 2.0 ** -18 * most) + 2.0 ** -20)
+            error = (w.weight[b, h, :n].double() - want).abs()
+            assert bool((error <= bound + 2.0 ** -23 * want).all()), (b, h, float(error.max()))
