@@ -345,7 +345,7 @@ struct DiffRow {
             d[32 * kHalf + e] = lane ? got - hi : lo - got;
         }
     }
-    __device__ __forceinline__ void write(const DiffCall& c, __nv_bfloat16* out, int lane, bool real) {
+    __device__ __forceinline__ void write(const DiffCall& c, __nv_bfloat16* out, int lane, bool real, bool seen) {
         float f = c.out_scale;
         if (c.gain) {
             float eps = c.eps;
@@ -384,7 +384,7 @@ struct DiffRow {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const __nv_bfloat162 v = __floats2bfloat162_rn(d[e + 2 * i], d[e + 2 * i + 1]);
-                wp[i] = *reinterpret_cast<const uint32_t*>(&v);
+                wp[i] = seen ? *reinterpret_cast<const uint32_t*>(&v) : 0u;  // 0 whatever the norm's weight
             }
             *reinterpret_cast<uint4*>(out + 64 * (e >> 5) + 32 * lane + (e & 31)) = w;
         }
@@ -712,12 +712,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         tmem_ld32(t_o, reinterpret_cast<uint32_t(&)[32]>(x[0]));
                         tmem_ld32(t_o + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
                         tmem_wait_ld();
-                        joined.take<0>(x, f * map_factor, head & 1);
+                        const float fm = l == 0.f ? 0.f : f * map_factor;  // (0 whatever the lambda)
+                        joined.take<0>(x, fm, head & 1);
                         tmem_ld32(t_o + 64, reinterpret_cast<uint32_t(&)[32]>(x[0]));
                         tmem_ld32(t_o + 96, reinterpret_cast<uint32_t(&)[32]>(x[32]));
                         tmem_wait_ld();
-                        joined.take<1>(x, f * map_factor, head & 1);
-                        joined.write(p.diff, out, head & 1, real);
+                        joined.take<1>(x, fm, head & 1);
+                        joined.write(p.diff, out, head & 1, real, l != 0.f);
                     } else {
                     float x[kHeadDim];
 #pragma unroll
@@ -793,7 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                             const float2 v = ml(c);
                             L = fmaf(fast_exp2(v.x - mu), v.y, L);
                         }
-                        const float inv = (L == 0.f ? 0.f : kWeightUnit / L) * map_factor;
+                        const float inv = L == 0.f ? 0.f : kWeightUnit / L * map_factor;
 #pragma unroll(kDiff ? 2 : 1)
                         for (int half = 0; half < 2; ++half) {
                             float x[64];
@@ -825,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                                 write(2 * half + 1, reinterpret_cast<const float(&)[32]>(x[32]));
                             }
                         }
-                        if constexpr (kDiff) joined.write(p.diff, out, head & 1, real);
+                        if constexpr (kDiff) joined.write(p.diff, out, head & 1, real, L != 0.f);
                     }
                 }
                 tc_fence_before();  // the next unit's products overwrite O after this thread's next arrival

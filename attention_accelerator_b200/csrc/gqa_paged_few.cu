@@ -428,9 +428,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             auto piece = [&](int c, int q, int e, int head) {
                 return a.partials + ((int64_t)(((c0 + c) * 2 + (c ? 0 : second)) * kUnitRows) + (2 * q + e) * kGroup + head) * kRowF;
             };
-            // kDiff: a row's values times f, and the joined row's output.
+            // kDiff: a row's values times f (0 where it sees nothing, whatever f is), and the joined row's output.
             auto times = [&](float4 x, float l, float f) {
-                f *= l == 0.f ? 0.f : kWeightUnit / l;
+                f = l == 0.f ? 0.f : f * (kWeightUnit / l);
                 return make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
             };
             auto lambda_of = [&](int token) {
@@ -438,8 +438,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                                                      walk.h * (kGroup / 2) + (hq >> 1)]
                                     : 0.f;
             };
-            auto write_diff = [&](int token, float4 x, float4 y) {
-                if (token < un.n)
+            auto write_diff = [&](int token, float4 x, float4 y, float l) {
+                if (token >= un.n) return;
+                if (l == 0.f)  // whatever the norm's weight
+                    *reinterpret_cast<uint2*>(p.out + (int64_t)(un.row0 + token) * p.out_row_stride +
+                                              (walk.h * (kGroup / 2) + (hq >> 1)) * p.out_head_stride + 4 * lane) = make_uint2(0u, 0u);
+                else
                     write_diff_row(p.diff, make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w),
                                    p.out + (int64_t)(un.row0 + token) * p.out_row_stride +
                                        (walk.h * (kGroup / 2) + (hq >> 1)) * p.out_head_stride,
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
                                 write_diff(2 * q + e, times(A[e], L[e], 1.f),
-                                           *reinterpret_cast<const float4*>(&rows[e][4 * lane]));
+                                           *reinterpret_cast<const float4*>(&rows[e][4 * lane]), L[e]);
                     }
                 }
 #pragma unroll
@@ -556,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
                             merge(hq | 1);
                             const float4 second_map = times(A, L, lambda_of(token));
                             merge(hq & ~1);
-                            write_diff(token, times(A, L, 1.f), second_map);
+                            write_diff(token, times(A, L, 1.f), second_map, L);
                         } else {
                             merge(hq);
                             write(q, e, A, L);
