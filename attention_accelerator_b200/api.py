@@ -90,7 +90,9 @@ _ws_lock = threading.Lock()
 _ws: dict[tuple[int, int], torch.Tensor] = {}
 # Buffers replaced by a larger one stay allocated: a CUDA graph captured with an
 # earlier call still holds their device address and would otherwise write into
-# memory the allocator has handed to another tensor.
+# memory the allocator has handed to another tensor.  Each is at least twice as
+# large as the one that it replaces, so that all that were replaced together are
+# no larger than the one in use, however small the steps of a growing batch are.
 _ws_retired: list[torch.Tensor] = []
 
 
@@ -99,9 +101,15 @@ def _workspace(device: torch.device, stream_ptr: int, nbytes: int) -> torch.Tens
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:
-            if buf is not None:
-                _ws_retired.append(buf)
-            buf = _zeroed(max(nbytes, 4096), device)
+            old, size = buf, max(nbytes, 4096)
+            try:
+                buf = _zeroed(size if old is None else max(size, 2 * old.numel()), device)
+            except torch.OutOfMemoryError:
+                if old is None or size >= 2 * old.numel():
+                    raise
+                buf = _zeroed(size, device)
+            if old is not None:
+                _ws_retired.append(old)
             _ws[key] = buf
         return buf
 

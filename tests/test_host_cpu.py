@@ -105,6 +105,34 @@ def test_workspace_grows_without_freeing_the_old_buffer():
     del api._ws[(None, stream)]
 
 
+def test_workspaces_of_a_growing_batch_stay_bounded(monkeypatch):
+    """Grown in small steps, all buffers that were replaced are together no larger than the one in use, and that one at
+    most twice what was asked; where twice the last one does not fit, what is asked has to."""
+    import torch
+    from attention_accelerator_b200 import api
+    monkeypatch.setattr(api, "_ws", {})
+    monkeypatch.setattr(api, "_ws_retired", [])
+    dev, stream, step = torch.device("cpu"), 0x5eed, 16 * 3000
+    for n in range(1, 129):
+        buf = api._workspace(dev, stream, n * step)
+        assert n * step <= buf.numel() <= max(4096, 2 * n * step)
+        assert sum(b.numel() for b in api._ws_retired) <= buf.numel()
+        assert api._workspace(dev, stream, n * step) is buf
+    held, zeroed = buf.numel(), api._zeroed
+
+    def small_card(nbytes, device):
+        if nbytes > held + 1000:
+            raise torch.OutOfMemoryError("no room")
+        return zeroed(nbytes, device)
+
+    monkeypatch.setattr(api, "_zeroed", small_card)
+    kept = len(api._ws_retired)
+    assert api._workspace(dev, stream, held + 1000).numel() == held + 1000 and len(api._ws_retired) == kept + 1
+    with pytest.raises(torch.OutOfMemoryError):
+        api._workspace(dev, stream, held + 1001)
+    assert api._workspace(dev, stream, held).numel() == held + 1000 and len(api._ws_retired) == kept + 1
+
+
 _NULL_PROBE = r"""
 import ctypes
 import os
