@@ -340,7 +340,7 @@ struct DiffRow {
     __device__ __forceinline__ void take(const float (&x)[64], float f, int lane) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-            const float lo = x[e] * f, hi = x[32 + e] * f;
+            const float lo = __fmul_rn(x[e], f), hi = __fmul_rn(x[32 + e], f);  // (rounded: equal maps leave nothing)
             const float got = __shfl_xor_sync(0xffffffffu, lane ? lo : hi, 1);
             d[32 * kHalf + e] = lane ? got - hi : lo - got;
         }

@@ -431,7 +431,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_con
             // kDiff: a row's values times f (0 where it sees nothing, whatever f is), and the joined row's output.
             auto times = [&](float4 x, float l, float f) {
                 f = l == 0.f ? 0.f : f * (kWeightUnit / l);
-                return make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+                // (Each rounded, not joined to the difference: equal maps leave nothing.)
+                return make_float4(__fmul_rn(x.x, f), __fmul_rn(x.y, f), __fmul_rn(x.z, f), __fmul_rn(x.w, f));
             };
             auto lambda_of = [&](int token) {
                 return token < un.n ? p.diff.lambdas[(int64_t)(un.row0 + token) * p.diff.lambda_stride +
