@@ -392,7 +392,7 @@ struct DiffRow {
 };
 
 // kDiff: Q heads 2 j and 2 j + 1 are joined to one output row; their rows are neighbouring lanes, which
-// exchange halves, so that each norms and writes 64 dims (ragged prompts of documents with cap 212 us).
+// exchange halves, so that each norms and writes 64 dims (ragged prompts of documents with cap 213 us).
 template <int kCode, bool kCap, bool kBias, bool kDiff>
 __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkPagedArgs a) {
     extern __shared__ uint8_t raw_smem[];

@@ -24,8 +24,10 @@ namespace {
 // both in order, and they are paired off.  One more CTA gives the pages back.
 //
 // Bound by the chain of loads, votes and barriers between the passes, not by the 8 bytes
-// a row: 64 requests of 1025 rows and 8 heads 11.5 us, 8 of up to 32768 26 us (64 clusters
-// of 4), one of 131072 28 us, 64 of up to 8192 35 us (replayed graph).
+// a row: 64 requests of 1025 rows and 8 heads 11.3 us in tables of up to 2048 rows, 15.7 in
+// tables of up to 8192 and 23.6 of 32768 (the shape goes by the table, and a block there has
+// its SM to itself), 8 of up to 32768 26 us (64 clusters of 4), one of 131072 28 us, 64 of up
+// to 8192 35 us (replayed graph).
 // ---------------------------------------------------------------------------
 constexpr int kMaxCluster = 8;
 constexpr int kMaxRows = 48 * 1024;  // of a CTA in shared memory; numbers of rows past that are computed again

@@ -278,7 +278,7 @@ __device__ __forceinline__ void consume_tile(State& st, const uint8_t* stage, co
 }
 
 // kDiff: Q heads 2 j and 2 j + 1 are joined to one output row, as in the one-token kernel (48 x 5
-// drafted tokens 128 us, 122 without).
+// drafted tokens 129 us, 122 without).
 template <int kCode, bool kCap, bool kBias, bool kDiff>
 __global__ void __launch_bounds__(kThreads, 1) paged_few_kernel(const __grid_constant__ FewPagedArgs a) {
     extern __shared__ uint8_t raw[];

@@ -30,9 +30,9 @@
 // Q) and 2048 of the special-function unit in each pass; overlapped they come to 3100
 // (rows: S has one place for each M tile, the queries' parts take the other half of TMEM)
 // and 3900 (keys).  Measured (B200): the last 64 queries of 8 prompts of up to 16384 keys,
-// e4m3, 189 to 213 us (10 + 93 + 112 + 3 one by one), 32 queries 138, 5 queries
-// 120; 6 ragged prompts of up to 2051 tokens, every query, int8, cap 50, 322 to 345 us (33 +
-// 147 + 160 + 7).  The keys' pass goes unit by unit: with a thread block for each key's
+// e4m3, 198 to 222 us (9 + 97 + 115 + 4 one by one), 32 queries 142, 5 queries
+// 122; 6 ragged prompts of up to 2051 tokens, every query, int8, cap 50, 328 to 348 us (32 +
+// 150 + 165 + 7).  The keys' pass goes unit by unit: with a thread block for each key's
 // tile, which needs no joining, a run has few tiles, the queries' 128 KB are loaded for
 // each, and the pass took 235 (for one unit a sequence the join costs 2, for two 9 of 348).
 // score_weights_kernel: 64 ragged sequences (2.3 M keys and heads, 90 MB, mostly

@@ -139,7 +139,7 @@ class EvictionPlan(NamedTuple):
     lens: torch.Tensor     # int32 [requests]: rows held after the step
     evicted: torch.Tensor  # int32 [requests]: tokens evicted after the step
     n_free: torch.Tensor   # int32 [1]: height of the free stack after the step
-    counts: torch.Tensor   # int32 [4]: requests cut, rows evicted a head, pages given back, status
+    counts: torch.Tensor   # int32 [4]: requests cut, rows evicted a head (2^31 - 1 at most), pages given back, status
 
     def check(self) -> None:
         """Wait for the plan; raise ``GqaError`` if it was refused (nothing was changed then)."""
@@ -157,9 +157,9 @@ def plan_eviction(weights: KeyWeights, lens: torch.Tensor, keep: torch.Tensor, b
     Pages past the new lengths are pushed on ``free_pages`` (int32 ``[capacity]``, entries below ``n_free``, int32
     ``[1]``, valid).  ``lens_out``, ``evicted_out`` and ``n_free_out`` may be ``lens``, ``weights.evicted`` and
     ``n_free``; where ``evicted_out`` is not given it is ``weights.evicted`` if ``lens_out`` is ``lens`` (the same memory),
-    else new.  A step
-    that cannot be met (a length past the table's row, no room on the stack) changes nothing and says so in ``counts[3]``
-    (:meth:`EvictionPlan.check`).  Follow it with :func:`evict_paged` before anything takes pages or changes the lengths.
+    else new.  A step that cannot be met (a length past the table's row, no room on the stack) changes nothing and says so
+    in ``counts[3]`` (:meth:`EvictionPlan.check`).  Follow it with :func:`evict_paged` before anything takes pages or
+    changes the lengths.
     """
     lib = _lib.load()
     device = lens.device

@@ -372,8 +372,9 @@ def decode_paged_diff(q: torch.Tensor, cache: PagedCache, block_table: torch.Ten
     with the scores, masks and arguments of :func:`decode_paged`; returns BF16 ``[batch, 2 * heads, 128]``.
     ``lambdas``: float32 ``[2 * heads]``, or ``[batch, 2 * heads]`` where they come from the tokens.  With
     ``norm_weight`` (float32 ``[128]``) each head's row is divided by its root mean square,
-    ``a / sqrt(mean(a^2) + norm_eps) * norm_weight``; ``out_scale`` multiplies the row (``1 - lambda_init`` in a
-    differential transformer's layer).  A row that sees no key is 0.
+    ``a / sqrt(mean(a^2) + norm_eps) * norm_weight``; ``out_scale`` multiplies the row (``1 - lambda_init``, say).  A row
+    that sees no key is 0.  The two maps of a pair share one K and one V head of 128 dims: layers whose V is twice as wide
+    as their K, normed over both halves, are not served.
     """
     return _attend_diff("decode_paged_diff", q, cache, block_table, seq_lens, None, lambdas, norm_weight, norm_eps,
                         out_scale, query_positions=query_positions, scale=scale, rope_theta=rope_theta,
@@ -389,7 +390,9 @@ def decode_paged_diff_chunked(q: torch.Tensor, cache: PagedCache, block_table: t
                               doc_starts: torch.Tensor | None = None, prefix_ends: torch.Tensor | None = None,
                               out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`decode_paged_diff` of any number of queries a sequence, packed as for :func:`decode_paged_chunked`;
-    ``lambdas`` float32 ``[2 * heads]`` or ``[rows, 2 * heads]``.  Returns BF16 ``[rows, 2 * heads, 128]``."""
+    ``lambdas`` float32 ``[2 * heads]`` or ``[rows, 2 * heads]``.  Returns BF16 ``[rows, 2 * heads, 128]``.  As in that
+    call rotated queries and softmax weights are rounded to FP16 (22 bits of them in :func:`decode_paged_diff`): an error
+    of up to 2^-11 of the maps, which is more of their difference the more of them cancels."""
     return _attend_diff("decode_paged_diff_chunked", q, cache, block_table, seq_lens, first_query, lambdas, norm_weight,
                         norm_eps, out_scale, query_positions=None, scale=scale, rope_theta=rope_theta,
                         q_rotated=q_rotated, score_cap=score_cap, distance_slopes=distance_slopes,

@@ -639,9 +639,15 @@ int gqa_decode_paged_chunked(const void *q, void *out, const gqa_paged_cache *ca
  *   out_j = out_scale * a_j, or with norm_weight
  *   out_j = out_scale * norm_weight * a_j / sqrt(mean(a_j^2) + norm_eps)   (mean over the 128 dims)
  * with z and the visible keys as for gqa_decode_paged; a row that sees no key is
- * 0.  `out` is BF16 [rows][2 * kv_heads][128], rounded once; both maps, their
- * difference and the norm are FP32.  Workspace: gqa_paged_workspace_bytes.
- * No reference counterpart.
+ * 0.  `out` is BF16 [rows][2 * kv_heads][128], rounded once; sums, the maps'
+ * difference and the norm are FP32.  The maps' operands are those of the plain
+ * calls: 22 bits of Q and of the softmax weights in gqa_decode_paged_diff, and in
+ * gqa_decode_paged_chunked_diff one rounding of each to FP16 (2^-11 at most), which
+ * is an error of the maps' size, not of the difference's: where they nearly cancel
+ * it is that much more of what is left, and the norm scales both up.  A pair shares
+ * one K and one V head of 128 dims, and the norm is over these 128 (a layer whose V
+ * is twice as wide as its K, with a norm over both halves, is not this one).
+ * Workspace: gqa_paged_workspace_bytes.  No reference counterpart.
  * ------------------------------------------------------------------------- */
 typedef struct gqa_paged_diff {
     const float *lambdas;       /* lambda(i, j) at lambdas[i * lambda_row_stride + j] */
@@ -679,9 +685,11 @@ typedef struct gqa_key_weights {
 
 /* Device workspace of either call below (0 on invalid input), under the rules of gqa_paged_workspace_bytes's; one
  * that is as large as both ask serves those calls as well.  One token a sequence (first_query NULL): 16 bytes for
- * each key that the table could name and KV head.  Else 136 KB for 64 queries and KV head, and with more than 64
- * rows in all the sums that thread blocks leave: at most 8 bytes for each key that the table could name, KV head
- * and sequence, and 1.2 KB for each key of one sequence. */
+ * each key that the table could name, sequence and KV head.  Else 132 KB for each KV head and unit of at most 64
+ * queries of one sequence, of which there is room for rows / 64 + batch + 1 (however few queries a sequence has:
+ * 9 GB for 8192 sequences and 8 heads), and with more than 64 rows in all the sums that thread blocks leave: at
+ * most 8 bytes for each key that the table could name, KV head and sequence, and 1.2 KB for each key of one
+ * sequence.  In all calls 4 MB more. */
 size_t gqa_key_weights_workspace_bytes(const gqa_paged_cache *cache, const gqa_paged_params *p);
 
 /*

@@ -1,6 +1,7 @@
 """GPU tests of the keys' weights and of eviction where numbers are largest: tables, lengths, positions, scores."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -9,6 +10,7 @@ import torch
 import attention_accelerator_b200 as gqa
 from attention_accelerator_b200 import _lib
 from test_eviction_gpu import exact_weights, some_weights
+from test_paged_cpu import c_cache, c_params
 from test_paged_gpu import Setup, ints
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +159,19 @@ def test_decode_steps_of_queries_of_any_size(power, v_scale):
                     bound = bound + p * (math.expm1(2 * 2.0 ** -18 * most) + 2.0 ** -20)
             error = (w.weight[b, h, :n].double() - want).abs()
             assert bool((error <= bound + 2.0 ** -23 * want).all()), (b, h, float(error.max()))
+
+
+@pytest.mark.parametrize("batch,rows,heads,width", [(1, 1, 1, 1), (64, 64, 8, 512), (8192, 8192, 8, 4), (8192, 8192, 1, 512),
+                                                    (8, 512, 8, 256), (6, 9000, 8, 129), (48, 4096, 3, 2048), (1, 100000, 8, 1 << 14)])
+def test_workspaces_are_of_the_stated_size(batch, rows, heads, width):
+    """As the header states it: 132 KB a unit and head, 16 bytes a key, sequence and head, and what thread blocks leave."""
+    lib, page_len = _lib.load(), 64
+    c = c_cache(kv_heads=heads, page_len=page_len)
+    keys = width * page_len
+    many = lib.gqa_key_weights_workspace_bytes(ctypes.byref(c), ctypes.byref(c_params(
+        batch=batch, rows=rows, table_width=width, table_stride=width, first_query=4096)))
+    sums = keys * (8 * heads * batch + 1200) if rows > 64 else 0
+    assert 0 < many <= 132 * 1024 * heads * (rows // 64 + batch + 1) + sums * 1.01 + 128 * 8 * heads * batch + (4 << 20)
+    one = lib.gqa_key_weights_workspace_bytes(ctypes.byref(c), ctypes.byref(c_params(
+        batch=batch, rows=batch, table_width=width, table_stride=width, first_query=None)))
+    assert 16 * keys * batch * heads < one <= 16 * keys * batch * heads + (4 << 20)
