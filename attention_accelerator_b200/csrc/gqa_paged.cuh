@@ -245,10 +245,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 // Up to |x| = 1/2 as x times a polynomial in t = x^2, interpolated at the Chebyshev
 // points of tanh(x) / x (2^-26 of it); beyond as 1 - 2 / (e^2x + 1).
 constexpr float kTanhNear = 0.25f;  // of t
+constexpr float kTanh3 = -0.333330691f, kTanh5 = 0.13324751f, kTanh7 = -0.0529842377f, kTanh9 = 0.0171313453f;  // of x^3, ...
 __device__ __forceinline__ float tanh_near(float x, float t) {
-    float p = fmaf(0.0171313453f, t, -0.0529842377f);
-    p = fmaf(p, t, 0.13324751f);
-    p = fmaf(p, t, -0.333330691f);
+    float p = fmaf(kTanh9, t, kTanh7);
+    p = fmaf(p, t, kTanh5);
+    p = fmaf(p, t, kTanh3);
     return x * fmaf(p, t, 1.f);
 }
 __device__ __forceinline__ float tanh_far(float x) {

@@ -463,9 +463,9 @@ __device__ __forceinline__ void cap_pairs(float (&z)[kN], float cap2) {
         x[i] = v.x;
         x[i + 1] = v.y;
         most = fmaxf(fmaxf(most, t.x), t.y);
-        float2 y = __ffma2_rn(both(0.0171313453f), t, both(-0.0529842377f));
-        y = __ffma2_rn(y, t, both(0.13324751f));
-        y = __ffma2_rn(y, t, both(-0.333330691f));
+        float2 y = __ffma2_rn(both(kTanh9), t, both(kTanh7));
+        y = __ffma2_rn(y, t, both(kTanh5));
+        y = __ffma2_rn(y, t, both(kTanh3));
         y = __fmul2_rn(__ffma2_rn(y, t, both(1.f)), __fmul2_rn(v, both(cap2)));
         z[i] = y.x;
         z[i + 1] = y.y;
